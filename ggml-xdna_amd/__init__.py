@@ -35,7 +35,7 @@ _c_p = ctypes.c_void_p
 _c_f = ctypes.c_float
 _c_i = ctypes.c_int
 
-# name -> (restype, argtypes), as declared in include/zest_hip.h
+# name -> (restype, argtypes), as declared in include/zest_hip.h and include/zest/kv.h
 SIGNATURES = {
     "zest_init": (_c_i, [_c_i]),
     "zest_self_test": (_c_i, []),
@@ -65,6 +65,18 @@ SIGNATURES = {
     "zest_check_finite": (_c_i, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p]),
     "zest_rope": (_c_i, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i, _c_i, _c_f, _c_f, _c_f, _c_f,
                          _c_f, _c_f, _c_p, _c_p]),
+    "zest_kv_page_bytes": (ctypes.c_size_t, [_c_p]),
+    "zest_kv_rope_freqs": (_c_i, [_c_i, *[ctypes.c_double] * 6, _c_p, _c_p, _c_p]),
+    "zest_kv_append": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_i, _c_p, _c_i64,
+                              _c_i, _c_p, _c_p]),
+    "zest_kv_attn_workspace": (ctypes.c_size_t, [_c_p, _c_p, _c_i]),
+    "zest_kv_attn": (_c_i, [_c_p, _c_p, _c_p, _c_i, _c_i64, _c_i, _c_f, _c_i, _c_i, _c_f, _c_p, _c_i, _c_i64, _c_p,
+                            ctypes.c_size_t, _c_p, _c_p]),
+    "zest_kv_scratch_bytes": (ctypes.c_size_t, [_c_i64, _c_i]),
+    "zest_kv_assign": (_c_i, [_c_p, _c_i, _c_i64, _c_p, _c_p, _c_p, _c_i, _c_i, _c_p, _c_p, _c_p, _c_i, _c_p, ctypes.c_size_t,
+                              _c_p, _c_p]),
+    "zest_kv_compact": (_c_i, [_c_p, _c_i, _c_i64, _c_p, _c_p, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p, ctypes.c_size_t, _c_p,
+                               _c_p]),
 }
 
 

@@ -1,0 +1,534 @@
+// Attention over the paged KV cache (include/zest/kv.h): one pass over the keys
+// with the running maximum and sum of a softmax, on v_mfma_f32_32x32x16.
+//
+// A column is one (new token, query head) pair of a k/v head, token-major: with
+// a group of G query heads column c is token c / G and head c % G of the group,
+// so one token's heads share the keys and values that a wave reads, and a chunk
+// of tokens fills whole tiles. Scores are computed as S^T = K Q^T: 32 tokens by
+// 32 columns, K the A operand and Q^T, held in registers, the B operand. A lane
+// then holds 16 scores of one column (column lane % 32; tokens 8k + 4h + 0..3
+// for k = 0..3, h = lane / 32), so the softmax statistics are one value a lane
+// and need one exchange between lane halves a tile. O^T = V^T P^T takes the
+// weights as its B operand from the registers they are in: the contraction runs
+// over tokens in the order 4h..4h+3, 8+4h..8+4h+3 of each 16, which is the order
+// the cache stores V in.
+#include <algorithm>
+
+#include "kv_device.h"
+#include "zest_common.h"
+
+namespace {
+
+using zest::kv_batch;
+using zest::kv_pages;
+using zest::kv_seq;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int COLS = 32;     // columns of a wave's tile
+constexpr int WAVES = 4;     // waves of a workgroup
+constexpr int GROUP = 32;    // tokens a wave takes at a time
+constexpr int UNIT = WAVES * GROUP;  // tokens of a unit of work
+constexpr int MAX_WORKGROUPS = 512;  // two a CU
+
+// The cache's element type: its fragment, its MFMA and its exponent field.
+template <int TYPE> struct elem;
+
+template <> struct elem<ZEST_TYPE_BF16> {
+    typedef bf16x8 frag;
+    static constexpr uint32_t EXP = 0x7f807f80u, ONE = 0x00800080u;
+    // exponent added to the softmax weights: none, bf16 has fp32's range
+    static constexpr float SHIFT = 0.0f;
+    static __device__ f32x16 mfma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __bf16 from(float v) { return (__bf16) v; }
+};
+
+template <> struct elem<ZEST_TYPE_F16> {
+    typedef f16x8 frag;
+    static constexpr uint32_t EXP = 0x7c007c00u, ONE = 0x04000400u;
+    // weights are held times 2^12 (the sum with them, so it cancels): the largest
+    // is 2^12, and one 2^-26 of it is still a normal fp16 number
+    static constexpr float SHIFT = 12.0f;
+    static __device__ f32x16 mfma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ _Float16 from(float v) { return (_Float16) v; }
+};
+
+struct attn_args {
+    kv_pages c;
+    kv_batch b;
+    const void * q;
+    void * out;
+    int64_t ldq, ldo;
+    int32_t q_type, out_type, group, causal, window;
+    float scale, softcap;  // softcap 0: none
+    float * partial;
+};
+
+// Tokens [lo, hi) that any of a sequence's rows i0 .. i1 sees.
+__device__ inline void seen_by(const attn_args & a, const kv_seq & s, int i0, int i1, int32_t & lo, int32_t & hi) {
+    const int32_t p0 = s.len - s.n + i0, p1 = s.len - s.n + i1;
+    hi = a.causal ? min(s.len, max(0, p1 + 1)) : s.len;
+    lo = a.window > 0 ? (int32_t) max((int64_t) 0, (int64_t) p0 - a.window + 1) : 0;
+    lo = min(lo, hi);
+}
+
+__device__ inline int32_t col_tiles(const attn_args & a, const kv_seq & s) {
+    return (int32_t) (((int64_t) s.n * a.group + COLS - 1) / COLS);
+}
+
+// Units of work of one column tile: whole UNITs from the first token seen.
+__device__ inline int32_t units_of(const attn_args & a, const kv_seq & s) {
+    int32_t lo, hi;
+    seen_by(a, s, 0, s.n - 1, lo, hi);
+    lo &= ~(GROUP - 1);
+    return max(1, (hi - lo + UNIT - 1) / UNIT);
+}
+
+__device__ inline int32_t cost_of(const attn_args & a, const kv_seq & s) {
+    return s.n > 0 ? units_of(a, s) * col_tiles(a, s) * a.c.kv_heads : 0;
+}
+
+// The largest or the sum of a value over a lane and its partner in the other half.
+__device__ inline float other_half(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// Query fragments of one column: 8 values at d = 16 ks + 8 half, from a row of
+// any type, rounded to the cache's; zeros for a column past the last.
+template <int TYPE, int D>
+__device__ inline void load_q(const attn_args & a, const kv_seq & s, int h, int c, bool valid, int half,
+                              typename elem<TYPE>::frag qf[D / 16]) {
+    const int i = c / a.group, g = c - i * a.group;
+    const int64_t at = (int64_t) (s.row0 + i) * a.ldq + (int64_t) (h * a.group + g) * D + half * 8;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ks++) {
+        typename elem<TYPE>::frag f = {};
+        if (valid) {
+            if (a.q_type == TYPE) {
+                f = *reinterpret_cast<const typename elem<TYPE>::frag *>((const uint16_t *) a.q + at + ks * 16);
+            } else if (a.q_type == ZEST_TYPE_F32) {
+                const float * x = (const float *) a.q + at + ks * 16;
+                const float4 u = *reinterpret_cast<const float4 *>(x), w = *reinterpret_cast<const float4 *>(x + 4);
+                const float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[j] = elem<TYPE>::from(v[j]);
+            } else if (a.q_type == ZEST_TYPE_BF16) {
+                const bf16x8 x = *reinterpret_cast<const bf16x8 *>((const uint16_t *) a.q + at + ks * 16);
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[j] = elem<TYPE>::from((float) x[j]);
+            } else {
+                const f16x8 x = *reinterpret_cast<const f16x8 *>((const uint16_t *) a.q + at + ks * 16);
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[j] = elem<TYPE>::from((float) x[j]);
+            }
+        }
+        qf[ks] = f;
+    }
+}
+
+// Whether any of a fragment's values is NaN or infinite (an exponent field of
+// ones carries into the next bit).
+template <int TYPE> __device__ inline bool nonfinite(typename elem<TYPE>::frag f) {
+    struct words { uint32_t w[4]; };
+    const words v = __builtin_bit_cast(words, f);
+    uint32_t carry = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) carry |= (v.w[i] & elem<TYPE>::EXP) + elem<TYPE>::ONE;
+    return (carry & 0x80008000u) != 0;
+}
+
+// The running softmax of a wave's 32 columns: a lane's maximum (of its column,
+// scores times log2 e), the sum of its own weights, and O^T.
+template <int D> struct softmax_state {
+    float m, l;
+    f32x16 o[D / 32];
+};
+
+// What of a group of 32 tokens a lane's column sees: tokens [lo, hi), and of
+// each 16 tokens whether their page is there.
+struct group_mask {
+    int32_t t0, lo, hi;
+    bool ok[2];
+};
+
+// One group of 32 tokens: scores, running maximum and sum, weights times V.
+// masked (the same in every lane): some column does not see some token.
+// v(dt, g): the V fragment of rows 32 dt .. of O^T and tokens 16 g .. of the group.
+template <int TYPE, int D, typename V>
+__device__ inline void attend(const attn_args & a, const typename elem<TYPE>::frag qf[D / 16],
+                              const typename elem<TYPE>::frag kf[D / 16], V && v, const group_mask & k, bool masked,
+                              softmax_state<D> & st) {
+    typedef typename elem<TYPE>::frag frag;
+    const int half = (threadIdx.x >> 5) & 1;
+    f32x16 s = {};
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ks++) s = elem<TYPE>::mfma(kf[ks], qf[ks], s);
+    if (a.softcap > 0.0f) {
+        const float in = a.scale / a.softcap * (2.0f * LOG2E), cap = a.softcap * LOG2E;
+#pragma unroll
+        for (int i = 0; i < 16; i++)  // cap * tanh(x): 1 - 2 / (e^2x + 1), off by 2^-23 of the cap at most
+            s[i] = cap - 2.0f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[i] * in) + 1.0f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] *= a.scale * LOG2E;
+    }
+    if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int32_t t = k.t0 + (i & 3) + 8 * (i >> 2) + 4 * half;
+            s[i] = t >= k.lo && t < k.hi && k.ok[i >> 3] ? s[i] : -INFINITY;
+        }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+    top = fmaxf(top, other_half(top));
+    const float m = fmaxf(st.m, top);
+    // a column that has seen nothing yet keeps -inf; its weights are 2^-inf = 0
+    const float base = (m == -INFINITY ? 0.0f : m) - elem<TYPE>::SHIFT;
+    const float shrink = __builtin_amdgcn_exp2f(st.m - (base + elem<TYPE>::SHIFT));
+    if (__any(m != st.m)) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) st.o[dt][i] *= shrink;
+        st.l *= shrink;
+    }
+    st.m = m;
+    float p[16], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        p[i] = __builtin_amdgcn_exp2f(s[i] - base);
+        sum += p[i];
+    }
+    st.l += sum;
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        frag pf;
+#pragma unroll
+        for (int j = 0; j < 8; j++) pf[j] = elem<TYPE>::from(p[8 * g + j]);
+        bool odd = false;
+        if (masked) {
+#pragma unroll
+            for (int dt = 0; dt < D / 32; dt++) odd |= nonfinite<TYPE>(v(dt, g));
+        }
+        if (masked && __any(odd)) {
+            // A weight of 0 does not silence a NaN or an infinity: the 16 tokens
+            // one at a time, each added where its column sees it
+            for (int tt = 0; tt < 16; tt++) {
+                const int j = (tt & 3) + (tt >> 3) * 4, h = (tt >> 2) & 1;
+                const int32_t t = k.t0 + 16 * g + tt;
+                const bool in = t >= k.lo && t < k.hi && k.ok[g];
+                if (!__any(in)) continue;
+                struct words { uint32_t w[4]; };
+                words keep;
+#pragma unroll
+                for (int w = 0; w < 4; w++) keep.w[w] = half == h && w == j >> 1 ? (j & 1 ? 0xffff0000u : 0xffffu) : 0u;
+#pragma unroll
+                for (int dt = 0; dt < D / 32; dt++) {
+                    words x = __builtin_bit_cast(words, v(dt, g));
+#pragma unroll
+                    for (int w = 0; w < 4; w++) x.w[w] &= keep.w[w];
+                    const f32x16 one = elem<TYPE>::mfma(__builtin_bit_cast(frag, x), pf, f32x16{});
+#pragma unroll
+                    for (int i = 0; i < 16; i++) st.o[dt][i] = in ? st.o[dt][i] + one[i] : st.o[dt][i];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int dt = 0; dt < D / 32; dt++) st.o[dt] = elem<TYPE>::mfma(v(dt, g), pf, st.o[dt]);
+        }
+    }
+}
+
+// A partial result of a column tile: O^T times its weights' sum as [32][D], the
+// maxima and the sums.
+template <int D> constexpr int PARTIAL = COLS * (D + 2);
+
+// Four values of an output row.
+__device__ inline void store4(const attn_args & a, int64_t at, const float v[4]) {
+    if (a.out_type == ZEST_TYPE_F32) {
+        *reinterpret_cast<float4 *>((float *) a.out + at) = make_float4(v[0], v[1], v[2], v[3]);
+        return;
+    }
+    uint16_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        w[i] = a.out_type == ZEST_TYPE_BF16 ? __builtin_bit_cast(uint16_t, (__bf16) v[i]) : __builtin_bit_cast(uint16_t, (_Float16) v[i]);
+    *reinterpret_cast<uint2 *>((uint16_t *) a.out + at) = make_uint2(w[0] | (uint32_t) w[1] << 16, w[2] | (uint32_t) w[3] << 16);
+}
+
+// Where the units of the whole call lie: workgroup w of W takes [u0, u1).
+__device__ inline void share_of(int32_t total, int w, int W, int32_t & u0, int32_t & u1) {
+    u0 = (int32_t) ((int64_t) total * w / W);
+    u1 = (int32_t) ((int64_t) total * (w + 1) / W);
+}
+
+// The units of every (sequence, k/v head, column tile) follow each other, and
+// each workgroup takes an equal share of them, however long each sequence is. A
+// piece of a share is one column tile's run of units; its four waves take 32
+// tokens of a unit each, straight from the cache into the MFMA's registers, and
+// are joined in shared memory. A piece that is the tile's whole run goes to the
+// output; else it is a partial result (slot 2w + 1 where it starts the run, 2w
+// where it continues one), and combine_kernel joins a run's pieces in order.
+template <int TYPE, int D>
+__global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_args a) {
+    typedef typename elem<TYPE>::frag frag;
+    extern __shared__ __align__(16) int32_t attn_sh[];
+    __shared__ float tile[WAVES][COLS][36];  // 32 columns' d values of a 32-row block of O^T
+    __shared__ float stat[WAVES][2][COLS];
+    int32_t * prefix = attn_sh;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+    const int ps = a.c.page_shift, P = 1 << ps;
+    zest::prefix_over_seqs(a.b, ps, prefix, [&](const kv_seq & s) { return cost_of(a, s); });
+    int32_t u, u1;
+    share_of(prefix[a.b.seqs], blockIdx.x, gridDim.x, u, u1);
+    bool bad = false;
+    while (u < u1) {
+        const int b = __builtin_amdgcn_readfirstlane(zest::seq_of(prefix, a.b.seqs, u));
+        const kv_seq s = zest::load_seq(a.b, b, ps, bad);
+        const int32_t run = units_of(a, s), at = u - prefix[b], tiles = col_tiles(a, s);
+        const int32_t ct = at / run % tiles, h = at / run / tiles, first = at % run;
+        const int32_t units = min(run - first, u1 - u);
+        const int32_t * row = a.b.tables + (int64_t) s.slot * a.b.table_cols;
+
+        const int c = ct * COLS + col, ncols = s.n * a.group;
+        const bool valid = c < ncols;
+        frag qf[D / 16];
+        load_q<TYPE, D>(a, s, h, c, valid, half, qf);
+        // what the lane's column sees, and what all the tile's columns see
+        int32_t lo, hi, all_lo, all_hi, any_lo, any_hi, seq_lo, seq_hi;
+        const int i0 = ct * COLS / a.group, i1 = min(ncols - 1, ct * COLS + COLS - 1) / a.group;
+        seen_by(a, s, c / a.group, c / a.group, lo, hi);
+        if (!valid) lo = hi = 0;
+        seen_by(a, s, i0, i0, any_lo, all_hi);
+        seen_by(a, s, i1, i1, all_lo, any_hi);
+        seen_by(a, s, 0, s.n - 1, seq_lo, seq_hi);
+        seq_lo &= ~(GROUP - 1);
+
+        softmax_state<D> st;
+        st.m = -INFINITY;
+        st.l = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++) st.o[dt] = f32x16{};
+        for (int32_t unit = first; unit < first + units; unit++) {
+            const int32_t t0 = seq_lo + unit * UNIT + wave * GROUP;
+            if (t0 >= any_hi || t0 + GROUP <= any_lo) continue;
+            group_mask k{t0, lo, hi, {true, true}};
+            const uint8_t * base[2];
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const int32_t tg = t0 + 16 * g;
+                int32_t id = 0;
+                k.ok[g] = tg < any_hi;
+                if (k.ok[g]) {
+                    id = row[tg >> ps];
+                    if ((uint32_t) id >= (uint32_t) a.c.pages) {
+                        id = 0;
+                        k.ok[g] = false;
+                        bad = true;
+                    }
+                }
+                base[g] = a.c.pool + id * a.c.page_bytes + (int64_t) h * (4 * P * D);
+            }
+            const uint32_t in0 = t0 & (P - 1), in1 = (t0 + 16) & (P - 1);
+            const uint8_t * kp = (lane & 16 ? base[1] + in1 * 16 : base[0] + in0 * 16) + (lane & 15) * 16 + half * P * 16;
+            frag kf[D / 16];
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ks++) kf[ks] = *reinterpret_cast<const frag *>(kp + ks * (P * 32));
+            const uint8_t * vp[2];
+#pragma unroll
+            for (int g = 0; g < 2; g++) vp[g] = base[g] + 2 * P * D + (g ? in1 : in0) * (2 * D) + half * (16 * D) + col * 16;
+            auto load_v = [&](int dt, int g) { return *reinterpret_cast<const frag *>(vp[g] + dt * 512); };
+            const bool masked = t0 < all_lo || t0 + GROUP > all_hi || !k.ok[0] || !k.ok[1];
+            if constexpr (D <= 128) {  // V requested with K; wider heads have no registers for it
+                frag vf[D / 32][2];
+#pragma unroll
+                for (int g = 0; g < 2; g++)
+#pragma unroll
+                    for (int dt = 0; dt < D / 32; dt++) vf[dt][g] = load_v(dt, g);
+                attend<TYPE, D>(a, qf, kf, [&](int dt, int g) { return vf[dt][g]; }, k, masked, st);
+            } else {
+                attend<TYPE, D>(a, qf, kf, load_v, k, masked, st);
+            }
+        }
+
+        // the waves' results joined: every column's maximum and sum, then O^T a
+        // 32-row block at a time, stored by columns
+        st.l += other_half(st.l);
+        __syncthreads();
+        if (half == 0) {
+            stat[wave][0][col] = st.m;
+            stat[wave][1][col] = st.l;
+        }
+        __syncthreads();
+        float m = stat[0][0][col];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) m = fmaxf(m, stat[w][0][col]);
+        const float base = m == -INFINITY ? 0.0f : m;
+        const float mine = __builtin_amdgcn_exp2f(st.m - base);
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) l += stat[w][1][col] * __builtin_amdgcn_exp2f(stat[w][0][col] - base);
+        const bool whole = units == run;
+        float * slot = a.partial + (int64_t) (2 * blockIdx.x + (first == 0)) * PARTIAL<D>;
+        if (!whole && wave == 0 && half == 0) {
+            slot[COLS * D + col] = m;
+            slot[COLS * D + COLS + col] = l;
+        }
+        const float factor = whole ? (l == 0.0f ? 0.0f : mine / l) : mine;
+        const int oc = threadIdx.x >> 3, od = (threadIdx.x & 7) * 4, cc = ct * COLS + oc;
+        const int64_t to = (int64_t) (s.row0 + cc / a.group) * a.ldo + (int64_t) (h * a.group + cc % a.group) * D + od;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float4 v = make_float4(st.o[dt][i] * factor, st.o[dt][i + 1] * factor, st.o[dt][i + 2] * factor, st.o[dt][i + 3] * factor);
+                *reinterpret_cast<float4 *>(&tile[wave][col][2 * i + 4 * half]) = v;
+            }
+            __syncthreads();
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float4 x = *reinterpret_cast<const float4 *>(&tile[w][oc][od]);
+                v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+            }
+            if (!whole) *reinterpret_cast<float4 *>(slot + oc * D + dt * 32 + od) = make_float4(v[0], v[1], v[2], v[3]);
+            else if (cc < ncols) store4(a, to + dt * 32, v);
+            __syncthreads();
+        }
+        u += units;
+    }
+    if (bad) zest::report(a.b.bad);
+}
+
+// Joins the pieces of the column tile whose run starts in workgroup w's share
+// and goes on past it, if there is one: theirs are the last of the share.
+template <int D>
+__global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
+    extern __shared__ __align__(16) int32_t attn_sh[];
+    int32_t * prefix = attn_sh;
+    const int ps = a.c.page_shift, W = gridDim.x;
+    zest::prefix_over_seqs(a.b, ps, prefix, [&](const kv_seq & s) { return cost_of(a, s); });
+    const int32_t total = prefix[a.b.seqs];
+    int32_t u0, u1;
+    share_of(total, blockIdx.x, W, u0, u1);
+    if (u0 == u1) return;
+    bool bad = false;
+    const int b = zest::seq_of(prefix, a.b.seqs, u1 - 1);
+    const kv_seq s = zest::load_seq(a.b, b, ps, bad);
+    const int32_t run = units_of(a, s), at = u1 - 1 - prefix[b], tiles = col_tiles(a, s);
+    const int32_t ct = at / run % tiles, h = at / run / tiles;
+    const int32_t start = prefix[b] + at / run * run, end = start + run;
+    if (start < u0 || end <= u1) return;
+    int last = blockIdx.x;
+    for (int32_t x0, x1 = u1; x1 < end;) share_of(total, ++last, W, x0, x1);
+    const int oc = threadIdx.x >> 3, od = (threadIdx.x & 7) * 4, cc = ct * COLS + oc;
+    if (cc >= s.n * a.group) return;
+    auto slot_of = [&](int w) { return a.partial + (int64_t) (2 * w + (w == (int) blockIdx.x)) * PARTIAL<D>; };
+    float m = -INFINITY;
+    for (int w = blockIdx.x; w <= last; w++) {
+        share_of(total, w, W, u0, u1);
+        if (u0 < u1) m = fmaxf(m, slot_of(w)[COLS * D + oc]);
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, o[D / 32][4] = {};
+    for (int w = blockIdx.x; w <= last; w++) {
+        share_of(total, w, W, u0, u1);
+        if (u0 == u1) continue;
+        const float * x = slot_of(w);
+        const float f = __builtin_amdgcn_exp2f(x[COLS * D + oc] - base);
+        l += x[COLS * D + COLS + oc] * f;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++) {
+            const float4 v = *reinterpret_cast<const float4 *>(x + oc * D + dt * 32 + od);
+            o[dt][0] += v.x * f, o[dt][1] += v.y * f, o[dt][2] += v.z * f, o[dt][3] += v.w * f;
+        }
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    const int64_t to = (int64_t) (s.row0 + cc / a.group) * a.ldo + (int64_t) (h * a.group + cc % a.group) * D + od;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; dt++) {
+        const float v[4] = {o[dt][0] * f, o[dt][1] * f, o[dt][2] * f, o[dt][3] * f};
+        store4(a, to + dt * 32, v);
+    }
+}
+
+// The most units a call's bounds allow, saturated.
+int64_t most_units(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
+    const int64_t run = std::max<int64_t>(1, ((int64_t) b->max_len + GROUP + UNIT - 1) / UNIT);
+    const int64_t tiles = std::min<int64_t>(((int64_t) b->rows * group + COLS - 1) / COLS + b->seqs,
+                                            ((int64_t) b->max_new * group + COLS - 1) / COLS * b->seqs);
+    return run * tiles * c->kv_heads;
+}
+
+int workgroups(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
+    return (int) std::min<int64_t>(most_units(c, b, group), MAX_WORKGROUPS);
+}
+
+template <int TYPE, int D> void launch(const attn_args & a, int W, hipStream_t s) {
+    const size_t lds = (size_t) ((a.b.seqs + 4) & ~3) * 4;
+    hipLaunchKernelGGL((attn_kernel<TYPE, D>), dim3(W), dim3(WAVES * 64), lds, s, a);
+    hipLaunchKernelGGL(combine_kernel<D>, dim3(W), dim3(256), lds, s, a);
+}
+
+template <int TYPE> void launch(const attn_args & a, int D, int W, hipStream_t s) {
+    switch (D) {
+        case 64: return launch<TYPE, 64>(a, W, s);
+        case 96: return launch<TYPE, 96>(a, W, s);
+        case 128: return launch<TYPE, 128>(a, W, s);
+        case 192: return launch<TYPE, 192>(a, W, s);
+        default: return launch<TYPE, 256>(a, W, s);
+    }
+}
+
+} // namespace
+
+extern "C" {
+
+size_t zest_kv_attn_workspace(const zest_kv_cache * cache, const zest_kv_batch * batch, int32_t q_heads) {
+    if (!cache || !batch || cache->kv_heads <= 0 || q_heads < cache->kv_heads || q_heads % cache->kv_heads) return 0;
+    if (batch->rows <= 0 || batch->seqs <= 0 || batch->max_new <= 0 || batch->max_len < 0) return 0;
+    return (size_t) 2 * workgroups(cache, batch, q_heads / cache->kv_heads) * COLS * (cache->head_dim + 2) * sizeof(float);
+}
+
+int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const void * q, int q_type, int64_t ldq,
+                 int32_t q_heads, float scale, int causal, int32_t window, float softcap, void * out, int out_type, int64_t ldo,
+                 void * workspace, size_t workspace_bytes, uint32_t * bad, void * stream) {
+    const char * me = "zest_kv_attn";
+    if (const int st = zest::kv_check_cache(cache, me)) return st;
+    if (const int st = zest::kv_check_batch(cache, batch, me)) return st;
+    ZEST_REQUIRE(q_heads > 0 && q_heads <= 4096 && q_heads % cache->kv_heads == 0, "%s: %d query heads for %d k/v heads", me,
+                 q_heads, cache->kv_heads);
+    const int64_t width = (int64_t) q_heads * cache->head_dim;
+    if (const int st = zest::kv_check_rows(q_type, q, ldq, width, me, "q")) return st;
+    if (const int st = zest::kv_check_rows(out_type, out, ldo, width, me, "out")) return st;
+    ZEST_REQUIRE(scale - scale == 0.0f && window >= 0 && softcap >= 0.0f && softcap - softcap == 0.0f,
+                 "%s: scale=%g window=%d softcap=%g", me, (double) scale, window, (double) softcap);
+    ZEST_REQUIRE(batch->rows * (int64_t) (q_heads / cache->kv_heads) < (1ll << 31) - 64, "%s: %lld rows of %d heads", me,
+                 (long long) batch->rows, q_heads);
+    const int64_t units = most_units(cache, batch, q_heads / cache->kv_heads);
+    ZEST_REQUIRE(units < (1ll << 31), "%s: a batch of %lld units of work", me, (long long) units);
+    const size_t need = zest_kv_attn_workspace(cache, batch, q_heads);
+    ZEST_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need,
+                 "%s: workspace of %zu bytes, 16-byte aligned, wanted", me, need);
+    attn_args a{};
+    a.c = zest::kv_pages_of(cache);
+    a.b = zest::kv_batch_of(batch, bad);
+    a.q = q, a.out = out, a.ldq = ldq, a.ldo = ldo;
+    a.q_type = q_type, a.out_type = out_type;
+    a.group = q_heads / cache->kv_heads;
+    a.causal = causal != 0, a.window = window, a.scale = scale, a.softcap = softcap;
+    a.partial = (float *) workspace;
+    const int W = workgroups(cache, batch, a.group);
+    const hipStream_t s = zest::as_stream(stream);
+    if (cache->type == ZEST_TYPE_BF16) launch<ZEST_TYPE_BF16>(a, cache->head_dim, W, s);
+    else launch<ZEST_TYPE_F16>(a, cache->head_dim, W, s);
+    return zest::check_launch(me);
+}
+
+} // extern "C"

@@ -1,0 +1,701 @@
+// The paged KV cache's upkeep: rope and the append into the pages, the
+// scheduler's step over the page tables, compaction of the pool.
+#include <algorithm>
+#include <cmath>
+
+#include "kv_device.h"
+#include "zest_common.h"
+
+namespace zest {
+
+int kv_check_cache(const zest_kv_cache * c, const char * what) {
+    ZEST_REQUIRE(c && c->pool, "%s: null cache", what);
+    ZEST_REQUIRE(c->pages > 0 && c->pages <= (1 << 24), "%s: %lld pages (1 to 2^24)", what, (long long) c->pages);
+    ZEST_REQUIRE(c->kv_heads > 0 && c->kv_heads <= 1024, "%s: kv_heads=%d (1 to 1024)", what, c->kv_heads);
+    const int d = c->head_dim, p = c->page_tokens;
+    if (c->type != ZEST_TYPE_F16 && c->type != ZEST_TYPE_BF16)
+        return fail(ZEST_E_UNSUPPORTED, "%s: cache type %d (F16 or BF16)", what, c->type);
+    if (d != 64 && d != 96 && d != 128 && d != 192 && d != 256)
+        return fail(ZEST_E_UNSUPPORTED, "%s: head_dim=%d (64, 96, 128, 192 or 256)", what, d);
+    if (p != 16 && p != 32 && p != 64 && p != 128 && p != 256)
+        return fail(ZEST_E_UNSUPPORTED, "%s: page_tokens=%d (16, 32, 64, 128 or 256)", what, p);
+    ZEST_REQUIRE((reinterpret_cast<uintptr_t>(c->pool) & 15) == 0, "%s: the pool must be 16-byte aligned", what);
+    return ZEST_OK;
+}
+
+int kv_check_batch(const zest_kv_cache * c, const zest_kv_batch * b, const char * what) {
+    ZEST_REQUIRE(b && b->tables && b->lens && b->starts, "%s: null batch", what);
+    ZEST_REQUIRE(b->seqs > 0 && b->seqs <= KV_MAX_SEQS, "%s: %d sequences (1 to %d)", what, b->seqs, KV_MAX_SEQS);
+    ZEST_REQUIRE(b->rows > 0 && b->rows < (1 << 30), "%s: %lld rows", what, (long long) b->rows);
+    ZEST_REQUIRE(b->table_rows > 0 && b->table_cols > 0 && (int64_t) b->table_cols * c->page_tokens < (1ll << 31),
+                 "%s: page tables of %d x %d", what, b->table_rows, b->table_cols);
+    ZEST_REQUIRE(b->slots || b->seqs <= b->table_rows, "%s: %d sequences of %d slots", what, b->seqs, b->table_rows);
+    ZEST_REQUIRE(b->max_new > 0 && b->max_new <= b->rows && b->max_len >= 0, "%s: max_new=%d max_len=%d of %lld rows", what,
+                 b->max_new, b->max_len, (long long) b->rows);
+    return ZEST_OK;
+}
+
+int kv_check_rows(int type, const void * p, int64_t ld, int64_t width, const char * what, const char * name) {
+    const int size = kv_type_bytes(type);
+    if (!size) return fail(ZEST_E_UNSUPPORTED, "%s: %s of type %d (F32, F16 or BF16)", what, name, type);
+    ZEST_REQUIRE(p, "%s: null %s", what, name);
+    ZEST_REQUIRE(ld >= width, "%s: %s rows of %lld values, %lld apart", what, name, (long long) width, (long long) ld);
+    ZEST_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * size % 16 == 0, "%s: %s rows must be 16-byte aligned", what,
+                 name);
+    return ZEST_OK;
+}
+
+} // namespace zest
+
+namespace {
+
+using zest::kv_batch;
+using zest::kv_pages;
+using zest::kv_seq;
+
+// ---- append ---------------------------------------------------------------------
+
+// Eight values of a row of type F32, F16 or BF16 at element offset e (a
+// multiple of 4 for F32 and 8 else: whole 16-byte pieces), as floats.
+__device__ inline void load8(const void * p, int type, int64_t e, float v[8]) {
+    if (type == ZEST_TYPE_F32) {
+        const float4 a = *reinterpret_cast<const float4 *>((const float *) p + e);
+        const float4 b = *reinterpret_cast<const float4 *>((const float *) p + e + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        return;
+    }
+    const uint4 q = *reinterpret_cast<const uint4 *>((const uint16_t *) p + e);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (type == ZEST_TYPE_BF16) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            v[2 * i] = (float) __builtin_bit_cast(_Float16, (uint16_t) w[i]);
+            v[2 * i + 1] = (float) __builtin_bit_cast(_Float16, (uint16_t) (w[i] >> 16));
+        }
+    }
+}
+
+__device__ inline float load1(const void * p, int type, int64_t e) {
+    if (type == ZEST_TYPE_F32) return ((const float *) p)[e];
+    const uint16_t w = ((const uint16_t *) p)[e];
+    return type == ZEST_TYPE_BF16 ? __uint_as_float((uint32_t) w << 16) : (float) __builtin_bit_cast(_Float16, w);
+}
+
+// One value in a 16-bit type, rounded to nearest even.
+__device__ inline uint16_t to16(float v, int type) {
+    return type == ZEST_TYPE_BF16 ? __builtin_bit_cast(uint16_t, (__bf16) v) : __builtin_bit_cast(uint16_t, (_Float16) v);
+}
+
+__device__ inline uint4 pack8(const float v[8], int type) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = (uint32_t) to16(v[2 * i], type) | ((uint32_t) to16(v[2 * i + 1], type) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct append_args {
+    kv_pages c;
+    kv_batch b;
+    int32_t d, cache_type, in_type, q_out_type, q_heads, heads_each;
+    const void * k, * v, * q;
+    void * q_out;
+    int64_t ldk, ldv, ldq, ldq_out;
+    const double * freqs;  // null: no rope
+    int32_t rot, neox;
+    float magnitude;
+    const int32_t * pos;
+};
+
+// One workgroup takes the new tokens within 16 consecutive places of a
+// sequence (the unit in which V is stored) and heads_each heads of q, then k,
+// then v. The angles of its tokens are made once, in shared memory: position *
+// frequency in 64 bits, reduced to a fraction of a turn there (rint and a
+// subtraction: exact to 2^-53 of the turns), and sine and cosine of that in 32.
+// HBM bound. K's lanes run over tokens first, so a piece row of 16 tokens is
+// 256 contiguous bytes; V's over columns, 8 tokens a lane, so a wave reads
+// whole rows and writes whole lines.
+__global__ __launch_bounds__(256) void append_kernel(append_args a) {
+    extern __shared__ __align__(16) int32_t append_sh[];
+    int32_t * prefix = append_sh;
+    float2 * turn = reinterpret_cast<float2 *>(append_sh + ((a.b.seqs + 1 + 3) & ~3));  // [16][rot / 2]
+    const int t = threadIdx.x, ps = a.c.page_shift;
+    zest::prefix_over_seqs(a.b, ps, prefix, [](const kv_seq & s) {
+        return s.n > 0 ? ((s.len - 1) >> 4) - ((s.len - s.n) >> 4) + 1 : 0;
+    });
+    if ((int32_t) blockIdx.x >= prefix[a.b.seqs]) return;
+    const int b = zest::seq_of(prefix, a.b.seqs, (int32_t) blockIdx.x);
+    bool bad = false;
+    const kv_seq s = zest::load_seq(a.b, b, ps, bad);
+    const int32_t first = s.len - s.n;                                               // place of the first new token
+    const int32_t p0 = ((first >> 4) + ((int32_t) blockIdx.x - prefix[b])) << 4;     // the 16 places
+    const int32_t lo = max(p0, first), hi = min(p0 + 16, s.len);                     // of them, new
+    const int32_t r0 = s.row0 + (lo - first);                                        // row of place lo
+    const int n = hi - lo, D = a.d, half = a.rot / 2;
+
+    int32_t page = -1;
+    if (p0 >= 0) {
+        page = a.b.tables[(int64_t) s.slot * a.b.table_cols + (p0 >> ps)];
+        if ((uint32_t) page >= (uint32_t) a.c.pages) page = -1;
+    }
+    if (page < 0 && t == 0 && blockIdx.y == 0) zest::report(a.b.bad);
+
+    const int total = a.q_heads + 2 * a.c.kv_heads;
+    const int head0 = blockIdx.y * a.heads_each, head1 = min(head0 + a.heads_each, total);
+    if (a.freqs && head0 < a.q_heads + a.c.kv_heads) {
+        for (int i = t; i < n * half; i += 256) {
+            const int tok = i / half, p = i - tok * half;
+            const double x = (double) (a.pos ? a.pos[r0 + tok] : lo + tok) * a.freqs[p] * 0.15915494309189535;  // turns
+            const float f = (float) (x - rint(x));
+            float sn, cs;
+            sincospif(2.0f * f, &sn, &cs);
+            turn[i] = make_float2(cs * a.magnitude, sn * a.magnitude);
+        }
+        __syncthreads();
+    }
+
+    const int P = 1 << ps;
+    uint16_t * held = reinterpret_cast<uint16_t *>(a.c.pool + (int64_t) (page < 0 ? 0 : page) * a.c.page_bytes);
+    // A token's head as items, each one lane's: two pieces of 8 that turn with
+    // each other (NeoX halves of whole pieces), one piece, or, where a half is
+    // not whole pieces, one pair or one value. An item is read before it is
+    // written, so q_out may be q.
+    const bool paired = a.neox && half % 8 == 0, single = a.neox && half % 8 != 0;
+    const int turning = paired ? half / 8 : single ? half : 0;
+    const int items = single ? half + (D - a.rot) : paired ? half / 8 + (D - a.rot) / 8 : D / 8;
+    auto item = [&](const void * x, int64_t ld, int head, int tok, int i, auto && put8, auto && put1) {
+        const int64_t at = (r0 + tok) * ld + (int64_t) head * D;
+        const float2 * cs = turn + tok * half;
+        float o[8], y[8];
+        if (paired && i < turning) {
+            load8(x, a.in_type, at + 8 * i, o);
+            load8(x, a.in_type, at + 8 * i + half, y);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float2 r = cs[8 * i + j];
+                const float x0 = o[j], x1 = y[j];
+                o[j] = fmaf(x0, r.x, -(x1 * r.y));
+                y[j] = fmaf(x0, r.y, x1 * r.x);
+            }
+            put8(8 * i, o);
+            put8(8 * i + half, y);
+        } else if (single) {
+            if (i < turning) {
+                const float x0 = load1(x, a.in_type, at + i), x1 = load1(x, a.in_type, at + i + half);
+                const float2 r = cs[i];
+                put1(i, fmaf(x0, r.x, -(x1 * r.y)));
+                put1(i + half, fmaf(x0, r.y, x1 * r.x));
+            } else {
+                put1(i + half, load1(x, a.in_type, at + i + half));
+            }
+        } else {
+            const int e = paired ? a.rot + 8 * (i - turning) : 8 * i;
+            load8(x, a.in_type, at + e, o);
+            if (a.freqs && !paired) {
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    if (e + j >= a.rot) break;
+                    const float2 r = cs[(e + j) / 2];
+                    const float x0 = o[j], x1 = o[j + 1];
+                    o[j] = fmaf(x0, r.x, -(x1 * r.y));
+                    o[j + 1] = fmaf(x0, r.y, x1 * r.x);
+                }
+            }
+            put8(e, o);
+        }
+    };
+
+    for (int head = head0; head < head1; head++) {
+        if (head < a.q_heads) {
+            for (int i = t; i < n * items; i += 256) {
+                const int tok = i / items;
+                const int64_t at = (r0 + tok) * a.ldq_out + (int64_t) head * D;
+                item(
+                    a.q, a.ldq, head, tok, i - tok * items,
+                    [&](int e, const float * o) {
+                        if (a.q_out_type == ZEST_TYPE_F32) {
+                            float * y = (float *) a.q_out + at + e;
+                            *reinterpret_cast<float4 *>(y) = make_float4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<float4 *>(y + 4) = make_float4(o[4], o[5], o[6], o[7]);
+                        } else {
+                            *reinterpret_cast<uint4 *>((uint16_t *) a.q_out + at + e) = pack8(o, a.q_out_type);
+                        }
+                    },
+                    [&](int e, float o) {
+                        if (a.q_out_type == ZEST_TYPE_F32) ((float *) a.q_out)[at + e] = o;
+                        else ((uint16_t *) a.q_out)[at + e] = to16(o, a.q_out_type);
+                    });
+            }
+            continue;
+        }
+        if (page < 0) continue;
+        const int kh = head - a.q_heads;
+        if (kh < a.c.kv_heads) {
+            uint16_t * dst = held + (int64_t) kh * 2 * P * D;
+            for (int i = t; i < 16 * items; i += 256) {
+                const int tok = (i & 15) + p0 - lo;
+                if (tok < 0 || tok >= n) continue;
+                uint16_t * y = dst + ((lo + tok) & (P - 1)) * 8;
+                item(
+                    a.k, a.ldk, kh, tok, i >> 4,
+                    [&](int e, const float * o) {
+                        *reinterpret_cast<uint4 *>(y + (int64_t) (e / 8) * P * 8) = pack8(o, a.cache_type);
+                    },
+                    [&](int e, float o) { y[(int64_t) (e / 8) * P * 8 + e % 8] = to16(o, a.cache_type); });
+            }
+            continue;
+        }
+        const int vh = kh - a.c.kv_heads;
+        uint16_t * dst = held + (int64_t) vh * 2 * P * D + (int64_t) P * D + (int64_t) ((p0 & (P - 1)) >> 4) * 16 * D;
+        for (int i = t; i < 2 * D; i += 256) {
+            const int h = i / D, e = i - h * D;
+            float o[8];
+            bool whole = true;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int tok = 4 * h + (j & 3) + (j >> 2) * 8 + p0 - lo;
+                const bool in = tok >= 0 && tok < n;
+                whole &= in;
+                o[j] = in ? load1(a.v, a.in_type, (r0 + tok) * a.ldv + (int64_t) vh * D + e) : 0.0f;
+            }
+            uint16_t * y = dst + (int64_t) i * 8;
+            if (whole) {
+                *reinterpret_cast<uint4 *>(y) = pack8(o, a.cache_type);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int tok = 4 * h + (j & 3) + (j >> 2) * 8 + p0 - lo;
+                    if (tok >= 0 && tok < n) y[j] = to16(o[j], a.cache_type);
+                }
+            }
+        }
+    }
+}
+
+// ---- the scheduler's step --------------------------------------------------------
+
+constexpr int MAX_SLOTS = 65536, MAX_ENTRIES = 65536;
+constexpr int STEP = 1024;  // threads of the one workgroup that walks the tables
+
+// A count that other threads of this workgroup changed with atomics: read past
+// the vector cache.
+__device__ inline int32_t fresh(const int32_t * p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Exclusive scan of one value a thread over a 1024-thread workgroup; *total its
+// sum. Ends in a barrier.
+__device__ inline int32_t scan_step(int32_t v, int32_t * total) {
+    __shared__ int32_t sums[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int32_t s = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int32_t u = __shfl_up(s, off);
+        if (lane >= off) s += u;
+    }
+    if (lane == 63) sums[wave] = s;
+    __syncthreads();
+    int32_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        before += w < wave ? sums[w] : 0;
+        all += sums[w];
+    }
+    __syncthreads();
+    *total = all;
+    return before + s - v;
+}
+
+// An entry between the phases of assign_kernel (base -1: left undone).
+struct assign_entry {
+    int32_t base, need, first, old_pages;
+};
+
+struct assign_args {
+    int32_t * refs, * tables, * lens;
+    const int32_t * dst, * src, * grow;
+    int32_t n, rows, cols, pages, page_shift;
+    assign_entry * entries;  // [n]
+    int2 * copies;           // [n]: the page a fork's open page is copied from, and to (-1: none)
+    int32_t * free_list;     // [pages]
+    uint32_t * bad;
+};
+
+// The tables' part of a step, by one workgroup: its phases are ordered by
+// barriers, so every count is exact and the result does not depend on the order
+// of the atomics (sums only). Latency bound: a few passes over the entries'
+// rows and one over refs up to the last page taken.
+__global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
+    __shared__ uint32_t seen[MAX_SLOTS / 32], twice[MAX_SLOTS / 32], replaced[MAX_SLOTS / 32];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int P = 1 << a.page_shift;
+    bool bad = false;
+    for (int i = t; i < (a.rows + 31) / 32; i += STEP) seen[i] = twice[i] = replaced[i] = 0;
+    __syncthreads();
+    for (int i = t; i < a.n; i += STEP) {
+        const int32_t d = a.dst[i];
+        if ((uint32_t) d >= (uint32_t) a.rows) continue;
+        const uint32_t bit = 1u << (d & 31);
+        if (atomicOr(&seen[d >> 5], bit) & bit) atomicOr(&twice[d >> 5], bit);
+        if (a.src[i] != d) atomicOr(&replaced[d >> 5], bit);
+    }
+    __syncthreads();
+    auto has = [](const uint32_t * set, int32_t d) { return (set[d >> 5] >> (d & 31)) & 1u; };
+
+    // what each entry needs
+    for (int i = t; i < a.n; i += STEP) {
+        const int32_t d = a.dst[i], s = a.src[i], g = a.grow[i];
+        assign_entry e{-1, 0, 0, 0};
+        const bool named = (uint32_t) d < (uint32_t) a.rows && s >= -1 && s < a.rows;
+        if (named && !has(twice, d) && (s < 0 || s == d || !has(replaced, s)) && g >= 0) {
+            const int64_t base = s >= 0 ? a.lens[s] : 0, room = (int64_t) a.cols << a.page_shift, old = a.lens[d];
+            if (base >= 0 && base + g <= room && old >= 0 && old <= room) {
+                e.base = (int32_t) base;
+                const int32_t held = (int32_t) (s == d ? (base + P - 1) >> a.page_shift : base >> a.page_shift);
+                e.need = (int32_t) ((base + g + P - 1) >> a.page_shift) - held;
+                e.old_pages = s == d ? 0 : (int32_t) ((old + P - 1) >> a.page_shift);
+            }
+        }
+        bad |= e.base < 0;
+        a.entries[i] = e;
+        a.copies[i] = make_int2(-1, -1);
+    }
+    __syncthreads();
+
+    // the replaced rows' pages are released, a wave an entry
+    for (int i = wave; i < a.n; i += STEP / 64) {
+        const assign_entry e = a.entries[i];
+        if (e.base < 0 || e.old_pages == 0) continue;
+        const int32_t * row = a.tables + (int64_t) a.dst[i] * a.cols;
+        for (int j = lane; j < e.old_pages; j += 64) {
+            const int32_t id = row[j];
+            if ((uint32_t) id >= (uint32_t) a.pages) bad = true;
+            else if (atomicSub(&a.refs[id], 1) <= 0) {  // not counted: left at what it was
+                atomicAdd(&a.refs[id], 1);
+                bad = true;
+            }
+        }
+    }
+    __threadfence();
+    __syncthreads();
+
+    // each entry's place in the list of free pages
+    int32_t want = 0;
+    for (int i0 = 0; i0 < a.n; i0 += STEP) {
+        const int i = i0 + t;
+        int32_t sum;
+        const int32_t before = scan_step(i < a.n ? a.entries[i].need : 0, &sum);
+        if (i < a.n) a.entries[i].first = want + before;
+        want += sum;
+    }
+    int32_t found = 0;
+    for (int p0 = 0; p0 < a.pages && found < want; p0 += STEP) {
+        const int p = p0 + t;
+        const bool is_free = p < a.pages && fresh(&a.refs[p]) <= 0;
+        int32_t sum;
+        const int32_t before = scan_step(is_free, &sum);
+        if (is_free && found + before < want) a.free_list[found + before] = p;
+        found += sum;
+    }
+    __threadfence();
+    __syncthreads();
+
+    // the new rows, a wave an entry
+    for (int i = wave; i < a.n; i += STEP / 64) {
+        const assign_entry e = a.entries[i];
+        if (e.base < 0) continue;
+        const int32_t d = a.dst[i], s = a.src[i], g = a.grow[i];
+        int32_t * row = a.tables + (int64_t) d * a.cols;
+        const bool fits = e.need == 0 || e.first + e.need <= found;
+        bad |= !fits;
+        if (s == d) {
+            if (!fits) continue;
+            const int32_t held = (e.base + P - 1) >> a.page_shift;
+            for (int j = lane; j < e.need; j += 64) {
+                const int32_t id = a.free_list[e.first + j];
+                row[held + j] = id;
+                a.refs[id] = 1;
+            }
+            if (lane == 0) a.lens[d] = e.base + g;
+            continue;
+        }
+        const int32_t * parent = a.tables + (int64_t) max(s, 0) * a.cols;
+        const int32_t shared = fits ? e.base >> a.page_shift : 0, total = fits ? shared + e.need : 0;
+        for (int j = lane; j < a.cols; j += 64) {
+            int32_t id = -1;
+            if (j < shared) {
+                id = parent[j];
+                if ((uint32_t) id < (uint32_t) a.pages) atomicAdd(&a.refs[id], 1);
+                else bad = true;
+            } else if (j < total) {
+                id = a.free_list[e.first + j - shared];
+                a.refs[id] = 1;
+                if (j == shared && (e.base & (P - 1))) {
+                    const int32_t from = parent[j];
+                    if ((uint32_t) from < (uint32_t) a.pages) a.copies[i] = make_int2(from, id);
+                    else bad = true;
+                }
+            }
+            row[j] = id;
+        }
+        if (lane == 0) a.lens[d] = fits ? e.base + g : 0;
+    }
+    if (bad) zest::report(a.bad);
+}
+
+// Copies whole pages in every layer: copies[i] = (from, to), -1 for none; with
+// `count` only the first *count. A workgroup takes COPY_BYTES of a page at a
+// time, four 16-byte loads a thread before the first store.
+constexpr int COPY_BYTES = 16384;
+
+__global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t * pool, int64_t page_bytes, int64_t layer_stride,
+                                                         int32_t layers, const int2 * copies, int32_t n,
+                                                         const int32_t * count) {
+    const int32_t parts = (int32_t) ((page_bytes + COPY_BYTES - 1) / COPY_BYTES);
+    const int64_t total = (int64_t) (count ? *count : n) * layers * parts;
+    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
+        const int32_t part = (int32_t) (w % parts), layer = (int32_t) (w / parts % layers);
+        const int2 c = copies[w / parts / layers];
+        if (c.x < 0) continue;
+        const int64_t at = layer * layer_stride + (int64_t) part * COPY_BYTES;
+        const int32_t left = (int32_t) min((int64_t) COPY_BYTES, page_bytes - (int64_t) part * COPY_BYTES);
+        const uint4 * from = reinterpret_cast<const uint4 *>(pool + at + c.x * page_bytes);
+        uint4 * to = reinterpret_cast<uint4 *>(pool + at + c.y * page_bytes);
+        const int t = threadIdx.x, last = left / 16 - 1;  // the part's end is read again rather than past it
+        const uint4 v0 = from[min(t, last)], v1 = from[min(t + 256, last)];
+        const uint4 v2 = from[min(t + 512, last)], v3 = from[min(t + 768, last)];
+        if (t <= last) to[t] = v0;
+        if (t + 256 <= last) to[t + 256] = v1;
+        if (t + 512 <= last) to[t + 512] = v2;
+        if (t + 768 <= last) to[t + 768] = v3;
+    }
+}
+
+// ---- compaction ------------------------------------------------------------------
+
+struct compact_args {
+    const int32_t * refs, * tables;
+    int32_t * refs_out, * tables_out, * live;
+    int32_t pages;
+    int64_t entries;
+    int2 * moves;       // [pages / 2 + 1]
+    int32_t * count;    // moves
+    int32_t * place;    // [pages]: where a page is afterwards, -1 for one without references
+    uint32_t * bad;
+};
+
+// Which page moves where, by one workgroup: a count of the live pages, then
+// the ranks of the free pages below it and of the live ones from it on, which
+// are equally many: rank k of one goes to rank k of the other.
+__global__ __launch_bounds__(STEP) void compact_plan_kernel(compact_args a) {
+    const int t = threadIdx.x;
+    int32_t mine = 0, live;
+    for (int p = t; p < a.pages; p += STEP) mine += a.refs[p] > 0;
+    scan_step(mine, &live);
+    int32_t holes = 0, movers = 0;
+    for (int p0 = 0; p0 < a.pages; p0 += STEP) {
+        const int p = p0 + t;
+        const bool used = p < a.pages && a.refs[p] > 0;
+        const bool hole = p < live && !used, moves = p >= live && used;
+        int32_t sum;
+        const int32_t before = scan_step(hole ? 1 : moves ? 0x10000 : 0, &sum);
+        if (hole) a.moves[holes + (before & 0xffff)].y = p;
+        if (moves) a.moves[movers + (before >> 16)].x = p;
+        if (p < a.pages) a.place[p] = used && !moves ? p : -1;
+        holes += sum & 0xffff;
+        movers += sum >> 16;
+    }
+    __threadfence();
+    __syncthreads();
+    for (int k = t; k < movers; k += STEP) a.place[a.moves[k].x] = a.moves[k].y;
+    if (t == 0) {
+        *a.count = movers;
+        *a.live = live;
+    }
+    // refs (refs_out may be refs): the live pages' counts at their new places,
+    // every free page below n filled, then zeros behind
+    for (int p = t; p < live; p += STEP) {
+        const int32_t r = a.refs[p];
+        if (r > 0) a.refs_out[p] = r;
+    }
+    for (int k = t; k < movers; k += STEP) a.refs_out[a.moves[k].y] = a.refs[a.moves[k].x];
+    __syncthreads();
+    for (int p = live + t; p < a.pages; p += STEP) a.refs_out[p] = 0;
+}
+
+__global__ __launch_bounds__(256) void compact_tables_kernel(compact_args a) {
+    bool bad = false;
+    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < a.entries; i += (int64_t) gridDim.x * 256) {
+        const int32_t id = a.tables[i];
+        const int32_t to = (uint32_t) id < (uint32_t) a.pages ? a.place[id] : -1;
+        bad |= to < 0 && id != -1;
+        a.tables_out[i] = to;
+    }
+    if (bad) zest::report(a.bad);
+}
+
+size_t round16(size_t n) { return (n + 15) & ~(size_t) 15; }
+
+int check_pool(const zest_kv_cache * c, int32_t layers, int64_t layer_stride, const int32_t * refs, const int32_t * tables,
+               int32_t table_rows, int32_t table_cols, const char * what) {
+    if (const int st = zest::kv_check_cache(c, what)) return st;
+    ZEST_REQUIRE(layers > 0 && layers <= 65536, "%s: %d layers", what, layers);
+    ZEST_REQUIRE(layers == 1 || (layer_stride % 16 == 0 && layer_stride >= c->pages * (int64_t) zest_kv_page_bytes(c)),
+                 "%s: layers %lld bytes apart", what, (long long) layer_stride);
+    ZEST_REQUIRE(refs && tables, "%s: null refs or tables", what);
+    ZEST_REQUIRE(table_rows > 0 && table_rows <= MAX_SLOTS && table_cols > 0 &&
+                     (int64_t) table_cols * c->page_tokens < (1ll << 31),
+                 "%s: page tables of %d x %d", what, table_rows, table_cols);
+    return ZEST_OK;
+}
+
+unsigned copy_grid(const zest_kv_cache * c, int32_t layers, int64_t n) {
+    const int64_t parts = ((int64_t) zest_kv_page_bytes(c) + COPY_BYTES - 1) / COPY_BYTES;
+    return (unsigned) std::min<int64_t>(n * layers * parts, 8192);
+}
+
+} // namespace
+
+extern "C" {
+
+size_t zest_kv_page_bytes(const zest_kv_cache * c) {
+    return c ? (size_t) c->kv_heads * 4 * (size_t) c->page_tokens * (size_t) c->head_dim : 0;
+}
+
+int zest_kv_rope_freqs(int32_t n_dims, double freq_base, double freq_scale, double ext_factor, double attn_factor,
+                       double corr0, double corr1, const float * ff, double * out, float * magnitude) {
+    ZEST_REQUIRE(out && magnitude, "zest_kv_rope_freqs: null pointer");
+    ZEST_REQUIRE(n_dims > 0 && n_dims % 2 == 0, "zest_kv_rope_freqs: n_dims=%d", n_dims);
+    ZEST_REQUIRE(freq_base > 0 && freq_scale > 0, "zest_kv_rope_freqs: base %g, scale %g", freq_base, freq_scale);
+    for (int p = 0; p < n_dims / 2; p++) {
+        const double f = std::pow(freq_base, -2.0 * p / n_dims) / (ff ? (double) ff[p] : 1.0);
+        const double y = (p - corr0) / std::max(0.001, corr1 - corr0);
+        const double mix = (1.0 - std::min(1.0, std::max(0.0, y))) * ext_factor;
+        out[p] = f * (freq_scale * (1.0 - mix) + mix);
+    }
+    *magnitude = (float) (attn_factor * (ext_factor != 0.0 ? 1.0 + 0.1 * std::log(1.0 / freq_scale) : 1.0));
+    return ZEST_OK;
+}
+
+int zest_kv_append(const zest_kv_cache * cache, const zest_kv_batch * batch, const zest_kv_rope * rope, const int32_t * pos,
+                   int in_type, const void * k, int64_t ldk, const void * v, int64_t ldv, const void * q, int64_t ldq,
+                   int32_t q_heads, void * q_out, int64_t ldq_out, int q_out_type, uint32_t * bad, void * stream) {
+    const char * me = "zest_kv_append";
+    if (const int st = zest::kv_check_cache(cache, me)) return st;
+    if (const int st = zest::kv_check_batch(cache, batch, me)) return st;
+    const int64_t width = (int64_t) cache->kv_heads * cache->head_dim;
+    if (const int st = zest::kv_check_rows(in_type, k, ldk, width, me, "k")) return st;
+    if (const int st = zest::kv_check_rows(in_type, v, ldv, width, me, "v")) return st;
+    if (q) {
+        ZEST_REQUIRE(q_heads > 0 && q_heads <= 4096, "%s: q_heads=%d (1 to 4096)", me, q_heads);
+        if (const int st = zest::kv_check_rows(in_type, q, ldq, (int64_t) q_heads * cache->head_dim, me, "q")) return st;
+        if (const int st = zest::kv_check_rows(q_out_type, q_out, ldq_out, (int64_t) q_heads * cache->head_dim, me, "q_out"))
+            return st;
+        const uint8_t * x = (const uint8_t *) q, * y = (const uint8_t *) q_out;
+        const int64_t last = batch->rows - 1, w = (int64_t) q_heads * cache->head_dim;  // spans of the rows in bytes
+        const int64_t xb = (last * ldq + w) * zest::kv_type_bytes(in_type), yb = (last * ldq_out + w) * zest::kv_type_bytes(q_out_type);
+        ZEST_REQUIRE((q == q_out && ldq == ldq_out && in_type == q_out_type) || x + xb <= y || y + yb <= x,
+                     "%s: q_out overlaps q without being q", me);
+    }
+    if (rope) {
+        ZEST_REQUIRE(rope->freqs && (reinterpret_cast<uintptr_t>(rope->freqs) & 7) == 0, "%s: null or misaligned freqs", me);
+        ZEST_REQUIRE(rope->n_dims > 0 && rope->n_dims % 2 == 0 && rope->n_dims <= cache->head_dim, "%s: n_dims=%d of %d", me,
+                     rope->n_dims, cache->head_dim);
+        ZEST_REQUIRE(rope->mode == 0 || rope->mode == 2, "%s: rope mode %d (normal 0 or neox 2)", me, rope->mode);
+    }
+    append_args a{};
+    a.c = zest::kv_pages_of(cache);
+    a.b = zest::kv_batch_of(batch, bad);
+    a.d = cache->head_dim;
+    a.cache_type = cache->type;
+    a.in_type = in_type;
+    a.q_out_type = q_out_type;
+    a.q_heads = q ? q_heads : 0;
+    a.k = k, a.v = v, a.q = q, a.q_out = q_out;
+    a.ldk = ldk, a.ldv = ldv, a.ldq = ldq, a.ldq_out = ldq_out;
+    if (rope) {
+        a.freqs = rope->freqs;
+        a.rot = rope->n_dims;
+        a.neox = rope->mode == 2;
+        a.magnitude = rope->magnitude;
+    }
+    a.pos = pos;
+    // n new tokens of a sequence touch at most n / 16 + 2 units of 16 places, and at most n
+    const int64_t units = std::min<int64_t>(batch->rows, batch->rows / 16 + 2ll * batch->seqs);
+    const int heads = a.q_heads + 2 * a.c.kv_heads;
+    a.heads_each = (int) std::max<int64_t>(1, std::min<int64_t>(8, units * heads / 1024));
+    const size_t lds = (size_t) ((batch->seqs + 4) & ~3) * 4 + (size_t) 16 * (a.rot / 2) * sizeof(float2);
+    hipLaunchKernelGGL(append_kernel, dim3((unsigned) units, (unsigned) ((heads + a.heads_each - 1) / a.heads_each)), dim3(256),
+                       lds, zest::as_stream(stream), a);
+    return zest::check_launch(me);
+}
+
+size_t zest_kv_scratch_bytes(int64_t pages, int32_t n) {
+    if (pages <= 0 || n < 0) return 0;
+    const size_t assign = round16((size_t) n * sizeof(assign_entry)) + round16((size_t) n * sizeof(int2)) + round16((size_t) pages * 4);
+    const size_t compact = round16((size_t) (pages / 2 + 1) * sizeof(int2)) + 16 + round16((size_t) pages * 4);
+    return std::max(assign, compact);
+}
+
+int zest_kv_assign(const zest_kv_cache * cache, int32_t layers, int64_t layer_stride, int32_t * refs, int32_t * tables,
+                   int32_t * lens, int32_t table_rows, int32_t table_cols, const int32_t * dst, const int32_t * src,
+                   const int32_t * grow, int32_t n, void * scratch, size_t scratch_bytes, uint32_t * bad, void * stream) {
+    const char * me = "zest_kv_assign";
+    if (const int st = check_pool(cache, layers, layer_stride, refs, tables, table_rows, table_cols, me)) return st;
+    ZEST_REQUIRE(lens && dst && src && grow, "%s: null pointer", me);
+    ZEST_REQUIRE(n > 0 && n <= MAX_ENTRIES, "%s: %d entries (1 to %d)", me, n, MAX_ENTRIES);
+    ZEST_REQUIRE(scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0 &&
+                     scratch_bytes >= zest_kv_scratch_bytes(cache->pages, n),
+                 "%s: scratch of %zu bytes, 16-byte aligned, wanted", me, zest_kv_scratch_bytes(cache->pages, n));
+    assign_args a{};
+    a.refs = refs, a.tables = tables, a.lens = lens;
+    a.dst = dst, a.src = src, a.grow = grow;
+    a.n = n, a.rows = table_rows, a.cols = table_cols, a.pages = (int32_t) cache->pages;
+    a.page_shift = zest::kv_page_shift(cache->page_tokens);
+    uint8_t * at = (uint8_t *) scratch;
+    a.entries = (assign_entry *) at;
+    at += round16((size_t) n * sizeof(assign_entry));
+    a.copies = (int2 *) at;
+    at += round16((size_t) n * sizeof(int2));
+    a.free_list = (int32_t *) at;
+    a.bad = bad;
+    const hipStream_t s = zest::as_stream(stream);
+    hipLaunchKernelGGL(assign_kernel, dim3(1), dim3(STEP), 0, s, a);
+    if (const int st = zest::check_launch(me)) return st;
+    hipLaunchKernelGGL(copy_pages_kernel, dim3(copy_grid(cache, layers, n)), dim3(256), 0, s, (uint8_t *) cache->pool,
+                       (int64_t) zest_kv_page_bytes(cache), layer_stride, layers, a.copies, n, (const int32_t *) nullptr);
+    return zest::check_launch(me);
+}
+
+int zest_kv_compact(const zest_kv_cache * cache, int32_t layers, int64_t layer_stride, const int32_t * refs,
+                    const int32_t * tables, int32_t table_rows, int32_t table_cols, int32_t * refs_out, int32_t * tables_out,
+                    int32_t * live, void * scratch, size_t scratch_bytes, uint32_t * bad, void * stream) {
+    const char * me = "zest_kv_compact";
+    if (const int st = check_pool(cache, layers, layer_stride, refs, tables, table_rows, table_cols, me)) return st;
+    ZEST_REQUIRE(refs_out && tables_out && live, "%s: null pointer", me);
+    ZEST_REQUIRE(scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0 &&
+                     scratch_bytes >= zest_kv_scratch_bytes(cache->pages, 0),
+                 "%s: scratch of %zu bytes, 16-byte aligned, wanted", me, zest_kv_scratch_bytes(cache->pages, 0));
+    compact_args a{};
+    a.refs = refs, a.tables = tables, a.refs_out = refs_out, a.tables_out = tables_out, a.live = live;
+    a.pages = (int32_t) cache->pages;
+    a.entries = (int64_t) table_rows * table_cols;
+    uint8_t * at = (uint8_t *) scratch;
+    a.moves = (int2 *) at;
+    at += round16((size_t) (cache->pages / 2 + 1) * sizeof(int2));
+    a.count = (int32_t *) at;
+    a.place = (int32_t *) (at + 16);
+    a.bad = bad;
+    const hipStream_t s = zest::as_stream(stream);
+    hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(STEP), 0, s, a);
+    if (const int st = zest::check_launch(me)) return st;
+    hipLaunchKernelGGL(compact_tables_kernel, dim3((unsigned) std::min<int64_t>((a.entries + 255) / 256, 1024)), dim3(256), 0, s,
+                       a);
+    if (const int st = zest::check_launch(me)) return st;
+    hipLaunchKernelGGL(copy_pages_kernel, dim3(copy_grid(cache, layers, cache->pages / 2 + 1)), dim3(256), 0, s,
+                       (uint8_t *) cache->pool, (int64_t) zest_kv_page_bytes(cache), layer_stride, layers, a.moves, 0, a.count);
+    return zest::check_launch(me);
+}
+
+} // extern "C"

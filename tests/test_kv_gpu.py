@@ -1,0 +1,505 @@
+"""The paged KV cache's kernels against their plain 64-bit forms (kv_ref), at the
+sizes, masks and contents where they can go wrong. The pool's unused places,
+behind a sequence's end included, hold NaN throughout."""
+from __future__ import annotations
+
+import math
+
+import kv_ref
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def kv(zest_gpu):
+    from ggml_xdna_amd import kv as m
+    return m
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _starts(new):
+    return [sum(new[:i]) for i in range(len(new) + 1)]
+
+
+def _flag():
+    return torch.zeros(1, dtype=torch.int32, device="cuda")
+
+
+class Case:
+    """A batch over a Book: q on the CPU, the cache and the batch on the GPU."""
+
+    def __init__(self, kv, seqs, page=16, kv_heads=2, group=2, d=64, dtype=BF16, q_dtype=None, seed=0, q_scale=2.0, **more):
+        self.new, lens = [n for n, _ in seqs], [m for _, m in seqs]
+        self.book = kv_ref.Book(lens, page, kv_heads, d, dtype, seed, **more)
+        self.starts, self.rows, self.heads = _starts(self.new), sum(self.new), kv_heads * group
+        g = torch.Generator().manual_seed(seed + 1)
+        self.q = (q_scale * torch.randn((self.rows, self.heads, d), generator=g)).to(q_dtype or dtype)
+        self.cache = self.book.cache(kv)
+        self.batch = kv.Batch(_i32(self.starts), self.rows, max(self.new + [1]), max(lens + [1]))
+
+    def check(self, got, causal=True, window=0, softcap=0.0, scale=None, unseen=None):
+        b = self.book
+        scale = 1.0 / math.sqrt(b.d) if scale is None else scale
+        got = got.cpu().reshape(self.rows, self.heads, b.d)
+        for i, n in enumerate(self.new):
+            r = slice(self.starts[i], self.starts[i] + n)
+            q = self.q[r].to(b.dtype)
+            out, spread, reach = kv_ref.attention(q, b.k[i], b.v[i], scale, causal, window, softcap,
+                                                  unseen=None if unseen is None else unseen[i])
+            bound = kv_ref.attention_bound(out, spread, reach, b.d, b.dtype, got.dtype)
+            off = (got[r].double() - out).abs()
+            assert bool((off <= bound).all()), (i, n, b.lens[i], float((off / bound).max()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d,group,page", [(64, 1, 16), (64, 2, 32), (96, 3, 64), (128, 4, 64), (128, 6, 128), (192, 5, 16),
+                                          (256, 8, 32), (128, 32, 256), (64, 33, 16)])
+def test_attention(kv, dtype, d, group, page):
+    """Every head width, page size and group shape (more columns than a tile among them) over one token to a few
+    hundred: lengths around the pages, the 16-, 32- and 128-token units and a tile's columns."""
+    seqs = [(1, 1), (1, 15), (1, 16), (1, 17), (2, 31), (1, 32), (3, 33), (1, 127), (5, 129), (1, 300), (40, 40), (33, 161)]
+    c = Case(kv, seqs, page, 2 if group < 8 else 1, group, d, dtype, seed=d + group)
+    bad = _flag()
+    got = kv.attention(c.cache, 0, c.batch, c.q.cuda(), bad=bad)
+    assert got.dtype == dtype and got.shape == c.q.shape
+    c.check(got)
+    assert int(bad) == 0
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window,softcap,scale", [(0, 0.0, 0.3), (1, 0.0, None), (7, 0.0, None), (40, 5.0, None), (500, 0.0, None),
+                                                 (0, 2.0, None), (0, 0.0, 0.0), (0, 0.0, -0.2)])
+def test_attention_masks(kv, causal, window, softcap, scale):
+    c = Case(kv, [(1, 50), (20, 20), (9, 200), (70, 130), (1, 1)], 32, 2, 3, 64, BF16, seed=window)
+    c.check(kv.attention(c.cache, 0, c.batch, c.q.cuda(), scale, causal, window, softcap), causal, window, softcap, scale)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("q_dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("out_dtype", [F32, F16, BF16])
+def test_attention_types_and_strides(kv, dtype, q_dtype, out_dtype):
+    """q and the output of any type, as column slices of wider buffers; the rest of the output's buffer stays as it was."""
+    c = Case(kv, [(3, 20), (1, 64), (17, 100)], 16, 2, 2, 64, dtype, q_dtype, seed=3)
+    wide = torch.full((c.rows, 3 * 256), math.nan, dtype=q_dtype, device="cuda")
+    wide[:, 256:512] = c.q.reshape(c.rows, 256)
+    out = torch.full((c.rows, 2 * 256 + 16), 7.0, dtype=out_dtype, device="cuda")
+    got = kv.attention(c.cache, 0, c.batch, wide[:, 256:512], out=out[:, 16:272])
+    c.check(got)
+    assert bool((out[:, :16] == 7).all()) and bool((out[:, 272:] == 7).all())
+
+
+def test_attention_split_over_workgroups(kv):
+    """Contexts long enough that a column tile's keys are split among workgroups and joined, beside short ones; the
+    same bits from run to run."""
+    c = Case(kv, [(1, 5000), (2, 700), (1, 1), (3, 9001)], 64, 2, 4, 128, BF16, seed=9)
+    q = c.q.cuda()
+    got = kv.attention(c.cache, 0, c.batch, q, out_dtype=F32)
+    c.check(got)
+    for _ in range(3):
+        assert torch.equal(kv.attention(c.cache, 0, c.batch, q, out_dtype=F32), got)
+
+
+def test_attention_long_chunk(kv):
+    """A chunk of many column tiles, on top of what its sequence holds."""
+    c = Case(kv, [(150, 400), (1, 70), (260, 260)], 32, 1, 2, 128, BF16, seed=11)
+    c.check(kv.attention(c.cache, 0, c.batch, c.q.cuda()))
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_values_a_row_does_not_see_do_not_reach_it(kv, value, dtype):
+    """K or V of a token that holds NaN or an infinity: only the rows that see it change."""
+    c = Case(kv, [(40, 90), (1, 33)], 16, 1, 2, 64, dtype, seed=5)
+    clean = kv.attention(c.cache, 0, c.batch, c.q.cuda()).cpu()
+    late = 70  # token 70 of 90 is seen by the new tokens from place 70 on: rows 20 to 39
+    c.book.v[0][late, 0, 5] = value
+    c.book.fill()
+    c.cache = c.book.cache(kv)
+    got = kv.attention(c.cache, 0, c.batch, c.q.cuda()).cpu()
+    assert torch.equal(got[:20], clean[:20]) and torch.equal(got[40:], clean[40:])
+    assert torch.equal(got[20:40, :, :5], clean[20:40, :, :5]) and torch.equal(got[20:40, :, 6:], clean[20:40, :, 6:])
+    hit = got[20:40, :, 5].float()
+    assert bool(hit.isnan().all()) if math.isnan(value) else bool((hit == value).all())
+    # a window that leaves the token behind
+    win = kv.attention(c.cache, 0, c.batch, c.q.cuda(), window=10).cpu()
+    assert bool(win[30:40].isfinite().all()) and not bool(win[20:30, :, 5].isfinite().any())
+    # and the same in K
+    c.book.v[0][late, 0, 5] = 1.0
+    c.book.k[0][late, 0, 5] = value
+    c.book.fill()
+    c.cache = c.book.cache(kv)
+    got = kv.attention(c.cache, 0, c.batch, c.q.cuda()).cpu()
+    assert torch.equal(got[:20], clean[:20])
+
+
+def test_rows_that_see_nothing_are_zero(kv):
+    """Rows before a sequence's start (lens below the new tokens), a sequence of length 0, scores of -infinity alone;
+    rows behind the last sequence and of one without new tokens stay as they were."""
+    c = Case(kv, [(6, 6), (2, 20), (3, 3)], 16, 1, 2, 64, BF16, seed=6)
+    c.cache.lens.copy_(_i32([4, 20, 0]))
+    out = torch.full((c.rows + 2, 2, 64), 9.0, dtype=BF16, device="cuda")
+    q = torch.cat([c.q, torch.zeros(2, 2, 64, dtype=BF16)]).cuda()
+    batch = kv.Batch(_i32(c.starts), c.rows + 2, 6, 20)
+    bad = _flag()
+    kv.attention(c.cache, 0, batch, q, out=out, bad=bad)
+    assert bool((out[:2] == 0).all()) and bool((out[8:11] == 0).all()) and bool((out[11:] == 9).all())
+    want, spread, reach = kv_ref.attention(c.q[2:6], c.book.k[0][:4], c.book.v[0][:4], 0.125)
+    assert bool(((out[2:6].cpu().double() - want).abs() <= kv_ref.attention_bound(want, spread, reach, 64, BF16, BF16)).all())
+    # without causal the rows before the start see the whole sequence
+    kv.attention(c.cache, 0, batch, q, causal=False, out=out)
+    want, spread, reach = kv_ref.attention(c.q[:6], c.book.k[0][:4], c.book.v[0][:4], 0.125, causal=False)
+    assert bool(((out[:6].cpu().double() - want).abs() <= kv_ref.attention_bound(want, spread, reach, 64, BF16, BF16)).all())
+    assert int(bad) == 0
+    # scores of -infinity alone
+    c.book.k[1][:] = -math.inf
+    c.book.fill()
+    c.cache = c.book.cache(kv)
+    q[6:8] = 1.0
+    kv.attention(c.cache, 0, batch, q, out=out)
+    assert bool((out[6:8] == 0).all())
+
+
+def test_large_scores(kv):
+    """Scores in the thousands: the running maximum keeps the weights in range."""
+    c = Case(kv, [(5, 300), (1, 40)], 32, 2, 2, 64, F16, seed=8, q_scale=300.0)
+    c.check(kv.attention(c.cache, 0, c.batch, c.q.cuda(), 1.0), scale=1.0)
+
+
+def test_bad_device_values_are_left_out_and_reported(kv):
+    """Pages outside the pool, slots outside the tables, starts outside the rows, lengths past the bounds."""
+    seqs = [(2, 60), (2, 60), (2, 60)]
+    for page_id in (-1, -7, 1 << 30, None):
+        c = Case(kv, seqs, 16, 1, 2, 64, BF16, seed=4)
+        wrong = c.book.pages if page_id is None else page_id
+        c.cache.tables[1, 2] = wrong
+        bad = _flag()
+        got = kv.attention(c.cache, 0, c.batch, c.q.cuda(), bad=bad)
+        unseen = torch.zeros(60, dtype=torch.bool)
+        unseen[32:48] = True
+        c.check(got, unseen=[torch.zeros(60, dtype=torch.bool), unseen, torch.zeros(60, dtype=torch.bool)])
+        assert int(bad) == 1
+        # the entry behind the length is not looked at
+        bad.zero_()
+        c.cache.tables[1, 2] = c.book.table[1, 2].cuda()
+        c.cache.lens[1] = 48
+        c.cache.tables[1, 3] = wrong
+        kv.attention(c.cache, 0, c.batch, c.q.cuda(), bad=bad)
+        assert int(bad) == 0
+    c = Case(kv, seqs, 16, 1, 2, 64, BF16, seed=4)
+    good = kv.attention(c.cache, 0, c.batch, c.q.cuda())
+    for starts, slots, lens in [([0, 2, 7, 6], None, None), ([0, 2, -3, 6], None, None), ([0, 2, 1, 6], None, None),
+                                ([0, 2, 4, 6], [0, 3, 2], None), ([0, 2, 4, 6], [0, -1, 2], None),
+                                ([0, 2, 4, 6], None, [60, 61, 60]), ([0, 2, 4, 6], None, [60, -1, 60])]:
+        cache = c.book.cache(kv)
+        if lens:
+            cache.lens.copy_(_i32(lens))
+        out, bad = torch.full_like(good, 3.0), _flag()
+        batch = kv.Batch(_i32(starts), 6, 2, 60, None if slots is None else _i32(slots))
+        kv.attention(cache, 0, batch, c.q.cuda(), out=out, bad=bad)
+        assert int(bad) == 1 and torch.equal(out[:2], good[:2]) and bool((out[2:4] == 3).all()), (starts, slots, lens)
+
+
+def test_slots_and_layers(kv):
+    """Sequences in any slots of a cache, in a layer past the first."""
+    c = Case(kv, [(2, 40), (1, 17), (3, 70)], 16, 2, 2, 64, BF16, seed=12)
+    pool = torch.full((3, *c.book.pool.shape[1:]), math.nan, dtype=BF16)
+    pool[2] = c.book.pool[0]
+    order = [4, 0, 3]
+    tables, lens = torch.full((6, c.book.table.shape[1]), -1, dtype=torch.int32), torch.zeros(6, dtype=torch.int32)
+    for b, s in enumerate(order):
+        tables[s], lens[s] = c.book.table[b], c.book.lens[b]
+    cache = kv.Cache(pool.cuda(), tables.cuda(), lens.cuda(), c.book.refs.cuda(), 16, 64)
+    c.check(kv.attention(cache, 2, kv.Batch(_i32(c.starts), c.rows, 3, 70, _i32(order)), c.q.cuda()))
+
+
+@pytest.mark.parametrize("dtype,in_dtype", [(BF16, F32), (F16, F32), (BF16, BF16), (F16, F16), (F16, BF16)])
+@pytest.mark.parametrize("mode,rot", [(2, 64), (0, 64), (2, 32), (0, 32), (2, 24), (0, 10), (2, 6), (0, 64), (None, 0)])
+def test_append(kv, dtype, in_dtype, mode, rot):
+    """New tokens into whole and broken units of 16 places, rope in both layouts over the whole head and parts of it:
+    each value rounded once (half a step of its type) from angles of positions far out."""
+    d, page, kvh, heads = 64, 32, 2, 4
+    new, lens = [1, 17, 40, 16, 3], [1, 200000, 45, 32, 90]
+    rows, starts = sum(new), _starts(new)
+    # a table wide enough for the long sequence, its page only where tokens are written
+    g = torch.Generator().manual_seed(rot)
+    cols = -(-200000 // page)
+    table = torch.full((5, cols), -1, dtype=torch.int32)
+    ids = iter(torch.randperm(40, generator=g).tolist())
+    for b, (n, m) in enumerate(zip(new, lens)):
+        for j in range((m - n) // page, -(-m // page)):
+            table[b, j] = next(ids)
+    before = torch.randn((1, 40, kvh, 2 * page * d), generator=g).to(dtype)
+    cache = kv.Cache(before.cuda(), table.cuda(), _i32(lens), torch.ones(40, dtype=torch.int32, device="cuda"), page, d)
+    batch = kv.Batch(_i32(starts), rows, 40, 200000)
+    q, k, v = (torch.randn((rows, h, d), generator=g).to(in_dtype) for h in (heads, kvh, kvh))
+    freqs = [1e4 ** (-2 * p / rot) for p in range(rot // 2)]
+    r = kv.Rope(torch.tensor(freqs, dtype=torch.float64, device="cuda"), mode, 1.25) if mode is not None else None
+    place = np.concatenate([np.arange(m - n, m) for n, m in zip(new, lens)])
+    for pos in (None, place[::-1].copy()):
+        bad = _flag()
+        cache.pool.copy_(before)
+        got = kv.append(cache, 0, batch, k.cuda(), v.cuda(), q.cuda(), r, None if pos is None else _i32(pos.tolist()), bad=bad)
+        at = place if pos is None else pos
+        wq, wk = (kv_ref.rope(x, at, freqs, mode, 1.25) if mode is not None else x.double() for x in (q, k))
+        # the rounding, and sine and cosine in fp32 (2^-22 of the pair's length)
+        tol = lambda w: torch.finfo(dtype).eps / 2 * w.abs() + 2.0 ** -22 * 1.25 * 8 + torch.finfo(dtype).smallest_normal  # noqa: E731
+        assert bool(((got.cpu().double() - wq).abs() <= tol(wq)).all())
+        pool, want = cache.pool.cpu(), before.clone()
+        ki, vi = kv_ref.page_index(page, d)
+        seq = np.concatenate([np.full(n, b) for b, n in enumerate(new)])
+        for row in range(rows):
+            held, t = int(table[seq[row], place[row] // page]), int(place[row] % page)
+            for h in range(kvh):
+                assert bool(((pool[0, held, h, ki[t]].double() - wk[row, h]).abs() <= tol(wk[row, h])).all())
+                assert torch.equal(pool[0, held, h, vi[t]], v[row, h].to(dtype))
+                want[0, held, h, ki[t]] = pool[0, held, h, ki[t]]
+                want[0, held, h, vi[t]] = pool[0, held, h, vi[t]]
+        assert torch.equal(pool, want) and int(bad) == 0  # nothing else was written
+
+
+@pytest.mark.parametrize("mode,rot", [(2, 64), (0, 64), (2, 24), (2, 32)])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_append_in_place_and_strided(kv, mode, rot, dtype):
+    """q turned in place; q, k and v as column slices of one wide buffer."""
+    cache = kv.empty_cache(1, 4, 2, 64, 16, slots=2)
+    cache.tables[:, 0], cache.tables[:, 1] = _i32([0, 2]), _i32([1, 3])
+    cache.lens.copy_(_i32([9, 20]))
+    batch = kv.Batch(_i32([0, 9, 14]), 14, 9, 20)
+    g = torch.Generator().manual_seed(1)
+    wide = torch.randn((14, 4 * 64 + 2 * 128 + 16), generator=g).to(dtype).cuda()
+    q, k, v = wide[:, :256], wide[:, 256:384], wide[:, 384:512]
+    r = kv.Rope(torch.tensor([1e4 ** (-2 * p / rot) for p in range(rot // 2)], dtype=torch.float64, device="cuda"), mode)
+    apart = kv.append(cache, 0, batch, k, v, q, r, q_dtype=dtype)
+    pool = cache.pool.clone()
+    rest = wide[:, 256:].clone()
+    cache.pool.zero_()
+    got = kv.append(cache, 0, batch, k, v, q, r, q_out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(q, apart) and torch.equal(cache.pool, pool) and torch.equal(wide[:, 256:], rest)
+    # without q: the same pages
+    cache.pool.zero_()
+    assert kv.append(cache, 0, batch, k, v, rope=r) is None and torch.equal(cache.pool, pool)
+
+
+def test_append_leaves_out_what_has_no_place(kv):
+    cache = kv.empty_cache(1, 4, 1, 64, 16, slots=3)
+    cache.tables[0, 0], cache.tables[1, 0], cache.tables[1, 1], cache.tables[2, 0] = 0, 1, 99, 3
+    cache.lens.copy_(_i32([3, 20, 5]))
+    cache.pool.fill_(5.0)
+    x = torch.ones((5 + 8 + 2 + 1, 1, 64), device="cuda")
+    bad = _flag()
+    # 5 tokens in a sequence of 3 (two have no place), 8 of 20 with the last 4 on a page outside the pool, 2 fine; a row behind
+    out = torch.full((16, 1, 64), 9.0, device="cuda")
+    kv.append(cache, 0, kv.Batch(_i32([0, 5, 13, 15]), 16, 8, 20), x, 2 * x, q=x, q_out=out, bad=bad)
+    assert int(bad) == 1 and bool((out[:15] == 1).all()) and bool((out[15] == 9).all())
+    pool = cache.pool.cpu()
+    for row, n, first in [([0], 3, 0), ([1], 16, 12), ([3], 5, 3)]:
+        k, v = kv_ref.read_cache(pool, row, 16, 16, 64)
+        want = torch.full((16, 1, 64), 5.0)
+        want[first:n] = 1.0
+        assert torch.equal(k.float(), want)
+        want[first:n] = 2.0
+        assert torch.equal(v.float(), want)
+    assert bool((pool[0, 2] == 5).all())
+    bad.zero_()
+    kv.append(cache, 0, kv.Batch(_i32([0, 2]), 2, 2, 20, _i32([7])), x[:2], x[:2], bad=bad)  # a slot outside the tables
+    assert int(bad) == 1 and torch.equal(cache.pool.cpu(), pool)
+
+
+def _random_cache(kv, rng, slots, cols, pages, page, layers=2):
+    """A cache whose counts are right: rows of pages of their own and of shared full pages."""
+    tables = np.full((slots, cols), -1, dtype=np.int32)
+    lens, refs = np.zeros(slots, dtype=np.int32), np.zeros(pages, dtype=np.int32)
+    free = list(rng.permutation(pages))
+    for s in range(slots):
+        n = int(rng.integers(0, cols * page // 2))
+        for j in range(-(-n // page)):
+            if s and j < lens[s - 1] // page and rng.random() < 0.3:
+                tables[s, j] = tables[s - 1, j]
+            elif free:
+                tables[s, j] = free.pop()
+            else:
+                n = j * page
+                break
+            refs[tables[s, j]] += 1
+        lens[s] = n
+    pool = torch.from_numpy(rng.standard_normal((layers, pages, 1, 2 * page * 64)).astype(np.float32)).to(BF16)
+    dev = lambda a: torch.from_numpy(a.copy()).cuda()  # noqa: E731
+    return kv.Cache(pool.cuda(), dev(tables), dev(lens), dev(refs), page, 64), pool, tables, lens, refs
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_assign(kv, seed):
+    """Random steps against the entries done one after the other: forks, admissions, growth and frees, entries that
+    name slots twice or not at all, chains of replaced slots, pools that run out."""
+    rng = np.random.default_rng(seed)
+    slots, cols, page = int(rng.integers(2, 40)), int(rng.integers(2, 9)), int(rng.choice([16, 32]))
+    cache, pool, tables, lens, refs = _random_cache(kv, rng, slots, cols, int(rng.integers(4, slots * cols + 5)), page)
+    n = int(rng.integers(1, slots + 1))
+    dst = rng.permutation(slots)[:n].astype(np.int32)
+    src = np.where(rng.random(n) < 0.4, dst, rng.integers(-1, slots, n)).astype(np.int32)
+    src = np.where(rng.random(n) < 0.2, -1, src).astype(np.int32)
+    grow = (rng.integers(0, cols * page // 2, n) * (rng.random(n) < 0.7)).astype(np.int32)
+    if seed % 3 == 0:  # entries that cannot be done
+        for a, values in ((dst, [dst[0], -1, slots, 1 << 30]), (src, [-2, slots, -(1 << 30)]), (grow, [-1, 1 << 30])):
+            a[rng.integers(0, n)] = rng.choice(values)
+    want = (tables.copy(), lens.copy(), refs.copy())
+    copies, wrong = kv_ref.assign(*want, page, dst.tolist(), src.tolist(), grow.tolist())
+    bad = _flag()
+    kv.assign(cache, *(torch.from_numpy(a).cuda() for a in (dst, src, grow)), bad=bad)
+    for name, got, w in zip(("tables", "lens", "refs"), (cache.tables, cache.lens, cache.refs), want):
+        assert np.array_equal(got.cpu().numpy(), w), name
+    for a, b in copies:
+        pool[:, b] = pool[:, a]
+    assert torch.equal(cache.pool.cpu(), pool)
+    assert int(bad) == int(wrong)
+
+
+def test_assign_many_entries_and_pages(kv):
+    """More entries than a workgroup's threads, more pages than one pass."""
+    rng = np.random.default_rng(5)
+    slots, cols, page, pages = 3000, 4, 16, 9000
+    cache, pool, tables, lens, refs = _random_cache(kv, rng, slots, cols, pages, page, layers=1)
+    dst = rng.permutation(slots).astype(np.int32)
+    src = np.where(np.arange(slots) < 1500, -1, dst).astype(np.int32)
+    grow = rng.integers(0, 20, slots).astype(np.int32)
+    want = (tables.copy(), lens.copy(), refs.copy())
+    copies, wrong = kv_ref.assign(*want, page, dst.tolist(), src.tolist(), grow.tolist())
+    bad = _flag()
+    kv.assign(cache, *(torch.from_numpy(a).cuda() for a in (dst, src, grow)), bad=bad)
+    for name, got, w in zip(("tables", "lens", "refs"), (cache.tables, cache.lens, cache.refs), want):
+        assert np.array_equal(got.cpu().numpy(), w), name
+    assert not copies and torch.equal(cache.pool.cpu(), pool) and int(bad) == int(wrong)
+
+
+def test_assign_reports_wrong_counts(kv):
+    """A released page that no count covers, a row's entry outside the pool: reported, and nothing outside is touched."""
+    cache = kv.empty_cache(1, 4, 1, 64, 16, slots=3)
+    cache.tables[0, 0], cache.tables[1, 0] = 2, 77
+    cache.lens.copy_(_i32([5, 5, 0]))
+    bad = _flag()
+    kv.assign(cache, _i32([0]), _i32([-1]), _i32([0]), bad=bad)  # page 2 has no reference
+    assert int(bad) == 1 and cache.refs.tolist() == [0, 0, 0, 0] and cache.lens.tolist() == [0, 5, 0]
+    bad.zero_()
+    kv.assign(cache, _i32([2]), _i32([1]), _i32([0]), bad=bad)  # the open page to copy is outside the pool
+    assert int(bad) == 1 and cache.tables[2, 0] == 0 and cache.lens.tolist() == [0, 5, 5]
+
+
+@pytest.mark.parametrize("seed", range(10))
+@pytest.mark.parametrize("inplace", [True, False])
+def test_compact(kv, seed, inplace):
+    rng = np.random.default_rng(seed)
+    slots, cols, page = int(rng.integers(1, 60)), int(rng.integers(1, 9)), 16
+    cache, pool, tables, lens, refs = _random_cache(kv, rng, slots, cols, int(rng.integers(1, slots * cols + 2000 * (seed % 2) + 9)), page)
+    if seed % 4 == 3:  # entries that name nothing: beyond the pool, or a page without references
+        tables[0, -1] = len(refs) + 3
+        empty = np.flatnonzero(refs == 0)
+        if len(empty):
+            tables[-1, -1] = empty[-1]
+        cache.tables.copy_(torch.from_numpy(tables))
+    want_tables, want_refs, moves, live, wrong = kv_ref.compact(tables, refs)
+    bad = _flag()
+    new = {} if inplace else dict(refs=torch.full_like(cache.refs, 9), tables=torch.full_like(cache.tables, 9))
+    got = kv.compact(cache, **new, bad=bad)
+    assert int(got) == live and int(bad) == int(wrong)
+    assert np.array_equal((cache.refs if inplace else new["refs"]).cpu().numpy(), want_refs)
+    assert np.array_equal((cache.tables if inplace else new["tables"]).cpu().numpy(), want_tables)
+    if not inplace:  # the old ones stay, and read the same
+        assert np.array_equal(cache.refs.cpu().numpy(), refs) and np.array_equal(cache.tables.cpu().numpy(), tables)
+    for a, b in moves:
+        pool[:, b] = pool[:, a]
+    assert torch.equal(cache.pool.cpu(), pool)
+
+
+def test_calls_on_a_stream_and_in_a_graph(kv):
+    """A decoding step (grow, append, attention) captured once on a stream of its own and replayed as the sequences
+    grow, eager work between the replays: each replay gives what the same calls give eagerly on a second cache."""
+    heads, kvh, d, page, slots = 4, 2, 64, 16, 3
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def fresh():
+        c = kv.empty_cache(1, 40, kvh, d, page, slots=slots, columns=12)
+        c.pool.fill_(math.nan)
+        kv.assign(c, _i32([0, 1, 2]), _i32([-1, -1, -1]), _i32([30, 5, 100]))
+        n = 135
+        x = torch.Generator(device="cuda").manual_seed(7)
+        k, v = (torch.randn((n, kvh, d), generator=x, device="cuda") for _ in range(2))
+        kv.append(c, 0, kv.Batch(_i32([0, 30, 35, 135]), n, 100, 192), k, v)
+        return c
+
+    rope = kv.Rope(torch.tensor(kv.rope_freqs(d, 1e4)[0], dtype=torch.float64, device="cuda"))
+    same, one = _i32([0, 1, 2]), _i32([1, 1, 1])
+    batch = kv.Batch(_i32([0, 1, 2, 3]), slots, 1, 12 * page)
+    q, k, v = (torch.zeros((slots, h, d), device="cuda") for h in (heads, kvh, kvh))
+
+    def step(c):
+        kv.assign(c, same, same, one)
+        return kv.attention(c, 0, batch, kv.append(c, 0, batch, k, v, q, rope))
+
+    eager, graphed = fresh(), fresh()
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step(graphed)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+        want = step(eager)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and bool(out.isfinite().all())
+        assert torch.equal(graphed.tables, eager.tables) and torch.equal(graphed.lens, eager.lens)
+
+
+def test_the_operators_together(kv):
+    """As a server uses them: a prompt in chunks, a fork, tokens for parent and child, a freed sequence, compaction,
+    more tokens. Every step's attention is that of plain keys and values kept beside."""
+    heads, kvh, d, page = 4, 2, 64, 16
+    c = kv.empty_cache(2, 24, kvh, d, page, slots=4, columns=8)
+    c.pool.fill_(math.nan)
+    rng = torch.Generator().manual_seed(3)
+    freqs, mag = kv.rope_freqs(d, 1e4)
+    rope = kv.Rope(torch.tensor(freqs, dtype=torch.float64, device="cuda"))
+    kept = {}  # slot -> (k, v) of layer 1
+
+    def tokens(slots, news):
+        rows, starts = sum(news), _starts(news)
+        kv.assign(c, _i32(slots), _i32(slots), _i32(news))
+        q, k, v = (torch.randn((rows, h, d), generator=rng) for h in (heads, kvh, kvh))
+        b = kv.Batch(_i32(starts), rows, max(news), 8 * page, _i32(slots))
+        for layer in (0, 1):
+            qt = kv.append(c, layer, b, k.cuda(), v.cuda(), q.cuda(), rope)
+        got = kv.attention(c, 1, b, qt, out_dtype=F32).cpu()
+        for s, n, r in zip(slots, news, starts):
+            k0, v0 = kept.get(s, (torch.zeros(0, kvh, d).to(BF16),) * 2)
+            place = np.arange(len(k0), len(k0) + n)
+            kk = torch.cat([k0, kv_ref.rope(k[r:r + n], place, freqs, 2, 1.0).to(BF16)])
+            vv = torch.cat([v0, v[r:r + n].to(BF16)])
+            kept[s] = kk, vv
+            out, spread, reach = kv_ref.attention(qt[r:r + n].cpu(), kk, vv, 0.125)
+            # the kept k may round the other way where sine and cosine in fp32 move it past a tie: one step more of a score
+            bound = kv_ref.attention_bound(out, spread, reach, d, BF16, F32) + 2 * 2.0 ** -7 * reach / 64 * spread
+            assert bool(((got[r:r + n].double() - out).abs() <= bound).all()), (s, n)
+
+    tokens([0], [37])
+    tokens([0, 2], [20, 9])
+    kv.assign(c, _i32([1, 3]), _i32([0, 2]), _i32([0, 0]))  # forks: 57 tokens (an open page), 9
+    kept[1], kept[3] = kept[0], kept[2]
+    tokens([1, 0, 3, 2], [1, 1, 5, 1])
+    kv.assign(c, _i32([0, 2]), _i32([-1, -1]), _i32([0, 0]))
+    del kept[0], kept[2]
+    live = int(kv.compact(c))
+    assert live == sum(-(-len(kept[s][0]) // page) for s in kept) == int((c.refs > 0).sum()) and int(c.tables.max()) == live - 1
+    tokens([3, 1], [30, 2])
+    tokens([1], [1])
