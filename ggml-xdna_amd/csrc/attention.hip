@@ -32,7 +32,9 @@ constexpr int COLS = 32;     // columns of a wave's tile
 constexpr int WAVES = 4;     // waves of a workgroup
 constexpr int GROUP = 32;    // tokens a wave takes at a time
 constexpr int UNIT = WAVES * GROUP;  // tokens of a unit of work
-constexpr int MAX_WORKGROUPS = 512;  // two a CU
+constexpr int CUS = 256;
+constexpr int MAX_WORKGROUPS = 2 * CUS;
+constexpr int MOST_SPLIT_COLS = 64;  // columns of a sequence that attn_kernel takes
 
 // The cache's element type: its fragment, its MFMA and its exponent field.
 template <int TYPE> struct elem;
@@ -49,9 +51,9 @@ template <> struct elem<ZEST_TYPE_BF16> {
 template <> struct elem<ZEST_TYPE_F16> {
     typedef f16x8 frag;
     static constexpr uint32_t EXP = 0x7c007c00u, ONE = 0x04000400u;
-    // weights are held times 2^12 (the sum with them, so it cancels): the largest
-    // is 2^12, and one 2^-26 of it is still a normal fp16 number
-    static constexpr float SHIFT = 12.0f;
+    // weights are held times 2^6 (the sum with them, so it cancels): one 2^-20 of
+    // the largest is still a normal fp16 number, and 2^(6 + SLACK) is in range
+    static constexpr float SHIFT = 6.0f;
     static __device__ f32x16 mfma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ _Float16 from(float v) { return (_Float16) v; }
 };
@@ -63,8 +65,12 @@ struct attn_args {
     void * out;
     int64_t ldq, ldo;
     int32_t q_type, out_type, group, causal, window;
-    float scale, softcap;  // softcap 0: none
+    float scale, softcap;  // scale >= 0, softcap 0: none
+    float sign;            // q is multiplied by it: -1 for a negative scale, 0 for a scale of 0 (scale is then 1)
+    int32_t chunk_cols;    // sequences of more columns than this are chunk_kernel's
     float * partial;
+    float * chunk_partial;
+    int32_t chunk_splits;
 };
 
 // Tokens [lo, hi) that any of a sequence's rows i0 .. i1 sees.
@@ -88,7 +94,7 @@ __device__ inline int32_t units_of(const attn_args & a, const kv_seq & s) {
 }
 
 __device__ inline int32_t cost_of(const attn_args & a, const kv_seq & s) {
-    return s.n > 0 ? units_of(a, s) * col_tiles(a, s) * a.c.kv_heads : 0;
+    return s.n > 0 && (int64_t) s.n * a.group <= a.chunk_cols ? units_of(a, s) * col_tiles(a, s) * a.c.kv_heads : 0;
 }
 
 // The largest or the sum of a value over a lane and its partner in the other half.
@@ -124,6 +130,10 @@ __device__ inline void load_q(const attn_args & a, const kv_seq & s, int h, int 
                 const f16x8 x = *reinterpret_cast<const f16x8 *>((const uint16_t *) a.q + at + ks * 16);
 #pragma unroll
                 for (int j = 0; j < 8; j++) f[j] = elem<TYPE>::from((float) x[j]);
+            }
+            if (a.sign != 1.0f) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[j] = elem<TYPE>::from((float) f[j] * a.sign);
             }
         }
         qf[ks] = f;
@@ -458,31 +468,462 @@ __global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
     }
 }
 
-// The most units a call's bounds allow, saturated.
-int64_t most_units(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
-    const int64_t run = std::max<int64_t>(1, ((int64_t) b->max_len + GROUP + UNIT - 1) / UNIT);
-    const int64_t tiles = std::min<int64_t>(((int64_t) b->rows * group + COLS - 1) / COLS + b->seqs,
-                                            ((int64_t) b->max_new * group + COLS - 1) / COLS * b->seqs);
-    return run * tiles * c->kv_heads;
+// ---- chunks: many columns ---------------------------------------------------------
+
+typedef __attribute__((address_space(3))) void * lds_ptr_t;
+typedef const __attribute__((address_space(1))) void * global_ptr_t;
+
+// Column tiles of 32 a wave of chunk_kernel takes: two where the registers hold
+// them (O^T of 64 columns is D values a lane, Q^T half of that).
+template <int D> constexpr int QT = 1;
+template <int D> constexpr int CHUNK = WAVES * 32 * QT<D>;  // columns of a workgroup
+constexpr int RING = 4;                                     // steps of K and V in shared memory
+template <int D> constexpr int STEP_BYTES = GROUP * D * 4;  // 32 tokens' K, then V
+// How far, in powers of two, a score may pass the maximum its column's weights
+// are relative to before O^T is rescaled: the sums are in fp32, so only the
+// weights' own range matters (bf16: fp32's; fp16: SHIFT + 8 stays below 2^16)
+constexpr float SLACK = 8.0f;
+
+template <int D> constexpr int CHUNK_PARTIAL = CHUNK<D> * (D + 2);
+
+__device__ inline int32_t chunk_tiles_of(const attn_args & a, const kv_seq & s, int chunk) {
+    const int64_t cols = (int64_t) s.n * a.group;
+    return cols > a.chunk_cols ? (int32_t) ((cols + chunk - 1) / chunk) : 0;
 }
 
-int workgroups(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
-    return (int) std::min<int64_t>(most_units(c, b, group), MAX_WORKGROUPS);
+// One column tile of a chunk: 4 waves of 32 QT columns each over the keys that
+// any of the tile's columns sees, 32 tokens a step. K and V of a step go from
+// the pool straight into shared memory (16 bytes a lane, in the pool's order,
+// which is the order they are read in: every read is 512 contiguous bytes a half
+// wave), a ring of four steps with one barrier a step. A step runs three stages
+// at once, so the matrix cores and the vector units both have work: the scores
+// of step j + 1, the softmax of step j and the weights of step j - 1 times V.
+template <int TYPE, int D>
+__global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn_args a) {
+    typedef typename elem<TYPE>::frag frag;
+    constexpr int NQ = QT<D>, KS = D / 16, DT = D / 32;
+    extern __shared__ __align__(1024) uint8_t ring[];  // [RING][K: D/8][32][8], V: [2][2][D][8]; then the prefix sums
+    __shared__ uint32_t missing[RING];                 // bit g: tokens 16g .. of the step have no page
+    int32_t * prefix = reinterpret_cast<int32_t *>(ring + RING * STEP_BYTES<D>);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+    const int ps = a.c.page_shift, P = 1 << ps;
+    zest::prefix_over_seqs(a.b, ps, prefix, [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
+    // the last tiles first: under a causal mask they see the most
+    const int h = blockIdx.x % a.c.kv_heads;
+    const int tile = prefix[a.b.seqs] - 1 - (int) (blockIdx.x / a.c.kv_heads);
+    if (tile < 0) return;
+    bool bad = false;
+    const int b = __builtin_amdgcn_readfirstlane(zest::seq_of(prefix, a.b.seqs, tile));
+    const kv_seq s = zest::load_seq(a.b, b, ps, bad);
+    const int c0 = (tile - prefix[b]) * CHUNK<D>, ncols = s.n * a.group;
+    const int32_t * row = a.b.tables + (int64_t) s.slot * a.b.table_cols;
+
+    // the tile's tokens, and of them this split's
+    int32_t lo, hi;
+    seen_by(a, s, c0 / a.group, min(ncols - 1, c0 + CHUNK<D> - 1) / a.group, lo, hi);
+    lo &= ~(GROUP - 1);
+    const int32_t steps = (hi - lo + GROUP - 1) / GROUP;
+    const int32_t first = (int32_t) ((int64_t) steps * blockIdx.y / gridDim.y);
+    const int32_t n = (int32_t) ((int64_t) steps * (blockIdx.y + 1) / gridDim.y) - first;
+    const int32_t t_first = lo + first * GROUP, t_hi = hi;
+
+    // this wave's columns
+    const int w0 = c0 + wave * 32 * NQ;
+    frag qf[NQ][KS];
+    int32_t see_lo[NQ], see_hi[NQ], all_lo = 0, all_hi = 0x7fffffff;
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+        const int c = w0 + 32 * q + col;
+        load_q<TYPE, D>(a, s, h, c, c < ncols, half, qf[q]);
+        seen_by(a, s, c / a.group, c / a.group, see_lo[q], see_hi[q]);
+        if (c >= ncols) see_lo[q] = see_hi[q] = 0;
+    }
+    if (w0 < ncols) {
+        int32_t unused;
+        seen_by(a, s, w0 / a.group, w0 / a.group, unused, all_hi);
+        const int last = min(ncols, w0 + 32 * NQ) - 1;
+        seen_by(a, s, last / a.group, last / a.group, all_lo, unused);
+    }
+
+    // A step's loads: waves 0 and 1 a half of K's rows each, waves 2 and 3 the V
+    // of 16 tokens each. A lane looks its page up one step before it loads.
+    const bool k_wave = wave < 2;
+    const int32_t head_at = h * (4 * P * D);
+    const uint32_t ring_at = (uint32_t) (uintptr_t) (lds_ptr_t) ring;
+    auto page_of = [&](int j) {  // the table's entry for this lane's token of step j; -1 behind the last token
+        const int32_t t = t_first + j * GROUP + (k_wave ? col : 16 * (wave - 2));
+        return j < n && t < t_hi ? row[t >> ps] : -1;
+    };
+    auto load_step = [&](int j, int32_t id) {
+        if (j >= n) return;
+        const int32_t t0 = t_first + j * GROUP, t = t0 + (k_wave ? col : 16 * (wave - 2));
+        const bool there = (uint32_t) id < (uint32_t) a.c.pages;
+        if (!k_wave && lane == 0) {
+            const bool gone = !there && t < t_hi;
+            bad |= gone;
+            reinterpret_cast<uint16_t *>(&missing[j % RING])[wave - 2] = gone;
+        }
+        const uint8_t * from = a.c.pool + (there ? id : 0) * a.c.page_bytes + head_at;
+        const uint32_t in = t & (P - 1);
+        const uint32_t to = ring_at + (j % RING) * STEP_BYTES<D>;
+        if (k_wave) {
+            from += in * 16 + (wave * (D / 16) + half) * (P * 16);
+#pragma unroll
+            for (int i = 0; i < D / 32; i++)
+                __builtin_amdgcn_global_load_lds((global_ptr_t) (from + i * (P * 32)),
+                                                 (lds_ptr_t) (uintptr_t) (to + (wave * (D / 32) + i) * 1024), 16, 0, 0);
+        } else {
+            from += 2 * P * D + in * (2 * D) + lane * 16;
+#pragma unroll
+            for (int i = 0; i < D / 32; i++)
+                __builtin_amdgcn_global_load_lds((global_ptr_t) (from + i * 1024),
+                                                 (lds_ptr_t) (uintptr_t) (to + GROUP * D * 2 + ((wave - 2) * (D / 32) + i) * 1024),
+                                                 16, 0, 0);
+        }
+    };
+    auto k_frag = [&](int j, int ks) {
+        return *reinterpret_cast<const frag *>(ring + (j % RING) * STEP_BYTES<D> + (2 * ks + half) * 512 + col * 16);
+    };
+    auto v_frag = [&](int j, int dt, int g) {
+        return *reinterpret_cast<const frag *>(ring + (j % RING) * STEP_BYTES<D> + GROUP * D * 2 + (2 * g + half) * (16 * D) + dt * 512 +
+                                               col * 16);
+    };
+
+    f32x16 o[DT][NQ], s_cur[NQ], s_next[NQ];
+    frag p[NQ][2];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+        m[q] = -INFINITY;
+        l[q] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) o[dt][q] = f32x16{};
+    }
+    auto scores = [&](int j, f32x16 to[NQ]) {
+#pragma unroll
+        for (int q = 0; q < NQ; q++) to[q] = f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const frag k = k_frag(j, ks);
+#pragma unroll
+            for (int q = 0; q < NQ; q++) to[q] = elem<TYPE>::mfma(k, qf[q][ks], to[q]);
+        }
+    };
+    auto weigh = [&](int j) {
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                const frag v = v_frag(j, dt, g);
+#pragma unroll
+                for (int q = 0; q < NQ; q++) o[dt][q] = elem<TYPE>::mfma(v, p[q][g], o[dt][q]);
+            }
+    };
+    // The same where a column does not see every token: a weight of 0 does not
+    // silence a NaN or an infinity, so 16 tokens that hold one are taken one at
+    // a time, each added where its column sees it.
+    auto weigh_masked = [&](int j, uint32_t gone) {
+        const int32_t t0 = t_first + j * GROUP;
+        for (int g = 0; g < 2; g++) {
+            bool odd = false;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) odd |= nonfinite<TYPE>(v_frag(j, dt, g));
+            const bool careful = __any(odd);
+            for (int tt = 0; tt < (careful ? 16 : 1); tt++) {
+                const int e = (tt & 3) + (tt >> 3) * 4, hh = (tt >> 2) & 1;
+                const int32_t t = t0 + 16 * g + tt;
+                bool in[NQ];
+                struct words { uint32_t w[4]; };
+                words keep;
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    keep.w[w] = !careful ? 0xffffffffu : half == hh && w == e >> 1 ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+#pragma unroll
+                for (int q = 0; q < NQ; q++) in[q] = !careful || (t >= see_lo[q] && t < see_hi[q] && !(gone >> (16 * g) & 1));
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    words x = __builtin_bit_cast(words, v_frag(j, dt, g));
+#pragma unroll
+                    for (int w = 0; w < 4; w++) x.w[w] &= keep.w[w];
+#pragma unroll
+                    for (int q = 0; q < NQ; q++) {
+                        const frag pg = g ? p[q][1] : p[q][0];
+                        const f32x16 one = elem<TYPE>::mfma(__builtin_bit_cast(frag, x), pg, f32x16{});
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[dt][q][i] = in[q] ? o[dt][q][i] + one[i] : o[dt][q][i];
+                    }
+                }
+            }
+        }
+    };
+    const float c = a.softcap > 0.0f ? 1.0f : a.scale * LOG2E;
+    float shrink[NQ];
+    // Maximum, sum and weights of s_cur; the weights go to `to`.
+    auto soften = [&](frag to[NQ][2]) {
+        bool any_rise = false;
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+            float top = s_cur[q][0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) top = fmaxf(top, s_cur[q][i]);
+            top = fmaxf(top, other_half(top)) * c;
+            // every column by itself, so that no row's result depends on others'
+            const bool rise = top > m[q] + SLACK;
+            any_rise |= rise;
+            const float now = rise ? top : m[q];
+            const float base = now == -INFINITY ? 0.0f : now;
+            shrink[q] = __builtin_amdgcn_exp2f(m[q] - base);
+            m[q] = now;
+            const float shift = elem<TYPE>::SHIFT - base;
+            float sum = 0.0f;
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(s_cur[q][8 * g + i], c, shift));
+                    sum += w;
+                    to[q][g][i] = elem<TYPE>::from(w);
+                }
+            l[q] = l[q] * shrink[q] + sum;
+        }
+        return any_rise;
+    };
+
+    int32_t id = page_of(0);
+    load_step(0, id);
+    id = page_of(1);
+    load_step(1, id);
+    id = page_of(2);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (n > 0) scores(0, s_cur);
+    bool masked_before = false;
+    uint32_t gone_before = 0, gone = 0;
+    // the barrier of step j: this wave's loads of step j + 1 are there and its
+    // reads of step j - 2 done; past it, every wave's. Whether step j is masked.
+    auto enter = [&](int j) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        gone = __builtin_amdgcn_readfirstlane(missing[j % RING]);
+        load_step(j + 2, id);
+        id = page_of(j + 3);
+        const int32_t t0 = t_first + j * GROUP;
+        return t0 < all_lo || t0 + GROUP > all_hi || gone != 0;
+    };
+    auto cap_scores = [&]() {
+        const float in = a.scale / a.softcap * (2.0f * LOG2E), cap = a.softcap * LOG2E;
+#pragma unroll
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int i = 0; i < 16; i++)  // as in attend
+                s_cur[q][i] = cap - 2.0f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s_cur[q][i] * in) + 1.0f);
+    };
+    auto finish = [&](bool rise, const frag pn[NQ][2]) {
+        if (__any(rise)) {
+#pragma unroll
+            for (int q = 0; q < NQ; q++)
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[dt][q][i] *= shrink[q];
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+            s_cur[q] = s_next[q];
+            p[q][0] = pn[q][0];
+            p[q][1] = pn[q][1];
+        }
+    };
+    int32_t j = 0;
+    bool masked = n > 0 ? enter(0) : false;
+    while (j < n) {
+        // a step that is masked, or follows one that is, or the first
+        if (a.softcap > 0.0f) cap_scores();
+        if (masked) {
+            const int32_t t0 = t_first + j * GROUP;
+#pragma unroll
+            for (int q = 0; q < NQ; q++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int32_t t = t0 + (i & 3) + 8 * (i >> 2) + 4 * half;
+                    const bool in = t >= see_lo[q] && t < see_hi[q] && !(gone >> (16 * (i >> 3)) & 1);
+                    s_cur[q][i] = in ? s_cur[q][i] : -INFINITY;
+                }
+        }
+        {
+            frag pn[NQ][2];
+            if (j > 0) {
+                if (masked_before) weigh_masked(j - 1, gone_before);
+                else weigh(j - 1);
+            }
+            scores(j + 1, s_next);
+            const bool rise = soften(pn);
+            finish(rise, pn);
+        }
+        masked_before = masked;
+        gone_before = gone;
+        if (++j < n) masked = enter(j);
+        // the steps that every column sees whole
+        while (j < n && !masked && !masked_before) {
+            if (a.softcap > 0.0f) cap_scores();
+            frag pn[NQ][2];
+            weigh(j - 1);
+            scores(j + 1, s_next);
+            const bool rise = soften(pn);
+            finish(rise, pn);
+            if (++j < n) masked = enter(j);
+        }
+    }
+    if (n > 0) {
+        if (masked_before) weigh_masked(n - 1, gone_before);
+        else weigh(n - 1);
+    }
+    if (bad) zest::report(a.b.bad);
+
+    if (gridDim.y > 1) {
+        // this split's part: O^T in the registers' own order, maxima and sums
+        float * slot = a.chunk_partial + ((int64_t) (tile * a.c.kv_heads + h) * gridDim.y + blockIdx.y) * CHUNK_PARTIAL<D>;
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+            const int cc = wave * 32 * NQ + 32 * q;
+            const float sum = l[q] + other_half(l[q]);
+            if (half == 0) {
+                slot[CHUNK<D> * D + cc + col] = m[q];
+                slot[CHUNK<D> * (D + 1) + cc + col] = sum;
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    *reinterpret_cast<float4 *>(slot + cc * D + ((dt * 4 + k) * 64 + lane) * 4) =
+                        make_float4(o[dt][q][4 * k], o[dt][q][4 * k + 1], o[dt][q][4 * k + 2], o[dt][q][4 * k + 3]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+        const float sum = l[q] + other_half(l[q]);
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int cc = w0 + 32 * q + col;
+        if (cc >= ncols) continue;
+        const int64_t to = (int64_t) (s.row0 + cc / a.group) * a.ldo + (int64_t) (h * a.group + cc % a.group) * D + 4 * half;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float v[4] = {o[dt][q][4 * k] * f, o[dt][q][4 * k + 1] * f, o[dt][q][4 * k + 2] * f, o[dt][q][4 * k + 3] * f};
+                store4(a, to + dt * 32 + 8 * k, v);
+            }
+    }
 }
 
-template <int TYPE, int D> void launch(const attn_args & a, int W, hipStream_t s) {
+// Joins the splits of chunk_kernel's column tiles, in their order: a workgroup a
+// tile of 32 columns, a thread four values of each of its 32-row blocks.
+template <int D>
+__global__ __launch_bounds__(256) void chunk_combine_kernel(attn_args a) {
+    extern __shared__ __align__(16) int32_t attn_sh[];
+    int32_t * prefix = attn_sh;
+    const int ps = a.c.page_shift;
+    zest::prefix_over_seqs(a.b, ps, prefix, [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
+    constexpr int PARTS = CHUNK<D> / 32;
+    const int part = blockIdx.x % PARTS, at = blockIdx.x / PARTS, h = at % a.c.kv_heads, tile = at / a.c.kv_heads;
+    if (tile >= prefix[a.b.seqs]) return;
+    bool bad = false;
+    const int b = zest::seq_of(prefix, a.b.seqs, tile);
+    const kv_seq s = zest::load_seq(a.b, b, ps, bad);
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, k = threadIdx.x >> 6;
+    const int cc = (tile - prefix[b]) * CHUNK<D> + part * 32 + col;
+    if (cc >= s.n * a.group) return;
+    const float * slots = a.chunk_partial + (int64_t) at * a.chunk_splits * CHUNK_PARTIAL<D>;
+    float m = -INFINITY, l = 0.0f;
+    for (int i = 0; i < a.chunk_splits; i++) m = fmaxf(m, slots[(int64_t) i * CHUNK_PARTIAL<D> + CHUNK<D> * D + part * 32 + col]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float o[D / 32][4] = {};
+    for (int i = 0; i < a.chunk_splits; i++) {
+        const float * x = slots + (int64_t) i * CHUNK_PARTIAL<D>;
+        const float f = __builtin_amdgcn_exp2f(x[CHUNK<D> * D + part * 32 + col] - base);
+        l += x[CHUNK<D> * (D + 1) + part * 32 + col] * f;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++) {
+            const float4 v = *reinterpret_cast<const float4 *>(x + part * 32 * D + ((dt * 4 + k) * 64 + lane) * 4);
+            o[dt][0] += v.x * f, o[dt][1] += v.y * f, o[dt][2] += v.z * f, o[dt][3] += v.w * f;
+        }
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    const int64_t to = (int64_t) (s.row0 + cc / a.group) * a.ldo + (int64_t) (h * a.group + cc % a.group) * D + 8 * k + 4 * half;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; dt++) {
+        const float v[4] = {o[dt][0] * f, o[dt][1] * f, o[dt][2] * f, o[dt][3] * f};
+        store4(a, to + dt * 32, v);
+    }
+}
+
+// ---- the host's plan ----------------------------------------------------------------
+
+// What a call launches, by its sizes and bounds alone.
+struct attn_plan {
+    int64_t units;              // of attn_kernel, at most
+    int workgroups;             // of attn_kernel, 0: not launched
+    int chunk_cols;             // sequences of more columns go to chunk_kernel
+    int64_t chunk_tiles;        // of chunk_kernel, a k/v head, at most; 0: not launched
+    int chunk_splits;
+    size_t partial_bytes, bytes;
+};
+
+attn_plan plan_of(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
+    attn_plan p{};
+    const int chunk = WAVES * 32;
+    const int64_t most = (int64_t) b->max_new * group;  // columns of a sequence
+    const bool chunks = most > MOST_SPLIT_COLS;
+    // one sequence alone is a chunk whatever its length turns out to be
+    p.chunk_cols = !chunks ? 0x7fffffff : b->seqs == 1 ? 0 : MOST_SPLIT_COLS;
+    if (chunks) {
+        p.chunk_tiles = std::min<int64_t>((b->rows * group + chunk - 1) / chunk + b->seqs, (most + chunk - 1) / chunk * b->seqs);
+        const int64_t items = p.chunk_tiles * c->kv_heads, steps = std::max<int64_t>(1, b->max_len / GROUP);
+        p.chunk_splits = (int) std::max<int64_t>(1, std::min<int64_t>({2 * CUS / items, steps / 8, 64}));
+    }
+    if (p.chunk_cols > 0) {
+        const int64_t cols = std::min<int64_t>(most, p.chunk_cols);
+        const int64_t run = std::max<int64_t>(1, ((int64_t) b->max_len + GROUP + UNIT - 1) / UNIT);
+        const int64_t tiles = std::min<int64_t>((b->rows * group + COLS - 1) / COLS + b->seqs, (cols + COLS - 1) / COLS * b->seqs);
+        p.units = run * tiles * c->kv_heads;
+        p.workgroups = (int) std::min<int64_t>(p.units, MAX_WORKGROUPS);
+    }
+    p.partial_bytes = (size_t) 2 * p.workgroups * COLS * (c->head_dim + 2) * sizeof(float);
+    p.bytes = p.partial_bytes;
+    if (p.chunk_splits > 1) p.bytes += (size_t) p.chunk_tiles * c->kv_heads * p.chunk_splits * chunk * (c->head_dim + 2) * sizeof(float);
+    p.bytes = std::max<size_t>(p.bytes, 16);
+    return p;
+}
+
+template <int TYPE, int D> int launch(const attn_args & a, const attn_plan & p, hipStream_t s) {
     const size_t lds = (size_t) ((a.b.seqs + 4) & ~3) * 4;
-    hipLaunchKernelGGL((attn_kernel<TYPE, D>), dim3(W), dim3(WAVES * 64), lds, s, a);
-    hipLaunchKernelGGL(combine_kernel<D>, dim3(W), dim3(256), lds, s, a);
+    if (p.chunk_tiles) {
+        const size_t ring = RING * STEP_BYTES<D> + lds;
+        if (ring + 1024 > 65536) {
+            static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&chunk_kernel<TYPE, D>),
+                                                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 1024);
+            if (e != hipSuccess) return zest::fail(ZEST_E_HIP, "zest_kv_attn: shared memory of %zu bytes: %s", ring, hipGetErrorString(e));
+        }
+        hipLaunchKernelGGL((chunk_kernel<TYPE, D>), dim3((unsigned) (p.chunk_tiles * a.c.kv_heads), p.chunk_splits), dim3(WAVES * 64), ring,
+                           s, a);
+    }
+    if (p.workgroups) hipLaunchKernelGGL((attn_kernel<TYPE, D>), dim3(p.workgroups), dim3(WAVES * 64), lds, s, a);
+    if (p.chunk_splits > 1)
+        hipLaunchKernelGGL(chunk_combine_kernel<D>, dim3((unsigned) (p.chunk_tiles * a.c.kv_heads * (CHUNK<D> / 32))), dim3(256), lds, s, a);
+    if (p.workgroups) hipLaunchKernelGGL(combine_kernel<D>, dim3(p.workgroups), dim3(256), lds, s, a);
+    return zest::check_launch("zest_kv_attn");
 }
 
-template <int TYPE> void launch(const attn_args & a, int D, int W, hipStream_t s) {
+template <int TYPE> int launch(const attn_args & a, int D, const attn_plan & p, hipStream_t s) {
     switch (D) {
-        case 64: return launch<TYPE, 64>(a, W, s);
-        case 96: return launch<TYPE, 96>(a, W, s);
-        case 128: return launch<TYPE, 128>(a, W, s);
-        case 192: return launch<TYPE, 192>(a, W, s);
-        default: return launch<TYPE, 256>(a, W, s);
+        case 64: return launch<TYPE, 64>(a, p, s);
+        case 96: return launch<TYPE, 96>(a, p, s);
+        case 128: return launch<TYPE, 128>(a, p, s);
+        case 192: return launch<TYPE, 192>(a, p, s);
+        default: return launch<TYPE, 256>(a, p, s);
     }
 }
 
@@ -493,7 +934,7 @@ extern "C" {
 size_t zest_kv_attn_workspace(const zest_kv_cache * cache, const zest_kv_batch * batch, int32_t q_heads) {
     if (!cache || !batch || cache->kv_heads <= 0 || q_heads < cache->kv_heads || q_heads % cache->kv_heads) return 0;
     if (batch->rows <= 0 || batch->seqs <= 0 || batch->max_new <= 0 || batch->max_len < 0) return 0;
-    return (size_t) 2 * workgroups(cache, batch, q_heads / cache->kv_heads) * COLS * (cache->head_dim + 2) * sizeof(float);
+    return plan_of(cache, batch, q_heads / cache->kv_heads).bytes;
 }
 
 int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const void * q, int q_type, int64_t ldq,
@@ -511,9 +952,10 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
                  "%s: scale=%g window=%d softcap=%g", me, (double) scale, window, (double) softcap);
     ZEST_REQUIRE(batch->rows * (int64_t) (q_heads / cache->kv_heads) < (1ll << 31) - 64, "%s: %lld rows of %d heads", me,
                  (long long) batch->rows, q_heads);
-    const int64_t units = most_units(cache, batch, q_heads / cache->kv_heads);
-    ZEST_REQUIRE(units < (1ll << 31), "%s: a batch of %lld units of work", me, (long long) units);
-    const size_t need = zest_kv_attn_workspace(cache, batch, q_heads);
+    const attn_plan plan = plan_of(cache, batch, q_heads / cache->kv_heads);
+    ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads * 8 < (1ll << 31), "%s: a batch of %lld units of work",
+                 me, (long long) std::max(plan.units, plan.chunk_tiles));
+    const size_t need = plan.bytes;
     ZEST_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need,
                  "%s: workspace of %zu bytes, 16-byte aligned, wanted", me, need);
     attn_args a{};
@@ -522,13 +964,16 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
     a.q = q, a.out = out, a.ldq = ldq, a.ldo = ldo;
     a.q_type = q_type, a.out_type = out_type;
     a.group = q_heads / cache->kv_heads;
-    a.causal = causal != 0, a.window = window, a.scale = scale, a.softcap = softcap;
+    a.causal = causal != 0, a.window = window, a.softcap = softcap;
+    a.sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
+    a.scale = scale == 0.0f ? 1.0f : scale < 0.0f ? -scale : scale;
+    a.chunk_cols = plan.chunk_cols;
+    a.chunk_splits = plan.chunk_splits;
     a.partial = (float *) workspace;
-    const int W = workgroups(cache, batch, a.group);
+    a.chunk_partial = (float *) ((uint8_t *) workspace + plan.partial_bytes);
     const hipStream_t s = zest::as_stream(stream);
-    if (cache->type == ZEST_TYPE_BF16) launch<ZEST_TYPE_BF16>(a, cache->head_dim, W, s);
-    else launch<ZEST_TYPE_F16>(a, cache->head_dim, W, s);
-    return zest::check_launch(me);
+    return cache->type == ZEST_TYPE_BF16 ? launch<ZEST_TYPE_BF16>(a, cache->head_dim, plan, s)
+                                         : launch<ZEST_TYPE_F16>(a, cache->head_dim, plan, s);
 }
 
 } // extern "C"
