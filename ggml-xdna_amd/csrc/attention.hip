@@ -23,17 +23,16 @@ using zest::kv_batch;
 using zest::kv_pages;
 using zest::kv_seq;
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int COLS = 32;     // columns of a wave's tile
 constexpr int WAVES = 4;     // waves of a workgroup
 constexpr int GROUP = 32;    // tokens a wave takes at a time
 constexpr int UNIT = WAVES * GROUP;  // tokens of a unit of work
 constexpr int CUS = 256;
-constexpr int MAX_WORKGROUPS = 2 * CUS;
 constexpr int MOST_SPLIT_COLS = 64;  // columns of a sequence that attn_kernel takes
 
 // The cache's element type: its fragment, its MFMA and its exponent field.
@@ -45,6 +44,7 @@ template <> struct elem<ZEST_TYPE_BF16> {
     // exponent added to the softmax weights: none, bf16 has fp32's range
     static constexpr float SHIFT = 0.0f;
     static __device__ f32x16 mfma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ f32x4 mfma16(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __bf16 from(float v) { return (__bf16) v; }
 };
 
@@ -55,6 +55,7 @@ template <> struct elem<ZEST_TYPE_F16> {
     // the largest is still a normal fp16 number, and 2^(6 + SLACK) is in range
     static constexpr float SHIFT = 6.0f;
     static __device__ f32x16 mfma(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ f32x4 mfma16(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ _Float16 from(float v) { return (_Float16) v; }
 };
 
@@ -81,11 +82,8 @@ __device__ inline void seen_by(const attn_args & a, const kv_seq & s, int i0, in
     lo = min(lo, hi);
 }
 
-__device__ inline int32_t col_tiles(const attn_args & a, const kv_seq & s) {
-    return (int32_t) (((int64_t) s.n * a.group + COLS - 1) / COLS);
-}
-
-// Units of work of one column tile: whole UNITs from the first token seen.
+// Units of work of one column tile of attn_kernel: whole UNITs from the first
+// token that any of the sequence's rows sees.
 __device__ inline int32_t units_of(const attn_args & a, const kv_seq & s) {
     int32_t lo, hi;
     seen_by(a, s, 0, s.n - 1, lo, hi);
@@ -93,41 +91,49 @@ __device__ inline int32_t units_of(const attn_args & a, const kv_seq & s) {
     return max(1, (hi - lo + UNIT - 1) / UNIT);
 }
 
-__device__ inline int32_t cost_of(const attn_args & a, const kv_seq & s) {
-    return s.n > 0 && (int64_t) s.n * a.group <= a.chunk_cols ? units_of(a, s) * col_tiles(a, s) * a.c.kv_heads : 0;
+__device__ inline int32_t col_tiles(const attn_args & a, const kv_seq & s, int cols) { return (s.n * a.group + cols - 1) / cols; }
+
+__device__ inline int32_t cost_of(const attn_args & a, const kv_seq & s, int cols) {
+    return s.n > 0 && (int64_t) s.n * a.group <= a.chunk_cols ? units_of(a, s) * col_tiles(a, s, cols) * a.c.kv_heads : 0;
 }
 
-// The largest or the sum of a value over a lane and its partner in the other half.
+// A value of the lane's partner in the other half of the wave, and in the other
+// 16 lanes of its half.
 __device__ inline float other_half(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-// Query fragments of one column: 8 values at d = 16 ks + 8 half, from a row of
-// any type, rounded to the cache's; zeros for a column past the last.
-template <int TYPE, int D>
-__device__ inline void load_q(const attn_args & a, const kv_seq & s, int h, int c, bool valid, int half,
-                              typename elem<TYPE>::frag qf[D / 16]) {
+__device__ inline float other_row(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 16) ? r[0] : r[1]);
+}
+
+// Query fragments of one column: 8 values each at d = at0, at0 + step, ..., from a
+// row of any type, rounded to the cache's; zeros for a column past the last.
+template <int TYPE, int N>
+__device__ inline void load_q(const attn_args & a, const kv_seq & s, int D, int h, int c, bool valid, int at0, int step,
+                              typename elem<TYPE>::frag qf[N]) {
     const int i = c / a.group, g = c - i * a.group;
-    const int64_t at = (int64_t) (s.row0 + i) * a.ldq + (int64_t) (h * a.group + g) * D + half * 8;
+    const int64_t at = (int64_t) (s.row0 + i) * a.ldq + (int64_t) (h * a.group + g) * D + at0;
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ks++) {
+    for (int k = 0; k < N; k++) {
         typename elem<TYPE>::frag f = {};
         if (valid) {
             if (a.q_type == TYPE) {
-                f = *reinterpret_cast<const typename elem<TYPE>::frag *>((const uint16_t *) a.q + at + ks * 16);
+                f = *reinterpret_cast<const typename elem<TYPE>::frag *>((const uint16_t *) a.q + at + k * step);
             } else if (a.q_type == ZEST_TYPE_F32) {
-                const float * x = (const float *) a.q + at + ks * 16;
+                const float * x = (const float *) a.q + at + k * step;
                 const float4 u = *reinterpret_cast<const float4 *>(x), w = *reinterpret_cast<const float4 *>(x + 4);
                 const float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int j = 0; j < 8; j++) f[j] = elem<TYPE>::from(v[j]);
             } else if (a.q_type == ZEST_TYPE_BF16) {
-                const bf16x8 x = *reinterpret_cast<const bf16x8 *>((const uint16_t *) a.q + at + ks * 16);
+                const bf16x8 x = *reinterpret_cast<const bf16x8 *>((const uint16_t *) a.q + at + k * step);
 #pragma unroll
                 for (int j = 0; j < 8; j++) f[j] = elem<TYPE>::from((float) x[j]);
             } else {
-                const f16x8 x = *reinterpret_cast<const f16x8 *>((const uint16_t *) a.q + at + ks * 16);
+                const f16x8 x = *reinterpret_cast<const f16x8 *>((const uint16_t *) a.q + at + k * step);
 #pragma unroll
                 for (int j = 0; j < 8; j++) f[j] = elem<TYPE>::from((float) x[j]);
             }
@@ -136,7 +142,7 @@ __device__ inline void load_q(const attn_args & a, const kv_seq & s, int h, int 
                 for (int j = 0; j < 8; j++) f[j] = elem<TYPE>::from((float) f[j] * a.sign);
             }
         }
-        qf[ks] = f;
+        qf[k] = f;
     }
 }
 
@@ -151,113 +157,14 @@ template <int TYPE> __device__ inline bool nonfinite(typename elem<TYPE>::frag f
     return (carry & 0x80008000u) != 0;
 }
 
-// The running softmax of a wave's 32 columns: a lane's maximum (of its column,
-// scores times log2 e), the sum of its own weights, and O^T.
-template <int D> struct softmax_state {
-    float m, l;
-    f32x16 o[D / 32];
-};
-
-// What of a group of 32 tokens a lane's column sees: tokens [lo, hi), and of
-// each 16 tokens whether their page is there.
-struct group_mask {
-    int32_t t0, lo, hi;
-    bool ok[2];
-};
-
-// One group of 32 tokens: scores, running maximum and sum, weights times V.
-// masked (the same in every lane): some column does not see some token.
-// v(dt, g): the V fragment of rows 32 dt .. of O^T and tokens 16 g .. of the group.
-template <int TYPE, int D, typename V>
-__device__ inline void attend(const attn_args & a, const typename elem<TYPE>::frag qf[D / 16],
-                              const typename elem<TYPE>::frag kf[D / 16], V && v, const group_mask & k, bool masked,
-                              softmax_state<D> & st) {
-    typedef typename elem<TYPE>::frag frag;
-    const int half = (threadIdx.x >> 5) & 1;
-    f32x16 s = {};
+// A fragment with only its value e, in the lanes that keep it (zeros else).
+template <int TYPE> __device__ inline typename elem<TYPE>::frag only(typename elem<TYPE>::frag f, bool keep, int e) {
+    struct words { uint32_t w[4]; };
+    words v = __builtin_bit_cast(words, f);
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ks++) s = elem<TYPE>::mfma(kf[ks], qf[ks], s);
-    if (a.softcap > 0.0f) {
-        const float in = a.scale / a.softcap * (2.0f * LOG2E), cap = a.softcap * LOG2E;
-#pragma unroll
-        for (int i = 0; i < 16; i++)  // cap * tanh(x): 1 - 2 / (e^2x + 1), off by 2^-23 of the cap at most
-            s[i] = cap - 2.0f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[i] * in) + 1.0f);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] *= a.scale * LOG2E;
-    }
-    if (masked) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int32_t t = k.t0 + (i & 3) + 8 * (i >> 2) + 4 * half;
-            s[i] = t >= k.lo && t < k.hi && k.ok[i >> 3] ? s[i] : -INFINITY;
-        }
-    }
-    float top = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
-    top = fmaxf(top, other_half(top));
-    const float m = fmaxf(st.m, top);
-    // a column that has seen nothing yet keeps -inf; its weights are 2^-inf = 0
-    const float base = (m == -INFINITY ? 0.0f : m) - elem<TYPE>::SHIFT;
-    const float shrink = __builtin_amdgcn_exp2f(st.m - (base + elem<TYPE>::SHIFT));
-    if (__any(m != st.m)) {
-#pragma unroll
-        for (int dt = 0; dt < D / 32; dt++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) st.o[dt][i] *= shrink;
-        st.l *= shrink;
-    }
-    st.m = m;
-    float p[16], sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        p[i] = __builtin_amdgcn_exp2f(s[i] - base);
-        sum += p[i];
-    }
-    st.l += sum;
-#pragma unroll
-    for (int g = 0; g < 2; g++) {
-        frag pf;
-#pragma unroll
-        for (int j = 0; j < 8; j++) pf[j] = elem<TYPE>::from(p[8 * g + j]);
-        bool odd = false;
-        if (masked) {
-#pragma unroll
-            for (int dt = 0; dt < D / 32; dt++) odd |= nonfinite<TYPE>(v(dt, g));
-        }
-        if (masked && __any(odd)) {
-            // A weight of 0 does not silence a NaN or an infinity: the 16 tokens
-            // one at a time, each added where its column sees it
-            for (int tt = 0; tt < 16; tt++) {
-                const int j = (tt & 3) + (tt >> 3) * 4, h = (tt >> 2) & 1;
-                const int32_t t = k.t0 + 16 * g + tt;
-                const bool in = t >= k.lo && t < k.hi && k.ok[g];
-                if (!__any(in)) continue;
-                struct words { uint32_t w[4]; };
-                words keep;
-#pragma unroll
-                for (int w = 0; w < 4; w++) keep.w[w] = half == h && w == j >> 1 ? (j & 1 ? 0xffff0000u : 0xffffu) : 0u;
-#pragma unroll
-                for (int dt = 0; dt < D / 32; dt++) {
-                    words x = __builtin_bit_cast(words, v(dt, g));
-#pragma unroll
-                    for (int w = 0; w < 4; w++) x.w[w] &= keep.w[w];
-                    const f32x16 one = elem<TYPE>::mfma(__builtin_bit_cast(frag, x), pf, f32x16{});
-#pragma unroll
-                    for (int i = 0; i < 16; i++) st.o[dt][i] = in ? st.o[dt][i] + one[i] : st.o[dt][i];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int dt = 0; dt < D / 32; dt++) st.o[dt] = elem<TYPE>::mfma(v(dt, g), pf, st.o[dt]);
-        }
-    }
+    for (int i = 0; i < 4; i++) v.w[i] &= keep && i == e >> 1 ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+    return __builtin_bit_cast(typename elem<TYPE>::frag, v);
 }
-
-// A partial result of a column tile: O^T times its weights' sum as [32][D], the
-// maxima and the sums.
-template <int D> constexpr int PARTIAL = COLS * (D + 2);
 
 // Four values of an output row.
 __device__ inline void store4(const attn_args & a, int64_t at, const float v[4]) {
@@ -272,145 +179,338 @@ __device__ inline void store4(const attn_args & a, int64_t at, const float v[4])
     *reinterpret_cast<uint2 *>((uint16_t *) a.out + at) = make_uint2(w[0] | (uint32_t) w[1] << 16, w[2] | (uint32_t) w[3] << 16);
 }
 
-// Where the units of the whole call lie: workgroup w of W takes [u0, u1).
-__device__ inline void share_of(int32_t total, int w, int W, int32_t & u0, int32_t & u1) {
-    u0 = (int32_t) ((int64_t) total * w / W);
-    u1 = (int32_t) ((int64_t) total * (w + 1) / W);
+// Scores with a softcap, in units of log2: cap * tanh(x) as 1 - 2 / (e^2x + 1),
+// off by 2^-23 of the cap at most.
+__device__ inline float capped(const attn_args & a, float s) {
+    const float cap = a.softcap * LOG2E;
+    return cap - 2.0f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * (a.scale / a.softcap * (2.0f * LOG2E))) + 1.0f);
 }
+
+// ---- few columns: decoding ----------------------------------------------------------
+
+typedef __attribute__((address_space(3))) void * lds_ptr_t;
+typedef const __attribute__((address_space(1))) void * global_ptr_t;
+
+// The call's units are shared out evenly: the first total % W workgroups of W
+// take one more than the others.
+struct unit_shares {
+    int32_t each, more;
+    __device__ unit_shares(int32_t total, int W) : each(total / W), more(total - total / W * W) {}
+    __device__ int32_t start(int w) const { return w * each + min(w, more); }
+    __device__ int32_t owner(int32_t u) const {
+        const int32_t big = more * (each + 1);
+        return u < big ? u / (each + 1) : more + (u - big) / max(each, 1);
+    }
+};
+
+// Tokens' K, then V, that a wave has in flight: RING_B steps of 32.
+template <int D> constexpr int RING_B = D <= 64 ? 2 : 1;
+template <int D> constexpr int STEP_BYTES = GROUP * D * 4;  // 32 tokens' K, then V
+// A partial result of a column tile: O^T relative to the maxima, by columns, the
+// maxima and the sums.
+constexpr int partial_floats(int cols, int D) { return cols * (D + 2); }
 
 // The units of every (sequence, k/v head, column tile) follow each other, and
 // each workgroup takes an equal share of them, however long each sequence is. A
 // piece of a share is one column tile's run of units; its four waves take 32
-// tokens of a unit each, straight from the cache into the MFMA's registers, and
-// are joined in shared memory. A piece that is the tile's whole run goes to the
-// output; else it is a partial result (slot 2w + 1 where it starts the run, 2w
-// where it continues one), and combine_kernel joins a run's pieces in order.
-template <int TYPE, int D>
+// tokens of a unit each and are joined in shared memory. A piece that is the
+// tile's whole run goes to the output; else it is a partial result (slot 2w + 1
+// where it starts the run, 2w where it continues one), and combine_kernel joins a
+// run's pieces in order.
+//
+// HBM bound: 4 D bytes of K and V a token for 4 D COLS operations. A wave keeps a
+// ring of its own in shared memory that direct loads fill (16 bytes a lane, whole
+// kilobytes, no registers): K of the step to come is requested as soon as the
+// scores are made, V as soon as it is weighed, and only this wave waits for them,
+// by counting its loads. Eight waves a CU so have 64 to 128 KB in flight.
+//
+// Tiles of 16 columns on v_mfma_f32_16x16x32, NT of them sharing the K and V read:
+// a token's group of query heads rarely fills 32 columns, and half the columns
+// are half the registers. The two 16-token score tiles of a step are tokens
+// {0..7, 16..23} and {8..15, 24..31}, so that a lane group's 8 weights, in the
+// registers they are in, are the 8 tokens of a V piece.
+template <int TYPE, int D, int NT>
 __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_args a) {
     typedef typename elem<TYPE>::frag frag;
-    extern __shared__ __align__(16) int32_t attn_sh[];
-    __shared__ float tile[WAVES][COLS][36];  // 32 columns' d values of a 32-row block of O^T
+    constexpr int COLS = 16 * NT, KS = D / 32, DT = D / 16, R = RING_B<D>, LOADS = D / 16;  // loads of K (or V) a step
+    extern __shared__ __align__(1024) uint8_t ring_sh[];  // a wave: [R][K: D/8][32][8], V: [4][D][8]; then the prefix sums
     __shared__ float stat[WAVES][2][COLS];
-    int32_t * prefix = attn_sh;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = lane >> 4, col = lane & 15;
     const int ps = a.c.page_shift, P = 1 << ps;
-    zest::prefix_over_seqs(a.b, ps, prefix, [&](const kv_seq & s) { return cost_of(a, s); });
-    int32_t u, u1;
-    share_of(prefix[a.b.seqs], blockIdx.x, gridDim.x, u, u1);
+    const zest::seq_index index(a.b, ps, reinterpret_cast<int32_t *>(ring_sh + WAVES * R * STEP_BYTES<D>),
+                                [&](const kv_seq & s) { return cost_of(a, s, COLS); });
+    const unit_shares shares(index.total, gridDim.x);
+    int32_t u = shares.start(blockIdx.x);
+    const int32_t u1 = shares.start(blockIdx.x + 1);
+    uint8_t * const mine = ring_sh + wave * R * STEP_BYTES<D>;
+    const uint32_t ring_at = (uint32_t) (uintptr_t) (lds_ptr_t) mine;
     bool bad = false;
     while (u < u1) {
-        const int b = __builtin_amdgcn_readfirstlane(zest::seq_of(prefix, a.b.seqs, u));
-        const kv_seq s = zest::load_seq(a.b, b, ps, bad);
-        const int32_t run = units_of(a, s), at = u - prefix[b], tiles = col_tiles(a, s);
-        const int32_t ct = at / run % tiles, h = at / run / tiles, first = at % run;
+        int32_t before;
+        const kv_seq s = index.at(u, before);
+        const int32_t run = units_of(a, s), at = u - before, tiles = col_tiles(a, s, COLS);
+        const int32_t item = at / run, first = at - item * run, h = item / tiles, ct = item - h * tiles;
         const int32_t units = min(run - first, u1 - u);
         const int32_t * row = a.b.tables + (int64_t) s.slot * a.b.table_cols;
-
-        const int c = ct * COLS + col, ncols = s.n * a.group;
-        const bool valid = c < ncols;
-        frag qf[D / 16];
-        load_q<TYPE, D>(a, s, h, c, valid, half, qf);
-        // what the lane's column sees, and what all the tile's columns see
-        int32_t lo, hi, all_lo, all_hi, any_lo, any_hi, seq_lo, seq_hi;
-        const int i0 = ct * COLS / a.group, i1 = min(ncols - 1, ct * COLS + COLS - 1) / a.group;
-        seen_by(a, s, c / a.group, c / a.group, lo, hi);
-        if (!valid) lo = hi = 0;
-        seen_by(a, s, i0, i0, any_lo, all_hi);
-        seen_by(a, s, i1, i1, all_lo, any_hi);
+        const int ncols = s.n * a.group, c0 = ct * COLS;
+        // what all the tile's columns see, and what any of them does
+        int32_t all_lo, all_hi, any_lo, any_hi, seq_lo, seq_hi;
+        seen_by(a, s, c0 / a.group, c0 / a.group, any_lo, all_hi);
+        const int last_row = (min(ncols, c0 + COLS) - 1) / a.group;
+        seen_by(a, s, last_row, last_row, all_lo, any_hi);
         seen_by(a, s, 0, s.n - 1, seq_lo, seq_hi);
         seq_lo &= ~(GROUP - 1);
 
-        softmax_state<D> st;
-        st.m = -INFINITY;
-        st.l = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < D / 32; dt++) st.o[dt] = f32x16{};
-        for (int32_t unit = first; unit < first + units; unit++) {
-            const int32_t t0 = seq_lo + unit * UNIT + wave * GROUP;
-            if (t0 >= any_hi || t0 + GROUP <= any_lo) continue;
-            group_mask k{t0, lo, hi, {true, true}};
-            const uint8_t * base[2];
+        // this wave's steps: tokens t_first + j * UNIT .. + 31, j < n
+        const int32_t t_first = seq_lo + first * UNIT + wave * GROUP;
+        const int32_t n = min(units, max(0, (any_hi - t_first + UNIT - 1) / UNIT));
+        const int64_t head_at = (int64_t) h * (4 * P * D);
+        // the pages of a step's two 16-token halves (0 where there is none), and
+        // which halves have one: bit g
+        auto pages_of = [&](int j, int32_t id[2]) {
+            uint32_t there = 0;
 #pragma unroll
             for (int g = 0; g < 2; g++) {
-                const int32_t tg = t0 + 16 * g;
-                int32_t id = 0;
-                k.ok[g] = tg < any_hi;
-                if (k.ok[g]) {
-                    id = row[tg >> ps];
-                    if ((uint32_t) id >= (uint32_t) a.c.pages) {
-                        id = 0;
-                        k.ok[g] = false;
+                const int32_t t = t_first + j * UNIT + 16 * g;
+                id[g] = 0;
+                if (j < n && t < any_hi) {
+                    const int32_t x = row[t >> ps];
+                    if ((uint32_t) x < (uint32_t) a.c.pages) {
+                        id[g] = x;
+                        there |= 1u << g;
+                    } else {
                         bad = true;
                     }
                 }
-                base[g] = a.c.pool + id * a.c.page_bytes + (int64_t) h * (4 * P * D);
             }
+            return there;
+        };
+        auto load_k = [&](int j, const int32_t id[2]) {
+            const int32_t t0 = t_first + j * UNIT;
             const uint32_t in0 = t0 & (P - 1), in1 = (t0 + 16) & (P - 1);
-            const uint8_t * kp = (lane & 16 ? base[1] + in1 * 16 : base[0] + in0 * 16) + (lane & 15) * 16 + half * P * 16;
-            frag kf[D / 16];
+            // a lane's token lane % 32 of K's rows 2i + lane / 32
+            const int64_t off0 = id[0] * a.c.page_bytes + in0 * 16, off1 = id[1] * a.c.page_bytes + in1 * 16;
+            const uint8_t * from = a.c.pool + head_at + (lane & 16 ? off1 : off0) + (lane & 15) * 16 + (lane >> 5) * (P * 16);
+            const uint32_t to = ring_at + (j % R) * STEP_BYTES<D>;
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ks++) kf[ks] = *reinterpret_cast<const frag *>(kp + ks * (P * 32));
-            const uint8_t * vp[2];
+            for (int i = 0; i < LOADS; i++)
+                __builtin_amdgcn_global_load_lds((global_ptr_t) (from + i * (P * 32)), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
+        };
+        auto load_v = [&](int j, const int32_t id[2]) {
+            const int32_t t0 = t_first + j * UNIT;
+            const uint32_t to = ring_at + (j % R) * STEP_BYTES<D> + GROUP * D * 2;
 #pragma unroll
-            for (int g = 0; g < 2; g++) vp[g] = base[g] + 2 * P * D + (g ? in1 : in0) * (2 * D) + half * (16 * D) + col * 16;
-            auto load_v = [&](int dt, int g) { return *reinterpret_cast<const frag *>(vp[g] + dt * 512); };
-            const bool masked = t0 < all_lo || t0 + GROUP > all_hi || !k.ok[0] || !k.ok[1];
-            if constexpr (D <= 128) {  // V requested with K; wider heads have no registers for it
-                frag vf[D / 32][2];
+            for (int g = 0; g < 2; g++) {
+                const uint32_t in = (t0 + 16 * g) & (P - 1);
+                const uint8_t * from = a.c.pool + head_at + id[g] * a.c.page_bytes + 2 * P * D + in * (2 * D) + lane * 16;
 #pragma unroll
-                for (int g = 0; g < 2; g++)
+                for (int i = 0; i < LOADS / 2; i++)
+                    __builtin_amdgcn_global_load_lds((global_ptr_t) (from + i * 1024),
+                                                     (lds_ptr_t) (uintptr_t) (to + (g * (LOADS / 2) + i) * 1024), 16, 0, 0);
+            }
+        };
+        int32_t id[R + 1][2];      // of steps j .. j + R
+        uint32_t there[R + 1];
 #pragma unroll
-                    for (int dt = 0; dt < D / 32; dt++) vf[dt][g] = load_v(dt, g);
-                attend<TYPE, D>(a, qf, kf, [&](int dt, int g) { return vf[dt][g]; }, k, masked, st);
-            } else {
-                attend<TYPE, D>(a, qf, kf, load_v, k, masked, st);
+        for (int r = 0; r < R; r++) {
+            there[r] = pages_of(r, id[r]);
+            if (r < n) {
+                load_k(r, id[r]);
+                load_v(r, id[r]);
             }
         }
 
-        // the waves' results joined: every column's maximum and sum, then O^T a
-        // 32-row block at a time, stored by columns
-        st.l += other_half(st.l);
-        __syncthreads();
-        if (half == 0) {
-            stat[wave][0][col] = st.m;
-            stat[wave][1][col] = st.l;
+        frag qf[NT][KS];
+        int32_t see_lo[NT], see_hi[NT];
+#pragma unroll
+        for (int q = 0; q < NT; q++) {
+            const int c = c0 + 16 * q + col;
+            load_q<TYPE, KS>(a, s, D, h, c, c < ncols, lg * 8, 32, qf[q]);
+            seen_by(a, s, c / a.group, c / a.group, see_lo[q], see_hi[q]);
+            if (c >= ncols) see_lo[q] = see_hi[q] = 0;
         }
-        __syncthreads();
-        float m = stat[0][0][col];
+        float m[NT], l[NT];
+        f32x4 o[DT][NT];
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) m = fmaxf(m, stat[w][0][col]);
-        const float base = m == -INFINITY ? 0.0f : m;
-        const float mine = __builtin_amdgcn_exp2f(st.m - base);
-        float l = 0.0f;
+        for (int q = 0; q < NT; q++) {
+            m[q] = -INFINITY;
+            l[q] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) l += stat[w][1][col] * __builtin_amdgcn_exp2f(stat[w][0][col] - base);
-        const bool whole = units == run;
-        float * slot = a.partial + (int64_t) (2 * blockIdx.x + (first == 0)) * PARTIAL<D>;
-        if (!whole && wave == 0 && half == 0) {
-            slot[COLS * D + col] = m;
-            slot[COLS * D + COLS + col] = l;
+            for (int dt = 0; dt < DT; dt++) o[dt][q] = f32x4{};
         }
-        const float factor = whole ? (l == 0.0f ? 0.0f : mine / l) : mine;
-        const int oc = threadIdx.x >> 3, od = (threadIdx.x & 7) * 4, cc = ct * COLS + oc;
-        const int64_t to = (int64_t) (s.row0 + cc / a.group) * a.ldo + (int64_t) (h * a.group + cc % a.group) * D + od;
+        for (int32_t j = 0; j < n; j++) {
+            const int32_t t0 = t_first + j * UNIT;
+            const uint8_t * slot = mine + (j % R) * STEP_BYTES<D>;
+            const bool more = j + R < n;
+            there[R] = pages_of(j + R, id[R]);
+            const bool masked = t0 < all_lo || t0 + GROUP > all_hi || there[0] != 3;
+
+            // K: all but the loads after it
+            if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((2 * R - 1) * LOADS) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            f32x4 sc[NT][2];
 #pragma unroll
-        for (int dt = 0; dt < D / 32; dt++) {
+            for (int q = 0; q < NT; q++) sc[q][0] = sc[q][1] = f32x4{};
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const float4 v = make_float4(st.o[dt][i] * factor, st.o[dt][i + 1] * factor, st.o[dt][i + 2] * factor, st.o[dt][i + 3] * factor);
-                *reinterpret_cast<float4 *>(&tile[wave][col][2 * i + 4 * half]) = v;
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int tok = (col & 7) + 16 * (col >> 3) + 8 * x;
+                    const frag k = *reinterpret_cast<const frag *>(slot + ((ks * 4 + lg) * 32 + tok) * 16);
+#pragma unroll
+                    for (int q = 0; q < NT; q++) sc[q][x] = elem<TYPE>::mfma16(k, qf[q][ks], sc[q][x]);
+                }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read before it is overwritten
+            if (more) load_k(j + R, id[R]);
+
+            const float c = a.softcap > 0.0f ? 1.0f : a.scale * LOG2E;
+            frag pf[NT];
+#pragma unroll
+            for (int q = 0; q < NT; q++) {
+                // value e of x: token t0 + base + e + 8x of the lane group's base
+                const int32_t base_t = t0 + 4 * (lg & 1) + 16 * (lg >> 1);
+                if (a.softcap > 0.0f) {
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sc[q][x][e] = capped(a, sc[q][x][e]);
+                }
+                if (masked) {
+                    const bool page = there[0] >> (lg >> 1) & 1;
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int32_t t = base_t + e + 8 * x;
+                            sc[q][x][e] = page && t >= see_lo[q] && t < see_hi[q] ? sc[q][x][e] : -INFINITY;
+                        }
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top = fmaxf(top, sc[q][x][e]);
+                top = fmaxf(top, other_row(top));
+                top = fmaxf(top, other_half(top)) * c;
+                const float now = fmaxf(m[q], top);
+                const float base = now == -INFINITY ? 0.0f : now;
+                const float shrink = __builtin_amdgcn_exp2f(m[q] - base), shift = elem<TYPE>::SHIFT - base;
+                if (__any(now != m[q])) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) o[dt][q] *= shrink;
+                }
+                m[q] = now;
+                float sum = 0.0f;
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float w = __builtin_amdgcn_exp2f(fmaf(sc[q][x][e], c, shift));
+                        sum += w;
+                        pf[q][4 * x + e] = elem<TYPE>::from(w);
+                    }
+                l[q] = l[q] * shrink + sum;
             }
-            __syncthreads();
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+
+            if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((2 * R - 1) * LOADS) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const uint8_t * vp = slot + GROUP * D * 2 + (lg * D + col) * 16;
+            bool odd = false;
+            if (masked) {
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) odd |= nonfinite<TYPE>(*reinterpret_cast<const frag *>(vp + dt * 256));
+            }
+            if (masked && __any(odd)) {
+                // A weight of 0 does not silence a NaN or an infinity: the tokens
+                // one at a time, each added where its column sees it
+                for (int tt = 0; tt < GROUP; tt++) {
+                    const int e = (tt & 3) + (tt >> 3 & 1) * 4, g = (tt >> 2 & 1) + 2 * (tt >> 4);  // its value of its lane group
+                    const bool page = there[0] >> (tt >> 4) & 1;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+                        const frag v = only<TYPE>(*reinterpret_cast<const frag *>(vp + dt * 256), lg == g, e);
+#pragma unroll
+                        for (int q = 0; q < NT; q++) {
+                            const bool in = page && t0 + tt >= see_lo[q] && t0 + tt < see_hi[q];
+                            const f32x4 one = elem<TYPE>::mfma16(v, pf[q], f32x4{});
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[dt][q][i] = in ? o[dt][q][i] + one[i] : o[dt][q][i];
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    const frag v = *reinterpret_cast<const frag *>(vp + dt * 256);
+#pragma unroll
+                    for (int q = 0; q < NT; q++) o[dt][q] = elem<TYPE>::mfma16(v, pf[q], o[dt][q]);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (more) load_v(j + R, id[R]);
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                there[r] = there[r + 1];
+                id[r][0] = id[r + 1][0];
+                id[r][1] = id[r + 1][1];
+            }
+        }
+
+        // the waves' results joined: every column's maximum and sum, then O^T,
+        // which each wave leaves in its ring by columns (units of 4 values, turned
+        // by the column so that a wave's writes spread over the banks)
+        constexpr int UNITS = D / 4;
+#pragma unroll
+        for (int q = 0; q < NT; q++) {
+            l[q] += other_row(l[q]);
+            l[q] += other_half(l[q]);
+            if (lg == 0) {
+                stat[wave][0][16 * q + col] = m[q];
+                stat[wave][1][16 * q + col] = l[q];
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                int unit = 4 * dt + lg + col;
+                if (unit >= UNITS) unit -= UNITS;
+                *reinterpret_cast<f32x4 *>(mine + ((16 * q + col) * UNITS + unit) * 16) = o[dt][q];
+            }
+        }
+        __syncthreads();
+        const bool whole = units == run;
+        float * part = a.partial + (int64_t) (2 * blockIdx.x + (first == 0)) * partial_floats(COLS, D);
+        for (int i = threadIdx.x; i < COLS * UNITS; i += WAVES * 64) {
+            const int oc = i / UNITS, unit = i - oc * UNITS;
+            int turned = unit + (oc & 15);
+            if (turned >= UNITS) turned -= UNITS;
+            float top = stat[0][0][oc];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) top = fmaxf(top, stat[w][0][oc]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int w = 0; w < WAVES; w++) {
-                const float4 x = *reinterpret_cast<const float4 *>(&tile[w][oc][od]);
-                v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+                const float f = __builtin_amdgcn_exp2f(stat[w][0][oc] - base);
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(ring_sh + w * R * STEP_BYTES<D> + (oc * UNITS + turned) * 16);
+                sum += stat[w][1][oc] * f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] += x[e] * f;
             }
-            if (!whole) *reinterpret_cast<float4 *>(slot + oc * D + dt * 32 + od) = make_float4(v[0], v[1], v[2], v[3]);
-            else if (cc < ncols) store4(a, to + dt * 32, v);
-            __syncthreads();
+            const int cc = c0 + oc;
+            if (!whole) {
+                *reinterpret_cast<float4 *>(part + oc * D + unit * 4) = make_float4(v[0], v[1], v[2], v[3]);
+                if (unit == 0) {
+                    part[COLS * D + oc] = top;
+                    part[COLS * D + COLS + oc] = sum;
+                }
+            } else if (cc < ncols) {
+                const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] *= f;
+                const int i0 = cc / a.group;
+                store4(a, (int64_t) (s.row0 + i0) * a.ldo + (int64_t) (h * a.group + cc - i0 * a.group) * D + unit * 4, v);
+            }
         }
+        __syncthreads();
         u += units;
     }
     if (bad) zest::report(a.b.bad);
@@ -418,67 +518,52 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_
 
 // Joins the pieces of the column tile whose run starts in workgroup w's share
 // and goes on past it, if there is one: theirs are the last of the share.
-template <int D>
+template <int D, int NT>
 __global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
     extern __shared__ __align__(16) int32_t attn_sh[];
-    int32_t * prefix = attn_sh;
-    const int ps = a.c.page_shift, W = gridDim.x;
-    zest::prefix_over_seqs(a.b, ps, prefix, [&](const kv_seq & s) { return cost_of(a, s); });
-    const int32_t total = prefix[a.b.seqs];
-    int32_t u0, u1;
-    share_of(total, blockIdx.x, W, u0, u1);
+    constexpr int COLS = 16 * NT, UNITS = D / 4;
+    const zest::seq_index index(a.b, a.c.page_shift, attn_sh, [&](const kv_seq & s) { return cost_of(a, s, COLS); });
+    const unit_shares shares(index.total, gridDim.x);
+    const int32_t u0 = shares.start(blockIdx.x), u1 = shares.start(blockIdx.x + 1);
     if (u0 == u1) return;
-    bool bad = false;
-    const int b = zest::seq_of(prefix, a.b.seqs, u1 - 1);
-    const kv_seq s = zest::load_seq(a.b, b, ps, bad);
-    const int32_t run = units_of(a, s), at = u1 - 1 - prefix[b], tiles = col_tiles(a, s);
-    const int32_t ct = at / run % tiles, h = at / run / tiles;
-    const int32_t start = prefix[b] + at / run * run, end = start + run;
+    int32_t before;
+    const kv_seq s = index.at(u1 - 1, before);
+    const int32_t run = units_of(a, s), at = u1 - 1 - before, tiles = col_tiles(a, s, COLS);
+    const int32_t item = at / run, start = before + item * run, end = start + run;
     if (start < u0 || end <= u1) return;
-    int last = blockIdx.x;
-    for (int32_t x0, x1 = u1; x1 < end;) share_of(total, ++last, W, x0, x1);
-    const int oc = threadIdx.x >> 3, od = (threadIdx.x & 7) * 4, cc = ct * COLS + oc;
-    if (cc >= s.n * a.group) return;
-    auto slot_of = [&](int w) { return a.partial + (int64_t) (2 * w + (w == (int) blockIdx.x)) * PARTIAL<D>; };
-    float m = -INFINITY;
-    for (int w = blockIdx.x; w <= last; w++) {
-        share_of(total, w, W, u0, u1);
-        if (u0 < u1) m = fmaxf(m, slot_of(w)[COLS * D + oc]);
-    }
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o[D / 32][4] = {};
-    for (int w = blockIdx.x; w <= last; w++) {
-        share_of(total, w, W, u0, u1);
-        if (u0 == u1) continue;
-        const float * x = slot_of(w);
-        const float f = __builtin_amdgcn_exp2f(x[COLS * D + oc] - base);
-        l += x[COLS * D + COLS + oc] * f;
-#pragma unroll
-        for (int dt = 0; dt < D / 32; dt++) {
-            const float4 v = *reinterpret_cast<const float4 *>(x + oc * D + dt * 32 + od);
-            o[dt][0] += v.x * f, o[dt][1] += v.y * f, o[dt][2] += v.z * f, o[dt][3] += v.w * f;
+    const int32_t h = item / tiles, ct = item - h * tiles, ncols = s.n * a.group;
+    const int last = shares.owner(end - 1);
+    for (int i = threadIdx.x; i < COLS * UNITS; i += 256) {
+        const int oc = i / UNITS, unit = i - oc * UNITS, cc = ct * COLS + oc;
+        if (cc >= ncols) return;
+        const float * x = a.partial + (int64_t) (2 * blockIdx.x + 1) * partial_floats(COLS, D);
+        float m = x[COLS * D + oc], l = x[COLS * D + COLS + oc];
+        float4 o = *reinterpret_cast<const float4 *>(x + oc * D + unit * 4);
+#pragma unroll 4
+        for (int w = blockIdx.x + 1; w <= last; w++) {
+            const float * y = a.partial + (int64_t) (2 * w) * partial_floats(COLS, D);
+            const float m1 = y[COLS * D + oc], l1 = y[COLS * D + COLS + oc], now = fmaxf(m, m1);
+            const float4 v = *reinterpret_cast<const float4 *>(y + oc * D + unit * 4);
+            const float base = now == -INFINITY ? 0.0f : now;
+            const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(m1 - base);
+            m = now;
+            l = l * f + l1 * g;
+            o = make_float4(o.x * f + v.x * g, o.y * f + v.y * g, o.z * f + v.z * g, o.w * f + v.w * g);
         }
-    }
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t to = (int64_t) (s.row0 + cc / a.group) * a.ldo + (int64_t) (h * a.group + cc % a.group) * D + od;
-#pragma unroll
-    for (int dt = 0; dt < D / 32; dt++) {
-        const float v[4] = {o[dt][0] * f, o[dt][1] * f, o[dt][2] * f, o[dt][3] * f};
-        store4(a, to + dt * 32, v);
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        const float v[4] = {o.x * f, o.y * f, o.z * f, o.w * f};
+        const int i0 = cc / a.group;
+        store4(a, (int64_t) (s.row0 + i0) * a.ldo + (int64_t) (h * a.group + cc - i0 * a.group) * D + unit * 4, v);
     }
 }
 
 // ---- chunks: many columns ---------------------------------------------------------
-
-typedef __attribute__((address_space(3))) void * lds_ptr_t;
-typedef const __attribute__((address_space(1))) void * global_ptr_t;
 
 // Column tiles of 32 a wave of chunk_kernel takes: two where the registers hold
 // them (O^T of 64 columns is D values a lane, Q^T half of that).
 template <int D> constexpr int QT = 1;
 template <int D> constexpr int CHUNK = WAVES * 32 * QT<D>;  // columns of a workgroup
 constexpr int RING = 4;                                     // steps of K and V in shared memory
-template <int D> constexpr int STEP_BYTES = GROUP * D * 4;  // 32 tokens' K, then V
 // How far, in powers of two, a score may pass the maximum its column's weights
 // are relative to before O^T is rescaled: the sums are in fp32, so only the
 // weights' own range matters (bf16: fp32's; fp16: SHIFT + 8 stays below 2^16)
@@ -504,18 +589,18 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
     constexpr int NQ = QT<D>, KS = D / 16, DT = D / 32;
     extern __shared__ __align__(1024) uint8_t ring[];  // [RING][K: D/8][32][8], V: [2][2][D][8]; then the prefix sums
     __shared__ uint32_t missing[RING];                 // bit g: tokens 16g .. of the step have no page
-    int32_t * prefix = reinterpret_cast<int32_t *>(ring + RING * STEP_BYTES<D>);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     const int ps = a.c.page_shift, P = 1 << ps;
-    zest::prefix_over_seqs(a.b, ps, prefix, [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
+    const zest::seq_index index(a.b, ps, reinterpret_cast<int32_t *>(ring + RING * STEP_BYTES<D>),
+                                [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
     // the last tiles first: under a causal mask they see the most
     const int h = blockIdx.x % a.c.kv_heads;
-    const int tile = prefix[a.b.seqs] - 1 - (int) (blockIdx.x / a.c.kv_heads);
+    const int tile = index.total - 1 - (int) (blockIdx.x / a.c.kv_heads);
     if (tile < 0) return;
     bool bad = false;
-    const int b = __builtin_amdgcn_readfirstlane(zest::seq_of(prefix, a.b.seqs, tile));
-    const kv_seq s = zest::load_seq(a.b, b, ps, bad);
-    const int c0 = (tile - prefix[b]) * CHUNK<D>, ncols = s.n * a.group;
+    int32_t before;
+    const kv_seq s = index.at(tile, before);
+    const int c0 = (tile - before) * CHUNK<D>, ncols = s.n * a.group;
     const int32_t * row = a.b.tables + (int64_t) s.slot * a.b.table_cols;
 
     // the tile's tokens, and of them this split's
@@ -534,7 +619,7 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
         const int c = w0 + 32 * q + col;
-        load_q<TYPE, D>(a, s, h, c, c < ncols, half, qf[q]);
+        load_q<TYPE, KS>(a, s, D, h, c, c < ncols, half * 8, 16, qf[q]);
         seen_by(a, s, c / a.group, c / a.group, see_lo[q], see_hi[q]);
         if (c >= ncols) see_lo[q] = see_hi[q] = 0;
     }
@@ -633,22 +718,14 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
                 const int e = (tt & 3) + (tt >> 3) * 4, hh = (tt >> 2) & 1;
                 const int32_t t = t0 + 16 * g + tt;
                 bool in[NQ];
-                struct words { uint32_t w[4]; };
-                words keep;
-#pragma unroll
-                for (int w = 0; w < 4; w++)
-                    keep.w[w] = !careful ? 0xffffffffu : half == hh && w == e >> 1 ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
 #pragma unroll
                 for (int q = 0; q < NQ; q++) in[q] = !careful || (t >= see_lo[q] && t < see_hi[q] && !(gone >> (16 * g) & 1));
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) {
-                    words x = __builtin_bit_cast(words, v_frag(j, dt, g));
-#pragma unroll
-                    for (int w = 0; w < 4; w++) x.w[w] &= keep.w[w];
+                    const frag v = careful ? only<TYPE>(v_frag(j, dt, g), half == hh, e) : v_frag(j, dt, g);
 #pragma unroll
                     for (int q = 0; q < NQ; q++) {
-                        const frag pg = g ? p[q][1] : p[q][0];
-                        const f32x16 one = elem<TYPE>::mfma(__builtin_bit_cast(frag, x), pg, f32x16{});
+                        const f32x16 one = elem<TYPE>::mfma(v, g ? p[q][1] : p[q][0], f32x16{});
 #pragma unroll
                         for (int i = 0; i < 16; i++) o[dt][q][i] = in[q] ? o[dt][q][i] + one[i] : o[dt][q][i];
                     }
@@ -713,12 +790,10 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
         return t0 < all_lo || t0 + GROUP > all_hi || gone != 0;
     };
     auto cap_scores = [&]() {
-        const float in = a.scale / a.softcap * (2.0f * LOG2E), cap = a.softcap * LOG2E;
 #pragma unroll
         for (int q = 0; q < NQ; q++)
 #pragma unroll
-            for (int i = 0; i < 16; i++)  // as in attend
-                s_cur[q][i] = cap - 2.0f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s_cur[q][i] * in) + 1.0f);
+            for (int i = 0; i < 16; i++) s_cur[q][i] = capped(a, s_cur[q][i]);
     };
     auto finish = [&](bool rise, const frag pn[NQ][2]) {
         if (__any(rise)) {
@@ -824,17 +899,14 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
 template <int D>
 __global__ __launch_bounds__(256) void chunk_combine_kernel(attn_args a) {
     extern __shared__ __align__(16) int32_t attn_sh[];
-    int32_t * prefix = attn_sh;
-    const int ps = a.c.page_shift;
-    zest::prefix_over_seqs(a.b, ps, prefix, [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
+    const zest::seq_index index(a.b, a.c.page_shift, attn_sh, [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
     constexpr int PARTS = CHUNK<D> / 32;
     const int part = blockIdx.x % PARTS, at = blockIdx.x / PARTS, h = at % a.c.kv_heads, tile = at / a.c.kv_heads;
-    if (tile >= prefix[a.b.seqs]) return;
-    bool bad = false;
-    const int b = zest::seq_of(prefix, a.b.seqs, tile);
-    const kv_seq s = zest::load_seq(a.b, b, ps, bad);
+    if (tile >= index.total) return;
+    int32_t before;
+    const kv_seq s = index.at(tile, before);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, k = threadIdx.x >> 6;
-    const int cc = (tile - prefix[b]) * CHUNK<D> + part * 32 + col;
+    const int cc = (tile - before) * CHUNK<D> + part * 32 + col;
     if (cc >= s.n * a.group) return;
     const float * slots = a.chunk_partial + (int64_t) at * a.chunk_splits * CHUNK_PARTIAL<D>;
     float m = -INFINITY, l = 0.0f;
@@ -864,8 +936,8 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(attn_args a) {
 
 // What a call launches, by its sizes and bounds alone.
 struct attn_plan {
-    int64_t units;              // of attn_kernel, at most
-    int workgroups;             // of attn_kernel, 0: not launched
+    int64_t units, run;         // of attn_kernel, at most: in all, and of a column tile
+    int workgroups, cols;       // of attn_kernel, 0: not launched; columns of its tiles
     int chunk_cols;             // sequences of more columns go to chunk_kernel
     int64_t chunk_tiles;        // of chunk_kernel, a k/v head, at most; 0: not launched
     int chunk_splits;
@@ -886,34 +958,47 @@ attn_plan plan_of(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
     }
     if (p.chunk_cols > 0) {
         const int64_t cols = std::min<int64_t>(most, p.chunk_cols);
-        const int64_t run = std::max<int64_t>(1, ((int64_t) b->max_len + GROUP + UNIT - 1) / UNIT);
-        const int64_t tiles = std::min<int64_t>((b->rows * group + COLS - 1) / COLS + b->seqs, (cols + COLS - 1) / COLS * b->seqs);
-        p.units = run * tiles * c->kv_heads;
-        p.workgroups = (int) std::min<int64_t>(p.units, MAX_WORKGROUPS);
+        p.cols = cols <= 16 ? 16 : 32;
+        p.run = std::max<int64_t>(1, ((int64_t) b->max_len + GROUP + UNIT - 1) / UNIT);
+        const int64_t tiles = std::min<int64_t>((b->rows * group + p.cols - 1) / p.cols + b->seqs, (cols + p.cols - 1) / p.cols * b->seqs);
+        p.units = p.run * tiles * c->kv_heads;
+        p.workgroups = (int) std::min<int64_t>(p.units, c->head_dim <= 128 ? 2 * CUS : CUS);
     }
-    p.partial_bytes = (size_t) 2 * p.workgroups * COLS * (c->head_dim + 2) * sizeof(float);
+    p.partial_bytes = (size_t) 2 * p.workgroups * partial_floats(p.cols, c->head_dim) * sizeof(float);
     p.bytes = p.partial_bytes;
     if (p.chunk_splits > 1) p.bytes += (size_t) p.chunk_tiles * c->kv_heads * p.chunk_splits * chunk * (c->head_dim + 2) * sizeof(float);
     p.bytes = std::max<size_t>(p.bytes, 16);
     return p;
 }
 
+template <typename K> int allow_lds(K kernel, size_t bytes) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
+    return e == hipSuccess ? ZEST_OK : zest::fail(ZEST_E_HIP, "zest_kv_attn: shared memory of %zu bytes: %s", bytes, hipGetErrorString(e));
+}
+
+template <int TYPE, int D, int NT> int launch_few(const attn_args & a, const attn_plan & p, hipStream_t s) {
+    const size_t ring = WAVES * RING_B<D> * STEP_BYTES<D> + zest::seq_index_bytes(a.b.seqs);
+    if (ring + 1024 > 65536)
+        if (const int st = allow_lds(&attn_kernel<TYPE, D, NT>, ring)) return st;
+    hipLaunchKernelGGL((attn_kernel<TYPE, D, NT>), dim3(p.workgroups), dim3(WAVES * 64), ring, s, a);
+    if (p.run > 1)  // else every piece is a whole run
+        hipLaunchKernelGGL((combine_kernel<D, NT>), dim3(p.workgroups), dim3(256), zest::seq_index_bytes(a.b.seqs), s, a);
+    return ZEST_OK;
+}
+
 template <int TYPE, int D> int launch(const attn_args & a, const attn_plan & p, hipStream_t s) {
-    const size_t lds = (size_t) ((a.b.seqs + 4) & ~3) * 4;
     if (p.chunk_tiles) {
-        const size_t ring = RING * STEP_BYTES<D> + lds;
-        if (ring + 1024 > 65536) {
-            static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&chunk_kernel<TYPE, D>),
-                                                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 1024);
-            if (e != hipSuccess) return zest::fail(ZEST_E_HIP, "zest_kv_attn: shared memory of %zu bytes: %s", ring, hipGetErrorString(e));
-        }
+        const size_t ring = RING * STEP_BYTES<D> + zest::seq_index_bytes(a.b.seqs);
+        if (ring + 1024 > 65536)
+            if (const int st = allow_lds(&chunk_kernel<TYPE, D>, ring)) return st;
         hipLaunchKernelGGL((chunk_kernel<TYPE, D>), dim3((unsigned) (p.chunk_tiles * a.c.kv_heads), p.chunk_splits), dim3(WAVES * 64), ring,
                            s, a);
     }
-    if (p.workgroups) hipLaunchKernelGGL((attn_kernel<TYPE, D>), dim3(p.workgroups), dim3(WAVES * 64), lds, s, a);
+    if (p.workgroups)
+        if (const int st = p.cols == 16 ? launch_few<TYPE, D, 1>(a, p, s) : launch_few<TYPE, D, 2>(a, p, s)) return st;
     if (p.chunk_splits > 1)
-        hipLaunchKernelGGL(chunk_combine_kernel<D>, dim3((unsigned) (p.chunk_tiles * a.c.kv_heads * (CHUNK<D> / 32))), dim3(256), lds, s, a);
-    if (p.workgroups) hipLaunchKernelGGL(combine_kernel<D>, dim3(p.workgroups), dim3(256), lds, s, a);
+        hipLaunchKernelGGL(chunk_combine_kernel<D>, dim3((unsigned) (p.chunk_tiles * a.c.kv_heads * (CHUNK<D> / 32))), dim3(256),
+                           zest::seq_index_bytes(a.b.seqs), s, a);
     return zest::check_launch("zest_kv_attn");
 }
 

@@ -119,18 +119,15 @@ struct append_args {
 // whole rows and writes whole lines.
 __global__ __launch_bounds__(256) void append_kernel(append_args a) {
     extern __shared__ __align__(16) int32_t append_sh[];
-    int32_t * prefix = append_sh;
-    float2 * turn = reinterpret_cast<float2 *>(append_sh + ((a.b.seqs + 1 + 3) & ~3));  // [16][rot / 2]
     const int t = threadIdx.x, ps = a.c.page_shift;
-    zest::prefix_over_seqs(a.b, ps, prefix, [](const kv_seq & s) {
-        return s.n > 0 ? ((s.len - 1) >> 4) - ((s.len - s.n) >> 4) + 1 : 0;
-    });
-    if ((int32_t) blockIdx.x >= prefix[a.b.seqs]) return;
-    const int b = zest::seq_of(prefix, a.b.seqs, (int32_t) blockIdx.x);
-    bool bad = false;
-    const kv_seq s = zest::load_seq(a.b, b, ps, bad);
+    const size_t prefix_words = a.b.seqs <= 64 ? 0 : (a.b.seqs + 4) & ~3;
+    float2 * turn = reinterpret_cast<float2 *>(append_sh + prefix_words);  // [16][rot / 2]
+    const zest::seq_index index(a.b, ps, append_sh, [](const kv_seq & s) { return s.n > 0 ? ((s.len - 1) >> 4) - ((s.len - s.n) >> 4) + 1 : 0; });
+    if ((int32_t) blockIdx.x >= index.total) return;
+    int32_t before;
+    const kv_seq s = index.at((int32_t) blockIdx.x, before);
     const int32_t first = s.len - s.n;                                               // place of the first new token
-    const int32_t p0 = ((first >> 4) + ((int32_t) blockIdx.x - prefix[b])) << 4;     // the 16 places
+    const int32_t p0 = ((first >> 4) + ((int32_t) blockIdx.x - before)) << 4;         // the 16 places
     const int32_t lo = max(p0, first), hi = min(p0 + 16, s.len);                     // of them, new
     const int32_t r0 = s.row0 + (lo - first);                                        // row of place lo
     const int n = hi - lo, D = a.d, half = a.rot / 2;
@@ -625,7 +622,7 @@ int zest_kv_append(const zest_kv_cache * cache, const zest_kv_batch * batch, con
     const int64_t units = std::min<int64_t>(batch->rows, batch->rows / 16 + 2ll * batch->seqs);
     const int heads = a.q_heads + 2 * a.c.kv_heads;
     a.heads_each = (int) std::max<int64_t>(1, std::min<int64_t>(8, units * heads / 1024));
-    const size_t lds = (size_t) ((batch->seqs + 4) & ~3) * 4 + (size_t) 16 * (a.rot / 2) * sizeof(float2);
+    const size_t lds = zest::seq_index_bytes(batch->seqs) + (size_t) 16 * (a.rot / 2) * sizeof(float2);
     hipLaunchKernelGGL(append_kernel, dim3((unsigned) units, (unsigned) ((heads + a.heads_each - 1) / a.heads_each)), dim3(256),
                        lds, zest::as_stream(stream), a);
     return zest::check_launch(me);

@@ -1,5 +1,5 @@
 // What the paged KV cache's kernels share: its layout, the checked view of a
-// batch's sequences, and the prefix sums by which a workgroup finds its work.
+// batch's sequences, and how a workgroup finds its work among them.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -52,48 +52,84 @@ __device__ inline kv_seq load_seq(const kv_batch & a, int b, int page_shift, boo
     return s;
 }
 
-// prefix[b] = sum of cost(sequence) over the sequences before b, for b = 0 ..
-// seqs, in shared memory: every thread sums a run of sequences, a wave's sums
-// are scanned by lane exchanges and the waves' by every thread. All threads of
-// the workgroup (a multiple of 64, at most 1024) call it; it ends in a barrier.
-template <typename Cost>
-__device__ inline void prefix_over_seqs(const kv_batch & a, int page_shift, int32_t * prefix, Cost cost) {
-    __shared__ int32_t wave_sum[16];
-    const int t = threadIdx.x, threads = blockDim.x, lane = t & 63;
-    const int run = (a.seqs + threads - 1) / threads, first = min(t * run, a.seqs), last = min(first + run, a.seqs);
-    bool bad = false;
-    int32_t sum = 0;
-    for (int b = first; b < last; b++) {
-        const int32_t c = cost(load_seq(a, b, page_shift, bad));
-        prefix[b + 1] = c;
-        sum += c;
-    }
-    int32_t scan = sum;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int32_t v = __shfl_up(scan, off);
-        if (lane >= off) scan += v;
-    }
-    if (lane == 63) wave_sum[t >> 6] = scan;
-    __syncthreads();
-    int32_t before = scan - sum;
-    for (int w = 0; w < (t >> 6); w++) before += wave_sum[w];
-    if (t == 0) prefix[0] = 0;
-    for (int b = first; b < last; b++) prefix[b + 1] = before += prefix[b + 1];
-    if (bad && blockIdx.x == 0) report(a.bad);
-    __syncthreads();
-}
+// Where the sequences' runs of work lie: the sum of a cost over the sequences,
+// and the sequence that holds a unit of it. Up to 64 sequences every wave keeps
+// one a lane and finds them by a scan and a ballot, with no shared memory and no
+// barrier (a call of few sequences is bound by such latencies); more go through
+// prefix sums in shared memory (prefix[seqs + 1], whose barriers every thread of
+// the workgroup reaches: threads a multiple of 64, at most 1024).
+template <typename Cost> struct seq_index {
+    const kv_batch & a;
+    const int page_shift;
+    int32_t * const prefix;
+    kv_seq mine;
+    int32_t incl, total;
 
-// The sequence whose run of the prefix sums holds u (u < prefix[seqs]).
-__device__ inline int seq_of(const int32_t * prefix, int seqs, int32_t u) {
-    int lo = 0, hi = seqs;  // prefix[lo] <= u < prefix[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (prefix[mid] <= u) lo = mid;
-        else hi = mid;
+    __device__ seq_index(const kv_batch & a, int page_shift, int32_t * prefix, Cost cost) : a(a), page_shift(page_shift), prefix(prefix) {
+        const int lane = threadIdx.x & 63;
+        bool bad = false;
+        if (a.seqs <= 64) {
+            mine = kv_seq{0, 0, 0, 0};
+            if (lane < a.seqs) mine = load_seq(a, lane, page_shift, bad);
+            incl = scan(lane < a.seqs ? cost(mine) : 0);
+            total = __builtin_amdgcn_readlane(incl, 63);
+        } else {
+            __shared__ int32_t wave_sum[16];
+            const int t = threadIdx.x, threads = blockDim.x;
+            const int run = (a.seqs + threads - 1) / threads, first = min(t * run, a.seqs), last = min(first + run, a.seqs);
+            int32_t sum = 0;
+            for (int b = first; b < last; b++) {
+                const int32_t c = cost(load_seq(a, b, page_shift, bad));
+                prefix[b + 1] = c;
+                sum += c;
+            }
+            const int32_t s = scan(sum);
+            if (lane == 63) wave_sum[t >> 6] = s;
+            __syncthreads();
+            int32_t before = s - sum;
+            for (int w = 0; w < (t >> 6); w++) before += wave_sum[w];
+            if (t == 0) prefix[0] = 0;
+            for (int b = first; b < last; b++) prefix[b + 1] = before += prefix[b + 1];
+            __syncthreads();
+            total = prefix[a.seqs];
+        }
+        if (bad && blockIdx.x == 0) report(a.bad);
     }
-    return lo;
-}
+
+    static __device__ int32_t scan(int32_t v) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int32_t u = __shfl_up(v, off);
+            if (lane >= off) v += u;
+        }
+        return v;
+    }
+
+    // The sequence that holds unit u < total (u and the answer the same in every
+    // lane), and the units before it.
+    __device__ kv_seq at(int32_t u, int32_t & before) const {
+        if (a.seqs <= 64) {
+            const int b = __popcll(__ballot(incl <= u));
+            before = b ? __builtin_amdgcn_readlane(incl, max(b - 1, 0)) : 0;
+            return kv_seq{__builtin_amdgcn_readlane(mine.row0, b), __builtin_amdgcn_readlane(mine.n, b),
+                          __builtin_amdgcn_readlane(mine.len, b), __builtin_amdgcn_readlane(mine.slot, b)};
+        }
+        int lo = 0, hi = a.seqs;  // prefix[lo] <= u < prefix[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (prefix[mid] <= u) lo = mid;
+            else hi = mid;
+        }
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        before = __builtin_amdgcn_readfirstlane(prefix[lo]);
+        bool bad = false;
+        return load_seq(a, lo, page_shift, bad);
+    }
+};
+
+// Bytes of shared memory for seq_index's prefix sums.
+inline size_t seq_index_bytes(int seqs) { return seqs <= 64 ? 0 : (size_t) ((seqs + 4) & ~3) * 4; }
 
 inline int kv_page_shift(int page_tokens) { return page_tokens > 0 ? __builtin_ctz((unsigned) page_tokens) : 0; }
 
