@@ -13,6 +13,7 @@
 // over tokens in the order 4h..4h+3, 8+4h..8+4h+3 of each 16, which is the order
 // the cache stores V in.
 #include <algorithm>
+#include <atomic>
 
 #include "kv_device.h"
 #include "zest_common.h"
@@ -157,13 +158,31 @@ template <int TYPE> __device__ inline bool nonfinite(typename elem<TYPE>::frag f
     return (carry & 0x80008000u) != 0;
 }
 
-// A fragment with only its value e, in the lanes that keep it (zeros else).
-template <int TYPE> __device__ inline typename elem<TYPE>::frag only(typename elem<TYPE>::frag f, bool keep, int e) {
-    struct words { uint32_t w[4]; };
-    words v = __builtin_bit_cast(words, f);
+// A weight of 0 does not silence a NaN or an infinity of V, so where a column may
+// not see a token that holds one, V is split: `clean` has zeros for them and goes
+// the usual way, `marks` has powers of 64 by their kind (1: +inf, 64: -inf, 4096:
+// NaN; 0 for finite values), whose product with the columns' ones and zeros of
+// the tokens they see counts each kind exactly (at most 32 of each).
+template <int TYPE>
+__device__ inline void split_nonfinite(typename elem<TYPE>::frag f, typename elem<TYPE>::frag & clean, typename elem<TYPE>::frag & marks) {
+    typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+    u16x8 v = __builtin_bit_cast(u16x8, f);
+    constexpr unsigned short EXP = elem<TYPE>::EXP & 0xffffu;
 #pragma unroll
-    for (int i = 0; i < 4; i++) v.w[i] &= keep && i == e >> 1 ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
-    return __builtin_bit_cast(typename elem<TYPE>::frag, v);
+    for (int i = 0; i < 8; i++) {
+        const unsigned short w = v[i];
+        const bool odd = (w & EXP) == EXP;
+        marks[i] = elem<TYPE>::from(!odd ? 0.0f : (w & 0x7fff) != EXP ? 4096.0f : w >> 15 ? 64.0f : 1.0f);
+        v[i] = odd ? 0 : w;
+    }
+    clean = __builtin_bit_cast(typename elem<TYPE>::frag, v);
+}
+
+// What such a count adds to a sum.
+__device__ inline float counted(float n) {
+    const int k = (int) n;
+    const float pos = k & 63 ? INFINITY : 0.0f, neg = k >> 6 & 63 ? -INFINITY : 0.0f;
+    return k >> 12 ? NAN : pos + neg;
 }
 
 // Four values of an output row.
@@ -184,6 +203,13 @@ __device__ inline void store4(const attn_args & a, int64_t at, const float v[4])
 __device__ inline float capped(const attn_args & a, float s) {
     const float cap = a.softcap * LOG2E;
     return cap - 2.0f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * (a.scale / a.softcap * (2.0f * LOG2E))) + 1.0f);
+}
+
+// A word that no wave changes while the kernel runs, at an address that is the
+// same in every lane: a scalar load, which does not wait behind the direct loads
+// in flight.
+__device__ inline int32_t load_uniform(const int32_t * p) {
+    return *(const __attribute__((address_space(4))) int32_t *) (uintptr_t) p;
 }
 
 // ---- few columns: decoding ----------------------------------------------------------
@@ -274,7 +300,7 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_
                 const int32_t t = t_first + j * UNIT + 16 * g;
                 id[g] = 0;
                 if (j < n && t < any_hi) {
-                    const int32_t x = row[t >> ps];
+                    const int32_t x = load_uniform(row + (t >> ps));
                     if ((uint32_t) x < (uint32_t) a.c.pages) {
                         id[g] = x;
                         there |= 1u << g;
@@ -340,7 +366,7 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_
         }
         for (int32_t j = 0; j < n; j++) {
             const int32_t t0 = t_first + j * UNIT;
-            const uint8_t * slot = mine + (j % R) * STEP_BYTES<D>;
+            uint8_t * const slot = mine + (j % R) * STEP_BYTES<D>;
             const bool more = j + R < n;
             there[R] = pages_of(j + R, id[R]);
             const bool masked = t0 < all_lo || t0 + GROUP > all_hi || there[0] != 3;
@@ -414,37 +440,42 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_
 
             if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((2 * R - 1) * LOADS) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            const uint8_t * vp = slot + GROUP * D * 2 + (lg * D + col) * 16;
+            uint8_t * vp = slot + GROUP * D * 2 + (lg * D + col) * 16;
             bool odd = false;
             if (masked) {
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) odd |= nonfinite<TYPE>(*reinterpret_cast<const frag *>(vp + dt * 256));
             }
             if (masked && __any(odd)) {
-                // A weight of 0 does not silence a NaN or an infinity: the tokens
-                // one at a time, each added where its column sees it
-                for (int tt = 0; tt < GROUP; tt++) {
-                    const int e = (tt & 3) + (tt >> 3 & 1) * 4, g = (tt >> 2 & 1) + 2 * (tt >> 4);  // its value of its lane group
-                    const bool page = there[0] >> (tt >> 4) & 1;
+                frag seen[NT];
 #pragma unroll
-                    for (int dt = 0; dt < DT; dt++) {
-                        const frag v = only<TYPE>(*reinterpret_cast<const frag *>(vp + dt * 256), lg == g, e);
+                for (int q = 0; q < NT; q++)
 #pragma unroll
-                        for (int q = 0; q < NT; q++) {
-                            const bool in = page && t0 + tt >= see_lo[q] && t0 + tt < see_hi[q];
-                            const f32x4 one = elem<TYPE>::mfma16(v, pf[q], f32x4{});
-#pragma unroll
-                            for (int i = 0; i < 4; i++) o[dt][q][i] = in ? o[dt][q][i] + one[i] : o[dt][q][i];
-                        }
+                    for (int e = 0; e < 8; e++) {
+                        const int32_t t = t0 + 4 * (lg & 1) + 16 * (lg >> 1) + (e & 3) + 8 * (e >> 2);
+                        const bool in = (there[0] >> (lg >> 1) & 1) && t >= see_lo[q] && t < see_hi[q];
+                        seen[q][e] = elem<TYPE>::from(in ? 1.0f : 0.0f);
                     }
-                }
-            } else {
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) {
-                    const frag v = *reinterpret_cast<const frag *>(vp + dt * 256);
+                    frag clean, marks;
+                    split_nonfinite<TYPE>(*reinterpret_cast<const frag *>(vp + dt * 256), clean, marks);
+                    *reinterpret_cast<frag *>(vp + dt * 256) = clean;  // the ring is this wave's own
 #pragma unroll
-                    for (int q = 0; q < NT; q++) o[dt][q] = elem<TYPE>::mfma16(v, pf[q], o[dt][q]);
+                    for (int q = 0; q < NT; q++) {
+                        const f32x4 n = elem<TYPE>::mfma16(marks, seen[q], f32x4{});
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[dt][q][i] += counted(n[i]);
+                    }
+                    asm volatile("" ::: "memory");
+                    __builtin_amdgcn_sched_barrier(0);  // one block's registers serve the next
                 }
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                const frag v = *reinterpret_cast<const frag *>(vp + dt * 256);
+#pragma unroll
+                for (int q = 0; q < NT; q++) o[dt][q] = elem<TYPE>::mfma16(v, pf[q], o[dt][q]);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (more) load_v(j + R, id[R]);
@@ -704,32 +735,41 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
                 for (int q = 0; q < NQ; q++) o[dt][q] = elem<TYPE>::mfma(v, p[q][g], o[dt][q]);
             }
     };
-    // The same where a column does not see every token: a weight of 0 does not
-    // silence a NaN or an infinity, so 16 tokens that hold one are taken one at
-    // a time, each added where its column sees it.
+    // The same where a column does not see every token.
     auto weigh_masked = [&](int j, uint32_t gone) {
-        const int32_t t0 = t_first + j * GROUP;
-        for (int g = 0; g < 2; g++) {
-            bool odd = false;
+        bool odd = false;
+#pragma unroll
+        for (int g = 0; g < 2; g++)
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) odd |= nonfinite<TYPE>(v_frag(j, dt, g));
-            const bool careful = __any(odd);
-            for (int tt = 0; tt < (careful ? 16 : 1); tt++) {
-                const int e = (tt & 3) + (tt >> 3) * 4, hh = (tt >> 2) & 1;
-                const int32_t t = t0 + 16 * g + tt;
-                bool in[NQ];
+        if (!__any(odd)) {
+            weigh(j);
+            return;
+        }
 #pragma unroll
-                for (int q = 0; q < NQ; q++) in[q] = !careful || (t >= see_lo[q] && t < see_hi[q] && !(gone >> (16 * g) & 1));
+        for (int g = 0; g < 2; g++) {
+            frag seen[NQ];
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    const frag v = careful ? only<TYPE>(v_frag(j, dt, g), half == hh, e) : v_frag(j, dt, g);
+            for (int q = 0; q < NQ; q++)
 #pragma unroll
-                    for (int q = 0; q < NQ; q++) {
-                        const f32x16 one = elem<TYPE>::mfma(v, g ? p[q][1] : p[q][0], f32x16{});
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[dt][q][i] = in[q] ? o[dt][q][i] + one[i] : o[dt][q][i];
-                    }
+                for (int e = 0; e < 8; e++) {
+                    const int32_t t = t_first + j * GROUP + 16 * g + 4 * half + (e & 3) + 8 * (e >> 2);
+                    const bool in = t >= see_lo[q] && t < see_hi[q] && !(gone >> (16 * g) & 1);
+                    seen[q][e] = elem<TYPE>::from(in ? 1.0f : 0.0f);
                 }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                frag clean, marks;
+                split_nonfinite<TYPE>(v_frag(j, dt, g), clean, marks);
+#pragma unroll
+                for (int q = 0; q < NQ; q++) {
+                    const f32x16 n = elem<TYPE>::mfma(marks, seen[q], f32x16{});
+                    o[dt][q] = elem<TYPE>::mfma(clean, p[q][g], o[dt][q]);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[dt][q][i] += counted(n[i]);
+                }
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);  // one block's registers serve the next
             }
         }
     };
@@ -971,16 +1011,22 @@ attn_plan plan_of(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
     return p;
 }
 
-template <typename K> int allow_lds(K kernel, size_t bytes) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
-    return e == hipSuccess ? ZEST_OK : zest::fail(ZEST_E_HIP, "zest_kv_attn: shared memory of %zu bytes: %s", bytes, hipGetErrorString(e));
+// Lets a kernel have its ring and the largest prefix sums in shared memory, once
+// (threads that launch it for the first time at once set the same value).
+template <auto KERNEL> int allow_lds(size_t ring) {
+    static std::atomic<bool> set{false};
+    if (set.load(std::memory_order_acquire)) return ZEST_OK;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int) (ring + zest::seq_index_bytes(zest::KV_MAX_SEQS)));
+    if (e != hipSuccess) return zest::fail(ZEST_E_HIP, "zest_kv_attn: shared memory attribute: %s", hipGetErrorString(e));
+    set.store(true, std::memory_order_release);
+    return ZEST_OK;
 }
 
 template <int TYPE, int D, int NT> int launch_few(const attn_args & a, const attn_plan & p, hipStream_t s) {
-    const size_t ring = WAVES * RING_B<D> * STEP_BYTES<D> + zest::seq_index_bytes(a.b.seqs);
-    if (ring + 1024 > 65536)
-        if (const int st = allow_lds(&attn_kernel<TYPE, D, NT>, ring)) return st;
-    hipLaunchKernelGGL((attn_kernel<TYPE, D, NT>), dim3(p.workgroups), dim3(WAVES * 64), ring, s, a);
+    constexpr size_t ring = WAVES * RING_B<D> * STEP_BYTES<D>;
+    if (const int st = allow_lds<&attn_kernel<TYPE, D, NT>>(ring)) return st;
+    hipLaunchKernelGGL((attn_kernel<TYPE, D, NT>), dim3(p.workgroups), dim3(WAVES * 64), ring + zest::seq_index_bytes(a.b.seqs), s, a);
     if (p.run > 1)  // else every piece is a whole run
         hipLaunchKernelGGL((combine_kernel<D, NT>), dim3(p.workgroups), dim3(256), zest::seq_index_bytes(a.b.seqs), s, a);
     return ZEST_OK;
@@ -988,11 +1034,10 @@ template <int TYPE, int D, int NT> int launch_few(const attn_args & a, const att
 
 template <int TYPE, int D> int launch(const attn_args & a, const attn_plan & p, hipStream_t s) {
     if (p.chunk_tiles) {
-        const size_t ring = RING * STEP_BYTES<D> + zest::seq_index_bytes(a.b.seqs);
-        if (ring + 1024 > 65536)
-            if (const int st = allow_lds(&chunk_kernel<TYPE, D>, ring)) return st;
-        hipLaunchKernelGGL((chunk_kernel<TYPE, D>), dim3((unsigned) (p.chunk_tiles * a.c.kv_heads), p.chunk_splits), dim3(WAVES * 64), ring,
-                           s, a);
+        constexpr size_t ring = RING * STEP_BYTES<D>;
+        if (const int st = allow_lds<&chunk_kernel<TYPE, D>>(ring)) return st;
+        hipLaunchKernelGGL((chunk_kernel<TYPE, D>), dim3((unsigned) (p.chunk_tiles * a.c.kv_heads), p.chunk_splits), dim3(WAVES * 64),
+                           ring + zest::seq_index_bytes(a.b.seqs), s, a);
     }
     if (p.workgroups)
         if (const int st = p.cols == 16 ? launch_few<TYPE, D, 1>(a, p, s) : launch_few<TYPE, D, 2>(a, p, s)) return st;

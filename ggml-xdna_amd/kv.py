@@ -43,28 +43,33 @@ def _need(ok: bool, what: str) -> None:
 
 
 def _list(t, what: str, device, dim: int = 1):
-    _need(t.dtype == torch.int32 and t.dim() == dim and t.is_contiguous() and t.device == device,
-          f"{what}: a contiguous int32 tensor of {dim} dimension(s) on {device} wanted")
+    if t.dtype != torch.int32 or t.dim() != dim or not t.is_contiguous() or t.device != device:
+        raise z.ZestError(f"{what}: a contiguous int32 tensor of {dim} dimension(s) on {device} wanted")
     return t
 
 
 def _here(device) -> None:
-    _need(device.type == "cuda" and device.index == torch.cuda.current_device(),
-          f"the cache is on {device}, which is not the current device")
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise z.ZestError(f"the cache is on {device}, which is not the current device")
 
 
 def _rows(t, what: str, rows: int, heads: int | None, dim: int, device):
     """A tensor [rows][heads][dim] or [rows][heads * dim], rows any stride apart; returns (type, pointer, stride, heads)."""
-    _need(t.dim() in (2, 3) and t.shape[0] == rows and t.dtype in _TYPES and t.device == device,
-          f"{what}: float32, float16 or bfloat16 rows, {rows} of them, on {device} wanted")
-    if t.dim() == 3:
-        ok = t.shape[2] == dim and t.stride(2) == 1 and (t.stride(1) == dim or t.shape[1] == 1)
-        have = t.shape[1]
+    # (the messages are made only when needed: these checks are a good part of a small call's time)
+    shape, kind = t.shape, _TYPES.get(t.dtype)
+    if kind is None or len(shape) not in (2, 3) or shape[0] != rows or t.device != device:
+        raise z.ZestError(f"{what}: float32, float16 or bfloat16 rows, {rows} of them, on {device} wanted")
+    stride = t.stride()
+    if len(shape) == 3:
+        have = shape[1]
+        ok = shape[2] == dim and stride[2] == 1 and (stride[1] == dim or have == 1)
     else:
-        ok, have = t.shape[1] % dim == 0 and t.stride(1) == 1, t.shape[1] // dim
-    _need(ok and have > 0 and heads in (None, have), f"{what}: rows of {heads or 'whole'} heads of {dim} contiguous values wanted")
+        have = shape[1] // dim
+        ok = shape[1] % dim == 0 and stride[1] == 1
+    if not ok or have <= 0 or (heads is not None and heads != have):
+        raise z.ZestError(f"{what}: rows of {heads or 'whole'} heads of {dim} contiguous values wanted")
     # a single row's stride is not used
-    return _TYPES[t.dtype], t.data_ptr(), t.stride(0) if rows > 1 else have * dim, have
+    return kind, t.data_ptr(), stride[0] if rows > 1 else have * dim, have
 
 
 class Cache:
@@ -77,7 +82,7 @@ class Cache:
         _need(pool.dim() == 4 and pool.dtype in (torch.float16, torch.bfloat16) and pool.is_contiguous() and
               pool.shape[3] == 2 * page_tokens * head_dim and pool.numel() > 0,
               "pool: a contiguous [layers][pages][kv_heads][2 * page_tokens * head_dim] of float16 or bfloat16 wanted")
-        self.pool, self.tables = pool, _list(tables, "tables", dev, 2)
+        self.pool, self.tables, self.device = pool, _list(tables, "tables", dev, 2), dev
         self.lens, self.refs = _list(lens, "lens", dev), _list(refs, "refs", dev)
         self.layers, self.pages, self.kv_heads = pool.shape[:3]
         _need(lens.numel() == tables.shape[0] and refs.numel() == self.pages, "lens: one a slot, refs: one a page, wanted")
@@ -89,7 +94,8 @@ class Cache:
         self._scratch = torch.empty(z.lib().zest_kv_scratch_bytes(self.pages, tables.shape[0]), dtype=torch.uint8, device=dev)
 
     def _batch(self, b: "Batch") -> _Batch:
-        _need(b.starts.device == self.pool.device, "the batch and the cache are on different devices")
+        if b.starts.device != self.device:
+            raise z.ZestError("the batch and the cache are on different devices")
         return _Batch(self.tables.data_ptr(), self.lens.data_ptr(), b.starts.data_ptr(),
                       None if b.slots is None else b.slots.data_ptr(), b.rows, b.seqs, self.tables.shape[0],
                       self.tables.shape[1], b.max_new, b.max_len)
@@ -141,34 +147,39 @@ def rope_freqs(n_dims: int, freq_base: float, freq_scale: float = 1.0, ext_facto
 
 
 def _bad(bad, device):
-    _need(bad is None or (bad.dtype in (torch.int32, torch.uint32) and bad.device == device and bad.numel() > 0),
+    if bad is None:
+        return None
+    _need(bad.dtype in (torch.int32, torch.uint32) and bad.device == device and bad.numel() > 0,
           f"bad: an int32 tensor on {device} wanted")
-    return z._ptr(bad)
+    return bad.data_ptr()
 
 
 def append(cache: Cache, layer: int, batch: Batch, k, v, q=None, rope: Rope | None = None, pos=None, q_out=None, q_dtype=None,
            bad=None):
     """zest_kv_append: the batch's new k (turned by rope) and v into layer's pages. With q, its turned rows are returned
     (of q_dtype, the cache's type unless given; or in q_out)."""
-    dev = cache.pool.device
+    dev = cache.device
     _here(dev)
-    _need(0 <= layer < cache.layers, f"layer {layer} of {cache.layers}")
+    if not 0 <= layer < cache.layers:
+        raise z.ZestError(f"layer {layer} of {cache.layers}")
     d = cache.head_dim
     tk, pk, ldk, _ = _rows(k, "k", batch.rows, cache.kv_heads, d, dev)
     tv, pv, ldv, _ = _rows(v, "v", batch.rows, cache.kv_heads, d, dev)
-    _need(tk == tv, "k and v of one type wanted")
+    if tk != tv:
+        raise z.ZestError("k and v of one type wanted")
     qa, oa, heads = (None, 0), (0, None, 0), 0
     if q is not None:
         tq, pq, ldq, heads = _rows(q, "q", batch.rows, None, d, dev)
-        _need(tq == tk, "q, k and v of one type wanted")
+        if tq != tk:
+            raise z.ZestError("q, k and v of one type wanted")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q_dtype or cache.pool.dtype, device=dev)
+            q_out = torch.empty_like(q, dtype=q_dtype or cache.pool.dtype, memory_format=torch.contiguous_format)
         to, po, ldo, _ = _rows(q_out, "q_out", batch.rows, heads, d, dev)
         qa, oa = (pq, ldq), (to, po, ldo)
     if pos is not None:
         _need(_list(pos, "pos", dev).numel() == batch.rows, "pos: one a row wanted")
-    if rope is not None:
-        _need(rope.freqs.device == dev, "the rope and the cache are on different devices")
+    if rope is not None and rope.freqs.device != dev:
+        raise z.ZestError("the rope and the cache are on different devices")
     z.check(z.lib().zest_kv_append(ctypes.byref(cache._layer[layer]), ctypes.byref(cache._batch(batch)),
                                    ctypes.byref(rope._c) if rope is not None else None, z._ptr(pos), tk, pk, ldk, pv, ldv, *qa,
                                    heads, oa[1], oa[2], oa[0], _bad(bad, dev), z._stream()), "zest_kv_append")
@@ -184,19 +195,22 @@ def attention(cache: Cache, layer: int, batch: Batch, q, scale: float | None = N
               softcap: float = 0.0, out=None, out_dtype=None, workspace=None, bad=None):
     """zest_kv_attn: attention of the batch's new tokens over layer's pages; returns out (of q's type and shape unless
     given). scale: 1 / sqrt(head_dim) unless given."""
-    dev = cache.pool.device
+    dev = cache.device
     _here(dev)
-    _need(0 <= layer < cache.layers, f"layer {layer} of {cache.layers}")
+    if not 0 <= layer < cache.layers:
+        raise z.ZestError(f"layer {layer} of {cache.layers}")
     d = cache.head_dim
     tq, pq, ldq, heads = _rows(q, "q", batch.rows, None, d, dev)
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=dev)
+        out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
     to, po, ldo, _ = _rows(out, "out", batch.rows, heads, d, dev)
+    lib = z.lib()
     c, b = ctypes.byref(cache._layer[layer]), ctypes.byref(cache._batch(batch))
     if workspace is None:
-        workspace = torch.empty(z.lib().zest_kv_attn_workspace(c, b, heads), dtype=torch.uint8, device=dev)
-    _need(workspace.device == dev and workspace.is_contiguous(), f"workspace: a contiguous tensor on {dev} wanted")
-    z.check(z.lib().zest_kv_attn(c, b, pq, tq, ldq, heads, 1.0 / math.sqrt(d) if scale is None else scale, int(causal), window,
+        workspace = torch.empty(lib.zest_kv_attn_workspace(c, b, heads), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise z.ZestError(f"workspace: a contiguous tensor on {dev} wanted")
+    z.check(lib.zest_kv_attn(c, b, pq, tq, ldq, heads, 1.0 / math.sqrt(d) if scale is None else scale, int(causal), window,
                                  softcap, po, to, ldo, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
                                  _bad(bad, dev), z._stream()), "zest_kv_attn")
     return out
@@ -205,11 +219,12 @@ def attention(cache: Cache, layer: int, batch: Batch, q, scale: float | None = N
 def assign(cache: Cache, dst, src, grow, bad=None) -> None:
     """zest_kv_assign: slot dst[i] becomes what src[i] was (-1: empty), grown by grow[i] tokens; int32 device tensors, at
     most one entry a slot."""
-    dev = cache.pool.device
+    dev = cache.device
     _here(dev)
     n = _list(dst, "dst", dev).numel()
     _need(_list(src, "src", dev).numel() == n and _list(grow, "grow", dev).numel() == n, "dst, src and grow of one length wanted")
-    _need(n <= cache.tables.shape[0], f"{n} entries for {cache.tables.shape[0]} slots")
+    if n > cache.tables.shape[0]:
+        raise z.ZestError(f"{n} entries for {cache.tables.shape[0]} slots")
     z.check(z.lib().zest_kv_assign(ctypes.byref(cache._layer[0]), cache.layers, cache.layer_stride, cache.refs.data_ptr(),
                                    cache.tables.data_ptr(), cache.lens.data_ptr(), cache.tables.shape[0], cache.tables.shape[1],
                                    dst.data_ptr(), src.data_ptr(), grow.data_ptr(), n, cache._scratch.data_ptr(),
@@ -219,7 +234,7 @@ def assign(cache: Cache, dst, src, grow, bad=None) -> None:
 def compact(cache: Cache, refs=None, tables=None, live=None, bad=None):
     """zest_kv_compact: the live pages moved to the front of the pool; returns their number (int32 [1], device). refs and
     tables: buffers for the new ones, the cache's own (in place) unless given."""
-    dev = cache.pool.device
+    dev = cache.device
     _here(dev)
     refs, tables = cache.refs if refs is None else refs, cache.tables if tables is None else tables
     _need(_list(refs, "refs", dev).numel() == cache.pages and _list(tables, "tables", dev, 2).shape == cache.tables.shape,
