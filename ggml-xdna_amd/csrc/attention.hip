@@ -594,7 +594,10 @@ __global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
 // them (O^T of 64 columns is D values a lane, Q^T half of that).
 template <int D> constexpr int QT = 1;
 template <int D> constexpr int CHUNK = WAVES * 32 * QT<D>;  // columns of a workgroup
-constexpr int RING = 4;                                     // steps of K and V in shared memory
+// Steps of K and of V in shared memory. At step j the scores read K of j + 1 while
+// those of j + 2 and j + 3 are on their way, the weights read V of j - 1.
+constexpr int K_RING = 3, V_RING = 5;
+template <int D> constexpr int CHUNK_RING = (K_RING + V_RING) * (STEP_BYTES<D> / 2);
 // How far, in powers of two, a score may pass the maximum its column's weights
 // are relative to before O^T is rescaled: the sums are in fp32, so only the
 // weights' own range matters (bf16: fp32's; fp16: SHIFT + 8 stays below 2^16)
@@ -611,18 +614,17 @@ __device__ inline int32_t chunk_tiles_of(const attn_args & a, const kv_seq & s, 
 // any of the tile's columns sees, 32 tokens a step. K and V of a step go from
 // the pool straight into shared memory (16 bytes a lane, in the pool's order,
 // which is the order they are read in: every read is 512 contiguous bytes a half
-// wave), a ring of four steps with one barrier a step. A step runs three stages
+// wave), two steps ahead of their use, with one barrier a step. A step runs three stages
 // at once, so the matrix cores and the vector units both have work: the scores
 // of step j + 1, the softmax of step j and the weights of step j - 1 times V.
 template <int TYPE, int D>
 __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn_args a) {
     typedef typename elem<TYPE>::frag frag;
     constexpr int NQ = QT<D>, KS = D / 16, DT = D / 32;
-    extern __shared__ __align__(1024) uint8_t ring[];  // [RING][K: D/8][32][8], V: [2][2][D][8]; then the prefix sums
-    __shared__ uint32_t missing[RING];                 // bit g: tokens 16g .. of the step have no page
+    extern __shared__ __align__(1024) uint8_t ring[];  // [K_RING][D/8][32][8], [V_RING][2][2][D][8]; then the prefix sums
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     const int ps = a.c.page_shift, P = 1 << ps;
-    const zest::seq_index index(a.b, ps, reinterpret_cast<int32_t *>(ring + RING * STEP_BYTES<D>),
+    const zest::seq_index index(a.b, ps, reinterpret_cast<int32_t *>(ring + CHUNK_RING<D>),
                                 [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
     // the last tiles first: under a causal mask they see the most
     const int h = blockIdx.x % a.c.kv_heads;
@@ -661,48 +663,58 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
         seen_by(a, s, last / a.group, last / a.group, all_lo, unused);
     }
 
+    // The pages of 64 table columns, one a lane, so that a step's page is a lane
+    // exchange: a load of it in the loop would wait behind the steps in flight.
+    int32_t window = 0, at_col = 0;
+    auto look_up = [&](int col0) {
+        at_col = col0;
+        window = ((int64_t) (col0 + lane) << ps) < t_hi ? row[col0 + lane] : -1;
+    };
+    look_up(t_first >> ps);
     // A step's loads: waves 0 and 1 a half of K's rows each, waves 2 and 3 the V
-    // of 16 tokens each. A lane looks its page up one step before it loads.
+    // of 16 tokens each. Returns which 16 tokens (bits) have no page.
     const bool k_wave = wave < 2;
     const int32_t head_at = h * (4 * P * D);
-    const uint32_t ring_at = (uint32_t) (uintptr_t) (lds_ptr_t) ring;
-    auto page_of = [&](int j) {  // the table's entry for this lane's token of step j; -1 behind the last token
-        const int32_t t = t_first + j * GROUP + (k_wave ? col : 16 * (wave - 2));
-        return j < n && t < t_hi ? row[t >> ps] : -1;
-    };
-    auto load_step = [&](int j, int32_t id) {
-        if (j >= n) return;
-        const int32_t t0 = t_first + j * GROUP, t = t0 + (k_wave ? col : 16 * (wave - 2));
-        const bool there = (uint32_t) id < (uint32_t) a.c.pages;
-        if (!k_wave && lane == 0) {
-            const bool gone = !there && t < t_hi;
-            bad |= gone;
-            reinterpret_cast<uint16_t *>(&missing[j % RING])[wave - 2] = gone;
+    const uint32_t ring_at = (uint32_t) (uintptr_t) (lds_ptr_t) ring, v_ring_at = ring_at + K_RING * (STEP_BYTES<D> / 2);
+    auto load_step = [&](int j, int k_slot, int v_slot) -> uint32_t {
+        if (j >= n) return 0;
+        const int32_t t0 = t_first + j * GROUP;
+        if (((t0 + 16) >> ps) - at_col >= 64) look_up(t0 >> ps);
+        int32_t id[2];
+        uint32_t gone = 0;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            id[g] = __builtin_amdgcn_readlane(window, ((t0 + 16 * g) >> ps) - at_col);
+            if ((uint32_t) id[g] >= (uint32_t) a.c.pages) {
+                bad |= t0 + 16 * g < t_hi;
+                id[g] = 0;
+                gone |= 1u << g;
+            }
         }
-        const uint8_t * from = a.c.pool + (there ? id : 0) * a.c.page_bytes + head_at;
-        const uint32_t in = t & (P - 1);
-        const uint32_t to = ring_at + (j % RING) * STEP_BYTES<D>;
         if (k_wave) {
-            from += in * 16 + (wave * (D / 16) + half) * (P * 16);
+            const uint32_t in0 = t0 & (P - 1), in1 = (t0 + 16) & (P - 1);
+            const int64_t off0 = id[0] * a.c.page_bytes + in0 * 16, off1 = id[1] * a.c.page_bytes + in1 * 16;
+            const uint8_t * from = a.c.pool + head_at + (lane & 16 ? off1 : off0) + (lane & 15) * 16 + (wave * (D / 16) + half) * (P * 16);
+            const uint32_t to = ring_at + k_slot * (STEP_BYTES<D> / 2) + wave * (D / 32) * 1024;
 #pragma unroll
             for (int i = 0; i < D / 32; i++)
-                __builtin_amdgcn_global_load_lds((global_ptr_t) (from + i * (P * 32)),
-                                                 (lds_ptr_t) (uintptr_t) (to + (wave * (D / 32) + i) * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_ptr_t) (from + i * (P * 32)), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
         } else {
-            from += 2 * P * D + in * (2 * D) + lane * 16;
+            const int g = wave - 2;
+            const uint32_t in = (t0 + 16 * g) & (P - 1);
+            const uint8_t * from = a.c.pool + head_at + (g ? id[1] : id[0]) * a.c.page_bytes + 2 * P * D + in * (2 * D) + lane * 16;
+            const uint32_t to = v_ring_at + v_slot * (STEP_BYTES<D> / 2) + g * (D / 32) * 1024;
 #pragma unroll
             for (int i = 0; i < D / 32; i++)
-                __builtin_amdgcn_global_load_lds((global_ptr_t) (from + i * 1024),
-                                                 (lds_ptr_t) (uintptr_t) (to + GROUP * D * 2 + ((wave - 2) * (D / 32) + i) * 1024),
-                                                 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_ptr_t) (from + i * 1024), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
         }
+        return gone;
     };
-    auto k_frag = [&](int j, int ks) {
-        return *reinterpret_cast<const frag *>(ring + (j % RING) * STEP_BYTES<D> + (2 * ks + half) * 512 + col * 16);
+    auto k_frag = [&](int slot, int ks) {
+        return *reinterpret_cast<const frag *>(ring + slot * (STEP_BYTES<D> / 2) + (2 * ks + half) * 512 + col * 16);
     };
-    auto v_frag = [&](int j, int dt, int g) {
-        return *reinterpret_cast<const frag *>(ring + (j % RING) * STEP_BYTES<D> + GROUP * D * 2 + (2 * g + half) * (16 * D) + dt * 512 +
-                                               col * 16);
+    auto v_frag = [&](int slot, int dt, int g) {
+        return *reinterpret_cast<const frag *>(ring + (K_RING + slot) * (STEP_BYTES<D> / 2) + (2 * g + half) * (16 * D) + dt * 512 + col * 16);
     };
 
     f32x16 o[DT][NQ], s_cur[NQ], s_next[NQ];
@@ -715,35 +727,35 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) o[dt][q] = f32x16{};
     }
-    auto scores = [&](int j, f32x16 to[NQ]) {
+    auto scores = [&](int slot, f32x16 to[NQ]) {
 #pragma unroll
         for (int q = 0; q < NQ; q++) to[q] = f32x16{};
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
-            const frag k = k_frag(j, ks);
+            const frag k = k_frag(slot, ks);
 #pragma unroll
             for (int q = 0; q < NQ; q++) to[q] = elem<TYPE>::mfma(k, qf[q][ks], to[q]);
         }
     };
-    auto weigh = [&](int j) {
+    auto weigh = [&](int slot) {
 #pragma unroll
         for (int g = 0; g < 2; g++)
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
-                const frag v = v_frag(j, dt, g);
+                const frag v = v_frag(slot, dt, g);
 #pragma unroll
                 for (int q = 0; q < NQ; q++) o[dt][q] = elem<TYPE>::mfma(v, p[q][g], o[dt][q]);
             }
     };
     // The same where a column does not see every token.
-    auto weigh_masked = [&](int j, uint32_t gone) {
+    auto weigh_masked = [&](int j, int slot, uint32_t gone) {
         bool odd = false;
 #pragma unroll
         for (int g = 0; g < 2; g++)
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) odd |= nonfinite<TYPE>(v_frag(j, dt, g));
+            for (int dt = 0; dt < DT; dt++) odd |= nonfinite<TYPE>(v_frag(slot, dt, g));
         if (!__any(odd)) {
-            weigh(j);
+            weigh(slot);
             return;
         }
 #pragma unroll
@@ -754,13 +766,13 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int32_t t = t_first + j * GROUP + 16 * g + 4 * half + (e & 3) + 8 * (e >> 2);
-                    const bool in = t >= see_lo[q] && t < see_hi[q] && !(gone >> (16 * g) & 1);
+                    const bool in = t >= see_lo[q] && t < see_hi[q] && !(gone >> g & 1);
                     seen[q][e] = elem<TYPE>::from(in ? 1.0f : 0.0f);
                 }
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
                 frag clean, marks;
-                split_nonfinite<TYPE>(v_frag(j, dt, g), clean, marks);
+                split_nonfinite<TYPE>(v_frag(slot, dt, g), clean, marks);
 #pragma unroll
                 for (int q = 0; q < NQ; q++) {
                     const f32x16 n = elem<TYPE>::mfma(marks, seen[q], f32x16{});
@@ -806,26 +818,27 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
         return any_rise;
     };
 
-    int32_t id = page_of(0);
-    load_step(0, id);
-    id = page_of(1);
-    load_step(1, id);
-    id = page_of(2);
+    // `gone` of the steps loaded, two bits each, the latest lowest
+    uint32_t gones = load_step(0, 0, 0);
+    gones = gones << 2 | load_step(1, 1, 1);
+    gones = gones << 2 | load_step(2, 2, 2);
+    int k_at = 0, v_at = 0;  // step j's places in the rings
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (n > 0) scores(0, s_cur);
     bool masked_before = false;
     uint32_t gone_before = 0, gone = 0;
-    // the barrier of step j: this wave's loads of step j + 1 are there and its
-    // reads of step j - 2 done; past it, every wave's. Whether step j is masked.
+    // The barrier of step j: this wave's loads of step j + 1 are there (those of
+    // j + 2 may not be) and its reads of step j - 1's scores and weights done;
+    // past it, every wave's. Whether step j is masked.
     auto enter = [&](int j) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (j + 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(D / 32) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        gone = __builtin_amdgcn_readfirstlane(missing[j % RING]);
-        load_step(j + 2, id);
-        id = page_of(j + 3);
+        gone = gones >> 4 & 3;
+        gones = gones << 2 | load_step(j + 3, k_at, v_at >= 2 ? v_at - 2 : v_at + 3);
         const int32_t t0 = t_first + j * GROUP;
         return t0 < all_lo || t0 + GROUP > all_hi || gone != 0;
     };
@@ -850,7 +863,11 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
             p[q][0] = pn[q][0];
             p[q][1] = pn[q][1];
         }
+        k_at = k_at == K_RING - 1 ? 0 : k_at + 1;
+        v_at = v_at == V_RING - 1 ? 0 : v_at + 1;
     };
+    auto k_next = [&]() { return k_at == K_RING - 1 ? 0 : k_at + 1; };
+    auto v_last = [&]() { return v_at == 0 ? V_RING - 1 : v_at - 1; };
     int32_t j = 0;
     bool masked = n > 0 ? enter(0) : false;
     while (j < n) {
@@ -863,17 +880,17 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int32_t t = t0 + (i & 3) + 8 * (i >> 2) + 4 * half;
-                    const bool in = t >= see_lo[q] && t < see_hi[q] && !(gone >> (16 * (i >> 3)) & 1);
+                    const bool in = t >= see_lo[q] && t < see_hi[q] && !(gone >> (i >> 3) & 1);
                     s_cur[q][i] = in ? s_cur[q][i] : -INFINITY;
                 }
         }
         {
             frag pn[NQ][2];
             if (j > 0) {
-                if (masked_before) weigh_masked(j - 1, gone_before);
-                else weigh(j - 1);
+                if (masked_before) weigh_masked(j - 1, v_last(), gone_before);
+                else weigh(v_last());
             }
-            scores(j + 1, s_next);
+            scores(k_next(), s_next);
             const bool rise = soften(pn);
             finish(rise, pn);
         }
@@ -884,16 +901,20 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
         while (j < n && !masked && !masked_before) {
             if (a.softcap > 0.0f) cap_scores();
             frag pn[NQ][2];
-            weigh(j - 1);
-            scores(j + 1, s_next);
+            weigh(v_last());
+            scores(k_next(), s_next);
             const bool rise = soften(pn);
+            // the weights are made here, beside the matrix instructions, not where
+            // the next step first needs them
+#pragma unroll
+            for (int q = 0; q < NQ; q++) asm volatile("" : "+v"(pn[q][0]), "+v"(pn[q][1]), "+v"(l[q]));
             finish(rise, pn);
             if (++j < n) masked = enter(j);
         }
     }
     if (n > 0) {
-        if (masked_before) weigh_masked(n - 1, gone_before);
-        else weigh(n - 1);
+        if (masked_before) weigh_masked(n - 1, v_last(), gone_before);
+        else weigh(v_last());
     }
     if (bad) zest::report(a.b.bad);
 
@@ -1034,7 +1055,7 @@ template <int TYPE, int D, int NT> int launch_few(const attn_args & a, const att
 
 template <int TYPE, int D> int launch(const attn_args & a, const attn_plan & p, hipStream_t s) {
     if (p.chunk_tiles) {
-        constexpr size_t ring = RING * STEP_BYTES<D>;
+        constexpr size_t ring = CHUNK_RING<D>;
         if (const int st = allow_lds<&chunk_kernel<TYPE, D>>(ring)) return st;
         hipLaunchKernelGGL((chunk_kernel<TYPE, D>), dim3((unsigned) (p.chunk_tiles * a.c.kv_heads), p.chunk_splits), dim3(WAVES * 64),
                            ring + zest::seq_index_bytes(a.b.seqs), s, a);
