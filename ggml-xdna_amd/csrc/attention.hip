@@ -626,10 +626,16 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
     const int ps = a.c.page_shift, P = 1 << ps;
     const zest::seq_index index(a.b, ps, reinterpret_cast<int32_t *>(ring + CHUNK_RING<D>),
                                 [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
-    // the last tiles first: under a causal mask they see the most
-    const int h = blockIdx.x % a.c.kv_heads;
-    const int tile = index.total - 1 - (int) (blockIdx.x / a.c.kv_heads);
+    // Under a causal mask the last tiles see the most. Where all fit the GPU at
+    // once, two a CU, a CU gets one from either end (workgroup i + CUS joins i);
+    // else the longest come first.
+    const int h = blockIdx.x % a.c.kv_heads, order = blockIdx.x / a.c.kv_heads;
+    int tile = index.total - 1 - order;
     if (tile < 0) return;
+    if (index.total * a.c.kv_heads <= 2 * CUS) {
+        const int head_start = CUS / a.c.kv_heads;
+        if (order >= head_start) tile = order - head_start;
+    }
     bool bad = false;
     int32_t before;
     const kv_seq s = index.at(tile, before);
@@ -665,48 +671,54 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
 
     // The pages of 64 table columns, one a lane, so that a step's page is a lane
     // exchange: a load of it in the loop would wait behind the steps in flight.
-    int32_t window = 0, at_col = 0;
+    // absent: the columns without a page (bits; theirs is page 0, read and unseen).
+    uint32_t window = 0;
+    uint64_t absent = 0;
+    int32_t at_col = 0;
     auto look_up = [&](int col0) {
         at_col = col0;
-        window = ((int64_t) (col0 + lane) << ps) < t_hi ? row[col0 + lane] : -1;
+        const bool wanted = ((int64_t) (col0 + lane) << ps) < t_hi;
+        window = wanted ? (uint32_t) row[col0 + lane] : 0xffffffffu;
+        const bool there = window < (uint32_t) a.c.pages;
+        absent = __ballot(!there);
+        bad |= wanted && !there;
+        window = there ? window : 0;
+        asm volatile("" : "+v"(window));  // waited for here, not at every use
     };
     look_up(t_first >> ps);
     // A step's loads: waves 0 and 1 a half of K's rows each, waves 2 and 3 the V
-    // of 16 tokens each. Returns which 16 tokens (bits) have no page.
+    // of 16 tokens each. Returns which 16 tokens (bits) have no page. Few
+    // instructions, as a wave makes them every step: a page's address is uniform,
+    // a lane's place in it one of the offsets made here.
     const bool k_wave = wave < 2;
-    const int32_t head_at = h * (4 * P * D);
+    const uint32_t page_bytes = (uint32_t) a.c.page_bytes;
     const uint32_t ring_at = (uint32_t) (uintptr_t) (lds_ptr_t) ring, v_ring_at = ring_at + K_RING * (STEP_BYTES<D> / 2);
+    const uint8_t * const part = a.c.pool + (int64_t) h * (4 * P * D) + (k_wave ? 0 : 2 * P * D);
+    uint32_t offset[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; i++)
+        offset[i] = k_wave ? col * 16 + (wave * (D / 16) + half + 2 * i) * (P * 16) : lane * 16 + i * 1024 + (wave - 2) * (32 * D);
     auto load_step = [&](int j, int k_slot, int v_slot) -> uint32_t {
         if (j >= n) return 0;
         const int32_t t0 = t_first + j * GROUP;
         if (((t0 + 16) >> ps) - at_col >= 64) look_up(t0 >> ps);
-        int32_t id[2];
-        uint32_t gone = 0;
-#pragma unroll
-        for (int g = 0; g < 2; g++) {
-            id[g] = __builtin_amdgcn_readlane(window, ((t0 + 16 * g) >> ps) - at_col);
-            if ((uint32_t) id[g] >= (uint32_t) a.c.pages) {
-                bad |= t0 + 16 * g < t_hi;
-                id[g] = 0;
-                gone |= 1u << g;
-            }
-        }
-        if (k_wave) {
-            const uint32_t in0 = t0 & (P - 1), in1 = (t0 + 16) & (P - 1);
-            const int64_t off0 = id[0] * a.c.page_bytes + in0 * 16, off1 = id[1] * a.c.page_bytes + in1 * 16;
-            const uint8_t * from = a.c.pool + head_at + (lane & 16 ? off1 : off0) + (lane & 15) * 16 + (wave * (D / 16) + half) * (P * 16);
-            const uint32_t to = ring_at + k_slot * (STEP_BYTES<D> / 2) + wave * (D / 32) * 1024;
+        const int c0 = (t0 >> ps) - at_col;
+        const uint32_t to = (k_wave ? ring_at + k_slot * (STEP_BYTES<D> / 2) + wave * (D / 32) * 1024
+                                    : v_ring_at + v_slot * (STEP_BYTES<D> / 2) + (wave - 2) * (D / 32) * 1024);
+        const uint8_t * from = part + (uint64_t) (uint32_t) __builtin_amdgcn_readlane(window, c0) * page_bytes;
+        uint32_t gone = absent >> c0 & 1 ? 3 : 0;
+        if (ps == 4) {  // two pages a step
+            const uint8_t * second = part + (uint64_t) (uint32_t) __builtin_amdgcn_readlane(window, c0 + 1) * page_bytes;
+            gone = (uint32_t) (absent >> c0) & 3;
+            const uint8_t * mine = k_wave ? (lane & 16 ? second - 256 : from) : wave == 3 ? second - 32 * D : from;
 #pragma unroll
             for (int i = 0; i < D / 32; i++)
-                __builtin_amdgcn_global_load_lds((global_ptr_t) (from + i * (P * 32)), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_ptr_t) (mine + offset[i]), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
         } else {
-            const int g = wave - 2;
-            const uint32_t in = (t0 + 16 * g) & (P - 1);
-            const uint8_t * from = a.c.pool + head_at + (g ? id[1] : id[0]) * a.c.page_bytes + 2 * P * D + in * (2 * D) + lane * 16;
-            const uint32_t to = v_ring_at + v_slot * (STEP_BYTES<D> / 2) + g * (D / 32) * 1024;
+            from += (t0 & (P - 1)) * (k_wave ? 16 : 2 * D);
 #pragma unroll
             for (int i = 0; i < D / 32; i++)
-                __builtin_amdgcn_global_load_lds((global_ptr_t) (from + i * 1024), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_ptr_t) (from + offset[i]), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
         }
         return gone;
     };
@@ -818,6 +830,8 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
         return any_rise;
     };
 
+    // the steps that all of the wave's columns see whole
+    const int whole_from = (max(all_lo - t_first, 0) + GROUP - 1) / GROUP, whole_to = (min(all_hi, t_hi) - t_first) / GROUP;
     // `gone` of the steps loaded, two bits each, the latest lowest
     uint32_t gones = load_step(0, 0, 0);
     gones = gones << 2 | load_step(1, 1, 1);
@@ -839,8 +853,7 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
         asm volatile("" ::: "memory");
         gone = gones >> 4 & 3;
         gones = gones << 2 | load_step(j + 3, k_at, v_at >= 2 ? v_at - 2 : v_at + 3);
-        const int32_t t0 = t_first + j * GROUP;
-        return t0 < all_lo || t0 + GROUP > all_hi || gone != 0;
+        return j < whole_from || j >= whole_to || gone != 0;
     };
     auto cap_scores = [&]() {
 #pragma unroll
@@ -901,8 +914,8 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
         while (j < n && !masked && !masked_before) {
             if (a.softcap > 0.0f) cap_scores();
             frag pn[NQ][2];
-            weigh(v_last());
             scores(k_next(), s_next);
+            weigh(v_last());
             const bool rise = soften(pn);
             // the weights are made here, beside the matrix instructions, not where
             // the next step first needs them
