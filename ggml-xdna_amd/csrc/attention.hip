@@ -34,7 +34,7 @@ constexpr int WAVES = 4;     // waves of a workgroup
 constexpr int GROUP = 32;    // tokens a wave takes at a time
 constexpr int UNIT = WAVES * GROUP;  // tokens of a unit of work
 constexpr int CUS = 256;
-constexpr int MOST_SPLIT_COLS = 64;  // columns of a sequence that attn_kernel takes
+constexpr int MOST_SPLIT_COLS = 64;  // columns of a sequence that attend_few takes
 
 // The cache's element type: its fragment, its MFMA and its exponent field.
 template <int TYPE> struct elem;
@@ -69,10 +69,10 @@ struct attn_args {
     int32_t q_type, out_type, group, causal, window;
     float scale, softcap;  // scale >= 0, softcap 0: none
     float sign;            // q is multiplied by it: -1 for a negative scale, 0 for a scale of 0 (scale is then 1)
-    int32_t chunk_cols;    // sequences of more columns than this are chunk_kernel's
+    int32_t chunk_cols;    // sequences of more columns than this are attend_chunk's
     float * partial;
     float * chunk_partial;
-    int32_t chunk_splits;
+    int32_t chunk_blocks, chunk_splits;
 };
 
 // Tokens [lo, hi) that any of a sequence's rows i0 .. i1 sees.
@@ -83,7 +83,7 @@ __device__ inline void seen_by(const attn_args & a, const kv_seq & s, int i0, in
     lo = min(lo, hi);
 }
 
-// Units of work of one column tile of attn_kernel: whole UNITs from the first
+// Units of work of one column tile of attend_few: whole UNITs from the first
 // token that any of the sequence's rows sees.
 __device__ inline int32_t units_of(const attn_args & a, const kv_seq & s) {
     int32_t lo, hi;
@@ -241,7 +241,7 @@ constexpr int partial_floats(int cols, int D) { return cols * (D + 2); }
 // piece of a share is one column tile's run of units; its four waves take 32
 // tokens of a unit each and are joined in shared memory. A piece that is the
 // tile's whole run goes to the output; else it is a partial result (slot 2w + 1
-// where it starts the run, 2w where it continues one), and combine_kernel joins a
+// where it starts the run, 2w where it continues one), and combine_few joins a
 // run's pieces in order.
 //
 // HBM bound: 4 D bytes of K and V a token for 4 D COLS operations. A wave keeps a
@@ -256,18 +256,18 @@ constexpr int partial_floats(int cols, int D) { return cols * (D + 2); }
 // {0..7, 16..23} and {8..15, 24..31}, so that a lane group's 8 weights, in the
 // registers they are in, are the 8 tokens of a V piece.
 template <int TYPE, int D, int NT>
-__global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_args a) {
+__device__ inline void attend_few(const attn_args & a, int block, int blocks, uint8_t * ring_sh) {
     typedef typename elem<TYPE>::frag frag;
     constexpr int COLS = 16 * NT, KS = D / 32, DT = D / 16, R = RING_B<D>, LOADS = D / 16;  // loads of K (or V) a step
-    extern __shared__ __align__(1024) uint8_t ring_sh[];  // a wave: [R][K: D/8][32][8], V: [4][D][8]; then the prefix sums
+    // ring_sh, a wave: [R][K: D/8][32][8], V: [4][D][8]; then the prefix sums
     __shared__ float stat[WAVES][2][COLS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = lane >> 4, col = lane & 15;
     const int ps = a.c.page_shift, P = 1 << ps;
     const zest::seq_index index(a.b, ps, reinterpret_cast<int32_t *>(ring_sh + WAVES * R * STEP_BYTES<D>),
                                 [&](const kv_seq & s) { return cost_of(a, s, COLS); });
-    const unit_shares shares(index.total, gridDim.x);
-    int32_t u = shares.start(blockIdx.x);
-    const int32_t u1 = shares.start(blockIdx.x + 1);
+    const unit_shares shares(index.total, blocks);
+    int32_t u = shares.start(block);
+    const int32_t u1 = shares.start(block + 1);
     uint8_t * const mine = ring_sh + wave * R * STEP_BYTES<D>;
     const uint32_t ring_at = (uint32_t) (uintptr_t) (lds_ptr_t) mine;
     bool bad = false;
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_
         }
         __syncthreads();
         const bool whole = units == run;
-        float * part = a.partial + (int64_t) (2 * blockIdx.x + (first == 0)) * partial_floats(COLS, D);
+        float * part = a.partial + (int64_t) (2 * block + (first == 0)) * partial_floats(COLS, D);
         for (int i = threadIdx.x; i < COLS * UNITS; i += WAVES * 64) {
             const int oc = i / UNITS, unit = i - oc * UNITS;
             int turned = unit + (oc & 15);
@@ -549,13 +549,11 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_
 
 // Joins the pieces of the column tile whose run starts in workgroup w's share
 // and goes on past it, if there is one: theirs are the last of the share.
-template <int D, int NT>
-__global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
-    extern __shared__ __align__(16) int32_t attn_sh[];
+template <int D, int NT> __device__ inline void combine_few(const attn_args & a, int block, int blocks, int32_t * attn_sh) {
     constexpr int COLS = 16 * NT, UNITS = D / 4;
     const zest::seq_index index(a.b, a.c.page_shift, attn_sh, [&](const kv_seq & s) { return cost_of(a, s, COLS); });
-    const unit_shares shares(index.total, gridDim.x);
-    const int32_t u0 = shares.start(blockIdx.x), u1 = shares.start(blockIdx.x + 1);
+    const unit_shares shares(index.total, blocks);
+    const int32_t u0 = shares.start(block), u1 = shares.start(block + 1);
     if (u0 == u1) return;
     int32_t before;
     const kv_seq s = index.at(u1 - 1, before);
@@ -567,11 +565,11 @@ __global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
     for (int i = threadIdx.x; i < COLS * UNITS; i += 256) {
         const int oc = i / UNITS, unit = i - oc * UNITS, cc = ct * COLS + oc;
         if (cc >= ncols) return;
-        const float * x = a.partial + (int64_t) (2 * blockIdx.x + 1) * partial_floats(COLS, D);
+        const float * x = a.partial + (int64_t) (2 * block + 1) * partial_floats(COLS, D);
         float m = x[COLS * D + oc], l = x[COLS * D + COLS + oc];
         float4 o = *reinterpret_cast<const float4 *>(x + oc * D + unit * 4);
 #pragma unroll 4
-        for (int w = blockIdx.x + 1; w <= last; w++) {
+        for (int w = block + 1; w <= last; w++) {
             const float * y = a.partial + (int64_t) (2 * w) * partial_floats(COLS, D);
             const float m1 = y[COLS * D + oc], l1 = y[COLS * D + COLS + oc], now = fmaxf(m, m1);
             const float4 v = *reinterpret_cast<const float4 *>(y + oc * D + unit * 4);
@@ -590,7 +588,7 @@ __global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
 
 // ---- chunks: many columns ---------------------------------------------------------
 
-// Column tiles of 32 a wave of chunk_kernel takes: two where the registers hold
+// Column tiles of 32 a wave of attend_chunk takes: two where the registers hold
 // them (O^T of 64 columns is D values a lane, Q^T half of that).
 template <int D> constexpr int QT = 1;
 template <int D> constexpr int CHUNK = WAVES * 32 * QT<D>;  // columns of a workgroup
@@ -617,11 +615,10 @@ __device__ inline int32_t chunk_tiles_of(const attn_args & a, const kv_seq & s, 
 // wave), two steps ahead of their use, with one barrier a step. A step runs three stages
 // at once, so the matrix cores and the vector units both have work: the scores
 // of step j + 1, the softmax of step j and the weights of step j - 1 times V.
-template <int TYPE, int D>
-__global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn_args a) {
+template <int TYPE, int D> __device__ inline void attend_chunk(const attn_args & a, int block, int split, uint8_t * ring) {
     typedef typename elem<TYPE>::frag frag;
     constexpr int NQ = QT<D>, KS = D / 16, DT = D / 32;
-    extern __shared__ __align__(1024) uint8_t ring[];  // [K_RING][D/8][32][8], [V_RING][2][2][D][8]; then the prefix sums
+    // ring: [K_RING][D/8][32][8], [V_RING][2][2][D][8]; then the prefix sums
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     const int ps = a.c.page_shift, P = 1 << ps;
     const zest::seq_index index(a.b, ps, reinterpret_cast<int32_t *>(ring + CHUNK_RING<D>),
@@ -629,7 +626,7 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
     // Under a causal mask the last tiles see the most. Where all fit the GPU at
     // once, two a CU, a CU gets one from either end (workgroup i + CUS joins i);
     // else the longest come first.
-    const int h = blockIdx.x % a.c.kv_heads, order = blockIdx.x / a.c.kv_heads;
+    const int h = block % a.c.kv_heads, order = block / a.c.kv_heads;
     int tile = index.total - 1 - order;
     if (tile < 0) return;
     if (index.total * a.c.kv_heads <= 2 * CUS) {
@@ -647,8 +644,8 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
     seen_by(a, s, c0 / a.group, min(ncols - 1, c0 + CHUNK<D> - 1) / a.group, lo, hi);
     lo &= ~(GROUP - 1);
     const int32_t steps = (hi - lo + GROUP - 1) / GROUP;
-    const int32_t first = (int32_t) ((int64_t) steps * blockIdx.y / gridDim.y);
-    const int32_t n = (int32_t) ((int64_t) steps * (blockIdx.y + 1) / gridDim.y) - first;
+    const int32_t first = (int32_t) ((int64_t) steps * split / a.chunk_splits);
+    const int32_t n = (int32_t) ((int64_t) steps * (split + 1) / a.chunk_splits) - first;
     const int32_t t_first = lo + first * GROUP, t_hi = hi;
 
     // this wave's columns
@@ -931,9 +928,9 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
     }
     if (bad) zest::report(a.b.bad);
 
-    if (gridDim.y > 1) {
+    if (a.chunk_splits > 1) {
         // this split's part: O^T in the registers' own order, maxima and sums
-        float * slot = a.chunk_partial + ((int64_t) (tile * a.c.kv_heads + h) * gridDim.y + blockIdx.y) * CHUNK_PARTIAL<D>;
+        float * slot = a.chunk_partial + ((int64_t) (tile * a.c.kv_heads + h) * a.chunk_splits + split) * CHUNK_PARTIAL<D>;
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
             const int cc = wave * 32 * NQ + 32 * q;
@@ -968,14 +965,12 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(attn
     }
 }
 
-// Joins the splits of chunk_kernel's column tiles, in their order: a workgroup a
+// Joins the splits of attend_chunk's column tiles, in their order: a workgroup a
 // tile of 32 columns, a thread four values of each of its 32-row blocks.
-template <int D>
-__global__ __launch_bounds__(256) void chunk_combine_kernel(attn_args a) {
-    extern __shared__ __align__(16) int32_t attn_sh[];
+template <int D> __device__ inline void combine_chunk(const attn_args & a, int block, int32_t * attn_sh) {
     const zest::seq_index index(a.b, a.c.page_shift, attn_sh, [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
     constexpr int PARTS = CHUNK<D> / 32;
-    const int part = blockIdx.x % PARTS, at = blockIdx.x / PARTS, h = at % a.c.kv_heads, tile = at / a.c.kv_heads;
+    const int part = block % PARTS, at = block / PARTS, h = at % a.c.kv_heads, tile = at / a.c.kv_heads;
     if (tile >= index.total) return;
     int32_t before;
     const kv_seq s = index.at(tile, before);
@@ -1006,14 +1001,43 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(attn_args a) {
     }
 }
 
+// ---- the kernels ----------------------------------------------------------------------
+
+// The chunks' workgroups (a.chunk_blocks of them, each in a.chunk_splits parts),
+// then the others: a batch that holds both runs them side by side. NT 0: none of
+// few columns.
+template <int TYPE, int D, int NT, bool CHUNKS>
+__global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_args a) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int chunks = CHUNKS ? a.chunk_blocks * a.chunk_splits : 0;
+    if constexpr (CHUNKS)
+        if ((int) blockIdx.x < chunks) {
+            const int split = blockIdx.x / a.chunk_blocks;
+            attend_chunk<TYPE, D>(a, blockIdx.x - split * a.chunk_blocks, split, smem);
+            return;
+        }
+    if constexpr (NT > 0) attend_few<TYPE, D, NT>(a, blockIdx.x - chunks, gridDim.x - chunks, smem);
+}
+
+template <int D, int NT, bool CHUNKS> __global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
+    extern __shared__ __align__(16) int32_t attn_sh[];
+    const int chunks = CHUNKS ? a.chunk_blocks * (CHUNK<D> / 32) : 0;
+    if constexpr (CHUNKS)
+        if ((int) blockIdx.x < chunks) {
+            combine_chunk<D>(a, blockIdx.x, attn_sh);
+            return;
+        }
+    if constexpr (NT > 0) combine_few<D, NT>(a, blockIdx.x - chunks, gridDim.x - chunks, attn_sh);
+}
+
 // ---- the host's plan ----------------------------------------------------------------
 
 // What a call launches, by its sizes and bounds alone.
 struct attn_plan {
-    int64_t units, run;         // of attn_kernel, at most: in all, and of a column tile
-    int workgroups, cols;       // of attn_kernel, 0: not launched; columns of its tiles
-    int chunk_cols;             // sequences of more columns go to chunk_kernel
-    int64_t chunk_tiles;        // of chunk_kernel, a k/v head, at most; 0: not launched
+    int64_t units, run;         // of attend_few, at most: in all, and of a column tile
+    int workgroups, cols;       // of attend_few, 0: none; columns of its tiles
+    int chunk_cols;             // sequences of more columns go to attend_chunk
+    int64_t chunk_tiles;        // of attend_chunk, a k/v head, at most; 0: none
     int chunk_splits;
     size_t partial_bytes, bytes;
 };
@@ -1057,31 +1081,30 @@ template <auto KERNEL> int allow_lds(size_t ring) {
     return ZEST_OK;
 }
 
-template <int TYPE, int D, int NT> int launch_few(const attn_args & a, const attn_plan & p, hipStream_t s) {
-    constexpr size_t ring = WAVES * RING_B<D> * STEP_BYTES<D>;
-    if (const int st = allow_lds<&attn_kernel<TYPE, D, NT>>(ring)) return st;
-    hipLaunchKernelGGL((attn_kernel<TYPE, D, NT>), dim3(p.workgroups), dim3(WAVES * 64), ring + zest::seq_index_bytes(a.b.seqs), s, a);
-    if (p.run > 1)  // else every piece is a whole run
-        hipLaunchKernelGGL((combine_kernel<D, NT>), dim3(p.workgroups), dim3(256), zest::seq_index_bytes(a.b.seqs), s, a);
-    return ZEST_OK;
-}
-
-template <int TYPE, int D> int launch(const attn_args & a, const attn_plan & p, hipStream_t s) {
-    if (p.chunk_tiles) {
-        constexpr size_t ring = CHUNK_RING<D>;
-        if (const int st = allow_lds<&chunk_kernel<TYPE, D>>(ring)) return st;
-        hipLaunchKernelGGL((chunk_kernel<TYPE, D>), dim3((unsigned) (p.chunk_tiles * a.c.kv_heads), p.chunk_splits), dim3(WAVES * 64),
-                           ring + zest::seq_index_bytes(a.b.seqs), s, a);
+template <int TYPE, int D, int NT, bool CHUNKS> int launch(attn_args & a, const attn_plan & p, hipStream_t s) {
+    constexpr size_t few = NT ? WAVES * RING_B<D> * STEP_BYTES<D> : 0, ring = CHUNKS && CHUNK_RING<D> > few ? CHUNK_RING<D> : few;
+    const size_t prefix = zest::seq_index_bytes(a.b.seqs);
+    if (const int st = allow_lds<&attn_kernel<TYPE, D, NT, CHUNKS>>(ring)) return st;
+    a.chunk_blocks = (int32_t) (p.chunk_tiles * a.c.kv_heads);
+    hipLaunchKernelGGL((attn_kernel<TYPE, D, NT, CHUNKS>), dim3((unsigned) (a.chunk_blocks * p.chunk_splits + p.workgroups)),
+                       dim3(WAVES * 64), ring + prefix, s, a);
+    // a run of one unit is never split, nor a chunk of one part
+    const bool join_few = NT && p.run > 1, join_chunks = CHUNKS && p.chunk_splits > 1;
+    if (join_chunks) {
+        const unsigned blocks = (unsigned) (a.chunk_blocks * (CHUNK<D> / 32));
+        hipLaunchKernelGGL((combine_kernel<D, NT, CHUNKS>), dim3(blocks + (join_few ? p.workgroups : 0)), dim3(256), prefix, s, a);
+    } else if (join_few) {
+        hipLaunchKernelGGL((combine_kernel<D, NT, false>), dim3(p.workgroups), dim3(256), prefix, s, a);
     }
-    if (p.workgroups)
-        if (const int st = p.cols == 16 ? launch_few<TYPE, D, 1>(a, p, s) : launch_few<TYPE, D, 2>(a, p, s)) return st;
-    if (p.chunk_splits > 1)
-        hipLaunchKernelGGL(chunk_combine_kernel<D>, dim3((unsigned) (p.chunk_tiles * a.c.kv_heads * (CHUNK<D> / 32))), dim3(256),
-                           zest::seq_index_bytes(a.b.seqs), s, a);
     return zest::check_launch("zest_kv_attn");
 }
 
-template <int TYPE> int launch(const attn_args & a, int D, const attn_plan & p, hipStream_t s) {
+template <int TYPE, int D> int launch(attn_args & a, const attn_plan & p, hipStream_t s) {
+    if (p.chunk_tiles) return p.workgroups ? launch<TYPE, D, 2, true>(a, p, s) : launch<TYPE, D, 0, true>(a, p, s);
+    return p.cols == 16 ? launch<TYPE, D, 1, false>(a, p, s) : launch<TYPE, D, 2, false>(a, p, s);
+}
+
+template <int TYPE> int launch(attn_args & a, int D, const attn_plan & p, hipStream_t s) {
     switch (D) {
         case 64: return launch<TYPE, 64>(a, p, s);
         case 96: return launch<TYPE, 96>(a, p, s);
@@ -1117,7 +1140,7 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
     ZEST_REQUIRE(batch->rows * (int64_t) (q_heads / cache->kv_heads) < (1ll << 31) - 64, "%s: %lld rows of %d heads", me,
                  (long long) batch->rows, q_heads);
     const attn_plan plan = plan_of(cache, batch, q_heads / cache->kv_heads);
-    ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads * 8 < (1ll << 31), "%s: a batch of %lld units of work",
+    ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads < (1ll << 23), "%s: a batch of %lld units of work",
                  me, (long long) std::max(plan.units, plan.chunk_tiles));
     const size_t need = plan.bytes;
     ZEST_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need,

@@ -26,7 +26,7 @@ int kv_check_cache(const zest_kv_cache * c, const char * what) {
 int kv_check_batch(const zest_kv_cache * c, const zest_kv_batch * b, const char * what) {
     ZEST_REQUIRE(b && b->tables && b->lens && b->starts, "%s: null batch", what);
     ZEST_REQUIRE(b->seqs > 0 && b->seqs <= KV_MAX_SEQS, "%s: %d sequences (1 to %d)", what, b->seqs, KV_MAX_SEQS);
-    ZEST_REQUIRE(b->rows > 0 && b->rows < (1 << 30), "%s: %lld rows", what, (long long) b->rows);
+    ZEST_REQUIRE(b->rows > 0 && b->rows <= (1 << 27), "%s: %lld rows (1 to 2^27)", what, (long long) b->rows);
     ZEST_REQUIRE(b->table_rows > 0 && b->table_cols > 0 && (int64_t) b->table_cols * c->page_tokens < (1ll << 31),
                  "%s: page tables of %d x %d", what, b->table_rows, b->table_cols);
     ZEST_REQUIRE(b->slots || b->seqs <= b->table_rows, "%s: %d sequences of %d slots", what, b->seqs, b->table_rows);

@@ -51,7 +51,7 @@ typedef struct {
     const int32_t *lens;   /* [table_rows], device */
     const int32_t *starts; /* [seqs + 1], device */
     const int32_t *slots;  /* [seqs], device, or NULL */
-    int64_t rows;          /* rows of q, k, v and the output */
+    int64_t rows;          /* rows of q, k, v and the output, 1 .. 2^27 */
     int32_t seqs;          /* 1 .. 4096 */
     int32_t table_rows, table_cols;
     int32_t max_new, max_len;

@@ -75,7 +75,7 @@ def test_entry_points_refuse_bad_arguments_before_the_gpu(kv):
                   (dict(type=0), E_UNSUPPORTED), (dict(type=8), E_UNSUPPORTED), (dict(kv_heads=0), E_ARG), (dict(kv_heads=1025), E_ARG),
                   (dict(head_dim=80), E_UNSUPPORTED), (dict(head_dim=512), E_UNSUPPORTED), (dict(page_tokens=8), E_UNSUPPORTED),
                   (dict(page_tokens=48), E_UNSUPPORTED), (dict(page_tokens=512), E_UNSUPPORTED)]
-    bad_batches = [(dict(tables=None), E_ARG), (dict(lens=None), E_ARG), (dict(starts=None), E_ARG), (dict(rows=0), E_ARG),
+    bad_batches = [(dict(tables=None), E_ARG), (dict(lens=None), E_ARG), (dict(starts=None), E_ARG), (dict(rows=0), E_ARG), (dict(rows=(1 << 27) + 1), E_ARG),
                    (dict(seqs=0), E_ARG), (dict(seqs=4097, slots=base), E_ARG), (dict(seqs=3), E_ARG), (dict(table_cols=0), E_ARG),
                    (dict(table_cols=1 << 27), E_ARG), (dict(max_new=0), E_ARG), (dict(max_new=5), E_ARG), (dict(max_len=-1), E_ARG)]
 
