@@ -55,10 +55,10 @@ using zest::kv_seq;
 
 // ---- append ---------------------------------------------------------------------
 
-// Eight values of a row of type F32, F16 or BF16 at element offset e (a
-// multiple of 4 for F32 and 8 else: whole 16-byte pieces), as floats.
-__device__ inline void load8(const void * p, int type, int64_t e, float v[8]) {
-    if (type == ZEST_TYPE_F32) {
+// Eight values of a row of type TYPE (F32, F16 or BF16) at element offset e (a
+// multiple of 8: whole 16-byte pieces), as floats; and one.
+template <int TYPE> __device__ inline void load8(const void * p, int64_t e, float v[8]) {
+    if constexpr (TYPE == ZEST_TYPE_F32) {
         const float4 a = *reinterpret_cast<const float4 *>((const float *) p + e);
         const float4 b = *reinterpret_cast<const float4 *>((const float *) p + e + 4);
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
@@ -68,7 +68,7 @@ __device__ inline void load8(const void * p, int type, int64_t e, float v[8]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if (type == ZEST_TYPE_BF16) {
+        if constexpr (TYPE == ZEST_TYPE_BF16) {
             v[2 * i] = __uint_as_float(w[i] << 16);
             v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         } else {
@@ -78,10 +78,10 @@ __device__ inline void load8(const void * p, int type, int64_t e, float v[8]) {
     }
 }
 
-__device__ inline float load1(const void * p, int type, int64_t e) {
-    if (type == ZEST_TYPE_F32) return ((const float *) p)[e];
+template <int TYPE> __device__ inline float load1(const void * p, int64_t e) {
+    if constexpr (TYPE == ZEST_TYPE_F32) return ((const float *) p)[e];
     const uint16_t w = ((const uint16_t *) p)[e];
-    return type == ZEST_TYPE_BF16 ? __uint_as_float((uint32_t) w << 16) : (float) __builtin_bit_cast(_Float16, w);
+    return TYPE == ZEST_TYPE_BF16 ? __uint_as_float((uint32_t) w << 16) : (float) __builtin_bit_cast(_Float16, w);
 }
 
 // One value in a 16-bit type, rounded to nearest even.
@@ -99,7 +99,7 @@ __device__ inline uint4 pack8(const float v[8], int type) {
 struct append_args {
     kv_pages c;
     kv_batch b;
-    int32_t d, cache_type, in_type, q_out_type, q_heads, heads_each;
+    int32_t d, cache_type, q_out_type, q_heads, heads_each, q_parts, kv_parts;  // grid.y: q_parts, then kv_parts of k and of v
     const void * k, * v, * q;
     void * q_out;
     int64_t ldk, ldv, ldq, ldq_out;
@@ -109,17 +109,24 @@ struct append_args {
     const int32_t * pos;
 };
 
-// One workgroup takes the new tokens within 16 consecutive places of a
-// sequence (the unit in which V is stored) and heads_each heads of q, then k,
-// then v. The angles of its tokens are made once, in shared memory: position *
-// frequency in 64 bits, reduced to a fraction of a turn there (rint and a
-// subtraction: exact to 2^-53 of the turns), and sine and cosine of that in 32.
-// HBM bound. K's lanes run over tokens first, so a piece row of 16 tokens is
-// 256 contiguous bytes; V's over columns, 8 tokens a lane, so a wave reads
-// whole rows and writes whole lines.
-__global__ __launch_bounds__(256) void append_kernel(append_args a) {
+// How a token's head is dealt out as items, each one lane's, which reads all of
+// an item before it writes any of it (q_out may be q): pieces of 8 values; with
+// NeoX rope of whole pieces, two pieces that turn with each other (and what is
+// behind the turned dims as pieces); with other NeoX rope, a pair or a value.
+enum { ITEM_PIECE = 0, ITEM_PAIR = 1, ITEM_SINGLE = 2 };
+
+// One workgroup takes the new tokens within 16 consecutive places of a sequence
+// (the unit in which V is stored) and heads_each heads of q, k or v. Every thread
+// requests its first BATCH items before the angles are made, once a workgroup in
+// shared memory: position * frequency in 64 bits, reduced to a fraction of a turn
+// there (rint and a subtraction: exact to 2^-53 of the turns), and sine and
+// cosine of that in 32. HBM bound. K's lanes run over tokens first, so a piece
+// row of 16 tokens is 256 contiguous bytes; V's over columns, 8 tokens a lane, so
+// a wave reads whole rows and writes whole lines.
+template <int IN, int MODE> __global__ __launch_bounds__(256) void append_kernel(append_args a) {
+    constexpr int BATCH = 4, WIDTH = MODE == ITEM_PAIR ? 16 : MODE == ITEM_PIECE ? 8 : 2;
     extern __shared__ __align__(16) int32_t append_sh[];
-    const int t = threadIdx.x, ps = a.c.page_shift;
+    const int t = threadIdx.x, ps = a.c.page_shift, P = 1 << ps;
     const size_t prefix_words = a.b.seqs <= 64 ? 0 : (a.b.seqs + 4) & ~3;
     float2 * turn = reinterpret_cast<float2 *>(append_sh + prefix_words);  // [16][rot / 2]
     const zest::seq_index index(a.b, ps, append_sh, [](const kv_seq & s) { return s.n > 0 ? ((s.len - 1) >> 4) - ((s.len - s.n) >> 4) + 1 : 0; });
@@ -138,134 +145,152 @@ __global__ __launch_bounds__(256) void append_kernel(append_args a) {
         if ((uint32_t) page >= (uint32_t) a.c.pages) page = -1;
     }
     if (page < 0 && t == 0 && blockIdx.y == 0) zest::report(a.b.bad);
-
-    const int total = a.q_heads + 2 * a.c.kv_heads;
-    const int head0 = blockIdx.y * a.heads_each, head1 = min(head0 + a.heads_each, total);
-    if (a.freqs && head0 < a.q_heads + a.c.kv_heads) {
-        for (int i = t; i < n * half; i += 256) {
-            const int tok = i / half, p = i - tok * half;
-            const double x = (double) (a.pos ? a.pos[r0 + tok] : lo + tok) * a.freqs[p] * 0.15915494309189535;  // turns
-            const float f = (float) (x - rint(x));
-            float sn, cs;
-            sincospif(2.0f * f, &sn, &cs);
-            turn[i] = make_float2(cs * a.magnitude, sn * a.magnitude);
-        }
-        __syncthreads();
-    }
-
-    const int P = 1 << ps;
     uint16_t * held = reinterpret_cast<uint16_t *>(a.c.pool + (int64_t) (page < 0 ? 0 : page) * a.c.page_bytes);
-    // A token's head as items, each one lane's: two pieces of 8 that turn with
-    // each other (NeoX halves of whole pieces), one piece, or, where a half is
-    // not whole pieces, one pair or one value. An item is read before it is
-    // written, so q_out may be q.
-    const bool paired = a.neox && half % 8 == 0, single = a.neox && half % 8 != 0;
-    const int turning = paired ? half / 8 : single ? half : 0;
-    const int items = single ? half + (D - a.rot) : paired ? half / 8 + (D - a.rot) / 8 : D / 8;
-    auto item = [&](const void * x, int64_t ld, int head, int tok, int i, auto && put8, auto && put1) {
-        const int64_t at = (r0 + tok) * ld + (int64_t) head * D;
-        const float2 * cs = turn + tok * half;
-        float o[8], y[8];
-        if (paired && i < turning) {
-            load8(x, a.in_type, at + 8 * i, o);
-            load8(x, a.in_type, at + 8 * i + half, y);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float2 r = cs[8 * i + j];
-                const float x0 = o[j], x1 = y[j];
-                o[j] = fmaf(x0, r.x, -(x1 * r.y));
-                y[j] = fmaf(x0, r.y, x1 * r.x);
-            }
-            put8(8 * i, o);
-            put8(8 * i + half, y);
-        } else if (single) {
-            if (i < turning) {
-                const float x0 = load1(x, a.in_type, at + i), x1 = load1(x, a.in_type, at + i + half);
-                const float2 r = cs[i];
-                put1(i, fmaf(x0, r.x, -(x1 * r.y)));
-                put1(i + half, fmaf(x0, r.y, x1 * r.x));
-            } else {
-                put1(i + half, load1(x, a.in_type, at + i + half));
-            }
-        } else {
-            const int e = paired ? a.rot + 8 * (i - turning) : 8 * i;
-            load8(x, a.in_type, at + e, o);
-            if (a.freqs && !paired) {
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    if (e + j >= a.rot) break;
-                    const float2 r = cs[(e + j) / 2];
-                    const float x0 = o[j], x1 = o[j + 1];
-                    o[j] = fmaf(x0, r.x, -(x1 * r.y));
-                    o[j + 1] = fmaf(x0, r.y, x1 * r.x);
-                }
-            }
-            put8(e, o);
-        }
-    };
 
-    for (int head = head0; head < head1; head++) {
-        if (head < a.q_heads) {
-            for (int i = t; i < n * items; i += 256) {
-                const int tok = i / items;
-                const int64_t at = (r0 + tok) * a.ldq_out + (int64_t) head * D;
-                item(
-                    a.q, a.ldq, head, tok, i - tok * items,
-                    [&](int e, const float * o) {
-                        if (a.q_out_type == ZEST_TYPE_F32) {
-                            float * y = (float *) a.q_out + at + e;
-                            *reinterpret_cast<float4 *>(y) = make_float4(o[0], o[1], o[2], o[3]);
-                            *reinterpret_cast<float4 *>(y + 4) = make_float4(o[4], o[5], o[6], o[7]);
-                        } else {
-                            *reinterpret_cast<uint4 *>((uint16_t *) a.q_out + at + e) = pack8(o, a.q_out_type);
-                        }
-                    },
-                    [&](int e, float o) {
-                        if (a.q_out_type == ZEST_TYPE_F32) ((float *) a.q_out)[at + e] = o;
-                        else ((uint16_t *) a.q_out)[at + e] = to16(o, a.q_out_type);
-                    });
-            }
-            continue;
-        }
-        if (page < 0) continue;
-        const int kh = head - a.q_heads;
-        if (kh < a.c.kv_heads) {
-            uint16_t * dst = held + (int64_t) kh * 2 * P * D;
-            for (int i = t; i < 16 * items; i += 256) {
-                const int tok = (i & 15) + p0 - lo;
-                if (tok < 0 || tok >= n) continue;
-                uint16_t * y = dst + ((lo + tok) & (P - 1)) * 8;
-                item(
-                    a.k, a.ldk, kh, tok, i >> 4,
-                    [&](int e, const float * o) {
-                        *reinterpret_cast<uint4 *>(y + (int64_t) (e / 8) * P * 8) = pack8(o, a.cache_type);
-                    },
-                    [&](int e, float o) { y[(int64_t) (e / 8) * P * 8 + e % 8] = to16(o, a.cache_type); });
-            }
-            continue;
-        }
-        const int vh = kh - a.c.kv_heads;
-        uint16_t * dst = held + (int64_t) vh * 2 * P * D + (int64_t) P * D + (int64_t) ((p0 & (P - 1)) >> 4) * 16 * D;
-        for (int i = t; i < 2 * D; i += 256) {
-            const int h = i / D, e = i - h * D;
-            float o[8];
-            bool whole = true;
+    const bool is_q = (int) blockIdx.y < a.q_parts;
+    const int part = is_q ? blockIdx.y : (blockIdx.y - a.q_parts) % a.kv_parts;
+    const int head0 = part * a.heads_each, heads = min(a.heads_each, (is_q ? a.q_heads : a.c.kv_heads) - head0);
+    if (!is_q && page < 0) return;
+
+    if (!is_q && (int) blockIdx.y >= a.q_parts + a.kv_parts) {  // v: 8 tokens of a column a lane
+        const uint32_t total = heads * 2 * D, per = 2 * D;
+        uint16_t * dst = held + (int64_t) P * D + (int64_t) ((p0 & (P - 1)) >> 4) * 16 * D;
+        const bool whole = n == 16;
+        for (uint32_t base = t; base < total; base += 256 * BATCH) {
+            float o[BATCH][8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int tok = 4 * h + (j & 3) + (j >> 2) * 8 + p0 - lo;
-                const bool in = tok >= 0 && tok < n;
-                whole &= in;
-                o[j] = in ? load1(a.v, a.in_type, (r0 + tok) * a.ldv + (int64_t) vh * D + e) : 0.0f;
-            }
-            uint16_t * y = dst + (int64_t) i * 8;
-            if (whole) {
-                *reinterpret_cast<uint4 *>(y) = pack8(o, a.cache_type);
-            } else {
+            for (int u = 0; u < BATCH; u++) {
+                const uint32_t x = base + 256 * u, head = head0 + x / per, i = x % per;
+                const int h = i >= (uint32_t) D, e = i - h * D;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int tok = 4 * h + (j & 3) + (j >> 2) * 8 + p0 - lo;
-                    if (tok >= 0 && tok < n) y[j] = to16(o[j], a.cache_type);
+                    o[u][j] = x < total && tok >= 0 && tok < n ? load1<IN>(a.v, (r0 + tok) * a.ldv + (int64_t) head * D + e) : 0.0f;
                 }
+            }
+#pragma unroll
+            for (int u = 0; u < BATCH; u++) {
+                const uint32_t x = base + 256 * u, head = head0 + x / per, i = x % per;
+                if (x >= total) break;
+                uint16_t * y = dst + (int64_t) head * 2 * P * D + i * 8;
+                if (whole) {
+                    *reinterpret_cast<uint4 *>(y) = pack8(o[u], a.cache_type);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int tok = 4 * (int) (i >= (uint32_t) D) + (j & 3) + (j >> 2) * 8 + p0 - lo;
+                        if (tok >= 0 && tok < n) y[j] = to16(o[u][j], a.cache_type);
+                    }
+                }
+            }
+        }
+        return;
+    }
+
+    const uint32_t turning = MODE == ITEM_PAIR ? half / 8 : MODE == ITEM_SINGLE ? half : 0;
+    const uint32_t items = MODE == ITEM_SINGLE ? half + (D - a.rot) : MODE == ITEM_PAIR ? half / 8 + (D - a.rot) / 8 : D / 8;
+    const uint32_t toks = is_q ? n : 16, total = heads * toks * items;
+    const void * const src = is_q ? a.q : a.k;
+    const int64_t ld = is_q ? a.ldq : a.ldk;
+    // item x: q's lanes over a token's items first, k's over the 16 places; -1
+    // for a place that is not new
+    auto place_of = [&](uint32_t x, uint32_t & head, uint32_t & i) {
+        const uint32_t inner = is_q ? items : 16, rest = x / inner, fast = x - rest * inner, outer = is_q ? toks : items;
+        head = rest / outer;
+        const uint32_t slow = rest - head * outer;
+        head += head0;
+        i = is_q ? fast : slow;
+        const int tok = is_q ? (int) slow : (int) fast + p0 - lo;
+        return x < total && tok >= 0 && tok < n ? tok : -1;
+    };
+    for (uint32_t base = 0; base < total || base == 0; base += 256 * BATCH) {
+        float o[BATCH][WIDTH];
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            uint32_t head, i;
+            const int tok = place_of(base + t + 256 * u, head, i);
+            if (tok < 0) continue;
+            const int64_t at = (r0 + tok) * ld + (int64_t) head * D;
+            if constexpr (MODE == ITEM_SINGLE) {
+                o[u][0] = load1<IN>(src, i < turning ? at + i : at + i + half);
+                if (i < turning) o[u][1] = load1<IN>(src, at + i + half);
+            } else if constexpr (MODE == ITEM_PAIR) {
+                load8<IN>(src, i < turning ? at + 8 * i : at + a.rot + 8 * (i - turning), o[u]);
+                if (i < turning) load8<IN>(src, at + 8 * i + half, o[u] + 8);
+            } else {
+                load8<IN>(src, at + 8 * i, o[u]);
+            }
+        }
+        if (base == 0 && a.freqs) {
+            for (int i = t; i < n * half; i += 256) {
+                const int tok = i / half, p = i - tok * half;
+                const double x = (double) (a.pos ? a.pos[r0 + tok] : lo + tok) * a.freqs[p] * 0.15915494309189535;  // turns
+                const float f = (float) (x - rint(x));
+                float sn, cs;
+                sincospif(2.0f * f, &sn, &cs);
+                turn[i] = make_float2(cs * a.magnitude, sn * a.magnitude);
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            uint32_t head, i;
+            const int tok = place_of(base + t + 256 * u, head, i);
+            if (tok < 0) continue;
+            const int64_t row = (r0 + tok) * a.ldq_out + (int64_t) head * D;
+            uint16_t * y = held + (int64_t) head * 2 * P * D + ((lo + tok) & (P - 1)) * 8;  // k: its token's first piece
+            auto put8 = [&](int e, const float * v) {
+                if (!is_q) {
+                    *reinterpret_cast<uint4 *>(y + (int64_t) e * P) = pack8(v, a.cache_type);
+                } else if (a.q_out_type == ZEST_TYPE_F32) {
+                    float * z = (float *) a.q_out + row + e;
+                    *reinterpret_cast<float4 *>(z) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4 *>(z + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                } else {
+                    *reinterpret_cast<uint4 *>((uint16_t *) a.q_out + row + e) = pack8(v, a.q_out_type);
+                }
+            };
+            auto put1 = [&](int e, float v) {
+                if (!is_q) y[(int64_t) (e / 8) * P * 8 + e % 8] = to16(v, a.cache_type);
+                else if (a.q_out_type == ZEST_TYPE_F32) ((float *) a.q_out)[row + e] = v;
+                else ((uint16_t *) a.q_out)[row + e] = to16(v, a.q_out_type);
+            };
+            const float2 * cs = turn + tok * half;
+            if constexpr (MODE == ITEM_SINGLE) {
+                if (i < turning) {
+                    const float2 r = cs[i];
+                    put1(i, fmaf(o[u][0], r.x, -(o[u][1] * r.y)));
+                    put1(i + half, fmaf(o[u][0], r.y, o[u][1] * r.x));
+                } else {
+                    put1(i + half, o[u][0]);
+                }
+            } else if constexpr (MODE == ITEM_PAIR) {
+                if (i < turning) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float2 r = cs[8 * i + j];
+                        const float x0 = o[u][j], x1 = o[u][8 + j];
+                        o[u][j] = fmaf(x0, r.x, -(x1 * r.y));
+                        o[u][8 + j] = fmaf(x0, r.y, x1 * r.x);
+                    }
+                    put8(8 * i, o[u]);
+                    put8(8 * i + half, o[u] + 8);
+                } else {
+                    put8(a.rot + 8 * (i - turning), o[u]);
+                }
+            } else {
+                if (a.freqs) {
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        if (8 * i + j < (uint32_t) a.rot) {
+                            const float2 r = cs[4 * i + j / 2];
+                            const float x0 = o[u][j], x1 = o[u][j + 1];
+                            o[u][j] = fmaf(x0, r.x, -(x1 * r.y));
+                            o[u][j + 1] = fmaf(x0, r.y, x1 * r.x);
+                        }
+                    }
+                }
+                put8(8 * i, o[u]);
             }
         }
     }
@@ -606,7 +631,6 @@ int zest_kv_append(const zest_kv_cache * cache, const zest_kv_batch * batch, con
     a.b = zest::kv_batch_of(batch, bad);
     a.d = cache->head_dim;
     a.cache_type = cache->type;
-    a.in_type = in_type;
     a.q_out_type = q_out_type;
     a.q_heads = q ? q_heads : 0;
     a.k = k, a.v = v, a.q = q, a.q_out = q_out;
@@ -621,10 +645,24 @@ int zest_kv_append(const zest_kv_cache * cache, const zest_kv_batch * batch, con
     // n new tokens of a sequence touch at most n / 16 + 2 units of 16 places, and at most n
     const int64_t units = std::min<int64_t>(batch->rows, batch->rows / 16 + 2ll * batch->seqs);
     const int heads = a.q_heads + 2 * a.c.kv_heads;
-    a.heads_each = (int) std::max<int64_t>(1, std::min<int64_t>(8, units * heads / 1024));
+    // eight heads a workgroup (four items a thread of a 128-wide NeoX head), fewer
+    // where that would leave CUs without one
+    a.heads_each = (int) std::max<int64_t>(1, std::min<int64_t>(8, units * heads / 512));
+    a.q_parts = (a.q_heads + a.heads_each - 1) / a.heads_each;
+    a.kv_parts = (a.c.kv_heads + a.heads_each - 1) / a.heads_each;
     const size_t lds = zest::seq_index_bytes(batch->seqs) + (size_t) 16 * (a.rot / 2) * sizeof(float2);
-    hipLaunchKernelGGL(append_kernel, dim3((unsigned) units, (unsigned) ((heads + a.heads_each - 1) / a.heads_each)), dim3(256),
-                       lds, zest::as_stream(stream), a);
+    const dim3 grid((unsigned) units, (unsigned) (a.q_parts + 2 * a.kv_parts));
+    const int mode = !a.neox ? ITEM_PIECE : a.rot % 16 == 0 ? ITEM_PAIR : ITEM_SINGLE;
+    const hipStream_t s = zest::as_stream(stream);
+#define ZEST_APPEND(IN)                                                                                              \
+    hipLaunchKernelGGL((mode == ITEM_PIECE  ? append_kernel<IN, ITEM_PIECE>                                          \
+                        : mode == ITEM_PAIR ? append_kernel<IN, ITEM_PAIR>                                           \
+                                            : append_kernel<IN, ITEM_SINGLE>),                                       \
+                       grid, dim3(256), lds, s, a)
+    if (in_type == ZEST_TYPE_F32) ZEST_APPEND(ZEST_TYPE_F32);
+    else if (in_type == ZEST_TYPE_BF16) ZEST_APPEND(ZEST_TYPE_BF16);
+    else ZEST_APPEND(ZEST_TYPE_F16);
+#undef ZEST_APPEND
     return zest::check_launch(me);
 }
 
