@@ -139,22 +139,18 @@ template <int IN, int MODE> __global__ __launch_bounds__(256) void append_kernel
     const int32_t r0 = s.row0 + (lo - first);                                        // row of place lo
     const int n = hi - lo, D = a.d, half = a.rot / 2;
 
-    int32_t page = -1;
-    if (p0 >= 0) {
-        page = a.b.tables[(int64_t) s.slot * a.b.table_cols + (p0 >> ps)];
-        if ((uint32_t) page >= (uint32_t) a.c.pages) page = -1;
-    }
-    if (page < 0 && t == 0 && blockIdx.y == 0) zest::report(a.b.bad);
-    uint16_t * held = reinterpret_cast<uint16_t *>(a.c.pool + (int64_t) (page < 0 ? 0 : page) * a.c.page_bytes);
+    // the page, looked at when the values requested after it are there
+    const int32_t page = p0 >= 0 ? a.b.tables[(int64_t) s.slot * a.b.table_cols + (p0 >> ps)] : -1;
+    auto there = [&]() { return (uint32_t) page < (uint32_t) a.c.pages; };
+    auto page_at = [&]() { return reinterpret_cast<uint16_t *>(a.c.pool + (int64_t) page * a.c.page_bytes); };
 
     const bool is_q = (int) blockIdx.y < a.q_parts;
     const int part = is_q ? blockIdx.y : (blockIdx.y - a.q_parts) % a.kv_parts;
     const int head0 = part * a.heads_each, heads = min(a.heads_each, (is_q ? a.q_heads : a.c.kv_heads) - head0);
-    if (!is_q && page < 0) return;
 
     if (!is_q && (int) blockIdx.y >= a.q_parts + a.kv_parts) {  // v: 8 tokens of a column a lane
         const uint32_t total = heads * 2 * D, per = 2 * D;
-        uint16_t * dst = held + (int64_t) P * D + (int64_t) ((p0 & (P - 1)) >> 4) * 16 * D;
+        const int64_t at = (int64_t) P * D + (int64_t) ((p0 & (P - 1)) >> 4) * 16 * D;
         const bool whole = n == 16;
         for (uint32_t base = t; base < total; base += 256 * BATCH) {
             float o[BATCH][8];
@@ -168,11 +164,15 @@ template <int IN, int MODE> __global__ __launch_bounds__(256) void append_kernel
                     o[u][j] = x < total && tok >= 0 && tok < n ? load1<IN>(a.v, (r0 + tok) * a.ldv + (int64_t) head * D + e) : 0.0f;
                 }
             }
+            if (!there()) {
+                if (t == 0) zest::report(a.b.bad);
+                return;
+            }
 #pragma unroll
             for (int u = 0; u < BATCH; u++) {
                 const uint32_t x = base + 256 * u, head = head0 + x / per, i = x % per;
                 if (x >= total) break;
-                uint16_t * y = dst + (int64_t) head * 2 * P * D + i * 8;
+                uint16_t * y = page_at() + at + (int64_t) head * 2 * P * D + i * 8;
                 if (whole) {
                     *reinterpret_cast<uint4 *>(y) = pack8(o[u], a.cache_type);
                 } else {
@@ -232,6 +232,8 @@ template <int IN, int MODE> __global__ __launch_bounds__(256) void append_kernel
             }
             __syncthreads();
         }
+        if (!is_q && !there()) return;  // v's workgroup reports it
+        uint16_t * const held = is_q ? nullptr : page_at();
 #pragma unroll
         for (int u = 0; u < BATCH; u++) {
             uint32_t head, i;

@@ -37,18 +37,16 @@ struct kv_seq {
 __device__ inline kv_seq load_seq(const kv_batch & a, int b, int page_shift, bool & bad) {
     kv_seq s{a.starts[b], 0, 0, a.slots ? a.slots[b] : b};
     const int32_t end = a.starts[b + 1];
+    const bool named = (uint32_t) s.slot < (uint32_t) a.table_rows;
+    const int32_t len = a.lens[named ? s.slot : 0];  // requested with the starts, not after them
     if (end == s.row0) return s;
-    if (s.row0 < 0 || end < s.row0 || end > a.rows || end - s.row0 > a.max_new || (uint32_t) s.slot >= (uint32_t) a.table_rows) {
+    if (!named || s.row0 < 0 || end < s.row0 || end > a.rows || end - s.row0 > a.max_new || len < 0 || len > a.max_len ||
+        len > ((int64_t) a.table_cols << page_shift)) {
         bad = true;
-        return s;
-    }
-    s.len = a.lens[s.slot];
-    if (s.len < 0 || s.len > a.max_len || s.len > ((int64_t) a.table_cols << page_shift)) {
-        bad = true;
-        s.len = 0;
         return s;
     }
     s.n = end - s.row0;
+    s.len = len;
     return s;
 }
 
