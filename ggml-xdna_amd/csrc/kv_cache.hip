@@ -90,10 +90,12 @@ __device__ inline uint16_t to16(float v, int type) {
 }
 
 __device__ inline uint4 pack8(const float v[8], int type) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = (uint32_t) to16(v[2 * i], type) | ((uint32_t) to16(v[2 * i + 1], type) << 16);
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    typedef float f32x8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    const f32x8 x = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+    if (type == ZEST_TYPE_BF16) return __builtin_bit_cast(uint4, __builtin_convertvector(x, bf16x8));
+    return __builtin_bit_cast(uint4, __builtin_convertvector(x, f16x8));
 }
 
 struct append_args {
@@ -123,8 +125,12 @@ enum { ITEM_PIECE = 0, ITEM_PAIR = 1, ITEM_SINGLE = 2 };
 // cosine of that in 32. HBM bound. K's lanes run over tokens first, so a piece
 // row of 16 tokens is 256 contiguous bytes; V's over columns, 8 tokens a lane, so
 // a wave reads whole rows and writes whole lines.
-template <int IN, int MODE> __global__ __launch_bounds__(256) void append_kernel(append_args a) {
-    constexpr int BATCH = 4, WIDTH = MODE == ITEM_PAIR ? 16 : MODE == ITEM_PIECE ? 8 : 2;
+//
+// BATCH 4, and 1 where no sequence has more than one new token: a quarter of the
+// code, whose first fetch is a good part of so small a call (64 sequences of the
+// Qwen3-4B shape 10.2 -> 5.1 us).
+template <int IN, int MODE, int BATCH> __global__ __launch_bounds__(256) void append_kernel(append_args a) {
+    constexpr int WIDTH = MODE == ITEM_PAIR ? 16 : MODE == ITEM_PIECE ? 8 : 2;
     extern __shared__ __align__(16) int32_t append_sh[];
     const int t = threadIdx.x, ps = a.c.page_shift, P = 1 << ps;
     const size_t prefix_words = a.b.seqs <= 64 ? 0 : (a.b.seqs + 4) & ~3;
@@ -149,9 +155,19 @@ template <int IN, int MODE> __global__ __launch_bounds__(256) void append_kernel
     const int head0 = part * a.heads_each, heads = min(a.heads_each, (is_q ? a.q_heads : a.c.kv_heads) - head0);
 
     if (!is_q && (int) blockIdx.y >= a.q_parts + a.kv_parts) {  // v: 8 tokens of a column a lane
+        const int64_t unit_at = (int64_t) P * D + (int64_t) ((p0 & (P - 1)) >> 4) * 16 * D;
+        if (n < 16) {  // not the whole unit: a value at a time
+            for (uint32_t x = t; x < (uint32_t) (heads * n * D); x += 256) {
+                const uint32_t rest = x / D, e = x - rest * D, head = rest / n, tok = rest - head * n, at = lo + tok - p0;
+                const float v = load1<IN>(a.v, (int64_t) (r0 + tok) * a.ldv + (int64_t) (head0 + head) * D + e);
+                if (there())
+                    page_at()[unit_at + (int64_t) (head0 + head) * 2 * P * D + ((at >> 2 & 1) * D + e) * 8 + (at & 3) + (at >> 3) * 4] =
+                        to16(v, a.cache_type);
+            }
+            if (!there() && t == 0) zest::report(a.b.bad);
+            return;
+        }
         const uint32_t total = heads * 2 * D, per = 2 * D;
-        const int64_t at = (int64_t) P * D + (int64_t) ((p0 & (P - 1)) >> 4) * 16 * D;
-        const bool whole = n == 16;
         for (uint32_t base = t; base < total; base += 256 * BATCH) {
             float o[BATCH][8];
 #pragma unroll
@@ -160,8 +176,8 @@ template <int IN, int MODE> __global__ __launch_bounds__(256) void append_kernel
                 const int h = i >= (uint32_t) D, e = i - h * D;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const int tok = 4 * h + (j & 3) + (j >> 2) * 8 + p0 - lo;
-                    o[u][j] = x < total && tok >= 0 && tok < n ? load1<IN>(a.v, (r0 + tok) * a.ldv + (int64_t) head * D + e) : 0.0f;
+                    const int tok = 4 * h + (j & 3) + (j >> 2) * 8;
+                    o[u][j] = x < total ? load1<IN>(a.v, (int64_t) (r0 + tok) * a.ldv + (int64_t) head * D + e) : 0.0f;
                 }
             }
             if (!there()) {
@@ -172,16 +188,7 @@ template <int IN, int MODE> __global__ __launch_bounds__(256) void append_kernel
             for (int u = 0; u < BATCH; u++) {
                 const uint32_t x = base + 256 * u, head = head0 + x / per, i = x % per;
                 if (x >= total) break;
-                uint16_t * y = page_at() + at + (int64_t) head * 2 * P * D + i * 8;
-                if (whole) {
-                    *reinterpret_cast<uint4 *>(y) = pack8(o[u], a.cache_type);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int tok = 4 * (int) (i >= (uint32_t) D) + (j & 3) + (j >> 2) * 8 + p0 - lo;
-                        if (tok >= 0 && tok < n) y[j] = to16(o[u][j], a.cache_type);
-                    }
-                }
+                *reinterpret_cast<uint4 *>(page_at() + unit_at + (int64_t) head * 2 * P * D + i * 8) = pack8(o[u], a.cache_type);
             }
         }
         return;
@@ -189,19 +196,17 @@ template <int IN, int MODE> __global__ __launch_bounds__(256) void append_kernel
 
     const uint32_t turning = MODE == ITEM_PAIR ? half / 8 : MODE == ITEM_SINGLE ? half : 0;
     const uint32_t items = MODE == ITEM_SINGLE ? half + (D - a.rot) : MODE == ITEM_PAIR ? half / 8 + (D - a.rot) / 8 : D / 8;
-    const uint32_t toks = is_q ? n : 16, total = heads * toks * items;
+    const uint32_t total = heads * n * items;
     const void * const src = is_q ? a.q : a.k;
     const int64_t ld = is_q ? a.ldq : a.ldk;
-    // item x: q's lanes over a token's items first, k's over the 16 places; -1
-    // for a place that is not new
+    // item x: q's lanes over a token's items first, k's over the tokens
     auto place_of = [&](uint32_t x, uint32_t & head, uint32_t & i) {
-        const uint32_t inner = is_q ? items : 16, rest = x / inner, fast = x - rest * inner, outer = is_q ? toks : items;
+        const uint32_t inner = is_q ? items : n, rest = x / inner, fast = x - rest * inner, outer = is_q ? n : items;
         head = rest / outer;
         const uint32_t slow = rest - head * outer;
         head += head0;
         i = is_q ? fast : slow;
-        const int tok = is_q ? (int) slow : (int) fast + p0 - lo;
-        return x < total && tok >= 0 && tok < n ? tok : -1;
+        return x < total ? (int) (is_q ? slow : fast) : -1;
     };
     for (uint32_t base = 0; base < total || base == 0; base += 256 * BATCH) {
         float o[BATCH][WIDTH];
@@ -346,50 +351,69 @@ struct assign_args {
     uint32_t * bad;
 };
 
+// Working memory of the one-workgroup kernels below that fits shared memory: a
+// round trip to global memory between phases costs more than the phase.
+constexpr int FEW_ENTRIES = 512, FEW_PAGES = 4096;
+
 // The tables' part of a step, by one workgroup: its phases are ordered by
 // barriers, so every count is exact and the result does not depend on the order
-// of the atomics (sums only). Latency bound: a few passes over the entries'
-// rows and one over refs up to the last page taken.
+// of the atomics (sums only). Latency bound: a chain of a few dependent accesses
+// (12 slots of up to 13 pages: 8.2 us, with entries and free pages in global memory
+// 12.3).
 __global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
     __shared__ uint32_t seen[MAX_SLOTS / 32], twice[MAX_SLOTS / 32], replaced[MAX_SLOTS / 32];
+    __shared__ assign_entry few_entries[FEW_ENTRIES];
+    __shared__ int32_t few_pages[FEW_PAGES];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int P = 1 << a.page_shift;
+    assign_entry * const entries = a.n <= FEW_ENTRIES ? few_entries : a.entries;
+    int32_t * const free_list = a.pages <= FEW_PAGES ? few_pages : a.free_list;
     bool bad = false;
     for (int i = t; i < (a.rows + 31) / 32; i += STEP) seen[i] = twice[i] = replaced[i] = 0;
     __syncthreads();
     for (int i = t; i < a.n; i += STEP) {
-        const int32_t d = a.dst[i];
+        const int32_t d = a.dst[i], s = a.src[i];
         if ((uint32_t) d >= (uint32_t) a.rows) continue;
         const uint32_t bit = 1u << (d & 31);
         if (atomicOr(&seen[d >> 5], bit) & bit) atomicOr(&twice[d >> 5], bit);
-        if (a.src[i] != d) atomicOr(&replaced[d >> 5], bit);
+        if (s != d) atomicOr(&replaced[d >> 5], bit);
     }
     __syncthreads();
     auto has = [](const uint32_t * set, int32_t d) { return (set[d >> 5] >> (d & 31)) & 1u; };
 
-    // what each entry needs
-    for (int i = t; i < a.n; i += STEP) {
-        const int32_t d = a.dst[i], s = a.src[i], g = a.grow[i];
+    // what each entry needs, and its place in the list of free pages
+    int32_t want = 0;
+    for (int i0 = 0; i0 < a.n; i0 += STEP) {
+        const int i = i0 + t;
         assign_entry e{-1, 0, 0, 0};
-        const bool named = (uint32_t) d < (uint32_t) a.rows && s >= -1 && s < a.rows;
-        if (named && !has(twice, d) && (s < 0 || s == d || !has(replaced, s)) && g >= 0) {
-            const int64_t base = s >= 0 ? a.lens[s] : 0, room = (int64_t) a.cols << a.page_shift, old = a.lens[d];
-            if (base >= 0 && base + g <= room && old >= 0 && old <= room) {
-                e.base = (int32_t) base;
-                const int32_t held = (int32_t) (s == d ? (base + P - 1) >> a.page_shift : base >> a.page_shift);
-                e.need = (int32_t) ((base + g + P - 1) >> a.page_shift) - held;
-                e.old_pages = s == d ? 0 : (int32_t) ((old + P - 1) >> a.page_shift);
+        if (i < a.n) {
+            const int32_t d = a.dst[i], s = a.src[i], g = a.grow[i];
+            const bool named = (uint32_t) d < (uint32_t) a.rows && s >= -1 && s < a.rows;
+            const int32_t held_base = a.lens[named && s >= 0 ? s : 0], held_old = a.lens[named ? d : 0];
+            if (named && !has(twice, d) && (s < 0 || s == d || !has(replaced, s)) && g >= 0) {
+                const int64_t base = s >= 0 ? held_base : 0, room = (int64_t) a.cols << a.page_shift, old = held_old;
+                if (base >= 0 && base + g <= room && old >= 0 && old <= room) {
+                    e.base = (int32_t) base;
+                    const int32_t held = (int32_t) (s == d ? (base + P - 1) >> a.page_shift : base >> a.page_shift);
+                    e.need = (int32_t) ((base + g + P - 1) >> a.page_shift) - held;
+                    e.old_pages = s == d ? 0 : (int32_t) ((old + P - 1) >> a.page_shift);
+                }
             }
+            bad |= e.base < 0;
         }
-        bad |= e.base < 0;
-        a.entries[i] = e;
-        a.copies[i] = make_int2(-1, -1);
+        int32_t sum;
+        e.first = want + scan_step(e.need, &sum);
+        want += sum;
+        if (i < a.n) {
+            entries[i] = e;
+            a.copies[i] = make_int2(-1, -1);
+        }
     }
     __syncthreads();
 
     // the replaced rows' pages are released, a wave an entry
     for (int i = wave; i < a.n; i += STEP / 64) {
-        const assign_entry e = a.entries[i];
+        const assign_entry e = entries[i];
         if (e.base < 0 || e.old_pages == 0) continue;
         const int32_t * row = a.tables + (int64_t) a.dst[i] * a.cols;
         for (int j = lane; j < e.old_pages; j += 64) {
@@ -404,30 +428,20 @@ __global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
     __threadfence();
     __syncthreads();
 
-    // each entry's place in the list of free pages
-    int32_t want = 0;
-    for (int i0 = 0; i0 < a.n; i0 += STEP) {
-        const int i = i0 + t;
-        int32_t sum;
-        const int32_t before = scan_step(i < a.n ? a.entries[i].need : 0, &sum);
-        if (i < a.n) a.entries[i].first = want + before;
-        want += sum;
-    }
     int32_t found = 0;
     for (int p0 = 0; p0 < a.pages && found < want; p0 += STEP) {
         const int p = p0 + t;
         const bool is_free = p < a.pages && fresh(&a.refs[p]) <= 0;
         int32_t sum;
         const int32_t before = scan_step(is_free, &sum);
-        if (is_free && found + before < want) a.free_list[found + before] = p;
+        if (is_free && found + before < want) free_list[found + before] = p;
         found += sum;
     }
-    __threadfence();
     __syncthreads();
 
     // the new rows, a wave an entry
     for (int i = wave; i < a.n; i += STEP / 64) {
-        const assign_entry e = a.entries[i];
+        const assign_entry e = entries[i];
         if (e.base < 0) continue;
         const int32_t d = a.dst[i], s = a.src[i], g = a.grow[i];
         int32_t * row = a.tables + (int64_t) d * a.cols;
@@ -437,7 +451,7 @@ __global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
             if (!fits) continue;
             const int32_t held = (e.base + P - 1) >> a.page_shift;
             for (int j = lane; j < e.need; j += 64) {
-                const int32_t id = a.free_list[e.first + j];
+                const int32_t id = free_list[e.first + j];
                 row[held + j] = id;
                 a.refs[id] = 1;
             }
@@ -453,7 +467,7 @@ __global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
                 if ((uint32_t) id < (uint32_t) a.pages) atomicAdd(&a.refs[id], 1);
                 else bad = true;
             } else if (j < total) {
-                id = a.free_list[e.first + j - shared];
+                id = free_list[e.first + j - shared];
                 a.refs[id] = 1;
                 if (j == shared && (e.base & (P - 1))) {
                     const int32_t from = parent[j];
@@ -468,17 +482,16 @@ __global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
     if (bad) zest::report(a.bad);
 }
 
-// Copies whole pages in every layer: copies[i] = (from, to), -1 for none; with
-// `count` only the first *count. A workgroup takes COPY_BYTES of a page at a
-// time, four 16-byte loads a thread before the first store.
+// Copies n whole pages in every layer, copies[i] = (from, to), -1 for none; by
+// `blocks` workgroups of 256 threads, each COPY_BYTES of a page at a time, four
+// 16-byte loads a thread before the first store.
 constexpr int COPY_BYTES = 16384;
 
-__global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t * pool, int64_t page_bytes, int64_t layer_stride,
-                                                         int32_t layers, const int2 * copies, int32_t n,
-                                                         const int32_t * count) {
+__device__ inline void copy_pages(uint8_t * pool, int64_t page_bytes, int64_t layer_stride, int32_t layers, const int2 * copies,
+                                  int32_t n, int32_t block, int32_t blocks) {
     const int32_t parts = (int32_t) ((page_bytes + COPY_BYTES - 1) / COPY_BYTES);
-    const int64_t total = (int64_t) (count ? *count : n) * layers * parts;
-    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
+    const int64_t total = (int64_t) n * layers * parts;
+    for (int64_t w = block; w < total; w += blocks) {
         const int32_t part = (int32_t) (w % parts), layer = (int32_t) (w / parts % layers);
         const int2 c = copies[w / parts / layers];
         if (c.x < 0) continue;
@@ -496,6 +509,11 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t * pool, int64_t
     }
 }
 
+__global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t * pool, int64_t page_bytes, int64_t layer_stride, int32_t layers,
+                                                         const int2 * copies, int32_t n) {
+    copy_pages(pool, page_bytes, layer_stride, layers, copies, n, blockIdx.x, gridDim.x);
+}
+
 // ---- compaction ------------------------------------------------------------------
 
 struct compact_args {
@@ -503,54 +521,71 @@ struct compact_args {
     int32_t * refs_out, * tables_out, * live;
     int32_t pages;
     int64_t entries;
-    int2 * moves;       // [pages / 2 + 1]
-    int32_t * count;    // moves
+    int2 * moves;       // [pages / 2 + 1]: from, to
+    int32_t * count;    // of them
     int32_t * place;    // [pages]: where a page is afterwards, -1 for one without references
     uint32_t * bad;
 };
 
-// Which page moves where, by one workgroup: a count of the live pages, then
-// the ranks of the free pages below it and of the live ones from it on, which
-// are equally many: rank k of one goes to rank k of the other.
+// Which page moves where, by one workgroup: a count of the live pages, then the
+// free pages below it and the live ones from it on, which are equally many: rank k
+// of these goes to rank k of those.
 __global__ __launch_bounds__(STEP) void compact_plan_kernel(compact_args a) {
+    __shared__ int32_t few_holes[FEW_PAGES];
     const int t = threadIdx.x;
     int32_t mine = 0, live;
     for (int p = t; p < a.pages; p += STEP) mine += a.refs[p] > 0;
     scan_step(mine, &live);
-    int32_t holes = 0, movers = 0;
-    for (int p0 = 0; p0 < a.pages; p0 += STEP) {
+    const bool few = live <= FEW_PAGES;
+    int32_t holes = 0;
+    for (int p0 = 0; p0 < live; p0 += STEP) {
         const int p = p0 + t;
-        const bool used = p < a.pages && a.refs[p] > 0;
-        const bool hole = p < live && !used, moves = p >= live && used;
+        const int32_t refs = p < live ? a.refs[p] : 1;
         int32_t sum;
-        const int32_t before = scan_step(hole ? 1 : moves ? 0x10000 : 0, &sum);
-        if (hole) a.moves[holes + (before & 0xffff)].y = p;
-        if (moves) a.moves[movers + (before >> 16)].x = p;
-        if (p < a.pages) a.place[p] = used && !moves ? p : -1;
-        holes += sum & 0xffff;
-        movers += sum >> 16;
+        const int32_t before = holes + scan_step(refs <= 0, &sum);
+        if (refs <= 0) {
+            if (few) few_holes[before] = p;
+            else a.moves[before].y = p;
+        }
+        if (p < live) {
+            a.place[p] = refs > 0 ? p : -1;
+            if (refs > 0) a.refs_out[p] = refs;
+        }
+        holes += sum;
     }
-    __threadfence();
     __syncthreads();
-    for (int k = t; k < movers; k += STEP) a.place[a.moves[k].x] = a.moves[k].y;
+    int32_t movers = 0;
+    for (int p0 = live; p0 < a.pages; p0 += STEP) {
+        const int p = p0 + t;
+        const int32_t refs = p < a.pages ? a.refs[p] : 0;
+        int32_t sum;
+        const int32_t k = movers + scan_step(refs > 0, &sum);
+        if (refs > 0) {
+            const int32_t to = few ? few_holes[k] : a.moves[k].y;
+            a.moves[k] = make_int2(p, to);
+            a.place[p] = to;
+            a.refs_out[to] = refs;
+        } else if (p < a.pages) {
+            a.place[p] = -1;
+        }
+        if (p < a.pages) a.refs_out[p] = 0;  // refs_out may be refs: this page's count has been read
+        movers += sum;
+    }
     if (t == 0) {
         *a.count = movers;
         *a.live = live;
     }
-    // refs (refs_out may be refs): the live pages' counts at their new places,
-    // every free page below n filled, then zeros behind
-    for (int p = t; p < live; p += STEP) {
-        const int32_t r = a.refs[p];
-        if (r > 0) a.refs_out[p] = r;
-    }
-    for (int k = t; k < movers; k += STEP) a.refs_out[a.moves[k].y] = a.refs[a.moves[k].x];
-    __syncthreads();
-    for (int p = live + t; p < a.pages; p += STEP) a.refs_out[p] = 0;
 }
 
-__global__ __launch_bounds__(256) void compact_tables_kernel(compact_args a) {
+// The tables, by the first table_blocks workgroups, and beside them the pages.
+__global__ __launch_bounds__(256) void compact_move_kernel(compact_args a, int32_t table_blocks, uint8_t * pool, int64_t page_bytes,
+                                                           int64_t layer_stride, int32_t layers) {
+    if ((int32_t) blockIdx.x >= table_blocks) {
+        copy_pages(pool, page_bytes, layer_stride, layers, a.moves, *a.count, blockIdx.x - table_blocks, gridDim.x - table_blocks);
+        return;
+    }
     bool bad = false;
-    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < a.entries; i += (int64_t) gridDim.x * 256) {
+    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < a.entries; i += (int64_t) table_blocks * 256) {
         const int32_t id = a.tables[i];
         const int32_t to = (uint32_t) id < (uint32_t) a.pages ? a.place[id] : -1;
         bad |= to < 0 && id != -1;
@@ -655,11 +690,12 @@ int zest_kv_append(const zest_kv_cache * cache, const zest_kv_batch * batch, con
     const size_t lds = zest::seq_index_bytes(batch->seqs) + (size_t) 16 * (a.rot / 2) * sizeof(float2);
     const dim3 grid((unsigned) units, (unsigned) (a.q_parts + 2 * a.kv_parts));
     const int mode = !a.neox ? ITEM_PIECE : a.rot % 16 == 0 ? ITEM_PAIR : ITEM_SINGLE;
+    const bool one = batch->max_new == 1;
     const hipStream_t s = zest::as_stream(stream);
 #define ZEST_APPEND(IN)                                                                                              \
-    hipLaunchKernelGGL((mode == ITEM_PIECE  ? append_kernel<IN, ITEM_PIECE>                                          \
-                        : mode == ITEM_PAIR ? append_kernel<IN, ITEM_PAIR>                                           \
-                                            : append_kernel<IN, ITEM_SINGLE>),                                       \
+    hipLaunchKernelGGL((mode == ITEM_PIECE  ? (one ? append_kernel<IN, ITEM_PIECE, 1> : append_kernel<IN, ITEM_PIECE, 4>) \
+                        : mode == ITEM_PAIR ? (one ? append_kernel<IN, ITEM_PAIR, 1> : append_kernel<IN, ITEM_PAIR, 4>)   \
+                                            : append_kernel<IN, ITEM_SINGLE, 4>),                                         \
                        grid, dim3(256), lds, s, a)
     if (in_type == ZEST_TYPE_F32) ZEST_APPEND(ZEST_TYPE_F32);
     else if (in_type == ZEST_TYPE_BF16) ZEST_APPEND(ZEST_TYPE_BF16);
@@ -701,7 +737,7 @@ int zest_kv_assign(const zest_kv_cache * cache, int32_t layers, int64_t layer_st
     hipLaunchKernelGGL(assign_kernel, dim3(1), dim3(STEP), 0, s, a);
     if (const int st = zest::check_launch(me)) return st;
     hipLaunchKernelGGL(copy_pages_kernel, dim3(copy_grid(cache, layers, n)), dim3(256), 0, s, (uint8_t *) cache->pool,
-                       (int64_t) zest_kv_page_bytes(cache), layer_stride, layers, a.copies, n, (const int32_t *) nullptr);
+                       (int64_t) zest_kv_page_bytes(cache), layer_stride, layers, a.copies, n);
     return zest::check_launch(me);
 }
 
@@ -727,11 +763,9 @@ int zest_kv_compact(const zest_kv_cache * cache, int32_t layers, int64_t layer_s
     const hipStream_t s = zest::as_stream(stream);
     hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(STEP), 0, s, a);
     if (const int st = zest::check_launch(me)) return st;
-    hipLaunchKernelGGL(compact_tables_kernel, dim3((unsigned) std::min<int64_t>((a.entries + 255) / 256, 1024)), dim3(256), 0, s,
-                       a);
-    if (const int st = zest::check_launch(me)) return st;
-    hipLaunchKernelGGL(copy_pages_kernel, dim3(copy_grid(cache, layers, cache->pages / 2 + 1)), dim3(256), 0, s,
-                       (uint8_t *) cache->pool, (int64_t) zest_kv_page_bytes(cache), layer_stride, layers, a.moves, 0, a.count);
+    const int32_t table_blocks = (int32_t) std::min<int64_t>((a.entries + 255) / 256, 1024);
+    hipLaunchKernelGGL(compact_move_kernel, dim3(table_blocks + copy_grid(cache, layers, cache->pages / 2 + 1)), dim3(256), 0, s, a,
+                       table_blocks, (uint8_t *) cache->pool, (int64_t) zest_kv_page_bytes(cache), layer_stride, layers);
     return zest::check_launch(me);
 }
 
