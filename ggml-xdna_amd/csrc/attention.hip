@@ -548,8 +548,12 @@ __device__ inline void attend_few(const attn_args & a, int block, int blocks, ui
 }
 
 // Joins the pieces of the column tile whose run starts in workgroup w's share
-// and goes on past it, if there is one: theirs are the last of the share.
-template <int D, int NT> __device__ inline void combine_few(const attn_args & a, int block, int blocks, int32_t * attn_sh) {
+// and goes on past it, if there is one: theirs are the last of the share. A
+// workgroup takes 256 of the tile's groups of four values, and requests eight
+// pieces at a time.
+template <int D, int NT> constexpr int COMBINE_PARTS = 16 * NT * D / 4 / 256;
+
+template <int D, int NT> __device__ inline void combine_few(const attn_args & a, int block, int part, int blocks, int32_t * attn_sh) {
     constexpr int COLS = 16 * NT, UNITS = D / 4;
     const zest::seq_index index(a.b, a.c.page_shift, attn_sh, [&](const kv_seq & s) { return cost_of(a, s, COLS); });
     const unit_shares shares(index.total, blocks);
@@ -562,22 +566,32 @@ template <int D, int NT> __device__ inline void combine_few(const attn_args & a,
     if (start < u0 || end <= u1) return;
     const int32_t h = item / tiles, ct = item - h * tiles, ncols = s.n * a.group;
     const int last = shares.owner(end - 1);
-    for (int i = threadIdx.x; i < COLS * UNITS; i += 256) {
-        const int oc = i / UNITS, unit = i - oc * UNITS, cc = ct * COLS + oc;
+    {
+        const int i = part * 256 + threadIdx.x, oc = i / UNITS, unit = i - oc * UNITS, cc = ct * COLS + oc;
         if (cc >= ncols) return;
         const float * x = a.partial + (int64_t) (2 * block + 1) * partial_floats(COLS, D);
         float m = x[COLS * D + oc], l = x[COLS * D + COLS + oc];
         float4 o = *reinterpret_cast<const float4 *>(x + oc * D + unit * 4);
-#pragma unroll 4
-        for (int w = block + 1; w <= last; w++) {
-            const float * y = a.partial + (int64_t) (2 * w) * partial_floats(COLS, D);
-            const float m1 = y[COLS * D + oc], l1 = y[COLS * D + COLS + oc], now = fmaxf(m, m1);
-            const float4 v = *reinterpret_cast<const float4 *>(y + oc * D + unit * 4);
-            const float base = now == -INFINITY ? 0.0f : now;
-            const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(m1 - base);
-            m = now;
-            l = l * f + l1 * g;
-            o = make_float4(o.x * f + v.x * g, o.y * f + v.y * g, o.z * f + v.z * g, o.w * f + v.w * g);
+        for (int w0 = block + 1; w0 <= last; w0 += 8) {
+            float m1[8], l1[8];
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {  // past the last piece, that piece again, left out below
+                const float * y = a.partial + (int64_t) (2 * min(w0 + k, last)) * partial_floats(COLS, D);
+                m1[k] = y[COLS * D + oc];
+                l1[k] = y[COLS * D + COLS + oc];
+                v[k] = *reinterpret_cast<const float4 *>(y + oc * D + unit * 4);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const bool in = w0 + k <= last;
+                const float now = in ? fmaxf(m, m1[k]) : m, base = now == -INFINITY ? 0.0f : now;
+                const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(m1[k] - base);
+                m = now;
+                const float4 x = make_float4(o.x * f + v[k].x * g, o.y * f + v[k].y * g, o.z * f + v[k].z * g, o.w * f + v[k].w * g);
+                l = in ? l * f + l1[k] * g : l;
+                o = make_float4(in ? x.x : o.x, in ? x.y : o.y, in ? x.z : o.z, in ? x.w : o.w);
+            }
         }
         const float f = l == 0.0f ? 0.0f : 1.0f / l;
         const float v[4] = {o.x * f, o.y * f, o.z * f, o.w * f};
@@ -979,17 +993,32 @@ template <int D> __device__ inline void combine_chunk(const attn_args & a, int b
     if (cc >= s.n * a.group) return;
     const float * slots = a.chunk_partial + (int64_t) at * a.chunk_splits * CHUNK_PARTIAL<D>;
     float m = -INFINITY, l = 0.0f;
+#pragma unroll 8
     for (int i = 0; i < a.chunk_splits; i++) m = fmaxf(m, slots[(int64_t) i * CHUNK_PARTIAL<D> + CHUNK<D> * D + part * 32 + col]);
     const float base = m == -INFINITY ? 0.0f : m;
     float o[D / 32][4] = {};
-    for (int i = 0; i < a.chunk_splits; i++) {
-        const float * x = slots + (int64_t) i * CHUNK_PARTIAL<D>;
-        const float f = __builtin_amdgcn_exp2f(x[CHUNK<D> * D + part * 32 + col] - base);
-        l += x[CHUNK<D> * (D + 1) + part * 32 + col] * f;
+    for (int i0 = 0; i0 < a.chunk_splits; i0 += 2) {
+        float4 v[2][D / 32];
+        float f[2], l1[2];
 #pragma unroll
-        for (int dt = 0; dt < D / 32; dt++) {
-            const float4 v = *reinterpret_cast<const float4 *>(x + part * 32 * D + ((dt * 4 + k) * 64 + lane) * 4);
-            o[dt][0] += v.x * f, o[dt][1] += v.y * f, o[dt][2] += v.z * f, o[dt][3] += v.w * f;
+        for (int e = 0; e < 2; e++) {  // past the last split, that split again, left out below
+            const float * x = slots + (int64_t) min(i0 + e, a.chunk_splits - 1) * CHUNK_PARTIAL<D>;
+            f[e] = x[CHUNK<D> * D + part * 32 + col];
+            l1[e] = x[CHUNK<D> * (D + 1) + part * 32 + col];
+#pragma unroll
+            for (int dt = 0; dt < D / 32; dt++) v[e][dt] = *reinterpret_cast<const float4 *>(x + part * 32 * D + ((dt * 4 + k) * 64 + lane) * 4);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const bool in = i0 + e < a.chunk_splits;
+            const float w = __builtin_amdgcn_exp2f(f[e] - base);
+            l = in ? l + l1[e] * w : l;
+#pragma unroll
+            for (int dt = 0; dt < D / 32; dt++) {
+                const float x[4] = {v[e][dt].x, v[e][dt].y, v[e][dt].z, v[e][dt].w};
+#pragma unroll
+                for (int c = 0; c < 4; c++) o[dt][c] = in ? o[dt][c] + x[c] * w : o[dt][c];
+            }
         }
     }
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1027,7 +1056,11 @@ template <int D, int NT, bool CHUNKS> __global__ __launch_bounds__(256) void com
             combine_chunk<D>(a, blockIdx.x, attn_sh);
             return;
         }
-    if constexpr (NT > 0) combine_few<D, NT>(a, blockIdx.x - chunks, gridDim.x - chunks, attn_sh);
+    if constexpr (NT > 0) {
+        constexpr int PARTS = COMBINE_PARTS<D, NT>;
+        const int at = blockIdx.x - chunks;
+        combine_few<D, NT>(a, at / PARTS, at % PARTS, (gridDim.x - chunks) / PARTS, attn_sh);
+    }
 }
 
 // ---- the host's plan ----------------------------------------------------------------
@@ -1089,12 +1122,13 @@ template <int TYPE, int D, int NT, bool CHUNKS> int launch(attn_args & a, const 
     hipLaunchKernelGGL((attn_kernel<TYPE, D, NT, CHUNKS>), dim3((unsigned) (a.chunk_blocks * p.chunk_splits + p.workgroups)),
                        dim3(WAVES * 64), ring + prefix, s, a);
     // a run of one unit is never split, nor a chunk of one part
+    constexpr int few_parts = NT ? COMBINE_PARTS<D, NT> : 1;
     const bool join_few = NT && p.run > 1, join_chunks = CHUNKS && p.chunk_splits > 1;
     if (join_chunks) {
         const unsigned blocks = (unsigned) (a.chunk_blocks * (CHUNK<D> / 32));
-        hipLaunchKernelGGL((combine_kernel<D, NT, CHUNKS>), dim3(blocks + (join_few ? p.workgroups : 0)), dim3(256), prefix, s, a);
+        hipLaunchKernelGGL((combine_kernel<D, NT, CHUNKS>), dim3(blocks + (join_few ? p.workgroups * few_parts : 0)), dim3(256), prefix, s, a);
     } else if (join_few) {
-        hipLaunchKernelGGL((combine_kernel<D, NT, false>), dim3(p.workgroups), dim3(256), prefix, s, a);
+        hipLaunchKernelGGL((combine_kernel<D, NT, false>), dim3(p.workgroups * few_parts), dim3(256), prefix, s, a);
     }
     return zest::check_launch("zest_kv_attn");
 }
