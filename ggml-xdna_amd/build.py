@@ -28,6 +28,12 @@ COMMON = [
     "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
 ]
 
+# Flags of single sources. attention.hip: MFMA results in vector registers, which
+# the vector units read, also where a kernel needs more than 256 of them (the
+# 256-wide heads' chunks; by default they go to accumulation registers and every
+# step copies O^T out and back).
+EXTRA = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+
 
 def sources() -> list[Path]:
     src = sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.cpp"))
@@ -37,7 +43,7 @@ def sources() -> list[Path]:
 
 def _compile(src: Path) -> Path:
     obj = OBJ / (src.relative_to(CSRC).as_posix().replace("/", "__") + ".o")
-    cmd = [HIPCC, *COMMON, "-c", str(src), "-o", str(obj)]
+    cmd = [HIPCC, *COMMON, *EXTRA.get(src.name, []), "-c", str(src), "-o", str(obj)]
     if src.suffix == ".cpp":
         cmd[1:1] = ["-x", "hip"]
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -34,7 +34,12 @@ constexpr int WAVES = 4;     // waves of a workgroup
 constexpr int GROUP = 32;    // tokens a wave takes at a time
 constexpr int UNIT = WAVES * GROUP;  // tokens of a unit of work
 constexpr int CUS = 256;
-constexpr int MOST_SPLIT_COLS = 64;  // columns of a sequence that attend_few takes
+// The most columns of a sequence that attend_few takes: two of its tiles, each of
+// which reads K and V, where all that a call's bounds let it read stays in the
+// 256 MB last-level cache (9 short sequences of the small model 20.6 us, with one
+// tile 25.4), else one (16 sequences of 12 drafted tokens, 48 columns, at 4096 to
+// 8192 tokens 105.7 us, with two tiles 126.2).
+constexpr int most_few_cols(double kv_bytes) { return kv_bytes <= 256e6 ? 64 : 32; }
 
 // The cache's element type: its fragment, its MFMA and its exponent field.
 template <int TYPE> struct elem;
@@ -256,7 +261,7 @@ constexpr int partial_floats(int cols, int D) { return cols * (D + 2); }
 // {0..7, 16..23} and {8..15, 24..31}, so that a lane group's 8 weights, in the
 // registers they are in, are the 8 tokens of a V piece.
 template <int TYPE, int D, int NT>
-__device__ inline void attend_few(const attn_args & a, int block, int blocks, uint8_t * ring_sh) {
+__device__ __forceinline__ void attend_few(const attn_args & a, int block, int blocks, uint8_t * ring_sh) {
     typedef typename elem<TYPE>::frag frag;
     constexpr int COLS = 16 * NT, KS = D / 32, DT = D / 16, R = RING_B<D>, LOADS = D / 16;  // loads of K (or V) a step
     // ring_sh, a wave: [R][K: D/8][32][8], V: [4][D][8]; then the prefix sums
@@ -553,7 +558,7 @@ __device__ inline void attend_few(const attn_args & a, int block, int blocks, ui
 // pieces at a time.
 template <int D, int NT> constexpr int COMBINE_PARTS = 16 * NT * D / 4 / 256;
 
-template <int D, int NT> __device__ inline void combine_few(const attn_args & a, int block, int part, int blocks, int32_t * attn_sh) {
+template <int D, int NT> __device__ __forceinline__ void combine_few(const attn_args & a, int block, int part, int blocks, int32_t * attn_sh) {
     constexpr int COLS = 16 * NT, UNITS = D / 4;
     const zest::seq_index index(a.b, a.c.page_shift, attn_sh, [&](const kv_seq & s) { return cost_of(a, s, COLS); });
     const unit_shares shares(index.total, blocks);
@@ -605,7 +610,8 @@ template <int D, int NT> __device__ inline void combine_few(const attn_args & a,
 // Column tiles of 32 a wave of attend_chunk takes: two where the registers hold
 // them (O^T of 64 columns is D values a lane, Q^T half of that).
 template <int D> constexpr int QT = 1;
-template <int D> constexpr int CHUNK = WAVES * 32 * QT<D>;  // columns of a workgroup
+constexpr int chunk_waves(int D) { return D == 192 ? 8 : 4; }
+template <int D> constexpr int CHUNK = chunk_waves(D) * 32 * QT<D>;  // columns of a workgroup
 // Steps of K and of V in shared memory. At step j the scores read K of j + 1 while
 // those of j + 2 and j + 3 are on their way, the weights read V of j - 1.
 constexpr int K_RING = 3, V_RING = 5;
@@ -622,14 +628,14 @@ __device__ inline int32_t chunk_tiles_of(const attn_args & a, const kv_seq & s, 
     return cols > a.chunk_cols ? (int32_t) ((cols + chunk - 1) / chunk) : 0;
 }
 
-// One column tile of a chunk: 4 waves of 32 QT columns each over the keys that
+// One column tile of a chunk: 4 or 8 waves of 32 QT columns each over the keys that
 // any of the tile's columns sees, 32 tokens a step. K and V of a step go from
 // the pool straight into shared memory (16 bytes a lane, in the pool's order,
 // which is the order they are read in: every read is 512 contiguous bytes a half
 // wave), two steps ahead of their use, with one barrier a step. A step runs three stages
 // at once, so the matrix cores and the vector units both have work: the scores
 // of step j + 1, the softmax of step j and the weights of step j - 1 times V.
-template <int TYPE, int D> __device__ inline void attend_chunk(const attn_args & a, int block, int split, uint8_t * ring) {
+template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const attn_args & a, int block, int split, uint8_t * ring) {
     typedef typename elem<TYPE>::frag frag;
     constexpr int NQ = QT<D>, KS = D / 16, DT = D / 32;
     // ring: [K_RING][D/8][32][8], [V_RING][2][2][D][8]; then the prefix sums
@@ -697,38 +703,39 @@ template <int TYPE, int D> __device__ inline void attend_chunk(const attn_args &
         asm volatile("" : "+v"(window));  // waited for here, not at every use
     };
     look_up(t_first >> ps);
-    // A step's loads: waves 0 and 1 a half of K's rows each, waves 2 and 3 the V
-    // of 16 tokens each. Returns which 16 tokens (bits) have no page. Few
+    // A step's loads: half of the waves make K's, half V's. Returns which 16 tokens (bits) have no page. Few
     // instructions, as a wave makes them every step: a page's address is uniform,
     // a lane's place in it one of the offsets made here.
-    const bool k_wave = wave < 2;
+    constexpr int CW = chunk_waves(D), LOADS = D / (8 * CW);  // loads a wave makes a step
+    const bool k_wave = wave < CW / 2;
+    const int v_first = (wave - CW / 2) * LOADS, v_group = v_first / (D / 32);  // of V's 2 D / 32 loads, and their 16 tokens
     const uint32_t page_bytes = (uint32_t) a.c.page_bytes;
     const uint32_t ring_at = (uint32_t) (uintptr_t) (lds_ptr_t) ring, v_ring_at = ring_at + K_RING * (STEP_BYTES<D> / 2);
     const uint8_t * const part = a.c.pool + (int64_t) h * (4 * P * D) + (k_wave ? 0 : 2 * P * D);
-    uint32_t offset[D / 32];
+    uint32_t offset[LOADS];
 #pragma unroll
-    for (int i = 0; i < D / 32; i++)
-        offset[i] = k_wave ? col * 16 + (wave * (D / 16) + half + 2 * i) * (P * 16) : lane * 16 + i * 1024 + (wave - 2) * (32 * D);
+    for (int i = 0; i < LOADS; i++)
+        offset[i] = k_wave ? col * 16 + (2 * (wave * LOADS + i) + half) * (P * 16) : lane * 16 + (v_first + i) * 1024;
     auto load_step = [&](int j, int k_slot, int v_slot) -> uint32_t {
         if (j >= n) return 0;
         const int32_t t0 = t_first + j * GROUP;
         if (((t0 + 16) >> ps) - at_col >= 64) look_up(t0 >> ps);
         const int c0 = (t0 >> ps) - at_col;
-        const uint32_t to = (k_wave ? ring_at + k_slot * (STEP_BYTES<D> / 2) + wave * (D / 32) * 1024
-                                    : v_ring_at + v_slot * (STEP_BYTES<D> / 2) + (wave - 2) * (D / 32) * 1024);
+        const uint32_t to = (k_wave ? ring_at + k_slot * (STEP_BYTES<D> / 2) + wave * LOADS * 1024
+                                    : v_ring_at + v_slot * (STEP_BYTES<D> / 2) + v_first * 1024);
         const uint8_t * from = part + (uint64_t) (uint32_t) __builtin_amdgcn_readlane(window, c0) * page_bytes;
         uint32_t gone = absent >> c0 & 1 ? 3 : 0;
         if (ps == 4) {  // two pages a step
             const uint8_t * second = part + (uint64_t) (uint32_t) __builtin_amdgcn_readlane(window, c0 + 1) * page_bytes;
             gone = (uint32_t) (absent >> c0) & 3;
-            const uint8_t * mine = k_wave ? (lane & 16 ? second - 256 : from) : wave == 3 ? second - 32 * D : from;
+            const uint8_t * mine = k_wave ? (lane & 16 ? second - 256 : from) : v_group ? second - 32 * D : from;
 #pragma unroll
-            for (int i = 0; i < D / 32; i++)
+            for (int i = 0; i < LOADS; i++)
                 __builtin_amdgcn_global_load_lds((global_ptr_t) (mine + offset[i]), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
         } else {
             from += (t0 & (P - 1)) * (k_wave ? 16 : 2 * D);
 #pragma unroll
-            for (int i = 0; i < D / 32; i++)
+            for (int i = 0; i < LOADS; i++)
                 __builtin_amdgcn_global_load_lds((global_ptr_t) (from + offset[i]), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
         }
         return gone;
@@ -858,7 +865,7 @@ template <int TYPE, int D> __device__ inline void attend_chunk(const attn_args &
     // j + 2 may not be) and its reads of step j - 1's scores and weights done;
     // past it, every wave's. Whether step j is masked.
     auto enter = [&](int j) {
-        if (j + 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(D / 32) : "memory");
+        if (j + 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -981,7 +988,7 @@ template <int TYPE, int D> __device__ inline void attend_chunk(const attn_args &
 
 // Joins the splits of attend_chunk's column tiles, in their order: a workgroup a
 // tile of 32 columns, a thread four values of each of its 32-row blocks.
-template <int D> __device__ inline void combine_chunk(const attn_args & a, int block, int32_t * attn_sh) {
+template <int D> __device__ __forceinline__ void combine_chunk(const attn_args & a, int block, int32_t * attn_sh) {
     const zest::seq_index index(a.b, a.c.page_shift, attn_sh, [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
     constexpr int PARTS = CHUNK<D> / 32;
     const int part = block % PARTS, at = block / PARTS, h = at % a.c.kv_heads, tile = at / a.c.kv_heads;
@@ -1036,7 +1043,8 @@ template <int D> __device__ inline void combine_chunk(const attn_args & a, int b
 // then the others: a batch that holds both runs them side by side. NT 0: none of
 // few columns.
 template <int TYPE, int D, int NT, bool CHUNKS>
-__global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void attn_kernel(attn_args a) {
+__global__ __launch_bounds__((CHUNKS ? chunk_waves(D) : WAVES) * 64, D > 192 || (D > 128 && !CHUNKS) ? 1 : 2) void attn_kernel(attn_args a) {
+    static_assert(!CHUNKS || NT == 0 || chunk_waves(D) == WAVES, "workgroups of one size");
     extern __shared__ __align__(1024) uint8_t smem[];
     const int chunks = CHUNKS ? a.chunk_blocks * a.chunk_splits : 0;
     if constexpr (CHUNKS)
@@ -1077,15 +1085,16 @@ struct attn_plan {
 
 attn_plan plan_of(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
     attn_plan p{};
-    const int chunk = WAVES * 32;
+    const int chunk = chunk_waves(c->head_dim) * 32;
     const int64_t most = (int64_t) b->max_new * group;  // columns of a sequence
-    const bool chunks = most > MOST_SPLIT_COLS;
+    const int few_cols = most_few_cols(4.0 * b->seqs * b->max_len * c->kv_heads * c->head_dim);
+    const bool chunks = most > few_cols;
     // one sequence alone is a chunk whatever its length turns out to be
-    p.chunk_cols = !chunks ? 0x7fffffff : b->seqs == 1 ? 0 : MOST_SPLIT_COLS;
+    p.chunk_cols = !chunks ? 0x7fffffff : b->seqs == 1 ? 0 : few_cols;
     if (chunks) {
         p.chunk_tiles = std::min<int64_t>((b->rows * group + chunk - 1) / chunk + b->seqs, (most + chunk - 1) / chunk * b->seqs);
         const int64_t items = p.chunk_tiles * c->kv_heads, steps = std::max<int64_t>(1, b->max_len / GROUP);
-        p.chunk_splits = (int) std::max<int64_t>(1, std::min<int64_t>({2 * CUS / items, steps / 8, 64}));
+        p.chunk_splits = (int) std::max<int64_t>(1, std::min<int64_t>({(c->head_dim <= 128 ? 2 : 1) * CUS / items, steps / 8, 64}));
     }
     if (p.chunk_cols > 0) {
         const int64_t cols = std::min<int64_t>(most, p.chunk_cols);
@@ -1119,8 +1128,8 @@ template <int TYPE, int D, int NT, bool CHUNKS> int launch(attn_args & a, const 
     const size_t prefix = zest::seq_index_bytes(a.b.seqs);
     if (const int st = allow_lds<&attn_kernel<TYPE, D, NT, CHUNKS>>(ring)) return st;
     a.chunk_blocks = (int32_t) (p.chunk_tiles * a.c.kv_heads);
-    hipLaunchKernelGGL((attn_kernel<TYPE, D, NT, CHUNKS>), dim3((unsigned) (a.chunk_blocks * p.chunk_splits + p.workgroups)),
-                       dim3(WAVES * 64), ring + prefix, s, a);
+    hipLaunchKernelGGL((attn_kernel<TYPE, D, NT, CHUNKS>), dim3((unsigned) (a.chunk_blocks * p.chunk_splits + (NT ? p.workgroups : 0))),
+                       dim3((CHUNKS ? chunk_waves(D) : WAVES) * 64), ring + prefix, s, a);
     // a run of one unit is never split, nor a chunk of one part
     constexpr int few_parts = NT ? COMBINE_PARTS<D, NT> : 1;
     const bool join_few = NT && p.run > 1, join_chunks = CHUNKS && p.chunk_splits > 1;
@@ -1134,7 +1143,15 @@ template <int TYPE, int D, int NT, bool CHUNKS> int launch(attn_args & a, const 
 }
 
 template <int TYPE, int D> int launch(attn_args & a, const attn_plan & p, hipStream_t s) {
-    if (p.chunk_tiles) return p.workgroups ? launch<TYPE, D, 2, true>(a, p, s) : launch<TYPE, D, 0, true>(a, p, s);
+    if (p.chunk_tiles && p.workgroups) {
+        if constexpr (chunk_waves(D) == WAVES) return launch<TYPE, D, 2, true>(a, p, s);
+        attn_plan few = p;
+        few.chunk_tiles = 0;
+        few.chunk_splits = 0;
+        if (const int st = launch<TYPE, D, 0, true>(a, p, s)) return st;
+        return launch<TYPE, D, 2, false>(a, few, s);
+    }
+    if (p.chunk_tiles) return launch<TYPE, D, 0, true>(a, p, s);
     return p.cols == 16 ? launch<TYPE, D, 1, false>(a, p, s) : launch<TYPE, D, 2, false>(a, p, s);
 }
 
