@@ -858,7 +858,6 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (n > 0) scores(0, s_cur);
     bool masked_before = false;
     uint32_t gone_before = 0, gone = 0;
     // The barrier of step j: this wave's loads of step j + 1 are there (those of
@@ -897,6 +896,16 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
         k_at = k_at == K_RING - 1 ? 0 : k_at + 1;
         v_at = v_at == V_RING - 1 ? 0 : v_at + 1;
     };
+    if (w0 >= ncols) {  // none of the tile's columns: this wave only loads
+        for (int32_t j = 0; j < n; j++) {
+            enter(j);
+            k_at = k_at == K_RING - 1 ? 0 : k_at + 1;
+            v_at = v_at == V_RING - 1 ? 0 : v_at + 1;
+        }
+        if (bad) zest::report(a.b.bad);
+        return;
+    }
+    if (n > 0) scores(0, s_cur);
     auto k_next = [&]() { return k_at == K_RING - 1 ? 0 : k_at + 1; };
     auto v_last = [&]() { return v_at == 0 ? V_RING - 1 : v_at - 1; };
     int32_t j = 0;
@@ -1039,21 +1048,22 @@ template <int D> __device__ __forceinline__ void combine_chunk(const attn_args &
 
 // ---- the kernels ----------------------------------------------------------------------
 
-// The chunks' workgroups (a.chunk_blocks of them, each in a.chunk_splits parts),
-// then the others: a batch that holds both runs them side by side. NT 0: none of
-// few columns.
+// The workgroups of few columns, then the chunks' (a.chunk_blocks of them, each in
+// a.chunk_splits parts). A batch that holds both runs them side by side, one of
+// the first a CU, as long as they last: they wait for memory while the others
+// multiply. NT 0: none of few columns.
 template <int TYPE, int D, int NT, bool CHUNKS>
 __global__ __launch_bounds__((CHUNKS ? chunk_waves(D) : WAVES) * 64, D > 192 || (D > 128 && !CHUNKS) ? 1 : 2) void attn_kernel(attn_args a) {
     static_assert(!CHUNKS || NT == 0 || chunk_waves(D) == WAVES, "workgroups of one size");
     extern __shared__ __align__(1024) uint8_t smem[];
-    const int chunks = CHUNKS ? a.chunk_blocks * a.chunk_splits : 0;
+    const int few = gridDim.x - (CHUNKS ? a.chunk_blocks * a.chunk_splits : 0);
     if constexpr (CHUNKS)
-        if ((int) blockIdx.x < chunks) {
-            const int split = blockIdx.x / a.chunk_blocks;
-            attend_chunk<TYPE, D>(a, blockIdx.x - split * a.chunk_blocks, split, smem);
+        if ((int) blockIdx.x >= few) {
+            const int at = blockIdx.x - few, split = at / a.chunk_blocks;
+            attend_chunk<TYPE, D>(a, at - split * a.chunk_blocks, split, smem);
             return;
         }
-    if constexpr (NT > 0) attend_few<TYPE, D, NT>(a, blockIdx.x - chunks, gridDim.x - chunks, smem);
+    if constexpr (NT > 0) attend_few<TYPE, D, NT>(a, blockIdx.x, few, smem);
 }
 
 template <int D, int NT, bool CHUNKS> __global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
@@ -1093,8 +1103,22 @@ attn_plan plan_of(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
     p.chunk_cols = !chunks ? 0x7fffffff : b->seqs == 1 ? 0 : few_cols;
     if (chunks) {
         p.chunk_tiles = std::min<int64_t>((b->rows * group + chunk - 1) / chunk + b->seqs, (most + chunk - 1) / chunk * b->seqs);
-        const int64_t items = p.chunk_tiles * c->kv_heads, steps = std::max<int64_t>(1, b->max_len / GROUP);
-        p.chunk_splits = (int) std::max<int64_t>(1, std::min<int64_t>({(c->head_dim <= 128 ? 2 : 1) * CUS / items, steps / 8, 64}));
+        // A tile's keys in the number of splits that keeps the CUs evenly busy:
+        // rounds of workgroups times a split's steps, and the join's launch and
+        // traffic (a step takes about 1.2 us, in which 6 MB are written or read
+        // again). One sequence of 2048 tokens at 8192, 24 heads of 256: 384 tiles
+        // on 256 CUs, in one part each 674 us, in two 566.
+        const int64_t tiles = std::min<int64_t>(p.chunk_tiles, ((b->rows + b->seqs - 1) / b->seqs * group + chunk - 1) / chunk * b->seqs);
+        const int64_t items = tiles * c->kv_heads, steps = b->max_len / GROUP + 1, slots = (c->head_dim <= 128 ? 2 : 1) * CUS;
+        const double part = 8.0 * chunk * c->head_dim / 6e6;
+        double best = 0;
+        for (int64_t n = 1; n <= 64 && (n == 1 || (n <= steps / 8 && p.chunk_tiles * c->kv_heads * n <= 4 * slots)); n++) {
+            const double cost = (double) ((items * n + slots - 1) / slots) * steps / n + (n > 1 ? 6.0 + part * items * n : 0.0);
+            if (n == 1 || cost < best) {
+                best = cost;
+                p.chunk_splits = (int) n;
+            }
+        }
     }
     if (p.chunk_cols > 0) {
         const int64_t cols = std::min<int64_t>(most, p.chunk_cols);
@@ -1102,7 +1126,7 @@ attn_plan plan_of(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
         p.run = std::max<int64_t>(1, ((int64_t) b->max_len + GROUP + UNIT - 1) / UNIT);
         const int64_t tiles = std::min<int64_t>((b->rows * group + p.cols - 1) / p.cols + b->seqs, (cols + p.cols - 1) / p.cols * b->seqs);
         p.units = p.run * tiles * c->kv_heads;
-        p.workgroups = (int) std::min<int64_t>(p.units, c->head_dim <= 128 ? 2 * CUS : CUS);
+        p.workgroups = (int) std::min<int64_t>(p.units, c->head_dim <= 128 && !chunks ? 2 * CUS : CUS);
     }
     p.partial_bytes = (size_t) 2 * p.workgroups * partial_floats(p.cols, c->head_dim) * sizeof(float);
     p.bytes = p.partial_bytes;
@@ -1191,7 +1215,7 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
     ZEST_REQUIRE(batch->rows * (int64_t) (q_heads / cache->kv_heads) < (1ll << 31) - 64, "%s: %lld rows of %d heads", me,
                  (long long) batch->rows, q_heads);
     const attn_plan plan = plan_of(cache, batch, q_heads / cache->kv_heads);
-    ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads < (1ll << 23), "%s: a batch of %lld units of work",
+    ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads * std::max(1, plan.chunk_splits) < (1ll << 23), "%s: a batch of %lld units of work",
                  me, (long long) std::max(plan.units, plan.chunk_tiles));
     const size_t need = plan.bytes;
     ZEST_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need,
