@@ -529,6 +529,36 @@ def sustain_summary(phases_log: str, smi_log: str) -> int:
     return 0
 
 
+def attention_stack(args) -> int:
+    """The workload's prompt with attention (the paged cache's append and attention in every layer) beside the same
+    stack without it."""
+    import torch
+    z = load_pkg()
+    from ggml_xdna_amd.stack import CONFIGS, Stack
+    torch.cuda.set_device(0)
+    z.init(0)
+    cfg, ms = CONFIGS[args.workload], {}
+    for attention in (True, False):
+        stack = Stack(cfg, seed=0, chunk=args.chunk, attention=attention)
+        for _ in range(args.warmup):
+            stack.run_prompt()
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for _ in range(args.steps):
+            stack.run_prompt()
+        torch.cuda.synchronize()
+        ms[attention] = (time.perf_counter() - t0) * 1e3 / args.steps
+        chunk = stack.chunk
+        del stack
+    pairs = cfg.tokens * (cfg.tokens + 1) / 2  # each token sees those up to its own
+    print(json.dumps({"workload": f"{cfg.name} stack with attention: {cfg.layers} layers, {cfg.tokens}-token prompt in {chunk}-token "
+                                  "chunks, bf16 cache in pages of 64", "ms_per_step": round(ms[True], 3),
+                      "ms_per_step_without": round(ms[False], 3), "tok_per_s": round(cfg.tokens / ms[True] * 1e3, 1),
+                      "attention_tflop": round(4.0 * pairs * cfg.q * cfg.layers / 1e12, 2), "steps": args.steps,
+                      "data": "synthetic"}), flush=True)
+    return 0
+
+
 CALIB_FLOATS = 64 << 20  # the calibration kernel's floats: 256 MiB each way
 
 
@@ -707,6 +737,7 @@ def main() -> int:
     ap.add_argument("--chunk", type=int, default=None, help="tokens per chunk (default: the workload's)")
     ap.add_argument("--traffic-probe", action="store_true", help="one step and the calibration kernel, for rocprofv3")
     ap.add_argument("--traffic-summary", nargs=2, metavar=("FETCH_DIR", "WRITE_DIR"))
+    ap.add_argument("--attention", action="store_true", help="the stack with attention over a paged cache, beside it without")
     ap.add_argument("--hbm", action="store_true", help="HBM rates of the converter (every type) and the pack")
     ap.add_argument("--kernel-configs", action="store_true",
                     help="BASELINE configs 1 and 2: one Q8_0 MUL_MAT and the SwiGLU FFN triple, launch by launch")
@@ -741,6 +772,8 @@ def main() -> int:
         return counter_summary(args)
     if args.traffic_summary:
         return traffic_summary(*args.traffic_summary)
+    if args.attention:
+        return attention_stack(args)
     if args.traffic_probe:
         return traffic_probe(args)
     if args.gpus != 1:

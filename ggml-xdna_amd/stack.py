@@ -11,7 +11,10 @@ A layer, for one chunk of M tokens with residual stream h [M][H] (fp32):
                                                     (xdna-exec's find_fusions)
     h = h + GEMM(., Wdown)
 With fused=False the gate and up are two GEMMs and the SwiGLU its own kernel,
-as for a GLU that cannot be fused.
+as for a GLU that cannot be fused. With attention=True a chunk's q and k are
+turned and its k and v appended to a paged cache (kv.append), and O's input is
+their attention over all of the prompt so far (kv.attention), fp32 rows packed
+as Q's output is without it.
 Weights are random-init N(0, 0.02), quantised to GGUF on the GPU, converted
 once into the resident bfp16 cache (timed separately, as the reference
 reports warm prefill with its one-time copy build apart).
@@ -21,7 +24,7 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 
 import ggml_xdna_amd as z
-from ggml_xdna_amd import quant
+from ggml_xdna_amd import kv, quant
 
 BF16_PEAK_TFLOPS = 2516.6  # MI355X dense bf16 MFMA: 256 CU x 2.4 GHz x 4096 FLOP/clk
 HBM_PEAK_GBS = 8000.0
@@ -43,6 +46,8 @@ class StackConfig:
     chunk: int        # tokens per chunk
     outlier_frac: float = 0.0
     outlier_scale: float = 1.0
+    head_dim: int = 128
+    rope_base: float = 1e6
 
     def matmuls(self):
         """(name, N, K, type) of one layer's weights."""
@@ -61,7 +66,7 @@ CONFIGS = {
                             z.TYPE_Q8_0, 8192, 2048),
     # hidden 1024, 16 layers, Q8_0, chunk swept by the caller
     "small-1024": StackConfig("small-1024", 16, 1024, 1024, 1024, 4096, z.TYPE_Q8_0, z.TYPE_Q8_0, z.TYPE_Q8_0,
-                              z.TYPE_Q8_0, 4096, 4096),
+                              z.TYPE_Q8_0, 4096, 4096, head_dim=64),
     # 27B-class, 64 layers, all Q4_K, one 4096-token chunk, 0.5% outliers x30
     "dense-27b": StackConfig("dense-27b", 64, 5120, 6144, 1024, 17408, z.TYPE_Q4_K, z.TYPE_Q4_K, z.TYPE_Q4_K,
                              z.TYPE_Q4_K, 4096, 4096, 0.005, 30.0),
@@ -78,9 +83,10 @@ class Layer:
 class Stack:
     """Weights resident in HBM plus per-chunk work buffers."""
 
-    def __init__(self, cfg: StackConfig, seed: int = 0, device: str = "cuda", fused: bool = True, chunk=None):
+    def __init__(self, cfg: StackConfig, seed: int = 0, device: str = "cuda", fused: bool = True, chunk=None,
+                 attention: bool = False):
         import torch
-        self.cfg, self.device, self.fused = cfg, device, fused
+        self.cfg, self.device, self.fused, self.attention = cfg, device, fused, attention
         g = torch.Generator(device=device)
         g.manual_seed(seed)
         self.layers: list[Layer] = []
@@ -144,6 +150,16 @@ class Stack:
         # the matmuls' activation operands (the bfp16 pack, expanded)
         self.pa = z.empty_act(m, c.hidden, dev)
         self.po = z.empty_act(m, c.q, dev)
+        if self.attention:
+            # one sequence of up to `tokens` tokens in slot 0, its pages taken from the pool as chunks arrive
+            page = 64
+            self.ao = torch.empty((m, c.q), **f32)
+            self.cache = kv.empty_cache(c.layers, -(-c.tokens // page), c.kv // c.head_dim, c.head_dim, page, slots=1, device=dev)
+            freqs, mag = kv.rope_freqs(c.head_dim, c.rope_base)
+            self.rope = kv.Rope(torch.tensor(freqs, dtype=torch.float64, device=dev), kv.ROPE_NEOX, mag)
+            one = lambda v: torch.tensor([v], dtype=torch.int32, device=dev)  # noqa: E731
+            self.slot, self.none = one(0), one(-1)
+            self.batches = {}  # of each chunk size: its rows, and the tokens the sequence grows by
         self.pd = z.empty_act(m, c.ffn, dev)
 
     def run_chunk(self, x_chunk, gemm_events=None):
@@ -157,6 +173,12 @@ class Stack:
         h, qo, ko, vo = (t[:m] for t in (self.h, self.qo, self.ko, self.vo))
         go, uo = (self.go[:m], self.uo[:m]) if not self.fused else (None, None)
         h.copy_(x_chunk)
+        if self.attention:
+            if m not in self.batches:
+                rows = torch.tensor([0, m], dtype=torch.int32, device=self.device)
+                self.batches[m] = kv.Batch(rows, m, m, c.tokens), rows[1:].clone()
+            batch, grow = self.batches[m]
+            kv.assign(self.cache, self.slot, self.slot, grow)
 
         def timed(fn, flops):
             if gemm_events is None:
@@ -171,13 +193,16 @@ class Stack:
         def gemm(a, wname, L, n, k, out):
             timed(lambda: z.gemm(a, m, L.w[wname], n, k, out=out), 2.0 * m * n * k)
 
-        for L in self.layers:
+        for li, L in enumerate(self.layers):
             z.rms_norm(h, eps, L.attn_norm, y=None, packed=self.pa)
             # q, k and v share their input: one launch (the reference's group)
             timed(lambda: z.gemm_group(self.pa, m, [L.w["attn_q"], L.w["attn_k"], L.w["attn_v"]],
                                        [c.q, c.kv, c.kv], c.hidden, outs=[qo, ko, vo]),
                   2.0 * m * (c.q + 2 * c.kv) * c.hidden)
-            z.pack_act_x(qo, out=self.po)
+            if self.attention:
+                q = kv.append(self.cache, li, batch, ko, vo, q=qo, rope=self.rope)
+                kv.attention(self.cache, li, batch, q, out=self.ao[:m])
+            z.pack_act_x(self.ao[:m] if self.attention else qo, out=self.po)
             timed(lambda: z.gemm_residual(self.po, m, L.w["attn_output"], c.hidden, c.q, h, out=h),
                   2.0 * m * c.hidden * c.q)
             z.rms_norm(h, eps, L.ffn_norm, y=None, packed=self.pa)
@@ -220,5 +245,7 @@ class Stack:
         return n, flops
 
     def run_prompt(self, gemm_events=None):
+        if self.attention:  # a prompt of its own: the sequence before it ends
+            kv.assign(self.cache, self.slot, self.none, self.none + 1)
         for t0 in range(0, self.cfg.tokens, self.chunk):
             self.run_chunk(self.x[t0:t0 + self.chunk], gemm_events)

@@ -481,16 +481,17 @@ def test_the_operators_together(kv):
         for layer in (0, 1):
             qt = kv.append(c, layer, b, k.cuda(), v.cuda(), q.cuda(), rope)
         got = kv.attention(c, 1, b, qt, out_dtype=F32).cpu()
+        pool, tables = c.pool.cpu(), c.tables.cpu()
         for s, n, r in zip(slots, news, starts):
-            k0, v0 = kept.get(s, (torch.zeros(0, kvh, d).to(BF16),) * 2)
+            k0, v0 = kept.get(s, (torch.zeros(0, kvh, d, dtype=torch.float64),) * 2)
             place = np.arange(len(k0), len(k0) + n)
-            kk = torch.cat([k0, kv_ref.rope(k[r:r + n], place, freqs, 2, 1.0).to(BF16)])
-            vv = torch.cat([v0, v[r:r + n].to(BF16)])
-            kept[s] = kk, vv
-            out, spread, reach = kv_ref.attention(qt[r:r + n].cpu(), kk, vv, 0.125)
-            # the kept k may round the other way where sine and cosine in fp32 move it past a tie: one step more of a score
-            bound = kv_ref.attention_bound(out, spread, reach, d, BF16, F32) + 2 * 2.0 ** -7 * reach / 64 * spread
-            assert bool(((got[r:r + n].double() - out).abs() <= bound).all()), (s, n)
+            kept[s] = torch.cat([k0, kv_ref.rope(k[r:r + n], place, freqs, 2, 1.0)]), torch.cat([v0, v[r:r + n].double()])
+            # what the cache holds of all of the sequence: each value rounded once, wherever its pages have been since
+            held = kv_ref.read_cache(pool, tables[s], len(kept[s][0]), page, d, layer=1)
+            for h, want in zip(held, kept[s]):
+                assert bool(((h.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -22 * 8).all()), (s, n)
+            out, spread, reach = kv_ref.attention(qt[r:r + n].cpu(), *held, 0.125)
+            assert bool(((got[r:r + n].double() - out).abs() <= kv_ref.attention_bound(out, spread, reach, d, BF16, F32)).all()), (s, n)
 
     tokens([0], [37])
     tokens([0, 2], [20, 9])
@@ -503,3 +504,48 @@ def test_the_operators_together(kv):
     assert live == sum(-(-len(kept[s][0]) // page) for s in kept) == int((c.refs > 0).sum()) and int(c.tables.max()) == live - 1
     tokens([3, 1], [30, 2])
     tokens([1], [1])
+
+
+def test_stack_with_attention(kv):
+    """The stack runner's layers with attention, a prompt in chunks (the last one ragged) and then another: every chunk's
+    O input against attention in 64 bits over the keys and values that the layer's own matmuls gave."""
+    from ggml_xdna_amd import stack
+    cfg = stack.StackConfig("tiny", 2, 256, 256, 128, 512, 8, 8, 8, 8, 300, 128, head_dim=64, rope_base=1e4)
+    s = stack.Stack(cfg, seed=1, attention=True)
+    freqs, _ = kv.rope_freqs(64, 1e4)
+    seen = []
+    plain_append, plain_attention = kv.append, kv.attention
+
+    def append(cache, layer, batch, k, v, **more):
+        q = plain_append(cache, layer, batch, k, v, **more)
+        seen.append((layer, k.clone().cpu(), v.clone().cpu(), q.clone().cpu()))
+        return q
+
+    def attention(cache, layer, batch, q, **more):
+        out = plain_attention(cache, layer, batch, q, **more)
+        seen[-1] += (out.clone().cpu(),)
+        return out
+
+    try:
+        kv.append, kv.attention = append, attention
+        s.run_prompt()
+        first = s.h[:44].clone()
+        s.run_prompt()
+        assert torch.equal(s.h[:44], first)  # a prompt starts anew
+    finally:
+        kv.append, kv.attention = plain_append, plain_attention
+    # the second prompt's keys and values are still in the cache: token t of every chunk's attention
+    pool, tables = s.cache.pool.cpu(), s.cache.tables.cpu()
+    done = {0: 0, 1: 0}
+    for layer, k, v, q, out in seen[6:]:
+        n = len(k)
+        place = np.arange(done[layer], done[layer] + n)
+        done[layer] += n
+        held = kv_ref.read_cache(pool, tables[0], done[layer], 64, 64, layer)
+        turned = kv_ref.rope(k.view(n, 2, 64), place, freqs, 2, 1.0)
+        assert bool(((held[0][-n:].double() - turned).abs() <= 2.0 ** -8 * turned.abs() + 2.0 ** -22 * 8).all())
+        assert torch.equal(held[1][-n:], v.view(n, 2, 64).to(BF16))
+        want, spread, reach = kv_ref.attention(q.view(n, 4, 64), *held, 0.125)
+        bound = kv_ref.attention_bound(want, spread, reach, 64, BF16, F32)
+        assert bool(((out.view(n, 4, 64).double() - want).abs() <= bound).all())
+    assert [len(x[1]) for x in seen[:6:2]] == [128, 128, 44] and len(seen) == 12
