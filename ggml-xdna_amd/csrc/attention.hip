@@ -290,6 +290,7 @@ __device__ __forceinline__ void attend_few(const attn_args & a, int block, int b
         const int last_row = (min(ncols, c0 + COLS) - 1) / a.group;
         seen_by(a, s, last_row, last_row, all_lo, any_hi);
         seen_by(a, s, 0, s.n - 1, seq_lo, seq_hi);
+        const int32_t from = seq_lo;  // 16 tokens before it need no page: a window may have left them
         seq_lo &= ~(GROUP - 1);
 
         // this wave's steps: tokens t_first + j * UNIT .. + 31, j < n
@@ -304,7 +305,7 @@ __device__ __forceinline__ void attend_few(const attn_args & a, int block, int b
             for (int g = 0; g < 2; g++) {
                 const int32_t t = t_first + j * UNIT + 16 * g;
                 id[g] = 0;
-                if (j < n && t < any_hi) {
+                if (j < n && t < any_hi && t + 16 > from) {
                     const int32_t x = load_uniform(row + (t >> ps));
                     if ((uint32_t) x < (uint32_t) a.c.pages) {
                         id[g] = x;
@@ -662,6 +663,7 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
     // the tile's tokens, and of them this split's
     int32_t lo, hi;
     seen_by(a, s, c0 / a.group, min(ncols - 1, c0 + CHUNK<D> - 1) / a.group, lo, hi);
+    const int32_t from = lo;  // pages wholly before it are not wanted: a window may have left them
     lo &= ~(GROUP - 1);
     const int32_t steps = (hi - lo + GROUP - 1) / GROUP;
     const int32_t first = (int32_t) ((int64_t) steps * split / a.chunk_splits);
@@ -694,7 +696,7 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
     int32_t at_col = 0;
     auto look_up = [&](int col0) {
         at_col = col0;
-        const bool wanted = ((int64_t) (col0 + lane) << ps) < t_hi;
+        const bool wanted = ((int64_t) (col0 + lane) << ps) < t_hi && ((int64_t) (col0 + lane + 1) << ps) > from;
         window = wanted ? (uint32_t) row[col0 + lane] : 0xffffffffu;
         const bool there = window < (uint32_t) a.c.pages;
         absent = __ballot(!there);
@@ -1215,7 +1217,7 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
     ZEST_REQUIRE(batch->rows * (int64_t) (q_heads / cache->kv_heads) < (1ll << 31) - 64, "%s: %lld rows of %d heads", me,
                  (long long) batch->rows, q_heads);
     const attn_plan plan = plan_of(cache, batch, q_heads / cache->kv_heads);
-    ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads * std::max(1, plan.chunk_splits) < (1ll << 23), "%s: a batch of %lld units of work",
+    ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads * std::max(1, plan.chunk_splits) < (1ll << 22), "%s: a batch of %lld units of work",
                  me, (long long) std::max(plan.units, plan.chunk_tiles));
     const size_t need = plan.bytes;
     ZEST_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need,

@@ -30,7 +30,7 @@ int kv_check_batch(const zest_kv_cache * c, const zest_kv_batch * b, const char 
     ZEST_REQUIRE(b->table_rows > 0 && b->table_cols > 0 && (int64_t) b->table_cols * c->page_tokens < (1ll << 31),
                  "%s: page tables of %d x %d", what, b->table_rows, b->table_cols);
     ZEST_REQUIRE(b->slots || b->seqs <= b->table_rows, "%s: %d sequences of %d slots", what, b->seqs, b->table_rows);
-    ZEST_REQUIRE(b->max_new > 0 && b->max_new <= b->rows && b->max_len >= 0, "%s: max_new=%d max_len=%d of %lld rows", what,
+    ZEST_REQUIRE(b->max_new > 0 && b->max_new <= b->rows && b->max_len >= 0 && b->max_len <= (1 << 30), "%s: max_new=%d max_len=%d of %lld rows", what,
                  b->max_new, b->max_len, (long long) b->rows);
     return ZEST_OK;
 }
@@ -312,8 +312,11 @@ constexpr int STEP = 1024;  // threads of the one workgroup that walks the table
 // the vector cache.
 __device__ inline int32_t fresh(const int32_t * p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// Exclusive scan of one value a thread over a 1024-thread workgroup; *total its
-// sum. Ends in a barrier.
+// Exclusive scan of one value a thread (0 to MOST) over a 1024-thread workgroup;
+// *total its sum. Sums stop at MOST, more than any pool has pages, so that no
+// list of wishes wraps around. Ends in a barrier.
+constexpr int32_t MOST = 1 << 29;
+
 __device__ inline int32_t scan_step(int32_t v, int32_t * total) {
     __shared__ int32_t sums[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -321,19 +324,20 @@ __device__ inline int32_t scan_step(int32_t v, int32_t * total) {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
         const int32_t u = __shfl_up(s, off);
-        if (lane >= off) s += u;
+        if (lane >= off) s = min(s + u, MOST);
     }
     if (lane == 63) sums[wave] = s;
     __syncthreads();
     int32_t before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < 16; w++) {
-        before += w < wave ? sums[w] : 0;
-        all += sums[w];
+        before = min(before + (w < wave ? sums[w] : 0), MOST);
+        all = min(all + sums[w], MOST);
     }
     __syncthreads();
     *total = all;
-    return before + s - v;
+    const int32_t left = __shfl_up(s, 1);
+    return min(before + (lane ? left : 0), MOST);
 }
 
 // An entry between the phases of assign_kernel (base -1: left undone).
@@ -395,15 +399,15 @@ __global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
                 if (base >= 0 && base + g <= room && old >= 0 && old <= room) {
                     e.base = (int32_t) base;
                     const int32_t held = (int32_t) (s == d ? (base + P - 1) >> a.page_shift : base >> a.page_shift);
-                    e.need = (int32_t) ((base + g + P - 1) >> a.page_shift) - held;
+                    e.need = min((int32_t) ((base + g + P - 1) >> a.page_shift) - held, MOST);
                     e.old_pages = s == d ? 0 : (int32_t) ((old + P - 1) >> a.page_shift);
                 }
             }
             bad |= e.base < 0;
         }
         int32_t sum;
-        e.first = want + scan_step(e.need, &sum);
-        want += sum;
+        e.first = min(want + scan_step(e.need, &sum), MOST);
+        want = min(want + sum, MOST);
         if (i < a.n) {
             entries[i] = e;
             a.copies[i] = make_int2(-1, -1);

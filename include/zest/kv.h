@@ -54,7 +54,8 @@ typedef struct {
     int64_t rows;          /* rows of q, k, v and the output, 1 .. 2^27 */
     int32_t seqs;          /* 1 .. 4096 */
     int32_t table_rows, table_cols;
-    int32_t max_new, max_len;
+    int32_t max_new;       /* 1 .. rows */
+    int32_t max_len;       /* 0 .. 2^30 */
 } zest_kv_batch;
 
 /* Rotary positions: pair p of the first n_dims of a head turns by position *
@@ -105,7 +106,8 @@ ZEST_API int zest_kv_append(const zest_kv_cache *cache, const zest_kv_batch *bat
  * whole sequence (an encoder's states: lens need not hold the rows). A row that
  * sees no token, or only scores of -infinity, is zero. Tokens that a row does
  * not see, and places behind len, do not reach it whatever they hold (NaN and
- * infinities too). A page outside the pool counts as unseen and is reported.
+ * infinities too); pages of which no row sees a token may be gone from the table.
+ * A page outside the pool counts as unseen and is reported.
  *
  * q_type and out_type: F32, F16 or BF16; q is rounded to the cache's type (the
  * matrix cores' operand), products and softmax statistics are in 32 bits, the

@@ -77,7 +77,7 @@ def test_entry_points_refuse_bad_arguments_before_the_gpu(kv):
                   (dict(page_tokens=48), E_UNSUPPORTED), (dict(page_tokens=512), E_UNSUPPORTED)]
     bad_batches = [(dict(tables=None), E_ARG), (dict(lens=None), E_ARG), (dict(starts=None), E_ARG), (dict(rows=0), E_ARG), (dict(rows=(1 << 27) + 1), E_ARG),
                    (dict(seqs=0), E_ARG), (dict(seqs=4097, slots=base), E_ARG), (dict(seqs=3), E_ARG), (dict(table_cols=0), E_ARG),
-                   (dict(table_cols=1 << 27), E_ARG), (dict(max_new=0), E_ARG), (dict(max_new=5), E_ARG), (dict(max_len=-1), E_ARG)]
+                   (dict(table_cols=1 << 27), E_ARG), (dict(max_new=0), E_ARG), (dict(max_new=5), E_ARG), (dict(max_len=-1), E_ARG), (dict(max_len=(1 << 30) + 1), E_ARG)]
 
     def append(c=None, b=None, rope=None, in_type=0, k=base, ldk=128, v=base, ldv=128, q=None, ldq=256, heads=4, q_out=None,
                ldo=256, to=0):

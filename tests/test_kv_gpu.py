@@ -207,6 +207,23 @@ def test_bad_device_values_are_left_out_and_reported(kv):
         assert int(bad) == 1 and torch.equal(out[:2], good[:2]) and bool((out[2:4] == 3).all()), (starts, slots, lens)
 
 
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("new", [1, 5, 90])
+def test_pages_that_a_window_has_left_may_be_gone(kv, page, new):
+    """The table's entries of pages before every row's window are -1: nothing is reported, nothing changes."""
+    c = Case(kv, [(new, 400), (1, 3)], page, 1, 2, 64, BF16, seed=new)
+    want = kv.attention(c.cache, 0, c.batch, c.q.cuda(), window=50)
+    first = 400 - new - 50 + 1  # the first token that the first row sees
+    c.cache.tables[0, :first // page] = -1
+    bad = _flag()
+    got = kv.attention(c.cache, 0, c.batch, c.q.cuda(), window=50, bad=bad)
+    assert int(bad) == 0 and torch.equal(got, want)
+    c.check(got, window=50)
+    c.cache.tables[0, first // page] = -1  # the one it does see
+    kv.attention(c.cache, 0, c.batch, c.q.cuda(), window=50, bad=bad)
+    assert int(bad) == 1
+
+
 def test_slots_and_layers(kv):
     """Sequences in any slots of a cache, in a layer past the first."""
     c = Case(kv, [(2, 40), (1, 17), (3, 70)], 16, 2, 2, 64, BF16, seed=12)
@@ -377,6 +394,24 @@ def test_assign_many_entries_and_pages(kv):
     for name, got, w in zip(("tables", "lens", "refs"), (cache.tables, cache.lens, cache.refs), want):
         assert np.array_equal(got.cpu().numpy(), w), name
     assert not copies and torch.equal(cache.pool.cpu(), pool) and int(bad) == int(wrong)
+
+
+def test_assign_wishes_beyond_any_pool(kv):
+    """Growth whose pages, summed over the entries, pass 32 bits: none fits, what needs none is done."""
+    cols, n = 1 << 20, 2200
+    tables = torch.full((n + 1, cols), -1, dtype=torch.int32, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cache = kv.Cache(torch.zeros((1, 8, 1, 2 * 16 * 64), dtype=BF16, device="cuda"), tables, torch.zeros(n + 1, **i32),
+                     torch.zeros(8, **i32), 16, 64)
+    cache.lens[n], cache.tables[n, 0], cache.refs[5] = 3, 5, 1
+    grow = torch.full((n + 1,), 16 * cols, **i32)
+    grow[0], grow[n] = 7 * 16, 4
+    bad = _flag()
+    order = torch.arange(n + 1, **i32)
+    kv.assign(cache, order, order, grow, bad=bad)
+    assert int(bad) == 1 and cache.lens[0] == 112 and cache.lens[n] == 7 and int(cache.lens[1:n].sum()) == 0
+    assert cache.tables[0, :8].tolist() == [0, 1, 2, 3, 4, 6, 7, -1] and cache.refs.tolist() == [1] * 8
+    assert int((tables >= 0).sum()) == 8
 
 
 def test_assign_reports_wrong_counts(kv):
