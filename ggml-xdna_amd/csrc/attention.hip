@@ -1,5 +1,6 @@
 // Attention over the paged KV cache (include/zest/kv.h): one pass over the keys
-// with the running maximum and sum of a softmax, on v_mfma_f32_32x32x16.
+// with the running maximum and sum of a softmax, on v_mfma_f32_32x32x16 (many
+// columns) or 16x16x32 (few).
 //
 // A column is one (new token, query head) pair of a k/v head, token-major: with
 // a group of G query heads column c is token c / G and head c % G of the group,
@@ -253,7 +254,10 @@ constexpr int partial_floats(int cols, int D) { return cols * (D + 2); }
 // ring of its own in shared memory that direct loads fill (16 bytes a lane, whole
 // kilobytes, no registers): K of the step to come is requested as soon as the
 // scores are made, V as soon as it is weighed, and only this wave waits for them,
-// by counting its loads. Eight waves a CU so have 64 to 128 KB in flight.
+// by counting its loads. Eight waves a CU so have 64 to 128 KB in flight: 64
+// sequences of 256 to 8192 tokens, 32 query and 8 k/v heads of 128, 104 us, 535 MB
+// at 5.1 TB/s, where a large copy reaches 5.2 (with K and V loaded to registers
+// 149 us); 4 of 20000 to 40000 with 5 new tokens and 48 heads 102 us.
 //
 // Tiles of 16 columns on v_mfma_f32_16x16x32, NT of them sharing the K and V read:
 // a token's group of query heads rarely fills 32 columns, and half the columns
@@ -608,11 +612,13 @@ template <int D, int NT> __device__ __forceinline__ void combine_few(const attn_
 
 // ---- chunks: many columns ---------------------------------------------------------
 
-// Column tiles of 32 a wave of attend_chunk takes: two where the registers hold
-// them (O^T of 64 columns is D values a lane, Q^T half of that).
-template <int D> constexpr int QT = 1;
+// Column tiles of 32 a wave of attend_chunk takes. Two would need 300 registers of
+// a 128-wide head's wave, which leaves one wave a SIMD.
+constexpr int QT = 1;
+// Waves of a workgroup: eight where the rings leave room for one workgroup a CU
+// and the registers for two waves a SIMD.
 constexpr int chunk_waves(int D) { return D == 192 ? 8 : 4; }
-template <int D> constexpr int CHUNK = chunk_waves(D) * 32 * QT<D>;  // columns of a workgroup
+template <int D> constexpr int CHUNK = chunk_waves(D) * 32 * QT;  // columns of a workgroup
 // Steps of K and of V in shared memory. At step j the scores read K of j + 1 while
 // those of j + 2 and j + 3 are on their way, the weights read V of j - 1.
 constexpr int K_RING = 3, V_RING = 5;
@@ -636,9 +642,21 @@ __device__ inline int32_t chunk_tiles_of(const attn_args & a, const kv_seq & s, 
 // wave), two steps ahead of their use, with one barrier a step. A step runs three stages
 // at once, so the matrix cores and the vector units both have work: the scores
 // of step j + 1, the softmax of step j and the weights of step j - 1 times V.
+//
+// 32 query and 8 k/v heads of 128, the last 2048 of 8192 tokens: 255 us, 945
+// TFLOP/s, where a large library product reaches 1216 on this card. A step of a
+// wave is 16 matrix instructions (512 cycles) and about 150 others; the board's
+// power limit costs 12%, and leaving out the softmax or the loads would save 15%
+// and 12%. On the way: K and V straight to registers, nothing shared, 891 us; one
+// step ahead 289; two steps ahead 282, and without waiting for a page's number in
+// every step and with a third of the address arithmetic 274; scores first in a
+// step 261. Four waves of 32 columns, two workgroups a CU: 64 columns a wave halve
+// the reads of shared memory (a third busy as it is) but leave one wave a SIMD.
+// 192-wide heads take eight waves, one workgroup a CU: with four, a wave a SIMD,
+// 765 us for 24 heads at 8192, with eight 342.
 template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const attn_args & a, int block, int split, uint8_t * ring) {
     typedef typename elem<TYPE>::frag frag;
-    constexpr int NQ = QT<D>, KS = D / 16, DT = D / 32;
+    constexpr int NQ = QT, KS = D / 16, DT = D / 32;
     // ring: [K_RING][D/8][32][8], [V_RING][2][2][D][8]; then the prefix sums
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     const int ps = a.c.page_shift, P = 1 << ps;

@@ -124,7 +124,9 @@ enum { ITEM_PIECE = 0, ITEM_PAIR = 1, ITEM_SINGLE = 2 };
 // there (rint and a subtraction: exact to 2^-53 of the turns), and sine and
 // cosine of that in 32. HBM bound. K's lanes run over tokens first, so a piece
 // row of 16 tokens is 256 contiguous bytes; V's over columns, 8 tokens a lane, so
-// a wave reads whole rows and writes whole lines.
+// a wave reads whole rows and writes whole lines. 2048 tokens of 32 query and 8
+// k/v heads of 128 from fp32: 21.5 us, 75 MB at 3.5 TB/s; a head at a time, its
+// items on half of the threads, 32.5.
 //
 // BATCH 4, and 1 where no sequence has more than one new token: a quarter of the
 // code, whose first fetch is a good part of so small a call (64 sequences of the
@@ -488,7 +490,8 @@ __global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
 
 // Copies n whole pages in every layer, copies[i] = (from, to), -1 for none; by
 // `blocks` workgroups of 256 threads, each COPY_BYTES of a page at a time, four
-// 16-byte loads a thread before the first store.
+// 16-byte loads a thread before the first store. Memory bound: 40 forks' open pages
+// in 36 layers, 755 MB, 113 us, and 3.4 GB in 680 us, at a copy's rate.
 constexpr int COPY_BYTES = 16384;
 
 __device__ inline void copy_pages(uint8_t * pool, int64_t page_bytes, int64_t layer_stride, int32_t layers, const int2 * copies,

@@ -9,7 +9,8 @@
  * Errors: a negative status, with zest_last_error() (thread-local) saying why.
  *
  * Each entry point names the reference interface it replaces (paths in the
- * Cyronius/ggml-xdna tree).
+ * Cyronius/ggml-xdna tree). The paged KV cache and attention over it are in
+ * zest/kv.h.
  */
 #ifndef ZEST_HIP_H
 #define ZEST_HIP_H
