@@ -350,9 +350,11 @@ __device__ __forceinline__ void attend_few(const attn_args & a, int block, int b
 #pragma unroll
         for (int r = 0; r < R; r++) {
             there[r] = pages_of(r, id[r]);
-            if (r < n) {
+            if (r < n) {  // in this order: the waits below count on it
                 load_k(r, id[r]);
+                asm volatile("" ::: "memory");
                 load_v(r, id[r]);
+                asm volatile("" ::: "memory");
             }
         }
 
@@ -723,9 +725,9 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
         asm volatile("" : "+v"(window));  // waited for here, not at every use
     };
     look_up(t_first >> ps);
-    // A step's loads: half of the waves make K's, half V's. Returns which 16 tokens (bits) have no page. Few
-    // instructions, as a wave makes them every step: a page's address is uniform,
-    // a lane's place in it one of the offsets made here.
+    // A step's loads: half of the waves make K's, half V's. Returns which 16 tokens
+    // (bits) have no page. Few instructions, as a wave makes them every step: a
+    // page's address is uniform, a lane's place in it one of the offsets made here.
     constexpr int CW = chunk_waves(D), LOADS = D / (8 * CW);  // loads a wave makes a step
     const bool k_wave = wave < CW / 2;
     const int v_first = (wave - CW / 2) * LOADS, v_group = v_first / (D / 32);  // of V's 2 D / 32 loads, and their 16 tokens

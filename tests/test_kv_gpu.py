@@ -113,6 +113,59 @@ def test_attention_long_chunk(kv):
     c.check(kv.attention(c.cache, 0, c.batch, c.q.cuda()))
 
 
+@pytest.mark.parametrize("d,page,dtype", [(64, 16, F16), (96, 32, BF16), (128, 16, BF16), (128, 64, F16), (192, 16, F16),
+                                          (256, 64, BF16)])
+@pytest.mark.parametrize("seqs", [[(40, 3000)], [(33, 2100), (1, 2500), (50, 1300)]])
+def test_chunks_split_over_their_keys(kv, d, page, dtype, seqs):
+    """Few tiles over long contexts, whose keys are split and joined: tables of more than 64 columns, a page that is not
+    there, NaN and infinities that only some rows see."""
+    c = Case(kv, seqs, page, 2, 4, d, dtype, seed=d)
+    q = c.q.cuda()
+    got = kv.attention(c.cache, 0, c.batch, q)
+    c.check(got)
+    c.check(kv.attention(c.cache, 0, c.batch, q, causal=False), causal=False)
+    c.check(kv.attention(c.cache, 0, c.batch, q, window=700, softcap=20.0), window=700, softcap=20.0)
+    bad = _flag()
+    c.cache.tables[0, 1100 // page] = -1
+    unseen = torch.zeros(seqs[0][1], dtype=torch.bool)
+    unseen[1100 // page * page:1100 // page * page + page] = True
+    c.check(kv.attention(c.cache, 0, c.batch, q, bad=bad), unseen=[unseen] + [None] * (len(seqs) - 1))
+    assert int(bad) == 1
+    # the last tokens of sequence 0 are NaN and infinite: row i sees those up to its own
+    n, m = seqs[0]
+    for t, v in ((m - 5, math.nan), (m - 3, math.inf), (m - 1, -math.inf)):
+        c.book.v[0][t, :, 7] = v
+    c.book.fill()
+    c.cache = c.book.cache(kv)
+    odd = kv.attention(c.cache, 0, c.batch, q).float().cpu()
+    assert torch.equal(odd[:n - 5], got[:n - 5].float().cpu()) and bool(odd[n - 5:n, :, 7].isnan().all())
+    rest = [e for e in range(d) if e != 7]
+    assert torch.equal(odd[..., rest], got.float().cpu()[..., rest])
+
+
+@pytest.mark.parametrize("count", [64, 65, 300, 1100])
+def test_many_sequences(kv, count):
+    """More sequences than a wave's lanes, than a workgroup's threads, than that many each: append and attention of one
+    or a few tokens each (and of a chunk among them), none of a sequence here and there."""
+    rng = np.random.default_rng(count)
+    new = [int(n) for n in rng.choice([0, 1, 1, 1, 2, 3], count)]
+    new[count // 2] = 70
+    lens = [n + int(rng.integers(0, 60)) for n in new]
+    c = Case(kv, list(zip(new, lens)), 16, 1, 2, 64, BF16, seed=count)
+    bad = _flag()
+    c.check(kv.attention(c.cache, 0, c.batch, c.q.cuda(), bad=bad))
+    k, v = (torch.randn((c.rows, 1, 64), generator=torch.Generator().manual_seed(i)) for i in (1, 2))
+    kv.append(c.cache, 0, c.batch, k.cuda(), v.cuda(), bad=bad)
+    assert int(bad) == 0
+    pool, want = c.cache.pool.cpu(), c.book.pool.clone()
+    ki, vi = kv_ref.page_index(16, 64)
+    for b, (n, m, r) in enumerate(zip(new, lens, c.starts)):
+        for i in range(n):
+            held, t = want[0, int(c.book.table[b, (m - n + i) // 16]), 0], (m - n + i) % 16
+            held[ki[t]], held[vi[t]] = k[r + i, 0].to(BF16), v[r + i, 0].to(BF16)
+    assert torch.equal(pool.view(torch.int16), want.view(torch.int16))
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_values_a_row_does_not_see_do_not_reach_it(kv, value, dtype):
