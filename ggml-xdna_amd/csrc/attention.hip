@@ -668,9 +668,12 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
     // once, two a CU, a CU gets one from either end (workgroup i + CUS joins i);
     // else the longest come first.
     const int h = block % a.c.kv_heads, order = block / a.c.kv_heads;
-    int tile = index.total - 1 - order;
+    // no more than the launch and the workspace are for: starts that go back make
+    // sequences overlap (reported), and the tiles more than the rows allow
+    const int total = min(index.total, a.chunk_blocks / a.c.kv_heads);
+    int tile = total - 1 - order;
     if (tile < 0) return;
-    if (index.total * a.c.kv_heads <= 2 * CUS) {
+    if (total * a.c.kv_heads <= 2 * CUS) {
         const int head_start = CUS / a.c.kv_heads;
         if (order >= head_start) tile = order - head_start;
     }

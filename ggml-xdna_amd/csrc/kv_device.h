@@ -79,27 +79,32 @@ template <typename Cost> struct seq_index {
             for (int b = first; b < last; b++) {
                 const int32_t c = cost(load_seq(a, b, page_shift, bad));
                 prefix[b + 1] = c;
-                sum += c;
+                sum = add(sum, c);
             }
             const int32_t s = scan(sum);
             if (lane == 63) wave_sum[t >> 6] = s;
             __syncthreads();
-            int32_t before = s - sum;
-            for (int w = 0; w < (t >> 6); w++) before += wave_sum[w];
+            const int32_t left = __shfl_up(s, 1);
+            int32_t before = lane ? left : 0;
+            for (int w = 0; w < (t >> 6); w++) before = add(before, wave_sum[w]);
             if (t == 0) prefix[0] = 0;
-            for (int b = first; b < last; b++) prefix[b + 1] = before += prefix[b + 1];
+            for (int b = first; b < last; b++) prefix[b + 1] = before = add(before, prefix[b + 1]);
             __syncthreads();
             total = prefix[a.seqs];
         }
         if (bad && blockIdx.x == 0) report(a.bad);
     }
 
+    // Sums stop at the type's limit: starts that go back make sequences overlap, and
+    // their costs no longer keep to what the host bounds by the rows.
+    static __device__ int32_t add(int32_t x, int32_t y) { return __builtin_elementwise_add_sat(x, y); }
+
     static __device__ int32_t scan(int32_t v) {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const int32_t u = __shfl_up(v, off);
-            if (lane >= off) v += u;
+            if (lane >= off) v = add(v, u);
         }
         return v;
     }

@@ -45,7 +45,8 @@ typedef struct {
  * the output, and the last of its lens[slot] tokens: row i of n is token
  * lens[slot] - n + i. Rows outside every sequence's are neither read nor
  * written. max_new and max_len bound n and lens from above: a sequence beyond
- * them is left out and reported. */
+ * them is left out and reported. Starts do not decrease: where they do, that is
+ * reported, and other sequences may be left out with the one it is seen at. */
 typedef struct {
     const int32_t *tables; /* [table_rows][table_cols], device */
     const int32_t *lens;   /* [table_rows], device */

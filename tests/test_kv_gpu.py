@@ -3,6 +3,7 @@ sizes, masks and contents where they can go wrong. The pool's unused places,
 behind a sequence's end included, hold NaN throughout."""
 from __future__ import annotations
 
+import ctypes
 import math
 
 import kv_ref
@@ -258,6 +259,56 @@ def test_bad_device_values_are_left_out_and_reported(kv):
         batch = kv.Batch(_i32(starts), 6, 2, 60, None if slots is None else _i32(slots))
         kv.attention(cache, 0, batch, c.q.cuda(), out=out, bad=bad)
         assert int(bad) == 1 and torch.equal(out[:2], good[:2]) and bool((out[2:4] == 3).all()), (starts, slots, lens)
+
+
+def _overlapping(kv, new, length, starts, group, page=16, d=64):
+    """A batch of sequences of `new` rows each whose starts go back to the first row time and again."""
+    c = Case(kv, [(new, length)] * (len(starts) // 2), page, 1, group, d, BF16, seed=len(starts))
+    slots = _i32([i // 2 for i in range(len(starts) - 1)])
+    return c, kv.Batch(_i32(starts), new, new, length, slots=slots)
+
+
+@pytest.mark.parametrize("new,group,seqs", [(1, 4, 9), (600, 4, 9), (600, 2, 91), (200, 4, 1001)])
+def test_starts_that_go_back(kv, new, group, seqs):
+    """More rows among the sequences than the call has, as each begins at the first again: reported, and nothing is
+    written beyond the output, the workspace's bytes and the new tokens' pages."""
+    import ggml_xdna_amd as z
+    starts = [0 if i % 2 == 0 else new for i in range(seqs + 1)]
+    c, b = _overlapping(kv, new, max(new, 40) + 700 * (seqs < 100), starts, group)
+    q, bad = c.q[:new].cuda(), _flag()
+    need = kv.attention_workspace(c.cache, b, group)
+    room = torch.full((need + (1 << 22),), 7, dtype=torch.uint8, device="cuda")
+    out = torch.full((new + 64, group, 64), 7.0, dtype=BF16, device="cuda")
+    ref = ctypes.byref
+    z.check(z.lib().zest_kv_attn(ref(c.cache._layer[0]), ref(c.cache._batch(b)), q.data_ptr(), kv.TYPE_BF16, group * 64, group, 0.125, 1, 0,
+                                 0.0, out.data_ptr(), kv.TYPE_BF16, group * 64, room.data_ptr(), need, bad.data_ptr(), z._stream()), "attn")
+    assert int(bad) == 1 and bool((room[need:] == 7).all()) and bool((out[new:] == 7).all())
+    bad.zero_()
+    pool = c.cache.pool.clone()
+    x = torch.zeros((new, 1, 64), dtype=BF16, device="cuda")
+    kv.append(c.cache, 0, b, x, x, bad=bad)
+    assert int(bad) == 1
+    new_pages = torch.zeros(c.cache.pages, dtype=torch.bool)
+    first = int(c.cache.lens[0]) - new
+    for row in c.cache.tables.cpu().tolist():
+        new_pages[[p for p in row[first // 16:] if p >= 0]] = True
+    assert torch.equal(pool[:, ~new_pages].view(torch.int16), c.cache.pool[:, ~new_pages].view(torch.int16))
+
+
+def test_two_calls_at_once(kv):
+    """Attention of the same queries on two streams: each call has its workspace."""
+    c = Case(kv, [(1, 3000), (40, 1500), (2, 64), (300, 300)], 64, 2, 4, 128, BF16, seed=4)
+    q = c.q.cuda()
+    want = kv.attention(c.cache, 0, c.batch, q)
+    c.check(want)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(kv.attention(c.cache, 0, c.batch, q))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for one in got for x in one)
 
 
 @pytest.mark.parametrize("page", [16, 64])
