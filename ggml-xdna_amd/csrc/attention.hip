@@ -1160,15 +1160,19 @@ attn_plan plan_of(const zest_kv_cache * c, const zest_kv_batch * b, int group) {
     return p;
 }
 
-// Lets a kernel have its ring and the largest prefix sums in shared memory, once
-// (threads that launch it for the first time at once set the same value).
+// Lets a kernel have its ring and the largest prefix sums in shared memory, once a
+// device (threads that launch it for the first time at once set the same value).
 template <auto KERNEL> int allow_lds(size_t ring) {
-    static std::atomic<bool> set{false};
-    if (set.load(std::memory_order_acquire)) return ZEST_OK;
+    static std::atomic<uint64_t> set{0};  // a bit a device, those past the 64th every time
+    int device = 0;
+    if (const hipError_t e = hipGetDevice(&device); e != hipSuccess)
+        return zest::fail(ZEST_E_HIP, "zest_kv_attn: current device: %s", hipGetErrorString(e));
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (set.load(std::memory_order_acquire) & bit) return ZEST_OK;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize,
                                              (int) (ring + zest::seq_index_bytes(zest::KV_MAX_SEQS)));
     if (e != hipSuccess) return zest::fail(ZEST_E_HIP, "zest_kv_attn: shared memory attribute: %s", hipGetErrorString(e));
-    set.store(true, std::memory_order_release);
+    set.fetch_or(bit, std::memory_order_release);
     return ZEST_OK;
 }
 
@@ -1214,6 +1218,17 @@ template <int TYPE> int launch(attn_args & a, int D, const attn_plan & p, hipStr
     }
 }
 
+// Whether two sets of rows (bytes apart, bytes long) share no byte: their spans lie
+// apart, or they are column ranges of one wider buffer.
+bool rows_apart(const void * x, size_t ldx, size_t wx, const void * y, size_t ldy, size_t wy, int64_t rows) {
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(y);
+    const size_t last = (size_t) (rows - 1);
+    if (x0 + last * ldx + wx <= y0 || y0 + last * ldy + wy <= x0) return true;
+    if (last == 0 || ldx != ldy) return false;
+    const size_t off = y0 >= x0 ? (y0 - x0) % ldx : (ldx - (x0 - y0) % ldx) % ldx;
+    return off >= wx && off + wy <= ldx;
+}
+
 } // namespace
 
 extern "C" {
@@ -1237,8 +1252,13 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
     if (const int st = zest::kv_check_rows(out_type, out, ldo, width, me, "out")) return st;
     ZEST_REQUIRE(scale - scale == 0.0f && window >= 0 && softcap >= 0.0f && softcap - softcap == 0.0f,
                  "%s: scale=%g window=%d softcap=%g", me, (double) scale, window, (double) softcap);
-    ZEST_REQUIRE(batch->rows * (int64_t) (q_heads / cache->kv_heads) < (1ll << 31) - 64, "%s: %lld rows of %d heads", me,
+    // (a tile's last column, past the rows' by less than a tile, is a 32-bit number too)
+    ZEST_REQUIRE(batch->rows * (int64_t) (q_heads / cache->kv_heads) < (1ll << 31) - 512, "%s: %lld rows of %d heads", me,
                  (long long) batch->rows, q_heads);
+    const size_t qs = zest::kv_type_bytes(q_type), os = zest::kv_type_bytes(out_type);
+    ZEST_REQUIRE(rows_apart(q, ldq * qs, width * qs, out, ldo * os, width * os, batch->rows), "%s: out overlaps q", me);
+    ZEST_REQUIRE(rows_apart(cache->pool, 0, cache->pages * zest_kv_page_bytes(cache), out, 0, ((batch->rows - 1) * ldo + width) * os, 1),
+                 "%s: out overlaps the pool", me);
     const attn_plan plan = plan_of(cache, batch, q_heads / cache->kv_heads);
     ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads * std::max(1, plan.chunk_splits) < (1ll << 22), "%s: a batch of %lld units of work",
                  me, (long long) std::max(plan.units, plan.chunk_tiles));

@@ -114,7 +114,7 @@ ZEST_API int zest_kv_append(const zest_kv_cache *cache, const zest_kv_batch *bat
  * matrix cores' operand), products and softmax statistics are in 32 bits, the
  * weights are rounded to the cache's type before they meet V. q_heads % kv_heads
  * == 0; row starts of q and out 16-byte aligned; out must not overlap q or the
- * pool.
+ * pool (columns of one wider buffer, equal strides, do not).
  *
  * workspace: zest_kv_attn_workspace's bytes for the same cache, batch and
  * q_heads (by sizes and bounds alone), 16-byte aligned. It holds nothing between

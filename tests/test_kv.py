@@ -123,8 +123,17 @@ def test_entry_points_refuse_bad_arguments_before_the_gpu(kv):
                          (dict(ldq=252), E_ARG), (dict(ldo=258), E_ARG), (dict(q=base + 8), E_ARG), (dict(heads=3), E_ARG),
                          (dict(heads=0), E_ARG), (dict(heads=8192, ldq=1 << 20, ldo=1 << 20), E_ARG), (dict(scale=math.nan), E_ARG),
                          (dict(scale=math.inf), E_ARG), (dict(window=-1), E_ARG), (dict(cap=-1.0), E_ARG), (dict(cap=math.nan), E_ARG),
+                         (dict(out=base), E_ARG), (dict(q=base + 65536, out=base + 65536), E_ARG), (dict(q=base + 65536 - 2048), E_ARG),
+                         (dict(q=base + 65536, ldq=512, out=base + 65536 + 512, ldo=512), E_ARG), (dict(out=base + 32768 - 16), E_ARG),
+                         (dict(c=cache(type=30, kv_heads=1), b=batch(rows=(1 << 27) - 16, max_new=1 << 20), heads=16, q=base + (1 << 42),
+                               ldq=1024, out=base + (1 << 45), ldo=1024), E_ARG),
                          (dict(ws=None), E_ARG), (dict(ws=base + 8), E_ARG), (dict(size=need - 1), E_ARG)]:
         refused("zest_kv_attn", attn(**broken), code)
+    # columns of one wider buffer: past that check, refused for the workspace
+    attn(q=base + 65536, ldq=512, out=base + 65536 + 1024, ldo=512, ws=None)
+    assert "workspace" in lib.zest_last_error().decode()
+    attn(q=base + 65536 + 1024, ldq=512, out=base + 65536, ldo=512, ws=None)
+    assert "workspace" in lib.zest_last_error().decode()
     need = lib.zest_kv_scratch_bytes(4, 2)
     for broken, code in [(dict(layers=0), E_ARG), (dict(layers=2, stride=8192), E_ARG), (dict(layers=2, stride=32776), E_ARG),
                          (dict(refs=None), E_ARG), (dict(tables=None), E_ARG), (dict(rows=0), E_ARG), (dict(rows=65537), E_ARG),
