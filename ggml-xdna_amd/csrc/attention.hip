@@ -561,9 +561,10 @@ __device__ __forceinline__ void attend_few(const attn_args & a, int block, int b
 
 // Joins the pieces of the column tile whose run starts in workgroup w's share
 // and goes on past it, if there is one: theirs are the last of the share. A
-// workgroup takes 256 of the tile's groups of four values, and requests eight
+// workgroup takes 256 of the tile's groups of four values, the last one what is
+// left (16 columns of 96 values are one and a half times 256), and requests eight
 // pieces at a time.
-template <int D, int NT> constexpr int COMBINE_PARTS = 16 * NT * D / 4 / 256;
+template <int D, int NT> constexpr int COMBINE_PARTS = (16 * NT * D / 4 + 255) / 256;
 
 template <int D, int NT> __device__ __forceinline__ void combine_few(const attn_args & a, int block, int part, int blocks, int32_t * attn_sh) {
     constexpr int COLS = 16 * NT, UNITS = D / 4;
@@ -580,7 +581,7 @@ template <int D, int NT> __device__ __forceinline__ void combine_few(const attn_
     const int last = shares.owner(end - 1);
     {
         const int i = part * 256 + threadIdx.x, oc = i / UNITS, unit = i - oc * UNITS, cc = ct * COLS + oc;
-        if (cc >= ncols) return;
+        if (i >= COLS * UNITS || cc >= ncols) return;
         const float * x = a.partial + (int64_t) (2 * block + 1) * partial_floats(COLS, D);
         float m = x[COLS * D + oc], l = x[COLS * D + COLS + oc];
         float4 o = *reinterpret_cast<const float4 *>(x + oc * D + unit * 4);

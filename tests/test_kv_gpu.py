@@ -108,6 +108,25 @@ def test_attention_split_over_workgroups(kv):
         assert torch.equal(kv.attention(c.cache, 0, c.batch, q, out_dtype=F32), got)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("new,group", [(1, 1), (2, 5), (1, 11), (3, 5), (4, 4), (1, 17), (8, 4)])
+def test_decoding_of_every_width(kv, dtype, d, new, group):
+    """Batches without a chunk, of one column a k/v head to two whole tiles (1, 10, 11, 15, 16, 17, 32), over contexts
+    that end inside a workgroup's share and that many workgroups share: every value of the output is written, and no
+    row behind the last sequence."""
+    seqs = [(new, 90), (new, 130), (1, 700), (new, 5000)]
+    c = Case(kv, seqs, 64, 2, group, d, dtype, seed=d + 10 * new + group)
+    bad = _flag()
+    out = torch.full((c.rows, c.heads, d), math.nan, dtype=dtype, device="cuda")
+    c.check(kv.attention(c.cache, 0, c.batch, c.q.cuda(), out=out, bad=bad))
+    more = torch.full((c.rows + 2, c.heads, d), math.nan, dtype=dtype, device="cuda")
+    batch = kv.Batch(c.batch.starts, c.rows + 2, new, 5000)
+    kv.attention(c.cache, 0, batch, torch.cat([c.q, c.q[:2]]).cuda(), out=more, bad=bad)
+    assert int(bad) == 0 and bool(more[c.rows:].isnan().all())
+    c.check(more[:c.rows])
+
+
 def test_attention_long_chunk(kv):
     """A chunk of many column tiles, on top of what its sequence holds."""
     c = Case(kv, [(150, 400), (1, 70), (260, 260)], 32, 1, 2, 128, BF16, seed=11)
