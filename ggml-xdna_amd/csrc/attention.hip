@@ -1219,17 +1219,6 @@ template <int TYPE> int launch(attn_args & a, int D, const attn_plan & p, hipStr
     }
 }
 
-// Whether two sets of rows (bytes apart, bytes long) share no byte: their spans lie
-// apart, or they are column ranges of one wider buffer.
-bool rows_apart(const void * x, size_t ldx, size_t wx, const void * y, size_t ldy, size_t wy, int64_t rows) {
-    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(y);
-    const size_t last = (size_t) (rows - 1);
-    if (x0 + last * ldx + wx <= y0 || y0 + last * ldy + wy <= x0) return true;
-    if (last == 0 || ldx != ldy) return false;
-    const size_t off = y0 >= x0 ? (y0 - x0) % ldx : (ldx - (x0 - y0) % ldx) % ldx;
-    return off >= wx && off + wy <= ldx;
-}
-
 } // namespace
 
 extern "C" {
@@ -1257,8 +1246,8 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
     ZEST_REQUIRE(batch->rows * (int64_t) (q_heads / cache->kv_heads) < (1ll << 31) - 512, "%s: %lld rows of %d heads", me,
                  (long long) batch->rows, q_heads);
     const size_t qs = zest::kv_type_bytes(q_type), os = zest::kv_type_bytes(out_type);
-    ZEST_REQUIRE(rows_apart(q, ldq * qs, width * qs, out, ldo * os, width * os, batch->rows), "%s: out overlaps q", me);
-    ZEST_REQUIRE(rows_apart(cache->pool, 0, cache->pages * zest_kv_page_bytes(cache), out, 0, ((batch->rows - 1) * ldo + width) * os, 1),
+    ZEST_REQUIRE(zest::kv_rows_apart(q, ldq * qs, width * qs, out, ldo * os, width * os, batch->rows), "%s: out overlaps q", me);
+    ZEST_REQUIRE(zest::kv_rows_apart(cache->pool, 0, cache->pages * zest_kv_page_bytes(cache), out, 0, ((batch->rows - 1) * ldo + width) * os, 1),
                  "%s: out overlaps the pool", me);
     const attn_plan plan = plan_of(cache, batch, q_heads / cache->kv_heads);
     ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads * std::max(1, plan.chunk_splits) < (1ll << 22), "%s: a batch of %lld units of work",

@@ -45,6 +45,15 @@ int kv_check_rows(int type, const void * p, int64_t ld, int64_t width, const cha
     return ZEST_OK;
 }
 
+bool kv_rows_apart(const void * x, size_t ldx, size_t wx, const void * y, size_t ldy, size_t wy, int64_t rows) {
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(y);
+    const size_t last = (size_t) (rows - 1);
+    if (x0 + last * ldx + wx <= y0 || y0 + last * ldy + wy <= x0) return true;
+    if (last == 0 || ldx != ldy) return false;
+    const size_t off = y0 >= x0 ? (y0 - x0) % ldx : (ldx - (x0 - y0) % ldx) % ldx;
+    return off >= wx && off + wy <= ldx;
+}
+
 } // namespace zest
 
 namespace {
@@ -658,11 +667,17 @@ int zest_kv_append(const zest_kv_cache * cache, const zest_kv_batch * batch, con
         if (const int st = zest::kv_check_rows(in_type, q, ldq, (int64_t) q_heads * cache->head_dim, me, "q")) return st;
         if (const int st = zest::kv_check_rows(q_out_type, q_out, ldq_out, (int64_t) q_heads * cache->head_dim, me, "q_out"))
             return st;
-        const uint8_t * x = (const uint8_t *) q, * y = (const uint8_t *) q_out;
-        const int64_t last = batch->rows - 1, w = (int64_t) q_heads * cache->head_dim;  // spans of the rows in bytes
-        const int64_t xb = (last * ldq + w) * zest::kv_type_bytes(in_type), yb = (last * ldq_out + w) * zest::kv_type_bytes(q_out_type);
-        ZEST_REQUIRE((q == q_out && ldq == ldq_out && in_type == q_out_type) || x + xb <= y || y + yb <= x,
-                     "%s: q_out overlaps q without being q", me);
+        // q, k and v are different workgroups' work, in no order
+        const size_t is = zest::kv_type_bytes(in_type), os = zest::kv_type_bytes(q_out_type), row = (size_t) q_heads * cache->head_dim;
+        auto apart = [&](const void * x, int64_t ld, size_t w) {
+            return zest::kv_rows_apart(x, ld * is, w * is, q_out, ldq_out * os, row * os, batch->rows);
+        };
+        ZEST_REQUIRE((q == q_out && ldq == ldq_out && in_type == q_out_type) || apart(q, ldq, row), "%s: q_out overlaps q without being q",
+                     me);
+        ZEST_REQUIRE(apart(k, ldk, width) && apart(v, ldv, width), "%s: q_out overlaps k or v", me);
+        ZEST_REQUIRE(zest::kv_rows_apart(cache->pool, 0, cache->pages * zest_kv_page_bytes(cache), q_out, 0,
+                                         ((batch->rows - 1) * ldq_out + row) * os, 1),
+                     "%s: q_out overlaps the pool", me);
     }
     if (rope) {
         ZEST_REQUIRE(rope->freqs && (reinterpret_cast<uintptr_t>(rope->freqs) & 7) == 0, "%s: null or misaligned freqs", me);

@@ -149,6 +149,10 @@ int kv_check_cache(const zest_kv_cache * c, const char * what);
 int kv_check_batch(const zest_kv_cache * c, const zest_kv_batch * b, const char * what);
 int kv_check_rows(int type, const void * p, int64_t ld, int64_t width, const char * what, const char * name);
 
+// Whether two sets of rows (bytes apart, bytes long) share no byte: their spans lie
+// apart, or they are column ranges of one wider buffer.
+bool kv_rows_apart(const void * x, size_t ldx, size_t wx, const void * y, size_t ldy, size_t wy, int64_t rows);
+
 // Bytes of a value of an F32, F16 or BF16 tensor, 0 for other types.
 inline int kv_type_bytes(int type) {
     return type == ZEST_TYPE_F32 ? 4 : type == ZEST_TYPE_F16 || type == ZEST_TYPE_BF16 ? 2 : 0;

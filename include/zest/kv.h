@@ -86,9 +86,9 @@ ZEST_API int zest_kv_rope_freqs(int32_t n_dims, double freq_base, double freq_sc
  * as it is) and v, rows of kv_heads * head_dim values of in_type (F32, F16 or
  * BF16), ldk and ldv values apart, rounded once to the cache's type. With q,
  * also q's rows of q_heads * head_dim turned by the same angles into q_out (of
- * q_out_type; q_out may be q itself where types and strides agree, else their
- * spans must not overlap). The angle's
- * position is the token's place in its sequence, or pos[row] (device, NULL: the
+ * q_out_type; q_out may be q itself where types and strides agree, and must not
+ * overlap q otherwise, nor k, v or the pool: columns of one wider buffer, equal
+ * strides, do not). The angle's position is the token's place in its sequence, or pos[row] (device, NULL: the
  * place). Row starts of q, k, v and q_out 16-byte aligned. A token whose place
  * is negative (lens below the new tokens) or whose page is not in the pool is
  * not stored, and reported; its q row is still turned. Two sequences of a call

@@ -147,6 +147,38 @@ def test_entry_points_refuse_bad_arguments_before_the_gpu(kv):
         refused("zest_kv_compact", compact(**broken), code)
 
 
+def test_append_refuses_an_output_that_overlaps_its_inputs(kv):
+    """q, k and v of a call are read and q_out and the pages written in no order: a q_out over k, v or the pool, or over
+    q without being q, is refused; columns of one wider buffer are not (no call here may launch: a rope without
+    frequencies is refused after the overlaps)."""
+    z = load_pkg()
+    lib = z.lib()
+    raw = ctypes.create_string_buffer(1 << 20)
+    base = (ctypes.addressof(raw) + 255) & ~255
+    pool = base + (1 << 19)  # 4 pages of 2 heads, 16 tokens of 64 values: 32 KB
+    cache = kv._Cache(pool, 4, kv.TYPE_BF16, 2, 64, 16)
+    batch = kv._Batch(base, base, base, None, 4, 2, 2, 2, 4, 32)
+    none = kv._Rope(None, 64, 2, 1.0)
+    ld = 1024  # fp32 values: q's 4 heads are 256 of a row, k's and v's 2 heads 128 each
+
+    def said(q_out, ldo=ld, to=0, q=0, k=256 * 4, v=384 * 4):
+        code = lib.zest_kv_append(ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(none), None, 0, base + k, ld, base + v, ld,
+                                  base + q, ld, 4, q_out, ldo, to, None, None)
+        assert code == -1
+        return lib.zest_last_error().decode()
+
+    for fine in (said(base), said(base + 512 * 4), said(base + 768 * 4), said(base + 65536), said(pool + 32768), said(pool - 4 * ld * 4),
+                 said(base + 65536, 256, kv.TYPE_BF16), said(pool + 32768, 256, kv.TYPE_F16), said(base, q=512 * 4)):
+        assert "freqs" in fine
+    for q_out, more, what in [(base + 256 * 4, {}, "k or v"), (base + 384 * 4, {}, "k or v"), (base + 496 * 4, {}, "k or v"),
+                              (base + 240 * 4, {}, "q_out overlaps q"), (base, dict(q=512 * 4, k=0), "k or v"),
+                              (base, dict(q=512 * 4, v=128 * 4), "k or v"), (base + 16, {}, "q_out overlaps q"),
+                              (base + 512 * 4, dict(ldo=512), "overlaps"), (base + 1024, dict(to=30, ldo=256), "overlaps"),
+                              (pool, {}, "the pool"), (pool + 32768 - 16, {}, "the pool"), (pool - 4 * ld * 4 + 3 * ld * 4, {}, "the pool"),
+                              (pool - 16, dict(to=1, ldo=256), "the pool")]:
+        assert what in said(q_out, **more), (q_out - base, more)
+
+
 def test_package_refuses_tensors_that_do_not_fit(kv):
     z = load_pkg()
     pool = torch.zeros((2, 3, 1, 2 * 16 * 64), dtype=torch.bfloat16)

@@ -428,6 +428,23 @@ def test_append_in_place_and_strided(kv, mode, rot, dtype):
     assert kv.append(cache, 0, batch, k, v, rope=r) is None and torch.equal(cache.pool, pool)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_append_into_columns_of_the_same_buffer(kv, dtype):
+    """q, k, v and the turned q side by side in one buffer's rows."""
+    cache = kv.empty_cache(1, 4, 2, 64, 16, slots=2)
+    cache.tables[:, 0], cache.tables[:, 1] = _i32([0, 2]), _i32([1, 3])
+    cache.lens.copy_(_i32([9, 20]))
+    batch = kv.Batch(_i32([0, 9, 14]), 14, 9, 20)
+    wide = torch.randn((14, 256 + 2 * 128 + 256), generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    q, k, v, out = wide[:, :256], wide[:, 256:384], wide[:, 384:512], wide[:, 512:]
+    r = kv.Rope(torch.tensor([1e4 ** (-2 * p / 64) for p in range(32)], dtype=torch.float64, device="cuda"))
+    want = kv.append(cache, 0, batch, k, v, q, r, q_dtype=dtype)
+    pool, before = cache.pool.clone(), wide[:, :512].clone()
+    cache.pool.zero_()
+    kv.append(cache, 0, batch, k, v, q, r, q_out=out)
+    assert torch.equal(out, want) and torch.equal(cache.pool, pool) and torch.equal(wide[:, :512], before)
+
+
 def test_append_leaves_out_what_has_no_place(kv):
     cache = kv.empty_cache(1, 4, 1, 64, 16, slots=3)
     cache.tables[0, 0], cache.tables[1, 0], cache.tables[1, 1], cache.tables[2, 0] = 0, 1, 99, 3
