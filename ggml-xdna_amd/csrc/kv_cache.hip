@@ -433,6 +433,7 @@ __global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
         const int32_t * row = a.tables + (int64_t) a.dst[i] * a.cols;
         for (int j = lane; j < e.old_pages; j += 64) {
             const int32_t id = row[j];
+            if (id == -1) continue;  // a window has left it
             if ((uint32_t) id >= (uint32_t) a.pages) bad = true;
             else if (atomicSub(&a.refs[id], 1) <= 0) {  // not counted: left at what it was
                 atomicAdd(&a.refs[id], 1);
@@ -480,7 +481,7 @@ __global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
             if (j < shared) {
                 id = parent[j];
                 if ((uint32_t) id < (uint32_t) a.pages) atomicAdd(&a.refs[id], 1);
-                else bad = true;
+                else bad |= id != -1;
             } else if (j < total) {
                 id = free_list[e.first + j - shared];
                 a.refs[id] = 1;

@@ -137,7 +137,10 @@ ZEST_API size_t zest_kv_scratch_bytes(int64_t pages, int32_t n);
  * is replaced are released first (refs - 1, free at 0); a fork shares its
  * parent's full pages (refs + 1) and gets a copy of its open one, whole, in
  * every layer; further pages are the lowest-numbered free ones, in the order of
- * the entries. Entries of a row past its pages become -1.
+ * the entries. Entries of a row past its pages become -1. An entry of -1 among
+ * its pages is one that a window has left and the program has given back: a
+ * release passes it over and a fork takes it over. Reported are the open page
+ * of a fork that is missing, and other numbers outside the pool.
  *
  * An entry is left undone and reported when it names a slot outside the tables
  * (src -1 apart), grows by a negative number or past table_cols pages, when dst

@@ -567,6 +567,43 @@ def test_assign_reports_wrong_counts(kv):
     assert int(bad) == 1 and cache.tables[2, 0] == 0 and cache.lens.tolist() == [0, 5, 5]
 
 
+def test_assign_passes_over_pages_that_a_window_has_left(kv):
+    """Rows whose first pages are given back (-1, as attention allows): forked, freed, replaced and grown without a
+    report, with exact counts; a fork's open page that is missing, and a number outside the pool, are reported."""
+    cache = kv.empty_cache(2, 8, 1, 64, 16, slots=4, columns=6)
+    cache.pool.copy_(torch.randn(cache.pool.shape, generator=torch.Generator().manual_seed(2)))
+    pool = cache.pool.clone()
+    cache.tables[0, :5] = _i32([-1, -1, 4, 2, 7])
+    cache.lens[0] = 70
+    cache.refs[[4, 2, 7]] = 1
+
+    def step(dst, src, grow, tables, lens, refs, wrong=0):
+        bad = _flag()
+        kv.assign(cache, _i32(dst), _i32(src), _i32(grow), bad=bad)
+        assert int(bad) == wrong and cache.tables.tolist() == tables and cache.lens.tolist() == lens and cache.refs.tolist() == refs
+
+    none, left = [-1] * 6, [-1, -1, 4, 2]
+    step([1], [0], [1], [left + [7, -1], left + [0, -1], none, none], [70, 71, 0, 0], [1, 0, 2, 0, 2, 0, 0, 1])
+    pool[:, 0] = pool[:, 7]
+    assert torch.equal(cache.pool, pool)
+    step([0], [-1], [0], [none, left + [0, -1], none, none], [0, 71, 0, 0], [1, 0, 1, 0, 1, 0, 0, 0])
+    step([1, 2], [1, 1], [10, 0], [none, left + [0, 1], left + [3, -1], none], [0, 81, 71, 0], [1, 1, 2, 1, 2, 0, 0, 0])
+    pool[:, 3] = pool[:, 0]
+    step([1], [-1], [20], [none, [0, 1] + none[2:], left + [3, -1], none], [0, 20, 71, 0], [1, 1, 1, 1, 1, 0, 0, 0])
+    # the open page given back as well: released without a word, but nothing to copy for a fork
+    cache.tables[2, 4], cache.refs[3] = -1, 0
+    step([3], [2], [0], [none, [0, 1] + none[2:], left + none[:2], left + [3, -1]], [0, 20, 71, 71], [1, 1, 2, 1, 2, 0, 0, 0], 1)
+    step([2], [-1], [0], [none, [0, 1] + none[2:], none, left + [3, -1]], [0, 20, 0, 71], [1, 1, 1, 1, 1, 0, 0, 0])
+    for wrong in (-2, 8):
+        cache.tables[3, 0] = wrong
+        step([2], [3], [0], [none, [0, 1] + none[2:], [wrong] + left[1:] + [5, -1], [wrong] + left[1:] + [3, -1]], [0, 20, 71, 71],
+             [1, 1, 2, 1, 2, 1, 0, 0], 1)
+        pool[:, 5] = pool[:, 3]
+        step([2], [-1], [0], [none, [0, 1] + none[2:], none, [wrong] + left[1:] + [3, -1]], [0, 20, 0, 71],
+             [1, 1, 1, 1, 1, 0, 0, 0], 1)
+    assert torch.equal(cache.pool, pool)
+
+
 @pytest.mark.parametrize("seed", range(10))
 @pytest.mark.parametrize("inplace", [True, False])
 def test_compact(kv, seed, inplace):
