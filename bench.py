@@ -548,6 +548,8 @@ def attention_stack(args) -> int:
             stack.run_prompt()
         torch.cuda.synchronize()
         ms[attention] = (time.perf_counter() - t0) * 1e3 / args.steps
+        if attention:
+            stack.cache.check()
         chunk = stack.chunk
         del stack
     pairs = cfg.tokens * (cfg.tokens + 1) / 2  # each token sees those up to its own

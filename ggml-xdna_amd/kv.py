@@ -6,7 +6,13 @@ Like the package's other calls these go straight to the HIP kernels, on torch's
 current stream, with device memory owned by torch tensors; a call that cannot
 be made raises ZestError. Nothing waits for the GPU, so a decoding loop (append
 and attention of every layer, assign) can be captured in a HIP graph; only
-attention's default workspace and output are allocated, from torch's allocator.
+attention's default workspace and outputs are allocated, from torch's allocator.
+
+What a call leaves out because of what the tables, lengths, starts or entries on
+the device hold, it reports in the flag it is given, else in the cache's, which
+Cache.check() looks at. Rows of an output that it does not write (those of a
+sequence left out, and those of no sequence) hold what they held: in an output
+that the call made, anything.
 """
 from __future__ import annotations
 
@@ -90,8 +96,18 @@ class Cache:
         self.layer_stride = pool.stride(0) * 2
         self._layer = [_Cache(pool.data_ptr() + i * self.layer_stride, self.pages, _TYPES[pool.dtype], self.kv_heads, head_dim,
                               page_tokens) for i in range(self.layers)]
+        # where calls that are given no flag of their own report what they leave out
+        self.bad = torch.zeros(1, dtype=torch.int32, device=dev)
         # assign's and compact's working memory: their calls change the cache, so they never run at once
         self._scratch = torch.empty(z.lib().zest_kv_scratch_bytes(self.pages, tables.shape[0]), dtype=torch.uint8, device=dev)
+
+    def check(self) -> None:
+        """Raises ZestError where calls without a flag of their own have left something out since the last check (a page
+        outside the pool, a slot outside the tables, a length past the bounds, a pool that ran out). Waits for the current
+        stream."""
+        if int(self.bad):
+            self.bad.zero_()
+            raise z.ZestError("a call left out what its tables, lengths, starts or entries name outside the cache or the bounds given")
 
     def _batch(self, b: "Batch") -> _Batch:
         if b.starts.device != self.device:
@@ -146,11 +162,11 @@ def rope_freqs(n_dims: int, freq_base: float, freq_scale: float = 1.0, ext_facto
     return list(out), mag.value
 
 
-def _bad(bad, device):
+def _bad(bad, cache: Cache) -> int:
     if bad is None:
-        return None
-    _need(bad.dtype in (torch.int32, torch.uint32) and bad.device == device and bad.numel() > 0,
-          f"bad: an int32 tensor on {device} wanted")
+        return cache.bad.data_ptr()
+    _need(bad.dtype in (torch.int32, torch.uint32) and bad.device == cache.device and bad.numel() > 0,
+          f"bad: an int32 tensor on {cache.device} wanted")
     return bad.data_ptr()
 
 
@@ -182,7 +198,7 @@ def append(cache: Cache, layer: int, batch: Batch, k, v, q=None, rope: Rope | No
         raise z.ZestError("the rope and the cache are on different devices")
     z.check(z.lib().zest_kv_append(ctypes.byref(cache._layer[layer]), ctypes.byref(cache._batch(batch)),
                                    ctypes.byref(rope._c) if rope is not None else None, z._ptr(pos), tk, pk, ldk, pv, ldv, *qa,
-                                   heads, oa[1], oa[2], oa[0], _bad(bad, dev), z._stream()), "zest_kv_append")
+                                   heads, oa[1], oa[2], oa[0], _bad(bad, cache), z._stream()), "zest_kv_append")
     return q_out
 
 
@@ -212,7 +228,7 @@ def attention(cache: Cache, layer: int, batch: Batch, q, scale: float | None = N
         raise z.ZestError(f"workspace: a contiguous tensor on {dev} wanted")
     z.check(lib.zest_kv_attn(c, b, pq, tq, ldq, heads, 1.0 / math.sqrt(d) if scale is None else scale, int(causal), window,
                                  softcap, po, to, ldo, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                                 _bad(bad, dev), z._stream()), "zest_kv_attn")
+                                 _bad(bad, cache), z._stream()), "zest_kv_attn")
     return out
 
 
@@ -228,7 +244,7 @@ def assign(cache: Cache, dst, src, grow, bad=None) -> None:
     z.check(z.lib().zest_kv_assign(ctypes.byref(cache._layer[0]), cache.layers, cache.layer_stride, cache.refs.data_ptr(),
                                    cache.tables.data_ptr(), cache.lens.data_ptr(), cache.tables.shape[0], cache.tables.shape[1],
                                    dst.data_ptr(), src.data_ptr(), grow.data_ptr(), n, cache._scratch.data_ptr(),
-                                   cache._scratch.numel(), _bad(bad, dev), z._stream()), "zest_kv_assign")
+                                   cache._scratch.numel(), _bad(bad, cache), z._stream()), "zest_kv_assign")
 
 
 def compact(cache: Cache, refs=None, tables=None, live=None, bad=None):
@@ -243,5 +259,5 @@ def compact(cache: Cache, refs=None, tables=None, live=None, bad=None):
     z.check(z.lib().zest_kv_compact(ctypes.byref(cache._layer[0]), cache.layers, cache.layer_stride, cache.refs.data_ptr(),
                                     cache.tables.data_ptr(), cache.tables.shape[0], cache.tables.shape[1], refs.data_ptr(),
                                     tables.data_ptr(), live.data_ptr(), cache._scratch.data_ptr(), cache._scratch.numel(),
-                                    _bad(bad, dev), z._stream()), "zest_kv_compact")
+                                    _bad(bad, cache), z._stream()), "zest_kv_compact")
     return live

@@ -14,7 +14,8 @@ With fused=False the gate and up are two GEMMs and the SwiGLU its own kernel,
 as for a GLU that cannot be fused. With attention=True a chunk's q and k are
 turned and its k and v appended to a paged cache (kv.append), and O's input is
 their attention over all of the prompt so far (kv.attention), fp32 rows packed
-as Q's output is without it.
+as Q's output is without it; cache.check() raises where more chunks than a prompt
+has were run on end.
 Weights are random-init N(0, 0.02), quantised to GGUF on the GPU, converted
 once into the resident bfp16 cache (timed separately, as the reference
 reports warm prefill with its one-time copy build apart).

@@ -199,3 +199,13 @@ def test_package_refuses_tensors_that_do_not_fit(kv):
                  lambda: kv.assign(cache, lens, lens, lens), lambda: kv.compact(cache)):
         with pytest.raises(z.ZestError, match="not the current device"):
             call()
+
+
+def test_a_cache_s_flag(kv):
+    z = load_pkg()
+    cache = kv.empty_cache(1, 3, 1, 64, 16, slots=2, device="cpu")
+    cache.check()
+    cache.bad[0] = 1
+    with pytest.raises(z.ZestError, match="left out"):
+        cache.check()
+    cache.check()

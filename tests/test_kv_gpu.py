@@ -280,6 +280,53 @@ def test_bad_device_values_are_left_out_and_reported(kv):
         assert int(bad) == 1 and torch.equal(out[:2], good[:2]) and bool((out[2:4] == 3).all()), (starts, slots, lens)
 
 
+def test_a_cache_tells_what_its_calls_left_out(kv):
+    """Calls without a flag of their own report to the cache's, captured ones too; check raises once and clears it."""
+    import ggml_xdna_amd as z
+    c = Case(kv, [(2, 60), (2, 60)], 16, 1, 2, 64, BF16, seed=4)
+    cache, q, x = c.cache, c.q.cuda(), torch.zeros((4, 1, 64), device="cuda")
+
+    def left_out(call):
+        call()
+        with pytest.raises(z.ZestError, match="left out"):
+            cache.check()
+        cache.check()
+
+    kv.attention(cache, 0, c.batch, q)
+    kv.append(cache, 0, c.batch, x, x)
+    kv.assign(cache, _i32([0]), _i32([0]), _i32([2]))
+    cache.check()
+    kv.assign(cache, _i32([0]), _i32([0]), _i32([-1]), bad=(own := _flag()))
+    assert int(own) == 1
+    cache.check()
+    left_out(lambda: kv.attention(cache, 0, kv.Batch(c.batch.starts, 4, 2, 59), q))
+    left_out(lambda: kv.append(cache, 0, kv.Batch(c.batch.starts, 4, 2, 62, _i32([0, 2])), x, x))
+    left_out(lambda: kv.assign(cache, _i32([0]), _i32([0]), _i32([16 * 4 + 3])))
+    cache.tables[1, 0] = cache.pages
+    left_out(lambda: kv.compact(cache))
+    cache.tables[0, 1] = cache.pages  # past this call's capture
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+        kv.attention(cache, 0, kv.Batch(c.batch.starts, 4, 2, 64), q)
+    torch.cuda.synchronize()
+    cache.check()
+    left_out(graph.replay)
+    left_out(graph.replay)
+
+
+def test_a_stack_that_outgrows_its_cache_is_told(kv):
+    import ggml_xdna_amd as z
+    from ggml_xdna_amd import stack
+    s = stack.Stack(stack.StackConfig("tiny", 1, 256, 256, 128, 512, 8, 8, 8, 8, 100, 64, head_dim=64), seed=1, attention=True)
+    s.run_prompt()
+    s.run_prompt()
+    s.cache.check()
+    s.run_chunk(s.x[:64])
+    with pytest.raises(z.ZestError, match="left out"):
+        s.cache.check()
+
+
 def _overlapping(kv, new, length, starts, group, page=16, d=64):
     """A batch of sequences of `new` rows each whose starts go back to the first row time and again."""
     c = Case(kv, [(new, length)] * (len(starts) // 2), page, 1, group, d, BF16, seed=len(starts))
