@@ -100,6 +100,7 @@ class Cache:
         self.bad = torch.zeros(1, dtype=torch.int32, device=dev)
         # assign's and compact's working memory: their calls change the cache, so they never run at once
         self._scratch = torch.empty(z.lib().zest_kv_scratch_bytes(self.pages, tables.shape[0]), dtype=torch.uint8, device=dev)
+        self._home = torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else None
 
     def check(self) -> None:
         """Raises ZestError where calls without a flag of their own have left something out since the last check (a page
@@ -108,6 +109,16 @@ class Cache:
         if int(self.bad):
             self.bad.zero_()
             raise z.ZestError("a call left out what its tables, lengths, starts or entries name outside the cache or the bounds given")
+
+    def _stream(self) -> int:
+        """The current stream's handle. The cache's own memory was allocated on the stream it was made on: on another one
+        it is marked as used there, so that dropping the cache does not hand it back under the work queued there."""
+        handle = z._stream()
+        if handle != self._home:
+            stream = torch.cuda.current_stream(self.device)
+            self.bad.record_stream(stream)
+            self._scratch.record_stream(stream)
+        return handle
 
     def _batch(self, b: "Batch") -> _Batch:
         if b.starts.device != self.device:
@@ -198,7 +209,7 @@ def append(cache: Cache, layer: int, batch: Batch, k, v, q=None, rope: Rope | No
         raise z.ZestError("the rope and the cache are on different devices")
     z.check(z.lib().zest_kv_append(ctypes.byref(cache._layer[layer]), ctypes.byref(cache._batch(batch)),
                                    ctypes.byref(rope._c) if rope is not None else None, z._ptr(pos), tk, pk, ldk, pv, ldv, *qa,
-                                   heads, oa[1], oa[2], oa[0], _bad(bad, cache), z._stream()), "zest_kv_append")
+                                   heads, oa[1], oa[2], oa[0], _bad(bad, cache), cache._stream()), "zest_kv_append")
     return q_out
 
 
@@ -228,7 +239,7 @@ def attention(cache: Cache, layer: int, batch: Batch, q, scale: float | None = N
         raise z.ZestError(f"workspace: a contiguous tensor on {dev} wanted")
     z.check(lib.zest_kv_attn(c, b, pq, tq, ldq, heads, 1.0 / math.sqrt(d) if scale is None else scale, int(causal), window,
                                  softcap, po, to, ldo, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                                 _bad(bad, cache), z._stream()), "zest_kv_attn")
+                                 _bad(bad, cache), cache._stream()), "zest_kv_attn")
     return out
 
 
@@ -244,7 +255,7 @@ def assign(cache: Cache, dst, src, grow, bad=None) -> None:
     z.check(z.lib().zest_kv_assign(ctypes.byref(cache._layer[0]), cache.layers, cache.layer_stride, cache.refs.data_ptr(),
                                    cache.tables.data_ptr(), cache.lens.data_ptr(), cache.tables.shape[0], cache.tables.shape[1],
                                    dst.data_ptr(), src.data_ptr(), grow.data_ptr(), n, cache._scratch.data_ptr(),
-                                   cache._scratch.numel(), _bad(bad, cache), z._stream()), "zest_kv_assign")
+                                   cache._scratch.numel(), _bad(bad, cache), cache._stream()), "zest_kv_assign")
 
 
 def compact(cache: Cache, refs=None, tables=None, live=None, bad=None):
@@ -259,5 +270,5 @@ def compact(cache: Cache, refs=None, tables=None, live=None, bad=None):
     z.check(z.lib().zest_kv_compact(ctypes.byref(cache._layer[0]), cache.layers, cache.layer_stride, cache.refs.data_ptr(),
                                     cache.tables.data_ptr(), cache.tables.shape[0], cache.tables.shape[1], refs.data_ptr(),
                                     tables.data_ptr(), live.data_ptr(), cache._scratch.data_ptr(), cache._scratch.numel(),
-                                    _bad(bad, cache), z._stream()), "zest_kv_compact")
+                                    _bad(bad, cache), cache._stream()), "zest_kv_compact")
     return live

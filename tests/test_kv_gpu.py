@@ -315,6 +315,30 @@ def test_a_cache_tells_what_its_calls_left_out(kv):
     left_out(graph.replay)
 
 
+def test_a_cache_dropped_while_another_stream_uses_it(kv):
+    """The working memory and the flag of a cache that another stream's queued work uses go to no new tensor before that
+    work is done."""
+    cache = kv.empty_cache(1, 40000, 1, 64, 16, slots=4, columns=100)
+    kept = cache.pool, cache.tables, cache.lens, cache.refs
+    assert int(cache.refs.sum()) == 0
+    used = [(t.data_ptr(), t.numel() * t.element_size()) for t in (cache._scratch, cache.bad)]
+    entries = _i32([0]), _i32([-1]), _i32([1000])
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(20_000_000)
+        kv.assign(cache, *entries)
+        done = torch.cuda.Event()
+        done.record()
+    del cache
+    new = [torch.empty(n, dtype=torch.uint8, device="cuda") for _, n in used for _ in range(4)]
+    assert not done.query()  # else this shows nothing
+    for t in new:
+        assert all(t.data_ptr() + t.numel() <= at or at + n <= t.data_ptr() for at, n in used)
+    torch.cuda.synchronize()
+    assert kept[2].tolist() == [1000, 0, 0, 0] and int(kept[3].sum()) == 63
+
+
 def test_a_stack_that_outgrows_its_cache_is_told(kv):
     import ggml_xdna_amd as z
     from ggml_xdna_amd import stack
