@@ -15,6 +15,7 @@
 // the cache stores V in.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "kv_device.h"
 #include "zest_common.h"
@@ -73,7 +74,8 @@ struct attn_args {
     void * out;
     int64_t ldq, ldo;
     int32_t q_type, out_type, group, causal, window;
-    float scale, softcap;  // scale >= 0, softcap 0: none
+    float scale2;          // scale log2 e, scale > 0
+    float cap2, cap_e;     // softcap log2 e (0: none), 2 log2 e scale / softcap
     float sign;            // q is multiplied by it: -1 for a negative scale, 0 for a scale of 0 (scale is then 1)
     int32_t chunk_cols;    // sequences of more columns than this are attend_chunk's
     float * partial;
@@ -205,10 +207,35 @@ __device__ inline void store4(const attn_args & a, int64_t at, const float v[4])
 }
 
 // Scores with a softcap, in units of log2: cap * tanh(x) as 1 - 2 / (e^2x + 1),
-// off by 2^-23 of the cap at most.
+// off by 2^-22 of the cap at most.
 __device__ inline float capped(const attn_args & a, float s) {
-    const float cap = a.softcap * LOG2E;
-    return cap - 2.0f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * (a.scale / a.softcap * (2.0f * LOG2E))) + 1.0f);
+    return a.cap2 - 2.0f * a.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.cap_e) + 1.0f);
+}
+
+// That is 2^-16 of a score's unit at a cap of 64, less than a weight's rounding to
+// 16 bits. From there on it would pass it, so scores below a quarter of the cap
+// are multiplied by the series of tanh(x) / x (to x^8: off by 2^-26), which leaves
+// an error of 2^-20 of the score at any cap. Not for all caps, as a chunk pays for
+// it: 32 heads of 128, 2048 tokens at 8192, 311 us at a cap of 30, 380 at 100 (a
+// decoding batch 165 and 166).
+constexpr float PLAIN_CAP = 64.0f;
+
+__device__ inline float capped_below(const attn_args & a, float s) {
+    const float e = s * a.cap_e, y = e * e;          // e = 2 log2 e x
+    constexpr float R = 0.25f / (LOG2E * LOG2E);     // x^2 / y
+    const float q = fmaf(y, fmaf(y, fmaf(y, fmaf(y, R * R * R * R * 62.0f / 2835.0f, -R * R * R * 17.0f / 315.0f), R * R * 2.0f / 15.0f),
+                                 -R / 3.0f), 1.0f);
+    return fabsf(e) < 0.5f * LOG2E ? s * a.scale2 * q : capped(a, s);
+}
+
+template <typename V, int N> __device__ inline void cap_all(const attn_args & a, V & s) {
+    if (a.cap2 > PLAIN_CAP * LOG2E) {
+#pragma unroll
+        for (int i = 0; i < N; i++) s[i] = capped_below(a, s[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) s[i] = capped(a, s[i]);
+    }
 }
 
 // A word that no wave changes while the kernel runs, at an address that is the
@@ -401,17 +428,15 @@ __device__ __forceinline__ void attend_few(const attn_args & a, int block, int b
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read before it is overwritten
             if (more) load_k(j + R, id[R]);
 
-            const float c = a.softcap > 0.0f ? 1.0f : a.scale * LOG2E;
+            const float c = a.cap2 > 0.0f ? 1.0f : a.scale2;
             frag pf[NT];
 #pragma unroll
             for (int q = 0; q < NT; q++) {
                 // value e of x: token t0 + base + e + 8x of the lane group's base
                 const int32_t base_t = t0 + 4 * (lg & 1) + 16 * (lg >> 1);
-                if (a.softcap > 0.0f) {
+                if (a.cap2 > 0.0f) {
 #pragma unroll
-                    for (int x = 0; x < 2; x++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) sc[q][x][e] = capped(a, sc[q][x][e]);
+                    for (int x = 0; x < 2; x++) cap_all<f32x4, 4>(a, sc[q][x]);
                 }
                 if (masked) {
                     const bool page = there[0] >> (lg >> 1) & 1;
@@ -841,7 +866,7 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
             }
         }
     };
-    const float c = a.softcap > 0.0f ? 1.0f : a.scale * LOG2E;
+    const float c = a.cap2 > 0.0f ? 1.0f : a.scale2;
     float shrink[NQ];
     // Maximum, sum and weights of s_cur; the weights go to `to`.
     auto soften = [&](frag to[NQ][2]) {
@@ -900,9 +925,7 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
     };
     auto cap_scores = [&]() {
 #pragma unroll
-        for (int q = 0; q < NQ; q++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) s_cur[q][i] = capped(a, s_cur[q][i]);
+        for (int q = 0; q < NQ; q++) cap_all<f32x16, 16>(a, s_cur[q]);
     };
     auto finish = [&](bool rise, const frag pn[NQ][2]) {
         if (__any(rise)) {
@@ -938,7 +961,7 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
     bool masked = n > 0 ? enter(0) : false;
     while (j < n) {
         // a step that is masked, or follows one that is, or the first
-        if (a.softcap > 0.0f) cap_scores();
+        if (a.cap2 > 0.0f) cap_scores();
         if (masked) {
             const int32_t t0 = t_first + j * GROUP;
 #pragma unroll
@@ -965,7 +988,7 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
         if (++j < n) masked = enter(j);
         // the steps that every column sees whole
         while (j < n && !masked && !masked_before) {
-            if (a.softcap > 0.0f) cap_scores();
+            if (a.cap2 > 0.0f) cap_scores();
             frag pn[NQ][2];
             scores(k_next(), s_next);
             weigh(v_last());
@@ -1242,6 +1265,9 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
     if (const int st = zest::kv_check_rows(out_type, out, ldo, width, me, "out")) return st;
     ZEST_REQUIRE(scale - scale == 0.0f && window >= 0 && softcap >= 0.0f && softcap - softcap == 0.0f,
                  "%s: scale=%g window=%d softcap=%g", me, (double) scale, window, (double) softcap);
+    // (its quotient with the scale, times 2 log2 e, is a 32-bit number too)
+    ZEST_REQUIRE(softcap == 0.0f || (scale == 0.0f ? 1.0 : std::fabs(scale)) / (double) softcap < 1e38, "%s: softcap=%g for scale=%g", me, (double) softcap,
+                 (double) scale);
     // (a tile's last column, past the rows' by less than a tile, is a 32-bit number too)
     ZEST_REQUIRE(batch->rows * (int64_t) (q_heads / cache->kv_heads) < (1ll << 31) - 512, "%s: %lld rows of %d heads", me,
                  (long long) batch->rows, q_heads);
@@ -1261,9 +1287,14 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
     a.q = q, a.out = out, a.ldq = ldq, a.ldo = ldo;
     a.q_type = q_type, a.out_type = out_type;
     a.group = q_heads / cache->kv_heads;
-    a.causal = causal != 0, a.window = window, a.softcap = softcap;
+    a.causal = causal != 0, a.window = window;
     a.sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
-    a.scale = scale == 0.0f ? 1.0f : scale < 0.0f ? -scale : scale;
+    const float by = scale == 0.0f ? 1.0f : std::fabs(scale);
+    a.scale2 = by * LOG2E;
+    if (softcap > 0.0f) {
+        a.cap2 = softcap * LOG2E;
+        a.cap_e = by / softcap * (2.0f * LOG2E);
+    }
     a.chunk_cols = plan.chunk_cols;
     a.chunk_splits = plan.chunk_splits;
     a.partial = (float *) workspace;

@@ -101,7 +101,8 @@ ZEST_API int zest_kv_append(const zest_kv_cache *cache, const zest_kv_batch *bat
 /* Attention of the new tokens over their sequences' tokens: for row i and query
  * head j (k/v head j / (q_heads / kv_heads)),
  *     out = sum_t softmax_t(s_t) v_t,  s_t = scale q.k_t,
- *     with softcap > 0: s_t = softcap tanh(scale q.k_t / softcap),
+ *     with softcap > 0: s_t = softcap tanh(scale q.k_t / softcap) (a softcap whose
+ *     quotient scale / softcap passes 10^38 is refused),
  * over the tokens t < len that the row sees: with `causal` t <= its place, with
  * window > 0 also t > its place - window. Without `causal` every row sees the
  * whole sequence (an encoder's states: lens need not hold the rows). A row that

@@ -179,6 +179,26 @@ def test_append_refuses_an_output_that_overlaps_its_inputs(kv):
         assert what in said(q_out, **more), (q_out - base, more)
 
 
+def test_attention_refuses_a_softcap_too_small_for_its_scale(kv):
+    """Where their quotient passes 32 bits, a score of 0 would become NaN. (No call here may launch: the workspace is missing.)"""
+    z = load_pkg()
+    lib = z.lib()
+    raw = ctypes.create_string_buffer(1 << 20)
+    base = (ctypes.addressof(raw) + 255) & ~255
+    cache, batch = kv._Cache(base, 4, kv.TYPE_BF16, 2, 64, 16), kv._Batch(base, base, base, None, 4, 2, 2, 2, 4, 32)
+
+    def said(scale, cap):
+        code = lib.zest_kv_attn(ctypes.byref(cache), ctypes.byref(batch), base + 65536, 0, 256, 4, scale, 1, 0, cap, base + 131072, 0, 256,
+                                None, 0, None, None)
+        assert code == -1
+        return lib.zest_last_error().decode()
+
+    for scale, cap in [(0.125, 1e-39), (-0.125, 1e-39), (1e20, 1e-20), (0.0, 1e-39)]:
+        assert "softcap" in said(scale, cap)
+    for scale, cap in [(0.125, 1e-38), (-0.125, 3e38), (0.0, 1e-37), (1e20, 0.0)]:
+        assert "workspace" in said(scale, cap)
+
+
 def test_package_refuses_tensors_that_do_not_fit(kv):
     z = load_pkg()
     pool = torch.zeros((2, 3, 1, 2 * 16 * 64), dtype=torch.bfloat16)

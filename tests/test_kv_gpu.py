@@ -83,6 +83,23 @@ def test_attention_masks(kv, causal, window, softcap, scale):
     c.check(kv.attention(c.cache, 0, c.batch, c.q.cuda(), scale, causal, window, softcap), causal, window, softcap, scale)
 
 
+@pytest.mark.parametrize("softcap", [1e-30, 0.05, 3.0, 64.0, 65.0, 1e3, 1e4, 1e6, 1e9, 3e38])
+@pytest.mark.parametrize("d,new", [(64, 1), (64, 70), (128, 3), (128, 90)])
+def test_softcap_of_any_size(kv, d, new, softcap):
+    """Caps that flatten every score to those that change none. Up to 64 a capped score is off by 2^-22 of the cap,
+    beyond by 2^-20 of the score (at most `reach`): twice that of a weight, above and below the line."""
+    c = Case(kv, [(new, 150), (1, 40), (new, 700)], 32, 2, 4, d, F16, seed=int(d + new))
+    scale = 1.0 / math.sqrt(d)
+    got = kv.attention(c.cache, 0, c.batch, c.q.cuda(), softcap=softcap, out_dtype=F32).cpu()
+    for i, n in enumerate(c.new):
+        r = slice(c.starts[i], c.starts[i] + n)
+        out, spread, reach = kv_ref.attention(c.q[r], c.book.k[i], c.book.v[i], scale, softcap=softcap)
+        bound = kv_ref.attention_bound(out, spread, reach, d, F16, F32)
+        bound += 2 * (2.0 ** -22 * softcap if softcap <= 64 else 2.0 ** -20 * reach) * spread
+        off = (got[r].double() - out).abs()
+        assert bool((off <= bound).all()), (i, float((off / bound).max()))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("q_dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("out_dtype", [F32, F16, BF16])
