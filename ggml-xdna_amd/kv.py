@@ -98,6 +98,7 @@ class Cache:
                               page_tokens) for i in range(self.layers)]
         # where calls that are given no flag of their own report what they leave out
         self.bad = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._bad_at = self.bad.data_ptr()
         # assign's and compact's working memory: their calls change the cache, so they never run at once
         self._scratch = torch.empty(z.lib().zest_kv_scratch_bytes(self.pages, tables.shape[0]), dtype=torch.uint8, device=dev)
         self._home = torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else None
@@ -175,7 +176,7 @@ def rope_freqs(n_dims: int, freq_base: float, freq_scale: float = 1.0, ext_facto
 
 def _bad(bad, cache: Cache) -> int:
     if bad is None:
-        return cache.bad.data_ptr()
+        return cache._bad_at
     _need(bad.dtype in (torch.int32, torch.uint32) and bad.device == cache.device and bad.numel() > 0,
           f"bad: an int32 tensor on {cache.device} wanted")
     return bad.data_ptr()
@@ -195,12 +196,16 @@ def append(cache: Cache, layer: int, batch: Batch, k, v, q=None, rope: Rope | No
     if tk != tv:
         raise z.ZestError("k and v of one type wanted")
     qa, oa, heads = (None, 0), (0, None, 0), 0
-    if q is not None:
+    if q is None:
+        _need(q_out is None, "q_out: rows of q wanted with it")
+    else:
         tq, pq, ldq, heads = _rows(q, "q", batch.rows, None, d, dev)
         if tq != tk:
             raise z.ZestError("q, k and v of one type wanted")
         if q_out is None:
             q_out = torch.empty_like(q, dtype=q_dtype or cache.pool.dtype, memory_format=torch.contiguous_format)
+        elif q_dtype is not None and q_out.dtype != q_dtype:
+            raise z.ZestError(f"q_out of {q_out.dtype}, q_dtype {q_dtype}")
         to, po, ldo, _ = _rows(q_out, "q_out", batch.rows, heads, d, dev)
         qa, oa = (pq, ldq), (to, po, ldo)
     if pos is not None:
@@ -230,6 +235,8 @@ def attention(cache: Cache, layer: int, batch: Batch, q, scale: float | None = N
     tq, pq, ldq, heads = _rows(q, "q", batch.rows, None, d, dev)
     if out is None:
         out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise z.ZestError(f"out of {out.dtype}, out_dtype {out_dtype}")
     to, po, ldo, _ = _rows(out, "out", batch.rows, heads, d, dev)
     lib = z.lib()
     c, b = ctypes.byref(cache._layer[layer]), ctypes.byref(cache._batch(batch))

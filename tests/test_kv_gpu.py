@@ -368,6 +368,22 @@ def test_a_stack_that_outgrows_its_cache_is_told(kv):
         s.cache.check()
 
 
+def test_outputs_that_contradict_the_call(kv):
+    """An output for queries that are not given, or of another type than the one asked for, is refused before the launch."""
+    import ggml_xdna_amd as z
+    c = Case(kv, [(2, 20)], 16, 1, 2, 64, BF16, seed=4)
+    q, x, out = c.q.cuda(), torch.zeros((2, 1, 64), dtype=BF16, device="cuda"), torch.empty((2, 2, 64), dtype=BF16, device="cuda")
+    pool = c.cache.pool.clone()
+    for call, said in [(lambda: kv.append(c.cache, 0, c.batch, x, x, q_out=out), "q_out"),
+                       (lambda: kv.append(c.cache, 0, c.batch, x, x, q, q_out=out, q_dtype=F32), "q_dtype"),
+                       (lambda: kv.attention(c.cache, 0, c.batch, q, out=out, out_dtype=F16), "out_dtype")]:
+        with pytest.raises(z.ZestError, match=said):
+            call()
+    assert torch.equal(c.cache.pool.view(torch.int16), pool.view(torch.int16))
+    assert kv.append(c.cache, 0, c.batch, x, x, q, q_out=out, q_dtype=BF16) is out
+    assert kv.attention(c.cache, 0, c.batch, q, out=out, out_dtype=BF16) is out
+
+
 def _overlapping(kv, new, length, starts, group, page=16, d=64):
     """A batch of sequences of `new` rows each whose starts go back to the first row time and again."""
     c = Case(kv, [(new, length)] * (len(starts) // 2), page, 1, group, d, BF16, seed=len(starts))
