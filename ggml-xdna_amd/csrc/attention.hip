@@ -600,7 +600,8 @@ template <int D, int NT> __device__ __forceinline__ void combine_few(const attn_
     int32_t before;
     const kv_seq s = index.at(u1 - 1, before);
     const int32_t run = units_of(a, s), at = u1 - 1 - before, tiles = col_tiles(a, s, COLS);
-    const int32_t item = at / run, start = before + item * run, end = start + run;
+    // (costs that reached the sums' limit end there, with the last run cut short)
+    const int32_t item = at / run, start = before + item * run, end = start + min(run, index.total - start);
     if (start < u0 || end <= u1) return;
     const int32_t h = item / tiles, ct = item - h * tiles, ncols = s.n * a.group;
     const int last = shares.owner(end - 1);
