@@ -203,6 +203,109 @@ def test_many_sequences(kv, count):
     assert torch.equal(pool.view(torch.int16), want.view(torch.int16))
 
 
+@pytest.mark.parametrize("d,count,new", [(192, 100, 70), (256, 70, 40), (96, 4096, 1), (256, 4096, 1)])
+def test_many_sequences_of_wide_heads(kv, d, count, new):
+    """Prefix sums in shared memory beside the widest rings, with and without a chunk in the batch."""
+    rng = np.random.default_rng(d + count)
+    news = [int(n) for n in rng.choice([0, 1, 1], count)]
+    news[count // 3] = new
+    c = Case(kv, [(n, n + int(rng.integers(0, 40))) for n in news], 16, 1, 1 if count > 1000 else 2, d, F16, seed=d)
+    bad = _flag()
+    c.check(kv.attention(c.cache, 0, c.batch, c.q.cuda(), bad=bad))
+    assert int(bad) == 0
+
+
+@pytest.mark.parametrize("new", [1, 5, 90])
+def test_a_place_near_the_largest(kv, new):
+    """A window over the end of a sequence of 2^30 tokens, whose other pages are gone, and the append of its last ones."""
+    d, page, length, window = 64, 256, 1 << 30, 150
+    book = kv_ref.Book([512], page, 1, d, BF16, seed=new)  # the last two pages' tokens
+    table = torch.full((1, length // page), -1, dtype=torch.int32)
+    table[0, -2:] = book.table[0, :2]
+    cache = kv.Cache(book.pool.cuda(), table.cuda(), _i32([length]), book.refs.cuda(), page, d)
+    batch, bad = kv.Batch(_i32([0, new]), new, new, length), _flag()
+    q = torch.randn((new, 4, d), generator=torch.Generator().manual_seed(new)).to(BF16)
+    got = kv.attention(cache, 0, batch, q.cuda(), window=window, bad=bad).cpu()
+    want, spread, reach = kv_ref.attention(q, book.k[0], book.v[0], 0.125, window=window)
+    assert bool(((got.double() - want).abs() <= kv_ref.attention_bound(want, spread, reach, d, BF16, BF16)).all()) and int(bad) == 0
+    k, v = (torch.randn((new, 1, d), generator=torch.Generator().manual_seed(i)) for i in (1, 2))
+    freqs = [1e4 ** (-2 * p / d) for p in range(d // 2)]
+    kv.append(cache, 0, batch, k.cuda(), v.cuda(), rope=kv.Rope(torch.tensor(freqs, dtype=torch.float64, device="cuda")), bad=bad)
+    k1, v1 = kv_ref.read_cache(cache.pool.cpu(), book.table[0], 512, page, d)
+    turned = kv_ref.rope(k, np.arange(length - new, length), freqs, 2, 1.0)
+    # the angle's own error: 2^28 turns in 64 bits, a product's and a constant's rounding of 2^-25 of a turn each
+    assert bool(((k1[-new:].double() - turned).abs() <= 2.0 ** -8 * turned.abs() + 8 * (2.0 ** -22 + 2 * math.pi * 2.0 ** -23)).all())
+    assert torch.equal(v1[-new:], v.to(BF16)) and torch.equal(k1[:-new], book.k[0][:-new]) and int(bad) == 0
+
+
+def test_offsets_past_32_bits(kv):
+    """The same calls over pages at the front of a pool of 10 GB, and at its end; rows 2^27 values apart."""
+    d, page, kvh, group = 128, 64, 8, 2
+    bytes_each = 4 * page * d * kvh
+    pages = 5 * (1 << 30) // bytes_each
+    seqs = [(70, 700), (1, 900), (3, 64)]
+    need = [-(-m // page) for _, m in seqs]
+    cache = kv.empty_cache(2, pages, kvh, d, page, slots=5, columns=max(need) + 1)
+    starts = _starts([n for n, _ in seqs])
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn((sum(m for _, m in seqs), kvh, d), generator=g, device="cuda") for _ in range(2))
+    q = torch.randn((starts[-1], kvh * group, d), generator=g, device="cuda")
+    wide = torch.empty((starts[-1], 1 << 27), dtype=BF16, device="cuda")  # 74 rows of 256 MB: 20 GB
+    fill = kv.Batch(_i32(_starts([m for _, m in seqs])), k.shape[0], 700 + 200, 1000)
+    batch = kv.Batch(_i32(starts), starts[-1], 70, 1000)
+    results = []
+    for first in (0, pages - sum(need)):
+        cache.tables.fill_(-1)
+        cache.refs.zero_()
+        at = first
+        for b, n in enumerate(need):
+            cache.tables[b, :n] = torch.arange(at, at + n, dtype=torch.int32, device="cuda")
+            at += n
+        cache.refs[first:at] = 1
+        cache.lens.copy_(_i32([m for _, m in seqs] + [0, 0]))
+        kv.append(cache, 1, fill, k, v)
+        out = wide[:, 4096:4096 + kvh * group * d]
+        wide[:, :kvh * group * d] = q.reshape(starts[-1], -1)
+        kv.attention(cache, 1, batch, wide[:, :kvh * group * d], out=out)
+        again = kv.append(cache, 1, batch, k[:starts[-1]], v[:starts[-1]], q)
+        results.append((out.clone(), again))
+    assert bool(results[0][0].isfinite().all()) and bool(results[0][0].any())
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    held = cache.pool[1, first:].clone()
+    kv.assign(cache, _i32([3]), _i32([0]), _i32([0]))  # the open page, to the front of both layers
+    assert cache.tables[3, need[0] - 1] == 0 and torch.equal(cache.pool[1, 0], held[need[0] - 1])
+    kv.assign(cache, _i32([3]), _i32([-1]), _i32([0]))
+    live = int(kv.compact(cache))
+    cache.check()
+    assert live == sum(need) and torch.equal(cache.pool[1, :live], held)
+    assert cache.tables[:3].max() == live - 1
+
+
+def test_batches_of_nothing(kv):
+    """No sequence has new tokens; every length is 0; two sequences name the same slot."""
+    c = Case(kv, [(2, 20), (40, 90)], 16, 1, 2, 64, BF16, seed=4)
+    q, x, bad = c.q.cuda(), torch.zeros((42, 1, 64), device="cuda"), _flag()
+    pool = c.cache.pool.clone()
+    for max_new in (1, 42):
+        batch = kv.Batch(_i32([0, 0, 0]), 42, max_new, 90)
+        out = torch.full_like(q, 3.0)
+        kv.attention(c.cache, 0, batch, q, out=out, bad=bad)
+        kv.append(c.cache, 0, batch, x, x, q=q.float(), q_out=(q_out := torch.full_like(q, 3.0)), bad=bad)
+        assert bool((out == 3).all()) and bool((q_out == 3).all()) and int(bad) == 0
+    assert torch.equal(c.cache.pool.view(torch.int16), pool.view(torch.int16))
+    want = kv.attention(c.cache, 0, c.batch, q)
+    twice = kv.attention(c.cache, 0, kv.Batch(_i32([0, 40, 80]), 80, 40, 90, _i32([1, 1])), q[2:].repeat(2, 1, 1), bad=bad)
+    assert torch.equal(twice[:40], twice[40:]) and int(bad) == 0
+    b = c.book
+    ref, spread, reach = kv_ref.attention(c.q[2:], b.k[1], b.v[1], 0.125)
+    assert bool(((twice[:40].cpu().double() - ref).abs() <= kv_ref.attention_bound(ref, spread, reach, 64, BF16, BF16)).all())
+    c.cache.lens.zero_()
+    for new in ([0, 2, 42], [0, 1, 2]):
+        got = kv.attention(c.cache, 0, kv.Batch(_i32(new), 42, new[2] - new[1], 0), q, out=torch.full_like(q, 3.0), bad=bad)
+        assert bool((got[:new[2]] == 0).all()) and bool((got[new[2]:] == 3).all()) and int(bad) == 0
+    assert bool(want.isfinite().all())
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_values_a_row_does_not_see_do_not_reach_it(kv, value, dtype):
@@ -532,6 +635,42 @@ def test_append_in_place_and_strided(kv, mode, rot, dtype):
     assert kv.append(cache, 0, batch, k, v, rope=r) is None and torch.equal(cache.pool, pool)
 
 
+@pytest.mark.parametrize("d,page,kvh,heads,mode,rot", [(64, 16, 16, 16, 2, 64), (96, 32, 5, 15, 2, 96), (96, 64, 3, 12, 0, 48), (128, 256, 8, 48, 2, 128),
+                                                       (128, 64, 9, 27, 2, 40), (192, 128, 8, 24, 0, 192), (192, 16, 2, 30, 2, 64),
+                                                       (256, 64, 7, 14, 2, 256), (256, 32, 11, 11, 0, 64)])
+def test_append_of_every_width(kv, d, page, kvh, heads, mode, rot):
+    """Several heads a workgroup, their last group ragged, for chunks that begin and end inside units of 16."""
+    new, lens = [700, 1, 333, 16, 450], [1000, 33, 333, 48, 451]
+    rows, starts = sum(new), _starts(new)
+    g = torch.Generator().manual_seed(d + rot)
+    count = [-(-m // page) for m in lens]
+    ids = torch.randperm(sum(count) + 2, generator=g).int()
+    table, at = torch.full((len(new), max(count)), -1, dtype=torch.int32), 0
+    for b, n in enumerate(count):
+        table[b, :n] = ids[at:at + n]
+        at += n
+    before = torch.randn((1, len(ids), kvh, 2 * page * d), generator=g).to(BF16)
+    cache = kv.Cache(before.cuda(), table.cuda(), _i32(lens), torch.ones(len(ids), dtype=torch.int32, device="cuda"), page, d)
+    q, k, v = (torch.randn((rows, h, d), generator=g) for h in (heads, kvh, kvh))
+    freqs = [1e4 ** (-2 * p / rot) for p in range(rot // 2)]
+    bad = _flag()
+    got = kv.append(cache, 0, kv.Batch(_i32(starts), rows, max(new), max(lens)), k.cuda(), v.cuda(), q.cuda(),
+                    kv.Rope(torch.tensor(freqs, dtype=torch.float64, device="cuda"), mode), bad=bad)
+    place = np.concatenate([np.arange(m - n, m) for n, m in zip(new, lens)])
+    seq = np.concatenate([np.full(n, b) for b, n in enumerate(new)])
+    tol = lambda w: 2.0 ** -8 * w.abs() + 2.0 ** -22 * 8  # noqa: E731
+    wq, wk = (kv_ref.rope(x, place, freqs, mode, 1.0) for x in (q, k))
+    assert bool(((got.cpu().double() - wq).abs() <= tol(wq)).all()) and int(bad) == 0
+    pool, want = cache.pool.cpu(), before.clone()
+    ki, vi = kv_ref.page_index(page, d)
+    held, t = table[torch.from_numpy(seq), torch.from_numpy(place // page)].long(), torch.from_numpy(place % page)
+    at_k = held[:, None, None], torch.arange(kvh)[None, :, None], ki[t][:, None, :]
+    assert bool(((pool[0][at_k].double() - wk).abs() <= tol(wk)).all())
+    want[0][at_k] = pool[0][at_k]
+    want[0][at_k[0], at_k[1], vi[t][:, None, :]] = v.to(BF16)
+    assert torch.equal(pool, want)  # v's values, and nothing else
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_append_into_columns_of_the_same_buffer(kv, dtype):
     """q, k, v and the turned q side by side in one buffer's rows."""
@@ -732,6 +871,73 @@ def test_compact(kv, seed, inplace):
     for a, b in moves:
         pool[:, b] = pool[:, a]
     assert torch.equal(cache.pool.cpu(), pool)
+
+
+@pytest.mark.parametrize("live", [4000, 4097, 9000])
+@pytest.mark.parametrize("inplace", [True, False])
+def test_compact_of_many_pages(kv, live, inplace):
+    """More pages than the plan keeps in shared memory, most of them in holes."""
+    rng = np.random.default_rng(live)
+    pages, page = 20000, 16
+    ids = np.sort(rng.permutation(pages)[:live])
+    tables = np.full((live // 50 + 1, 60), -1, dtype=np.int32)
+    for s, part in enumerate(np.array_split(rng.permutation(ids), len(tables))):
+        tables[s, :len(part)] = part
+    refs = np.zeros(pages, dtype=np.int32)
+    refs[ids] = rng.integers(1, 4, live)
+    pool = torch.from_numpy(rng.integers(0, 1 << 15, (1, pages, 1, 2 * page * 64), dtype=np.int16)).view(BF16)
+    dev = lambda a: torch.from_numpy(a.copy()).cuda()  # noqa: E731
+    cache = kv.Cache(pool.cuda(), dev(tables), torch.zeros(len(tables), dtype=torch.int32, device="cuda"), dev(refs), page, 64)
+    want_tables, want_refs, moves, n, wrong = kv_ref.compact(tables, refs)
+    new = {} if inplace else dict(refs=torch.full_like(cache.refs, 9), tables=torch.full_like(cache.tables, 9))
+    bad = _flag()
+    assert int(kv.compact(cache, **new, bad=bad)) == n == live and not wrong and int(bad) == 0
+    assert np.array_equal((cache.refs if inplace else new["refs"]).cpu().numpy(), want_refs)
+    assert np.array_equal((cache.tables if inplace else new["tables"]).cpu().numpy(), want_tables)
+    bits = pool.view(torch.int16)
+    bits[:, [b for _, b in moves]] = bits[:, [a for a, _ in moves]]
+    assert torch.equal(cache.pool.cpu().view(torch.int16), bits)
+
+
+def test_batches_that_change_between_replays(kv):
+    """A captured batch of chunks and single tokens, and a captured compaction: starts, lengths and tables are other ones
+    at each replay, eager work runs in between."""
+    heads, kvh, d, page = 8, 2, 128, 16
+    cache = kv.empty_cache(1, 300, kvh, d, page, slots=4, columns=60)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    cache.pool.copy_(torch.randn(cache.pool.shape, generator=g, device="cuda"))
+    starts, rows = _i32([0, 0, 0, 0, 0]), 150
+    batch = kv.Batch(starts, rows, 100, 900)
+    q = torch.randn((rows, heads, d), generator=g, device="cuda").to(BF16)
+    kv.assign(cache, _i32([0, 1, 2, 3]), _i32([-1] * 4), _i32([100, 500, 3, 800]))
+    out = torch.full_like(q, 5.0)
+    kv.attention(cache, 0, batch, q, out=out)
+    torch.cuda.synchronize()
+    stream, graph, tidy = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        with torch.cuda.graph(graph, stream=stream):
+            kv.attention(cache, 0, batch, q, out=out)
+        with torch.cuda.graph(tidy, stream=stream):
+            live = kv.compact(cache)
+    torch.cuda.synchronize()
+    for step, new in enumerate([[0, 100, 0, 1], [1, 1, 3, 1], [50, 33, 2, 60], [0, 0, 0, 9], [100, 0, 1, 40]]):
+        starts.copy_(_i32(_starts(new)))
+        out.fill_(5.0)
+        want = kv.attention(cache, 0, batch, q, out=torch.full_like(q, 5.0))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and bool((out[sum(new):] == 5).all()) and bool(out.isfinite().all())
+        kv.assign(cache, _i32([step % 4, (step + 1) % 4]), _i32([-1, (step + 2) % 4]), _i32([0, 60]))
+        torch.cuda.synchronize()
+        tidy.replay()
+        torch.cuda.synchronize()
+        used = int((cache.refs > 0).sum())
+        assert int(live) == used and bool((cache.refs[:used] > 0).all())
+        after = kv.attention(cache, 0, batch, q, out=torch.full_like(q, 5.0))
+        assert bool(after.isfinite().all())
+        kv.assign(cache, _i32([step % 4]), _i32([-1]), _i32([int(np.random.default_rng(step).integers(100, 800))]))
+    cache.check()
 
 
 def test_calls_on_a_stream_and_in_a_graph(kv):
