@@ -97,11 +97,15 @@ class Cache:
         self._layer = [_Cache(pool.data_ptr() + i * self.layer_stride, self.pages, _TYPES[pool.dtype], self.kv_heads, head_dim,
                               page_tokens) for i in range(self.layers)]
         # where calls that are given no flag of their own report what they leave out
-        self.bad = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._bad_at = self.bad.data_ptr()
+        self._bad = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._bad_at = self._bad.data_ptr()
         # assign's and compact's working memory: their calls change the cache, so they never run at once
         self._scratch = torch.empty(z.lib().zest_kv_scratch_bytes(self.pages, tables.shape[0]), dtype=torch.uint8, device=dev)
         self._home = torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else None
+
+    @property
+    def bad(self) -> torch.Tensor:
+        return self._bad
 
     def check(self) -> None:
         """Raises ZestError where calls without a flag of their own have left something out since the last check (a page
@@ -117,7 +121,7 @@ class Cache:
         handle = z._stream()
         if handle != self._home:
             stream = torch.cuda.current_stream(self.device)
-            self.bad.record_stream(stream)
+            self._bad.record_stream(stream)
             self._scratch.record_stream(stream)
         return handle
 

@@ -229,3 +229,5 @@ def test_a_cache_s_flag(kv):
     with pytest.raises(z.ZestError, match="left out"):
         cache.check()
     cache.check()
+    with pytest.raises(AttributeError):  # calls hold its address
+        cache.bad = torch.zeros(1, dtype=torch.int32)
