@@ -153,6 +153,7 @@ class Batch:
         self.starts, self.slots = _list(starts, "starts", starts.device), slots
         self.seqs, self.rows, self.max_new, self.max_len = starts.numel() - 1, rows, max_new, max_len
         _need(self.seqs > 0, "starts: one more entry than sequences wanted")
+        _need(all(0 <= x < 1 << 31 for x in (max_new, max_len)), f"max_new={max_new}, max_len={max_len}: 31 bits wanted")
         if slots is not None:
             _need(_list(slots, "slots", starts.device).numel() == self.seqs, "slots: one a sequence wanted")
 
@@ -235,6 +236,8 @@ def attention(cache: Cache, layer: int, batch: Batch, q, scale: float | None = N
     _here(dev)
     if not 0 <= layer < cache.layers:
         raise z.ZestError(f"layer {layer} of {cache.layers}")
+    if not 0 <= window < 1 << 31:  # ctypes would cut it to 32 bits
+        raise z.ZestError(f"window={window}")
     d = cache.head_dim
     tq, pq, ldq, heads = _rows(q, "q", batch.rows, None, d, dev)
     if out is None:

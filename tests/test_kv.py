@@ -231,3 +231,12 @@ def test_a_cache_s_flag(kv):
     cache.check()
     with pytest.raises(AttributeError):  # calls hold its address
         cache.bad = torch.zeros(1, dtype=torch.int32)
+
+
+def test_bounds_that_32_bits_would_cut(kv):
+    z = load_pkg()
+    starts = torch.zeros(3, dtype=torch.int32)
+    for max_new, max_len in [((1 << 32) + 1, 8), (1, (1 << 32) + 8), (-1, 8), (1, -1)]:
+        with pytest.raises(z.ZestError, match="31 bits"):
+            kv.Batch(starts, 2, max_new, max_len)
+    assert kv.Batch(starts, 2, 1, 1 << 30).max_len == 1 << 30

@@ -487,6 +487,16 @@ def test_outputs_that_contradict_the_call(kv):
     assert kv.attention(c.cache, 0, c.batch, q, out=out, out_dtype=BF16) is out
 
 
+def test_windows_that_32_bits_would_cut(kv):
+    import ggml_xdna_amd as z
+    c = Case(kv, [(2, 20)], 16, 1, 2, 64, BF16, seed=4)
+    q = c.q.cuda()
+    for window in ((1 << 32) + 5, 1 << 31, -1):
+        with pytest.raises(z.ZestError, match="window"):
+            kv.attention(c.cache, 0, c.batch, q, window=window)
+    assert torch.equal(kv.attention(c.cache, 0, c.batch, q, window=(1 << 31) - 1), kv.attention(c.cache, 0, c.batch, q))
+
+
 def _overlapping(kv, new, length, starts, group, page=16, d=64):
     """A batch of sequences of `new` rows each whose starts go back to the first row time and again."""
     c = Case(kv, [(new, length)] * (len(starts) // 2), page, 1, group, d, BF16, seed=len(starts))
