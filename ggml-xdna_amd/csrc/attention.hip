@@ -463,6 +463,13 @@ __device__ __forceinline__ void attend_few(const attn_args & a, int block, int b
                     for (int dt = 0; dt < DT; dt++) o[dt][q] *= shrink;
                 }
                 m[q] = now;
+                // The weights are the matrix instruction's operand, so they are rounded to
+                // its 16 bits, each off by half a step at most and independently of the
+                // others; their sum is of the unrounded ones, in 32 bits. Against 64 bits
+                // that makes a bf16 chunk's outputs off by 0.0021 to 0.0023 of their size
+                // where their own rounding costs 0.0017, a decoding batch's by 0.0018 to
+                // 0.0020. A second operand for what the rounding leaves would halve the rate
+                // at which a chunk meets V.
                 float sum = 0.0f;
 #pragma unroll
                 for (int x = 0; x < 2; x++)
@@ -672,8 +679,8 @@ __device__ inline int32_t chunk_tiles_of(const attn_args & a, const kv_seq & s, 
 // at once, so the matrix cores and the vector units both have work: the scores
 // of step j + 1, the softmax of step j and the weights of step j - 1 times V.
 //
-// 32 query and 8 k/v heads of 128, the last 2048 of 8192 tokens: 255 us, 945
-// TFLOP/s, where a large library product reaches 1216 on this card. A step of a
+// 32 query and 8 k/v heads of 128, the last 2048 of 8192 tokens: 255 to 266 us by
+// card, 945 to 904 TFLOP/s, where a large library product reaches 1216. A step of a
 // wave is 16 matrix instructions (512 cycles) and about 150 others; the board's
 // power limit costs 12%, and leaving out the softmax or the loads would save 15%
 // and 12%. On the way: K and V straight to registers, nothing shared, 891 us; one
@@ -874,6 +881,7 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
         bool any_rise = false;
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
+            // (the weights' rounding: see attend_few's)
             float top = s_cur[q][0];
 #pragma unroll
             for (int i = 1; i < 16; i++) top = fmaxf(top, s_cur[q][i]);

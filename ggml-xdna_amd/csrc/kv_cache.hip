@@ -373,7 +373,7 @@ constexpr int FEW_ENTRIES = 512, FEW_PAGES = 4096;
 // The tables' part of a step, by one workgroup: its phases are ordered by
 // barriers, so every count is exact and the result does not depend on the order
 // of the atomics (sums only). Latency bound: a chain of a few dependent accesses
-// (12 slots of up to 13 pages: 8.2 us, with entries and free pages in global memory
+// (12 slots of up to 13 pages: 8.2 to 9.0 us, with entries and free pages in global memory
 // 12.3).
 __global__ __launch_bounds__(STEP) void assign_kernel(assign_args a) {
     __shared__ uint32_t seen[MAX_SLOTS / 32], twice[MAX_SLOTS / 32], replaced[MAX_SLOTS / 32];
