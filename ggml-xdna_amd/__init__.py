@@ -19,6 +19,7 @@ PKG_DIR = Path(__file__).resolve().parent
 LIB_PATH = PKG_DIR / "libggml-zest.so"
 
 TYPE_F32, TYPE_Q8_0, TYPE_Q4_K = 0, 8, 12
+TYPE_Q4_0, TYPE_Q4_1, TYPE_IQ4_NL, TYPE_IQ4_XS = 2, 3, 20, 23
 GLU_REGLU, GLU_GEGLU, GLU_SWIGLU, GLU_GEGLU_ERF, GLU_GEGLU_QUICK = 0, 1, 2, 3, 4
 
 TILE_ROWS, TILE_K, TILE_MANT, TILE_BYTES, ROW_ALIGN = 16, 64, 1024, 1152, 256
@@ -35,7 +36,7 @@ _c_p = ctypes.c_void_p
 _c_f = ctypes.c_float
 _c_i = ctypes.c_int
 
-# name -> (restype, argtypes), as declared in include/zest_hip.h and include/zest/kv.h
+# name -> (restype, argtypes), as declared in include/zest_hip.h, include/zest/kv.h and include/zest/decode.h
 SIGNATURES = {
     "zest_init": (_c_i, [_c_i]),
     "zest_self_test": (_c_i, []),
@@ -72,11 +73,20 @@ SIGNATURES = {
     "zest_kv_attn_workspace": (ctypes.c_size_t, [_c_p, _c_p, _c_i]),
     "zest_kv_attn": (_c_i, [_c_p, _c_p, _c_p, _c_i, _c_i64, _c_i, _c_f, _c_i, _c_i, _c_f, _c_p, _c_i, _c_i64, _c_p,
                             ctypes.c_size_t, _c_p, _c_p]),
+    "zest_kv_attn_shared_workspace": (ctypes.c_size_t, [_c_p, _c_p, _c_p, _c_i]),
+    "zest_kv_attn_shared": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_i, _c_i64, _c_i, _c_f, _c_i, _c_i, _c_f, _c_p, _c_i, _c_i64, _c_p,
+                                   ctypes.c_size_t, _c_p, _c_p]),
     "zest_kv_scratch_bytes": (ctypes.c_size_t, [_c_i64, _c_i]),
     "zest_kv_assign": (_c_i, [_c_p, _c_i, _c_i64, _c_p, _c_p, _c_p, _c_i, _c_i, _c_p, _c_p, _c_p, _c_i, _c_p, ctypes.c_size_t,
                               _c_p, _c_p]),
     "zest_kv_compact": (_c_i, [_c_p, _c_i, _c_i64, _c_p, _c_p, _c_i, _c_i, _c_p, _c_p, _c_p, _c_p, ctypes.c_size_t, _c_p,
                                _c_p]),
+    "zest_matvec_workspace": (ctypes.c_size_t, [_c_i, _c_i64, _c_i64, _c_i, _c_p]),
+    "zest_matvec": (_c_i, [_c_i, _c_p, _c_i64, _c_i64, _c_i64, _c_i, *[_c_p] * 7, ctypes.c_size_t, _c_p]),
+    "zest_matvec_glu": (_c_i, [_c_i, _c_i, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, ctypes.c_size_t,
+                               _c_p]),
+    "zest_sample_workspace": (ctypes.c_size_t, [_c_i64, _c_i64]),
+    "zest_sample": (_c_i, [_c_p, _c_i, _c_i64, _c_i64, _c_i64, *[_c_p] * 8, ctypes.c_size_t, _c_p]),
 }
 
 
@@ -301,6 +311,81 @@ def gemm_glu(kind: int, a_packed, m: int, w_gu, f: int, k: int, xout=True, h=Non
     check(lib().zest_gemm_glu(kind, _ptr(a_packed), m, _ptr(w_gu), f, k, _ptr(xo), _ptr(ht), ldh, _ptr(nonfinite),
                               _stream()), "zest_gemm_glu")
     return xo, ht
+
+
+def _need_here(device) -> None:
+    if device.type != "cuda" or device.index != _torch().cuda.current_device():
+        raise ZestError(f"the tensors are on {device}, which is not the current device")
+
+
+def _fp32_rows(t, what: str, rows: int, cols: int, device):
+    """The pointer and row stride of an fp32 tensor [rows][cols], rows any stride apart."""
+    if t.dtype != _torch().float32 or t.shape != (rows, cols) or t.device != device or (t.stride(1) != 1 and cols > 1):
+        raise ZestError(f"{what}: float32 rows [{rows}][{cols}] on {device} wanted")
+    return t.data_ptr(), t.stride(0) if rows > 1 else cols
+
+
+def _gguf(t, what: str, wtype: int, n: int, k: int, device) -> int:
+    """The pointer of n GGUF rows of k values: a contiguous uint8 tensor of their bytes."""
+    size = n * lib().zest_raw_row_bytes(wtype, k)
+    if t.dtype != _torch().uint8 or not t.is_contiguous() or t.device != device or size == 0 or t.numel() != size:
+        raise ZestError(f"{what}: a contiguous uint8 tensor on {device} of {n} rows of {k} values of type {wtype} wanted")
+    return t.data_ptr()
+
+
+def _matvec_workspace(workspace, wtype: int, m: int, k: int, ns, device):
+    torch, n = _torch(), len(ns)
+    need = lib().zest_matvec_workspace(wtype, m, k, n, (ctypes.c_int64 * n)(*ns))
+    if workspace is None:
+        return torch.empty(max(need, 1), dtype=torch.uint8, device=device)
+    if workspace.device != device or not workspace.is_contiguous():
+        raise ZestError(f"workspace: a contiguous tensor on {device} wanted")
+    return workspace
+
+
+def matvec_workspace(wtype: int, m: int, k: int, ns) -> int:
+    """Bytes of matvec's workspace, by sizes alone (matvec_glu: ns = [f, f])."""
+    return lib().zest_matvec_workspace(wtype, m, k, len(ns), (ctypes.c_int64 * len(ns))(*ns))
+
+
+def matvec(wtype: int, x, weights, ns, outs=None, residuals=None, workspace=None):
+    """zest_matvec: outs[i][m][ns[i]] = x . W_i^T (+ residuals[i]) for up to 4 GGUF weights (uint8 device tensors of
+    ns[i] rows, as a model file holds them) on one fp32 x of 1 to 16 rows. Returns the outputs."""
+    torch, n = _torch(), len(weights)
+    dev = x.device
+    _need_here(dev)
+    if x.dim() != 2:
+        raise ZestError("x: rows [m][k] wanted")
+    m, k = x.shape
+    if len(ns) != n or any(l is not None and len(l) != n for l in (outs, residuals)):
+        raise ZestError(f"{n} weights: as many sizes, outputs and residuals wanted")
+    px, ldx = _fp32_rows(x, "x", m, k, dev)
+    w = [_gguf(t, f"weight {i}", wtype, ns[i], k, dev) for i, t in enumerate(weights)]
+    outs = [torch.empty((m, ni), dtype=torch.float32, device=dev) for ni in ns] if outs is None else outs
+    y = [_fp32_rows(t, f"output {i}", m, ns[i], dev) for i, t in enumerate(outs)]
+    res = [(None, 0) if t is None else _fp32_rows(t, f"residual {i}", m, ns[i], dev) for i, t in enumerate(residuals or [None] * n)]
+    ws = _matvec_workspace(workspace, wtype, m, k, ns, dev)
+    P, I64 = ctypes.c_void_p * n, ctypes.c_int64 * n
+    check(lib().zest_matvec(wtype, px, m, k, ldx, n, P(*w), I64(*ns), P(*[p for p, _ in res]), I64(*[l for _, l in res]),
+                            P(*[p for p, _ in y]), I64(*[l for _, l in y]), ws.data_ptr(), ws.numel() * ws.element_size(),
+                            _stream()), "zest_matvec")
+    return outs
+
+
+def matvec_glu(kind: int, wtype: int, x, gate, up, f: int, out=None, workspace=None):
+    """zest_matvec_glu: out[m][f] = glu(x . gate^T, x . up^T) for two GGUF weights of f rows."""
+    torch, dev = _torch(), x.device
+    _need_here(dev)
+    if x.dim() != 2:
+        raise ZestError("x: rows [m][k] wanted")
+    m, k = x.shape
+    px, ldx = _fp32_rows(x, "x", m, k, dev)
+    out = torch.empty((m, f), dtype=torch.float32, device=dev) if out is None else out
+    py, ldy = _fp32_rows(out, "out", m, f, dev)
+    ws = _matvec_workspace(workspace, wtype, m, k, [f, f], dev)
+    check(lib().zest_matvec_glu(kind, wtype, px, m, k, ldx, _gguf(gate, "gate", wtype, f, k, dev), _gguf(up, "up", wtype, f, k, dev),
+                                f, py, ldy, ws.data_ptr(), ws.numel() * ws.element_size(), _stream()), "zest_matvec_glu")
+    return out
 
 
 def rms_norm(x, eps: float, w=None, y=True, packed=None):

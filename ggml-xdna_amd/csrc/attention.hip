@@ -1251,6 +1251,13 @@ template <int TYPE> int launch(attn_args & a, int D, const attn_plan & p, hipStr
     }
 }
 
+// Reports groups whose starts do not fit the batch.
+__global__ __launch_bounds__(256) void groups_kernel(const int32_t * starts, int groups, int seqs, uint32_t * bad) {
+    bool odd = false;
+    for (int g = threadIdx.x; g < groups; g += 256) odd |= starts[g] < 0 || starts[g + 1] < starts[g] || starts[g + 1] > seqs;
+    if (odd) zest::report(bad);
+}
+
 } // namespace
 
 extern "C" {
@@ -1311,6 +1318,26 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
     const hipStream_t s = zest::as_stream(stream);
     return cache->type == ZEST_TYPE_BF16 ? launch<ZEST_TYPE_BF16>(a, cache->head_dim, plan, s)
                                          : launch<ZEST_TYPE_F16>(a, cache->head_dim, plan, s);
+}
+
+size_t zest_kv_attn_shared_workspace(const zest_kv_cache * cache, const zest_kv_batch * batch, const zest_kv_groups * groups,
+                                     int32_t q_heads) {
+    if (!groups || groups->groups <= 0 || groups->max_shared < 0) return 0;
+    return zest_kv_attn_workspace(cache, batch, q_heads);
+}
+
+int zest_kv_attn_shared(const zest_kv_cache * cache, const zest_kv_batch * batch, const zest_kv_groups * groups, const void * q, int q_type,
+                        int64_t ldq, int32_t q_heads, float scale, int causal, int32_t window, float softcap, void * out, int out_type,
+                        int64_t ldo, void * workspace, size_t workspace_bytes, uint32_t * bad, void * stream) {
+    const char * me = "zest_kv_attn_shared";
+    ZEST_REQUIRE(groups && groups->starts && (reinterpret_cast<uintptr_t>(groups->starts) & 3) == 0, "%s: null or misaligned groups", me);
+    ZEST_REQUIRE(groups->groups > 0 && groups->groups <= zest::KV_MAX_SEQS && groups->max_shared >= 0 && groups->max_shared <= (1 << 30),
+                 "%s: groups=%d max_shared=%d", me, groups->groups, groups->max_shared);
+    if (const int st = zest_kv_attn(cache, batch, q, q_type, ldq, q_heads, scale, causal, window, softcap, out, out_type, ldo, workspace,
+                                    workspace_bytes, bad, stream))
+        return st;
+    hipLaunchKernelGGL(groups_kernel, dim3(1), dim3(256), 0, zest::as_stream(stream), groups->starts, groups->groups, batch->seqs, bad);
+    return zest::check_launch(me);
 }
 
 } // extern "C"

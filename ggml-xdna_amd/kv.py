@@ -43,6 +43,10 @@ class _Rope(ctypes.Structure):
     _fields_ = [("freqs", ctypes.c_void_p), ("n_dims", ctypes.c_int32), ("mode", ctypes.c_int32), ("magnitude", ctypes.c_float)]
 
 
+class _Groups(ctypes.Structure):
+    _fields_ = [("starts", ctypes.c_void_p), ("groups", ctypes.c_int32), ("max_shared", ctypes.c_int32)]
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise z.ZestError(what)
@@ -158,6 +162,17 @@ class Batch:
             _need(_list(slots, "slots", starts.device).numel() == self.seqs, "slots: one a sequence wanted")
 
 
+class Groups:
+    """Sequences of a batch that share their leading pages: group g is the sequences starts[g] .. starts[g+1]-1 (int32,
+    device), which share at most max_shared tokens; what they do share is found from their tables on the device."""
+
+    def __init__(self, starts, max_shared: int):
+        self.starts, self.groups, self.max_shared = _list(starts, "starts", starts.device), starts.numel() - 1, max_shared
+        _need(self.groups > 0, "starts: one more entry than groups wanted")
+        _need(0 <= max_shared < 1 << 31, f"max_shared={max_shared}: 31 bits wanted")
+        self._c = _Groups(starts.data_ptr(), self.groups, max_shared)
+
+
 class Rope:
     """Rotary positions: freqs (float64, device), one a pair; mode ROPE_NORMAL or ROPE_NEOX; a magnitude."""
 
@@ -223,15 +238,19 @@ def append(cache: Cache, layer: int, batch: Batch, k, v, q=None, rope: Rope | No
     return q_out
 
 
-def attention_workspace(cache: Cache, batch: Batch, q_heads: int) -> int:
-    """Bytes of attention's workspace, by the batch's sizes and bounds alone."""
+def attention_workspace(cache: Cache, batch: Batch, q_heads: int, groups: Groups | None = None) -> int:
+    """Bytes of attention's workspace, by the batch's (and the groups') sizes and bounds alone."""
+    if groups is not None:
+        return z.lib().zest_kv_attn_shared_workspace(ctypes.byref(cache._layer[0]), ctypes.byref(cache._batch(batch)),
+                                                     ctypes.byref(groups._c), q_heads)
     return z.lib().zest_kv_attn_workspace(ctypes.byref(cache._layer[0]), ctypes.byref(cache._batch(batch)), q_heads)
 
 
 def attention(cache: Cache, layer: int, batch: Batch, q, scale: float | None = None, causal: bool = True, window: int = 0,
-              softcap: float = 0.0, out=None, out_dtype=None, workspace=None, bad=None):
+              softcap: float = 0.0, out=None, out_dtype=None, workspace=None, bad=None, groups: Groups | None = None):
     """zest_kv_attn: attention of the batch's new tokens over layer's pages; returns out (of q's type and shape unless
-    given). scale: 1 / sqrt(head_dim) unless given."""
+    given). scale: 1 / sqrt(head_dim) unless given. groups: sequences that share leading pages, which are then read once
+    for all of them (zest_kv_attn_shared)."""
     dev = cache.device
     _here(dev)
     if not 0 <= layer < cache.layers:
@@ -247,13 +266,20 @@ def attention(cache: Cache, layer: int, batch: Batch, q, scale: float | None = N
     to, po, ldo, _ = _rows(out, "out", batch.rows, heads, d, dev)
     lib = z.lib()
     c, b = ctypes.byref(cache._layer[layer]), ctypes.byref(cache._batch(batch))
+    if groups is None:
+        size, call, more, name = lib.zest_kv_attn_workspace, lib.zest_kv_attn, (), "zest_kv_attn"
+    else:
+        if groups.starts.device != dev:
+            raise z.ZestError("the groups and the cache are on different devices")
+        size, call, more, name = (lib.zest_kv_attn_shared_workspace, lib.zest_kv_attn_shared, (ctypes.byref(groups._c),),
+                                  "zest_kv_attn_shared")
     if workspace is None:
-        workspace = torch.empty(lib.zest_kv_attn_workspace(c, b, heads), dtype=torch.uint8, device=dev)
+        workspace = torch.empty(size(c, b, *more, heads), dtype=torch.uint8, device=dev)
     elif workspace.device != dev or not workspace.is_contiguous():
         raise z.ZestError(f"workspace: a contiguous tensor on {dev} wanted")
-    z.check(lib.zest_kv_attn(c, b, pq, tq, ldq, heads, 1.0 / math.sqrt(d) if scale is None else scale, int(causal), window,
-                                 softcap, po, to, ldo, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                                 _bad(bad, cache), cache._stream()), "zest_kv_attn")
+    z.check(call(c, b, *more, pq, tq, ldq, heads, 1.0 / math.sqrt(d) if scale is None else scale, int(causal), window,
+                 softcap, po, to, ldo, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                 _bad(bad, cache), cache._stream()), name)
     return out
 
 

@@ -128,6 +128,32 @@ ZEST_API int zest_kv_attn(const zest_kv_cache *cache, const zest_kv_batch *batch
                           void *out, int out_type, int64_t ldo, void *workspace, size_t workspace_bytes, uint32_t *bad,
                           void *stream);
 
+/* Sequences that share what they say first: group g is the sequences
+ * starts[g] .. starts[g+1]-1 of a batch (device; they do not decrease; a sequence
+ * outside all groups shares nothing). What a group shares is found on the device:
+ * the leading whole pages that the tables of all its members name alike, as far as
+ * all its rows see all of them, and max_shared tokens at most. So a group is only
+ * ever a hint, and forks of one prompt (zest_kv_assign) one after the other in a
+ * batch are such a group. */
+typedef struct {
+    const int32_t *starts; /* [groups + 1], device */
+    int32_t groups;        /* 1 .. 4096 */
+    int32_t max_shared;    /* 0 .. 2^30 */
+} zest_kv_groups;
+
+/* zest_kv_attn where the batch's sequences come in groups: the same result but for
+ * the order in which its sums are rounded, what a group shares being read once for
+ * all its rows and joined with what each sequence holds of its own. Arguments and
+ * limits as zest_kv_attn's; a group's starts outside 0 .. seqs, or going back, are
+ * reported, and that group shares nothing. table_rows * table_cols < 2^31. The
+ * workspace is zest_kv_attn_shared_workspace's. */
+ZEST_API size_t zest_kv_attn_shared_workspace(const zest_kv_cache *cache, const zest_kv_batch *batch,
+                                              const zest_kv_groups *groups, int32_t q_heads);
+ZEST_API int zest_kv_attn_shared(const zest_kv_cache *cache, const zest_kv_batch *batch, const zest_kv_groups *groups,
+                                 const void *q, int q_type, int64_t ldq, int32_t q_heads, float scale, int causal,
+                                 int32_t window, float softcap, void *out, int out_type, int64_t ldo, void *workspace,
+                                 size_t workspace_bytes, uint32_t *bad, void *stream);
+
 /* Scratch bytes of zest_kv_assign (n entries) and zest_kv_compact (n = 0). */
 ZEST_API size_t zest_kv_scratch_bytes(int64_t pages, int32_t n);
 
