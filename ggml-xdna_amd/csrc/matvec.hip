@@ -5,6 +5,7 @@
 // halves of 16: the low and the high nibbles (Q8_0: 32 bytes, its first and last
 // 16). Every half is code * scale + offset, codes signed bytes.
 #include <algorithm>
+#include <atomic>
 
 #include "kv_device.h"
 #include "zest/decode.h"
@@ -178,73 +179,296 @@ template <> struct quant<ZEST_TYPE_IQ4_XS> {
     }
 };
 
+constexpr int GROUPS = 4;        // lane groups of a wave: each takes a chunk of a step
+constexpr int CELL = 112;        // bytes of a chunk of one row of x, as prepared: digits, factors, sums
+constexpr int LDS_MOST = 160 * 1024;
+
 struct matvec_args {
     const float * x;
     int64_t ldx, row_bytes;
-    int32_t M, chunks, n, glu;   // chunks of a row; glu: the kind, -1: none
+    int32_t M, chunks, glu;      // chunks of a row; glu: the kind, -1: none
     const uint8_t * w[MAX_N];
     const float * res[MAX_N];
     float * y[MAX_N];
     int64_t ldy[MAX_N], ldr[MAX_N];
-    int32_t N[MAX_N];
-    int32_t rows;                // output rows in all (of a GLU: of one weight)
+    int32_t N[MAX_N], tiles[MAX_N];  // tiles: of the weights up to this one
+    int32_t n, all_tiles;
+    int32_t wk, wr;              // waves that share a tile's chunks, tiles of a workgroup
+    int32_t seg_steps, segs;     // steps of a segment of K, segments
+    uint8_t * cells;             // prepared by prepare_kernel, [chunk][row]
 };
 
-// A wave an output row (a pair of them for a GLU), a lane every 64th chunk.
-template <int TYPE> __device__ inline void dot_row(const matvec_args & a, const uint8_t * row, float acc[MAX_M]) {
-    typedef quant<TYPE> Q;
-    const int lane = threadIdx.x & 63;
+// x as whole numbers: of every 32 consecutive values (whose largest magnitude lies
+// in [2^e, 2^(e+1))) v = rint(x 2^(21-e)), |v| < 2^22, cut in three signed bytes v =
+// d0 2^16 + d1 2^8 + d2. So products with the weights' codes are exact, in 32 bits,
+// and a row of x is met to 2^-22 of the largest of its 32. A cell: [half][digit][16
+// bytes], the halves' factors 2^(e-21) (NaN where a value is not finite), their sums.
+//
+// Eight lanes prepare 32 values of a row, four each; the values past 2^-126 of
+// nothing (e below -105) count as zeros.
+template <int TYPE> __device__ inline void prepare(const float * x, int64_t ldx, int block, int m, int M, int j, uint8_t * cells) {
+    const float4 f = *reinterpret_cast<const float4 *>(x + m * ldx + (int64_t) block * 32 + j * 4);
+    const float v[4] = {f.x, f.y, f.z, f.w};
+    uint32_t e = 22;
 #pragma unroll
-    for (int m = 0; m < MAX_M; m++) acc[m] = 0.0f;
-    for (int c = lane; c < a.chunks; c += 64) {
-        const typename Q::raw r = Q::load(row, c);
-        uint32_t q[2][4];
-        Q::codes(r, q);
-        const half_scales s = Q::scales(r, c);
+    for (int i = 0; i < 4; i++) e = max(e, __float_as_uint(v[i]) >> 23 & 0xffu);
+    float sum = (v[0] + v[1]) + (v[2] + v[3]);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const float * x = a.x + half_column<TYPE>(c, h);
+    for (int off = 1; off < 8; off <<= 1) e = max(e, (uint32_t) __shfl_xor((int) e, off));
+    sum += __shfl_xor(sum, 1);
+    sum += __shfl_xor(sum, 2);
+    const bool odd = e == 255;
+    const float up = odd ? 0.0f : __uint_as_float((275 - e) << 23), down = odd ? NAN : __uint_as_float((e - 21) << 23);
+    uint32_t d[3] = {0, 0, 0};
 #pragma unroll
-            for (int m = 0; m < MAX_M; m++) {
-                if (m >= a.M) continue;
-                float dot = 0.0f, sum = 0.0f, odd = 0.0f;  // odd: NaN where a value of x is not finite
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4 v = *reinterpret_cast<const float4 *>(x + m * a.ldx + 4 * i);
-                    const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        dot = fmaf(e[j], (float) (int8_t) (q[h][i] >> 8 * j), dot);
-                        sum += e[j];
-                        odd = fmaf(e[j], 0.0f, odd);
-                    }
-                }
-                acc[m] = fmaf(dot, s.scale[h], fmaf(sum, s.offset[h], acc[m])) + odd;
-            }
-        }
+    for (int i = 0; i < 4; i++) {
+        const int q = odd ? 0 : (int) __builtin_rintf(v[i] * up);
+        const int d2 = (int8_t) q, q1 = (q - d2) >> 8, d1 = (int8_t) q1, d0 = (q1 - d1) >> 8;
+        d[0] |= (uint32_t) (d0 & 255) << 8 * i;
+        d[1] |= (uint32_t) (d1 & 255) << 8 * i;
+        d[2] |= (uint32_t) (d2 & 255) << 8 * i;
     }
+    // the half's place: Q4_K's chunks hold a half each of two sub-blocks
+    const int chunk = TYPE == ZEST_TYPE_Q4_K ? (block & ~1) + (j >> 2) : block, half = TYPE == ZEST_TYPE_Q4_K ? block & 1 : j >> 2;
+    uint8_t * cell = cells + (int64_t) (chunk * M + m) * CELL;
 #pragma unroll
-    for (int m = 0; m < MAX_M; m++)
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) acc[m] += __shfl_xor(acc[m], off);
+    for (int i = 0; i < 3; i++) *reinterpret_cast<uint32_t *>(cell + half * 48 + i * 16 + (j & 3) * 4) = d[i];
+    if ((j & 3) == 0) {
+        *reinterpret_cast<float *>(cell + 96 + half * 4) = down;
+        *reinterpret_cast<float *>(cell + 104 + half * 4) = sum;
+    }
 }
 
-template <int TYPE> __global__ __launch_bounds__(256) void matvec_kernel(matvec_args a) {
-    int64_t row = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.rows) return;
+template <int TYPE> __global__ __launch_bounds__(256) void prepare_kernel(matvec_args a) {
+    const int i = (blockIdx.x * 256 + threadIdx.x) >> 3, m = blockIdx.y;
+    if (i < a.chunks) prepare<TYPE>(a.x, a.ldx, i, m, a.M, threadIdx.x & 7, a.cells);
+}
+
+// The rows of a tile: of a weight, or of a GLU's gate and up.
+struct tile_rows {
+    int32_t weight, row0;
+};
+__device__ inline tile_rows tile_of(const matvec_args & a, int tile) {
     int i = 0;
-    if (a.glu < 0)
-        while (row >= a.N[i]) row -= a.N[i++];
-    float acc[MAX_M], up[MAX_M];
-    dot_row<TYPE>(a, a.w[i] + row * a.row_bytes, acc);
-    if (a.glu >= 0) dot_row<TYPE>(a, a.w[1] + row * a.row_bytes, up);
-    if ((threadIdx.x & 63) != 0) return;
-    for (int m = 0; m < MAX_M; m++) {
-        if (m >= a.M) continue;
-        float v = a.glu >= 0 ? zest::glu(a.glu, acc[m], up[m]) : acc[m];
-        if (a.res[i]) v += a.res[i][m * a.ldr[i] + row];
-        a.y[i][m * a.ldy[i] + row] = v;
+    while (i < a.n - 1 && tile >= a.tiles[i]) i++;
+    return {i, (tile - (i ? a.tiles[i - 1] : 0)) * 16};
+}
+
+// A tile is 16 rows of a weight (S = 2: of a GLU's two), a step four chunks of them:
+// a lane loads one chunk of one row, 16 bytes of codes (lane l: row l % 16, chunk l /
+// 16), and v_mfma_i32_16x16x64_i8 multiplies each lane's 16 codes of a half with the
+// three digits of a row of x for its own chunk: the first operand's row 4 b + i is
+// digit i of lane group b's chunk, and zero for the other groups' places, so that
+// lane (row, b) of the result holds its own chunk's three sums in its first three
+// registers. Scales are then one value a lane, and a chunk costs a lane a conversion
+// and a few fused products for a row of x.
+//
+// HBM bound: a weight's bytes once. The waves of a tile (a.wk of them) share out its
+// steps and are joined in shared memory; BLOCK steps of a wave are in flight while it
+// computes the last BLOCK.
+template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) void matvec_kernel(matvec_args a) {
+    typedef quant<TYPE> Q;
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    constexpr int BLOCK = S == 2 ? 2 : 4;
+    constexpr bool ONE_SCALE = TYPE != ZEST_TYPE_Q4_K, OFFSETS = TYPE == ZEST_TYPE_Q4_K || TYPE == ZEST_TYPE_Q4_1;
+    extern __shared__ __align__(16) uint8_t sh[];
+    // sh: 16 zeros, the cells of a segment, the waves' results
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 4, col = lane & 15;
+    const int wr = wave / a.wk, wk = wave - wr * a.wk;
+    const int M = a.M, steps = (a.chunks + GROUPS - 1) / GROUPS, segs = COPY ? a.segs : 1, seg_steps = COPY ? a.seg_steps : steps;
+    uint8_t * const cells = sh + 16;
+    float * const red = reinterpret_cast<float *>(cells + (int64_t) min(seg_steps * GROUPS, a.chunks) * M * CELL);
+    const int wg_tiles = (a.all_tiles + a.wr - 1) / a.wr, rounds = (wg_tiles - (int) blockIdx.x + gridDim.x - 1) / gridDim.x;
+
+    struct place {
+        int round, seg, first;  // of a block of this wave's steps
+    };
+    // steps of segment s that are this wave's: s * seg_steps + wk + i * a.wk
+    auto count = [&](int seg) { return max(0, (min(seg_steps, steps - seg * seg_steps) - wk + a.wk - 1) / a.wk); };
+    auto rows_of = [&](int round) { return ((int) blockIdx.x + round * (int) gridDim.x) * a.wr + wr; };
+    auto next = [&](place p) {
+        p.first += BLOCK;
+        if (p.first >= count(p.seg)) {
+            p.first = 0;
+            if (++p.seg == segs) {
+                p.seg = 0;
+                p.round++;
+            }
+        }
+        return p;
+    };
+    auto load = [&](typename Q::raw (&buf)[BLOCK][S], place p) {
+        if (p.round >= rounds) return;
+        const int tile = rows_of(p.round);
+        if (tile >= a.all_tiles) return;
+        const tile_rows t = tile_of(a, tile);
+        const int row = min(t.row0 + col, a.N[t.weight] - 1), n = count(p.seg);
+        const uint8_t * at[S];
+#pragma unroll
+        for (int s = 0; s < S; s++) at[s] = a.w[S == 2 ? s : t.weight] + row * a.row_bytes;
+#pragma unroll
+        for (int i = 0; i < BLOCK; i++) {
+            if (p.first + i >= n) continue;
+            const int chunk = min((p.seg * seg_steps + wk + (p.first + i) * a.wk) * GROUPS + group, a.chunks - 1);
+#pragma unroll
+            for (int s = 0; s < S; s++) buf[i][s] = Q::load(at[s], chunk);
+        }
+    };
+
+    float acc[T][S];
+    auto clear = [&]() {
+#pragma unroll
+        for (int m = 0; m < T; m++)
+#pragma unroll
+            for (int s = 0; s < S; s++) acc[m][s] = 0.0f;
+    };
+    // this lane's part of the first operand: digit col % 4 of its group's chunk, if its
+    // row is the group's, else zeros
+    const bool digit = (col >> 2) == group && (col & 3) < 3;
+    auto compute = [&](const typename Q::raw (&buf)[BLOCK][S], place p) {
+        const int n = count(p.seg);
+#pragma unroll
+        for (int i = 0; i < BLOCK; i++) {
+            if (p.first + i >= n) continue;
+            const int step = wk + (p.first + i) * a.wk, chunk = (p.seg * seg_steps + step) * GROUPS + group;
+            const bool in = chunk < a.chunks;
+            const int local = step * GROUPS + (in ? group : 0);
+            i32x4 code[S][2];
+            half_scales sc[S];
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                uint32_t c[2][4];
+                Q::codes(buf[i][s], c);
+#pragma unroll
+                for (int h = 0; h < 2; h++) code[s][h] = i32x4{(int) c[h][0], (int) c[h][1], (int) c[h][2], (int) c[h][3]};
+                sc[s] = Q::scales(buf[i][s], min(chunk, a.chunks - 1));
+                if (!in) sc[s] = half_scales{{0.0f, 0.0f}, {0.0f, 0.0f}};
+            }
+            const uint8_t * cell = cells + local * M * CELL;
+            const uint8_t * from = digit && in ? cell + (col & 3) * 16 : sh;
+            const int stride = digit && in ? CELL : 0, half_at = digit && in ? 48 : 0;
+#pragma unroll
+            for (int m = 0; m < T; m++) {
+                if (m >= M) continue;
+                const i32x4 x0 = *reinterpret_cast<const i32x4 *>(from + m * stride), x1 = *reinterpret_cast<const i32x4 *>(from + m * stride + half_at);
+                const float4 f = *reinterpret_cast<const float4 *>(cell + m * CELL + 96);  // the halves' factors and sums
+#pragma unroll
+                for (int s = 0; s < S; s++) {
+                    auto number = [](i32x4 d) { return fmaf((float) d[0], 65536.0f, (float) ((d[1] << 8) + d[2])); };
+                    i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x0, code[s][0], i32x4{}, 0, 0, 0);
+                    if constexpr (ONE_SCALE) {
+                        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x1, code[s][1], d, 0, 0, 0);
+                        acc[m][s] = fmaf(number(d), sc[s].scale[0] * f.x, acc[m][s]);
+                        if constexpr (OFFSETS) acc[m][s] = fmaf(f.z + f.w, sc[s].offset[0], acc[m][s]);
+                    } else {
+                        const i32x4 e = __builtin_amdgcn_mfma_i32_16x16x64_i8(x1, code[s][1], i32x4{}, 0, 0, 0);
+                        acc[m][s] = fmaf(number(d), sc[s].scale[0] * f.x, acc[m][s]);
+                        acc[m][s] = fmaf(number(e), sc[s].scale[1] * f.y, acc[m][s]);
+                        acc[m][s] = fmaf(f.z, sc[s].offset[0], acc[m][s]);
+                        acc[m][s] = fmaf(f.w, sc[s].offset[1], acc[m][s]);
+                    }
+                }
+            }
+        }
+    };
+    // the cells of a segment, in shared memory
+    auto fill = [&](int seg) {
+        if (threadIdx.x < 4) reinterpret_cast<uint32_t *>(sh)[threadIdx.x] = 0;
+        if constexpr (COPY) {
+            const int first = seg * seg_steps * GROUPS, n = min(seg_steps * GROUPS, a.chunks - first) * M * (CELL / 16);
+            const uint4 * from = reinterpret_cast<const uint4 *>(a.cells + (int64_t) first * M * CELL);
+            for (int i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<uint4 *>(cells)[i] = from[i];
+        } else {
+            const int lanes = a.chunks * 8;
+            for (int i = threadIdx.x; i < lanes; i += blockDim.x)
+                for (int m = 0; m < M; m++) prepare<TYPE>(a.x, a.ldx, i >> 3, m, M, i & 7, cells);
+        }
+        __syncthreads();
+    };
+    // the waves' sums of a round's tiles: of the lane groups, then of the waves
+    auto finish = [&](int round) {
+        float * const mine = red + wave * T * S * 16;
+#pragma unroll
+        for (int m = 0; m < T; m++) {
+            if (m >= M) continue;
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                float v = acc[m][s];
+                v += __shfl_xor(v, 16);
+                v += __shfl_xor(v, 32);
+                if (group == 0) mine[(m * S + s) * 16 + col] = v;
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.wr * M * 16; i += blockDim.x) {
+            const int c = i & 15, m = (i >> 4) % M, r = (i >> 4) / M, tile = ((int) blockIdx.x + round * (int) gridDim.x) * a.wr + r;
+            if (tile >= a.all_tiles) continue;
+            const tile_rows t = tile_of(a, tile);
+            const int row = t.row0 + c;
+            if (row >= a.N[t.weight]) continue;
+            float v[S];
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                v[s] = 0.0f;
+                for (int w = 0; w < a.wk; w++) v[s] += red[((r * a.wk + w) * T * S + m * S + s) * 16 + c];
+            }
+            float out = S == 2 ? zest::glu(a.glu, v[0], v[S - 1]) : v[0];
+            if (a.res[t.weight]) out += a.res[t.weight][m * a.ldr[t.weight] + row];
+            a.y[t.weight][m * a.ldy[t.weight] + row] = out;
+        }
+        __syncthreads();
+    };
+    // one block: the next one requested, this one computed; what follows it
+    auto turn = [&](typename Q::raw (&now)[BLOCK][S], typename Q::raw (&then)[BLOCK][S], place p) {
+        const place q = next(p);
+        if (p.first == 0) {
+            if (p.seg == 0) clear();
+            if (segs > 1 || p.round == 0) {
+                if (segs > 1) __syncthreads();
+                fill(p.seg);
+            }
+        }
+        load(then, q);
+        if (rows_of(p.round) < a.all_tiles) compute(now, p);
+        if (q.round != p.round) finish(p.round);
+        return q;
+    };
+    typename Q::raw one[BLOCK][S], two[BLOCK][S];
+    place p{0, 0, 0};
+    load(one, p);
+    while (p.round < rounds) {
+        p = turn(one, two, p);
+        if (p.round < rounds) p = turn(two, one, p);
     }
+}
+
+// ---- the host's plan ----------------------------------------------------------------
+
+struct matvec_plan {
+    int wk, wr, workgroups, seg_steps, segs;
+    bool copy;        // x is prepared by a kernel of its own
+    size_t lds, bytes;
+};
+
+matvec_plan plan_of(int64_t M, int64_t K, int n, const int64_t * N, bool glu) {
+    matvec_plan p{};
+    const int chunks = (int) (K / 32), steps = (chunks + GROUPS - 1) / GROUPS, T = M <= 4 ? 4 : M <= 8 ? 8 : 16, S = glu ? 2 : 1;
+    int64_t tiles = 0;
+    for (int i = 0; i < (glu ? 1 : n); i++) tiles += (N[i] + 15) / 16;
+    p.wr = tiles <= 2 * 256 ? 1 : tiles <= 8 * 256 ? 2 : 4;
+    const int most = p.wr == 1 && tiles > 256 ? 8 : 16 / p.wr;
+    p.wk = 1;
+    for (int w = 1; w <= most; w++)
+        if ((steps + w - 1) / w < (steps + p.wk - 1) / p.wk) p.wk = w;
+    const size_t red = (size_t) p.wk * p.wr * T * S * 16 * 4, room = LDS_MOST - 16 - red;
+    p.seg_steps = (int) std::min<size_t>(steps, room / ((size_t) GROUPS * M * CELL));
+    p.segs = (steps + p.seg_steps - 1) / p.seg_steps;
+    p.copy = p.segs > 1 || M > 4;
+    p.lds = 16 + (size_t) std::min(p.seg_steps * GROUPS, chunks) * M * CELL + red;
+    p.workgroups = (int) std::min<int64_t>((tiles + p.wr - 1) / p.wr, 512);
+    if (p.lds > LDS_MOST / 2 || p.wk * p.wr > 8) p.workgroups = std::min(p.workgroups, 256);
+    p.bytes = std::max<size_t>(16, p.copy ? (size_t) chunks * M * CELL : 0);
+    return p;
 }
 
 bool supported(int type) {
@@ -261,17 +485,48 @@ bool supported(int type) {
 
 bool aligned(const void * p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-int launch(int type, const matvec_args & a, hipStream_t s, const char * me) {
-    const dim3 grid((unsigned) ((a.rows + 3) / 4)), block(256);
-    switch (type) {
-        case ZEST_TYPE_Q4_0: hipLaunchKernelGGL(matvec_kernel<ZEST_TYPE_Q4_0>, grid, block, 0, s, a); break;
-        case ZEST_TYPE_Q4_1: hipLaunchKernelGGL(matvec_kernel<ZEST_TYPE_Q4_1>, grid, block, 0, s, a); break;
-        case ZEST_TYPE_Q8_0: hipLaunchKernelGGL(matvec_kernel<ZEST_TYPE_Q8_0>, grid, block, 0, s, a); break;
-        case ZEST_TYPE_Q4_K: hipLaunchKernelGGL(matvec_kernel<ZEST_TYPE_Q4_K>, grid, block, 0, s, a); break;
-        case ZEST_TYPE_IQ4_NL: hipLaunchKernelGGL(matvec_kernel<ZEST_TYPE_IQ4_NL>, grid, block, 0, s, a); break;
-        default: hipLaunchKernelGGL(matvec_kernel<ZEST_TYPE_IQ4_XS>, grid, block, 0, s, a); break;
-    }
+// Lets a kernel have all of a CU's shared memory, once a device (threads that launch
+// it for the first time at once set the same value).
+template <auto KERNEL> int allow_lds(const char * me) {
+    static std::atomic<uint64_t> set{0};  // a bit a device, those past the 64th every time
+    int device = 0;
+    if (const hipError_t e = hipGetDevice(&device); e != hipSuccess) return zest::fail(ZEST_E_HIP, "%s: current device: %s", me, hipGetErrorString(e));
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (set.load(std::memory_order_acquire) & bit) return ZEST_OK;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, LDS_MOST);
+    if (e != hipSuccess) return zest::fail(ZEST_E_HIP, "%s: shared memory attribute: %s", me, hipGetErrorString(e));
+    set.fetch_or(bit, std::memory_order_release);
+    return ZEST_OK;
+}
+
+template <int TYPE, int T, int S, bool COPY> int launch(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
+    if (const int st = allow_lds<&matvec_kernel<TYPE, T, S, COPY>>(me)) return st;
+    if (COPY) hipLaunchKernelGGL(prepare_kernel<TYPE>, dim3((unsigned) ((a.chunks * 8 + 255) / 256), (unsigned) a.M), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((matvec_kernel<TYPE, T, S, COPY>), dim3((unsigned) p.workgroups), dim3((unsigned) (p.wk * p.wr * 64)), p.lds, s, a);
     return zest::check_launch(me);
+}
+
+template <int TYPE, int S> int launch(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
+    if (a.M > 8) return launch<TYPE, 16, S, true>(a, p, s, me);
+    if (a.M > 4) return launch<TYPE, 8, S, true>(a, p, s, me);
+    if (p.copy) return launch<TYPE, 4, S, true>(a, p, s, me);
+    if (a.M > 2) return launch<TYPE, 4, S, false>(a, p, s, me);
+    return a.M > 1 ? launch<TYPE, 2, S, false>(a, p, s, me) : launch<TYPE, 1, S, false>(a, p, s, me);
+}
+
+template <int TYPE> int launch(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
+    return a.glu >= 0 ? launch<TYPE, 2>(a, p, s, me) : launch<TYPE, 1>(a, p, s, me);
+}
+
+int launch(int type, const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
+    switch (type) {
+        case ZEST_TYPE_Q4_0: return launch<ZEST_TYPE_Q4_0>(a, p, s, me);
+        case ZEST_TYPE_Q4_1: return launch<ZEST_TYPE_Q4_1>(a, p, s, me);
+        case ZEST_TYPE_Q8_0: return launch<ZEST_TYPE_Q8_0>(a, p, s, me);
+        case ZEST_TYPE_Q4_K: return launch<ZEST_TYPE_Q4_K>(a, p, s, me);
+        case ZEST_TYPE_IQ4_NL: return launch<ZEST_TYPE_IQ4_NL>(a, p, s, me);
+        default: return launch<ZEST_TYPE_IQ4_XS>(a, p, s, me);
+    }
 }
 
 // The checks and the launch of both entry points; glu: the kind, -1: none.
@@ -291,15 +546,16 @@ int matvec(const char * me, int glu, int type, const float * x, int64_t M, int64
     a.row_bytes = (int64_t) row_bytes;
     a.M = (int32_t) M;
     a.chunks = (int32_t) (K / 32);
-    a.n = n;
+    a.n = outs;
     a.glu = glu;
-    int64_t rows = 0;
+    int64_t tiles = 0;
     for (int i = 0; i < n; i++) {
         ZEST_REQUIRE(w[i] && aligned(w[i], row_align(type)), "%s: weight %d: rows %d-byte aligned wanted", me, i, row_align(type));
         ZEST_REQUIRE(N[i] > 0 && N[i] <= (1 << 26), "%s: weight %d: N=%lld", me, i, (long long) N[i]);
         a.w[i] = (const uint8_t *) w[i];
         a.N[i] = (int32_t) N[i];
-        if (i < outs) rows += N[i];
+        if (i < outs) tiles += (N[i] + 15) / 16;
+        a.tiles[i] = (int32_t) tiles;
     }
     for (int i = 0; i < outs; i++) {
         ZEST_REQUIRE(y[i] && aligned(y[i], 4) && (M == 1 || (ldy[i] >= N[i] && ldy[i] < (1ll << 31))), "%s: output %d: ldy=%lld for N=%lld", me, i, (long long) (M == 1 ? 0 : ldy[i]),
@@ -325,10 +581,13 @@ int matvec(const char * me, int glu, int type, const float * x, int64_t M, int64
                          "%s: output %d overlaps residual %d without being it", me, i, j);
         }
     }
-    ZEST_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= zest_matvec_workspace(type, M, K, n, N), "%s: workspace of %zu bytes, 16-byte aligned, wanted", me,
-                 zest_matvec_workspace(type, M, K, n, N));
-    a.rows = (int32_t) rows;
-    return launch(type, a, zest::as_stream(stream), me);
+    // (a GLU's plan is that of two weights as far as its workspace goes)
+    const matvec_plan p = plan_of(M, K, n, N, glu >= 0);
+    ZEST_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= p.bytes, "%s: workspace of %zu bytes, 16-byte aligned, wanted", me, p.bytes);
+    a.all_tiles = (int32_t) tiles;
+    a.wk = p.wk, a.wr = p.wr, a.seg_steps = p.seg_steps, a.segs = p.segs;
+    a.cells = (uint8_t *) workspace;
+    return launch(type, a, p, zest::as_stream(stream), me);
 }
 
 } // namespace
@@ -337,7 +596,7 @@ extern "C" {
 
 size_t zest_matvec_workspace(int type, int64_t M, int64_t K, int n, const int64_t * N) {
     if (!supported(type) || M <= 0 || M > MAX_M || K <= 0 || K > (1 << 20) || n < 1 || n > MAX_N || !N) return 0;
-    return 16;
+    return std::max<size_t>(16, (size_t) (K / 32) * M * CELL);
 }
 
 int zest_matvec(int type, const float * x, int64_t M, int64_t K, int64_t ldx, int n, const void * const * w, const int64_t * N,
