@@ -1,11 +1,12 @@
 // Products of a few rows with GGUF weights as they are (include/zest/decode.h):
 // y[m][n] = sum_k x[m][k] W[n][k], HBM bound by the weights' bytes.
 //
-// A chunk is 32 of a weight row's values, of which 16 bytes of codes hold two
-// halves of 16: the low and the high nibbles (Q8_0: 32 bytes, its first and last
-// 16). Every half is code * scale + offset, codes signed bytes.
+// A chunk is what a lane loads of a weight row at a time: 32 values, of Q4_K 64. Its
+// codes, signed bytes, come in parts of 16; two parts are a block of 32 consecutive
+// values, w = code * scale + offset.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kv_device.h"
 #include "zest/decode.h"
@@ -25,63 +26,62 @@ template <typename T> __device__ inline T load_as(const uint8_t * p) {
     return v;
 }
 
-// The published levels of IQ4_NL and IQ4_XS, four codes (0..15, one a byte) at a
-// time: two byte permutes look up the low and the high eight, bit 3 picks.
-__device__ inline uint32_t iq4_levels(uint32_t n) {
-    constexpr auto b = [](int v) { return (uint32_t) (v & 255); };
+// The published levels of IQ4_NL and IQ4_XS, for the low or the high nibbles of four
+// bytes: two byte permutes look up the low and the high eight, and a mask that a
+// permute makes of the codes' top bits (it can spread the sign of every other byte)
+// picks.
+__device__ inline uint32_t iq4_levels(uint32_t n, bool high) {
     constexpr auto four = [](int x, int y, int z, int w) { return (uint32_t) (x & 255) | (uint32_t) (y & 255) << 8 | (uint32_t) (z & 255) << 16 | (uint32_t) (w & 255) << 24; };
     constexpr uint32_t T0 = four(-127, -104, -83, -65), T1 = four(-49, -35, -22, -10), T2 = four(1, 13, 25, 38), T3 = four(53, 69, 89, 113);
-    const uint32_t sel = n & 0x07070707u;
-    const uint32_t lo = __builtin_amdgcn_perm(T1, T0, sel), hi = __builtin_amdgcn_perm(T3, T2, sel);
-    const uint32_t m = ((n >> 3) & 0x01010101u) * 0xffu;
-    return (hi & m) | (lo & ~m);
-}
-
-// Of a type: bytes of a block, chunks of a block, the loads of a chunk, and what
-// they stand for.
-template <int TYPE> struct quant;
-
-// A chunk's halves: codes (four to a word) and w = scale * code + offset.
-struct half_scales {
-    float scale[2], offset[2];
-};
-
-// The first of a half's 16 columns, and the row's alignment.
-template <int TYPE> __device__ inline int64_t half_column(int64_t chunk, int half) {
-    if constexpr (TYPE == ZEST_TYPE_Q4_K) return chunk / 2 * 64 + chunk % 2 * 16 + half * 32;
-    return chunk * 32 + half * 16;
+    const uint32_t sel = (high ? n >> 4 : n) & 0x07070707u, top = high ? n : n << 4;  // top bits in bit 7
+    const uint32_t m = __builtin_amdgcn_perm(top << 8, top, 0x090b080au);
+    return (__builtin_amdgcn_perm(T3, T2, sel) & m) | (__builtin_amdgcn_perm(T1, T0, sel) & ~m);
 }
 
 constexpr int row_align(int type) {
     return type == ZEST_TYPE_Q4_K ? 16 : type == ZEST_TYPE_IQ4_XS ? 8 : type == ZEST_TYPE_Q4_1 ? 4 : 2;
 }
 
-// d, qs[16]: w = d (q - 8), or d level[q]
+// Of a type: blocks of a chunk, whether codes are nibbles as they are (0..15), whether
+// there are offsets; a chunk's loads, codes and scales.
+template <int TYPE> struct quant;
+
+template <int BLOCKS> struct block_scales {
+    float scale[BLOCKS], offset[BLOCKS];
+};
+
+__device__ inline void words(const uint4 & q, uint32_t w[4]) {
+    w[0] = q.x;
+    w[1] = q.y;
+    w[2] = q.z;
+    w[3] = q.w;
+}
+
+// d, qs[16], the low nibbles the first 16 values: w = d (q - 8), or d level[q]
 template <int TYPE> struct quant_nibbles {
     struct raw { uint4 q; uint32_t d; };
-    static constexpr int BYTES = 18, CHUNKS = 1;
-    static __device__ raw load(const uint8_t * row, int64_t chunk) {
-        const uint8_t * p = row + chunk * BYTES;
+    static constexpr int BLOCKS = 1;
+    static constexpr bool NIBBLES = false, OFFSETS = false;
+    static __device__ raw load(const uint8_t * row, int chunk) {
+        const uint8_t * p = row + chunk * 18;
         return {load_as<uint4>(p + 2), load_as<uint16_t>(p)};
     }
-    static __device__ void codes(const raw & r, uint32_t c[2][4]) {
-        const uint32_t w[4] = {r.q.x, r.q.y, r.q.z, r.q.w};
+    static __device__ void codes(const raw & r, uint32_t c[1][2][4]) {
+        uint32_t w[4];
+        words(r.q, w);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if constexpr (TYPE == ZEST_TYPE_Q4_0) {
                 const uint32_t s = w[i] ^ 0x88888888u;  // 16 (q - 8), the nibble as a byte's high half
-                c[0][i] = s << 4 & 0xf0f0f0f0u;
-                c[1][i] = s & 0xf0f0f0f0u;
+                c[0][0][i] = s << 4 & 0xf0f0f0f0u;
+                c[0][1][i] = s & 0xf0f0f0f0u;
             } else {
-                c[0][i] = iq4_levels(w[i] & 0x0f0f0f0fu);
-                c[1][i] = iq4_levels(w[i] >> 4 & 0x0f0f0f0fu);
+                c[0][0][i] = iq4_levels(w[i], false);
+                c[0][1][i] = iq4_levels(w[i], true);
             }
         }
     }
-    static __device__ half_scales scales(const raw & r, int64_t) {
-        const float d = half_to_float(r.d) * (TYPE == ZEST_TYPE_Q4_0 ? 0.0625f : 1.0f);
-        return {{d, d}, {0.0f, 0.0f}};
-    }
+    static __device__ block_scales<1> scales(const raw & r, int) { return {{half_to_float(r.d) * (TYPE == ZEST_TYPE_Q4_0 ? 0.0625f : 1.0f)}, {0.0f}}; }
 };
 template <> struct quant<ZEST_TYPE_Q4_0> : quant_nibbles<ZEST_TYPE_Q4_0> {};
 template <> struct quant<ZEST_TYPE_IQ4_NL> : quant_nibbles<ZEST_TYPE_IQ4_NL> {};
@@ -89,104 +89,101 @@ template <> struct quant<ZEST_TYPE_IQ4_NL> : quant_nibbles<ZEST_TYPE_IQ4_NL> {};
 // d, m, qs[16]: w = d q + m
 template <> struct quant<ZEST_TYPE_Q4_1> {
     struct raw { uint4 q; uint32_t dm; };
-    static constexpr int BYTES = 20, CHUNKS = 1;
-    static __device__ raw load(const uint8_t * row, int64_t chunk) {
-        const uint8_t * p = row + chunk * BYTES;
+    static constexpr int BLOCKS = 1;
+    static constexpr bool NIBBLES = true, OFFSETS = true;
+    static __device__ raw load(const uint8_t * row, int chunk) {
+        const uint8_t * p = row + chunk * 20;
         return {load_as<uint4>(p + 4), load_as<uint32_t>(p)};
     }
-    static __device__ void codes(const raw & r, uint32_t c[2][4]) {
-        const uint32_t w[4] = {r.q.x, r.q.y, r.q.z, r.q.w};
+    static __device__ void codes(const raw & r, uint32_t c[1][2][4]) {
+        uint32_t w[4];
+        words(r.q, w);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            c[0][i] = w[i] & 0x0f0f0f0fu;
-            c[1][i] = w[i] >> 4 & 0x0f0f0f0fu;
+            c[0][0][i] = w[i] & 0x0f0f0f0fu;
+            c[0][1][i] = w[i] >> 4 & 0x0f0f0f0fu;
         }
     }
-    static __device__ half_scales scales(const raw & r, int64_t) {
-        const float d = half_to_float(r.dm), m = half_to_float(r.dm >> 16);
-        return {{d, d}, {m, m}};
-    }
+    static __device__ block_scales<1> scales(const raw & r, int) { return {{half_to_float(r.dm)}, {half_to_float(r.dm >> 16)}}; }
 };
 
 // d, qs[32]: w = d q
 template <> struct quant<ZEST_TYPE_Q8_0> {
     struct raw { uint4 q[2]; uint32_t d; };
-    static constexpr int BYTES = 34, CHUNKS = 1;
-    static __device__ raw load(const uint8_t * row, int64_t chunk) {
-        const uint8_t * p = row + chunk * BYTES;
+    static constexpr int BLOCKS = 1;
+    static constexpr bool NIBBLES = false, OFFSETS = false;
+    static __device__ raw load(const uint8_t * row, int chunk) {
+        const uint8_t * p = row + chunk * 34;
         return {{load_as<uint4>(p + 2), load_as<uint4>(p + 18)}, load_as<uint16_t>(p)};
     }
-    static __device__ void codes(const raw & r, uint32_t c[2][4]) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            c[h][0] = r.q[h].x;
-            c[h][1] = r.q[h].y;
-            c[h][2] = r.q[h].z;
-            c[h][3] = r.q[h].w;
-        }
+    static __device__ void codes(const raw & r, uint32_t c[1][2][4]) {
+        words(r.q[0], c[0][0]);
+        words(r.q[1], c[0][1]);
     }
-    static __device__ half_scales scales(const raw & r, int64_t) {
-        const float d = half_to_float(r.d);
-        return {{d, d}, {0.0f, 0.0f}};
-    }
+    static __device__ block_scales<1> scales(const raw & r, int) { return {{half_to_float(r.d)}, {0.0f}}; }
 };
 
-// d, dmin, 12 bytes of 6-bit scales and minima of 8 sub-blocks of 32, qs[128]: 64
-// values to 32 bytes, sub-block 2r in the low nibbles, 2r + 1 in the high ones;
+// d, dmin, 12 bytes of 6-bit scales and minima of 8 blocks of 32, qs[128]: a chunk's
+// 64 values in 32 bytes, block 2r in the low nibbles, 2r + 1 in the high ones;
 // w = d sc q - dmin m
 template <> struct quant<ZEST_TYPE_Q4_K> {
-    struct raw { uint4 q, head; };
-    static constexpr int BYTES = 144, CHUNKS = 8;
-    static __device__ raw load(const uint8_t * row, int64_t chunk) {
-        const uint8_t * p = row + (chunk >> 3) * BYTES;
-        return {*reinterpret_cast<const uint4 *>(p + 16 + (chunk & 7) * 16), *reinterpret_cast<const uint4 *>(p)};
+    struct raw { uint4 q[2], head; };
+    static constexpr int BLOCKS = 2;
+    static constexpr bool NIBBLES = true, OFFSETS = true;
+    static __device__ raw load(const uint8_t * row, int chunk) {
+        const uint8_t * p = row + (chunk >> 2) * 144;
+        const uint4 * q = reinterpret_cast<const uint4 *>(p + 16 + (chunk & 3) * 32);
+        return {{q[0], q[1]}, *reinterpret_cast<const uint4 *>(p)};
     }
-    static __device__ void codes(const raw & r, uint32_t c[2][4]) {
-        const uint32_t w[4] = {r.q.x, r.q.y, r.q.z, r.q.w};
+    static __device__ void codes(const raw & r, uint32_t c[2][2][4]) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            c[0][i] = w[i] & 0x0f0f0f0fu;
-            c[1][i] = w[i] >> 4 & 0x0f0f0f0fu;
+        for (int part = 0; part < 2; part++) {
+            uint32_t w[4];
+            words(r.q[part], w);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                c[0][part][i] = w[i] & 0x0f0f0f0fu;
+                c[1][part][i] = w[i] >> 4 & 0x0f0f0f0fu;
+            }
         }
     }
-    static __device__ half_scales scales(const raw & r, int64_t chunk) {
-        const int run = (int) (chunk & 7) >> 1;  // sub-blocks 2 run and 2 run + 1
+    static __device__ block_scales<2> scales(const raw & r, int chunk) {
         const float d = half_to_float(r.head.x), dmin = half_to_float(r.head.x >> 16);
-        // the first four sub-blocks' fields are low 6 bits, the others' 4 bits and the first's top two
-        const bool far = run >= 2;
-        const uint32_t sc = far ? (r.head.w & 0x0f0f0f0fu) | (r.head.y >> 2 & 0x30303030u) : r.head.y & 0x3f3f3f3fu;
-        const uint32_t m = far ? (r.head.w >> 4 & 0x0f0f0f0fu) | (r.head.z >> 2 & 0x30303030u) : r.head.z & 0x3f3f3f3fu;
-        const uint32_t s = sc >> 16 * (run & 1), n = m >> 16 * (run & 1);
+        // the first four blocks' fields are low 6 bits, the others' 4 bits and the first's top two
+        const bool far = chunk & 2;
+        const uint32_t a = far ? r.head.y >> 2 & 0x30303030u : r.head.y & 0x3f3f3f3fu, b = far ? r.head.z >> 2 & 0x30303030u : r.head.z & 0x3f3f3f3fu;
+        const uint32_t both = far ? r.head.w : 0u;
+        const int by = 16 * (chunk & 1);
+        const uint32_t s = ((both & 0x0f0f0f0fu) | a) >> by, n = ((both >> 4 & 0x0f0f0f0fu) | b) >> by;
         return {{d * (float) (s & 0xff), d * (float) (s >> 8 & 0xff)}, {-dmin * (float) (n & 0xff), -dmin * (float) (n >> 8 & 0xff)}};
     }
 };
 
-// d, 8 scales of 6 bits (2 above, 4 below), qs[128]: 16 bytes a sub-block of 32;
+// d, 8 scales of 6 bits (2 above, 4 below), qs[128]: 16 bytes a block of 32;
 // w = d (ls - 32) level[q]
 template <> struct quant<ZEST_TYPE_IQ4_XS> {
     struct raw { uint4 q; uint2 head; };
-    static constexpr int BYTES = 136, CHUNKS = 8;
-    static __device__ raw load(const uint8_t * row, int64_t chunk) {
-        const uint8_t * p = row + (chunk >> 3) * BYTES;
+    static constexpr int BLOCKS = 1;
+    static constexpr bool NIBBLES = false, OFFSETS = false;
+    static __device__ raw load(const uint8_t * row, int chunk) {
+        const uint8_t * p = row + (chunk >> 3) * 136;
         return {load_as<uint4>(p + 8 + (chunk & 7) * 16), *reinterpret_cast<const uint2 *>(p)};
     }
-    static __device__ void codes(const raw & r, uint32_t c[2][4]) { quant<ZEST_TYPE_IQ4_NL>::codes({r.q, 0}, c); }
-    static __device__ half_scales scales(const raw & r, int64_t chunk) {
-        const int s = (int) (chunk & 7);
-        const int ls = (r.head.y >> 4 * s & 15) | (r.head.x >> (16 + 2 * s) & 3) << 4;
-        const float d = half_to_float(r.head.x) * (float) (ls - 32);
-        return {{d, d}, {0.0f, 0.0f}};
+    static __device__ void codes(const raw & r, uint32_t c[1][2][4]) { quant<ZEST_TYPE_IQ4_NL>::codes({r.q, 0}, c); }
+    static __device__ block_scales<1> scales(const raw & r, int chunk) {
+        const int s = chunk & 7, ls = (r.head.y >> 4 * s & 15) | (r.head.x >> (16 + 2 * s) & 3) << 4;
+        return {{half_to_float(r.head.x) * (float) (ls - 32)}, {0.0f}};
     }
 };
 
 constexpr int GROUPS = 4;        // lane groups of a wave: each takes a chunk of a step
-constexpr int CELL = 112;        // bytes of a chunk of one row of x, as prepared: digits, factors, sums
+constexpr int CELL = 112;        // bytes of 32 values of a row of x, as prepared: digits, factor, sum
 constexpr int LDS_MOST = 160 * 1024;
 
 struct matvec_args {
     const float * x;
     int64_t ldx, row_bytes;
-    int32_t M, chunks, glu;      // chunks of a row; glu: the kind, -1: none
+    int32_t M, blocks, chunks, glu;  // blocks and chunks of a row; glu: the kind, -1: none
     const uint8_t * w[MAX_N];
     const float * res[MAX_N];
     float * y[MAX_N];
@@ -195,53 +192,102 @@ struct matvec_args {
     int32_t n, all_tiles;
     int32_t wk, wr;              // waves that share a tile's chunks, tiles of a workgroup
     int32_t seg_steps, segs;     // steps of a segment of K, segments
-    uint8_t * cells;             // prepared by prepare_kernel, [chunk][row]
+    uint8_t * cells;             // prepared by prepare_kernel, [block][row]
+    int32_t rows[MAX_N];         // rows: of the weights up to this one
+    int32_t pieces, each, more;  // pieces of a row; rows of a stream's workgroup
 };
+
+// Another lane's value: 0xb1 and 0x4e swap lanes and pairs of a quad, 0x141 mirrors eight.
+template <int CTRL> __device__ inline float dpp(float v) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, false)); }
+
+// The sum of a value over the four lane groups of 16.
+__device__ inline float over_groups(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
 
 // x as whole numbers: of every 32 consecutive values (whose largest magnitude lies
 // in [2^e, 2^(e+1))) v = rint(x 2^(21-e)), |v| < 2^22, cut in three signed bytes v =
 // d0 2^16 + d1 2^8 + d2. So products with the weights' codes are exact, in 32 bits,
-// and a row of x is met to 2^-22 of the largest of its 32. A cell: [half][digit][16
-// bytes], the halves' factors 2^(e-21) (NaN where a value is not finite), their sums.
+// and a row of x is met to 2^-22 of the largest of its 32. A cell: [part][digit][16
+// bytes], the factor 2^(e-21) (NaN where a value is not finite), the values' sum.
 //
-// Eight lanes prepare 32 values of a row, four each; the values past 2^-126 of
-// nothing (e below -105) count as zeros.
-template <int TYPE> __device__ inline void prepare(const float * x, int64_t ldx, int block, int m, int M, int j, uint8_t * cells) {
-    const float4 f = *reinterpret_cast<const float4 *>(x + m * ldx + (int64_t) block * 32 + j * 4);
+// Eight lanes prepare a block of a row, four values each: the four digits of each kind,
+// the factor and the sum. Where e is below -105 (the last bit below 2^-126), it counts
+// as -105.
+struct prepared {
+    uint32_t digits[3];
+    float factor, sum;
+};
+__device__ inline prepared prepare(float4 f) {
     const float v[4] = {f.x, f.y, f.z, f.w};
     uint32_t e = 22;
 #pragma unroll
     for (int i = 0; i < 4; i++) e = max(e, __float_as_uint(v[i]) >> 23 & 0xffu);
-    float sum = (v[0] + v[1]) + (v[2] + v[3]);
-#pragma unroll
-    for (int off = 1; off < 8; off <<= 1) e = max(e, (uint32_t) __shfl_xor((int) e, off));
-    sum += __shfl_xor(sum, 1);
-    sum += __shfl_xor(sum, 2);
+    prepared r{{0, 0, 0}, 0.0f, (v[0] + v[1]) + (v[2] + v[3])};
+    // over the quad, then the other quad of the eight
+    e = max(e, (uint32_t) __builtin_amdgcn_mov_dpp((int) e, 0xb1, 0xf, 0xf, false));
+    e = max(e, (uint32_t) __builtin_amdgcn_mov_dpp((int) e, 0x4e, 0xf, 0xf, false));
+    e = max(e, (uint32_t) __builtin_amdgcn_mov_dpp((int) e, 0x141, 0xf, 0xf, false));
+    r.sum += dpp<0xb1>(r.sum);
+    r.sum += dpp<0x4e>(r.sum);
+    r.sum += dpp<0x141>(r.sum);
     const bool odd = e == 255;
-    const float up = odd ? 0.0f : __uint_as_float((275 - e) << 23), down = odd ? NAN : __uint_as_float((e - 21) << 23);
-    uint32_t d[3] = {0, 0, 0};
+    const float up = odd ? 0.0f : __uint_as_float((275 - e) << 23);
+    r.factor = odd ? NAN : __uint_as_float((e - 21) << 23);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int q = odd ? 0 : (int) __builtin_rintf(v[i] * up);
         const int d2 = (int8_t) q, q1 = (q - d2) >> 8, d1 = (int8_t) q1, d0 = (q1 - d1) >> 8;
-        d[0] |= (uint32_t) (d0 & 255) << 8 * i;
-        d[1] |= (uint32_t) (d1 & 255) << 8 * i;
-        d[2] |= (uint32_t) (d2 & 255) << 8 * i;
+        r.digits[0] |= (uint32_t) (d0 & 255) << 8 * i;
+        r.digits[1] |= (uint32_t) (d1 & 255) << 8 * i;
+        r.digits[2] |= (uint32_t) (d2 & 255) << 8 * i;
     }
-    // the half's place: Q4_K's chunks hold a half each of two sub-blocks
-    const int chunk = TYPE == ZEST_TYPE_Q4_K ? (block & ~1) + (j >> 2) : block, half = TYPE == ZEST_TYPE_Q4_K ? block & 1 : j >> 2;
-    uint8_t * cell = cells + (int64_t) (chunk * M + m) * CELL;
+    return r;
+}
+
+// A thread's share of the values of all rows, four at a time in the order [block][row][8]:
+// item i of `items`, several requested together.
+__device__ inline void prepare_all(const matvec_args & a, int first, int by, uint8_t * cells) {
+    constexpr int AT_ONCE = 4;
+    const int items = a.blocks * a.M * 8;
+    for (int i0 = first; i0 < items; i0 += AT_ONCE * by) {  // (a block's eight lanes go in step)
+        float4 f[AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < 3; i++) *reinterpret_cast<uint32_t *>(cell + half * 48 + i * 16 + (j & 3) * 4) = d[i];
-    if ((j & 3) == 0) {
-        *reinterpret_cast<float *>(cell + 96 + half * 4) = down;
-        *reinterpret_cast<float *>(cell + 104 + half * 4) = sum;
+        for (int u = 0; u < AT_ONCE; u++) {
+            const int i = i0 + u * by, cell = i >> 3, block = cell / a.M, m = cell - block * a.M;
+            if (i < items) f[u] = *reinterpret_cast<const float4 *>(a.x + m * a.ldx + block * 32 + (i & 7) * 4);
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            const int i = i0 + u * by;
+            if (i >= items) continue;
+            const prepared r = prepare(f[u]);
+            const int j = i & 7;
+            uint8_t * cell = cells + (int64_t) (i >> 3) * CELL;
+#pragma unroll
+            for (int d = 0; d < 3; d++) *reinterpret_cast<uint32_t *>(cell + (j >> 2) * 48 + d * 16 + (j & 3) * 4) = r.digits[d];
+            if (j == 0) *reinterpret_cast<float2 *>(cell + 96) = make_float2(r.factor, r.sum);
+        }
     }
 }
 
-template <int TYPE> __global__ __launch_bounds__(256) void prepare_kernel(matvec_args a) {
-    const int i = (blockIdx.x * 256 + threadIdx.x) >> 3, m = blockIdx.y;
-    if (i < a.chunks) prepare<TYPE>(a.x, a.ldx, i, m, a.M, threadIdx.x & 7, a.cells);
+__global__ __launch_bounds__(256) void prepare_kernel(matvec_args a) { prepare_all(a, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, a.cells); }
+
+// Entry i of an argument's list, by selection among scalar registers: an index that
+// differs between lanes would be a load of the arguments' memory each time, to which
+// the compiler would turn a plain selection back.
+template <typename V> __device__ inline V pick(const V (&list)[MAX_N], int i) {
+    V v = list[0];
+#pragma unroll
+    for (int k = 1; k < MAX_N; k++) {
+        V one = list[k];
+        asm("" : "+s"(one));
+        v = i == k ? one : v;
+    }
+    return v;
 }
 
 // The rows of a tile: of a weight, or of a GLU's gate and up.
@@ -249,67 +295,79 @@ struct tile_rows {
     int32_t weight, row0;
 };
 __device__ inline tile_rows tile_of(const matvec_args & a, int tile) {
-    int i = 0;
-    while (i < a.n - 1 && tile >= a.tiles[i]) i++;
-    return {i, (tile - (i ? a.tiles[i - 1] : 0)) * 16};
+    int weight = 0, before = 0;
+#pragma unroll
+    for (int k = 0; k < MAX_N - 1; k++) {
+        const bool past = k < a.n - 1 && tile >= a.tiles[k];
+        weight = past ? k + 1 : weight;
+        before = past ? a.tiles[k] : before;
+    }
+    return {weight, (tile - before) * 16};
+}
+
+// What becomes of the sums v (S of them, a GLU's gate and up) of a weight's row and row
+// m of x.
+template <int S> __device__ inline void store_row(const matvec_args & a, int weight, int row, int m, const float v[S]) {
+    float out = S == 2 ? zest::glu(a.glu, v[0], v[S - 1]) : v[0];
+    typedef __attribute__((address_space(1))) float * global_floats;
+    const global_floats res = (global_floats) pick(a.res, weight), y = (global_floats) pick(a.y, weight);
+    if (res) out += res[m * pick(a.ldr, weight) + row];
+    y[m * pick(a.ldy, weight) + row] = out;
 }
 
 // A tile is 16 rows of a weight (S = 2: of a GLU's two), a step four chunks of them:
-// a lane loads one chunk of one row, 16 bytes of codes (lane l: row l % 16, chunk l /
-// 16), and v_mfma_i32_16x16x64_i8 multiplies each lane's 16 codes of a half with the
-// three digits of a row of x for its own chunk: the first operand's row 4 b + i is
-// digit i of lane group b's chunk, and zero for the other groups' places, so that
-// lane (row, b) of the result holds its own chunk's three sums in its first three
-// registers. Scales are then one value a lane, and a chunk costs a lane a conversion
+// a lane loads one chunk of one row (lane l: row l % 16, chunk l / 16), and
+// v_mfma_i32_16x16x64_i8 multiplies the 16 codes of a part that each lane holds with
+// the three digits of a row of x for its own chunk: the first operand's row 4 b + i is
+// digit i of lane group b's chunk, and zero in the other groups' places, so that lane
+// (row, b) of the result holds its own chunk's three sums in its first three
+// registers. Scales are then one value a lane, and a block costs a lane a conversion
 // and a few fused products for a row of x.
 //
-// HBM bound: a weight's bytes once. The waves of a tile (a.wk of them) share out its
-// steps and are joined in shared memory; BLOCK steps of a wave are in flight while it
-// computes the last BLOCK.
+// HBM bound: a weight's bytes once. The waves of a tile (a.wk of them) each take a run
+// of its steps and are joined in shared memory; AHEAD steps of a wave are in flight
+// while it computes the AHEAD before them.
 template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) void matvec_kernel(matvec_args a) {
     typedef quant<TYPE> Q;
     typedef int i32x4 __attribute__((ext_vector_type(4)));
-    constexpr int BLOCK = S == 2 ? 2 : 4;
-    constexpr bool ONE_SCALE = TYPE != ZEST_TYPE_Q4_K, OFFSETS = TYPE == ZEST_TYPE_Q4_K || TYPE == ZEST_TYPE_Q4_1;
+    constexpr int B = Q::BLOCKS, AHEAD = 4 / (S * B);
     extern __shared__ __align__(16) uint8_t sh[];
     // sh: 16 zeros, the cells of a segment, the waves' results
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 4, col = lane & 15;
     const int wr = wave / a.wk, wk = wave - wr * a.wk;
     const int M = a.M, steps = (a.chunks + GROUPS - 1) / GROUPS, segs = COPY ? a.segs : 1, seg_steps = COPY ? a.seg_steps : steps;
     uint8_t * const cells = sh + 16;
-    float * const red = reinterpret_cast<float *>(cells + (int64_t) min(seg_steps * GROUPS, a.chunks) * M * CELL);
+    float * const red = reinterpret_cast<float *>(cells + min(seg_steps * GROUPS, a.chunks) * B * M * CELL);
     const int wg_tiles = (a.all_tiles + a.wr - 1) / a.wr, rounds = (wg_tiles - (int) blockIdx.x + gridDim.x - 1) / gridDim.x;
 
+    // A block of this wave's steps: of round `round` and segment `seg`, from step `at` of
+    // the segment on, up to `end`.
     struct place {
-        int round, seg, first;  // of a block of this wave's steps
+        int round, seg, at, end;
     };
-    // steps of segment s that are this wave's: s * seg_steps + wk + i * a.wk
-    auto count = [&](int seg) { return max(0, (min(seg_steps, steps - seg * seg_steps) - wk + a.wk - 1) / a.wk); };
-    auto rows_of = [&](int round) { return ((int) blockIdx.x + round * (int) gridDim.x) * a.wr + wr; };
+    auto start = [&](int round, int seg) {
+        const int n = min(seg_steps, steps - seg * seg_steps);
+        return place{round, seg, n * wk / a.wk, n * (wk + 1) / a.wk};
+    };
     auto next = [&](place p) {
-        p.first += BLOCK;
-        if (p.first >= count(p.seg)) {
-            p.first = 0;
-            if (++p.seg == segs) {
-                p.seg = 0;
-                p.round++;
-            }
-        }
-        return p;
+        p.at += AHEAD;
+        if (p.at < p.end) return p;
+        return p.seg + 1 < segs ? start(p.round, p.seg + 1) : start(p.round + 1, 0);
     };
-    auto load = [&](typename Q::raw (&buf)[BLOCK][S], place p) {
+    auto tile_at = [&](int round) { return ((int) blockIdx.x + round * (int) gridDim.x) * a.wr + wr; };
+    auto load = [&](typename Q::raw (&buf)[AHEAD][S], place p) {
         if (p.round >= rounds) return;
-        const int tile = rows_of(p.round);
+        const int tile = tile_at(p.round);
         if (tile >= a.all_tiles) return;
         const tile_rows t = tile_of(a, tile);
-        const int row = min(t.row0 + col, a.N[t.weight] - 1), n = count(p.seg);
+        const int row = min(t.row0 + col, pick(a.N, t.weight) - 1);
         const uint8_t * at[S];
 #pragma unroll
-        for (int s = 0; s < S; s++) at[s] = a.w[S == 2 ? s : t.weight] + row * a.row_bytes;
+        for (int s = 0; s < S; s++) at[s] = (S == 2 ? a.w[s] : pick(a.w, t.weight)) + row * a.row_bytes;
 #pragma unroll
-        for (int i = 0; i < BLOCK; i++) {
-            if (p.first + i >= n) continue;
-            const int chunk = min((p.seg * seg_steps + wk + (p.first + i) * a.wk) * GROUPS + group, a.chunks - 1);
+        for (int i = 0; i < AHEAD; i++) {
+            if (p.at + i >= p.end) continue;
+            const int chunk = min((p.seg * seg_steps + p.at + i) * GROUPS + group, a.chunks - 1);
 #pragma unroll
             for (int s = 0; s < S; s++) buf[i][s] = Q::load(at[s], chunk);
         }
@@ -325,47 +383,45 @@ template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) 
     // this lane's part of the first operand: digit col % 4 of its group's chunk, if its
     // row is the group's, else zeros
     const bool digit = (col >> 2) == group && (col & 3) < 3;
-    auto compute = [&](const typename Q::raw (&buf)[BLOCK][S], place p) {
-        const int n = count(p.seg);
+    auto compute = [&](const typename Q::raw (&buf)[AHEAD][S], place p) {
 #pragma unroll
-        for (int i = 0; i < BLOCK; i++) {
-            if (p.first + i >= n) continue;
-            const int step = wk + (p.first + i) * a.wk, chunk = (p.seg * seg_steps + step) * GROUPS + group;
+        for (int i = 0; i < AHEAD; i++) {
+            if (p.at + i >= p.end) continue;
+            const int chunk = (p.seg * seg_steps + p.at + i) * GROUPS + group;
             const bool in = chunk < a.chunks;
-            const int local = step * GROUPS + (in ? group : 0);
-            i32x4 code[S][2];
-            half_scales sc[S];
+            i32x4 code[S][B][2];
+            block_scales<B> sc[S];
 #pragma unroll
             for (int s = 0; s < S; s++) {
-                uint32_t c[2][4];
+                uint32_t c[B][2][4];
                 Q::codes(buf[i][s], c);
-#pragma unroll
-                for (int h = 0; h < 2; h++) code[s][h] = i32x4{(int) c[h][0], (int) c[h][1], (int) c[h][2], (int) c[h][3]};
                 sc[s] = Q::scales(buf[i][s], min(chunk, a.chunks - 1));
-                if (!in) sc[s] = half_scales{{0.0f, 0.0f}, {0.0f, 0.0f}};
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) code[s][b][h] = i32x4{(int) c[b][h][0], (int) c[b][h][1], (int) c[b][h][2], (int) c[b][h][3]};
+                    if (!in) sc[s].scale[b] = sc[s].offset[b] = 0.0f;
+                }
             }
-            const uint8_t * cell = cells + local * M * CELL;
+            const uint8_t * cell = cells + ((p.at + i) * GROUPS + (in ? group : 0)) * B * M * CELL;
             const uint8_t * from = digit && in ? cell + (col & 3) * 16 : sh;
-            const int stride = digit && in ? CELL : 0, half_at = digit && in ? 48 : 0;
+            const int stride = digit && in ? CELL : 0, part = digit && in ? 48 : 0;
 #pragma unroll
             for (int m = 0; m < T; m++) {
                 if (m >= M) continue;
-                const i32x4 x0 = *reinterpret_cast<const i32x4 *>(from + m * stride), x1 = *reinterpret_cast<const i32x4 *>(from + m * stride + half_at);
-                const float4 f = *reinterpret_cast<const float4 *>(cell + m * CELL + 96);  // the halves' factors and sums
 #pragma unroll
-                for (int s = 0; s < S; s++) {
-                    auto number = [](i32x4 d) { return fmaf((float) d[0], 65536.0f, (float) ((d[1] << 8) + d[2])); };
-                    i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x0, code[s][0], i32x4{}, 0, 0, 0);
-                    if constexpr (ONE_SCALE) {
-                        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x1, code[s][1], d, 0, 0, 0);
-                        acc[m][s] = fmaf(number(d), sc[s].scale[0] * f.x, acc[m][s]);
-                        if constexpr (OFFSETS) acc[m][s] = fmaf(f.z + f.w, sc[s].offset[0], acc[m][s]);
-                    } else {
-                        const i32x4 e = __builtin_amdgcn_mfma_i32_16x16x64_i8(x1, code[s][1], i32x4{}, 0, 0, 0);
-                        acc[m][s] = fmaf(number(d), sc[s].scale[0] * f.x, acc[m][s]);
-                        acc[m][s] = fmaf(number(e), sc[s].scale[1] * f.y, acc[m][s]);
-                        acc[m][s] = fmaf(f.z, sc[s].offset[0], acc[m][s]);
-                        acc[m][s] = fmaf(f.w, sc[s].offset[1], acc[m][s]);
+                for (int b = 0; b < B; b++) {
+                    const i32x4 x0 = *reinterpret_cast<const i32x4 *>(from + (b * M + m) * stride);
+                    const i32x4 x1 = *reinterpret_cast<const i32x4 *>(from + (b * M + m) * stride + part);
+                    const float2 f = *reinterpret_cast<const float2 *>(cell + (b * M + m) * CELL + 96);  // the factor and the sum
+#pragma unroll
+                    for (int s = 0; s < S; s++) {
+                        i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x0, code[s][b][0], i32x4{}, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x1, code[s][b][1], d, 0, 0, 0);
+                        // (|d0| <= 64 15 32 < 2^15 for nibbles, so they fit in 32 bits together)
+                        const float v = Q::NIBBLES ? (float) ((((d[0] << 8) + d[1]) << 8) + d[2]) : fmaf((float) d[0], 65536.0f, (float) ((d[1] << 8) + d[2]));
+                        acc[m][s] = fmaf(v, sc[s].scale[b] * f.x, acc[m][s]);
+                        if constexpr (Q::OFFSETS) acc[m][s] = fmaf(f.y, sc[s].offset[b], acc[m][s]);
                     }
                 }
             }
@@ -375,13 +431,11 @@ template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) 
     auto fill = [&](int seg) {
         if (threadIdx.x < 4) reinterpret_cast<uint32_t *>(sh)[threadIdx.x] = 0;
         if constexpr (COPY) {
-            const int first = seg * seg_steps * GROUPS, n = min(seg_steps * GROUPS, a.chunks - first) * M * (CELL / 16);
+            const int first = seg * seg_steps * GROUPS * B, n = min(seg_steps * GROUPS * B, a.blocks - first) * M * (CELL / 16);
             const uint4 * from = reinterpret_cast<const uint4 *>(a.cells + (int64_t) first * M * CELL);
             for (int i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<uint4 *>(cells)[i] = from[i];
         } else {
-            const int lanes = a.chunks * 8;
-            for (int i = threadIdx.x; i < lanes; i += blockDim.x)
-                for (int m = 0; m < M; m++) prepare<TYPE>(a.x, a.ldx, i >> 3, m, M, i & 7, cells);
+            prepare_all(a, threadIdx.x, blockDim.x, cells);
         }
         __syncthreads();
     };
@@ -393,9 +447,7 @@ template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) 
             if (m >= M) continue;
 #pragma unroll
             for (int s = 0; s < S; s++) {
-                float v = acc[m][s];
-                v += __shfl_xor(v, 16);
-                v += __shfl_xor(v, 32);
+                const float v = over_groups(acc[m][s]);
                 if (group == 0) mine[(m * S + s) * 16 + col] = v;
             }
         }
@@ -403,25 +455,21 @@ template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) 
         for (int i = threadIdx.x; i < a.wr * M * 16; i += blockDim.x) {
             const int c = i & 15, m = (i >> 4) % M, r = (i >> 4) / M, tile = ((int) blockIdx.x + round * (int) gridDim.x) * a.wr + r;
             if (tile >= a.all_tiles) continue;
-            const tile_rows t = tile_of(a, tile);
-            const int row = t.row0 + c;
-            if (row >= a.N[t.weight]) continue;
             float v[S];
 #pragma unroll
             for (int s = 0; s < S; s++) {
                 v[s] = 0.0f;
                 for (int w = 0; w < a.wk; w++) v[s] += red[((r * a.wk + w) * T * S + m * S + s) * 16 + c];
             }
-            float out = S == 2 ? zest::glu(a.glu, v[0], v[S - 1]) : v[0];
-            if (a.res[t.weight]) out += a.res[t.weight][m * a.ldr[t.weight] + row];
-            a.y[t.weight][m * a.ldy[t.weight] + row] = out;
+            const tile_rows t = tile_of(a, tile);
+            if (t.row0 + c < pick(a.N, t.weight)) store_row<S>(a, t.weight, t.row0 + c, m, v);
         }
         __syncthreads();
     };
     // one block: the next one requested, this one computed; what follows it
-    auto turn = [&](typename Q::raw (&now)[BLOCK][S], typename Q::raw (&then)[BLOCK][S], place p) {
+    auto turn = [&](typename Q::raw (&now)[AHEAD][S], typename Q::raw (&then)[AHEAD][S], place p, bool first) {
         const place q = next(p);
-        if (p.first == 0) {
+        if (first) {  // of a segment
             if (p.seg == 0) clear();
             if (segs > 1 || p.round == 0) {
                 if (segs > 1) __syncthreads();
@@ -429,45 +477,441 @@ template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) 
             }
         }
         load(then, q);
-        if (rows_of(p.round) < a.all_tiles) compute(now, p);
+        if (tile_at(p.round) < a.all_tiles) compute(now, p);
         if (q.round != p.round) finish(p.round);
         return q;
     };
-    typename Q::raw one[BLOCK][S], two[BLOCK][S];
-    place p{0, 0, 0};
+    typename Q::raw one[AHEAD][S], two[AHEAD][S];
+    place p = start(0, 0);
+    bool first = true;
     load(one, p);
     while (p.round < rounds) {
-        p = turn(one, two, p);
-        if (p.round < rounds) p = turn(two, one, p);
+        place q = turn(one, two, p, first);
+        first = q.round != p.round || q.seg != p.seg;
+        p = q;
+        if (p.round >= rounds) break;
+        q = turn(two, one, p, first);
+        first = q.round != p.round || q.seg != p.seg;
+        p = q;
+    }
+}
+
+// ---- few rows of x: streams through shared memory ---------------------------------------
+
+// What a type's rows look like to a stream: a unit is UNIT bytes of a row, CHUNKS
+// chunks (whole blocks of the format; a multiple of GROUPS, so whole steps), and a
+// chunk is read from shared memory, where its row may begin at any multiple of the
+// row's alignment.
+template <int TYPE> struct stream;
+
+// Shared memory by its address: a read through a pointer that the compiler can follow
+// to an object waits for all direct loads into that object.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <typename V> __device__ inline V lds(uint32_t at) { return *(const __attribute__((address_space(3))) V *) at; }
+template <typename V> __device__ inline void lds(uint32_t at, V v) { *(__attribute__((address_space(3))) V *) at = v; }
+
+// A chunk of 2 bytes of scale and N words of codes, at an even address: whole words are
+// read from a whole address on, of which the codes come out by a permute, or are words.
+template <int N> __device__ inline void read_scaled(uint32_t at, uint32_t codes[N], uint32_t & scale) {
+    uint32_t w[N + 1];
+#pragma unroll
+    for (int i = 0; i <= N; i++) w[i] = lds<uint32_t>((at & ~3u) + 4 * i);
+    const bool odd = at & 2;
+    const uint32_t sel = odd ? 0x07060504u : 0x05040302u;
+#pragma unroll
+    for (int i = 0; i < N; i++) codes[i] = __builtin_amdgcn_perm(w[i + 1], w[i], sel);
+    scale = odd ? w[0] >> 16 : w[0] & 0xffffu;
+}
+
+template <int TYPE> struct stream_nibbles {
+    static constexpr int UNIT = 144, CHUNKS = 8;
+    static __device__ typename quant<TYPE>::raw read(uint32_t unit, int chunk) {
+        uint32_t w[4], d;
+        read_scaled<4>(unit + chunk * 18, w, d);
+        return {make_uint4(w[0], w[1], w[2], w[3]), d};
+    }
+};
+template <> struct stream<ZEST_TYPE_Q4_0> : stream_nibbles<ZEST_TYPE_Q4_0> {};
+template <> struct stream<ZEST_TYPE_IQ4_NL> : stream_nibbles<ZEST_TYPE_IQ4_NL> {};
+template <> struct stream<ZEST_TYPE_Q4_1> {
+    static constexpr int UNIT = 160, CHUNKS = 8;
+    static __device__ quant<ZEST_TYPE_Q4_1>::raw read(uint32_t unit, int chunk) {
+        uint32_t w[5];
+#pragma unroll
+        for (int i = 0; i < 5; i++) w[i] = lds<uint32_t>(unit + chunk * 20 + 4 * i);
+        return {make_uint4(w[1], w[2], w[3], w[4]), w[0]};
+    }
+};
+template <> struct stream<ZEST_TYPE_Q8_0> {
+    static constexpr int UNIT = 136, CHUNKS = 4;
+    static __device__ quant<ZEST_TYPE_Q8_0>::raw read(uint32_t unit, int chunk) {
+        uint32_t w[8], d;
+        read_scaled<8>(unit + chunk * 34, w, d);
+        return {{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])}, d};
+    }
+};
+__device__ inline uint4 as_uint4(u32x4 v) { return make_uint4(v.x, v.y, v.z, v.w); }
+template <> struct stream<ZEST_TYPE_Q4_K> {
+    static constexpr int UNIT = 144, CHUNKS = 4;
+    static __device__ quant<ZEST_TYPE_Q4_K>::raw read(uint32_t unit, int chunk) {
+        return {{as_uint4(lds<u32x4>(unit + 16 + 32 * chunk)), as_uint4(lds<u32x4>(unit + 32 + 32 * chunk))}, as_uint4(lds<u32x4>(unit))};
+    }
+};
+template <> struct stream<ZEST_TYPE_IQ4_XS> {
+    static constexpr int UNIT = 136, CHUNKS = 8;
+    static __device__ quant<ZEST_TYPE_IQ4_XS>::raw read(uint32_t unit, int chunk) {
+        const u32x2 head = lds<u32x2>(unit), a = lds<u32x2>(unit + 8 + 16 * chunk), b = lds<u32x2>(unit + 16 + 16 * chunk);
+        return {make_uint4(a.x, a.y, b.x, b.y), make_uint2(head.x, head.y)};
+    }
+};
+
+constexpr int STREAM_WAVES = 8;
+constexpr int RAW_CELL = 128;  // of 32 values of x where a stream's workgroups prepare them, over the values themselves
+// Units of a row in a piece; the 16-byte granules that hold them wherever the row
+// begins; their places in shared memory, an odd number, so that 16 rows' reads spread
+// over the banks; a piece's loads.
+template <int S> constexpr int UNITS = 2 / S;
+template <int TYPE, int S> constexpr int GRANULES = (UNITS<S> * stream<TYPE>::UNIT + 16 - row_align(TYPE) + 15) / 16;
+template <int TYPE, int S> constexpr int PLACES = GRANULES<TYPE, S> | 1;
+template <int TYPE, int S> constexpr int LOADS = (16 * S * PLACES<TYPE, S> + 63) / 64;
+
+typedef __attribute__((address_space(3))) void * lds_ptr_t;
+typedef const __attribute__((address_space(1))) void * global_ptr_t;
+
+// The call's rows are shared out evenly over the workgroups, a workgroup's pieces, 16
+// rows by 16, over its waves; the first of either take one more where they do not come
+// out even.
+struct run {
+    int each, more;
+    __device__ int start(int i) const { return i * each + min(i, more); }
+};
+
+// A row of the call: of which weight, and its number there.
+struct call_row {
+    int weight, row;
+};
+__device__ inline call_row row_of(const matvec_args & a, int r) {
+    int weight = 0, before = 0;
+#pragma unroll
+    for (int k = 0; k < MAX_N - 1; k++) {
+        const bool past = k < a.n - 1 && r >= a.rows[k];
+        weight = past ? k + 1 : weight;
+        before = past ? a.rows[k] : before;
+    }
+    return {weight, r - before};
+}
+
+// The products as matvec_kernel's, the weights' bytes by another way: not chunk by chunk
+// into registers, where an instruction touches 16 lines or more and a line is asked for
+// three times, but as whole granules of contiguous bytes straight into shared memory:
+// RING pieces (two units of 16 rows, 4.6 KB) a wave, requested as soon as their place
+// is read. A workgroup's last 16 rows are as many as are left of its share: a row that
+// is not there is its neighbour again. So all CUs stream whatever the number of rows.
+template <int TYPE, int M, int S, int RING, bool READY> __global__ __launch_bounds__(STREAM_WAVES * 64) void stream_kernel(matvec_args a) {
+    typedef quant<TYPE> Q;
+    typedef stream<TYPE> ST;
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    constexpr int B = Q::BLOCKS, U = UNITS<S>, G = GRANULES<TYPE, S>, GP = PLACES<TYPE, S>, NL = LOADS<TYPE, S>, ALIGN = row_align(TYPE);
+    constexpr int STEPS = U * (ST::CHUNKS / GROUPS);  // of a piece
+    constexpr int CELL_AT = READY ? CELL : RAW_CELL;
+    extern __shared__ __align__(1024) uint8_t sh[];
+    // sh: the rings, the cells, 16 zeros, the waves' results
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 4, col = lane & 15;
+    const int pieces = a.pieces, row_bytes = (int) a.row_bytes;
+    const run all{a.each, a.more};
+    const int first_row = all.start(blockIdx.x), end_row = all.start(blockIdx.x + 1), tiles = (end_row - first_row + 15) / 16;
+    const int n = tiles * pieces;
+    const run waves{n / STREAM_WAVES, n % STREAM_WAVES};
+    const int u0 = waves.start(wave), u1 = waves.start(wave + 1);
+    const uint32_t base = (uint32_t) (uintptr_t) (lds_ptr_t) sh, ring = base + wave * (RING * NL * 1024), cells = base + STREAM_WAVES * RING * NL * 1024;
+    const uint32_t cell_bytes = (uint32_t) (a.blocks * M * CELL_AT + 1023) & ~1023u, zeros = cells + cell_bytes;
+    float * const red = reinterpret_cast<float *>(sh + (zeros + 16 - base));
+
+    // x, or its cells, straight into shared memory, before the weights so that it is not
+    // waited for behind them (all of these are waits that this kernel counts itself: one
+    // of the compiler's would be for everything on its way)
+    for (uint32_t at = wave * 1024; at < cell_bytes; at += STREAM_WAVES * 1024) {
+        const uint32_t mine_at = at + lane * 16;
+        const uint8_t * from = a.cells + min(mine_at, (uint32_t) (a.blocks * M * CELL_AT) - 16);
+        if constexpr (!READY) {  // cell c: row c % M's block c / M
+            const int cell = min((int) (mine_at / RAW_CELL), a.blocks * M - 1), block = cell / M, m = cell - block * M;
+            from = (const uint8_t *) (a.x + m * a.ldx + block * 32 + (lane & 7) * 4);
+        }
+        __builtin_amdgcn_global_load_lds((global_ptr_t) from, (lds_ptr_t) (uintptr_t) (cells + at), 16, 0, 0);
+    }
+    asm volatile("" ::: "memory");
+
+    // This lane's granules of a piece: at[i] bytes on in row from[i] of the tile that is
+    // being loaded. (Every lane loads, so that the loads in flight are known: a place that
+    // holds none of a row's granules gets its last one again.)
+    int32_t at[NL];
+    const uint8_t * from[NL];
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+        const int p = i * 64 + lane;
+        at[i] = min(p - (p / GP) * GP, G - 1) * 16;
+    }
+    auto rows_from = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int r = min((i * 64 + lane) / GP, 16 * S - 1);
+            const call_row c = row_of(a, min(first_row + tile * 16 + (r & 15), end_row - 1));
+            from[i] = (S == 1 ? pick(a.w, c.weight) : r >= 16 ? a.w[1] : a.w[0]) + (int64_t) c.row * row_bytes;
+        }
+    };
+    // A granule holds bytes of its row: those before its first or behind its last that are
+    // read with them are within the granule's own 16.
+    struct place {
+        int tile, piece;
+    };
+    auto load = [&](place p, int slot) {
+        const uint32_t to = ring + slot * (NL * 1024);
+        const int on = p.piece * (U * ST::UNIT);
+        if (p.piece < pieces - 1) {
+#pragma unroll
+            for (int i = 0; i < NL; i++)
+                __builtin_amdgcn_global_load_lds((global_ptr_t) (((uintptr_t) (from[i] + on) & ~(uintptr_t) 15) + at[i]), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
+        } else {  // behind a row's end, its last granule again
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const uintptr_t q = ((uintptr_t) (from[i] + on) & ~(uintptr_t) 15) + at[i], last = (uintptr_t) (from[i] + row_bytes - 1) & ~(uintptr_t) 15;
+                __builtin_amdgcn_global_load_lds((global_ptr_t) (q < last ? q : last), (lds_ptr_t) (uintptr_t) (to + i * 1024), 16, 0, 0);
+            }
+        }
+    };
+    auto after = [&](place p) {
+        p.piece++;
+        if (p.piece == pieces) {
+            p.piece = 0;
+            p.tile++;
+        }
+        return p;
+    };
+    place now{u0 / pieces, 0};
+    now.piece = u0 - now.tile * pieces;
+    place then = now;
+    // (a wave without that many pieces loads what follows, or the last)
+    rows_from(min(then.tile, tiles - 1));
+#pragma unroll
+    for (int r = 0; r < RING; r++) {
+        load(then, r);
+        then = after(then);
+        if (then.piece == 0) rows_from(min(then.tile, tiles - 1));
+        asm volatile("" ::: "memory");
+    }
+    // x is there: this wave's loads of it, then (READY) everybody's
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(RING * NL) : "memory");
+    if (threadIdx.x == 0) lds(zeros, u32x4{0, 0, 0, 0});
+    if constexpr (!READY) {  // the cells that the wave has loaded, each over its own values, which its eight lanes have read
+        for (uint32_t at = wave * 1024; at < cell_bytes; at += STREAM_WAVES * 1024) {
+            const f32x4 v = lds<f32x4>(cells + at + lane * 16);
+            const prepared r = prepare(make_float4(v.x, v.y, v.z, v.w));
+            const int j = lane & 7;
+            const uint32_t cell = cells + at + (lane >> 3) * RAW_CELL;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int d = 0; d < 3; d++) lds(cell + (j >> 2) * 48 + d * 16 + (j & 3) * 4, r.digits[d]);
+            if (j == 0) lds(cell + 96, f32x2{r.factor, r.sum});
+        }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // (not __syncthreads, which waits for the weights too)
+    asm volatile("" ::: "memory");
+
+    float acc[M][S];
+    auto clear = [&]() {
+#pragma unroll
+        for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int s = 0; s < S; s++) acc[m][s] = 0.0f;
+    };
+    uint32_t begins[S];  // where this lane's row begins in its first granule
+    auto rows_of_tile = [&](int tile) {
+        if constexpr (ALIGN < 16) {
+            const call_row c = row_of(a, min(first_row + tile * 16 + col, end_row - 1));
+#pragma unroll
+            for (int s = 0; s < S; s++) begins[s] = (uint32_t) (uintptr_t) (S == 1 ? pick(a.w, c.weight) : a.w[s]) + (uint32_t) c.row * (uint32_t) row_bytes;
+        }
+    };
+    const bool digit = (col >> 2) == group && (col & 3) < 3;
+    const int ragged = a.chunks - (pieces - 1) * (STEPS * GROUPS) < STEPS * GROUPS ? pieces - 1 : pieces;  // the piece that is not whole
+    auto compute = [&](int piece, uint32_t slot, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        uint32_t unit[S];
+#pragma unroll
+        for (int s = 0; s < S; s++) unit[s] = slot + (s * 16 + col) * (GP * 16) + (ALIGN < 16 ? (begins[s] + (uint32_t) piece * (U * ST::UNIT)) & 15 : 0);
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            const int step = piece * STEPS + i, chunk = step * GROUPS + group;
+            if (EDGE && step * GROUPS >= a.chunks) continue;
+            const bool in = !EDGE || chunk < a.chunks;
+            i32x4 code[S][B][2];
+            block_scales<B> sc[S];
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                // (past the row's end: any bytes, whose scales are then replaced)
+                const typename Q::raw r = ST::read(unit[s] + i / (ST::CHUNKS / GROUPS) * ST::UNIT, (i % (ST::CHUNKS / GROUPS)) * GROUPS + group);
+                uint32_t c[B][2][4];
+                Q::codes(r, c);
+                sc[s] = Q::scales(r, chunk);
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) code[s][b][h] = i32x4{(int) c[b][h][0], (int) c[b][h][1], (int) c[b][h][2], (int) c[b][h][3]};
+                    if (!in) sc[s].scale[b] = sc[s].offset[b] = 0.0f;
+                }
+            }
+            const uint32_t cell = cells + (step * GROUPS + (in ? group : 0)) * (B * M * CELL_AT);
+            const uint32_t x_at = digit && in ? cell + (col & 3) * 16 : zeros;
+            const uint32_t stride = digit && in ? CELL_AT : 0, part = digit && in ? 48 : 0;
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    const i32x4 x0 = lds<i32x4>(x_at + (b * M + m) * stride), x1 = lds<i32x4>(x_at + (b * M + m) * stride + part);
+                    const f32x2 f = lds<f32x2>(cell + (b * M + m) * CELL_AT + 96);  // the factor and the sum
+#pragma unroll
+                    for (int s = 0; s < S; s++) {
+                        i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x0, code[s][b][0], i32x4{}, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x1, code[s][b][1], d, 0, 0, 0);
+                        const float v = Q::NIBBLES ? (float) ((((d[0] << 8) + d[1]) << 8) + d[2]) : fmaf((float) d[0], 65536.0f, (float) ((d[1] << 8) + d[2]));
+                        acc[m][s] = fmaf(v, sc[s].scale[b] * f.x, acc[m][s]);
+                        if constexpr (Q::OFFSETS) acc[m][s] = fmaf(f.y, sc[s].offset[b], acc[m][s]);
+                    }
+                }
+            }
+        }
+    };
+    // a wave's sums of a tile; waves share a tile with their neighbours, so a tile's
+    // place plus the wave's number is each result's own place
+    auto leave = [&](int tile) {
+        float * const to = red + (tile + wave) * (M * S * 16);
+#pragma unroll
+        for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                const float v = over_groups(acc[m][s]);
+                if (group == 0) to[(m * S + s) * 16 + col] = v;
+            }
+    };
+    clear();
+    rows_of_tile(now.tile);
+    int slot = 0;
+    for (int u = u0; u < u1; u++) {
+        // the piece is there when no more than the loads after it are on their way (the
+        // first RING are requested whether or not there are as many)
+        if (u + RING <= u1 || u == u0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 1) * NL) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (now.piece == ragged) compute(now.piece, ring + slot * (NL * 1024), std::true_type{});
+        else compute(now.piece, ring + slot * (NL * 1024), std::false_type{});
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before it is overwritten
+        if (u + RING < u1) {
+            load(then, slot);
+            then = after(then);
+            if (then.piece == 0) rows_from(min(then.tile, tiles - 1));
+        }
+        slot = slot + 1 == RING ? 0 : slot + 1;
+        const place next = after(now);
+        if (next.piece == 0 || u + 1 == u1) {
+            leave(now.tile);
+            clear();
+            rows_of_tile(next.tile);
+        }
+        now = next;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing is on its way to a wave that has ended)
+    __syncthreads();
+    for (int i = threadIdx.x; i < tiles * M * 16; i += STREAM_WAVES * 64) {
+        const int c = i & 15, m = (i >> 4) % M, k = (i >> 4) / M, r = first_row + k * 16 + c;
+        if (r >= end_row) continue;
+        float v[S];
+#pragma unroll
+        for (int s = 0; s < S; s++) v[s] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < STREAM_WAVES; w++) {
+            const bool has = max(waves.start(w), k * pieces) < min(waves.start(w + 1), (k + 1) * pieces);
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                const float one = red[(k + w) * (M * S * 16) + (m * S + s) * 16 + c];
+                v[s] += has ? one : 0.0f;
+            }
+        }
+        const call_row to = row_of(a, r);
+        store_row<S>(a, to.weight, to.row, m, v);
     }
 }
 
 // ---- the host's plan ----------------------------------------------------------------
 
 struct matvec_plan {
-    int wk, wr, workgroups, seg_steps, segs;
-    bool copy;        // x is prepared by a kernel of its own
+    int ring;             // of stream_kernel; 0: matvec_kernel
+    int wk, wr, workgroups, seg_steps, segs, pieces;
+    bool copy;            // x is prepared by a kernel of its own
     size_t lds, bytes;
 };
 
-matvec_plan plan_of(int64_t M, int64_t K, int n, const int64_t * N, bool glu) {
+// Streams' sizes by type, as the kernels have them.
+struct stream_sizes {
+    int pieces, loads;
+};
+template <int S> stream_sizes sizes_of(int type, int chunks) {
+#define ZEST_SIZES(T) \
+    case T: return {(chunks + stream<T>::CHUNKS * UNITS<S> - 1) / (stream<T>::CHUNKS * UNITS<S>), LOADS<T, S>}
+    switch (type) {
+        ZEST_SIZES(ZEST_TYPE_Q4_0);
+        ZEST_SIZES(ZEST_TYPE_Q4_1);
+        ZEST_SIZES(ZEST_TYPE_Q8_0);
+        ZEST_SIZES(ZEST_TYPE_Q4_K);
+        ZEST_SIZES(ZEST_TYPE_IQ4_NL);
+        default: ZEST_SIZES(ZEST_TYPE_IQ4_XS);
+    }
+#undef ZEST_SIZES
+}
+
+constexpr int CUS = 256;
+constexpr int STREAM_ROWS = 512;  // of a workgroup at most
+
+matvec_plan plan_of(int type, int64_t M, int64_t K, int n, const int64_t * N, bool glu) {
     matvec_plan p{};
-    const int chunks = (int) (K / 32), steps = (chunks + GROUPS - 1) / GROUPS, T = M <= 4 ? 4 : M <= 8 ? 8 : 16, S = glu ? 2 : 1;
+    const int B = type == ZEST_TYPE_Q4_K ? 2 : 1, chunks = (int) (K / 32 / B), steps = (chunks + GROUPS - 1) / GROUPS, T = M <= 4 ? 4 : M <= 8 ? 8 : 16, S = glu ? 2 : 1;
     int64_t tiles = 0;
     for (int i = 0; i < (glu ? 1 : n); i++) tiles += (N[i] + 15) / 16;
+    if (M <= 4) {
+        const stream_sizes z = glu ? sizes_of<2>(type, chunks) : sizes_of<1>(type, chunks);
+        int64_t rows = 0;
+        for (int i = 0; i < (glu ? 1 : n); i++) rows += N[i];
+        p.pieces = z.pieces;
+        p.workgroups = (int) std::max<int64_t>(std::min<int64_t>(rows, CUS), (rows + STREAM_ROWS - 1) / STREAM_ROWS);
+        const int64_t wg_tiles = ((rows + p.workgroups - 1) / p.workgroups + 15) / 16;
+        const auto lds_of = [&](int ring, int cell) {
+            return (size_t) STREAM_WAVES * ring * z.loads * 1024 + (((size_t) B * chunks * M * cell + 1023) & ~(size_t) 1023) + 16 +
+                   (size_t) (wg_tiles + STREAM_WAVES) * M * S * 16 * 4;
+        };
+        for (p.ring = 3; p.ring >= 2; p.ring--)
+            for (const int cell : {RAW_CELL, CELL}) {
+                p.lds = lds_of(p.ring, cell);
+                p.copy = cell == CELL;
+                p.bytes = p.copy ? (size_t) B * chunks * M * CELL : 16;
+                if (p.lds <= LDS_MOST && (p.ring == 2 || !p.copy)) return p;
+            }
+        p.ring = 0;
+    }
     p.wr = tiles <= 2 * 256 ? 1 : tiles <= 8 * 256 ? 2 : 4;
     const int most = p.wr == 1 && tiles > 256 ? 8 : 16 / p.wr;
     p.wk = 1;
     for (int w = 1; w <= most; w++)
         if ((steps + w - 1) / w < (steps + p.wk - 1) / p.wk) p.wk = w;
     const size_t red = (size_t) p.wk * p.wr * T * S * 16 * 4, room = LDS_MOST - 16 - red;
-    p.seg_steps = (int) std::min<size_t>(steps, room / ((size_t) GROUPS * M * CELL));
+    p.seg_steps = (int) std::min<size_t>(steps, room / ((size_t) GROUPS * B * M * CELL));
     p.segs = (steps + p.seg_steps - 1) / p.seg_steps;
-    p.copy = p.segs > 1 || M > 4;
-    p.lds = 16 + (size_t) std::min(p.seg_steps * GROUPS, chunks) * M * CELL + red;
+    p.copy = true;
+    p.lds = 16 + (size_t) std::min(p.seg_steps * GROUPS, chunks) * B * M * CELL + red;
     p.workgroups = (int) std::min<int64_t>((tiles + p.wr - 1) / p.wr, 512);
     if (p.lds > LDS_MOST / 2 || p.wk * p.wr > 8) p.workgroups = std::min(p.workgroups, 256);
-    p.bytes = std::max<size_t>(16, p.copy ? (size_t) chunks * M * CELL : 0);
+    p.bytes = std::max<size_t>(16, p.copy ? (size_t) chunks * B * M * CELL : 0);
     return p;
 }
 
@@ -499,19 +943,37 @@ template <auto KERNEL> int allow_lds(const char * me) {
     return ZEST_OK;
 }
 
+void launch_prepare(const matvec_args & a, hipStream_t s) {
+    hipLaunchKernelGGL(prepare_kernel, dim3((unsigned) std::min<int64_t>(((int64_t) a.blocks * a.M * 8 + 255) / 256, 1024)), dim3(256), 0, s, a);
+}
+
 template <int TYPE, int T, int S, bool COPY> int launch(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
     if (const int st = allow_lds<&matvec_kernel<TYPE, T, S, COPY>>(me)) return st;
-    if (COPY) hipLaunchKernelGGL(prepare_kernel<TYPE>, dim3((unsigned) ((a.chunks * 8 + 255) / 256), (unsigned) a.M), dim3(256), 0, s, a);
+    if (COPY) launch_prepare(a, s);
     hipLaunchKernelGGL((matvec_kernel<TYPE, T, S, COPY>), dim3((unsigned) p.workgroups), dim3((unsigned) (p.wk * p.wr * 64)), p.lds, s, a);
     return zest::check_launch(me);
 }
 
+template <int TYPE, int M, int S, int RING, bool READY> int launch_stream(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
+    if (const int st = allow_lds<&stream_kernel<TYPE, M, S, RING, READY>>(me)) return st;
+    if (READY) launch_prepare(a, s);
+    hipLaunchKernelGGL((stream_kernel<TYPE, M, S, RING, READY>), dim3((unsigned) p.workgroups), dim3(STREAM_WAVES * 64), p.lds, s, a);
+    return zest::check_launch(me);
+}
+
+template <int TYPE, int M, int S> int launch_stream(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
+    if (p.copy) return launch_stream<TYPE, M, S, 2, true>(a, p, s, me);
+    return p.ring == 3 ? launch_stream<TYPE, M, S, 3, false>(a, p, s, me) : launch_stream<TYPE, M, S, 2, false>(a, p, s, me);
+}
+
 template <int TYPE, int S> int launch(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
+    if (p.ring) {
+        if (a.M > 2) return a.M > 3 ? launch_stream<TYPE, 4, S>(a, p, s, me) : launch_stream<TYPE, 3, S>(a, p, s, me);
+        return a.M > 1 ? launch_stream<TYPE, 2, S>(a, p, s, me) : launch_stream<TYPE, 1, S>(a, p, s, me);
+    }
     if (a.M > 8) return launch<TYPE, 16, S, true>(a, p, s, me);
     if (a.M > 4) return launch<TYPE, 8, S, true>(a, p, s, me);
-    if (p.copy) return launch<TYPE, 4, S, true>(a, p, s, me);
-    if (a.M > 2) return launch<TYPE, 4, S, false>(a, p, s, me);
-    return a.M > 1 ? launch<TYPE, 2, S, false>(a, p, s, me) : launch<TYPE, 1, S, false>(a, p, s, me);
+    return launch<TYPE, 4, S, true>(a, p, s, me);
 }
 
 template <int TYPE> int launch(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
@@ -545,17 +1007,18 @@ int matvec(const char * me, int glu, int type, const float * x, int64_t M, int64
     a.ldx = M == 1 ? K : ldx;
     a.row_bytes = (int64_t) row_bytes;
     a.M = (int32_t) M;
-    a.chunks = (int32_t) (K / 32);
+    a.blocks = (int32_t) (K / 32);
+    a.chunks = a.blocks / (type == ZEST_TYPE_Q4_K ? 2 : 1);
     a.n = outs;
     a.glu = glu;
-    int64_t tiles = 0;
+    int64_t tiles = 0, rows = 0;
     for (int i = 0; i < n; i++) {
         ZEST_REQUIRE(w[i] && aligned(w[i], row_align(type)), "%s: weight %d: rows %d-byte aligned wanted", me, i, row_align(type));
         ZEST_REQUIRE(N[i] > 0 && N[i] <= (1 << 26), "%s: weight %d: N=%lld", me, i, (long long) N[i]);
         a.w[i] = (const uint8_t *) w[i];
         a.N[i] = (int32_t) N[i];
-        if (i < outs) tiles += (N[i] + 15) / 16;
-        a.tiles[i] = (int32_t) tiles;
+        if (i < outs) tiles += (N[i] + 15) / 16, rows += N[i];
+        a.tiles[i] = (int32_t) tiles, a.rows[i] = (int32_t) rows;
     }
     for (int i = 0; i < outs; i++) {
         ZEST_REQUIRE(y[i] && aligned(y[i], 4) && (M == 1 || (ldy[i] >= N[i] && ldy[i] < (1ll << 31))), "%s: output %d: ldy=%lld for N=%lld", me, i, (long long) (M == 1 ? 0 : ldy[i]),
@@ -582,11 +1045,12 @@ int matvec(const char * me, int glu, int type, const float * x, int64_t M, int64
         }
     }
     // (a GLU's plan is that of two weights as far as its workspace goes)
-    const matvec_plan p = plan_of(M, K, n, N, glu >= 0);
+    const matvec_plan p = plan_of(type, M, K, n, N, glu >= 0);
     ZEST_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= p.bytes, "%s: workspace of %zu bytes, 16-byte aligned, wanted", me, p.bytes);
     a.all_tiles = (int32_t) tiles;
     a.wk = p.wk, a.wr = p.wr, a.seg_steps = p.seg_steps, a.segs = p.segs;
     a.cells = (uint8_t *) workspace;
+    a.pieces = p.pieces, a.each = (int32_t) (rows / p.workgroups), a.more = (int32_t) (rows % p.workgroups);
     return launch(type, a, p, zest::as_stream(stream), me);
 }
 
