@@ -11,6 +11,8 @@ Loaded as ``ggml_xdna_amd`` (the directory name has a hyphen):
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -169,9 +171,15 @@ def raw_row_bytes(wtype: int, k: int) -> int:
 
 # ---- torch-facing calls --------------------------------------------------------
 
+_torch_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def _stream() -> int:
@@ -314,77 +322,102 @@ def gemm_glu(kind: int, a_packed, m: int, w_gu, f: int, k: int, xout=True, h=Non
 
 
 def _need_here(device) -> None:
-    if device.type != "cuda" or device.index != _torch().cuda.current_device():
+    if device.type != "cuda" or device.index != _torch()._C._cuda_getDevice():
         raise ZestError(f"the tensors are on {device}, which is not the current device")
 
 
-def _fp32_rows(t, what: str, rows: int, cols: int, device):
+def _fp32_rows(t, what: str, rows: int, cols: int, device, f32):
     """The pointer and row stride of an fp32 tensor [rows][cols], rows any stride apart."""
-    if t.dtype != _torch().float32 or t.shape != (rows, cols) or t.device != device or (t.stride(1) != 1 and cols > 1):
+    stride = t.stride()
+    if t.dtype is not f32 or t.shape != (rows, cols) or t.device != device or (stride[1] != 1 and cols > 1):
         raise ZestError(f"{what}: float32 rows [{rows}][{cols}] on {device} wanted")
-    return t.data_ptr(), t.stride(0) if rows > 1 else cols
+    return t.data_ptr(), stride[0] if rows > 1 else cols
 
 
-def _gguf(t, what: str, wtype: int, n: int, k: int, device) -> int:
+def _gguf(t, what: str, wtype: int, size: int, n: int, k: int, device, u8) -> int:
     """The pointer of n GGUF rows of k values: a contiguous uint8 tensor of their bytes."""
-    size = n * lib().zest_raw_row_bytes(wtype, k)
-    if t.dtype != _torch().uint8 or not t.is_contiguous() or t.device != device or size == 0 or t.numel() != size:
+    if t.dtype is not u8 or size == 0 or t.numel() != n * size or t.device != device or not t.is_contiguous():
         raise ZestError(f"{what}: a contiguous uint8 tensor on {device} of {n} rows of {k} values of type {wtype} wanted")
     return t.data_ptr()
 
 
-def _matvec_workspace(workspace, wtype: int, m: int, k: int, ns, device):
-    torch, n = _torch(), len(ns)
-    need = lib().zest_matvec_workspace(wtype, m, k, n, (ctypes.c_int64 * n)(*ns))
+@functools.lru_cache(maxsize=4096)
+def _matvec_sizes(wtype: int, m: int, k: int, ns: tuple) -> tuple[int, int]:
+    """Bytes of a weight's row, and of the workspace (host arithmetic, kept by sizes: it is a good part of a small call's
+    time)."""
+    n = len(ns)
+    return lib().zest_raw_row_bytes(wtype, k), lib().zest_matvec_workspace(wtype, m, k, n, (ctypes.c_int64 * n)(*ns))
+
+
+def _matvec_workspace(workspace, need: int, device):
+    """(The tensor, so that it lives until the launch is queued,) its pointer and its bytes."""
     if workspace is None:
-        return torch.empty(max(need, 1), dtype=torch.uint8, device=device)
-    if workspace.device != device or not workspace.is_contiguous():
+        if not need:
+            return None, None, 0
+        workspace = _torch().empty(need, dtype=_torch().uint8, device=device)
+    elif workspace.device != device or not workspace.is_contiguous():
         raise ZestError(f"workspace: a contiguous tensor on {device} wanted")
-    return workspace
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def matvec_workspace(wtype: int, m: int, k: int, ns) -> int:
-    """Bytes of matvec's workspace, by sizes alone (matvec_glu: ns = [f, f])."""
-    return lib().zest_matvec_workspace(wtype, m, k, len(ns), (ctypes.c_int64 * len(ns))(*ns))
+    """Bytes of matvec's workspace, by sizes alone, 0: none is wanted (matvec_glu: ns = [f, f])."""
+    return _matvec_sizes(wtype, m, k, tuple(ns))[1]
 
 
 def matvec(wtype: int, x, weights, ns, outs=None, residuals=None, workspace=None):
     """zest_matvec: outs[i][m][ns[i]] = x . W_i^T (+ residuals[i]) for up to 4 GGUF weights (uint8 device tensors of
     ns[i] rows, as a model file holds them) on one fp32 x of 1 to 16 rows. Returns the outputs."""
-    torch, n = _torch(), len(weights)
-    dev = x.device
+    torch, n, dev = _torch(), len(weights), x.device
+    f32, u8 = torch.float32, torch.uint8
     _need_here(dev)
     if x.dim() != 2:
         raise ZestError("x: rows [m][k] wanted")
     m, k = x.shape
-    if len(ns) != n or any(l is not None and len(l) != n for l in (outs, residuals)):
+    if len(ns) != n or (outs is not None and len(outs) != n) or (residuals is not None and len(residuals) != n):
         raise ZestError(f"{n} weights: as many sizes, outputs and residuals wanted")
-    px, ldx = _fp32_rows(x, "x", m, k, dev)
-    w = [_gguf(t, f"weight {i}", wtype, ns[i], k, dev) for i, t in enumerate(weights)]
-    outs = [torch.empty((m, ni), dtype=torch.float32, device=dev) for ni in ns] if outs is None else outs
-    y = [_fp32_rows(t, f"output {i}", m, ns[i], dev) for i, t in enumerate(outs)]
-    res = [(None, 0) if t is None else _fp32_rows(t, f"residual {i}", m, ns[i], dev) for i, t in enumerate(residuals or [None] * n)]
-    ws = _matvec_workspace(workspace, wtype, m, k, ns, dev)
-    P, I64 = ctypes.c_void_p * n, ctypes.c_int64 * n
-    check(lib().zest_matvec(wtype, px, m, k, ldx, n, P(*w), I64(*ns), P(*[p for p, _ in res]), I64(*[l for _, l in res]),
-                            P(*[p for p, _ in y]), I64(*[l for _, l in y]), ws.data_ptr(), ws.numel() * ws.element_size(),
-                            _stream()), "zest_matvec")
+    px, ldx = _fp32_rows(x, "x", m, k, dev, f32)
+    size, need = _matvec_sizes(wtype, m, k, tuple(ns))
+    if outs is None:
+        outs = [torch.empty((m, ni), dtype=f32, device=dev) for ni in ns]
+    w, py, ldy, pr, ldr = [], [], [], [], []
+    for i in range(n):
+        ni = ns[i]
+        w.append(_gguf(weights[i], "weight", wtype, size, ni, k, dev, u8))
+        p, ld = _fp32_rows(outs[i], "output", m, ni, dev, f32)
+        py.append(p)
+        ldy.append(ld)
+        if residuals is not None and residuals[i] is not None:
+            p, ld = _fp32_rows(residuals[i], "residual", m, ni, dev, f32)
+        else:
+            p = ld = 0
+        pr.append(p)
+        ldr.append(ld)
+    keep, ws, ws_bytes = _matvec_workspace(workspace, need, dev)
+    q = _PACK[n] if n <= 4 else struct.Struct(f"{n}q").pack  # (arrays of pointers and sizes, as bytes)
+    check(lib().zest_matvec(wtype, px, m, k, ldx, n, q(*w), q(*ns), q(*pr) if residuals is not None else None,
+                            q(*ldr) if residuals is not None else None, q(*py), q(*ldy), ws, ws_bytes, _stream()), "zest_matvec")
     return outs
+
+
+_PACK = [struct.Struct(f"{n}q").pack for n in range(5)]
 
 
 def matvec_glu(kind: int, wtype: int, x, gate, up, f: int, out=None, workspace=None):
     """zest_matvec_glu: out[m][f] = glu(x . gate^T, x . up^T) for two GGUF weights of f rows."""
     torch, dev = _torch(), x.device
+    f32, u8 = torch.float32, torch.uint8
     _need_here(dev)
     if x.dim() != 2:
         raise ZestError("x: rows [m][k] wanted")
     m, k = x.shape
-    px, ldx = _fp32_rows(x, "x", m, k, dev)
-    out = torch.empty((m, f), dtype=torch.float32, device=dev) if out is None else out
-    py, ldy = _fp32_rows(out, "out", m, f, dev)
-    ws = _matvec_workspace(workspace, wtype, m, k, [f, f], dev)
-    check(lib().zest_matvec_glu(kind, wtype, px, m, k, ldx, _gguf(gate, "gate", wtype, f, k, dev), _gguf(up, "up", wtype, f, k, dev),
-                                f, py, ldy, ws.data_ptr(), ws.numel() * ws.element_size(), _stream()), "zest_matvec_glu")
+    px, ldx = _fp32_rows(x, "x", m, k, dev, f32)
+    size, need = _matvec_sizes(wtype, m, k, (f, f))
+    out = torch.empty((m, f), dtype=f32, device=dev) if out is None else out
+    py, ldy = _fp32_rows(out, "out", m, f, dev, f32)
+    keep, ws, ws_bytes = _matvec_workspace(workspace, need, dev)
+    check(lib().zest_matvec_glu(kind, wtype, px, m, k, ldx, _gguf(gate, "gate", wtype, size, f, k, dev, u8),
+                                _gguf(up, "up", wtype, size, f, k, dev, u8), f, py, ldy, ws, ws_bytes, _stream()), "zest_matvec_glu")
     return out
 
 

@@ -608,7 +608,8 @@ __device__ inline call_row row_of(const matvec_args & a, int r) {
 // RING pieces (two units of 16 rows, 4.6 KB) a wave, requested as soon as their place
 // is read. A workgroup's last 16 rows are as many as are left of its share: a row that
 // is not there is its neighbour again. So all CUs stream whatever the number of rows.
-template <int TYPE, int M, int S, int RING, bool READY> __global__ __launch_bounds__(STREAM_WAVES * 64) void stream_kernel(matvec_args a) {
+template <int TYPE, int M, int S, int RING, bool READY>
+__global__ __launch_bounds__(STREAM_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void stream_kernel(matvec_args a) {
     typedef quant<TYPE> Q;
     typedef stream<TYPE> ST;
     typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -738,48 +739,64 @@ template <int TYPE, int M, int S, int RING, bool READY> __global__ __launch_boun
     };
     const bool digit = (col >> 2) == group && (col & 3) < 3;
     const int ragged = a.chunks - (pieces - 1) * (STEPS * GROUPS) < STEPS * GROUPS ? pieces - 1 : pieces;  // the piece that is not whole
+    // What a step takes from shared memory: requested a step ahead.
+    struct operands {
+        typename Q::raw w[S];
+        i32x4 x[M][B][2];
+        f32x2 f[M][B];  // the factor and the sum
+    };
     auto compute = [&](int piece, uint32_t slot, auto edge) {
         constexpr bool EDGE = decltype(edge)::value;
         uint32_t unit[S];
 #pragma unroll
         for (int s = 0; s < S; s++) unit[s] = slot + (s * 16 + col) * (GP * 16) + (ALIGN < 16 ? (begins[s] + (uint32_t) piece * (U * ST::UNIT)) & 15 : 0);
+        const int step0 = piece * STEPS;
+        auto request = [&](int i, operands & o) {
 #pragma unroll
-        for (int i = 0; i < STEPS; i++) {
-            const int step = piece * STEPS + i, chunk = step * GROUPS + group;
-            if (EDGE && step * GROUPS >= a.chunks) continue;
-            const bool in = !EDGE || chunk < a.chunks;
-            i32x4 code[S][B][2];
-            block_scales<B> sc[S];
-#pragma unroll
-            for (int s = 0; s < S; s++) {
-                // (past the row's end: any bytes, whose scales are then replaced)
-                const typename Q::raw r = ST::read(unit[s] + i / (ST::CHUNKS / GROUPS) * ST::UNIT, (i % (ST::CHUNKS / GROUPS)) * GROUPS + group);
-                uint32_t c[B][2][4];
-                Q::codes(r, c);
-                sc[s] = Q::scales(r, chunk);
-#pragma unroll
-                for (int b = 0; b < B; b++) {
-#pragma unroll
-                    for (int h = 0; h < 2; h++) code[s][b][h] = i32x4{(int) c[b][h][0], (int) c[b][h][1], (int) c[b][h][2], (int) c[b][h][3]};
-                    if (!in) sc[s].scale[b] = sc[s].offset[b] = 0.0f;
-                }
-            }
-            const uint32_t cell = cells + (step * GROUPS + (in ? group : 0)) * (B * M * CELL_AT);
+            for (int s = 0; s < S; s++)  // (past the row's end: any bytes, whose scales are then replaced)
+                o.w[s] = ST::read(unit[s] + i / (ST::CHUNKS / GROUPS) * ST::UNIT, (i % (ST::CHUNKS / GROUPS)) * GROUPS + group);
+            const bool in = !EDGE || (step0 + i) * GROUPS + group < a.chunks;
+            const uint32_t cell = cells + (EDGE ? min((step0 + i) * GROUPS + group, a.chunks - 1) : (step0 + i) * GROUPS + group) * (B * M * CELL_AT);
             const uint32_t x_at = digit && in ? cell + (col & 3) * 16 : zeros;
             const uint32_t stride = digit && in ? CELL_AT : 0, part = digit && in ? 48 : 0;
 #pragma unroll
-            for (int m = 0; m < M; m++) {
+            for (int m = 0; m < M; m++)
 #pragma unroll
                 for (int b = 0; b < B; b++) {
-                    const i32x4 x0 = lds<i32x4>(x_at + (b * M + m) * stride), x1 = lds<i32x4>(x_at + (b * M + m) * stride + part);
-                    const f32x2 f = lds<f32x2>(cell + (b * M + m) * CELL_AT + 96);  // the factor and the sum
+                    o.x[m][b][0] = lds<i32x4>(x_at + (b * M + m) * stride);
+                    o.x[m][b][1] = lds<i32x4>(x_at + (b * M + m) * stride + part);
+                    o.f[m][b] = lds<f32x2>(cell + (b * M + m) * CELL_AT + 96);
+                }
+        };
+        operands o[2];
+        request(0, o[0]);
 #pragma unroll
-                    for (int s = 0; s < S; s++) {
-                        i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x0, code[s][b][0], i32x4{}, 0, 0, 0);
-                        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x1, code[s][b][1], d, 0, 0, 0);
-                        const float v = Q::NIBBLES ? (float) ((((d[0] << 8) + d[1]) << 8) + d[2]) : fmaf((float) d[0], 65536.0f, (float) ((d[1] << 8) + d[2]));
-                        acc[m][s] = fmaf(v, sc[s].scale[b] * f.x, acc[m][s]);
-                        if constexpr (Q::OFFSETS) acc[m][s] = fmaf(f.y, sc[s].offset[b], acc[m][s]);
+        for (int i = 0; i < STEPS; i++) {
+            if (i + 1 < STEPS) request(i + 1, o[(i + 1) & 1]);
+            asm volatile("" ::: "memory");
+            const operands & now = o[i & 1];
+            const int chunk = (step0 + i) * GROUPS + group;
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                uint32_t c[B][2][4];
+                Q::codes(now.w[s], c);
+                block_scales<B> sc = Q::scales(now.w[s], chunk);
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    if (EDGE && chunk >= a.chunks) sc.scale[b] = sc.offset[b] = 0.0f;
+                    i32x4 d[M];
+#pragma unroll
+                    for (int m = 0; m < M; m++)
+                        d[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.x[m][b][0], i32x4{(int) c[b][0][0], (int) c[b][0][1], (int) c[b][0][2], (int) c[b][0][3]}, i32x4{}, 0, 0, 0);
+#pragma unroll
+                    for (int m = 0; m < M; m++)
+                        d[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.x[m][b][1], i32x4{(int) c[b][1][0], (int) c[b][1][1], (int) c[b][1][2], (int) c[b][1][3]}, d[m], 0, 0, 0);
+#pragma unroll
+                    for (int m = 0; m < M; m++) {
+                        // (|d0| <= 64 15 32 < 2^15 for nibbles, so they fit in 32 bits together)
+                        const float v = Q::NIBBLES ? (float) ((((d[m][0] << 8) + d[m][1]) << 8) + d[m][2]) : fmaf((float) d[m][0], 65536.0f, (float) ((d[m][1] << 8) + d[m][2]));
+                        acc[m][s] = fmaf(v, sc.scale[b] * now.f[m][b].x, acc[m][s]);
+                        if constexpr (Q::OFFSETS) acc[m][s] = fmaf(now.f[m][b].y, sc.offset[b], acc[m][s]);
                     }
                 }
             }
@@ -894,7 +911,7 @@ matvec_plan plan_of(int type, int64_t M, int64_t K, int n, const int64_t * N, bo
             for (const int cell : {RAW_CELL, CELL}) {
                 p.lds = lds_of(p.ring, cell);
                 p.copy = cell == CELL;
-                p.bytes = p.copy ? (size_t) B * chunks * M * CELL : 16;
+                p.bytes = p.copy ? (size_t) B * chunks * M * CELL : 0;
                 if (p.lds <= LDS_MOST && (p.ring == 2 || !p.copy)) return p;
             }
         p.ring = 0;
@@ -911,7 +928,7 @@ matvec_plan plan_of(int type, int64_t M, int64_t K, int n, const int64_t * N, bo
     p.lds = 16 + (size_t) std::min(p.seg_steps * GROUPS, chunks) * B * M * CELL + red;
     p.workgroups = (int) std::min<int64_t>((tiles + p.wr - 1) / p.wr, 512);
     if (p.lds > LDS_MOST / 2 || p.wk * p.wr > 8) p.workgroups = std::min(p.workgroups, 256);
-    p.bytes = std::max<size_t>(16, p.copy ? (size_t) chunks * B * M * CELL : 0);
+    p.bytes = (size_t) chunks * B * M * CELL;
     return p;
 }
 
@@ -1046,7 +1063,7 @@ int matvec(const char * me, int glu, int type, const float * x, int64_t M, int64
     }
     // (a GLU's plan is that of two weights as far as its workspace goes)
     const matvec_plan p = plan_of(type, M, K, n, N, glu >= 0);
-    ZEST_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= p.bytes, "%s: workspace of %zu bytes, 16-byte aligned, wanted", me, p.bytes);
+    ZEST_REQUIRE(!p.bytes || (workspace && aligned(workspace, 16) && workspace_bytes >= p.bytes), "%s: workspace of %zu bytes, 16-byte aligned, wanted", me, p.bytes);
     a.all_tiles = (int32_t) tiles;
     a.wk = p.wk, a.wr = p.wr, a.seg_steps = p.seg_steps, a.segs = p.segs;
     a.cells = (uint8_t *) workspace;
@@ -1059,8 +1076,11 @@ int matvec(const char * me, int glu, int type, const float * x, int64_t M, int64
 extern "C" {
 
 size_t zest_matvec_workspace(int type, int64_t M, int64_t K, int n, const int64_t * N) {
-    if (!supported(type) || M <= 0 || M > MAX_M || K <= 0 || K > (1 << 20) || n < 1 || n > MAX_N || !N) return 0;
-    return std::max<size_t>(16, (size_t) (K / 32) * M * CELL);
+    if (!supported(type) || M <= 0 || M > MAX_M || K <= 0 || K > (1 << 20) || !zest_raw_row_bytes(type, K) || n < 1 || n > MAX_N || !N) return 0;
+    for (int i = 0; i < n; i++)
+        if (N[i] <= 0 || N[i] > (1 << 26)) return 0;
+    const size_t bytes = plan_of(type, M, K, n, N, false).bytes;
+    return n == 2 && N[0] == N[1] ? std::max(bytes, plan_of(type, M, K, n, N, true).bytes) : bytes;
 }
 
 int zest_matvec(int type, const float * x, int64_t M, int64_t K, int64_t ldx, int n, const void * const * w, const int64_t * N,

@@ -9,8 +9,9 @@
  * claims matmuls of 1024 rows and more), so these have no counterpart in it.
  *
  * Workspaces are the caller's, 16-byte aligned, of the size that a host call
- * gives by sizes alone. They hold nothing between calls; calls that may overlap
- * (on two streams, or as replays of two graphs) need one each.
+ * gives by sizes alone (0: none is wanted, and NULL will do). They hold nothing
+ * between calls; calls that may overlap (on two streams, or as replays of two
+ * graphs) need one each.
  */
 #ifndef ZEST_DECODE_H
 #define ZEST_DECODE_H

@@ -62,7 +62,7 @@ def test_matvec_refuses():
                          (dict(n=(0,)), E_ARG), (dict(n=((1 << 26) + 1,)), E_ARG), (dict(y=(None,)), E_ARG), (dict(y=(y + 2,)), E_ARG), (dict(ldy=(7,)), E_ARG),
                          (dict(count=0), E_ARG), (dict(w=(w,) * 5, n=(8,) * 5, y=tuple(y + 4096 * i for i in range(5)), ldy=(8,) * 5), E_ARG),
                          (dict(res=(r + 2,), ldr=(8,)), E_ARG), (dict(res=(r,), ldr=(7,)), E_ARG), (dict(res=(r,)), E_ARG),
-                         (dict(ws=None), E_ARG), (dict(ws=base + (1 << 20) + 4), E_ARG), (dict(size=0), E_ARG)]:
+                         (dict(m=9, ws=None), E_ARG), (dict(m=9, ws=base + (1 << 20) + 4), E_ARG), (dict(m=9, size=9 * 2 * 112 - 1), E_ARG)]:
         _refused("zest_matvec", call(**broken), code)
     # overlaps: of an output with x, a weight, another output, a residual that it is not
     two = dict(w=(w, w), n=(8, 8), ldy=(8, 8))
@@ -72,9 +72,17 @@ def test_matvec_refuses():
         assert "overlap" in lib.zest_last_error().decode(), broken
     # columns of one buffer, a residual in place: past that check, refused for the workspace
     wide = dict(w=(w, w), n=(8, 8), ldy=(16, 16), y=(y, y + 32))
-    for fine in (wide, dict(res=(y,), ldr=(8,)), dict(res=(y + 32, y), ldr=(16, 16), **dict(wide, y=(y + 32, y)))):
+    for fine in (dict(m=9, **wide), dict(m=9, res=(y,), ldr=(8,)), dict(m=9, res=(y + 32, y), ldr=(16, 16), **dict(wide, y=(y + 32, y)))):
         _refused("zest_matvec", call(ws=None, **fine), E_ARG)
         assert "workspace" in lib.zest_last_error().decode(), fine
+
+
+def test_matvec_workspace_goes_by_sizes():
+    lib = _lib()
+    ws = lambda t, m, k, *n: lib.zest_matvec_workspace(t, m, k, len(n), (ctypes.c_int64 * len(n))(*n))  # noqa: E731
+    assert ws(12, 1, 2560, 4096) == 0 and ws(12, 9, 2560, 4096) == 80 * 9 * 112
+    assert ws(12, 4, 5120, 17408, 17408) == 160 * 4 * 112  # as a GLU's
+    assert [ws(0, 1, 256, 8), ws(12, 1, 128, 8), ws(12, 0, 256, 8), ws(12, 17, 256, 8), ws(12, 9, 256, 0), ws(12, 9, 256)] == [0] * 6
 
 
 def test_matvec_glu_refuses():
@@ -86,7 +94,7 @@ def test_matvec_glu_refuses():
 
     for broken, code in [(dict(kind=5), E_UNSUPPORTED), (dict(kind=-1), E_UNSUPPORTED), (dict(type=1), E_UNSUPPORTED), (dict(m=0), E_ARG), (dict(m=17), E_ARG),
                          (dict(k=33), E_ARG), (dict(x=None), E_ARG), (dict(gate=None), E_ARG), (dict(up=None), E_ARG), (dict(up=w + 1), E_ARG), (dict(f=0), E_ARG),
-                         (dict(y=None), E_ARG), (dict(ldy=4), E_ARG), (dict(y=base), E_ARG), (dict(y=w + 4096), E_ARG), (dict(ws=None), E_ARG), (dict(size=1), E_ARG)]:
+                         (dict(y=None), E_ARG), (dict(ldy=4), E_ARG), (dict(y=base), E_ARG), (dict(y=w + 4096), E_ARG), (dict(m=16, ws=None), E_ARG), (dict(m=16, size=1), E_ARG)]:
         _refused("zest_matvec_glu", call(**broken), code)
 
 
