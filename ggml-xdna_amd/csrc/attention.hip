@@ -25,6 +25,7 @@ namespace {
 using zest::kv_batch;
 using zest::kv_pages;
 using zest::kv_seq;
+using zest::kv_view;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -81,7 +82,20 @@ struct attn_args {
     float * partial;
     float * chunk_partial;
     int32_t chunk_blocks, chunk_splits;
+    // sequences that share leading pages: the view's, and where attend_few's whole
+    // results go, [row][query head][D], then their maxima and sums
+    kv_view view;
+    float * own;
 };
+
+// The sequences that a kernel works on.
+template <bool VIEW> __device__ inline const auto & seqs_of(const attn_args & a) {
+    if constexpr (VIEW) return a.view;
+    else return a.b;
+}
+template <bool VIEW> __device__ inline const int32_t * table_of(const attn_args & a, const kv_seq & s) {
+    return VIEW ? a.b.tables + s.slot : zest::table_of(a.b, s);
+}
 
 // Tokens [lo, hi) that any of a sequence's rows i0 .. i1 sees.
 __device__ inline void seen_by(const attn_args & a, const kv_seq & s, int i0, int i1, int32_t & lo, int32_t & hi) {
@@ -291,7 +305,10 @@ constexpr int partial_floats(int cols, int D) { return cols * (D + 2); }
 // are half the registers. The two 16-token score tiles of a step are tokens
 // {0..7, 16..23} and {8..15, 24..31}, so that a lane group's 8 weights, in the
 // registers they are in, are the 8 tokens of a V piece.
-template <int TYPE, int D, int NT>
+//
+// VIEW: of sequences that share leading pages, what each holds of its own; nothing
+// goes to the output but to a.own, for join_shared.
+template <int TYPE, int D, int NT, bool VIEW>
 __device__ __forceinline__ void attend_few(const attn_args & a, int block, int blocks, uint8_t * ring_sh) {
     typedef typename elem<TYPE>::frag frag;
     constexpr int COLS = 16 * NT, KS = D / 32, DT = D / 16, R = RING_B<D>, LOADS = D / 16;  // loads of K (or V) a step
@@ -299,7 +316,7 @@ __device__ __forceinline__ void attend_few(const attn_args & a, int block, int b
     __shared__ float stat[WAVES][2][COLS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = lane >> 4, col = lane & 15;
     const int ps = a.c.page_shift, P = 1 << ps;
-    const zest::seq_index index(a.b, ps, reinterpret_cast<int32_t *>(ring_sh + WAVES * R * STEP_BYTES<D>),
+    const zest::seq_index index(seqs_of<VIEW>(a), ps, reinterpret_cast<int32_t *>(ring_sh + WAVES * R * STEP_BYTES<D>),
                                 [&](const kv_seq & s) { return cost_of(a, s, COLS); });
     const unit_shares shares(index.total, blocks);
     int32_t u = shares.start(block);
@@ -313,7 +330,7 @@ __device__ __forceinline__ void attend_few(const attn_args & a, int block, int b
         const int32_t run = units_of(a, s), at = u - before, tiles = col_tiles(a, s, COLS);
         const int32_t item = at / run, first = at - item * run, h = item / tiles, ct = item - h * tiles;
         const int32_t units = min(run - first, u1 - u);
-        const int32_t * row = a.b.tables + (int64_t) s.slot * a.b.table_cols;
+        const int32_t * row = table_of<VIEW>(a, s);
         const int ncols = s.n * a.group, c0 = ct * COLS;
         // what all the tile's columns see, and what any of them does
         int32_t all_lo, all_hi, any_lo, any_hi, seq_lo, seq_hi;
@@ -578,10 +595,17 @@ __device__ __forceinline__ void attend_few(const attn_args & a, int block, int b
                     part[COLS * D + COLS + oc] = sum;
                 }
             } else if (cc < ncols) {
+                const int i0 = cc / a.group;
+                if constexpr (VIEW) {
+                    const int heads = a.group * a.c.kv_heads;
+                    const int64_t at = (int64_t) (s.row0 + i0) * heads + h * a.group + cc - i0 * a.group;
+                    *reinterpret_cast<float4 *>(a.own + at * D + unit * 4) = make_float4(v[0], v[1], v[2], v[3]);
+                    if (unit == 0) *reinterpret_cast<float2 *>(a.own + a.b.rows * heads * D + at * 2) = make_float2(top, sum);
+                    continue;
+                }
                 const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] *= f;
-                const int i0 = cc / a.group;
                 store4(a, (int64_t) (s.row0 + i0) * a.ldo + (int64_t) (h * a.group + cc - i0 * a.group) * D + unit * 4, v);
             }
         }
@@ -690,13 +714,16 @@ __device__ inline int32_t chunk_tiles_of(const attn_args & a, const kv_seq & s, 
 // the reads of shared memory (a third busy as it is) but leave one wave a SIMD.
 // 192-wide heads take eight waves, one workgroup a CU: with four, a wave a SIMD,
 // 765 us for 24 heads at 8192, with eight 342.
-template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const attn_args & a, int block, int split, uint8_t * ring) {
+//
+// VIEW: what groups of sequences share, all rows of a group being one chunk that sees
+// all of it; the parts stay parts, for join_shared.
+template <int TYPE, int D, bool VIEW> __device__ __forceinline__ void attend_chunk(const attn_args & a, int block, int split, uint8_t * ring) {
     typedef typename elem<TYPE>::frag frag;
     constexpr int NQ = QT, KS = D / 16, DT = D / 32;
     // ring: [K_RING][D/8][32][8], [V_RING][2][2][D][8]; then the prefix sums
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     const int ps = a.c.page_shift, P = 1 << ps;
-    const zest::seq_index index(a.b, ps, reinterpret_cast<int32_t *>(ring + CHUNK_RING<D>),
+    const zest::seq_index index(seqs_of<VIEW>(a), ps, reinterpret_cast<int32_t *>(ring + CHUNK_RING<D>),
                                 [&](const kv_seq & s) { return chunk_tiles_of(a, s, CHUNK<D>); });
     // Under a causal mask the last tiles see the most. Where all fit the GPU at
     // once, two a CU, a CU gets one from either end (workgroup i + CUS joins i);
@@ -715,7 +742,7 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
     int32_t before;
     const kv_seq s = index.at(tile, before);
     const int c0 = (tile - before) * CHUNK<D>, ncols = s.n * a.group;
-    const int32_t * row = a.b.tables + (int64_t) s.slot * a.b.table_cols;
+    const int32_t * row = table_of<VIEW>(a, s);
 
     // the tile's tokens, and of them this split's
     int32_t lo, hi;
@@ -1016,7 +1043,7 @@ template <int TYPE, int D> __device__ __forceinline__ void attend_chunk(const at
     }
     if (bad) zest::report(a.b.bad);
 
-    if (a.chunk_splits > 1) {
+    if (VIEW || a.chunk_splits > 1) {
         // this split's part: O^T in the registers' own order, maxima and sums
         float * slot = a.chunk_partial + ((int64_t) (tile * a.c.kv_heads + h) * a.chunk_splits + split) * CHUNK_PARTIAL<D>;
 #pragma unroll
@@ -1118,10 +1145,26 @@ __global__ __launch_bounds__((CHUNKS ? chunk_waves(D) : WAVES) * 64, D > 192 || 
     if constexpr (CHUNKS)
         if ((int) blockIdx.x >= few) {
             const int at = blockIdx.x - few, split = at / a.chunk_blocks;
-            attend_chunk<TYPE, D>(a, at - split * a.chunk_blocks, split, smem);
+            attend_chunk<TYPE, D, false>(a, at - split * a.chunk_blocks, split, smem);
             return;
         }
-    if constexpr (NT > 0) attend_few<TYPE, D, NT>(a, blockIdx.x, few, smem);
+    if constexpr (NT > 0) attend_few<TYPE, D, NT, false>(a, blockIdx.x, few, smem);
+}
+
+// The same over shared leading pages: few columns of what each sequence holds of its
+// own (a), chunks of what groups share (g).
+template <int TYPE, int D, int NT, bool CHUNKS>
+__global__ __launch_bounds__((CHUNKS ? chunk_waves(D) : WAVES) * 64, D > 192 || (D > 128 && !CHUNKS) ? 1 : 2) void shared_kernel(attn_args a, attn_args g) {
+    static_assert(!CHUNKS || NT == 0 || chunk_waves(D) == WAVES, "workgroups of one size");
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int few = gridDim.x - (CHUNKS ? g.chunk_blocks * g.chunk_splits : 0);
+    if constexpr (CHUNKS)
+        if ((int) blockIdx.x >= few) {
+            const int at = blockIdx.x - few, split = at / g.chunk_blocks;
+            attend_chunk<TYPE, D, true>(g, at - split * g.chunk_blocks, split, smem);
+            return;
+        }
+    if constexpr (NT > 0) attend_few<TYPE, D, NT, true>(a, blockIdx.x, few, smem);
 }
 
 template <int D, int NT, bool CHUNKS> __global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
@@ -1137,6 +1180,240 @@ template <int D, int NT, bool CHUNKS> __global__ __launch_bounds__(256) void com
         const int at = blockIdx.x - chunks;
         combine_few<D, NT>(a, at / PARTS, at % PARTS, (gridDim.x - chunks) / PARTS, attn_sh);
     }
+}
+
+// ---- shared leading pages -------------------------------------------------------------
+
+// What share_kernel finds of a sequence beside its view: its group's first row and first
+// tile (of attend_chunk, in all), what the group shares, and the units of attend_few
+// before it.
+struct share {
+    int32_t group_row0, group_tile, tokens, units_before;
+};
+
+struct share_args {
+    attn_args a;               // of attend_few, a.view not yet written
+    const int32_t * starts;    // the groups'
+    int32_t groups, max_shared, chunk, cols;
+    kv_seq * seqs, * group_list;
+    share * shares;
+};
+
+constexpr int SHARE_THREADS = 1024, SHARE_LANES = 16, SHARE_PAGES = 128;
+constexpr int MAX_GROUPS = 2048;
+inline size_t share_lds(int seqs, int groups) { return (size_t) seqs * 16 + (size_t) groups * 32 + (size_t) ((std::max(seqs, groups) + 4) & ~3) * 4 + (size_t) seqs * 2; }
+
+// One workgroup looks the batch over: the sequences, checked; of each group the leading
+// pages that all its members with new tokens name alike, each of them in the pool, as
+// far as all their rows see all of them; and where everyone's work lies. Sixteen lanes
+// compare 128 pages of a member with the first one's at once.
+__global__ __launch_bounds__(SHARE_THREADS) void share_kernel(share_args p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const attn_args & a = p.a;
+    const int t = threadIdx.x, ps = a.c.page_shift, seqs = a.b.seqs, most = max(seqs, p.groups);
+    kv_seq * const seq = reinterpret_cast<kv_seq *>(smem), * const group = seq + seqs;
+    int32_t * const limit = reinterpret_cast<int32_t *>(group + p.groups), * const members = limit + p.groups, * const first = members + p.groups,
+                    * const begin = first + p.groups, * const prefix = begin + p.groups;
+    uint16_t * const groups_of = reinterpret_cast<uint16_t *>(prefix + ((most + 4) & ~3));  // 0xffff: of none
+    const auto group_of = [&](int b) { return groups_of[b] == 0xffff ? -1 : (int) groups_of[b]; };
+    bool bad = false, odd = false;
+    for (int g = t; g < p.groups; g += SHARE_THREADS) {
+        const int s0 = p.starts[g], s1 = p.starts[g + 1];
+        odd |= s0 < 0 || s1 < s0 || s1 > seqs;
+        limit[g] = p.max_shared >> ps;  // pages
+        members[g] = 0;
+        first[g] = 0x7fffffff;
+        begin[g] = s0;
+    }
+    for (int b = t; b < seqs; b += SHARE_THREADS) {
+        seq[b] = zest::load_seq(a.b, b, ps, bad);
+        groups_of[b] = 0xffff;
+    }
+    odd = __syncthreads_or(odd);
+    bad |= odd;
+    if (!odd)
+        for (int g = t >> 6; g < p.groups; g += SHARE_THREADS / 64) {
+            const int s1 = g + 1 < p.groups ? begin[g + 1] : p.starts[p.groups];
+            for (int b = begin[g] + (t & 63); b < s1; b += 64) groups_of[b] = (uint16_t) g;
+        }
+    __syncthreads();
+    for (int b = t; b < seqs; b += SHARE_THREADS) {
+        const int g = group_of(b);
+        if (g < 0 || seq[b].n == 0) continue;
+        const kv_seq s = seq[b];
+        int sees = a.causal ? min(s.len, s.len - s.n + 1) : s.len;  // of the first row
+        if (a.window > 0 && s.len > a.window) sees = 0;             // of the last one
+        atomicMin(&limit[g], max(sees, 0) >> ps);
+        atomicAdd(&members[g], 1);
+        atomicMin(&first[g], b);
+    }
+    __syncthreads();
+    for (int g = t; g < p.groups; g += SHARE_THREADS)
+        if (members[g] < 2) limit[g] = 0;
+    __syncthreads();
+    for (int b0 = 0; b0 < seqs; b0 += SHARE_THREADS / SHARE_LANES) {
+        const int b = b0 + t / SHARE_LANES, lane = t % SHARE_LANES, g = b < seqs ? group_of(b) : -1;
+        if (g < 0 || seq[b].n == 0) continue;
+        const int pages = limit[g];  // (it falls while others compare: no more than this is looked at)
+        const int32_t * mine = zest::table_of(a.b, seq[b]), * theirs = zest::table_of(a.b, seq[first[g]]);
+        for (int j0 = 0; j0 < pages; j0 += SHARE_PAGES) {
+            int32_t x[SHARE_PAGES / SHARE_LANES], y[SHARE_PAGES / SHARE_LANES];
+#pragma unroll
+            for (int i = 0; i < SHARE_PAGES / SHARE_LANES; i++) {
+                const int j = min(j0 + i * SHARE_LANES + lane, pages - 1);
+                x[i] = mine[j];
+                y[i] = theirs[j];
+            }
+            int apart = 0x7fffffff;
+#pragma unroll
+            for (int i = 0; i < SHARE_PAGES / SHARE_LANES; i++)
+                if (x[i] != y[i] || (uint32_t) x[i] >= (uint32_t) a.c.pages) apart = min(apart, min(j0 + i * SHARE_LANES + lane, pages - 1));
+            if (apart < pages) atomicMin(&limit[g], apart);
+            if (limit[g] <= j0) break;
+        }
+    }
+    __syncthreads();
+    for (int g = t; g < p.groups; g += SHARE_THREADS) {
+        // its rows, first to last member's (those of a member that is left out among them)
+        const int pages = limit[g];
+        kv_seq s{0, 0, 0, 0};
+        if (pages > 0) {
+            const kv_seq f = seq[first[g]];
+            s = kv_seq{f.row0, 0, pages << ps, f.slot * a.b.table_cols};
+        }
+        group[g] = s;
+        members[g] = 0;  // now the rows' end
+    }
+    __syncthreads();
+    for (int b = t; b < seqs; b += SHARE_THREADS) {
+        const int g = group_of(b);
+        if (g >= 0 && seq[b].n > 0 && group[g].len > 0) {
+            atomicMax(&members[g], seq[b].row0 + seq[b].n);
+            atomicMin(&group[g].row0, seq[b].row0);
+        }
+    }
+    __syncthreads();
+    for (int g = t; g < p.groups; g += SHARE_THREADS)
+        if (group[g].len > 0) group[g].n = members[g] - group[g].row0;
+    __syncthreads();
+    {
+        const kv_view view{group, p.groups, nullptr};
+        const zest::seq_index index(view, ps, prefix, [&](const kv_seq & s) { return (int32_t) (((int64_t) s.n * a.group + p.chunk - 1) / p.chunk); });
+        for (int g0 = 0; g0 < p.groups; g0 += SHARE_THREADS) {
+            const int g = g0 + t, at = index.before(min(g, p.groups - 1));
+            if (g < p.groups) {
+                first[g] = at;
+                p.group_list[g] = group[g];
+            }
+        }
+    }
+    __syncthreads();
+    for (int b = t; b < seqs; b += SHARE_THREADS) {
+        const int g = group_of(b);
+        kv_seq s = seq[b];
+        share h{0, 0, 0, 0};
+        s.slot *= s.n > 0 ? a.b.table_cols : 0;
+        if (g >= 0 && s.n > 0 && group[g].len > 0) {
+            h = share{group[g].row0, first[g], group[g].len, 0};
+            s.len -= h.tokens;
+            s.slot += h.tokens >> ps;
+        }
+        seq[b] = s;
+        p.seqs[b] = s;
+        p.shares[b] = h;
+    }
+    __syncthreads();
+    {
+        const kv_view view{seq, seqs, nullptr};
+        const zest::seq_index index(view, ps, prefix, [&](const kv_seq & s) { return cost_of(a, s, p.cols); });
+        for (int b0 = 0; b0 < seqs; b0 += SHARE_THREADS) {
+            const int b = b0 + t, at = index.before(min(b, seqs - 1));
+            if (b < seqs) p.shares[b].units_before = at;
+        }
+    }
+    if (bad) zest::report(a.b.bad);
+}
+
+// A running maximum, sum and four values of an output, joined with a part's.
+struct joined {
+    float m, l;
+    float4 o;
+    __device__ void add(float m1, float l1, float4 v) {
+        const float now = fmaxf(m, m1), base = now == -INFINITY ? 0.0f : now;
+        const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(m1 - base);
+        m = now;
+        l = l * f + l1 * g;
+        o = make_float4(o.x * f + v.x * g, o.y * f + v.y * g, o.z * f + v.z * g, o.w * f + v.w * g);
+    }
+};
+
+// Every output from what its sequence holds of its own, whole or in attend_few's pieces
+// (few workgroups of it ran), and the parts of what its group shares, in their order: a
+// thread four values.
+template <int D, int NT> __global__ __launch_bounds__(256) void join_shared(attn_args a, attn_args g, const share * shares, int few) {
+    constexpr int COLS = 16 * NT, UNITS = D / 4;
+    extern __shared__ __align__(16) int32_t row0s[];
+    const int seqs = a.view.seqs, heads = a.group * a.c.kv_heads;
+    for (int b = threadIdx.x; b < seqs; b += 256) row0s[b] = a.view.list[b].row0;
+    const kv_seq last_seq = a.view.list[seqs - 1];
+    const share last_share = shares[seqs - 1];
+    __syncthreads();
+    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x, pair = i / UNITS;
+    const int unit = (int) (i - pair * UNITS), head = (int) (pair % heads), row = (int) (pair / heads);
+    if (row >= a.b.rows) return;
+    int lo = 0, hi = seqs;  // the last sequence that begins at or before the row and has rows
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (row0s[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    const kv_seq s = a.view.list[lo];
+    if (row < s.row0 || row >= s.row0 + s.n) return;
+    const share sh = shares[lo];
+    const int h = head / a.group, c = (row - s.row0) * a.group + head - h * a.group;  // the column
+    const int total = zest::seq_index<int, kv_view>::add(last_share.units_before, cost_of(a, last_seq, COLS));
+    const unit_shares units(total, few);
+    const int tiles = col_tiles(a, s, COLS), ct = c / COLS, oc = c - ct * COLS, run = units_of(a, s);
+    const int from = sh.units_before + (h * tiles + ct) * run, to = min(from + run, total);
+    if (from >= to) return;  // (costs that reached the sums' limit end there)
+    const int w0 = units.owner(from), w1 = units.owner(to - 1);
+    joined r;
+    if (w0 == w1) {
+        const int64_t at = (int64_t) row * heads + head;
+        r.o = *reinterpret_cast<const float4 *>(a.own + at * D + unit * 4);
+        const float2 ml = *reinterpret_cast<const float2 *>(a.own + a.b.rows * heads * D + at * 2);
+        r.m = ml.x, r.l = ml.y;
+    } else {
+        r = joined{-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+        for (int w = w0; w <= w1; w++) {
+            const float * x = a.partial + (int64_t) (2 * w + (w == w0)) * partial_floats(COLS, D);
+            r.add(x[COLS * D + oc], x[COLS * D + COLS + oc], *reinterpret_cast<const float4 *>(x + oc * D + unit * 4));
+        }
+    }
+    if (sh.tokens > 0) {
+        // the column of the group, and its place in a part: attend_chunk's registers' order
+        const int gc = (row - sh.group_row0) * a.group + head - h * a.group, tile = sh.group_tile + gc / CHUNK<D>, in = gc % CHUNK<D>;
+        const int lane = (in & 31) + 32 * (unit & 1), dt = unit >> 3, k = unit >> 1 & 3;
+        const float * x = g.chunk_partial + (int64_t) (tile * a.c.kv_heads + h) * g.chunk_splits * CHUNK_PARTIAL<D>;
+        const int64_t o_at = (in & ~31) * D + ((dt * 4 + k) * 64 + lane) * 4;
+        for (int i0 = 0; i0 < g.chunk_splits; i0 += 8) {
+            float m1[8], l1[8];
+            float4 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {  // past the last part, that part again, left out below
+                const float * y = x + (int64_t) min(i0 + e, g.chunk_splits - 1) * CHUNK_PARTIAL<D>;
+                m1[e] = y[CHUNK<D> * D + in];
+                l1[e] = y[CHUNK<D> * (D + 1) + in];
+                v[e] = *reinterpret_cast<const float4 *>(y + o_at);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (i0 + e < g.chunk_splits) r.add(m1[e], l1[e], v[e]);
+        }
+    }
+    const float f = r.l == 0.0f ? 0.0f : 1.0f / r.l;
+    const float v[4] = {r.o.x * f, r.o.y * f, r.o.z * f, r.o.w * f};
+    store4(a, (int64_t) row * a.ldo + (int64_t) head * D + unit * 4, v);
 }
 
 // ---- the host's plan ----------------------------------------------------------------
@@ -1251,6 +1528,93 @@ template <int TYPE> int launch(attn_args & a, int D, const attn_plan & p, hipStr
     }
 }
 
+// What a call with groups launches, by its sizes and bounds alone.
+struct shared_plan {
+    bool plain;             // zest_kv_attn's: nothing to share, or nothing to gain by it
+    int cols, workgroups;   // of attend_few
+    int64_t units, chunk_tiles;
+    int chunk_splits;
+    size_t seqs_at, shares_at, own_at, partial_at, chunk_at, bytes;
+};
+
+// Sequences of so many columns keep the matrix cores busy by themselves, and what is
+// shared is then no longer what bounds them.
+constexpr int64_t MOST_SHARED_COLS = 128;
+
+shared_plan shared_plan_of(const zest_kv_cache * c, const zest_kv_batch * b, const zest_kv_groups * g, int group) {
+    shared_plan p{};
+    const int D = c->head_dim, chunk = chunk_waves(D) * 32;
+    const int64_t most = (int64_t) b->max_new * group, shared = std::min(g->max_shared, b->max_len);
+    p.plain = most > MOST_SHARED_COLS || shared < c->page_tokens || b->seqs < 2;
+    if (p.plain) {
+        p.bytes = plan_of(c, b, group).bytes;
+        return p;
+    }
+    p.cols = most <= 16 ? 16 : 32;
+    const int64_t run = std::max<int64_t>(1, ((int64_t) b->max_len + GROUP + UNIT - 1) / UNIT);
+    const int64_t tiles = std::min<int64_t>((b->rows * group + p.cols - 1) / p.cols + b->seqs, (most + p.cols - 1) / p.cols * b->seqs);
+    p.units = run * tiles * c->kv_heads;
+    p.workgroups = (int) std::min<int64_t>(p.units, CUS);
+    p.chunk_tiles = (b->rows * group + chunk - 1) / chunk + g->groups;
+    // The shared keys in the number of parts that keeps the CUs evenly busy: rounds of
+    // workgroups, one a CU, times a part's steps of 0.65 us, and the parts' traffic.
+    const int64_t items = ((b->rows + g->groups - 1) / g->groups * group + chunk - 1) / chunk * g->groups * c->kv_heads, steps = shared / GROUP + 1;
+    const double part = 8.0 * chunk * D / 6e6;
+    double best = 0;
+    for (int64_t n = 1; n <= 64 && (n == 1 || (n <= steps / 4 && p.chunk_tiles * c->kv_heads * n <= 8 * CUS)); n++) {
+        const double cost = 0.65 * (double) ((items * n + CUS - 1) / CUS) * (double) ((steps + n - 1) / n) + part * items * n;
+        if (n == 1 || cost < best) {
+            best = cost;
+            p.chunk_splits = (int) n;
+        }
+    }
+    const auto take = [&](size_t bytes) {
+        const size_t at = p.bytes;
+        p.bytes += (bytes + 15) & ~(size_t) 15;
+        return at;
+    };
+    take((size_t) g->groups * sizeof(kv_seq));
+    p.seqs_at = take((size_t) b->seqs * sizeof(kv_seq));
+    p.shares_at = take((size_t) b->seqs * sizeof(share));
+    p.own_at = take((size_t) b->rows * group * c->kv_heads * (D + 2) * sizeof(float));
+    p.partial_at = take((size_t) 2 * p.workgroups * partial_floats(p.cols, D) * sizeof(float));
+    p.chunk_at = take((size_t) p.chunk_tiles * c->kv_heads * p.chunk_splits * chunk * (D + 2) * sizeof(float));
+    return p;
+}
+
+template <int TYPE, int D, int NT, bool CHUNKS> int launch_shared(const attn_args & a, const attn_args & g, const shared_plan & p, int groups, hipStream_t s) {
+    constexpr size_t few = NT ? WAVES * RING_B<D> * STEP_BYTES<D> : 0, ring = CHUNKS && CHUNK_RING<D> > few ? CHUNK_RING<D> : few;
+    if (const int st = allow_lds<&shared_kernel<TYPE, D, NT, CHUNKS>>(ring)) return st;
+    hipLaunchKernelGGL((shared_kernel<TYPE, D, NT, CHUNKS>), dim3((unsigned) ((CHUNKS ? g.chunk_blocks * g.chunk_splits : 0) + (NT ? p.workgroups : 0))),
+                       dim3((CHUNKS ? chunk_waves(D) : WAVES) * 64), ring + zest::seq_index_bytes(std::max(a.b.seqs, groups)), s, a, g);
+    return zest::check_launch("zest_kv_attn_shared");
+}
+
+template <int TYPE, int D, int NT> int launch_shared(const attn_args & a, const attn_args & g, const shared_plan & p, const share * shares, int groups, hipStream_t s) {
+    if constexpr (chunk_waves(D) == WAVES) {
+        if (const int st = launch_shared<TYPE, D, NT, true>(a, g, p, groups, s)) return st;
+    } else {
+        if (const int st = launch_shared<TYPE, D, 0, true>(a, g, p, groups, s)) return st;
+        if (const int st = launch_shared<TYPE, D, NT, false>(a, g, p, groups, s)) return st;
+    }
+    const int64_t threads = a.b.rows * a.group * a.c.kv_heads * (D / 4);
+    hipLaunchKernelGGL((join_shared<D, NT>), dim3((unsigned) ((threads + 255) / 256)), dim3(256), (size_t) a.b.seqs * 4, s, a, g, shares, p.workgroups);
+    return zest::check_launch("zest_kv_attn_shared");
+}
+
+template <int TYPE> int launch_shared(const attn_args & a, const attn_args & g, int D, const shared_plan & p, const share * shares, int groups, hipStream_t s) {
+#define ZEST_SHARED(W) \
+    case W: return p.cols == 16 ? launch_shared<TYPE, W, 1>(a, g, p, shares, groups, s) : launch_shared<TYPE, W, 2>(a, g, p, shares, groups, s)
+    switch (D) {
+        ZEST_SHARED(64);
+        ZEST_SHARED(96);
+        ZEST_SHARED(128);
+        ZEST_SHARED(192);
+        default: ZEST_SHARED(256);
+    }
+#undef ZEST_SHARED
+}
+
 // Reports groups whose starts do not fit the batch.
 __global__ __launch_bounds__(256) void groups_kernel(const int32_t * starts, int groups, int seqs, uint32_t * bad) {
     bool odd = false;
@@ -1258,20 +1622,9 @@ __global__ __launch_bounds__(256) void groups_kernel(const int32_t * starts, int
     if (odd) zest::report(bad);
 }
 
-} // namespace
-
-extern "C" {
-
-size_t zest_kv_attn_workspace(const zest_kv_cache * cache, const zest_kv_batch * batch, int32_t q_heads) {
-    if (!cache || !batch || cache->kv_heads <= 0 || q_heads < cache->kv_heads || q_heads % cache->kv_heads) return 0;
-    if (batch->rows <= 0 || batch->seqs <= 0 || batch->max_new <= 0 || batch->max_len < 0) return 0;
-    return plan_of(cache, batch, q_heads / cache->kv_heads).bytes;
-}
-
-int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const void * q, int q_type, int64_t ldq,
-                 int32_t q_heads, float scale, int causal, int32_t window, float softcap, void * out, int out_type, int64_t ldo,
-                 void * workspace, size_t workspace_bytes, uint32_t * bad, void * stream) {
-    const char * me = "zest_kv_attn";
+// The checks of a call's arguments, and the arguments that do not depend on its plan.
+int check_attn(const char * me, const zest_kv_cache * cache, const zest_kv_batch * batch, const void * q, int q_type, int64_t ldq, int32_t q_heads,
+               float scale, int causal, int32_t window, float softcap, void * out, int out_type, int64_t ldo, uint32_t * bad, attn_args & a) {
     if (const int st = zest::kv_check_cache(cache, me)) return st;
     if (const int st = zest::kv_check_batch(cache, batch, me)) return st;
     ZEST_REQUIRE(q_heads > 0 && q_heads <= 4096 && q_heads % cache->kv_heads == 0, "%s: %d query heads for %d k/v heads", me,
@@ -1291,13 +1644,6 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
     ZEST_REQUIRE(zest::kv_rows_apart(q, ldq * qs, width * qs, out, ldo * os, width * os, batch->rows), "%s: out overlaps q", me);
     ZEST_REQUIRE(zest::kv_rows_apart(cache->pool, 0, cache->pages * zest_kv_page_bytes(cache), out, 0, ((batch->rows - 1) * ldo + width) * os, 1),
                  "%s: out overlaps the pool", me);
-    const attn_plan plan = plan_of(cache, batch, q_heads / cache->kv_heads);
-    ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads * std::max(1, plan.chunk_splits) < (1ll << 22), "%s: a batch of %lld units of work",
-                 me, (long long) std::max(plan.units, plan.chunk_tiles));
-    const size_t need = plan.bytes;
-    ZEST_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need,
-                 "%s: workspace of %zu bytes, 16-byte aligned, wanted", me, need);
-    attn_args a{};
     a.c = zest::kv_pages_of(cache);
     a.b = zest::kv_batch_of(batch, bad);
     a.q = q, a.out = out, a.ldq = ldq, a.ldo = ldo;
@@ -1311,6 +1657,20 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
         a.cap2 = softcap * LOG2E;
         a.cap_e = by / softcap * (2.0f * LOG2E);
     }
+    return ZEST_OK;
+}
+
+int attend(const char * me, const zest_kv_cache * cache, const zest_kv_batch * batch, const void * q, int q_type, int64_t ldq, int32_t q_heads,
+           float scale, int causal, int32_t window, float softcap, void * out, int out_type, int64_t ldo, void * workspace,
+           size_t workspace_bytes, uint32_t * bad, void * stream) {
+    attn_args a{};
+    if (const int st = check_attn(me, cache, batch, q, q_type, ldq, q_heads, scale, causal, window, softcap, out, out_type, ldo, bad, a)) return st;
+    const attn_plan plan = plan_of(cache, batch, q_heads / cache->kv_heads);
+    ZEST_REQUIRE(plan.units < (1ll << 31) && plan.chunk_tiles * cache->kv_heads * std::max(1, plan.chunk_splits) < (1ll << 22), "%s: a batch of %lld units of work",
+                 me, (long long) std::max(plan.units, plan.chunk_tiles));
+    const size_t need = plan.bytes;
+    ZEST_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need,
+                 "%s: workspace of %zu bytes, 16-byte aligned, wanted", me, need);
     a.chunk_cols = plan.chunk_cols;
     a.chunk_splits = plan.chunk_splits;
     a.partial = (float *) workspace;
@@ -1320,24 +1680,71 @@ int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const
                                          : launch<ZEST_TYPE_F16>(a, cache->head_dim, plan, s);
 }
 
+} // namespace
+
+extern "C" {
+
+size_t zest_kv_attn_workspace(const zest_kv_cache * cache, const zest_kv_batch * batch, int32_t q_heads) {
+    if (!cache || !batch || cache->kv_heads <= 0 || q_heads < cache->kv_heads || q_heads % cache->kv_heads) return 0;
+    if (batch->rows <= 0 || batch->seqs <= 0 || batch->max_new <= 0 || batch->max_len < 0) return 0;
+    return plan_of(cache, batch, q_heads / cache->kv_heads).bytes;
+}
+
+int zest_kv_attn(const zest_kv_cache * cache, const zest_kv_batch * batch, const void * q, int q_type, int64_t ldq,
+                 int32_t q_heads, float scale, int causal, int32_t window, float softcap, void * out, int out_type, int64_t ldo,
+                 void * workspace, size_t workspace_bytes, uint32_t * bad, void * stream) {
+    return attend("zest_kv_attn", cache, batch, q, q_type, ldq, q_heads, scale, causal, window, softcap, out, out_type, ldo, workspace,
+                  workspace_bytes, bad, stream);
+}
+
 size_t zest_kv_attn_shared_workspace(const zest_kv_cache * cache, const zest_kv_batch * batch, const zest_kv_groups * groups,
                                      int32_t q_heads) {
-    if (!groups || groups->groups <= 0 || groups->max_shared < 0) return 0;
-    return zest_kv_attn_workspace(cache, batch, q_heads);
+    if (!groups || groups->groups <= 0 || groups->max_shared < 0 || !zest_kv_attn_workspace(cache, batch, q_heads)) return 0;
+    if (cache->page_tokens <= 0 || cache->head_dim <= 0) return 0;
+    return shared_plan_of(cache, batch, groups, q_heads / cache->kv_heads).bytes;
 }
 
 int zest_kv_attn_shared(const zest_kv_cache * cache, const zest_kv_batch * batch, const zest_kv_groups * groups, const void * q, int q_type,
                         int64_t ldq, int32_t q_heads, float scale, int causal, int32_t window, float softcap, void * out, int out_type,
                         int64_t ldo, void * workspace, size_t workspace_bytes, uint32_t * bad, void * stream) {
     const char * me = "zest_kv_attn_shared";
+    attn_args a{};
+    if (const int st = check_attn(me, cache, batch, q, q_type, ldq, q_heads, scale, causal, window, softcap, out, out_type, ldo, bad, a)) return st;
     ZEST_REQUIRE(groups && groups->starts && (reinterpret_cast<uintptr_t>(groups->starts) & 3) == 0, "%s: null or misaligned groups", me);
-    ZEST_REQUIRE(groups->groups > 0 && groups->groups <= zest::KV_MAX_SEQS && groups->max_shared >= 0 && groups->max_shared <= (1 << 30),
+    ZEST_REQUIRE(groups->groups > 0 && groups->groups <= MAX_GROUPS && groups->max_shared >= 0 && groups->max_shared <= (1 << 30),
                  "%s: groups=%d max_shared=%d", me, groups->groups, groups->max_shared);
-    if (const int st = zest_kv_attn(cache, batch, q, q_type, ldq, q_heads, scale, causal, window, softcap, out, out_type, ldo, workspace,
-                                    workspace_bytes, bad, stream))
-        return st;
-    hipLaunchKernelGGL(groups_kernel, dim3(1), dim3(256), 0, zest::as_stream(stream), groups->starts, groups->groups, batch->seqs, bad);
-    return zest::check_launch(me);
+    ZEST_REQUIRE((int64_t) batch->table_rows * batch->table_cols < (1ll << 31), "%s: tables of %d x %d", me, batch->table_rows, batch->table_cols);
+    const hipStream_t s = zest::as_stream(stream);
+    const shared_plan p = shared_plan_of(cache, batch, groups, a.group);
+    if (p.plain) {
+        if (const int st = attend(me, cache, batch, q, q_type, ldq, q_heads, scale, causal, window, softcap, out, out_type, ldo, workspace,
+                                  workspace_bytes, bad, stream))
+            return st;
+        hipLaunchKernelGGL(groups_kernel, dim3(1), dim3(256), 0, s, groups->starts, groups->groups, batch->seqs, bad);
+        return zest::check_launch(me);
+    }
+    const int64_t threads = batch->rows * q_heads * (int64_t) (cache->head_dim / 4);
+    ZEST_REQUIRE(p.units < (1ll << 31) && p.chunk_tiles * cache->kv_heads * p.chunk_splits < (1ll << 22) && threads < (1ll << 38), "%s: a batch of %lld units of work", me,
+                 (long long) std::max(p.units, p.chunk_tiles));
+    ZEST_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= p.bytes, "%s: workspace of %zu bytes, 16-byte aligned, wanted",
+                 me, p.bytes);
+    uint8_t * const ws = (uint8_t *) workspace;
+    a.chunk_cols = 0x7fffffff;
+    a.partial = (float *) (ws + p.partial_at);
+    a.own = (float *) (ws + p.own_at);
+    a.view = kv_view{(const kv_seq *) (ws + p.seqs_at), batch->seqs, bad};
+    attn_args g = a;
+    g.causal = g.window = g.chunk_cols = 0;
+    g.view = kv_view{(const kv_seq *) ws, groups->groups, bad};
+    g.chunk_blocks = (int32_t) (p.chunk_tiles * cache->kv_heads);
+    g.chunk_splits = p.chunk_splits;
+    g.chunk_partial = (float *) (ws + p.chunk_at);
+    share_args look{a, groups->starts, groups->groups, groups->max_shared, chunk_waves(cache->head_dim) * 32, p.cols, (kv_seq *) (ws + p.seqs_at), (kv_seq *) ws,
+                    (share *) (ws + p.shares_at)};
+    if (const int st = allow_lds<&share_kernel>(share_lds(zest::KV_MAX_SEQS, MAX_GROUPS) - zest::seq_index_bytes(zest::KV_MAX_SEQS))) return st;
+    hipLaunchKernelGGL(share_kernel, dim3(1), dim3(SHARE_THREADS), share_lds(batch->seqs, groups->groups), s, look);
+    return cache->type == ZEST_TYPE_BF16 ? launch_shared<ZEST_TYPE_BF16>(a, g, cache->head_dim, p, look.shares, groups->groups, s)
+                                         : launch_shared<ZEST_TYPE_F16>(a, g, cache->head_dim, p, look.shares, groups->groups, s);
 }
 
 } // extern "C"

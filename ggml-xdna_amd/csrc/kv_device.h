@@ -50,20 +50,32 @@ __device__ inline kv_seq load_seq(const kv_batch & a, int b, int page_shift, boo
     return s;
 }
 
+// Sequences that a kernel before has looked at: checked, and each with its own place
+// in the tables (slot is the number of its first entry there).
+struct kv_view {
+    const kv_seq * list;
+    int32_t seqs;
+    uint32_t * bad;
+};
+
+__device__ inline kv_seq load_seq(const kv_view & a, int b, int, bool &) { return a.list[b]; }
+
+__device__ inline const int32_t * table_of(const kv_batch & a, const kv_seq & s) { return a.tables + (int64_t) s.slot * a.table_cols; }
+
 // Where the sequences' runs of work lie: the sum of a cost over the sequences,
 // and the sequence that holds a unit of it. Up to 64 sequences every wave keeps
 // one a lane and finds them by a scan and a ballot, with no shared memory and no
 // barrier (a call of few sequences is bound by such latencies); more go through
 // prefix sums in shared memory (prefix[seqs + 1], whose barriers every thread of
 // the workgroup reaches: threads a multiple of 64, at most 1024).
-template <typename Cost> struct seq_index {
-    const kv_batch & a;
+template <typename Cost, typename Batch> struct seq_index {
+    const Batch & a;
     const int page_shift;
     int32_t * const prefix;
     kv_seq mine;
     int32_t incl, total;
 
-    __device__ seq_index(const kv_batch & a, int page_shift, int32_t * prefix, Cost cost) : a(a), page_shift(page_shift), prefix(prefix) {
+    __device__ seq_index(const Batch & a, int page_shift, int32_t * prefix, Cost cost) : a(a), page_shift(page_shift), prefix(prefix) {
         const int lane = threadIdx.x & 63;
         bool bad = false;
         if (a.seqs <= 64) {
@@ -93,6 +105,14 @@ template <typename Cost> struct seq_index {
             total = prefix[a.seqs];
         }
         if (bad && blockIdx.x == 0) report(a.bad);
+    }
+
+    // The units before sequence b, which need not be the same in every lane (every lane
+    // calls it).
+    __device__ int32_t before(int b) const {
+        if (a.seqs > 64) return prefix[b];
+        const int32_t upto = __shfl(incl, max(b - 1, 0));
+        return b ? upto : 0;
     }
 
     // Sums stop at the type's limit: starts that go back make sequences overlap, and

@@ -137,15 +137,15 @@ ZEST_API int zest_kv_attn(const zest_kv_cache *cache, const zest_kv_batch *batch
  * batch are such a group. */
 typedef struct {
     const int32_t *starts; /* [groups + 1], device */
-    int32_t groups;        /* 1 .. 4096 */
+    int32_t groups;        /* 1 .. 2048 */
     int32_t max_shared;    /* 0 .. 2^30 */
 } zest_kv_groups;
 
 /* zest_kv_attn where the batch's sequences come in groups: the same result but for
  * the order in which its sums are rounded, what a group shares being read once for
  * all its rows and joined with what each sequence holds of its own. Arguments and
- * limits as zest_kv_attn's; a group's starts outside 0 .. seqs, or going back, are
- * reported, and that group shares nothing. table_rows * table_cols < 2^31. The
+ * limits as zest_kv_attn's; groups' starts outside 0 .. seqs, or going back, are
+ * reported, and no group shares anything then. table_rows * table_cols < 2^31. The
  * workspace is zest_kv_attn_shared_workspace's. */
 ZEST_API size_t zest_kv_attn_shared_workspace(const zest_kv_cache *cache, const zest_kv_batch *batch,
                                               const zest_kv_groups *groups, int32_t q_heads);
