@@ -1151,20 +1151,20 @@ __global__ __launch_bounds__((CHUNKS ? chunk_waves(D) : WAVES) * 64, D > 192 || 
     if constexpr (NT > 0) attend_few<TYPE, D, NT, false>(a, blockIdx.x, few, smem);
 }
 
-// The same over shared leading pages: few columns of what each sequence holds of its
-// own (a), chunks of what groups share (g).
+// The same over shared leading pages: chunks of what groups share (g), few columns of
+// what each sequence holds of its own (a).
 template <int TYPE, int D, int NT, bool CHUNKS>
 __global__ __launch_bounds__((CHUNKS ? chunk_waves(D) : WAVES) * 64, D > 192 || (D > 128 && !CHUNKS) ? 1 : 2) void shared_kernel(attn_args a, attn_args g) {
     static_assert(!CHUNKS || NT == 0 || chunk_waves(D) == WAVES, "workgroups of one size");
     extern __shared__ __align__(1024) uint8_t smem[];
-    const int few = gridDim.x - (CHUNKS ? g.chunk_blocks * g.chunk_splits : 0);
+    const int chunks = CHUNKS ? g.chunk_blocks * g.chunk_splits : 0;  // first, as they last longest
     if constexpr (CHUNKS)
-        if ((int) blockIdx.x >= few) {
-            const int at = blockIdx.x - few, split = at / g.chunk_blocks;
-            attend_chunk<TYPE, D, true>(g, at - split * g.chunk_blocks, split, smem);
+        if ((int) blockIdx.x < chunks) {
+            const int split = blockIdx.x / g.chunk_blocks;
+            attend_chunk<TYPE, D, true>(g, blockIdx.x - split * g.chunk_blocks, split, smem);
             return;
         }
-    if constexpr (NT > 0) attend_few<TYPE, D, NT, true>(a, blockIdx.x, few, smem);
+    if constexpr (NT > 0) attend_few<TYPE, D, NT, true>(a, blockIdx.x - chunks, gridDim.x - chunks, smem);
 }
 
 template <int D, int NT, bool CHUNKS> __global__ __launch_bounds__(256) void combine_kernel(attn_args a) {
@@ -1345,75 +1345,121 @@ struct joined {
         l = l * f + l1 * g;
         o = make_float4(o.x * f + v.x * g, o.y * f + v.y * g, o.z * f + v.z * g, o.w * f + v.w * g);
     }
+    struct four {
+        float v[4];
+    };
+    __device__ four mean() const {
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        return {{o.x * f, o.y * f, o.z * f, o.w * f}};
+    }
 };
 
-// Every output from what its sequence holds of its own, whole or in attend_few's pieces
-// (few workgroups of it ran), and the parts of what its group shares, in their order: a
-// thread four values.
-template <int D, int NT> __global__ __launch_bounds__(256) void join_shared(attn_args a, attn_args g, const share * shares, int few) {
-    constexpr int COLS = 16 * NT, UNITS = D / 4;
-    extern __shared__ __align__(16) int32_t row0s[];
-    const int seqs = a.view.seqs, heads = a.group * a.c.kv_heads;
-    for (int b = threadIdx.x; b < seqs; b += 256) row0s[b] = a.view.list[b].row0;
-    const kv_seq last_seq = a.view.list[seqs - 1];
-    const share last_share = shares[seqs - 1];
-    __syncthreads();
-    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x, pair = i / UNITS;
-    const int unit = (int) (i - pair * UNITS), head = (int) (pair % heads), row = (int) (pair / heads);
-    if (row >= a.b.rows) return;
-    int lo = 0, hi = seqs;  // the last sequence that begins at or before the row and has rows
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (row0s[mid] <= row) lo = mid;
-        else hi = mid;
+// Where the join finds what a column's sequence holds of its own: whole in a.own, or
+// in attend_few's pieces.
+template <int D, int NT> struct own_part {
+    static constexpr int COLS = 16 * NT;
+    const attn_args & a;
+    int64_t pair;        // row and query head
+    int w0, w1, oc;      // workgroups of attend_few, the column of its tile
+    bool any;
+
+    __device__ own_part(const attn_args & a, const kv_seq & s, const share & sh, const unit_shares & units, int total, int row, int head)
+        : a(a), pair((int64_t) row * (a.group * a.c.kv_heads) + head) {
+        const int h = head / a.group, c = (row - s.row0) * a.group + head - h * a.group;
+        const int tiles = col_tiles(a, s, COLS), ct = c / COLS, run = units_of(a, s);
+        const int from = sh.units_before + (h * tiles + ct) * run, to = min(from + run, total);
+        oc = c - ct * COLS;
+        any = from < to;  // (costs that reached the sums' limit end there)
+        w0 = units.owner(from);
+        w1 = any ? units.owner(to - 1) : w0;
     }
-    const kv_seq s = a.view.list[lo];
-    if (row < s.row0 || row >= s.row0 + s.n) return;
-    const share sh = shares[lo];
-    const int h = head / a.group, c = (row - s.row0) * a.group + head - h * a.group;  // the column
-    const int total = zest::seq_index<int, kv_view>::add(last_share.units_before, cost_of(a, last_seq, COLS));
-    const unit_shares units(total, few);
-    const int tiles = col_tiles(a, s, COLS), ct = c / COLS, oc = c - ct * COLS, run = units_of(a, s);
-    const int from = sh.units_before + (h * tiles + ct) * run, to = min(from + run, total);
-    if (from >= to) return;  // (costs that reached the sums' limit end there)
-    const int w0 = units.owner(from), w1 = units.owner(to - 1);
-    joined r;
-    if (w0 == w1) {
-        const int64_t at = (int64_t) row * heads + head;
-        r.o = *reinterpret_cast<const float4 *>(a.own + at * D + unit * 4);
-        const float2 ml = *reinterpret_cast<const float2 *>(a.own + a.b.rows * heads * D + at * 2);
-        r.m = ml.x, r.l = ml.y;
-    } else {
-        r = joined{-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    __device__ void add_to(joined & r, int unit) const {
+        if (w0 == w1) {
+            const float2 ml = *reinterpret_cast<const float2 *>(a.own + a.b.rows * (a.group * a.c.kv_heads) * D + pair * 2);
+            r.add(ml.x, ml.y, *reinterpret_cast<const float4 *>(a.own + pair * D + unit * 4));
+            return;
+        }
         for (int w = w0; w <= w1; w++) {
             const float * x = a.partial + (int64_t) (2 * w + (w == w0)) * partial_floats(COLS, D);
             r.add(x[COLS * D + oc], x[COLS * D + COLS + oc], *reinterpret_cast<const float4 *>(x + oc * D + unit * 4));
         }
     }
-    if (sh.tokens > 0) {
-        // the column of the group, and its place in a part: attend_chunk's registers' order
-        const int gc = (row - sh.group_row0) * a.group + head - h * a.group, tile = sh.group_tile + gc / CHUNK<D>, in = gc % CHUNK<D>;
-        const int lane = (in & 31) + 32 * (unit & 1), dt = unit >> 3, k = unit >> 1 & 3;
-        const float * x = g.chunk_partial + (int64_t) (tile * a.c.kv_heads + h) * g.chunk_splits * CHUNK_PARTIAL<D>;
-        const int64_t o_at = (in & ~31) * D + ((dt * 4 + k) * 64 + lane) * 4;
-        for (int i0 = 0; i0 < g.chunk_splits; i0 += 8) {
-            float m1[8], l1[8];
-            float4 v[8];
+};
+
+// Every output, four values a thread: of rows whose sequence shares, a workgroup takes 32
+// columns of a group and 32 of their values and joins the parts of what the group
+// shares, in their order, in the order attend_chunk left them, so that a wave's loads
+// are whole kilobytes, and what the sequence holds of its own (few workgroups of
+// attend_few ran); the other rows follow.
+template <int D, int NT> __global__ __launch_bounds__(256) void join_shared(attn_args a, attn_args g, const share * shares, int few) {
+    constexpr int COLS = 16 * NT, UNITS = D / 4, PARTS = CHUNK<D> / 32, AT_ONCE = 8;
+    extern __shared__ __align__(16) int32_t attn_sh[];
+    const int seqs = a.view.seqs, heads = a.group * a.c.kv_heads;
+    int32_t * const row0s = attn_sh;
+    for (int b = threadIdx.x; b < seqs; b += 256) row0s[b] = a.view.list[b].row0;
+    const kv_seq last_seq = a.view.list[seqs - 1];
+    const int total = zest::seq_index<int, kv_view>::add(shares[seqs - 1].units_before, cost_of(a, last_seq, COLS));
+    const unit_shares units(total, few);
+    auto sequence_of = [&](int row) {  // the last that begins at or before the row
+        int lo = 0, hi = seqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (row0s[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    const int shared_blocks = g.chunk_blocks * PARTS * (D / 32);
+    if ((int) blockIdx.x < shared_blocks) {
+        const zest::seq_index index(g.view, a.c.page_shift, attn_sh + ((seqs + 3) & ~3), [&](const kv_seq & s) { return chunk_tiles_of(g, s, CHUNK<D>); });
+        __syncthreads();
+        const int dt = blockIdx.x % (D / 32), rest = blockIdx.x / (D / 32), part = rest % PARTS, at = rest / PARTS, h = at % a.c.kv_heads, tile = at / a.c.kv_heads;
+        if (tile >= index.total) return;
+        int32_t before;
+        const kv_seq group = index.at(tile, before);
+        const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, k = threadIdx.x >> 6, unit = dt * 8 + 2 * k + half;
+        const int in = part * 32 + col, gc = (tile - before) * CHUNK<D> + in;
+        if (gc >= group.n * a.group) return;
+        const float * x = g.chunk_partial + (int64_t) at * g.chunk_splits * CHUNK_PARTIAL<D>;
+        const int row = group.row0 + gc / a.group, head = h * a.group + gc % a.group, lo = sequence_of(row);
+        const kv_seq s = a.view.list[lo];
+        const share sh = shares[lo];
+        joined r{-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+        for (int i0 = 0; i0 < g.chunk_splits; i0 += AT_ONCE) {
+            float m1[AT_ONCE], l1[AT_ONCE];
+            float4 v[AT_ONCE];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {  // past the last part, that part again, left out below
+            for (int e = 0; e < AT_ONCE; e++) {  // past the last part, that part again, left out below
                 const float * y = x + (int64_t) min(i0 + e, g.chunk_splits - 1) * CHUNK_PARTIAL<D>;
                 m1[e] = y[CHUNK<D> * D + in];
                 l1[e] = y[CHUNK<D> * (D + 1) + in];
-                v[e] = *reinterpret_cast<const float4 *>(y + o_at);
+                v[e] = *reinterpret_cast<const float4 *>(y + part * 32 * D + ((dt * 4 + k) * 64 + lane) * 4);
             }
 #pragma unroll
-            for (int e = 0; e < 8; e++)
+            for (int e = 0; e < AT_ONCE; e++)
                 if (i0 + e < g.chunk_splits) r.add(m1[e], l1[e], v[e]);
         }
+        // (a row between the members' that none of them has is not written)
+        if (row < s.row0 || row >= s.row0 + s.n || sh.tokens == 0) return;
+        const own_part<D, NT> own(a, s, sh, units, total, row, head);
+        if (!own.any) return;
+        own.add_to(r, unit);
+        store4(a, (int64_t) row * a.ldo + (int64_t) head * D + unit * 4, r.mean().v);
+        return;
     }
-    const float f = r.l == 0.0f ? 0.0f : 1.0f / r.l;
-    const float v[4] = {r.o.x * f, r.o.y * f, r.o.z * f, r.o.w * f};
-    store4(a, (int64_t) row * a.ldo + (int64_t) head * D + unit * 4, v);
+    __syncthreads();
+    const int64_t i = (int64_t) (blockIdx.x - shared_blocks) * 256 + threadIdx.x, pair = i / UNITS;
+    const int unit = (int) (i - pair * UNITS), head = (int) (pair % heads), row = (int) (pair / heads);
+    if (row >= a.b.rows) return;
+    const int lo = sequence_of(row);
+    const share sh = shares[lo];
+    const kv_seq s = a.view.list[lo];
+    if (row < s.row0 || row >= s.row0 + s.n || sh.tokens > 0) return;
+    const own_part<D, NT> own(a, s, sh, units, total, row, head);
+    if (!own.any) return;
+    joined r{-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    own.add_to(r, unit);
+    store4(a, (int64_t) row * a.ldo + (int64_t) head * D + unit * 4, r.mean().v);
 }
 
 // ---- the host's plan ----------------------------------------------------------------
@@ -1554,15 +1600,20 @@ shared_plan shared_plan_of(const zest_kv_cache * c, const zest_kv_batch * b, con
     const int64_t run = std::max<int64_t>(1, ((int64_t) b->max_len + GROUP + UNIT - 1) / UNIT);
     const int64_t tiles = std::min<int64_t>((b->rows * group + p.cols - 1) / p.cols + b->seqs, (most + p.cols - 1) / p.cols * b->seqs);
     p.units = run * tiles * c->kv_heads;
-    p.workgroups = (int) std::min<int64_t>(p.units, CUS);
+    p.workgroups = (int) std::min<int64_t>(p.units, 2 * CUS);
     p.chunk_tiles = (b->rows * group + chunk - 1) / chunk + g->groups;
-    // The shared keys in the number of parts that keeps the CUs evenly busy: rounds of
-    // workgroups, one a CU, times a part's steps of 0.65 us, and the parts' traffic.
+    // The shared keys in the number of parts that keeps the CUs evenly busy. A step of a
+    // workgroup alone on its CU takes 1.05 us, one of two that share a CU 1.2 (16 samples
+    // of 32000 tokens, 32 tiles of 1000 steps: 8 parts 133 us, 16 parts 94; deeper rings
+    // for one workgroup a CU do not change its step). A part is written and read again, 20
+    // bytes' worth of a copy a value (64 samples of 8192 tokens: 32 parts 43.8 us with the
+    // join, 16 parts 38.4).
     const int64_t items = ((b->rows + g->groups - 1) / g->groups * group + chunk - 1) / chunk * g->groups * c->kv_heads, steps = shared / GROUP + 1;
-    const double part = 8.0 * chunk * D / 6e6;
+    const int64_t slots = (D <= 128 ? 2 : 1) * CUS;
+    const double part = 20.0 * chunk * D / 6e6;
     double best = 0;
-    for (int64_t n = 1; n <= 64 && (n == 1 || (n <= steps / 4 && p.chunk_tiles * c->kv_heads * n <= 8 * CUS)); n++) {
-        const double cost = 0.65 * (double) ((items * n + CUS - 1) / CUS) * (double) ((steps + n - 1) / n) + part * items * n;
+    for (int64_t n = 1; n <= 64 && (n == 1 || (n <= steps / 4 && p.chunk_tiles * c->kv_heads * n <= 4 * slots)); n++) {
+        const double cost = (items * n <= CUS ? 1.05 : 1.2 * (double) ((items * n + slots - 1) / slots)) * (double) ((steps + n - 1) / n) + part * items * n;
         if (n == 1 || cost < best) {
             best = cost;
             p.chunk_splits = (int) n;
@@ -1598,7 +1649,9 @@ template <int TYPE, int D, int NT> int launch_shared(const attn_args & a, const 
         if (const int st = launch_shared<TYPE, D, NT, false>(a, g, p, groups, s)) return st;
     }
     const int64_t threads = a.b.rows * a.group * a.c.kv_heads * (D / 4);
-    hipLaunchKernelGGL((join_shared<D, NT>), dim3((unsigned) ((threads + 255) / 256)), dim3(256), (size_t) a.b.seqs * 4, s, a, g, shares, p.workgroups);
+    const int64_t blocks = (int64_t) g.chunk_blocks * (CHUNK<D> / 32) * (D / 32) + (threads + 255) / 256;
+    hipLaunchKernelGGL((join_shared<D, NT>), dim3((unsigned) blocks), dim3(256), (size_t) ((a.b.seqs + 3) & ~3) * 4 + zest::seq_index_bytes(groups), s, a, g, shares,
+                       p.workgroups);
     return zest::check_launch("zest_kv_attn_shared");
 }
 
