@@ -4,7 +4,17 @@
 // by a 32-bit key, and a weight exp((x - max) / T) is computed in 64 bits and
 // rounded to a whole number of 2^-45, so that 2^18 of them sum without a rounding
 // or an overflow in 64 bits, in any order. What top-k and top-p keep is a cut: all
-// logits above a key and the first few, by index, of those equal to it.
+// logits above a key and those equal to it up to an index. It is found by radix
+// selection, of counts or of weights: a histogram of eight bits of the key at a
+// time among what agrees so far.
+//
+// Rows of up to 16384 logits are one workgroup's, which holds them in registers.
+// Longer ones are cut in parts of 4096, a workgroup each, and the call is HBM bound by
+// one reading (the next ones come from the last-level cache): stats_kernel finds the
+// parts' largest logits, weigh_kernel the parts' weights, or a histogram of them by
+// distance from the largest, and collect_kernel, where a row has a top-k or a top-p, the
+// few logits among which its cut lies. The last workgroup of a row to finish goes on
+// with the row; the tickets that tell it are cleared by the kernel before.
 #include <algorithm>
 
 #include "zest/decode.h"
@@ -12,21 +22,42 @@
 
 namespace {
 
-typedef __bf16 bf16_t;
 typedef unsigned long long u64;
 
 constexpr double ONE = 35184372088832.0;  // 2^45: the largest weight
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
+constexpr int PART = 4096, THREADS = 256, MAX_PARTS = ZEST_SAMPLE_MAX_VOCAB / PART;
+constexpr int BINS = 512, LIST = 4096;    // of a row's histogram; logits that collect_kernel holds
+constexpr int BATCH = 256;                // rows that a workspace is for: more go in several launches
+constexpr int SHORT = 2048, MIDDLE = 16384;  // longest rows of the two sizes of row_kernel
+
+// What a row's workgroups leave each other.
+struct row_state {
+    u64 top[MAX_PARTS];      // the largest key, then ~index of its first place
+    uint32_t low[MAX_PARTS]; // the smallest key above -infinity's (none: 2^32 - 1)
+    u64 mass[MAX_PARTS];
+    u64 goal;                // of weights, within the bins that are listed
+    uint32_t tickets[2], listed;
+    int32_t from, to, mode;  // the bins that are listed
+    u64 list[LIST];          // keys and indices
+};
+enum { DONE, KEEP_K, KEEP_P, SLOW };
+
+struct bin {
+    u64 mass;
+    uint32_t count, unused;
+};
 
 struct sample_args {
     const void * logits;
     int64_t ld;
-    int32_t type, vocab;
+    int32_t type, vocab, parts;
     const float * u, * temperature;
     const int32_t * top_k;
     const float * top_p, * min_p;
     int32_t * token;
     float * prob;
+    row_state * rows;
+    bin * bins;              // [row][part][BINS]
 };
 
 // Keys order as the values do; NaN below all, -0 as 0.
@@ -40,13 +71,35 @@ constexpr uint32_t KEY_MINUS_INF = 0x007fffffu;
 __device__ inline float logit(const sample_args & a, int64_t row, int i) {
     const int64_t at = row * a.ld + i;
     if (a.type == ZEST_TYPE_F32) return ((const float *) a.logits)[at];
-    if (a.type == ZEST_TYPE_BF16) return (float) ((const bf16_t *) a.logits)[at];
+    if (a.type == ZEST_TYPE_BF16) return (float) ((const __bf16 *) a.logits)[at];
     return (float) ((const _Float16 *) a.logits)[at];
+}
+
+// Four logits from index i on, of which those from `end` on are NaN (never taken).
+__device__ inline void logits4(const sample_args & a, int64_t row, int i, int end, float x[4]) {
+    if (i + 4 <= end) {
+        const int64_t at = row * a.ld + i;
+        if (a.type == ZEST_TYPE_F32) {  // (rows need not be aligned to the load)
+            float4 v;
+            __builtin_memcpy(&v, (const float *) a.logits + at, 16);
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        } else {
+            uint2 v;
+            __builtin_memcpy(&v, (const uint16_t *) a.logits + at, 8);
+            const uint32_t w[4] = {v.x & 0xffffu, v.x >> 16, v.y & 0xffffu, v.y >> 16};
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = a.type == ZEST_TYPE_BF16 ? __uint_as_float(w[e] << 16) : (float) __builtin_bit_cast(_Float16, (uint16_t) w[e]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = i + e < end ? logit(a, row, i + e) : NAN;
 }
 
 // A row's parameters, as the definition reads them.
 struct params {
-    double scale, p, m, u;  // p 1, m 0: off
+    double scale, p, m, u;  // scale in powers of two; p 1, m 0: off
+    float width;            // logits further than this below the largest have no weight
     int k;                  // vocab: off
     bool greedy;
 };
@@ -55,7 +108,8 @@ __device__ inline params params_of(const sample_args & a, int64_t row) {
     params r;
     const float t = a.temperature ? a.temperature[row] : 1.0f;
     r.greedy = !(t > 0.0f);
-    r.scale = 1.0 / (double) t;
+    r.scale = 1.4426950408889634074 / (double) t;
+    r.width = 32.0f * t;
     const float p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
     r.p = p < 1.0f ? fmax((double) p, 0.0) : 1.0;  // (a NaN is off)
     r.m = m > 0.0f ? fmin((double) m, 1.0) : 0.0;
@@ -65,136 +119,180 @@ __device__ inline params params_of(const sample_args & a, int64_t row) {
     return r;
 }
 
-// A logit's weight relative to the largest, and as an integer.
+// A logit's weight relative to the largest: 2^y by the series of e^(f ln 2) for the
+// part of y within half a unit (to its 12th power: off by 2^-52 at most).
 __device__ inline double weight_of(float x, float top, double scale) {
     if (x == top) return 1.0;
-    return x > -INFINITY && top < INFINITY ? exp(((double) x - (double) top) * scale) : 0.0;  // (a NaN: 0)
+    if (!(x > -INFINITY) || top == INFINITY) return 0.0;  // (a NaN: 0)
+    const double y = ((double) x - (double) top) * scale;
+    if (y < -60.0) return 0.0;
+    const double n = __builtin_rint(y), f = (y - n) * 0.69314718055994530942;
+    double s = 1.0 / 479001600.0;
+    s = fma(s, f, 1.0 / 39916800.0);
+    s = fma(s, f, 1.0 / 3628800.0);
+    s = fma(s, f, 1.0 / 362880.0);
+    s = fma(s, f, 1.0 / 40320.0);
+    s = fma(s, f, 1.0 / 5040.0);
+    s = fma(s, f, 1.0 / 720.0);
+    s = fma(s, f, 1.0 / 120.0);
+    s = fma(s, f, 1.0 / 24.0);
+    s = fma(s, f, 1.0 / 6.0);
+    s = fma(s, f, 0.5);
+    s = fma(s, f, 1.0);
+    s = fma(s, f, 1.0);
+    return __builtin_ldexp(s, (int) n);
 }
 __device__ inline u64 whole(double w) { return (u64) __builtin_rint(w * ONE); }
 
-// ---- one workgroup a row -----------------------------------------------------------
+// ---- sums over a workgroup -----------------------------------------------------------
 
-__device__ inline u64 wave_sum(u64 v) {
+template <int N> struct group_memory {
+    u64 wave[N / 64];
+    u64 mass[256];
+    uint32_t count[256];
+    u64 found, one;
+    uint32_t digit;
+    int32_t index;
+};
+
+template <typename V> __device__ inline V wave_sum(V v) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
     return v;
 }
 
-struct shared_row {
-    u64 wave[WAVES];
-    u64 mass[256];
-    uint32_t count[256];
-    u64 found;
-    uint32_t key;
-};
-
-// The sum over the workgroup, in every thread.
-__device__ inline u64 group_sum(shared_row & sh, u64 v) {
+// The sum, in every thread; and the largest.
+template <int N> __device__ inline u64 group_sum(group_memory<N> & sh, u64 v) {
     v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = v;
     __syncthreads();
     u64 sum = 0;
-    for (int w = 0; w < WAVES; w++) sum += sh.wave[w];
+#pragma unroll
+    for (int w = 0; w < N / 64; w++) sum += sh.wave[w];
     return sum;
+}
+template <int N> __device__ inline u64 group_max(group_memory<N> & sh, u64 v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = max(v, (u64) __shfl_xor(v, off));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < N / 64; w++) v = max(v, sh.wave[w]);
+    return v;
+}
+
+__device__ inline u64 wave_upto(u64 v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const u64 left = __shfl_up(v, off);
+        if (lane >= off) v += left;
+    }
+    return v;
 }
 
 // What the threads before this one hold, and the workgroup's sum.
-__device__ inline u64 group_before(shared_row & sh, u64 v, u64 & sum) {
+template <int N> __device__ inline u64 group_before(group_memory<N> & sh, u64 v, u64 & sum) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    u64 incl = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const u64 left = __shfl_up(incl, off);
-        if (lane >= off) incl += left;
-    }
+    const u64 incl = wave_upto(v);
     __syncthreads();
     if (lane == 63) sh.wave[wave] = incl;
     __syncthreads();
     u64 before = incl - v;
     sum = 0;
-    for (int w = 0; w < WAVES; w++) {
+#pragma unroll
+    for (int w = 0; w < N / 64; w++) {
         if (w < wave) before += sh.wave[w];
         sum += sh.wave[w];
     }
     return before;
 }
 
-// Logits with a key above `key`, and the first `ties` with that key.
+// Logits with a key above `key`, and those with that key up to `index`.
 struct cut {
-    uint32_t key, ties;
+    uint32_t key;
+    int32_t index;
+    __device__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= index); }
 };
+constexpr cut EVERYTHING = {0, 0x7fffffff};
 
-// The cut behind which a running sum, from the largest logit on, reaches `goal`:
-// of counts (MASS false) or weights, over the logits above `in`. Eight bits of the
-// key at a time, from the top: a histogram of the logits that agree so far.
-template <bool MASS>
-__device__ cut find_cut(shared_row & sh, const sample_args & a, int64_t row, float top, double scale, cut in, double goal) {
+// The cut behind which a running sum, from the largest logit on, first reaches `goal`
+// (above 0): of counts, or of weights. `each` calls its argument with the key, the index
+// and the weight of every logit that may be kept, the threads' in the order of their
+// indices; ties go by index: `ties` finds the place of the r-th logit of a key.
+template <bool MASS, int N, typename Each, typename Nth> __device__ cut find_cut(group_memory<N> & sh, u64 goal, Each each, Nth nth) {
     uint32_t prefix = 0;
-    u64 above = 0;  // sum over the keys above the prefix's
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
-        for (int i = threadIdx.x; i < 256; i += THREADS) {
+        for (int i = threadIdx.x; i < 256; i += N) {
             sh.mass[i] = 0;
             sh.count[i] = 0;
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < a.vocab; i += THREADS) {
-            const float x = logit(a, row, i);
-            const uint32_t k = key_of(x);
-            if (k < in.key || (shift < 24 && (k >> (shift + 8)) != prefix >> (shift + 8))) continue;
-            atomicAdd(&sh.count[k >> shift & 255], 1u);
-            if (MASS && k != in.key) atomicAdd(&sh.mass[k >> shift & 255], whole(weight_of(x, top, scale)));
-        }
+        each([&](uint32_t k, int, u64 w) {
+            if (shift < 24 && (k ^ prefix) >> (shift + 8)) return;
+            if (MASS) atomicAdd(&sh.mass[k >> shift & 255], w);
+            else atomicAdd(&sh.count[k >> shift & 255], 1u);
+        });
         __syncthreads();
-        // ties at `in` count as far as it keeps them
-        if (MASS && threadIdx.x == 0 && (shift == 24 || (in.key >> (shift + 8)) == prefix >> (shift + 8)) && in.key > KEY_MINUS_INF)
-            sh.mass[in.key >> shift & 255] += in.ties * whole(weight_of(value_of(in.key), top, scale));
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int d = 255;
-            for (; d > 0; d--) {
-                const u64 here = MASS ? sh.mass[d] : sh.count[d];
-                if ((double) (above + here) >= goal) break;
-                above += here;
+        if (threadIdx.x < 64) {  // four digits a lane, from the largest
+            u64 here[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int d = 255 - 4 * (int) threadIdx.x - i;
+                here[i] = MASS ? sh.mass[d] : sh.count[d];
+                sum += here[i];
             }
-            // (where no sum reaches it the last digit with anything stays)
-            sh.found = above;
-            sh.key = prefix | (uint32_t) d << shift;
+            const u64 upto = wave_upto(sum), all = __shfl(upto, 63);
+            goal = min(goal, all);  // (a product of the total may be rounded past it)
+            const bool reached = upto >= goal;
+            if (reached && upto - sum < goal) {
+                u64 above = upto - sum;
+                int d = 255 - 4 * (int) threadIdx.x;
+#pragma unroll
+                for (int i = 0; i < 3; i++) {
+                    if (above + here[i] >= goal) break;
+                    above += here[i];
+                    d--;
+                }
+                sh.digit = (uint32_t) d;
+                sh.found = goal - above;
+            }
         }
         __syncthreads();
-        above = sh.found;
-        prefix = sh.key;
+        prefix |= sh.digit << shift;
+        goal = sh.found;
     }
-    cut r{prefix, 0};
-    uint32_t have = sh.count[prefix & 255];
-    if (prefix == in.key) have = min(have, in.ties);
+    // of the ties, as many as it takes
     if (MASS) {
-        const u64 one = prefix > KEY_MINUS_INF ? whole(weight_of(value_of(prefix), top, scale)) : 0;
-        // the first of them is kept if what lies above does not reach the goal
-        const double left = goal - (double) above;
-        r.ties = one == 0 ? have : (uint32_t) fmin(fmax(ceil(left / (double) one), 1.0), (double) have);
-    } else {
-        r.ties = (uint32_t) min((u64) have, (u64) goal - above);
+        each([&](uint32_t k, int, u64 w) {
+            if (k == prefix) sh.one = w;  // the same of all of them
+        });
+        __syncthreads();
+        const u64 one = sh.one;
+        goal = (goal + one - 1) / max(one, (u64) 1);
     }
-    return r;
+    return {prefix, nth(prefix, goal)};
 }
 
-__global__ __launch_bounds__(THREADS) void sample_kernel(sample_args a) {
-    __shared__ shared_row sh;
+// ---- short rows ----------------------------------------------------------------------
+
+// A workgroup a row, E consecutive logits a thread. Latency: 1003 logits with top-k, top-p
+// and min-p.
+template <int N, int E> __global__ __launch_bounds__(N) void row_kernel(sample_args a) {
+    __shared__ group_memory<N> sh;
     const int64_t row = blockIdx.x;
-    const params p = params_of(a, row);
-    // the largest logit and its first place
-    u64 best = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += THREADS) {
-        const u64 v = (u64) key_of(logit(a, row, i)) << 32 | (uint32_t) ~i;
-        best = max(best, v);
-    }
+    const int first = threadIdx.x * E;
+    float x[E];
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) best = max(best, (u64) __shfl_xor(best, off));
-    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = best;
-    __syncthreads();
-    for (int w = 0; w < WAVES; w++) best = max(best, sh.wave[w]);
+    for (int i = 0; i < E; i += 4) logits4(a, row, first + i, a.vocab, x + i);
+    const params p = params_of(a, row);
+    u64 best = 0;
+#pragma unroll
+    for (int i = 0; i < E; i++) best = max(best, first + i < a.vocab ? (u64) key_of(x[i]) << 32 | (uint32_t) ~(first + i) : 0);
+    best = group_max(sh, best);
     const uint32_t top_key = (uint32_t) (best >> 32);
     if (top_key <= KEY_MINUS_INF || p.greedy) {
         if (threadIdx.x == 0) {
@@ -204,53 +302,420 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(sample_args a) {
         return;
     }
     const float top = value_of(top_key);
-    cut c{0, 0};
-    if (p.k < a.vocab) c = find_cut<false>(sh, a, row, top, p.scale, c, (double) p.k);
-    auto kept = [&](float x, uint32_t k, u64 tie) { return k > c.key || (k == c.key && tie < c.ties); };
+    u64 w[E];
+    uint32_t fit = 0;  // those of at least min_p
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        const double v = weight_of(x[i], top, p.scale);
+        w[i] = whole(v);
+        fit |= (uint32_t) (v >= p.m) << i;
+    }
+    cut c = EVERYTHING;
+    auto each = [&](auto what) {
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            const uint32_t k = key_of(x[i]);
+            if (w[i] && c.keeps(k, first + i)) what(k, first + i, w[i]);
+        }
+    };
+    auto nth = [&](uint32_t key, u64 r) {  // of one key, those that the cut so far keeps
+        u64 n = 0, all;
+        each([&](uint32_t k, int, u64) { n += k == key; });
+        u64 before = group_before(sh, n, all);
+        r = min(r, all);
+        each([&](uint32_t k, int i, u64) {
+            if (k == key && ++before == r) sh.index = i;
+        });
+        __syncthreads();
+        return sh.index;
+    };
+    if (p.k < a.vocab) c = find_cut<false>(sh, (u64) p.k, each, nth);
     if (p.p < 1.0) {
         u64 sum = 0;
-        for (int i = threadIdx.x; i < a.vocab; i += THREADS) {
-            const float x = logit(a, row, i);
-            if (key_of(x) > c.key) sum += whole(weight_of(x, top, p.scale));
-        }
+        each([&](uint32_t, int, u64 v) { sum += v; });
         sum = group_sum(sh, sum);
-        if (c.key > KEY_MINUS_INF) sum += c.ties * whole(weight_of(value_of(c.key), top, p.scale));
-        c = find_cut<true>(sh, a, row, top, p.scale, c, fmax(p.p * (double) sum, 1.0));
+        c = find_cut<true>(sh, max((u64) __builtin_ceil(p.p * (double) sum), (u64) 1), each, nth);
     }
-    // What stays, in index order: first its sum, then the place that u points at.
-    // (Which of the cut's ties stay goes by their rank, so they are counted along.)
-    u64 total = 0, goal = 0;
-    for (int pass = 0; pass < 2; pass++) {
-        u64 run = 0, ties = 0;
-        for (int i0 = 0; i0 < a.vocab; i0 += THREADS) {
-            const int i = i0 + threadIdx.x;
-            const float x = i < a.vocab ? logit(a, row, i) : -INFINITY;
-            const uint32_t k = i < a.vocab ? key_of(x) : 0;
-            u64 tie_sum;
-            const u64 tie = ties + group_before(sh, k == c.key && i < a.vocab, tie_sum);
-            ties += tie_sum;
-            const double w = weight_of(x, top, p.scale);
-            const u64 mine = i < a.vocab && kept(x, k, tie) && w >= p.m ? whole(w) : 0;
-            u64 sum;
-            const u64 before = run + group_before(sh, mine, sum);
-            run += sum;
-            if (pass == 1 && mine && before <= goal && goal < before + mine) {
+    u64 mine = 0, total;
+    each([&](uint32_t, int i, u64 v) { mine += fit >> (i - first) & 1 ? v : 0; });
+    u64 before = group_before(sh, mine, total);
+    const u64 goal = min((u64) (p.u * (double) total), total - 1);
+    if (before <= goal && goal < before + mine)
+        each([&](uint32_t, int i, u64 v) {
+            v = fit >> (i - first) & 1 ? v : 0;
+            if (before <= goal && goal < before + v) {
                 a.token[row] = i;
-                if (a.prob) a.prob[row] = (float) ((double) mine / (double) total);
+                if (a.prob) a.prob[row] = (float) ((double) v / (double) total);
             }
+            before += v;
+        });
+}
+
+// ---- long rows -----------------------------------------------------------------------
+
+// This workgroup's part of a row: logit e of step j is PART part + (j THREADS + thread) 4 + e.
+constexpr int STEPS = PART / THREADS / 4;
+__device__ inline int index_of(int part, int j) { return part * PART + (j * THREADS + (int) threadIdx.x) * 4; }
+__device__ inline void load_part(const sample_args & a, int64_t row, int part, float x[STEPS][4]) {
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) logits4(a, row, index_of(part, j), a.vocab, x[j]);
+}
+
+// The distance of a logit from the largest in bins; what has no weight is in the last.
+__device__ inline int bin_of(float x, float top, float per) {
+    if (x == top) return 0;
+    const float d = (top - x) * per;
+    return d < (float) (BINS - 1) ? (int) d : BINS - 1;  // (a NaN: the last)
+}
+
+struct row_top {
+    float top, per;   // the largest logit, bins for each unit below it
+    bool none;
+    int32_t first;    // the largest one's first place
+    __device__ row_top(const sample_args & a, const row_state & s, const params & p) {
+        const int lane = threadIdx.x & 63;
+        u64 t = lane < a.parts ? s.top[lane] : 0;
+        uint32_t l = lane < a.parts ? s.low[lane] : 0xffffffffu;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
+            t = max(t, (u64) __shfl_xor(t, off));
+            l = min(l, (uint32_t) __shfl_xor((int) l, off));
         }
-        total = run;
-        goal = min((u64) (p.u * (double) total), total - 1);
+        const uint32_t key = (uint32_t) (t >> 32);
+        none = key <= KEY_MINUS_INF;
+        top = value_of(key);
+        first = (int32_t) ~(uint32_t) t;
+        const float range = none || top == INFINITY ? 0.0f : fminf(top - value_of(min(l, key)), p.width);
+        per = range > 0.0f ? fminf((float) BINS / range, 3e38f) : 0.0f;
+    }
+};
+
+// Whether this workgroup is the last of the row's to come here; what the others have
+// written before is then there to read.
+__device__ inline bool last_of(const sample_args & a, row_state & s, int which) {
+    __shared__ bool last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(&s.tickets[which], 1u) == (uint32_t) a.parts - 1;
+    __syncthreads();
+    if (last) __threadfence();
+    return last;
+}
+
+__global__ __launch_bounds__(THREADS) void stats_kernel(sample_args a) {
+    __shared__ group_memory<THREADS> sh;
+    __shared__ uint32_t lows[THREADS / 64];
+    const int part = blockIdx.x;
+    const int64_t row = blockIdx.y;
+    float x[STEPS][4];
+    load_part(a, row, part, x);
+    u64 best = 0;
+    uint32_t low = 0xffffffffu;
+#pragma unroll
+    for (int j = 0; j < STEPS; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t k = key_of(x[j][e]);
+            best = max(best, k ? (u64) k << 32 | (uint32_t) ~(index_of(part, j) + e) : 0);
+            if (k > KEY_MINUS_INF) low = min(low, k);
+        }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) low = min(low, (uint32_t) __shfl_xor((int) low, off));
+    if ((threadIdx.x & 63) == 0) lows[threadIdx.x >> 6] = low;
+    best = group_max(sh, best);
+    row_state & s = a.rows[row];
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < THREADS / 64; w++) low = min(low, lows[w]);
+        s.top[part] = best;
+        s.low[part] = low;
+        if (part == 0) s.tickets[0] = s.tickets[1] = s.listed = 0;
     }
 }
+
+// The draw, by the last workgroup: the part in which u lies by the parts' weights (mass,
+// in shared memory), then the logit, of those that the cut and min_p keep.
+__device__ void draw(group_memory<THREADS> & sh, const sample_args & a, int64_t row, const params & p, float top, cut c, const u64 * mass) {
+    const int lane = threadIdx.x & 63;
+    const u64 upto = wave_upto(lane < a.parts ? mass[lane] : 0), total = __shfl(upto, 63);
+    const u64 goal = min((u64) (p.u * (double) total), total - 1);
+    const int part = __popcll(__ballot(upto <= goal));
+    u64 run = part ? __shfl(upto, max(part - 1, 0)) : 0;
+    float x[STEPS][4];
+    load_part(a, row, part, x);
+    for (int j = 0; j < STEPS; j++) {
+        u64 w[4], mine = 0, sum;
+        for (int e = 0; e < 4; e++) {
+            const double v = weight_of(x[j][e], top, p.scale);
+            w[e] = v >= p.m && c.keeps(key_of(x[j][e]), index_of(part, j) + e) ? whole(v) : 0;
+            mine += w[e];
+        }
+        u64 before = run + group_before(sh, mine, sum);
+        run += sum;
+        for (int e = 0; e < 4; e++) {
+            if (before <= goal && goal < before + w[e]) {
+                a.token[row] = index_of(part, j) + e;
+                if (a.prob) a.prob[row] = (float) ((double) w[e] / (double) total);
+            }
+            before += w[e];
+        }
+    }
+}
+
+// Of each part the weights that min_p keeps, and the row's draw; where the row has a
+// top-k or a top-p a histogram of weights and counts by distance from the largest
+// logit, and the bins among which the cut lies.
+__global__ __launch_bounds__(THREADS) void weigh_kernel(sample_args a) {
+    __shared__ group_memory<THREADS> sh;
+    __shared__ u64 mass[BINS];
+    __shared__ uint32_t count[BINS];
+    const int part = blockIdx.x;
+    const int64_t row = blockIdx.y;
+    row_state & s = a.rows[row];
+    float x[STEPS][4];
+    load_part(a, row, part, x);
+    const params p = params_of(a, row);
+    const row_top t(a, s, p);
+    if (t.none || p.greedy) {
+        if (part == 0 && threadIdx.x == 0) {
+            a.token[row] = t.none ? -1 : t.first;
+            if (a.prob) a.prob[row] = t.none ? 0.0f : 1.0f;
+            s.mode = DONE;
+        }
+        return;
+    }
+    const bool whole_row = p.k >= a.vocab && p.p >= 1.0;
+    if (whole_row) {
+        u64 sum = 0;
+#pragma unroll
+        for (int j = 0; j < STEPS; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double w = weight_of(x[j][e], t.top, p.scale);
+                sum += w >= p.m ? whole(w) : 0;
+            }
+        sum = group_sum(sh, sum);
+        if (threadIdx.x == 0) s.mass[part] = sum;
+        if (!last_of(a, s, 0)) return;
+        if (threadIdx.x == 0) s.mode = DONE;
+        draw(sh, a, row, p, t.top, EVERYTHING, s.mass);
+        return;
+    }
+    for (int i = threadIdx.x; i < BINS; i += THREADS) {
+        mass[i] = 0;
+        count[i] = 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < STEPS; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const u64 w = whole(weight_of(x[j][e], t.top, p.scale));
+            if (w) {
+                const int b = bin_of(x[j][e], t.top, t.per);
+                atomicAdd(&mass[b], w);
+                atomicAdd(&count[b], 1u);
+            }
+        }
+    __syncthreads();
+    bin * const bins = a.bins + row * a.parts * BINS;
+    for (int i = threadIdx.x; i < BINS; i += THREADS) bins[part * BINS + i] = bin{mass[i], count[i], 0};
+    if (!last_of(a, s, 0)) return;
+    // the row's bins, two a thread, and their running sums
+    u64 m[2] = {0, 0}, n[2] = {0, 0};
+    for (int q = 0; q < a.parts; q++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const bin b = bins[q * BINS + 2 * threadIdx.x + i];
+            m[i] += b.mass;
+            n[i] += b.count;
+        }
+    u64 all_mass, all_count;
+    u64 mass_before = group_before(sh, m[0] + m[1], all_mass), count_before = group_before(sh, n[0] + n[1], all_count);
+    const bool by_k = (u64) p.k < all_count;  // (top-k keeps all there is otherwise)
+    if (!by_k && p.p >= 1.0) {
+        if (threadIdx.x == 0) s.mode = KEEP_P, s.from = BINS, s.to = -1, s.goal = 0;  // everything, nothing listed
+        return;
+    }
+    const u64 goal = by_k ? (u64) p.k : min(max((u64) __builtin_ceil(p.p * (double) all_mass), (u64) 1), all_mass);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const u64 before = by_k ? count_before : mass_before, here = by_k ? n[i] : m[i];
+        if (before < goal && before + here >= goal) {
+            const u64 listed = by_k ? count_before + n[i] : n[i];
+            s.mode = listed > LIST ? SLOW : by_k ? KEEP_K : KEEP_P;
+            s.from = by_k ? 0 : 2 * threadIdx.x + i;
+            s.to = 2 * threadIdx.x + i;
+            s.goal = goal - (by_k ? 0 : before);
+        }
+        mass_before += m[i];
+        count_before += n[i];
+    }
+}
+
+// One row whose cut lies among more logits than a list holds (very many equal ones, or a
+// top-k of thousands): the row is read for every digit of the key.
+__device__ void sample_slowly(group_memory<THREADS> & sh, const sample_args & a, int64_t row, const params & p, float top) {
+    __shared__ u64 mass[MAX_PARTS];
+    cut c = EVERYTHING;
+    auto each = [&](auto what) {
+        for (int i = threadIdx.x; i < a.vocab; i += THREADS) {
+            const float x = logit(a, row, i);
+            const uint32_t k = key_of(x);
+            const u64 w = c.keeps(k, i) ? whole(weight_of(x, top, p.scale)) : 0;
+            if (w) what(k, i, w);
+        }
+    };
+    auto nth = [&](uint32_t key, u64 r) {
+        u64 run = 0;
+        for (int i0 = 0; i0 < a.vocab; i0 += THREADS) {
+            const int i = i0 + threadIdx.x;
+            const float x = i < a.vocab ? logit(a, row, i) : NAN;
+            u64 sum;
+            const bool is = key_of(x) == key && i < a.vocab && c.keeps(key, i);
+            const u64 before = run + group_before(sh, is, sum);
+            run += sum;
+            if (is && before < r) atomicMax(&sh.index, i);  // the last of the first r
+        }
+        __syncthreads();
+        return sh.index;
+    };
+    auto reset = [&]() {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.index = -1;
+        __syncthreads();
+    };
+    if (p.k < a.vocab) {
+        reset();
+        c = find_cut<false>(sh, (u64) p.k, each, nth);
+    }
+    if (p.p < 1.0) {
+        u64 sum = 0;
+        each([&](uint32_t, int, u64 w) { sum += w; });
+        sum = group_sum(sh, sum);
+        reset();
+        c = find_cut<true>(sh, max((u64) __builtin_ceil(p.p * (double) sum), (u64) 1), each, nth);
+    }
+    __syncthreads();
+    for (int q = threadIdx.x; q < a.parts; q += THREADS) mass[q] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.vocab; i += THREADS) {
+        const float x = logit(a, row, i);
+        const double w = weight_of(x, top, p.scale);
+        if (w >= p.m && c.keeps(key_of(x), i) && whole(w)) atomicAdd(&mass[i / PART], whole(w));
+    }
+    __syncthreads();
+    draw(sh, a, row, p, top, c, mass);
+}
+
+// The logits of the bins among which the cut lies, into the row's list, of the parts the
+// weights above them; then the cut and the draw.
+__global__ __launch_bounds__(THREADS) void collect_kernel(sample_args a) {
+    __shared__ group_memory<THREADS> sh;
+    __shared__ u64 list[LIST], mass[MAX_PARTS];
+    __shared__ uint32_t at;
+    const int part = blockIdx.x;
+    const int64_t row = blockIdx.y;
+    row_state & s = a.rows[row];
+    const int mode = s.mode, from = s.from, to = s.to;
+    if (mode == DONE || (mode == SLOW && part)) return;
+    const params p = params_of(a, row);
+    const row_top t(a, s, p);
+    if (mode == SLOW) {
+        sample_slowly(sh, a, row, p, t.top);
+        return;
+    }
+    float x[STEPS][4];
+    load_part(a, row, part, x);
+    if (threadIdx.x == 0) at = 0;
+    __syncthreads();
+    u64 above = 0;
+    uint32_t mine = 0, place[STEPS][4];
+#pragma unroll
+    for (int j = 0; j < STEPS; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int b = bin_of(x[j][e], t.top, t.per);
+            place[j][e] = 0xffffffffu;
+            if (b > to && b >= from) continue;
+            const double w = weight_of(x[j][e], t.top, p.scale);
+            if (!whole(w)) continue;
+            if (b >= from) place[j][e] = atomicAdd(&at, 1u);
+            else if (w >= p.m) above += whole(w);
+        }
+    __syncthreads();
+    if (threadIdx.x == 0) mine = at ? atomicAdd(&s.listed, at) : 0;
+    above = group_sum(sh, above);
+    if (threadIdx.x == 0) {
+        s.mass[part] = above;
+        at = mine;
+    }
+    __syncthreads();
+    mine = at;
+#pragma unroll
+    for (int j = 0; j < STEPS; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (place[j][e] != 0xffffffffu && mine + place[j][e] < LIST)
+                s.list[mine + place[j][e]] = (u64) key_of(x[j][e]) << 32 | (uint32_t) (index_of(part, j) + e);
+    if (!last_of(a, s, 1)) return;
+    const int n = min((int) __hip_atomic_load(&s.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), LIST);
+    for (int i = threadIdx.x; i < n; i += THREADS) list[i] = s.list[i];
+    for (int q = threadIdx.x; q < a.parts; q += THREADS) mass[q] = mode == KEEP_P ? s.mass[q] : 0;
+    __syncthreads();
+    cut c = EVERYTHING;
+    if (n > 0) {
+        auto each = [&](auto what) {
+            for (int i = threadIdx.x; i < n; i += THREADS) {
+                const uint32_t k = (uint32_t) (list[i] >> 32);
+                const int index = (int) (uint32_t) list[i];
+                if (c.keeps(k, index)) what(k, index, whole(weight_of(value_of(k), t.top, p.scale)));
+            }
+        };
+        // (the list is in no order: the r-th place of a key has r - 1 of its places before it)
+        auto nth = [&](uint32_t key, u64 r) {
+            u64 ties = 0;
+            each([&](uint32_t k, int, u64) { ties += k == key; });
+            ties = group_sum(sh, ties);
+            if (r >= ties) return 0x7fffffff;
+            int lo = -1, hi = a.vocab;  // at or before lo there are less than r, at or before hi r
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                u64 some = 0;
+                each([&](uint32_t k, int i, u64) { some += k == key && i <= mid; });
+                if (group_sum(sh, some) >= r) hi = mid;
+                else lo = mid;
+            }
+            return hi;
+        };
+        if (mode == KEEP_K) {
+            c = find_cut<false>(sh, s.goal, each, nth);
+            if (p.p < 1.0) {
+                u64 sum = 0;
+                each([&](uint32_t, int, u64 w) { sum += w; });
+                sum = group_sum(sh, sum);
+                c = find_cut<true>(sh, max((u64) __builtin_ceil(p.p * (double) sum), (u64) 1), each, nth);
+            }
+        } else {
+            c = find_cut<true>(sh, s.goal, each, nth);
+        }
+        each([&](uint32_t k, int i, u64 w) {
+            if (weight_of(value_of(k), t.top, p.scale) >= p.m) atomicAdd(&mass[i / PART], w);
+        });
+        __syncthreads();
+    }
+    draw(sh, a, row, p, t.top, c, mass);
+}
+
+size_t bins_bytes(int64_t rows, int64_t parts) { return (size_t) rows * parts * BINS * sizeof(bin); }
 
 } // namespace
 
 extern "C" {
 
 size_t zest_sample_workspace(int64_t rows, int64_t vocab) {
-    if (rows <= 0 || rows > 65536 || vocab <= 0 || vocab > ZEST_SAMPLE_MAX_VOCAB) return 0;
-    return 16;
+    if (rows <= 0 || rows > 65536 || vocab <= 0 || vocab > ZEST_SAMPLE_MAX_VOCAB || vocab <= MIDDLE) return 0;
+    rows = std::min<int64_t>(rows, BATCH);
+    return (size_t) rows * sizeof(row_state) + bins_bytes(rows, (vocab + PART - 1) / PART);
 }
 
 int zest_sample(const void * logits, int type, int64_t rows, int64_t vocab, int64_t ld, const float * u, const float * temperature,
@@ -269,7 +734,7 @@ int zest_sample(const void * logits, int type, int64_t rows, int64_t vocab, int6
                            (const void *) token, (const void *) prob})
         ZEST_REQUIRE(reinterpret_cast<uintptr_t>(p) % 4 == 0, "%s: parameters and results 4-byte aligned wanted", me);
     const size_t need = zest_sample_workspace(rows, vocab);
-    ZEST_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= need,
+    ZEST_REQUIRE(!need || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= need),
                  "%s: workspace of %zu bytes, 16-byte aligned, wanted", me, need);
     sample_args a{};
     a.logits = logits;
@@ -278,8 +743,31 @@ int zest_sample(const void * logits, int type, int64_t rows, int64_t vocab, int6
     a.vocab = (int32_t) vocab;
     a.u = u, a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
     a.token = token, a.prob = prob;
-    hipLaunchKernelGGL(sample_kernel, dim3((unsigned) rows), dim3(THREADS), 0, zest::as_stream(stream), a);
-    return zest::check_launch(me);
+    const hipStream_t s = zest::as_stream(stream);
+    if (vocab <= SHORT) {
+        hipLaunchKernelGGL((row_kernel<256, SHORT / 256>), dim3((unsigned) rows), dim3(256), 0, s, a);
+        return zest::check_launch(me);
+    }
+    if (vocab <= MIDDLE) {
+        hipLaunchKernelGGL((row_kernel<1024, MIDDLE / 1024>), dim3((unsigned) rows), dim3(1024), 0, s, a);
+        return zest::check_launch(me);
+    }
+    a.parts = (int32_t) ((vocab + PART - 1) / PART);
+    a.rows = (row_state *) workspace;
+    a.bins = (bin *) ((uint8_t *) workspace + std::min<int64_t>(rows, BATCH) * sizeof(row_state));
+    for (int64_t r0 = 0; r0 < rows; r0 += BATCH) {
+        const dim3 grid((unsigned) a.parts, (unsigned) std::min<int64_t>(rows - r0, BATCH));
+        hipLaunchKernelGGL(stats_kernel, grid, dim3(THREADS), 0, s, a);
+        hipLaunchKernelGGL(weigh_kernel, grid, dim3(THREADS), 0, s, a);
+        if (top_k || top_p) hipLaunchKernelGGL(collect_kernel, grid, dim3(THREADS), 0, s, a);
+        if (const int st = zest::check_launch(me)) return st;
+        a.logits = (const uint8_t *) a.logits + BATCH * a.ld * size;
+        a.u += BATCH, a.token += BATCH;
+        for (const float ** q : {&a.temperature, &a.top_p, &a.min_p}) *q = *q ? *q + BATCH : nullptr;
+        a.top_k = a.top_k ? a.top_k + BATCH : nullptr;
+        a.prob = a.prob ? a.prob + BATCH : nullptr;
+    }
+    return ZEST_OK;
 }
 
 } // extern "C"

@@ -101,16 +101,17 @@ def test_matvec_glu_refuses():
 def test_sample_refuses():
     lib, base = _lib(), _base()
 
-    def call(logits=base, type=0, rows=2, vocab=100, ld=100, u=base, t=None, k=None, p=None, m=None, token=base, prob=None, ws=base + (1 << 20), size=1 << 20):
+    def call(logits=base, type=0, rows=2, vocab=20000, ld=20000, u=base, t=None, k=None, p=None, m=None, token=base, prob=None, ws=base + (1 << 20), size=1 << 20):
         return lib.zest_sample(logits, type, rows, vocab, ld, u, t, k, p, m, token, prob, ws, size, None)
 
     for broken, code in [(dict(type=2), E_UNSUPPORTED), (dict(type=8), E_UNSUPPORTED), (dict(logits=None), E_ARG), (dict(u=None), E_ARG), (dict(token=None), E_ARG),
-                         (dict(rows=0), E_ARG), (dict(rows=65537), E_ARG), (dict(vocab=0), E_ARG), (dict(vocab=(1 << 18) + 1, ld=1 << 19), E_ARG), (dict(ld=99), E_ARG),
+                         (dict(rows=0), E_ARG), (dict(rows=65537), E_ARG), (dict(vocab=0), E_ARG), (dict(vocab=(1 << 18) + 1, ld=1 << 19), E_ARG), (dict(ld=19999), E_ARG),
                          (dict(ld=1 << 31), E_ARG), (dict(logits=base + 2), E_ARG), (dict(type=1, logits=base + 1), E_ARG), (dict(u=base + 2), E_ARG), (dict(t=base + 1), E_ARG),
                          (dict(k=base + 2), E_ARG), (dict(p=base + 3), E_ARG), (dict(m=base + 2), E_ARG), (dict(token=base + 2), E_ARG), (dict(prob=base + 2), E_ARG),
                          (dict(ws=None), E_ARG), (dict(ws=base + 8), E_ARG), (dict(size=8), E_ARG)]:
         _refused("zest_sample", call(**broken), code)
-    assert lib.zest_sample_workspace(0, 5) == 0 and lib.zest_sample_workspace(1, 1 << 19) == 0 and lib.zest_sample_workspace(3, 1000) > 0
+    assert lib.zest_sample_workspace(0, 5) == 0 and lib.zest_sample_workspace(1, 1 << 19) == 0 and lib.zest_sample_workspace(3, 1000) == 0
+    assert 0 < lib.zest_sample_workspace(1, 20000) < lib.zest_sample_workspace(256, 20000) == lib.zest_sample_workspace(65536, 20000)
 
 
 def test_shared_attention_refuses():
