@@ -4,17 +4,18 @@
 // by a 32-bit key, and a weight exp((x - max) / T) is computed in 64 bits and
 // rounded to a whole number of 2^-45, so that 2^18 of them sum without a rounding
 // or an overflow in 64 bits, in any order. What top-k and top-p keep is a cut: all
-// logits above a key and those equal to it up to an index. It is found by radix
-// selection, of counts or of weights: a histogram of eight bits of the key at a
-// time among what agrees so far.
+// logits above a key and those equal to it up to an index. It is found by histograms,
+// of counts or of weights, first by the distance from the largest logit, then, if need
+// be, by digits of the key, until no more than a wave's lanes are left to compare.
 //
 // Rows of up to 16384 logits are one workgroup's, which holds them in registers.
 // Longer ones are cut in parts of 4096, a workgroup each, and the call is HBM bound by
 // one reading (the next ones come from the last-level cache): stats_kernel finds the
-// parts' largest logits, weigh_kernel the parts' weights, or a histogram of them by
-// distance from the largest, and collect_kernel, where a row has a top-k or a top-p, the
-// few logits among which its cut lies. The last workgroup of a row to finish goes on
-// with the row; the tickets that tell it are cleared by the kernel before.
+// parts' largest logits, weigh_kernel the parts' weights, or a histogram of them,
+// border_kernel, a workgroup a row, draws or finds the bins among which the cut lies,
+// and, where there is a top-k or a top-p, collect_kernel lists their logits and
+// finish_kernel cuts and draws. (With the last workgroup of a row to finish going on by
+// itself, in three launches, the fences that takes cost 300 us for 64 rows of 151936.)
 #include <algorithm>
 
 #include "zest/decode.h"
@@ -26,7 +27,8 @@ typedef unsigned long long u64;
 
 constexpr double ONE = 35184372088832.0;  // 2^45: the largest weight
 constexpr int PART = 4096, THREADS = 256, MAX_PARTS = ZEST_SAMPLE_MAX_VOCAB / PART;
-constexpr int BINS = 512, LIST = 4096;    // of a row's histogram; logits that collect_kernel holds
+constexpr int BINS = 256, LIST = 8192;    // of a histogram; logits that finish_kernel holds
+constexpr int ROW_THREADS = 1024;         // of the kernels that are a workgroup a row
 constexpr int BATCH = 256;                // rows that a workspace is for: more go in several launches
 constexpr int SHORT = 2048, MIDDLE = 16384;  // longest rows of the two sizes of row_kernel
 
@@ -36,15 +38,16 @@ struct row_state {
     uint32_t low[MAX_PARTS]; // the smallest key above -infinity's (none: 2^32 - 1)
     u64 mass[MAX_PARTS];
     u64 goal;                // of weights, within the bins that are listed
-    uint32_t tickets[2], listed;
+    uint32_t listed;
     int32_t from, to, mode;  // the bins that are listed
     u64 list[LIST];          // keys and indices
 };
 enum { DONE, KEEP_K, KEEP_P, SLOW };
 
-struct bin {
-    u64 mass;
-    uint32_t count, unused;
+// A part's histogram.
+struct part_bins {
+    u64 mass[BINS];
+    uint32_t count[BINS];
 };
 
 struct sample_args {
@@ -57,7 +60,7 @@ struct sample_args {
     int32_t * token;
     float * prob;
     row_state * rows;
-    bin * bins;              // [row][part][BINS]
+    part_bins * bins;        // [row][part]
 };
 
 // Keys order as the values do; NaN below all, -0 as 0.
@@ -148,10 +151,14 @@ __device__ inline u64 whole(double w) { return (u64) __builtin_rint(w * ONE); }
 
 template <int N> struct group_memory {
     u64 wave[N / 64];
-    u64 mass[256];
-    uint32_t count[256];
-    u64 found, one;
-    uint32_t digit;
+    u64 mass[BINS];
+    uint32_t count[BINS];
+    u64 rest, one;           // of the goal, within the digit that is left
+    uint32_t digit, left;    // and the logits in it
+    uint32_t listed;
+    uint32_t keys[64], indices[64];
+    u64 weights[64];
+    uint32_t key;
     int32_t index;
 };
 
@@ -218,61 +225,109 @@ struct cut {
 };
 constexpr cut EVERYTHING = {0, 0x7fffffff};
 
+// Bins of equal width below `origin`, the last for all that is further away.
+struct scale_of {
+    float origin, per;
+    __device__ int operator()(float x) const {
+        if (x >= origin) return 0;
+        const float d = (origin - x) * per;
+        return d < (float) (BINS - 1) ? (int) d : BINS - 1;  // (a NaN: the last)
+    }
+    // from the largest logit to the smallest, or as far as there are weights
+    static __device__ scale_of row(float top, float low, float width) {
+        const float range = top == INFINITY ? 0.0f : fminf(top - low, width);
+        return {top, range > 0.0f ? fminf((float) BINS / range, 3e38f) : 0.0f};
+    }
+};
+
 // The cut behind which a running sum, from the largest logit on, first reaches `goal`
 // (above 0): of counts, or of weights. `each` calls its argument with the key, the index
-// and the weight of every logit that may be kept, the threads' in the order of their
-// indices; ties go by index: `ties` finds the place of the r-th logit of a key.
-template <bool MASS, int N, typename Each, typename Nth> __device__ cut find_cut(group_memory<N> & sh, u64 goal, Each each, Nth nth) {
+// and the weight of every logit that may be kept, in any order; where more than 64
+// logits are equal at the cut, nth(key, r) is the index of the r-th of them (by index).
+template <bool MASS, int N, typename Each, typename Nth> __device__ cut find_cut(group_memory<N> & sh, u64 goal, scale_of bins, Each each, Nth nth) {
+    int bin = -1;          // of the distance; then digits of the key, from `shift` on
     uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
+    int shift = 32;
+    auto in = [&](uint32_t k) { return bin < 0 || (bins(value_of(k)) == bin && (shift == 32 || k >> shift == prefix >> shift)); };
+    for (;;) {
         __syncthreads();
-        for (int i = threadIdx.x; i < 256; i += N) {
+        for (int i = threadIdx.x; i < BINS; i += N) {
             sh.mass[i] = 0;
             sh.count[i] = 0;
         }
+        if (threadIdx.x == 0) sh.listed = 0;
         __syncthreads();
         each([&](uint32_t k, int, u64 w) {
-            if (shift < 24 && (k ^ prefix) >> (shift + 8)) return;
-            if (MASS) atomicAdd(&sh.mass[k >> shift & 255], w);
-            else atomicAdd(&sh.count[k >> shift & 255], 1u);
+            if (!in(k)) return;
+            const int d = bin < 0 ? bins(value_of(k)) : 255 - (int) (k >> (shift - 8) & 255);  // the largest first
+            if (MASS) atomicAdd(&sh.mass[d], w);
+            atomicAdd(&sh.count[d], 1u);
         });
         __syncthreads();
-        if (threadIdx.x < 64) {  // four digits a lane, from the largest
+        if (threadIdx.x < 64) {  // four bins a lane
             u64 here[4], sum = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int d = 255 - 4 * (int) threadIdx.x - i;
-                here[i] = MASS ? sh.mass[d] : sh.count[d];
+                here[i] = MASS ? sh.mass[4 * threadIdx.x + i] : sh.count[4 * threadIdx.x + i];
                 sum += here[i];
             }
             const u64 upto = wave_upto(sum), all = __shfl(upto, 63);
             goal = min(goal, all);  // (a product of the total may be rounded past it)
-            const bool reached = upto >= goal;
-            if (reached && upto - sum < goal) {
+            if (upto >= goal && upto - sum < goal) {
                 u64 above = upto - sum;
-                int d = 255 - 4 * (int) threadIdx.x;
+                int d = 0;
 #pragma unroll
                 for (int i = 0; i < 3; i++) {
                     if (above + here[i] >= goal) break;
                     above += here[i];
-                    d--;
+                    d++;
                 }
-                sh.digit = (uint32_t) d;
-                sh.found = goal - above;
+                sh.digit = 4 * threadIdx.x + d;
+                sh.left = sh.count[4 * threadIdx.x + d];
+                sh.rest = goal - above;
             }
         }
         __syncthreads();
-        prefix |= sh.digit << shift;
-        goal = sh.found;
+        goal = sh.rest;
+        if (bin < 0) {
+            bin = (int) sh.digit;
+        } else {
+            shift -= 8;
+            prefix |= (255 - sh.digit) << shift;
+        }
+        if (sh.left <= 64 || shift == 0) break;
     }
-    // of the ties, as many as it takes
+    if (sh.left <= 64) {
+        each([&](uint32_t k, int i, u64 w) {
+            if (!in(k)) return;
+            const uint32_t at = atomicAdd(&sh.listed, 1u);
+            sh.keys[at] = k;
+            sh.indices[at] = (uint32_t) i;
+            sh.weights[at] = MASS ? w : 1;
+        });
+        __syncthreads();
+        const uint32_t n = sh.listed, lane = threadIdx.x;
+        if (lane < n) {
+            const uint32_t k = sh.keys[lane], i = sh.indices[lane];
+            u64 before = 0;
+            for (uint32_t j = 0; j < n; j++) before += sh.keys[j] > k || (sh.keys[j] == k && sh.indices[j] < i) ? sh.weights[j] : 0;
+            if (before < goal && before + sh.weights[lane] >= goal) {
+                sh.key = k;
+                sh.index = (int) i;
+            }
+        }
+        __syncthreads();
+        const cut c{sh.key, sh.index};
+        __syncthreads();
+        return c;
+    }
+    // of the equal ones, as many as it takes
     if (MASS) {
         each([&](uint32_t k, int, u64 w) {
             if (k == prefix) sh.one = w;  // the same of all of them
         });
         __syncthreads();
-        const u64 one = sh.one;
-        goal = (goal + one - 1) / max(one, (u64) 1);
+        goal = (goal + sh.one - 1) / max(sh.one, (u64) 1);
     }
     return {prefix, nth(prefix, goal)};
 }
@@ -310,6 +365,10 @@ template <int N, int E> __global__ __launch_bounds__(N) void row_kernel(sample_a
         w[i] = whole(v);
         fit |= (uint32_t) (v >= p.m) << i;
     }
+    u64 low = 0;  // the smallest key that has a weight, as the largest of the others' distances
+#pragma unroll
+    for (int i = 0; i < E; i++) low = max(low, w[i] ? (u64) (top_key - key_of(x[i])) : 0);
+    const scale_of bins = scale_of::row(top, value_of(top_key - (uint32_t) group_max(sh, low)), p.width);
     cut c = EVERYTHING;
     auto each = [&](auto what) {
 #pragma unroll
@@ -329,12 +388,12 @@ template <int N, int E> __global__ __launch_bounds__(N) void row_kernel(sample_a
         __syncthreads();
         return sh.index;
     };
-    if (p.k < a.vocab) c = find_cut<false>(sh, (u64) p.k, each, nth);
+    if (p.k < a.vocab) c = find_cut<false>(sh, (u64) p.k, bins, each, nth);
     if (p.p < 1.0) {
         u64 sum = 0;
         each([&](uint32_t, int, u64 v) { sum += v; });
         sum = group_sum(sh, sum);
-        c = find_cut<true>(sh, max((u64) __builtin_ceil(p.p * (double) sum), (u64) 1), each, nth);
+        c = find_cut<true>(sh, max((u64) __builtin_ceil(p.p * (double) sum), (u64) 1), bins, each, nth);
     }
     u64 mine = 0, total;
     each([&](uint32_t, int i, u64 v) { mine += fit >> (i - first) & 1 ? v : 0; });
@@ -353,23 +412,18 @@ template <int N, int E> __global__ __launch_bounds__(N) void row_kernel(sample_a
 
 // ---- long rows -----------------------------------------------------------------------
 
-// This workgroup's part of a row: logit e of step j is PART part + (j THREADS + thread) 4 + e.
-constexpr int STEPS = PART / THREADS / 4;
-__device__ inline int index_of(int part, int j) { return part * PART + (j * THREADS + (int) threadIdx.x) * 4; }
-__device__ inline void load_part(const sample_args & a, int64_t row, int part, float x[STEPS][4]) {
+// A part of a row in a workgroup of N threads: logit e of step j is PART part + (j N +
+// thread) 4 + e.
+template <int N> __device__ inline int index_of(int part, int j) { return part * PART + (j * N + (int) threadIdx.x) * 4; }
+template <int N> __device__ inline void load_part(const sample_args & a, int64_t row, int part, float x[PART / N / 4][4]) {
 #pragma unroll
-    for (int j = 0; j < STEPS; j++) logits4(a, row, index_of(part, j), a.vocab, x[j]);
+    for (int j = 0; j < PART / N / 4; j++) logits4(a, row, index_of<N>(part, j), a.vocab, x[j]);
 }
-
-// The distance of a logit from the largest in bins; what has no weight is in the last.
-__device__ inline int bin_of(float x, float top, float per) {
-    if (x == top) return 0;
-    const float d = (top - x) * per;
-    return d < (float) (BINS - 1) ? (int) d : BINS - 1;  // (a NaN: the last)
-}
+constexpr int STEPS = PART / THREADS / 4;
 
 struct row_top {
-    float top, per;   // the largest logit, bins for each unit below it
+    float top;        // the largest logit
+    scale_of bins;
     bool none;
     int32_t first;    // the largest one's first place
     __device__ row_top(const sample_args & a, const row_state & s, const params & p) {
@@ -385,22 +439,9 @@ struct row_top {
         none = key <= KEY_MINUS_INF;
         top = value_of(key);
         first = (int32_t) ~(uint32_t) t;
-        const float range = none || top == INFINITY ? 0.0f : fminf(top - value_of(min(l, key)), p.width);
-        per = range > 0.0f ? fminf((float) BINS / range, 3e38f) : 0.0f;
+        bins = none ? scale_of{0.0f, 0.0f} : scale_of::row(top, value_of(min(l, key)), p.width);
     }
 };
-
-// Whether this workgroup is the last of the row's to come here; what the others have
-// written before is then there to read.
-__device__ inline bool last_of(const sample_args & a, row_state & s, int which) {
-    __shared__ bool last;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(&s.tickets[which], 1u) == (uint32_t) a.parts - 1;
-    __syncthreads();
-    if (last) __threadfence();
-    return last;
-}
 
 __global__ __launch_bounds__(THREADS) void stats_kernel(sample_args a) {
     __shared__ group_memory<THREADS> sh;
@@ -408,7 +449,7 @@ __global__ __launch_bounds__(THREADS) void stats_kernel(sample_args a) {
     const int part = blockIdx.x;
     const int64_t row = blockIdx.y;
     float x[STEPS][4];
-    load_part(a, row, part, x);
+    load_part<THREADS>(a, row, part, x);
     u64 best = 0;
     uint32_t low = 0xffffffffu;
 #pragma unroll
@@ -416,7 +457,7 @@ __global__ __launch_bounds__(THREADS) void stats_kernel(sample_args a) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const uint32_t k = key_of(x[j][e]);
-            best = max(best, k ? (u64) k << 32 | (uint32_t) ~(index_of(part, j) + e) : 0);
+            best = max(best, k ? (u64) k << 32 | (uint32_t) ~(index_of<THREADS>(part, j) + e) : 0);
             if (k > KEY_MINUS_INF) low = min(low, k);
         }
 #pragma unroll
@@ -428,63 +469,26 @@ __global__ __launch_bounds__(THREADS) void stats_kernel(sample_args a) {
         for (int w = 1; w < THREADS / 64; w++) low = min(low, lows[w]);
         s.top[part] = best;
         s.low[part] = low;
-        if (part == 0) s.tickets[0] = s.tickets[1] = s.listed = 0;
+        if (part == 0) s.listed = 0;
     }
 }
 
-// The draw, by the last workgroup: the part in which u lies by the parts' weights (mass,
-// in shared memory), then the logit, of those that the cut and min_p keep.
-__device__ void draw(group_memory<THREADS> & sh, const sample_args & a, int64_t row, const params & p, float top, cut c, const u64 * mass) {
-    const int lane = threadIdx.x & 63;
-    const u64 upto = wave_upto(lane < a.parts ? mass[lane] : 0), total = __shfl(upto, 63);
-    const u64 goal = min((u64) (p.u * (double) total), total - 1);
-    const int part = __popcll(__ballot(upto <= goal));
-    u64 run = part ? __shfl(upto, max(part - 1, 0)) : 0;
-    float x[STEPS][4];
-    load_part(a, row, part, x);
-    for (int j = 0; j < STEPS; j++) {
-        u64 w[4], mine = 0, sum;
-        for (int e = 0; e < 4; e++) {
-            const double v = weight_of(x[j][e], top, p.scale);
-            w[e] = v >= p.m && c.keeps(key_of(x[j][e]), index_of(part, j) + e) ? whole(v) : 0;
-            mine += w[e];
-        }
-        u64 before = run + group_before(sh, mine, sum);
-        run += sum;
-        for (int e = 0; e < 4; e++) {
-            if (before <= goal && goal < before + w[e]) {
-                a.token[row] = index_of(part, j) + e;
-                if (a.prob) a.prob[row] = (float) ((double) w[e] / (double) total);
-            }
-            before += w[e];
-        }
-    }
-}
+// Whether a row has neither a top-k nor a top-p.
+__device__ inline bool uncut(const sample_args & a, const params & p) { return p.k >= a.vocab && p.p >= 1.0; }
 
-// Of each part the weights that min_p keeps, and the row's draw; where the row has a
-// top-k or a top-p a histogram of weights and counts by distance from the largest
-// logit, and the bins among which the cut lies.
+// Of each part the weights that min_p keeps or, where the row has a top-k or a top-p, a
+// histogram of weights and counts by distance from the largest logit.
 __global__ __launch_bounds__(THREADS) void weigh_kernel(sample_args a) {
     __shared__ group_memory<THREADS> sh;
-    __shared__ u64 mass[BINS];
-    __shared__ uint32_t count[BINS];
     const int part = blockIdx.x;
     const int64_t row = blockIdx.y;
     row_state & s = a.rows[row];
     float x[STEPS][4];
-    load_part(a, row, part, x);
+    load_part<THREADS>(a, row, part, x);
     const params p = params_of(a, row);
     const row_top t(a, s, p);
-    if (t.none || p.greedy) {
-        if (part == 0 && threadIdx.x == 0) {
-            a.token[row] = t.none ? -1 : t.first;
-            if (a.prob) a.prob[row] = t.none ? 0.0f : 1.0f;
-            s.mode = DONE;
-        }
-        return;
-    }
-    const bool whole_row = p.k >= a.vocab && p.p >= 1.0;
-    if (whole_row) {
+    if (t.none || p.greedy) return;
+    if (uncut(a, p)) {
         u64 sum = 0;
 #pragma unroll
         for (int j = 0; j < STEPS; j++)
@@ -495,14 +499,11 @@ __global__ __launch_bounds__(THREADS) void weigh_kernel(sample_args a) {
             }
         sum = group_sum(sh, sum);
         if (threadIdx.x == 0) s.mass[part] = sum;
-        if (!last_of(a, s, 0)) return;
-        if (threadIdx.x == 0) s.mode = DONE;
-        draw(sh, a, row, p, t.top, EVERYTHING, s.mass);
         return;
     }
     for (int i = threadIdx.x; i < BINS; i += THREADS) {
-        mass[i] = 0;
-        count[i] = 0;
+        sh.mass[i] = 0;
+        sh.count[i] = 0;
     }
     __syncthreads();
 #pragma unroll
@@ -511,121 +512,118 @@ __global__ __launch_bounds__(THREADS) void weigh_kernel(sample_args a) {
         for (int e = 0; e < 4; e++) {
             const u64 w = whole(weight_of(x[j][e], t.top, p.scale));
             if (w) {
-                const int b = bin_of(x[j][e], t.top, t.per);
-                atomicAdd(&mass[b], w);
-                atomicAdd(&count[b], 1u);
+                const int b = t.bins(x[j][e]);
+                atomicAdd(&sh.mass[b], w);
+                atomicAdd(&sh.count[b], 1u);
             }
         }
     __syncthreads();
-    bin * const bins = a.bins + row * a.parts * BINS;
-    for (int i = threadIdx.x; i < BINS; i += THREADS) bins[part * BINS + i] = bin{mass[i], count[i], 0};
-    if (!last_of(a, s, 0)) return;
-    // the row's bins, two a thread, and their running sums
-    u64 m[2] = {0, 0}, n[2] = {0, 0};
-    for (int q = 0; q < a.parts; q++)
+    part_bins & bins = a.bins[row * a.parts + part];
+    for (int i = threadIdx.x; i < BINS; i += THREADS) {
+        bins.mass[i] = sh.mass[i];
+        bins.count[i] = sh.count[i];
+    }
+}
+
+// The draw: the part in which u lies by the parts' weights, then the logit, of those that
+// the cut and min_p keep.
+template <int N> __device__ void draw(group_memory<N> & sh, const sample_args & a, int64_t row, const params & p, float top, cut c, const u64 * mass) {
+    const int lane = threadIdx.x & 63;
+    const u64 upto = wave_upto(lane < a.parts ? mass[lane] : 0), total = __shfl(upto, 63);
+    const u64 goal = min((u64) (p.u * (double) total), total - 1);
+    const int part = __popcll(__ballot(upto <= goal));
+    u64 run = part ? __shfl(upto, max(part - 1, 0)) : 0;
+    float x[PART / N / 4][4];
+    load_part<N>(a, row, part, x);
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const bin b = bins[q * BINS + 2 * threadIdx.x + i];
-            m[i] += b.mass;
-            n[i] += b.count;
+    for (int j = 0; j < PART / N / 4; j++) {
+        u64 w[4], mine = 0, sum;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const double v = weight_of(x[j][e], top, p.scale);
+            w[e] = v >= p.m && c.keeps(key_of(x[j][e]), index_of<N>(part, j) + e) ? whole(v) : 0;
+            mine += w[e];
         }
+        u64 before = run + group_before(sh, mine, sum);
+        run += sum;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (before <= goal && goal < before + w[e]) {
+                a.token[row] = index_of<N>(part, j) + e;
+                if (a.prob) a.prob[row] = (float) ((double) w[e] / (double) total);
+            }
+            before += w[e];
+        }
+    }
+}
+
+// Rows without a cut drawn; of the others the bins among which it lies.
+__global__ __launch_bounds__(ROW_THREADS) void border_kernel(sample_args a) {
+    __shared__ group_memory<ROW_THREADS> sh;
+    const int64_t row = blockIdx.x;
+    row_state & s = a.rows[row];
+    const params p = params_of(a, row);
+    const row_top t(a, s, p);
+    if (t.none || p.greedy) {
+        if (threadIdx.x == 0) {
+            a.token[row] = t.none ? -1 : t.first;
+            if (a.prob) a.prob[row] = t.none ? 0.0f : 1.0f;
+            s.mode = DONE;
+        }
+        return;
+    }
+    if (uncut(a, p)) {
+        if (threadIdx.x == 0) s.mode = DONE;
+        draw(sh, a, row, p, t.top, EVERYTHING, s.mass);
+        return;
+    }
+    // the parts' bins, every fourth part a quarter of the threads
+    const int i = threadIdx.x % BINS, q0 = threadIdx.x / BINS;
+    if (q0 == 0) sh.mass[i] = sh.count[i] = 0;
+    __syncthreads();
+    u64 m = 0;
+    uint32_t n = 0;
+#pragma unroll 4
+    for (int q = q0; q < a.parts; q += ROW_THREADS / BINS) {
+        m += a.bins[row * a.parts + q].mass[i];
+        n += a.bins[row * a.parts + q].count[i];
+    }
+    atomicAdd(&sh.mass[i], m);
+    atomicAdd(&sh.count[i], n);
+    __syncthreads();
+    m = q0 == 0 ? sh.mass[i] : 0;
+    n = q0 == 0 ? sh.count[i] : 0;
     u64 all_mass, all_count;
-    u64 mass_before = group_before(sh, m[0] + m[1], all_mass), count_before = group_before(sh, n[0] + n[1], all_count);
+    const u64 mass_before = group_before(sh, m, all_mass), count_before = group_before(sh, (u64) n, all_count);
     const bool by_k = (u64) p.k < all_count;  // (top-k keeps all there is otherwise)
     if (!by_k && p.p >= 1.0) {
         if (threadIdx.x == 0) s.mode = KEEP_P, s.from = BINS, s.to = -1, s.goal = 0;  // everything, nothing listed
         return;
     }
     const u64 goal = by_k ? (u64) p.k : min(max((u64) __builtin_ceil(p.p * (double) all_mass), (u64) 1), all_mass);
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const u64 before = by_k ? count_before : mass_before, here = by_k ? n[i] : m[i];
-        if (before < goal && before + here >= goal) {
-            const u64 listed = by_k ? count_before + n[i] : n[i];
-            s.mode = listed > LIST ? SLOW : by_k ? KEEP_K : KEEP_P;
-            s.from = by_k ? 0 : 2 * threadIdx.x + i;
-            s.to = 2 * threadIdx.x + i;
-            s.goal = goal - (by_k ? 0 : before);
-        }
-        mass_before += m[i];
-        count_before += n[i];
+    const u64 before = by_k ? count_before : mass_before, here = by_k ? (u64) n : m;
+    if (before < goal && before + here >= goal) {
+        s.mode = (by_k ? count_before + n : n) > LIST ? SLOW : by_k ? KEEP_K : KEEP_P;
+        s.from = by_k ? 0 : i;
+        s.to = i;
+        s.goal = goal - (by_k ? 0 : before);
     }
 }
 
-// One row whose cut lies among more logits than a list holds (very many equal ones, or a
-// top-k of thousands): the row is read for every digit of the key.
-__device__ void sample_slowly(group_memory<THREADS> & sh, const sample_args & a, int64_t row, const params & p, float top) {
-    __shared__ u64 mass[MAX_PARTS];
-    cut c = EVERYTHING;
-    auto each = [&](auto what) {
-        for (int i = threadIdx.x; i < a.vocab; i += THREADS) {
-            const float x = logit(a, row, i);
-            const uint32_t k = key_of(x);
-            const u64 w = c.keeps(k, i) ? whole(weight_of(x, top, p.scale)) : 0;
-            if (w) what(k, i, w);
-        }
-    };
-    auto nth = [&](uint32_t key, u64 r) {
-        u64 run = 0;
-        for (int i0 = 0; i0 < a.vocab; i0 += THREADS) {
-            const int i = i0 + threadIdx.x;
-            const float x = i < a.vocab ? logit(a, row, i) : NAN;
-            u64 sum;
-            const bool is = key_of(x) == key && i < a.vocab && c.keeps(key, i);
-            const u64 before = run + group_before(sh, is, sum);
-            run += sum;
-            if (is && before < r) atomicMax(&sh.index, i);  // the last of the first r
-        }
-        __syncthreads();
-        return sh.index;
-    };
-    auto reset = [&]() {
-        __syncthreads();
-        if (threadIdx.x == 0) sh.index = -1;
-        __syncthreads();
-    };
-    if (p.k < a.vocab) {
-        reset();
-        c = find_cut<false>(sh, (u64) p.k, each, nth);
-    }
-    if (p.p < 1.0) {
-        u64 sum = 0;
-        each([&](uint32_t, int, u64 w) { sum += w; });
-        sum = group_sum(sh, sum);
-        reset();
-        c = find_cut<true>(sh, max((u64) __builtin_ceil(p.p * (double) sum), (u64) 1), each, nth);
-    }
-    __syncthreads();
-    for (int q = threadIdx.x; q < a.parts; q += THREADS) mass[q] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.vocab; i += THREADS) {
-        const float x = logit(a, row, i);
-        const double w = weight_of(x, top, p.scale);
-        if (w >= p.m && c.keeps(key_of(x), i) && whole(w)) atomicAdd(&mass[i / PART], whole(w));
-    }
-    __syncthreads();
-    draw(sh, a, row, p, top, c, mass);
-}
-
-// The logits of the bins among which the cut lies, into the row's list, of the parts the
-// weights above them; then the cut and the draw.
+// The logits of the bins among which the cut lies, into the row's list, and of the parts
+// the weights above them.
 __global__ __launch_bounds__(THREADS) void collect_kernel(sample_args a) {
     __shared__ group_memory<THREADS> sh;
-    __shared__ u64 list[LIST], mass[MAX_PARTS];
     __shared__ uint32_t at;
     const int part = blockIdx.x;
     const int64_t row = blockIdx.y;
     row_state & s = a.rows[row];
     const int mode = s.mode, from = s.from, to = s.to;
-    if (mode == DONE || (mode == SLOW && part)) return;
+    if (mode == DONE || mode == SLOW) return;
+    float x[STEPS][4];
+    load_part<THREADS>(a, row, part, x);
     const params p = params_of(a, row);
     const row_top t(a, s, p);
-    if (mode == SLOW) {
-        sample_slowly(sh, a, row, p, t.top);
-        return;
-    }
-    float x[STEPS][4];
-    load_part(a, row, part, x);
     if (threadIdx.x == 0) at = 0;
     __syncthreads();
     u64 above = 0;
@@ -634,7 +632,7 @@ __global__ __launch_bounds__(THREADS) void collect_kernel(sample_args a) {
     for (int j = 0; j < STEPS; j++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int b = bin_of(x[j][e], t.top, t.per);
+            const int b = t.bins(x[j][e]);
             place[j][e] = 0xffffffffu;
             if (b > to && b >= from) continue;
             const double w = weight_of(x[j][e], t.top, p.scale);
@@ -656,22 +654,38 @@ __global__ __launch_bounds__(THREADS) void collect_kernel(sample_args a) {
 #pragma unroll
         for (int e = 0; e < 4; e++)
             if (place[j][e] != 0xffffffffu && mine + place[j][e] < LIST)
-                s.list[mine + place[j][e]] = (u64) key_of(x[j][e]) << 32 | (uint32_t) (index_of(part, j) + e);
-    if (!last_of(a, s, 1)) return;
-    const int n = min((int) __hip_atomic_load(&s.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), LIST);
-    for (int i = threadIdx.x; i < n; i += THREADS) list[i] = s.list[i];
-    for (int q = threadIdx.x; q < a.parts; q += THREADS) mass[q] = mode == KEEP_P ? s.mass[q] : 0;
-    __syncthreads();
+                s.list[mine + place[j][e]] = (u64) key_of(x[j][e]) << 32 | (uint32_t) (index_of<THREADS>(part, j) + e);
+}
+
+// The cut and the draw. A row whose cut lies among more logits than a list holds (very
+// many equal ones, or a top-k of thousands) is read itself for every histogram.
+__global__ __launch_bounds__(ROW_THREADS) void finish_kernel(sample_args a) {
+    __shared__ group_memory<ROW_THREADS> sh;
+    __shared__ u64 list[LIST], mass[MAX_PARTS];
+    const int64_t row = blockIdx.x;
+    row_state & s = a.rows[row];
+    const int mode = s.mode;
+    if (mode == DONE) return;
+    const params p = params_of(a, row);
+    const row_top t(a, s, p);
     cut c = EVERYTHING;
+    const bool listed = mode != SLOW;
+    const int n = listed ? min((int) s.listed, LIST) : a.vocab;
+    if (listed)
+        for (int i = threadIdx.x; i < n; i += ROW_THREADS) list[i] = s.list[i];
+    for (int q = threadIdx.x; q < a.parts; q += ROW_THREADS) mass[q] = mode == KEEP_P ? s.mass[q] : 0;
+    __syncthreads();
     if (n > 0) {
         auto each = [&](auto what) {
-            for (int i = threadIdx.x; i < n; i += THREADS) {
-                const uint32_t k = (uint32_t) (list[i] >> 32);
-                const int index = (int) (uint32_t) list[i];
-                if (c.keeps(k, index)) what(k, index, whole(weight_of(value_of(k), t.top, p.scale)));
+            for (int i = threadIdx.x; i < n; i += ROW_THREADS) {
+                const uint32_t k = listed ? (uint32_t) (list[i] >> 32) : key_of(logit(a, row, i));
+                const int index = listed ? (int) (uint32_t) list[i] : i;
+                if (!c.keeps(k, index)) continue;
+                const u64 w = whole(weight_of(value_of(k), t.top, p.scale));
+                if (w) what(k, index, w);
             }
         };
-        // (the list is in no order: the r-th place of a key has r - 1 of its places before it)
+        // (in no order: the r-th place of a key has r - 1 of its places before it)
         auto nth = [&](uint32_t key, u64 r) {
             u64 ties = 0;
             each([&](uint32_t k, int, u64) { ties += k == key; });
@@ -687,16 +701,22 @@ __global__ __launch_bounds__(THREADS) void collect_kernel(sample_args a) {
             }
             return hi;
         };
-        if (mode == KEEP_K) {
-            c = find_cut<false>(sh, s.goal, each, nth);
-            if (p.p < 1.0) {
+        // the histogram's bins are those of what is listed
+        scale_of bins = t.bins;
+        if (listed) {
+            bins.origin -= bins.per > 0.0f ? (float) s.from / bins.per : 0.0f;
+            bins.per = fminf(bins.per * ((float) BINS / (float) (s.to - s.from + 1)), 3e38f);
+        }
+        const bool by_k = mode == KEEP_K || (!listed && p.k < a.vocab);
+        if (by_k) c = find_cut<false>(sh, (u64) p.k, bins, each, nth);
+        if (p.p < 1.0) {
+            u64 goal = s.goal;
+            if (mode != KEEP_P) {
                 u64 sum = 0;
                 each([&](uint32_t, int, u64 w) { sum += w; });
-                sum = group_sum(sh, sum);
-                c = find_cut<true>(sh, max((u64) __builtin_ceil(p.p * (double) sum), (u64) 1), each, nth);
+                goal = max((u64) __builtin_ceil(p.p * (double) group_sum(sh, sum)), (u64) 1);
             }
-        } else {
-            c = find_cut<true>(sh, s.goal, each, nth);
+            c = find_cut<true>(sh, goal, bins, each, nth);
         }
         each([&](uint32_t k, int i, u64 w) {
             if (weight_of(value_of(k), t.top, p.scale) >= p.m) atomicAdd(&mass[i / PART], w);
@@ -706,7 +726,7 @@ __global__ __launch_bounds__(THREADS) void collect_kernel(sample_args a) {
     draw(sh, a, row, p, t.top, c, mass);
 }
 
-size_t bins_bytes(int64_t rows, int64_t parts) { return (size_t) rows * parts * BINS * sizeof(bin); }
+size_t bins_bytes(int64_t rows, int64_t parts) { return (size_t) rows * parts * sizeof(part_bins); }
 
 } // namespace
 
@@ -754,12 +774,16 @@ int zest_sample(const void * logits, int type, int64_t rows, int64_t vocab, int6
     }
     a.parts = (int32_t) ((vocab + PART - 1) / PART);
     a.rows = (row_state *) workspace;
-    a.bins = (bin *) ((uint8_t *) workspace + std::min<int64_t>(rows, BATCH) * sizeof(row_state));
+    a.bins = (part_bins *) ((uint8_t *) workspace + std::min<int64_t>(rows, BATCH) * sizeof(row_state));
     for (int64_t r0 = 0; r0 < rows; r0 += BATCH) {
         const dim3 grid((unsigned) a.parts, (unsigned) std::min<int64_t>(rows - r0, BATCH));
         hipLaunchKernelGGL(stats_kernel, grid, dim3(THREADS), 0, s, a);
         hipLaunchKernelGGL(weigh_kernel, grid, dim3(THREADS), 0, s, a);
-        if (top_k || top_p) hipLaunchKernelGGL(collect_kernel, grid, dim3(THREADS), 0, s, a);
+        hipLaunchKernelGGL(border_kernel, dim3(grid.y), dim3(ROW_THREADS), 0, s, a);
+        if (top_k || top_p) {
+            hipLaunchKernelGGL(collect_kernel, grid, dim3(THREADS), 0, s, a);
+            hipLaunchKernelGGL(finish_kernel, dim3(grid.y), dim3(ROW_THREADS), 0, s, a);
+        }
         if (const int st = zest::check_launch(me)) return st;
         a.logits = (const uint8_t *) a.logits + BATCH * a.ld * size;
         a.u += BATCH, a.token += BATCH;
