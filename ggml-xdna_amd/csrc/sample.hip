@@ -8,7 +8,7 @@
 // of counts or of weights, first by the distance from the largest logit, then, if need
 // be, by digits of the key, until no more than a wave's lanes are left to compare.
 //
-// Rows of up to 16384 logits are one workgroup's, which holds them in registers.
+// Rows of up to 8192 logits are one workgroup's, which holds them in registers.
 // Longer ones are cut in parts of 4096, a workgroup each, and the call is HBM bound by
 // one reading (the next ones come from the last-level cache): stats_kernel finds the
 // parts' largest logits, weigh_kernel the parts' weights, or a histogram of them,
@@ -25,12 +25,12 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr double ONE = 35184372088832.0;  // 2^45: the largest weight
 constexpr int PART = 4096, THREADS = 256, MAX_PARTS = ZEST_SAMPLE_MAX_VOCAB / PART;
 constexpr int BINS = 256, LIST = 8192;    // of a histogram; logits that finish_kernel holds
 constexpr int ROW_THREADS = 1024;         // of the kernels that are a workgroup a row
+static_assert(THREADS == BINS, "a thread a bin");
 constexpr int BATCH = 256;                // rows that a workspace is for: more go in several launches
-constexpr int SHORT = 2048, MIDDLE = 16384;  // longest rows of the two sizes of row_kernel
+constexpr int SHORT = 2048, MIDDLE = 8192;  // longest rows of the two sizes of row_kernel
 
 // What a row's workgroups leave each other.
 struct row_state {
@@ -105,6 +105,7 @@ struct params {
     float width;            // logits further than this below the largest have no weight
     int k;                  // vocab: off
     bool greedy;
+    template <typename W> __device__ bool fits(const W & w) const { return m == 0.0 || w.value() >= m; }  // min_p
 };
 
 __device__ inline params params_of(const sample_args & a, int64_t row) {
@@ -122,14 +123,26 @@ __device__ inline params params_of(const sample_args & a, int64_t row) {
     return r;
 }
 
-// A logit's weight relative to the largest: 2^y by the series of e^(f ln 2) for the
-// part of y within half a unit (to its 12th power: off by 2^-52 at most).
-__device__ inline double weight_of(float x, float top, double scale) {
-    if (x == top) return 1.0;
-    if (!(x > -INFINITY) || top == INFINITY) return 0.0;  // (a NaN: 0)
-    const double y = ((double) x - (double) top) * scale;
-    if (y < -60.0) return 0.0;
-    const double n = __builtin_rint(y), f = (y - n) * 0.69314718055994530942;
+// A logit's weight relative to the largest, s 2^n: 2^y by the series of e^(f ln 2) for
+// the part of y within half a unit (to its 12th power: off by 2^-52 at most). Adding
+// 1.5 2^52 leaves a sum's whole part in its low bits.
+struct weight {
+    double s;
+    int n;
+    __device__ double value() const { return s * __hiloint2double((1023 + n) << 20, 0); }
+    // in whole numbers of 2^-45
+    __device__ u64 whole() const {
+        constexpr double TWO52 = 4503599627370496.0;
+        return (u64) (__double_as_longlong(fma(s, __hiloint2double((1023 + 45 + n) << 20, 0), TWO52)) - __double_as_longlong(TWO52));
+    }
+};
+
+__device__ inline weight weight_of(float x, float top, double scale) {
+    if (x == top) return {1.0, 0};
+    const double d = (double) x - (double) top;
+    if (!(d * scale >= -60.0) || top == INFINITY) return {0.0, 0};  // (a NaN, an infinity: none)
+    constexpr double MAGIC = 6755399441055744.0;
+    const double t = fma(d, scale, MAGIC), f = fma(d, scale, MAGIC - t) * 0.69314718055994530942;
     double s = 1.0 / 479001600.0;
     s = fma(s, f, 1.0 / 39916800.0);
     s = fma(s, f, 1.0 / 3628800.0);
@@ -143,9 +156,9 @@ __device__ inline double weight_of(float x, float top, double scale) {
     s = fma(s, f, 0.5);
     s = fma(s, f, 1.0);
     s = fma(s, f, 1.0);
-    return __builtin_ldexp(s, (int) n);
+    return {s, (int) (uint32_t) __double_as_longlong(t)};
 }
-__device__ inline u64 whole(double w) { return (u64) __builtin_rint(w * ONE); }
+__device__ inline u64 whole(const weight & w) { return w.whole(); }
 
 // ---- sums over a workgroup -----------------------------------------------------------
 
@@ -334,7 +347,8 @@ template <bool MASS, int N, typename Each, typename Nth> __device__ cut find_cut
 
 // ---- short rows ----------------------------------------------------------------------
 
-// A workgroup a row, E consecutive logits a thread. Latency: 1003 logits with top-k, top-p
+// A workgroup a row, E consecutive logits a thread: 8, since 16 of 1024 threads' take more
+// registers than there are (120 spilled). Latency: 1003 logits with top-k, top-p
 // and min-p.
 template <int N, int E> __global__ __launch_bounds__(N) void row_kernel(sample_args a) {
     __shared__ group_memory<N> sh;
@@ -361,9 +375,9 @@ template <int N, int E> __global__ __launch_bounds__(N) void row_kernel(sample_a
     uint32_t fit = 0;  // those of at least min_p
 #pragma unroll
     for (int i = 0; i < E; i++) {
-        const double v = weight_of(x[i], top, p.scale);
+        const weight v = weight_of(x[i], top, p.scale);
         w[i] = whole(v);
-        fit |= (uint32_t) (v >= p.m) << i;
+        fit |= (uint32_t) p.fits(v) << i;
     }
     u64 low = 0;  // the smallest key that has a weight, as the largest of the others' distances
 #pragma unroll
@@ -494,8 +508,8 @@ __global__ __launch_bounds__(THREADS) void weigh_kernel(sample_args a) {
         for (int j = 0; j < STEPS; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const double w = weight_of(x[j][e], t.top, p.scale);
-                sum += w >= p.m ? whole(w) : 0;
+                const weight w = weight_of(x[j][e], t.top, p.scale);
+                sum += p.fits(w) ? whole(w) : 0;
             }
         sum = group_sum(sh, sum);
         if (threadIdx.x == 0) s.mass[part] = sum;
@@ -540,8 +554,8 @@ template <int N> __device__ void draw(group_memory<N> & sh, const sample_args & 
         u64 w[4], mine = 0, sum;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const double v = weight_of(x[j][e], top, p.scale);
-            w[e] = v >= p.m && c.keeps(key_of(x[j][e]), index_of<N>(part, j) + e) ? whole(v) : 0;
+            const weight v = weight_of(x[j][e], top, p.scale);
+            w[e] = p.fits(v) && c.keeps(key_of(x[j][e]), index_of<N>(part, j) + e) ? whole(v) : 0;
             mine += w[e];
         }
         u64 before = run + group_before(sh, mine, sum);
@@ -634,12 +648,14 @@ __global__ __launch_bounds__(THREADS) void collect_kernel(sample_args a) {
         for (int e = 0; e < 4; e++) {
             const int b = t.bins(x[j][e]);
             place[j][e] = 0xffffffffu;
-            if (b > to && b >= from) continue;
-            const double w = weight_of(x[j][e], t.top, p.scale);
-            if (!whole(w)) continue;
-            if (b >= from) place[j][e] = atomicAdd(&at, 1u);
-            else if (w >= p.m) above += whole(w);
+            if (b < from && p.m > 0.0) {
+                const weight w = weight_of(x[j][e], t.top, p.scale);
+                above += p.fits(w) ? whole(w) : 0;
+            } else if (b >= from && b <= to && whole(weight_of(x[j][e], t.top, p.scale))) {
+                place[j][e] = atomicAdd(&at, 1u);
+            }
         }
+    if (p.m == 0.0 && (int) threadIdx.x < from) above = a.bins[row * a.parts + part].mass[threadIdx.x];
     __syncthreads();
     if (threadIdx.x == 0) mine = at ? atomicAdd(&s.listed, at) : 0;
     above = group_sum(sh, above);
@@ -719,7 +735,7 @@ __global__ __launch_bounds__(ROW_THREADS) void finish_kernel(sample_args a) {
             c = find_cut<true>(sh, goal, bins, each, nth);
         }
         each([&](uint32_t k, int i, u64 w) {
-            if (weight_of(value_of(k), t.top, p.scale) >= p.m) atomicAdd(&mass[i / PART], w);
+            if (p.fits(weight_of(value_of(k), t.top, p.scale))) atomicAdd(&mass[i / PART], w);
         });
         __syncthreads();
     }
