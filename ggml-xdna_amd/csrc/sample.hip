@@ -102,7 +102,7 @@ __device__ inline void logits4(const sample_args & a, int64_t row, int i, int en
 // A row's parameters, as the definition reads them.
 struct params {
     double scale, p, m, u;  // scale in powers of two; p 1, m 0: off
-    float width;            // logits further than this below the largest have no weight
+    float width, near;      // logits further than this below the largest have no weight, or less than min_p
     int k;                  // vocab: off
     bool greedy;
     template <typename W> __device__ bool fits(const W & w) const { return m == 0.0 || w.value() >= m; }  // min_p
@@ -117,6 +117,7 @@ __device__ inline params params_of(const sample_args & a, int64_t row) {
     const float p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
     r.p = p < 1.0f ? fmax((double) p, 0.0) : 1.0;  // (a NaN is off)
     r.m = m > 0.0f ? fmin((double) m, 1.0) : 0.0;
+    r.near = r.m > 0.0 ? fminf(1.0001f * t * (0.01f - __logf((float) r.m)), r.width) : r.width;
     r.u = u > 0.0f ? (double) u : 0.0;
     const int k = a.top_k ? a.top_k[row] : 0;
     r.k = k > 0 ? min(k, a.vocab) : a.vocab;
@@ -508,6 +509,7 @@ __global__ __launch_bounds__(THREADS) void weigh_kernel(sample_args a) {
         for (int j = 0; j < STEPS; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
+                if (t.top - x[j][e] > p.near) continue;  // (most: a wave passes over the series)
                 const weight w = weight_of(x[j][e], t.top, p.scale);
                 sum += p.fits(w) ? whole(w) : 0;
             }
@@ -648,7 +650,7 @@ __global__ __launch_bounds__(THREADS) void collect_kernel(sample_args a) {
         for (int e = 0; e < 4; e++) {
             const int b = t.bins(x[j][e]);
             place[j][e] = 0xffffffffu;
-            if (b < from && p.m > 0.0) {
+            if (b < from && p.m > 0.0 && !(t.top - x[j][e] > p.near)) {
                 const weight w = weight_of(x[j][e], t.top, p.scale);
                 above += p.fits(w) ? whole(w) : 0;
             } else if (b >= from && b <= to && whole(weight_of(x[j][e], t.top, p.scale))) {

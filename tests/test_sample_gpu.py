@@ -99,24 +99,25 @@ def test_ties_go_to_the_lowest_index(s):
     assert {_check(s, x, [u], None, [2])[0] for u in (0.0, 0.3, 0.6, 0.99)} == {0, 1}
 
 
-def test_masked_and_odd_logits(s):
+@pytest.mark.parametrize("vocab", [1000, 5000, 30000])
+def test_masked_and_odd_logits(s, vocab):
     """-infinity and NaN are never taken, whatever u; +infinity takes all; a row of nothing gives -1."""
-    x = torch.full((8, 1000), -math.inf)
+    x = torch.full((8, vocab), -math.inf)
     x[0, 321] = -5.0
     x[1, ::3] = math.nan
     x[1, 10::50] = 1.0
-    x[2, 5] = x[2, 900] = math.inf
+    x[2, 5] = x[2, vocab - 100] = math.inf
     x[2, 30:60] = 1e30
     x[4] = math.nan
-    x[5, 999] = -3e38
+    x[5, vocab - 1] = -3e38
     x[6, 0] = 3.4e38
     x[6, 1] = -3.4e38
-    x[7] = torch.randn(1000, generator=torch.Generator().manual_seed(1))
+    x[7] = torch.randn(vocab, generator=torch.Generator().manual_seed(1))
     x[7, ::2] = -math.inf
     for u in (0.0, 0.4, 0.6, 1.0 - 2.0 ** -24):
-        for more in (dict(), dict(k=[100] * 8), dict(p=[0.9] * 8), dict(m=[0.5] * 8), dict(t=[0.0] * 8), dict(t=[math.inf] * 8)):
+        for more in (dict(), dict(k=[vocab // 10] * 8), dict(p=[0.9] * 8), dict(m=[0.5] * 8), dict(p=[0.9] * 8, m=[1e-3] * 8), dict(t=[0.0] * 8), dict(t=[math.inf] * 8)):
             tokens = _check(s, x, [u] * 8, **more)
-            assert tokens[0] == 321 and tokens[3] == tokens[4] == -1 and tokens[2] in (5, 900) and tokens[5] == 999 and tokens[6] <= 1
+            assert tokens[0] == 321 and tokens[3] == tokens[4] == -1 and tokens[2] in (5, vocab - 100) and tokens[5] == vocab - 1 and tokens[6] <= 1
             assert tokens[7] % 2 == 1
 
 
@@ -143,11 +144,12 @@ def test_rows_of_any_stride_and_alignment(s, dtype):
         _check(s, wide.cuda()[:, at:at + 2900], [0.1 * i for i in range(7)])
 
 
-@pytest.mark.parametrize("rows,vocab", [(300, 500), (2000, 100), (65, 40000)])
+@pytest.mark.parametrize("rows,vocab", [(300, 500), (2000, 100), (65, 40000), (270, 8193), (257, 16385)])
 def test_many_rows(s, rows, vocab):
     x = _logits(rows, vocab, seed=rows)
     u = [(i * 0.6180339887) % 1.0 for i in range(rows)]
-    _check(s, x, u, [0.5 + (i % 5) * 0.3 for i in range(rows)], [(i * 7) % 60 for i in range(rows)], [1.0 - (i % 4) * 0.1 for i in range(rows)])
+    _check(s, x, u, [0.5 + (i % 5) * 0.3 for i in range(rows)], [(i * 7) % 60 for i in range(rows)], [1.0 - (i % 4) * 0.1 for i in range(rows)],
+           [0.0 if i % 3 else 0.02 for i in range(rows)])
 
 
 def test_draws_follow_the_distribution(s):
