@@ -19,13 +19,17 @@ has were run on end.
 Weights are random-init N(0, 0.02), quantised to GGUF on the GPU, converted
 once into the resident bfp16 cache (timed separately, as the reference
 reports warm prefill with its one-time copy build apart).
+
+Decode runs the same layers a token at a time, for several answers to one
+prompt: the GGUF weights as they are (matvec), attention that reads the prompt
+the answers share once, and the next tokens drawn from the logits.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass, field
 
 import ggml_xdna_amd as z
-from ggml_xdna_amd import kv, quant
+from ggml_xdna_amd import kv, quant, sampling
 
 BF16_PEAK_TFLOPS = 2516.6  # MI355X dense bf16 MFMA: 256 CU x 2.4 GHz x 4096 FLOP/clk
 HBM_PEAK_GBS = 8000.0
@@ -250,3 +254,87 @@ class Stack:
             kv.assign(self.cache, self.slot, self.none, self.none + 1)
         for t0 in range(0, self.cfg.tokens, self.chunk):
             self.run_chunk(self.x[t0:t0 + self.chunk], gemm_events)
+
+
+class Decode:
+    """`answers` (up to 16) to one prompt, a token each a step:
+        RMS_NORM(h) * w_attn ; Q, K, V = matvec           one launch, GGUF weights
+        kv.append (turned) ; kv.attention with the answers as one group
+        h = h + matvec(Wo) ; RMS_NORM(h) * w_ffn ; matvec_glu ; h = h + matvec(Wdown)
+    and, after the last layer, RMS_NORM * w_out, the logits' matvec and
+    sampling.sample, whose tokens are the next step's. prompt() fills slot 0 and
+    makes the others its forks; step() waits for nothing and allocates from torch's
+    allocator alone, so it can be captured in a graph and replayed."""
+
+    def __init__(self, cfg: StackConfig, vocab: int, answers: int, max_len: int, seed: int = 0, device: str = "cuda",
+                 page: int = 64):
+        import torch
+        self.cfg, self.vocab, self.answers, self.max_len = cfg, vocab, answers, max_len
+        g = torch.Generator(device=device)
+        g.manual_seed(seed)
+
+        def weight(n, k, t):
+            return quant.quantize(t, torch.randn((n, k), generator=g, device=device) * 0.02)
+
+        by_shape = {}  # layers share the GGUF source bytes, as Stack's do
+        self.layers = []
+        for _ in range(cfg.layers):
+            L = Layer()
+            for name, n, k, t in cfg.matmuls():
+                if name not in by_shape:
+                    by_shape[name] = weight(n, k, t)
+                L.w[name] = by_shape[name]
+            L.attn_norm = 1.0 + 0.1 * torch.randn(cfg.hidden, generator=g, device=device)
+            L.ffn_norm = 1.0 + 0.1 * torch.randn(cfg.hidden, generator=g, device=device)
+            self.layers.append(L)
+        self.out_norm = 1.0 + 0.1 * torch.randn(cfg.hidden, generator=g, device=device)
+        self.embed = torch.randn((vocab, cfg.hidden), generator=g, device=device)
+        self.logits_w = weight(vocab, cfg.hidden, cfg.qkv_type)
+        self.cache = kv.empty_cache(cfg.layers, answers * -(-max_len // page), cfg.kv // cfg.head_dim, cfg.head_dim, page,
+                                    slots=answers, columns=-(-max_len // page), device=device)
+        freqs, mag = kv.rope_freqs(cfg.head_dim, cfg.rope_base)
+        self.rope = kv.Rope(torch.tensor(freqs, dtype=torch.float64, device=device), kv.ROPE_NEOX, mag)
+        self._i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=device)
+        self.slots, self.one = self._i32(list(range(answers))), self._i32([1] * answers)
+        self.batch = kv.Batch(self._i32(list(range(answers + 1))), answers, 1, max_len)
+        self.groups = kv.Groups(self._i32([0, answers]), max_len)
+        # a step's state and parameters: tokens in and out, u and the choice's settings the caller's to fill
+        self.tokens = torch.zeros(answers, dtype=torch.int32, device=device)
+        self.u, self.probs = (torch.zeros(answers, device=device) for _ in range(2))
+        self.temperature, self.top_p, self.min_p = (torch.full((answers,), v, device=device) for v in (1.0, 1.0, 0.0))
+        self.top_k = torch.zeros(answers, dtype=torch.int32, device=device)
+
+    def _run(self, tokens, batch, groups):
+        c, eps = self.cfg, 1e-6
+        h = self.embed[tokens.clamp(min=0).long()]
+        for li, L in enumerate(self.layers):
+            a = z.rms_norm(h, eps, L.attn_norm)
+            q, k, v = z.matvec(c.qkv_type, a, [L.w[n] for n in ("attn_q", "attn_k", "attn_v")], [c.q, c.kv, c.kv])
+            q = kv.append(self.cache, li, batch, k, v, q=q, rope=self.rope)
+            a = kv.attention(self.cache, li, batch, q, out_dtype=h.dtype, groups=groups)
+            z.matvec(c.o_type, a, [L.w["attn_output"]], [c.hidden], outs=[h], residuals=[h])
+            a = z.rms_norm(h, eps, L.ffn_norm)
+            a = z.matvec_glu(z.GLU_SWIGLU, c.ffn_type, a, L.w["ffn_gate"], L.w["ffn_up"], c.ffn)
+            z.matvec(c.down_type, a, [L.w["ffn_down"]], [c.hidden], outs=[h], residuals=[h])
+        return h
+
+    def prompt(self, tokens) -> None:
+        """A prompt (int32, at least one token) into slot 0, up to 16 tokens at a time, the others its forks; its last
+        token is left to the first step, whose rows all begin with it."""
+        kv.assign(self.cache, self.slots, self._i32([-1] * self.answers), self._i32([0] * self.answers))
+        for t0 in range(0, len(tokens) - 1, 16):
+            piece = tokens[t0:min(t0 + 16, len(tokens) - 1)]
+            n = len(piece)
+            kv.assign(self.cache, self.slots[:1], self.slots[:1], self._i32([n]))
+            self._run(piece, kv.Batch(self._i32([0, n]), n, n, self.max_len), None)
+        if self.answers > 1:
+            kv.assign(self.cache, self.slots[1:], self._i32([0] * (self.answers - 1)), self._i32([0] * (self.answers - 1)))
+        self.tokens.fill_(tokens[-1])
+
+    def step(self):
+        """One token more of every answer: self.tokens become the next ones, drawn by self.u."""
+        kv.assign(self.cache, self.slots, self.slots, self.one)
+        h = self._run(self.tokens, self.batch, self.groups)
+        logits, = z.matvec(self.cfg.qkv_type, z.rms_norm(h, 1e-6, self.out_norm), [self.logits_w], [self.vocab])
+        sampling.sample(logits, self.u, self.temperature, self.top_k, self.top_p, self.min_p, probs=self.probs, out=self.tokens)
+        return self.tokens
