@@ -81,6 +81,16 @@ template <int TYPE> struct quant_nibbles {
             }
         }
     }
+    static constexpr int WORDS = 4;
+    static __device__ void packed(const raw & r, uint32_t w[1][4]) { words(r.q, w[0]); }
+    static __device__ void eight(const uint32_t w[1][4], int chunk, int, uint32_t & low, uint32_t & high) {
+        if constexpr (TYPE == ZEST_TYPE_Q4_0) {
+            const uint32_t s = w[0][chunk] ^ 0x88888888u;
+            low = s << 4 & 0xf0f0f0f0u, high = s & 0xf0f0f0f0u;
+        } else {
+            low = iq4_levels(w[0][chunk], false), high = iq4_levels(w[0][chunk], true);
+        }
+    }
     static __device__ block_scales<1> scales(const raw & r, int) { return {{half_to_float(r.d) * (TYPE == ZEST_TYPE_Q4_0 ? 0.0625f : 1.0f)}, {0.0f}}; }
 };
 template <> struct quant<ZEST_TYPE_Q4_0> : quant_nibbles<ZEST_TYPE_Q4_0> {};
@@ -104,6 +114,11 @@ template <> struct quant<ZEST_TYPE_Q4_1> {
             c[0][1][i] = w[i] >> 4 & 0x0f0f0f0fu;
         }
     }
+    static constexpr int WORDS = 4;
+    static __device__ void packed(const raw & r, uint32_t w[1][4]) { words(r.q, w[0]); }
+    static __device__ void eight(const uint32_t w[1][4], int chunk, int, uint32_t & low, uint32_t & high) {
+        low = w[0][chunk] & 0x0f0f0f0fu, high = w[0][chunk] >> 4 & 0x0f0f0f0fu;
+    }
     static __device__ block_scales<1> scales(const raw & r, int) { return {{half_to_float(r.dm)}, {half_to_float(r.dm >> 16)}}; }
 };
 
@@ -120,6 +135,12 @@ template <> struct quant<ZEST_TYPE_Q8_0> {
         words(r.q[0], c[0][0]);
         words(r.q[1], c[0][1]);
     }
+    static constexpr int WORDS = 8;
+    static __device__ void packed(const raw & r, uint32_t w[2][4]) {
+        words(r.q[0], w[0]);
+        words(r.q[1], w[1]);
+    }
+    static __device__ void eight(const uint32_t w[2][4], int chunk, int, uint32_t & low, uint32_t & high) { low = w[0][chunk], high = w[1][chunk]; }
     static __device__ block_scales<1> scales(const raw & r, int) { return {{half_to_float(r.d)}, {0.0f}}; }
 };
 
@@ -147,6 +168,14 @@ template <> struct quant<ZEST_TYPE_Q4_K> {
             }
         }
     }
+    static constexpr int WORDS = 8;
+    static __device__ void packed(const raw & r, uint32_t w[2][4]) {
+        words(r.q[0], w[0]);
+        words(r.q[1], w[1]);
+    }
+    static __device__ void eight(const uint32_t w[2][4], int chunk, int block, uint32_t & low, uint32_t & high) {
+        low = w[0][chunk] >> 4 * block & 0x0f0f0f0fu, high = w[1][chunk] >> 4 * block & 0x0f0f0f0fu;
+    }
     static __device__ block_scales<2> scales(const raw & r, int chunk) {
         const float d = half_to_float(r.head.x), dmin = half_to_float(r.head.x >> 16);
         // the first four blocks' fields are low 6 bits, the others' 4 bits and the first's top two
@@ -170,6 +199,9 @@ template <> struct quant<ZEST_TYPE_IQ4_XS> {
         return {load_as<uint4>(p + 8 + (chunk & 7) * 16), *reinterpret_cast<const uint2 *>(p)};
     }
     static __device__ void codes(const raw & r, uint32_t c[1][2][4]) { quant<ZEST_TYPE_IQ4_NL>::codes({r.q, 0}, c); }
+    static constexpr int WORDS = 4;
+    static __device__ void packed(const raw & r, uint32_t w[1][4]) { words(r.q, w[0]); }
+    static __device__ void eight(const uint32_t w[1][4], int chunk, int, uint32_t & low, uint32_t & high) { quant<ZEST_TYPE_IQ4_NL>::eight(w, chunk, 0, low, high); }
     static __device__ block_scales<1> scales(const raw & r, int chunk) {
         const int s = chunk & 7, ls = (r.head.y >> 4 * s & 15) | (r.head.x >> (16 + 2 * s) & 3) << 4;
         return {{half_to_float(r.head.x) * (float) (ls - 32)}, {0.0f}};
@@ -248,33 +280,27 @@ __device__ inline prepared prepare(float4 f) {
     return r;
 }
 
-// A thread's share of the values of all rows, four at a time in the order [block][row][8]:
-// item i of `items`, several requested together.
-__device__ inline void prepare_all(const matvec_args & a, int first, int by, uint8_t * cells) {
-    constexpr int AT_ONCE = 4;
-    const int items = a.blocks * a.M * 8;
-    for (int i0 = first; i0 < items; i0 += AT_ONCE * by) {  // (a block's eight lanes go in step)
-        float4 f[AT_ONCE];
+// Cells in global memory: a stream's, of a block and a row, or (of TILE bytes) a tile's, of
+// a block for MAX_M rows of x: [digit][lane group][row][8 bytes], the rows' factors, and
+// their sums where the type has offsets. A lane group's 8 bytes are the digits of values
+// 4g..4g+3 and 16+4g..16+4g+3. (Rows of a tile from M on hold anything; nothing is made of them.)
+template <int BYTES> __global__ __launch_bounds__(256) void prepare_kernel(matvec_args a) {
+    const int items = a.blocks * a.M * 8, by = gridDim.x * 256;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < items; i += by) {  // (a block's eight lanes go in step)
+        const int cell = i >> 3, block = cell / a.M, m = cell - block * a.M, j = i & 7;
+        const prepared r = prepare(*reinterpret_cast<const float4 *>(a.x + m * a.ldx + block * 32 + j * 4));
+        uint8_t * const to = a.cells + (int64_t) (BYTES == CELL ? cell : block) * BYTES;
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; u++) {
-            const int i = i0 + u * by, cell = i >> 3, block = cell / a.M, m = cell - block * a.M;
-            if (i < items) f[u] = *reinterpret_cast<const float4 *>(a.x + m * a.ldx + block * 32 + (i & 7) * 4);
-        }
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; u++) {
-            const int i = i0 + u * by;
-            if (i >= items) continue;
-            const prepared r = prepare(f[u]);
-            const int j = i & 7;
-            uint8_t * cell = cells + (int64_t) (i >> 3) * CELL;
-#pragma unroll
-            for (int d = 0; d < 3; d++) *reinterpret_cast<uint32_t *>(cell + (j >> 2) * 48 + d * 16 + (j & 3) * 4) = r.digits[d];
-            if (j == 0) *reinterpret_cast<float2 *>(cell + 96) = make_float2(r.factor, r.sum);
+        for (int d = 0; d < 3; d++) *reinterpret_cast<uint32_t *>(to + (BYTES == CELL ? (j >> 2) * 48 + d * 16 + (j & 3) * 4 : d * 512 + (j & 3) * 128 + m * 8 + (j >> 2) * 4)) = r.digits[d];
+        if (j) continue;
+        if constexpr (BYTES == CELL) {
+            *reinterpret_cast<float2 *>(to + 96) = make_float2(r.factor, r.sum);
+        } else {
+            *reinterpret_cast<float *>(to + 1536 + m * 4) = r.factor;
+            if (BYTES > 1600) *reinterpret_cast<float *>(to + 1600 + m * 4) = r.sum;
         }
     }
 }
-
-__global__ __launch_bounds__(256) void prepare_kernel(matvec_args a) { prepare_all(a, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, a.cells); }
 
 // Entry i of an argument's list, by selection among scalar registers: an index that
 // differs between lanes would be a load of the arguments' memory each time, to which
@@ -290,11 +316,11 @@ template <typename V> __device__ inline V pick(const V (&list)[MAX_N], int i) {
     return v;
 }
 
-// The rows of a tile: of a weight, or of a GLU's gate and up.
-struct tile_rows {
-    int32_t weight, row0;
+// A tile: its weight (a GLU's gate and up are one) and its number there.
+struct tile_place {
+    int32_t weight, number;
 };
-__device__ inline tile_rows tile_of(const matvec_args & a, int tile) {
+__device__ inline tile_place tile_of(const matvec_args & a, int tile) {
     int weight = 0, before = 0;
 #pragma unroll
     for (int k = 0; k < MAX_N - 1; k++) {
@@ -302,7 +328,7 @@ __device__ inline tile_rows tile_of(const matvec_args & a, int tile) {
         weight = past ? k + 1 : weight;
         before = past ? a.tiles[k] : before;
     }
-    return {weight, (tile - before) * 16};
+    return {weight, tile - before};
 }
 
 // What becomes of the sums v (S of them, a GLU's gate and up) of a weight's row and row
@@ -315,29 +341,47 @@ template <int S> __device__ inline void store_row(const matvec_args & a, int wei
     y[m * pick(a.ldy, weight) + row] = out;
 }
 
-// A tile is 16 rows of a weight (S = 2: of a GLU's two), a step four chunks of them:
-// a lane loads one chunk of one row (lane l: row l % 16, chunk l / 16), and
-// v_mfma_i32_16x16x64_i8 multiplies the 16 codes of a part that each lane holds with
-// the three digits of a row of x for its own chunk: the first operand's row 4 b + i is
-// digit i of lane group b's chunk, and zero in the other groups' places, so that lane
-// (row, b) of the result holds its own chunk's three sums in its first three
-// registers. Scales are then one value a lane, and a block costs a lane a conversion
-// and a few fused products for a row of x.
+// ---- up to 16 rows of x, tile by tile -------------------------------------------------
+
+// The four lane groups' values of four words as a 4 x 4 matrix, transposed: w[c] becomes,
+// in group g, what group c's word g was.
+__device__ inline void transpose(uint32_t w[4]) {
+    const auto p = __builtin_amdgcn_permlane16_swap(w[0], w[1], false, false), q = __builtin_amdgcn_permlane16_swap(w[2], w[3], false, false);
+    const auto even = __builtin_amdgcn_permlane32_swap(p[0], q[0], false, false), odd = __builtin_amdgcn_permlane32_swap(p[1], q[1], false, false);
+    w[0] = even[0], w[1] = odd[0], w[2] = even[1], w[3] = odd[1];
+}
+// Every group's value, in all of them.
+__device__ inline void gather(float v, float out[4]) {
+    const uint32_t u = __float_as_uint(v);
+    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const auto even = __builtin_amdgcn_permlane32_swap(p[0], p[0], false, false), odd = __builtin_amdgcn_permlane32_swap(p[1], p[1], false, false);
+    out[0] = __uint_as_float(even[0]), out[1] = __uint_as_float(odd[0]), out[2] = __uint_as_float(even[1]), out[3] = __uint_as_float(odd[1]);
+}
+
+template <int TYPE> constexpr int TILE_CELL = quant<TYPE>::OFFSETS ? 1664 : 1600;
+
+// A tile is 16 rows of a weight (H = 2: 32, or with S = 2 a GLU's gate and up), a step four
+// chunks of them. A lane loads one chunk of one row (lane l: row l % 16, chunk l / 16),
+// 16 bytes or more at a time; a transposition among the four lane groups then gives each of
+// them its eight values of every block, which is what v_mfma_i32_16x16x32_i8 takes of a
+// block of 16 rows, and the scales go to all groups. Three products, one a digit of x, give
+// the 16 rows' sums with all rows of x: a lane has those of its weight row and four rows of
+// x, and puts the digits together and to its fp32 sums by scale and factor.
 //
-// HBM bound: a weight's bytes once. The waves of a tile (a.wk of them) each take a run
-// of its steps and are joined in shared memory; AHEAD steps of a wave are in flight
-// while it computes the AHEAD before them.
-template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) void matvec_kernel(matvec_args a) {
+// x's cells lie in shared memory, all of K's or a segment's. The waves of a tile (a.wk of
+// them) each take a run of its steps; AHEAD steps of a wave are in flight while it computes
+// the AHEAD before them, and the waves' sums are joined in shared memory.
+template <int TYPE, int H, int S> __global__ __launch_bounds__(1024) void matvec_kernel(matvec_args a) {
     typedef quant<TYPE> Q;
     typedef int i32x4 __attribute__((ext_vector_type(4)));
-    constexpr int B = Q::BLOCKS, AHEAD = 4 / (S * B);
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    constexpr int B = Q::BLOCKS, AHEAD = 16 / (H * Q::WORDS), ROWS = S == 2 ? 16 : 16 * H, CELLS = TILE_CELL<TYPE>;
     extern __shared__ __align__(16) uint8_t sh[];
-    // sh: 16 zeros, the cells of a segment, the waves' results
+    // sh: the cells of a segment, the waves' results
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 4, col = lane & 15;
     const int wr = wave / a.wk, wk = wave - wr * a.wk;
-    const int M = a.M, steps = (a.chunks + GROUPS - 1) / GROUPS, segs = COPY ? a.segs : 1, seg_steps = COPY ? a.seg_steps : steps;
-    uint8_t * const cells = sh + 16;
-    float * const red = reinterpret_cast<float *>(cells + min(seg_steps * GROUPS, a.chunks) * B * M * CELL);
+    const int steps = (a.chunks + GROUPS - 1) / GROUPS, segs = a.segs, seg_steps = a.seg_steps;
+    f32x4 * const red = reinterpret_cast<f32x4 *>(sh + min(seg_steps * GROUPS, a.chunks) * B * CELLS);
     const int wg_tiles = (a.all_tiles + a.wr - 1) / a.wr, rounds = (wg_tiles - (int) blockIdx.x + gridDim.x - 1) / gridDim.x;
 
     // A block of this wave's steps: of round `round` and segment `seg`, from step `at` of
@@ -355,73 +399,79 @@ template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) 
         return p.seg + 1 < segs ? start(p.round, p.seg + 1) : start(p.round + 1, 0);
     };
     auto tile_at = [&](int round) { return ((int) blockIdx.x + round * (int) gridDim.x) * a.wr + wr; };
-    auto load = [&](typename Q::raw (&buf)[AHEAD][S], place p) {
+    auto load = [&](typename Q::raw (&buf)[AHEAD][H], place p) {
         if (p.round >= rounds) return;
         const int tile = tile_at(p.round);
         if (tile >= a.all_tiles) return;
-        const tile_rows t = tile_of(a, tile);
-        const int row = min(t.row0 + col, pick(a.N, t.weight) - 1);
-        const uint8_t * at[S];
+        const tile_place t = tile_of(a, tile);
+        const int last = pick(a.N, t.weight) - 1;
+        const uint8_t * at[H];
 #pragma unroll
-        for (int s = 0; s < S; s++) at[s] = (S == 2 ? a.w[s] : pick(a.w, t.weight)) + row * a.row_bytes;
+        for (int h = 0; h < H; h++)
+            at[h] = (S == 2 ? a.w[h] : pick(a.w, t.weight)) + (int64_t) min(t.number * ROWS + (S == 2 ? 0 : h * 16) + col, last) * a.row_bytes;
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             if (p.at + i >= p.end) continue;
             const int chunk = min((p.seg * seg_steps + p.at + i) * GROUPS + group, a.chunks - 1);
 #pragma unroll
-            for (int s = 0; s < S; s++) buf[i][s] = Q::load(at[s], chunk);
+            for (int h = 0; h < H; h++) buf[i][h] = Q::load(at[h], chunk);
         }
     };
 
-    float acc[T][S];
+    float acc[H][4];
     auto clear = [&]() {
 #pragma unroll
-        for (int m = 0; m < T; m++)
+        for (int h = 0; h < H; h++)
 #pragma unroll
-            for (int s = 0; s < S; s++) acc[m][s] = 0.0f;
+            for (int r = 0; r < 4; r++) acc[h][r] = 0.0f;
     };
-    // this lane's part of the first operand: digit col % 4 of its group's chunk, if its
-    // row is the group's, else zeros
-    const bool digit = (col >> 2) == group && (col & 3) < 3;
-    auto compute = [&](const typename Q::raw (&buf)[AHEAD][S], place p) {
+    auto compute = [&](const typename Q::raw (&buf)[AHEAD][H], place p) {
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             if (p.at + i >= p.end) continue;
-            const int chunk = (p.seg * seg_steps + p.at + i) * GROUPS + group;
-            const bool in = chunk < a.chunks;
-            i32x4 code[S][B][2];
-            block_scales<B> sc[S];
+            const int chunk0 = (p.seg * seg_steps + p.at + i) * GROUPS;  // group 0's
+            uint32_t w[H][Q::WORDS / 4][4];
+            float scale[H][B][4], offset[H][B][4];
 #pragma unroll
-            for (int s = 0; s < S; s++) {
-                uint32_t c[B][2][4];
-                Q::codes(buf[i][s], c);
-                sc[s] = Q::scales(buf[i][s], min(chunk, a.chunks - 1));
+            for (int h = 0; h < H; h++) {
+                Q::packed(buf[i][h], w[h]);
+#pragma unroll
+                for (int q = 0; q < Q::WORDS / 4; q++) transpose(w[h][q]);
+                // (past the row's end: any bytes, by a scale of 0)
+                const bool in = chunk0 + group < a.chunks;
+                const block_scales<B> sc = Q::scales(buf[i][h], min(chunk0 + group, a.chunks - 1));
 #pragma unroll
                 for (int b = 0; b < B; b++) {
-#pragma unroll
-                    for (int h = 0; h < 2; h++) code[s][b][h] = i32x4{(int) c[b][h][0], (int) c[b][h][1], (int) c[b][h][2], (int) c[b][h][3]};
-                    if (!in) sc[s].scale[b] = sc[s].offset[b] = 0.0f;
+                    gather(in ? sc.scale[b] : 0.0f, scale[h][b]);
+                    if constexpr (Q::OFFSETS) gather(in ? sc.offset[b] : 0.0f, offset[h][b]);
                 }
             }
-            const uint8_t * cell = cells + ((p.at + i) * GROUPS + (in ? group : 0)) * B * M * CELL;
-            const uint8_t * from = digit && in ? cell + (col & 3) * 16 : sh;
-            const int stride = digit && in ? CELL : 0, part = digit && in ? 48 : 0;
 #pragma unroll
-            for (int m = 0; m < T; m++) {
-                if (m >= M) continue;
+            for (int c = 0; c < GROUPS; c++) {
+                const uint8_t * cell = sh + (min(chunk0 + c, a.chunks - 1) - p.seg * seg_steps * GROUPS) * (B * CELLS);
 #pragma unroll
                 for (int b = 0; b < B; b++) {
-                    const i32x4 x0 = *reinterpret_cast<const i32x4 *>(from + (b * M + m) * stride);
-                    const i32x4 x1 = *reinterpret_cast<const i32x4 *>(from + (b * M + m) * stride + part);
-                    const float2 f = *reinterpret_cast<const float2 *>(cell + (b * M + m) * CELL + 96);  // the factor and the sum
+                    long x[3];
 #pragma unroll
-                    for (int s = 0; s < S; s++) {
-                        i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x0, code[s][b][0], i32x4{}, 0, 0, 0);
-                        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x1, code[s][b][1], d, 0, 0, 0);
-                        // (|d0| <= 64 15 32 < 2^15 for nibbles, so they fit in 32 bits together)
-                        const float v = Q::NIBBLES ? (float) ((((d[0] << 8) + d[1]) << 8) + d[2]) : fmaf((float) d[0], 65536.0f, (float) ((d[1] << 8) + d[2]));
-                        acc[m][s] = fmaf(v, sc[s].scale[b] * f.x, acc[m][s]);
-                        if constexpr (Q::OFFSETS) acc[m][s] = fmaf(f.y, sc[s].offset[b], acc[m][s]);
+                    for (int d = 0; d < 3; d++) x[d] = *reinterpret_cast<const long *>(cell + b * CELLS + d * 512 + lane * 8);
+                    const f32x4 f = *reinterpret_cast<const f32x4 *>(cell + b * CELLS + 1536 + group * 16);
+                    f32x4 sum{};
+                    if constexpr (Q::OFFSETS) sum = *reinterpret_cast<const f32x4 *>(cell + b * CELLS + 1600 + group * 16);
+#pragma unroll
+                    for (int h = 0; h < H; h++) {
+                        uint32_t low, high;  // the values' first and second half
+                        Q::eight(w[h], c, b, low, high);
+                        const long code = (long) ((uint64_t) high << 32 | low);
+                        i32x4 d[3];
+#pragma unroll
+                        for (int k = 0; k < 3; k++) d[k] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x[k], code, i32x4{}, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            // (|d0| <= 64 15 32 < 2^15 for nibbles, so they fit in 32 bits together)
+                            const float v = Q::NIBBLES ? (float) ((((d[0][r] << 8) + d[1][r]) << 8) + d[2][r]) : fmaf((float) d[0][r], 65536.0f, (float) ((d[1][r] << 8) + d[2][r]));
+                            acc[h][r] = fmaf(v, scale[h][b][c] * f[r], acc[h][r]);
+                            if constexpr (Q::OFFSETS) acc[h][r] = fmaf(sum[r], offset[h][b][c], acc[h][r]);
+                        }
                     }
                 }
             }
@@ -429,45 +479,44 @@ template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) 
     };
     // the cells of a segment, in shared memory
     auto fill = [&](int seg) {
-        if (threadIdx.x < 4) reinterpret_cast<uint32_t *>(sh)[threadIdx.x] = 0;
-        if constexpr (COPY) {
-            const int first = seg * seg_steps * GROUPS * B, n = min(seg_steps * GROUPS * B, a.blocks - first) * M * (CELL / 16);
-            const uint4 * from = reinterpret_cast<const uint4 *>(a.cells + (int64_t) first * M * CELL);
-            for (int i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<uint4 *>(cells)[i] = from[i];
-        } else {
-            prepare_all(a, threadIdx.x, blockDim.x, cells);
-        }
+        const int first = seg * seg_steps * GROUPS * B, n = min(seg_steps * GROUPS * B, a.blocks - first) * (CELLS / 16);
+        const uint4 * from = reinterpret_cast<const uint4 *>(a.cells + (int64_t) first * CELLS);
+        for (int i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<uint4 *>(sh)[i] = from[i];
         __syncthreads();
     };
-    // the waves' sums of a round's tiles: of the lane groups, then of the waves
+    // a round's tiles: the first wave of each adds the others' sums to its own
     auto finish = [&](int round) {
-        float * const mine = red + wave * T * S * 16;
+        const int others = a.wk - 1, tile = tile_at(round);
+        if (wk) {
 #pragma unroll
-        for (int m = 0; m < T; m++) {
-            if (m >= M) continue;
+            for (int h = 0; h < H; h++) red[((wr * others + wk - 1) * H + h) * 64 + lane] = f32x4{acc[h][0], acc[h][1], acc[h][2], acc[h][3]};
+        }
+        if (others) __syncthreads();
+        if (wk == 0 && tile < a.all_tiles) {
 #pragma unroll
-            for (int s = 0; s < S; s++) {
-                const float v = over_groups(acc[m][s]);
-                if (group == 0) mine[(m * S + s) * 16 + col] = v;
+            for (int h = 0; h < H; h++)
+                for (int k = 0; k < others; k++) {
+                    const f32x4 v = red[((wr * others + k) * H + h) * 64 + lane];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[h][r] += v[r];
+                }
+            const tile_place t = tile_of(a, tile);
+#pragma unroll
+            for (int h = 0; h < H / S; h++) {
+                const int row = t.number * ROWS + h * 16 + col;
+                if (row >= pick(a.N, t.weight)) continue;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    if (group * 4 + r >= a.M) continue;
+                    const float v[2] = {acc[h][r], acc[S == 2 ? 1 : h][r]};
+                    store_row<S>(a, t.weight, row, group * 4 + r, v);
+                }
             }
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < a.wr * M * 16; i += blockDim.x) {
-            const int c = i & 15, m = (i >> 4) % M, r = (i >> 4) / M, tile = ((int) blockIdx.x + round * (int) gridDim.x) * a.wr + r;
-            if (tile >= a.all_tiles) continue;
-            float v[S];
-#pragma unroll
-            for (int s = 0; s < S; s++) {
-                v[s] = 0.0f;
-                for (int w = 0; w < a.wk; w++) v[s] += red[((r * a.wk + w) * T * S + m * S + s) * 16 + c];
-            }
-            const tile_rows t = tile_of(a, tile);
-            if (t.row0 + c < pick(a.N, t.weight)) store_row<S>(a, t.weight, t.row0 + c, m, v);
-        }
-        __syncthreads();
+        if (others) __syncthreads();
     };
     // one block: the next one requested, this one computed; what follows it
-    auto turn = [&](typename Q::raw (&now)[AHEAD][S], typename Q::raw (&then)[AHEAD][S], place p, bool first) {
+    auto turn = [&](typename Q::raw (&now)[AHEAD][H], typename Q::raw (&then)[AHEAD][H], place p, bool first) {
         const place q = next(p);
         if (first) {  // of a segment
             if (p.seg == 0) clear();
@@ -481,7 +530,7 @@ template <int TYPE, int T, int S, bool COPY> __global__ __launch_bounds__(1024) 
         if (q.round != p.round) finish(p.round);
         return q;
     };
-    typename Q::raw one[AHEAD][S], two[AHEAD][S];
+    typename Q::raw one[AHEAD][H], two[AHEAD][H];
     place p = start(0, 0);
     bool first = true;
     load(one, p);
@@ -602,9 +651,15 @@ __device__ inline call_row row_of(const matvec_args & a, int r) {
     return {weight, r - before};
 }
 
-// The products as matvec_kernel's, the weights' bytes by another way: not chunk by chunk
-// into registers, where an instruction touches 16 lines or more and a line is asked for
-// three times, but as whole granules of contiguous bytes straight into shared memory:
+// v_mfma_i32_16x16x64_i8 multiplies the 16 codes of a part that each lane holds of its own
+// chunk (lane l: row l % 16, chunk l / 16 of a step) with the three digits of a row of x for
+// that chunk: the first operand's row 4 b + i is digit i of lane group b's chunk, and zero
+// in the other groups' places, so that lane (row, b) of the result holds its own chunk's
+// three sums in its first three registers. Scales are then one value a lane, and a block
+// costs a lane a conversion and a few fused products for a row of x.
+//
+// HBM bound: a weight's bytes once. They come not chunk by chunk into registers, where an
+// instruction touches 16 lines or more and a line is asked for three times, but as whole granules of contiguous bytes straight into shared memory:
 // RING pieces (two units of 16 rows, 4.6 KB) a wave, requested as soon as their place
 // is read. A workgroup's last 16 rows are as many as are left of its share: a row that
 // is not there is its neighbour again. So all CUs stream whatever the number of rows.
@@ -865,7 +920,7 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) __attribute__((amdgpu_waves_per_
 
 struct matvec_plan {
     int ring;             // of stream_kernel; 0: matvec_kernel
-    int wk, wr, workgroups, seg_steps, segs, pieces;
+    int wk, wr, height, workgroups, seg_steps, segs, pieces;
     bool copy;            // x is prepared by a kernel of its own
     size_t lds, bytes;
 };
@@ -893,9 +948,7 @@ constexpr int STREAM_ROWS = 512;  // of a workgroup at most
 
 matvec_plan plan_of(int type, int64_t M, int64_t K, int n, const int64_t * N, bool glu) {
     matvec_plan p{};
-    const int B = type == ZEST_TYPE_Q4_K ? 2 : 1, chunks = (int) (K / 32 / B), steps = (chunks + GROUPS - 1) / GROUPS, T = M <= 4 ? 4 : M <= 8 ? 8 : 16, S = glu ? 2 : 1;
-    int64_t tiles = 0;
-    for (int i = 0; i < (glu ? 1 : n); i++) tiles += (N[i] + 15) / 16;
+    const int B = type == ZEST_TYPE_Q4_K ? 2 : 1, chunks = (int) (K / 32 / B), steps = (chunks + GROUPS - 1) / GROUPS, S = glu ? 2 : 1;
     if (M <= 4) {
         const stream_sizes z = glu ? sizes_of<2>(type, chunks) : sizes_of<1>(type, chunks);
         int64_t rows = 0;
@@ -916,19 +969,24 @@ matvec_plan plan_of(int type, int64_t M, int64_t K, int n, const int64_t * N, bo
             }
         p.ring = 0;
     }
-    p.wr = tiles <= 2 * 256 ? 1 : tiles <= 8 * 256 ? 2 : 4;
-    const int most = p.wr == 1 && tiles > 256 ? 8 : 16 / p.wr;
+    // 32 rows a tile where there are enough of them: x is read from shared memory half as often
+    int64_t wide = 0, narrow = 0;
+    for (int i = 0; i < (glu ? 1 : n); i++) wide += (N[i] + 31) / 32, narrow += (N[i] + 15) / 16;
+    p.height = glu || wide > 4 * CUS ? 2 : 1;
+    const int64_t tiles = glu || p.height == 1 ? narrow : wide;
+    p.wr = tiles <= 2 * CUS ? 1 : tiles <= 8 * CUS ? 2 : 4;
+    const int most = p.wr == 1 && tiles > CUS ? 8 : 16 / p.wr;
     p.wk = 1;
     for (int w = 1; w <= most; w++)
         if ((steps + w - 1) / w < (steps + p.wk - 1) / p.wk) p.wk = w;
-    const size_t red = (size_t) p.wk * p.wr * T * S * 16 * 4, room = LDS_MOST - 16 - red;
-    p.seg_steps = (int) std::min<size_t>(steps, room / ((size_t) GROUPS * B * M * CELL));
+    const size_t cell = type == ZEST_TYPE_Q4_K || type == ZEST_TYPE_Q4_1 ? 1664 : 1600, red = (size_t) (p.wk - 1) * p.wr * p.height * 1024;
+    p.seg_steps = (int) std::min<size_t>(steps, (LDS_MOST - red) / ((size_t) GROUPS * B * cell));
     p.segs = (steps + p.seg_steps - 1) / p.seg_steps;
     p.copy = true;
-    p.lds = 16 + (size_t) std::min(p.seg_steps * GROUPS, chunks) * B * M * CELL + red;
-    p.workgroups = (int) std::min<int64_t>((tiles + p.wr - 1) / p.wr, 512);
-    if (p.lds > LDS_MOST / 2 || p.wk * p.wr > 8) p.workgroups = std::min(p.workgroups, 256);
-    p.bytes = (size_t) chunks * B * M * CELL;
+    p.lds = (size_t) std::min(p.seg_steps * GROUPS, chunks) * B * cell + red;
+    p.workgroups = (int) std::min<int64_t>((tiles + p.wr - 1) / p.wr, 2 * CUS);
+    if (p.lds > LDS_MOST / 2 || p.wk * p.wr > 8) p.workgroups = std::min(p.workgroups, CUS);
+    p.bytes = (size_t) chunks * B * cell;
     return p;
 }
 
@@ -960,20 +1018,20 @@ template <auto KERNEL> int allow_lds(const char * me) {
     return ZEST_OK;
 }
 
-void launch_prepare(const matvec_args & a, hipStream_t s) {
-    hipLaunchKernelGGL(prepare_kernel, dim3((unsigned) std::min<int64_t>(((int64_t) a.blocks * a.M * 8 + 255) / 256, 1024)), dim3(256), 0, s, a);
+template <int BYTES> void launch_prepare(const matvec_args & a, hipStream_t s) {
+    hipLaunchKernelGGL(prepare_kernel<BYTES>, dim3((unsigned) std::min<int64_t>(((int64_t) a.blocks * a.M * 8 + 255) / 256, 1024)), dim3(256), 0, s, a);
 }
 
-template <int TYPE, int T, int S, bool COPY> int launch(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
-    if (const int st = allow_lds<&matvec_kernel<TYPE, T, S, COPY>>(me)) return st;
-    if (COPY) launch_prepare(a, s);
-    hipLaunchKernelGGL((matvec_kernel<TYPE, T, S, COPY>), dim3((unsigned) p.workgroups), dim3((unsigned) (p.wk * p.wr * 64)), p.lds, s, a);
+template <int TYPE, int H, int S> int launch(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
+    if (const int st = allow_lds<&matvec_kernel<TYPE, H, S>>(me)) return st;
+    launch_prepare<TILE_CELL<TYPE>>(a, s);
+    hipLaunchKernelGGL((matvec_kernel<TYPE, H, S>), dim3((unsigned) p.workgroups), dim3((unsigned) (p.wk * p.wr * 64)), p.lds, s, a);
     return zest::check_launch(me);
 }
 
 template <int TYPE, int M, int S, int RING, bool READY> int launch_stream(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
     if (const int st = allow_lds<&stream_kernel<TYPE, M, S, RING, READY>>(me)) return st;
-    if (READY) launch_prepare(a, s);
+    if (READY) launch_prepare<CELL>(a, s);
     hipLaunchKernelGGL((stream_kernel<TYPE, M, S, RING, READY>), dim3((unsigned) p.workgroups), dim3(STREAM_WAVES * 64), p.lds, s, a);
     return zest::check_launch(me);
 }
@@ -988,9 +1046,9 @@ template <int TYPE, int S> int launch(const matvec_args & a, const matvec_plan &
         if (a.M > 2) return a.M > 3 ? launch_stream<TYPE, 4, S>(a, p, s, me) : launch_stream<TYPE, 3, S>(a, p, s, me);
         return a.M > 1 ? launch_stream<TYPE, 2, S>(a, p, s, me) : launch_stream<TYPE, 1, S>(a, p, s, me);
     }
-    if (a.M > 8) return launch<TYPE, 16, S, true>(a, p, s, me);
-    if (a.M > 4) return launch<TYPE, 8, S, true>(a, p, s, me);
-    return launch<TYPE, 4, S, true>(a, p, s, me);
+    if constexpr (S == 1)
+        if (p.height == 1) return launch<TYPE, 1, 1>(a, p, s, me);
+    return launch<TYPE, 2, S>(a, p, s, me);
 }
 
 template <int TYPE> int launch(const matvec_args & a, const matvec_plan & p, hipStream_t s, const char * me) {
@@ -1028,14 +1086,14 @@ int matvec(const char * me, int glu, int type, const float * x, int64_t M, int64
     a.chunks = a.blocks / (type == ZEST_TYPE_Q4_K ? 2 : 1);
     a.n = outs;
     a.glu = glu;
-    int64_t tiles = 0, rows = 0;
+    int64_t rows = 0;
     for (int i = 0; i < n; i++) {
         ZEST_REQUIRE(w[i] && aligned(w[i], row_align(type)), "%s: weight %d: rows %d-byte aligned wanted", me, i, row_align(type));
         ZEST_REQUIRE(N[i] > 0 && N[i] <= (1 << 26), "%s: weight %d: N=%lld", me, i, (long long) N[i]);
         a.w[i] = (const uint8_t *) w[i];
         a.N[i] = (int32_t) N[i];
-        if (i < outs) tiles += (N[i] + 15) / 16, rows += N[i];
-        a.tiles[i] = (int32_t) tiles, a.rows[i] = (int32_t) rows;
+        if (i < outs) rows += N[i];
+        a.rows[i] = (int32_t) rows;
     }
     for (int i = 0; i < outs; i++) {
         ZEST_REQUIRE(y[i] && aligned(y[i], 4) && (M == 1 || (ldy[i] >= N[i] && ldy[i] < (1ll << 31))), "%s: output %d: ldy=%lld for N=%lld", me, i, (long long) (M == 1 ? 0 : ldy[i]),
@@ -1064,7 +1122,8 @@ int matvec(const char * me, int glu, int type, const float * x, int64_t M, int64
     // (a GLU's plan is that of two weights as far as its workspace goes)
     const matvec_plan p = plan_of(type, M, K, n, N, glu >= 0);
     ZEST_REQUIRE(!p.bytes || (workspace && aligned(workspace, 16) && workspace_bytes >= p.bytes), "%s: workspace of %zu bytes, 16-byte aligned, wanted", me, p.bytes);
-    a.all_tiles = (int32_t) tiles;
+    const int tile_rows = glu < 0 && p.height == 2 ? 32 : 16;
+    for (int i = 0; i < outs; i++) a.tiles[i] = a.all_tiles += (int32_t) ((N[i] + tile_rows - 1) / tile_rows);
     a.wk = p.wk, a.wr = p.wr, a.seg_steps = p.seg_steps, a.segs = p.segs;
     a.cells = (uint8_t *) workspace;
     a.pieces = p.pieces, a.each = (int32_t) (rows / p.workgroups), a.more = (int32_t) (rows % p.workgroups);
