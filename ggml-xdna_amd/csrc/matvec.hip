@@ -19,12 +19,27 @@ constexpr int MAX_M = ZEST_MATVEC_MAX_ROWS, MAX_N = ZEST_MATVEC_MAX_GROUP;
 
 __device__ inline float half_to_float(uint32_t h) { return (float) __builtin_bit_cast(_Float16, (uint16_t) h); }
 
-// Bytes of a row that need not be aligned to the load (the hardware takes any).
-template <typename T> __device__ inline T load_as(const uint8_t * p) {
-    T v;
-    __builtin_memcpy(&v, p, sizeof(T));
-    return v;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+__device__ inline uint4 as_uint4(u32x4 v) { return make_uint4(v.x, v.y, v.z, v.w); }
+
+// Words of a row, which need not be aligned to the load (the hardware takes any). By a
+// pointer to global memory: a load by a generic one is waited for with all others.
+typedef const __attribute__((address_space(1))) uint8_t * bytes_t;
+__device__ inline uint4 load_words4(bytes_t p) {
+    typedef u32x4 any __attribute__((aligned(2)));
+    return as_uint4(*(const __attribute__((address_space(1))) any *) p);
 }
+__device__ inline uint2 load_words2(bytes_t p) {
+    typedef u32x2 any __attribute__((aligned(2)));
+    const u32x2 v = *(const __attribute__((address_space(1))) any *) p;
+    return make_uint2(v.x, v.y);
+}
+__device__ inline uint32_t load_word(bytes_t p) {
+    typedef uint32_t any __attribute__((aligned(2)));
+    return *(const __attribute__((address_space(1))) any *) p;
+}
+__device__ inline uint32_t load_half(bytes_t p) { return *(const __attribute__((address_space(1))) uint16_t *) p; }
 
 // The published levels of IQ4_NL and IQ4_XS, for the low or the high nibbles of four
 // bytes: two byte permutes look up the low and the high eight, and a mask that a
@@ -62,9 +77,9 @@ template <int TYPE> struct quant_nibbles {
     struct raw { uint4 q; uint32_t d; };
     static constexpr int BLOCKS = 1;
     static constexpr bool NIBBLES = false, OFFSETS = false;
-    static __device__ raw load(const uint8_t * row, int chunk) {
-        const uint8_t * p = row + chunk * 18;
-        return {load_as<uint4>(p + 2), load_as<uint16_t>(p)};
+    static __device__ raw load(bytes_t row, int chunk) {
+        const bytes_t p = row + chunk * 18;
+        return {load_words4(p + 2), load_half(p)};
     }
     static __device__ void codes(const raw & r, uint32_t c[1][2][4]) {
         uint32_t w[4];
@@ -101,9 +116,9 @@ template <> struct quant<ZEST_TYPE_Q4_1> {
     struct raw { uint4 q; uint32_t dm; };
     static constexpr int BLOCKS = 1;
     static constexpr bool NIBBLES = true, OFFSETS = true;
-    static __device__ raw load(const uint8_t * row, int chunk) {
-        const uint8_t * p = row + chunk * 20;
-        return {load_as<uint4>(p + 4), load_as<uint32_t>(p)};
+    static __device__ raw load(bytes_t row, int chunk) {
+        const bytes_t p = row + chunk * 20;
+        return {load_words4(p + 4), load_word(p)};
     }
     static __device__ void codes(const raw & r, uint32_t c[1][2][4]) {
         uint32_t w[4];
@@ -127,9 +142,9 @@ template <> struct quant<ZEST_TYPE_Q8_0> {
     struct raw { uint4 q[2]; uint32_t d; };
     static constexpr int BLOCKS = 1;
     static constexpr bool NIBBLES = false, OFFSETS = false;
-    static __device__ raw load(const uint8_t * row, int chunk) {
-        const uint8_t * p = row + chunk * 34;
-        return {{load_as<uint4>(p + 2), load_as<uint4>(p + 18)}, load_as<uint16_t>(p)};
+    static __device__ raw load(bytes_t row, int chunk) {
+        const bytes_t p = row + chunk * 34;
+        return {{load_words4(p + 2), load_words4(p + 18)}, load_half(p)};
     }
     static __device__ void codes(const raw & r, uint32_t c[1][2][4]) {
         words(r.q[0], c[0][0]);
@@ -151,10 +166,10 @@ template <> struct quant<ZEST_TYPE_Q4_K> {
     struct raw { uint4 q[2], head; };
     static constexpr int BLOCKS = 2;
     static constexpr bool NIBBLES = true, OFFSETS = true;
-    static __device__ raw load(const uint8_t * row, int chunk) {
-        const uint8_t * p = row + (chunk >> 2) * 144;
-        const uint4 * q = reinterpret_cast<const uint4 *>(p + 16 + (chunk & 3) * 32);
-        return {{q[0], q[1]}, *reinterpret_cast<const uint4 *>(p)};
+    static __device__ raw load(bytes_t row, int chunk) {
+        const bytes_t p = row + (chunk >> 2) * 144;
+        const bytes_t q = p + 16 + (chunk & 3) * 32;
+        return {{load_words4(q), load_words4(q + 16)}, load_words4(p)};
     }
     static __device__ void codes(const raw & r, uint32_t c[2][2][4]) {
 #pragma unroll
@@ -194,9 +209,9 @@ template <> struct quant<ZEST_TYPE_IQ4_XS> {
     struct raw { uint4 q; uint2 head; };
     static constexpr int BLOCKS = 1;
     static constexpr bool NIBBLES = false, OFFSETS = false;
-    static __device__ raw load(const uint8_t * row, int chunk) {
-        const uint8_t * p = row + (chunk >> 3) * 136;
-        return {load_as<uint4>(p + 8 + (chunk & 7) * 16), *reinterpret_cast<const uint2 *>(p)};
+    static __device__ raw load(bytes_t row, int chunk) {
+        const bytes_t p = row + (chunk >> 3) * 136;
+        return {load_words4(p + 8 + (chunk & 7) * 16), load_words2(p)};
     }
     static __device__ void codes(const raw & r, uint32_t c[1][2][4]) { quant<ZEST_TYPE_IQ4_NL>::codes({r.q, 0}, c); }
     static constexpr int WORDS = 4;
@@ -343,45 +358,47 @@ template <int S> __device__ inline void store_row(const matvec_args & a, int wei
 
 // ---- up to 16 rows of x, tile by tile -------------------------------------------------
 
-// The four lane groups' values of four words as a 4 x 4 matrix, transposed: w[c] becomes,
-// in group g, what group c's word g was.
-__device__ inline void transpose(uint32_t w[4]) {
-    const auto p = __builtin_amdgcn_permlane16_swap(w[0], w[1], false, false), q = __builtin_amdgcn_permlane16_swap(w[2], w[3], false, false);
-    const auto even = __builtin_amdgcn_permlane32_swap(p[0], q[0], false, false), odd = __builtin_amdgcn_permlane32_swap(p[1], q[1], false, false);
-    w[0] = even[0], w[1] = odd[0], w[2] = even[1], w[3] = odd[1];
-}
-// Every group's value, in all of them.
-__device__ inline void gather(float v, float out[4]) {
-    const uint32_t u = __float_as_uint(v);
-    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const auto even = __builtin_amdgcn_permlane32_swap(p[0], p[0], false, false), odd = __builtin_amdgcn_permlane32_swap(p[1], p[1], false, false);
-    out[0] = __uint_as_float(even[0]), out[1] = __uint_as_float(odd[0]), out[2] = __uint_as_float(even[1]), out[3] = __uint_as_float(odd[1]);
+// What the lanes of a wave wrote to shared memory, which it serves in order, is read after it.
+__device__ inline void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 template <int TYPE> constexpr int TILE_CELL = quant<TYPE>::OFFSETS ? 1664 : 1600;
+// Words of a weight row's four chunks where they change lanes: codes, scales and offsets, an
+// odd number of fours, so that 16 rows' reads spread over all banks; and a wave's bytes, which
+// hold its sums afterwards.
+template <int TYPE> constexpr int TRADE = (quant<TYPE>::WORDS * 4 + quant<TYPE>::BLOCKS * (quant<TYPE>::OFFSETS ? 8 : 4)) | 4;
+template <int TYPE, int H> constexpr int WAVE_BYTES = TRADE<TYPE> * 64 > H * 1024 ? TRADE<TYPE> * 64 : H * 1024;
 
 // A tile is 16 rows of a weight (H = 2: 32, or with S = 2 a GLU's gate and up), a step four
-// chunks of them. A lane loads one chunk of one row (lane l: row l % 16, chunk l / 16),
-// 16 bytes or more at a time; a transposition among the four lane groups then gives each of
-// them its eight values of every block, which is what v_mfma_i32_16x16x32_i8 takes of a
-// block of 16 rows, and the scales go to all groups. Three products, one a digit of x, give
+// chunks of them. A lane loads one chunk of one row (lane l: row l / 4, chunk l % 4, so that
+// four lanes read consecutive bytes), and the wave trades in its own shared memory: lane (row
+// l % 16, group l / 16) gets its eight values of every block, which is what v_mfma_i32_16x16x32_i8 takes of a block of 16 rows,
+// and all four scales. Three products, one a digit of x, give
 // the 16 rows' sums with all rows of x: a lane has those of its weight row and four rows of
 // x, and puts the digits together and to its fp32 sums by scale and factor.
 //
 // x's cells lie in shared memory, all of K's or a segment's. The waves of a tile (a.wk of
 // them) each take a run of its steps; AHEAD steps of a wave are in flight while it computes
-// the AHEAD before them, and the waves' sums are joined in shared memory.
+// the AHEAD before them (twice as many were slower: 154 us for 115), and the waves' sums are
+// joined in shared memory. 151936 rows of 2560 IQ4_XS by 16: 104 us, of which the loads alone
+// take 76 and the products alone 82; with products of a lane's own 16 codes, a row of x at a
+// time as below, 190.
 template <int TYPE, int H, int S> __global__ __launch_bounds__(1024) void matvec_kernel(matvec_args a) {
     typedef quant<TYPE> Q;
     typedef int i32x4 __attribute__((ext_vector_type(4)));
     typedef float f32x4 __attribute__((ext_vector_type(4)));
     constexpr int B = Q::BLOCKS, AHEAD = 16 / (H * Q::WORDS), ROWS = S == 2 ? 16 : 16 * H, CELLS = TILE_CELL<TYPE>;
     extern __shared__ __align__(16) uint8_t sh[];
-    // sh: the cells of a segment, the waves' results
+    // sh: the cells of a segment, the waves' own
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 4, col = lane & 15;
     const int wr = wave / a.wk, wk = wave - wr * a.wk;
     const int steps = (a.chunks + GROUPS - 1) / GROUPS, segs = a.segs, seg_steps = a.seg_steps;
-    f32x4 * const red = reinterpret_cast<f32x4 *>(sh + min(seg_steps * GROUPS, a.chunks) * B * CELLS);
+    uint8_t * const own = sh + min(seg_steps * GROUPS, a.chunks) * B * CELLS + wave * WAVE_BYTES<TYPE, H>;
+    uint32_t * const to = reinterpret_cast<uint32_t *>(own) + (lane >> 2) * TRADE<TYPE>;
+    const uint32_t * const from = reinterpret_cast<const uint32_t *>(own) + col * TRADE<TYPE>;
     const int wg_tiles = (a.all_tiles + a.wr - 1) / a.wr, rounds = (wg_tiles - (int) blockIdx.x + gridDim.x - 1) / gridDim.x;
 
     // A block of this wave's steps: of round `round` and segment `seg`, from step `at` of
@@ -400,19 +417,16 @@ template <int TYPE, int H, int S> __global__ __launch_bounds__(1024) void matvec
     };
     auto tile_at = [&](int round) { return ((int) blockIdx.x + round * (int) gridDim.x) * a.wr + wr; };
     auto load = [&](typename Q::raw (&buf)[AHEAD][H], place p) {
-        if (p.round >= rounds) return;
-        const int tile = tile_at(p.round);
-        if (tile >= a.all_tiles) return;
-        const tile_place t = tile_of(a, tile);
+        // (every lane loads, whatever there is left to load, so that the loads in flight are known)
+        const tile_place t = tile_of(a, min(tile_at(p.round), a.all_tiles - 1));
         const int last = pick(a.N, t.weight) - 1;
-        const uint8_t * at[H];
+        bytes_t at[H];
 #pragma unroll
         for (int h = 0; h < H; h++)
-            at[h] = (S == 2 ? a.w[h] : pick(a.w, t.weight)) + (int64_t) min(t.number * ROWS + (S == 2 ? 0 : h * 16) + col, last) * a.row_bytes;
+            at[h] = (bytes_t) (S == 2 ? a.w[h] : pick(a.w, t.weight)) + (int64_t) min(t.number * ROWS + (S == 2 ? 0 : h * 16) + (lane >> 2), last) * a.row_bytes;
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
-            if (p.at + i >= p.end) continue;
-            const int chunk = min((p.seg * seg_steps + p.at + i) * GROUPS + group, a.chunks - 1);
+            const int chunk = min((p.seg * seg_steps + min(p.at + i, max(p.end - 1, 0))) * GROUPS + (lane & 3), a.chunks - 1);
 #pragma unroll
             for (int h = 0; h < H; h++) buf[i][h] = Q::load(at[h], chunk);
         }
@@ -431,20 +445,33 @@ template <int TYPE, int H, int S> __global__ __launch_bounds__(1024) void matvec
             if (p.at + i >= p.end) continue;
             const int chunk0 = (p.seg * seg_steps + p.at + i) * GROUPS;  // group 0's
             uint32_t w[H][Q::WORDS / 4][4];
-            float scale[H][B][4], offset[H][B][4];
+            f32x4 scale[H][B], offset[H][B];
 #pragma unroll
             for (int h = 0; h < H; h++) {
-                Q::packed(buf[i][h], w[h]);
-#pragma unroll
-                for (int q = 0; q < Q::WORDS / 4; q++) transpose(w[h][q]);
+                const int c = lane & 3;
+                uint32_t mine[Q::WORDS / 4][4];
+                Q::packed(buf[i][h], mine);
                 // (past the row's end: any bytes, by a scale of 0)
-                const bool in = chunk0 + group < a.chunks;
-                const block_scales<B> sc = Q::scales(buf[i][h], min(chunk0 + group, a.chunks - 1));
+                const bool in = chunk0 + c < a.chunks;
+                const block_scales<B> sc = Q::scales(buf[i][h], min(chunk0 + c, a.chunks - 1));
+#pragma unroll
+                for (int q = 0; q < Q::WORDS / 4; q++) *reinterpret_cast<u32x4 *>(to + q * 16 + c * 4) = u32x4{mine[q][0], mine[q][1], mine[q][2], mine[q][3]};
 #pragma unroll
                 for (int b = 0; b < B; b++) {
-                    gather(in ? sc.scale[b] : 0.0f, scale[h][b]);
-                    if constexpr (Q::OFFSETS) gather(in ? sc.offset[b] : 0.0f, offset[h][b]);
+                    to[Q::WORDS * 4 + b * 4 + c] = __float_as_uint(in ? sc.scale[b] : 0.0f);
+                    if constexpr (Q::OFFSETS) to[Q::WORDS * 4 + (B + b) * 4 + c] = __float_as_uint(in ? sc.offset[b] : 0.0f);
                 }
+                wave_sync();
+#pragma unroll
+                for (int k = 0; k < GROUPS; k++)
+#pragma unroll
+                    for (int q = 0; q < Q::WORDS / 4; q++) w[h][q][k] = from[q * 16 + k * 4 + group];
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    scale[h][b] = *reinterpret_cast<const f32x4 *>(from + Q::WORDS * 4 + b * 4);
+                    if constexpr (Q::OFFSETS) offset[h][b] = *reinterpret_cast<const f32x4 *>(from + Q::WORDS * 4 + (B + b) * 4);
+                }
+                wave_sync();
             }
 #pragma unroll
             for (int c = 0; c < GROUPS; c++) {
@@ -481,39 +508,43 @@ template <int TYPE, int H, int S> __global__ __launch_bounds__(1024) void matvec
     auto fill = [&](int seg) {
         const int first = seg * seg_steps * GROUPS * B, n = min(seg_steps * GROUPS * B, a.blocks - first) * (CELLS / 16);
         const uint4 * from = reinterpret_cast<const uint4 *>(a.cells + (int64_t) first * CELLS);
-        for (int i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<uint4 *>(sh)[i] = from[i];
+        constexpr int AT_ONCE = 9;  // requested together
+        for (int i0 = threadIdx.x; i0 < n; i0 += AT_ONCE * blockDim.x) {
+            uint4 v[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) v[u] = from[min(i0 + u * (int) blockDim.x, n - 1)];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++)
+                if (i0 + u * (int) blockDim.x < n) reinterpret_cast<uint4 *>(sh)[i0 + u * (int) blockDim.x] = v[u];
+        }
         __syncthreads();
     };
-    // a round's tiles: the first wave of each adds the others' sums to its own
+    // a round's tiles: the waves of each share out its sums
     auto finish = [&](int round) {
-        const int others = a.wk - 1, tile = tile_at(round);
-        if (wk) {
+        const int tile = tile_at(round);
 #pragma unroll
-            for (int h = 0; h < H; h++) red[((wr * others + wk - 1) * H + h) * 64 + lane] = f32x4{acc[h][0], acc[h][1], acc[h][2], acc[h][3]};
-        }
-        if (others) __syncthreads();
-        if (wk == 0 && tile < a.all_tiles) {
+        for (int h = 0; h < H; h++)
 #pragma unroll
-            for (int h = 0; h < H; h++)
-                for (int k = 0; k < others; k++) {
-                    const f32x4 v = red[((wr * others + k) * H + h) * 64 + lane];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) acc[h][r] += v[r];
-                }
+            for (int r = 0; r < 4; r++) reinterpret_cast<float *>(own)[(h * 4 + r) * 64 + lane] = acc[h][r];
+        if (a.wk > 1) __syncthreads();
+        else wave_sync();
+        if (tile < a.all_tiles) {
             const tile_place t = tile_of(a, tile);
+            const int rows = pick(a.N, t.weight);
+            const float * sums = reinterpret_cast<const float *>(own - wk * WAVE_BYTES<TYPE, H>);
+            for (int i = wk; i < H / S * 4; i += a.wk) {
+                float v[S];
 #pragma unroll
-            for (int h = 0; h < H / S; h++) {
-                const int row = t.number * ROWS + h * 16 + col;
-                if (row >= pick(a.N, t.weight)) continue;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    if (group * 4 + r >= a.M) continue;
-                    const float v[2] = {acc[h][r], acc[S == 2 ? 1 : h][r]};
-                    store_row<S>(a, t.weight, row, group * 4 + r, v);
+                for (int s = 0; s < S; s++) {
+                    v[s] = 0.0f;
+                    for (int k = 0; k < a.wk; k++) v[s] += sums[k * (WAVE_BYTES<TYPE, H> / 4) + (s * 4 + i) * 64 + lane];
                 }
+                const int row = t.number * ROWS + (i >> 2) * 16 + col, m = group * 4 + (i & 3);
+                if (row < rows && m < a.M) store_row<S>(a, t.weight, row, m, v);
             }
         }
-        if (others) __syncthreads();
+        if (a.wk > 1) __syncthreads();
+        else wave_sync();
     };
     // one block: the next one requested, this one computed; what follows it
     auto turn = [&](typename Q::raw (&now)[AHEAD][H], typename Q::raw (&then)[AHEAD][H], place p, bool first) {
@@ -555,10 +586,8 @@ template <int TYPE> struct stream;
 
 // Shared memory by its address: a read through a pointer that the compiler can follow
 // to an object waits for all direct loads into that object.
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-template <typename V> __device__ inline V lds(uint32_t at) { return *(const __attribute__((address_space(3))) V *) at; }
-template <typename V> __device__ inline void lds(uint32_t at, V v) { *(__attribute__((address_space(3))) V *) at = v; }
+template <typename V> __device__ inline V lds(uint32_t at) { return *(const __attribute__((address_space(3))) V *) (uintptr_t) at; }
+template <typename V> __device__ inline void lds(uint32_t at, V v) { *(__attribute__((address_space(3))) V *) (uintptr_t) at = v; }
 
 // A chunk of 2 bytes of scale and N words of codes, at an even address: whole words are
 // read from a whole address on, of which the codes come out by a permute, or are words.
@@ -600,7 +629,6 @@ template <> struct stream<ZEST_TYPE_Q8_0> {
         return {{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])}, d};
     }
 };
-__device__ inline uint4 as_uint4(u32x4 v) { return make_uint4(v.x, v.y, v.z, v.w); }
 template <> struct stream<ZEST_TYPE_Q4_K> {
     static constexpr int UNIT = 144, CHUNKS = 4;
     static __device__ quant<ZEST_TYPE_Q4_K>::raw read(uint32_t unit, int chunk) {
@@ -943,6 +971,24 @@ template <int S> stream_sizes sizes_of(int type, int chunks) {
 #undef ZEST_SIZES
 }
 
+// Tiles' sizes by type: a block's cell, a wave's own shared memory.
+struct tile_sizes {
+    int cell, wave;
+};
+tile_sizes tile_sizes_of(int type, int height) {
+#define ZEST_SIZES(T) \
+    case T: return {TILE_CELL<T>, height == 2 ? WAVE_BYTES<T, 2> : WAVE_BYTES<T, 1>}
+    switch (type) {
+        ZEST_SIZES(ZEST_TYPE_Q4_0);
+        ZEST_SIZES(ZEST_TYPE_Q4_1);
+        ZEST_SIZES(ZEST_TYPE_Q8_0);
+        ZEST_SIZES(ZEST_TYPE_Q4_K);
+        ZEST_SIZES(ZEST_TYPE_IQ4_NL);
+        default: ZEST_SIZES(ZEST_TYPE_IQ4_XS);
+    }
+#undef ZEST_SIZES
+}
+
 constexpr int CUS = 256;
 constexpr int STREAM_ROWS = 512;  // of a workgroup at most
 
@@ -979,11 +1025,12 @@ matvec_plan plan_of(int type, int64_t M, int64_t K, int n, const int64_t * N, bo
     p.wk = 1;
     for (int w = 1; w <= most; w++)
         if ((steps + w - 1) / w < (steps + p.wk - 1) / p.wk) p.wk = w;
-    const size_t cell = type == ZEST_TYPE_Q4_K || type == ZEST_TYPE_Q4_1 ? 1664 : 1600, red = (size_t) (p.wk - 1) * p.wr * p.height * 1024;
-    p.seg_steps = (int) std::min<size_t>(steps, (LDS_MOST - red) / ((size_t) GROUPS * B * cell));
+    const tile_sizes z = tile_sizes_of(type, p.height);
+    const size_t cell = z.cell, own = (size_t) p.wk * p.wr * z.wave;
+    p.seg_steps = (int) std::min<size_t>(steps, (LDS_MOST - own) / ((size_t) GROUPS * B * cell));
     p.segs = (steps + p.seg_steps - 1) / p.seg_steps;
     p.copy = true;
-    p.lds = (size_t) std::min(p.seg_steps * GROUPS, chunks) * B * cell + red;
+    p.lds = (size_t) std::min(p.seg_steps * GROUPS, chunks) * B * cell + own;
     p.workgroups = (int) std::min<int64_t>((tiles + p.wr - 1) / p.wr, 2 * CUS);
     if (p.lds > LDS_MOST / 2 || p.wk * p.wr > 8) p.workgroups = std::min(p.workgroups, CUS);
     p.bytes = (size_t) chunks * B * cell;
