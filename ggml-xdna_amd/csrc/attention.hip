@@ -1586,12 +1586,20 @@ struct shared_plan {
 // Sequences of so many columns keep the matrix cores busy by themselves, and what is
 // shared is then no longer what bounds them.
 constexpr int64_t MOST_SHARED_COLS = 128;
+// Bytes of keys and values below which sequences are better read one by one: the search and
+// the join take 10 us or more, and repeated reads are the caches'. Single tokens of n sequences
+// that share all but 100 tokens, 8 k/v heads of 128, one by one and shared in us: 2 of 8192 (34
+// MB) 25.1 and 31.6, 4 of 8192 (101 MB) 33.2 and 31.3, 16 of 2048 (126 MB) 24.9 and 24.3, 64 of
+// 512 (132 MB) 17.5 and 29.2, 2 of 32768 (134 MB) 52.1 and 64.0, 4 of 32768 (403 MB) 87.6 and
+// 63.6, 16 of 8192 (503 MB) 82.7 and 34.5, 64 of 2048 (529 MB) 34.0 and 34.9.
+constexpr int64_t LEAST_SAVED = 160 << 20;
 
 shared_plan shared_plan_of(const zest_kv_cache * c, const zest_kv_batch * b, const zest_kv_groups * g, int group) {
     shared_plan p{};
     const int D = c->head_dim, chunk = chunk_waves(D) * 32;
     const int64_t most = (int64_t) b->max_new * group, shared = std::min(g->max_shared, b->max_len);
-    p.plain = most > MOST_SHARED_COLS || shared < c->page_tokens || b->seqs < 2;
+    const int64_t saved = std::max<int64_t>(b->seqs - g->groups, 0) * shared * c->kv_heads * D * 4;
+    p.plain = most > MOST_SHARED_COLS || shared < c->page_tokens || b->seqs < 2 || (!g->always && saved < LEAST_SAVED);
     if (p.plain) {
         p.bytes = plan_of(c, b, group).bytes;
         return p;
@@ -1764,8 +1772,8 @@ int zest_kv_attn_shared(const zest_kv_cache * cache, const zest_kv_batch * batch
     attn_args a{};
     if (const int st = check_attn(me, cache, batch, q, q_type, ldq, q_heads, scale, causal, window, softcap, out, out_type, ldo, bad, a)) return st;
     ZEST_REQUIRE(groups && groups->starts && (reinterpret_cast<uintptr_t>(groups->starts) & 3) == 0, "%s: null or misaligned groups", me);
-    ZEST_REQUIRE(groups->groups > 0 && groups->groups <= MAX_GROUPS && groups->max_shared >= 0 && groups->max_shared <= (1 << 30),
-                 "%s: groups=%d max_shared=%d", me, groups->groups, groups->max_shared);
+    ZEST_REQUIRE(groups->groups > 0 && groups->groups <= MAX_GROUPS && groups->max_shared >= 0 && groups->max_shared <= (1 << 30) && (groups->always == 0 || groups->always == 1),
+                 "%s: groups=%d max_shared=%d always=%d", me, groups->groups, groups->max_shared, groups->always);
     ZEST_REQUIRE((int64_t) batch->table_rows * batch->table_cols < (1ll << 31), "%s: tables of %d x %d", me, batch->table_rows, batch->table_cols);
     const hipStream_t s = zest::as_stream(stream);
     const shared_plan p = shared_plan_of(cache, batch, groups, a.group);

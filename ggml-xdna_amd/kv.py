@@ -44,7 +44,7 @@ class _Rope(ctypes.Structure):
 
 
 class _Groups(ctypes.Structure):
-    _fields_ = [("starts", ctypes.c_void_p), ("groups", ctypes.c_int32), ("max_shared", ctypes.c_int32)]
+    _fields_ = [("starts", ctypes.c_void_p), ("groups", ctypes.c_int32), ("max_shared", ctypes.c_int32), ("always", ctypes.c_int32)]
 
 
 def _need(ok: bool, what: str) -> None:
@@ -164,13 +164,14 @@ class Batch:
 
 class Groups:
     """Sequences of a batch that share their leading pages: group g is the sequences starts[g] .. starts[g+1]-1 (int32,
-    device), which share at most max_shared tokens; what they do share is found from their tables on the device."""
+    device), which share at most max_shared tokens; what they do share is found from their tables on the device. Groups
+    that save too little by these bounds are passed over unless `always` is set."""
 
-    def __init__(self, starts, max_shared: int):
+    def __init__(self, starts, max_shared: int, always: bool = False):
         self.starts, self.groups, self.max_shared = _list(starts, "starts", starts.device), starts.numel() - 1, max_shared
         _need(self.groups > 0, "starts: one more entry than groups wanted")
         _need(0 <= max_shared < 1 << 31, f"max_shared={max_shared}: 31 bits wanted")
-        self._c = _Groups(starts.data_ptr(), self.groups, max_shared)
+        self._c = _Groups(starts.data_ptr(), self.groups, max_shared, int(always))
 
 
 class Rope:

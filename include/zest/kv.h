@@ -134,11 +134,13 @@ ZEST_API int zest_kv_attn(const zest_kv_cache *cache, const zest_kv_batch *batch
  * the leading whole pages that the tables of all its members name alike, as far as
  * all its rows see all of them, and max_shared tokens at most. So a group is only
  * ever a hint, and forks of one prompt (zest_kv_assign) one after the other in a
- * batch are such a group. */
+ * batch are such a group. Unless `always` is set, groups that by the sizes and bounds
+ * alone save too little to pay for the search and the join are passed over. */
 typedef struct {
     const int32_t *starts; /* [groups + 1], device */
     int32_t groups;        /* 1 .. 2048 */
     int32_t max_shared;    /* 0 .. 2^30 */
+    int32_t always;        /* 0 or 1 */
 } zest_kv_groups;
 
 /* zest_kv_attn where the batch's sequences come in groups: the same result but for

@@ -129,7 +129,7 @@ def test_shared_attention_refuses():
     need = lib.zest_kv_attn_shared_workspace(ctypes.byref(cache), ctypes.byref(batch()), ctypes.byref(kv._Groups(base, 1, 32)), 4)
     assert need > 0
     for broken in (dict(g=None), dict(g=(None, 1, 32)), dict(g=(base + 2, 1, 32)), dict(g=(base, 0, 32)), dict(g=(base, 2049, 32)), dict(g=(base, 1, -1)),
-                   dict(g=(base, 1, (1 << 30) + 1)), dict(heads=3), dict(q=None), dict(out=base), dict(ws=None), dict(ws=base + 8), dict(size=need - 1),
+                   dict(g=(base, 1, (1 << 30) + 1)), dict(g=(base, 1, 32, 2)), dict(heads=3), dict(q=None), dict(out=base), dict(ws=None), dict(ws=base + 8), dict(size=need - 1),
                    dict(b=batch(max_new=0)), dict(b=batch(seqs=0)), dict(c=kv._Cache(base, 0, 30, 2, 64, 16))):
         _refused("zest_kv_attn", call(**broken), E_ARG)
     _refused("zest_kv_attn", call(c=kv._Cache(base, 4, 8, 2, 64, 16)), E_UNSUPPORTED)

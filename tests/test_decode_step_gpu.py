@@ -23,6 +23,7 @@ def _config(st, types=(12, 8, 12, 8), layers=2):
 
 def _start(st, cfg, answers, prompt, seed=1, page=16, vocab=700):
     d = st.Decode(cfg, vocab, answers, 160, seed=seed, page=page)
+    d.groups = type(d.groups)(d.groups.starts, 160, always=True)  # (so few tokens would be read one by one)
     d.prompt(torch.randint(0, vocab, (prompt,), generator=torch.Generator().manual_seed(seed), dtype=torch.int32).cuda())
     d.temperature.fill_(0.9)
     d.top_k.fill_(50)

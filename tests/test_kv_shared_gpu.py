@@ -50,7 +50,7 @@ class Case:
         b.fill()
         self.cache = b.cache(kv)
         self.batch = kv.Batch(_i32(self.starts), self.rows, max(self.new + [1]), max(self.lens + [1]))
-        self.groups = kv.Groups(_i32(starts), max(self.lens) if max_shared is None else max_shared)
+        self.groups = kv.Groups(_i32(starts), max(self.lens) if max_shared is None else max_shared, always=True)
 
     def run(self, kv, **more):
         return kv.attention(self.cache, 0, self.batch, self.q.cuda(), groups=self.groups, **more)
@@ -190,7 +190,7 @@ def test_rows_left_as_they_were(kv):
     batch = kv.Batch(c.batch.starts, c.rows + 3, 2, 50)
     for starts in ([0, 3, 5], [1, 3], [0, 0, 5], [5, 5], [0, 2]):
         out.fill_(7.0)
-        kv.attention(c.cache, 0, batch, q[:, 256:], out=out[:, 24:280], groups=kv.Groups(_i32(starts), 64))
+        kv.attention(c.cache, 0, batch, q[:, 256:], out=out[:, 24:280], groups=kv.Groups(_i32(starts), 64, always=True))
         c.check(out[:c.rows, 24:280])
         assert bool((out[c.rows:] == 7).all()) and bool((out[:, :24] == 7).all()) and bool((out[:, 280:] == 7).all())
     order = [3, 0, 4, 2, 1]
@@ -205,7 +205,7 @@ def test_bad_groups_are_reported(kv):
     c = Case(kv, [(2, [(1, 50), (1, 40), (1, 35)]), (2, [(1, 60), (1, 61)])], 16, 2, 2, 64, BF16, seed=9)
     for starts in ([0, 9], [-1, 3], [3, 0, 5], [2, 1], [0, 3, 2 ** 31 - 1], [-2 ** 31, 5]):
         bad = _flag()
-        c.check(kv.attention(c.cache, 0, c.batch, c.q.cuda(), groups=kv.Groups(_i32(starts), 64), bad=bad))
+        c.check(kv.attention(c.cache, 0, c.batch, c.q.cuda(), groups=kv.Groups(_i32(starts), 64, always=True), bad=bad))
         assert int(bad) == 1, starts
 
 
@@ -239,7 +239,7 @@ def test_in_a_graph_with_forks(kv):
     kv.append(cache, 0, batch, *(torch.randn((prompt, kvh * d), generator=g, device="cuda") for _ in range(2)))
     kv.assign(cache, _i32(list(range(1, 8))), _i32([0] * 7), _i32([0] * 7))
     step = kv.Batch(_i32(list(range(9))), 8, 1, 400)
-    groups = kv.Groups(_i32([0, 8]), 400)
+    groups = kv.Groups(_i32([0, 8]), 400, always=True)
     q, k, v = (torch.randn((8, n * d), generator=g, device="cuda") for n in (heads, kvh, kvh))
     every, one = _i32(list(range(8))), _i32([1] * 8)
     out = torch.zeros((8, heads * d), device="cuda")
@@ -262,6 +262,19 @@ def test_in_a_graph_with_forks(kv):
         b = 2.0 ** -8 * 4.0 + 2.0 ** -10
         assert bool(((out - want).abs() <= b).all()), turn
     cache.check()
+
+
+def test_groups_that_save_little_are_passed_over(kv):
+    """By sizes and bounds: the sequences are then read one by one, bit for bit as without groups, and bad starts are
+    still reported."""
+    c = Case(kv, [(20, [(1, 100 + 3 * i) for i in range(6)])], 32, 2, 4, 128, BF16, seed=4)
+    q, want = c.q.cuda(), kv.attention(c.cache, 0, c.batch, c.q.cuda())
+    few = kv.Groups(c.groups.starts, 10 ** 4)
+    assert torch.equal(kv.attention(c.cache, 0, c.batch, q, groups=few), want)
+    assert kv.attention_workspace(c.cache, c.batch, 8, few) == kv.attention_workspace(c.cache, c.batch, 8)
+    assert kv.attention_workspace(c.cache, c.batch, 8, c.groups) > kv.attention_workspace(c.cache, c.batch, 8)
+    bad = _flag()
+    assert torch.equal(kv.attention(c.cache, 0, c.batch, q, groups=kv.Groups(_i32([0, 99]), 64), bad=bad), want) and int(bad) == 1
 
 
 def test_two_calls_at_once(kv):
