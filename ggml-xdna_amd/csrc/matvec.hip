@@ -57,7 +57,10 @@ constexpr int row_align(int type) {
     return type == ZEST_TYPE_Q4_K ? 16 : type == ZEST_TYPE_IQ4_XS ? 8 : type == ZEST_TYPE_Q4_1 ? 4 : 2;
 }
 
-// Of a type: blocks of a chunk, whether codes are nibbles as they are (0..15), whether
+// Four nibbles less 8, as signed bytes (no byte carries into the next).
+__device__ inline uint32_t less_8(uint32_t n) { return ((n & 0x0f0f0f0fu) + 0x78787878u) ^ 0x80808080u; }
+
+// Of a type: blocks of a chunk, whether codes are nibbles less 8 (-8..7), whether
 // there are offsets; a chunk's loads, codes and scales.
 template <int TYPE> struct quant;
 
@@ -111,7 +114,7 @@ template <int TYPE> struct quant_nibbles {
 template <> struct quant<ZEST_TYPE_Q4_0> : quant_nibbles<ZEST_TYPE_Q4_0> {};
 template <> struct quant<ZEST_TYPE_IQ4_NL> : quant_nibbles<ZEST_TYPE_IQ4_NL> {};
 
-// d, m, qs[16]: w = d q + m
+// d, m, qs[16]: w = d q + m = d (q - 8) + (m + 8 d)
 template <> struct quant<ZEST_TYPE_Q4_1> {
     struct raw { uint4 q; uint32_t dm; };
     static constexpr int BLOCKS = 1;
@@ -125,16 +128,19 @@ template <> struct quant<ZEST_TYPE_Q4_1> {
         words(r.q, w);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            c[0][0][i] = w[i] & 0x0f0f0f0fu;
-            c[0][1][i] = w[i] >> 4 & 0x0f0f0f0fu;
+            c[0][0][i] = less_8(w[i]);
+            c[0][1][i] = less_8(w[i] >> 4);
         }
     }
     static constexpr int WORDS = 4;
     static __device__ void packed(const raw & r, uint32_t w[1][4]) { words(r.q, w[0]); }
     static __device__ void eight(const uint32_t w[1][4], int chunk, int, uint32_t & low, uint32_t & high) {
-        low = w[0][chunk] & 0x0f0f0f0fu, high = w[0][chunk] >> 4 & 0x0f0f0f0fu;
+        low = less_8(w[0][chunk]), high = less_8(w[0][chunk] >> 4);
     }
-    static __device__ block_scales<1> scales(const raw & r, int) { return {{half_to_float(r.dm)}, {half_to_float(r.dm >> 16)}}; }
+    static __device__ block_scales<1> scales(const raw & r, int) {
+        const float d = half_to_float(r.dm);
+        return {{d}, {fmaf(8.0f, d, half_to_float(r.dm >> 16))}};
+    }
 };
 
 // d, qs[32]: w = d q
@@ -161,7 +167,8 @@ template <> struct quant<ZEST_TYPE_Q8_0> {
 
 // d, dmin, 12 bytes of 6-bit scales and minima of 8 blocks of 32, qs[128]: a chunk's
 // 64 values in 32 bytes, block 2r in the low nibbles, 2r + 1 in the high ones;
-// w = d sc q - dmin m
+// w = d sc q - dmin m, taken about q = 8 too: the codes' products are then no larger than the
+// sum they make, and the offsets of weights that were quantised evenly about 0 all but vanish
 template <> struct quant<ZEST_TYPE_Q4_K> {
     struct raw { uint4 q[2], head; };
     static constexpr int BLOCKS = 2;
@@ -178,8 +185,8 @@ template <> struct quant<ZEST_TYPE_Q4_K> {
             words(r.q[part], w);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                c[0][part][i] = w[i] & 0x0f0f0f0fu;
-                c[1][part][i] = w[i] >> 4 & 0x0f0f0f0fu;
+                c[0][part][i] = less_8(w[i]);
+                c[1][part][i] = less_8(w[i] >> 4);
             }
         }
     }
@@ -189,7 +196,7 @@ template <> struct quant<ZEST_TYPE_Q4_K> {
         words(r.q[1], w[1]);
     }
     static __device__ void eight(const uint32_t w[2][4], int chunk, int block, uint32_t & low, uint32_t & high) {
-        low = w[0][chunk] >> 4 * block & 0x0f0f0f0fu, high = w[1][chunk] >> 4 * block & 0x0f0f0f0fu;
+        low = less_8(w[0][chunk] >> 4 * block), high = less_8(w[1][chunk] >> 4 * block);
     }
     static __device__ block_scales<2> scales(const raw & r, int chunk) {
         const float d = half_to_float(r.head.x), dmin = half_to_float(r.head.x >> 16);
@@ -199,7 +206,8 @@ template <> struct quant<ZEST_TYPE_Q4_K> {
         const uint32_t both = far ? r.head.w : 0u;
         const int by = 16 * (chunk & 1);
         const uint32_t s = ((both & 0x0f0f0f0fu) | a) >> by, n = ((both >> 4 & 0x0f0f0f0fu) | b) >> by;
-        return {{d * (float) (s & 0xff), d * (float) (s >> 8 & 0xff)}, {-dmin * (float) (n & 0xff), -dmin * (float) (n >> 8 & 0xff)}};
+        const float d0 = d * (float) (s & 0xff), d1 = d * (float) (s >> 8 & 0xff);
+        return {{d0, d1}, {fmaf(-dmin, (float) (n & 0xff), 8.0f * d0), fmaf(-dmin, (float) (n >> 8 & 0xff), 8.0f * d1)}};
     }
 };
 
@@ -255,24 +263,25 @@ __device__ inline float over_groups(float v) {
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
-// x as whole numbers: of every 32 consecutive values (whose largest magnitude lies
-// in [2^e, 2^(e+1))) v = rint(x 2^(21-e)), |v| < 2^22, cut in three signed bytes v =
-// d0 2^16 + d1 2^8 + d2. So products with the weights' codes are exact, in 32 bits,
-// and a row of x is met to 2^-22 of the largest of its 32. A cell: [part][digit][16
-// bytes], the factor 2^(e-21) (NaN where a value is not finite), the values' sum.
+// x as whole numbers: of every 32 consecutive values (whose largest magnitude is below
+// 2^(e+1) (1 - 2^-8 - 2^-15): the last 2^-8 counts to the next e) v = rint(x 2^(22-e)), cut
+// in three signed bytes v = d0 2^16 + d1 2^8 + d2, |d0| <= 127. So products with the
+// weights' codes are exact, in 32 bits, and a row of x is met to 2^-22 of the largest of its
+// 32 (2^-23 and a little). A cell: [part][digit][16 bytes], the factor 2^(e-22) (NaN where a
+// value is not finite), the values' sum.
 //
 // Eight lanes prepare a block of a row, four values each: the four digits of each kind,
-// the factor and the sum. Where e is below -105 (the last bit below 2^-126), it counts
-// as -105.
+// the factor and the sum. Where e is below -104 (the last bit below 2^-126), it counts
+// as -104.
 struct prepared {
     uint32_t digits[3];
     float factor, sum;
 };
 __device__ inline prepared prepare(float4 f) {
     const float v[4] = {f.x, f.y, f.z, f.w};
-    uint32_t e = 22;
+    uint32_t e = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) e = max(e, __float_as_uint(v[i]) >> 23 & 0xffu);
+    for (int i = 0; i < 4; i++) e = max(e, __float_as_uint(v[i]) & 0x7fffffffu);
     prepared r{{0, 0, 0}, 0.0f, (v[0] + v[1]) + (v[2] + v[3])};
     // over the quad, then the other quad of the eight
     e = max(e, (uint32_t) __builtin_amdgcn_mov_dpp((int) e, 0xb1, 0xf, 0xf, false));
@@ -281,9 +290,10 @@ __device__ inline prepared prepare(float4 f) {
     r.sum += dpp<0xb1>(r.sum);
     r.sum += dpp<0x4e>(r.sum);
     r.sum += dpp<0x141>(r.sum);
-    const bool odd = e == 255;
-    const float up = odd ? 0.0f : __uint_as_float((275 - e) << 23);
-    r.factor = odd ? NAN : __uint_as_float((e - 21) << 23);
+    const bool odd = e >= 0x7f800000u;
+    e = max((e + 0x10200u) >> 23, 23u);
+    const float up = odd ? 0.0f : __uint_as_float((276 - e) << 23);
+    r.factor = odd ? NAN : __uint_as_float((e - 22) << 23);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int q = odd ? 0 : (int) __builtin_rintf(v[i] * up);
@@ -494,7 +504,7 @@ template <int TYPE, int H, int S> __global__ __launch_bounds__(1024) void matvec
                         for (int k = 0; k < 3; k++) d[k] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x[k], code, i32x4{}, 0, 0, 0);
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
-                            // (|d0| <= 64 15 32 < 2^15 for nibbles, so they fit in 32 bits together)
+                            // (nibbles' sums |d0| <= 127 8 32 and |d1|, |d2| <= 128 8 32 fit in 32 bits together)
                             const float v = Q::NIBBLES ? (float) ((((d[0][r] << 8) + d[1][r]) << 8) + d[2][r]) : fmaf((float) d[0][r], 65536.0f, (float) ((d[1][r] << 8) + d[2][r]));
                             acc[h][r] = fmaf(v, scale[h][b][c] * f[r], acc[h][r]);
                             if constexpr (Q::OFFSETS) acc[h][r] = fmaf(sum[r], offset[h][b][c], acc[h][r]);
@@ -876,7 +886,7 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) __attribute__((amdgpu_waves_per_
                         d[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.x[m][b][1], i32x4{(int) c[b][1][0], (int) c[b][1][1], (int) c[b][1][2], (int) c[b][1][3]}, d[m], 0, 0, 0);
 #pragma unroll
                     for (int m = 0; m < M; m++) {
-                        // (|d0| <= 64 15 32 < 2^15 for nibbles, so they fit in 32 bits together)
+                        // (nibbles' sums |d0| <= 127 8 32 and |d1|, |d2| <= 128 8 32 fit in 32 bits together)
                         const float v = Q::NIBBLES ? (float) ((((d[m][0] << 8) + d[m][1]) << 8) + d[m][2]) : fmaf((float) d[m][0], 65536.0f, (float) ((d[m][1] << 8) + d[m][2]));
                         acc[m][s] = fmaf(v, sc.scale[b] * now.f[m][b].x, acc[m][s]);
                         if constexpr (Q::OFFSETS) acc[m][s] = fmaf(now.f[m][b].y, sc.offset[b], acc[m][s]);
