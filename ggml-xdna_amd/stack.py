@@ -306,7 +306,7 @@ class Decode:
 
     def _run(self, tokens, batch, groups):
         c, eps = self.cfg, 1e-6
-        h = self.embed[tokens.clamp(min=0).long()]
+        h = self.embed[tokens.clamp(0, self.vocab - 1).long()]
         for li, L in enumerate(self.layers):
             a = z.rms_norm(h, eps, L.attn_norm)
             q, k, v = z.matvec(c.qkv_type, a, [L.w[n] for n in ("attn_q", "attn_k", "attn_v")], [c.q, c.kv, c.kv])
@@ -321,6 +321,8 @@ class Decode:
     def prompt(self, tokens) -> None:
         """A prompt (int32, at least one token) into slot 0, up to 16 tokens at a time, the others its forks; its last
         token is left to the first step, whose rows all begin with it."""
+        if len(tokens) < 1:
+            raise z.ZestError("a prompt of at least one token wanted")
         kv.assign(self.cache, self.slots, self._i32([-1] * self.answers), self._i32([0] * self.answers))
         for t0 in range(0, len(tokens) - 1, 16):
             piece = tokens[t0:min(t0 + 16, len(tokens) - 1)]

@@ -76,6 +76,17 @@ def test_many_rows(z):
 
 
 @pytest.mark.parametrize("wtype", TYPES)
+@pytest.mark.parametrize("m,ns", [(5, [33001]), (16, [20015, 1, 17003])])
+def test_tall_weights_by_more_rows(z, wtype, m, ns):
+    """32 weight rows a wave: heights that end inside 32 and inside 16, a weight of one row between two of many."""
+    k = 768
+    x, raws = _x(m, k, 8), [decode_ref.gguf(wtype, n, k, 20 + i) for i, n in enumerate(ns)]
+    got = z.matvec(wtype, x.cuda(), [torch.from_numpy(r).cuda() for r in raws], ns)
+    for y, raw in zip(got, raws):
+        _check(y, wtype, x, raw)
+
+
+@pytest.mark.parametrize("wtype", TYPES)
 @pytest.mark.parametrize("m", [1, 4, 11])
 def test_group_residuals_and_strides(z, wtype, m):
     """Four weights of different heights on an x with a stride, one output in columns of a wider buffer whose rest
@@ -155,19 +166,21 @@ def test_a_weight_s_infinite_scale(z, wtype):
 def test_unaligned_weights(z):
     """Rows at the least alignment that the header asks for."""
     for wtype, align in ((2, 2), (20, 2), (8, 2), (3, 4), (23, 8), (12, 16)):
-        k, n, m = 768, 37, 2
+        k, n = 768, 37
         raw = decode_ref.gguf(wtype, n, k, 7)
         buf = torch.zeros(raw.size + 256, dtype=torch.uint8, device="cuda")
         w = buf[align:align + raw.size]
         w.copy_(torch.from_numpy(raw.reshape(-1)))
-        x = _x(m, k, 3)
-        _check(z.matvec(wtype, x.cuda(), [w], [n])[0], wtype, x, raw)
+        for m in (2, 9):
+            x = _x(m, k, 3)
+            _check(z.matvec(wtype, x.cuda(), [w], [n])[0], wtype, x, raw)
 
 
-def test_bits_do_not_vary(z):
-    """The same bits from run to run, on another stream, and for a group as for its weights alone on equal sizes."""
+@pytest.mark.parametrize("m", [2, 13])
+def test_bits_do_not_vary(z, m):
+    """The same bits from run to run and on another stream."""
     k, n, wtype = 2560, 1000, 12
-    x, raw = _x(2, k, 4).cuda(), torch.from_numpy(decode_ref.gguf(wtype, n, k, 8)).cuda()
+    x, raw = _x(m, k, 4).cuda(), torch.from_numpy(decode_ref.gguf(wtype, n, k, 8)).cuda()
     want = z.matvec(wtype, x, [raw], [n])[0].clone()
     torch.cuda.synchronize()
     with torch.cuda.stream(torch.cuda.Stream()):
@@ -175,16 +188,17 @@ def test_bits_do_not_vary(z):
             assert torch.equal(z.matvec(wtype, x, [raw], [n])[0], want)
 
 
-def test_in_graphs_and_at_once(z):
+@pytest.mark.parametrize("m", [3, 16])
+def test_in_graphs_and_at_once(z, m):
     """Captured with a workspace of its own, replayed with the program's work between, new x and weights; two graphs and
     an eager call with a workspace each run at once."""
     k, n, wtype = 1024, 3000, 2
     raws = [decode_ref.gguf(wtype, n, k, s) for s in (1, 2, 3)]
-    xs = [_x(3, k, s).cuda() for s in (1, 2, 3)]
+    xs = [_x(m, k, s).cuda() for s in (1, 2, 3)]
     ws = [torch.from_numpy(r).cuda() for r in raws]
     eager = [z.matvec(wtype, x, [w], [n])[0].clone() for x, w in zip(xs, ws)]
-    bytes_ = z.matvec_workspace(wtype, 3, k, [n])
-    outs = [torch.zeros((3, n), device="cuda") for _ in range(3)]
+    bytes_ = z.matvec_workspace(wtype, m, k, [n])
+    outs = [torch.zeros((m, n), device="cuda") for _ in range(3)]
     spaces = [torch.empty(max(16, bytes_), dtype=torch.uint8, device="cuda") for _ in range(3)]
     graphs = []
     for i in range(2):
