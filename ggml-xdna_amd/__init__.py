@@ -378,15 +378,17 @@ def matvec(wtype: int, x, weights, ns, outs=None, residuals=None, workspace=None
         raise ZestError(f"{n} weights: as many sizes, outputs and residuals wanted")
     px, ldx = _fp32_rows(x, "x", m, k, dev, f32)
     size, need = _matvec_sizes(wtype, m, k, tuple(ns))
-    if outs is None:
-        outs = [torch.empty((m, ni), dtype=f32, device=dev) for ni in ns]
     w, py, ldy, pr, ldr = [], [], [], [], []
+    if outs is None:
+        outs = [x.new_empty((m, ni)) for ni in ns]
+        py, ldy = [y.data_ptr() for y in outs], ns
     for i in range(n):
         ni = ns[i]
         w.append(_gguf(weights[i], "weight", wtype, size, ni, k, dev, u8))
-        p, ld = _fp32_rows(outs[i], "output", m, ni, dev, f32)
-        py.append(p)
-        ldy.append(ld)
+        if ldy is not ns:
+            p, ld = _fp32_rows(outs[i], "output", m, ni, dev, f32)
+            py.append(p)
+            ldy.append(ld)
         if residuals is not None and residuals[i] is not None:
             p, ld = _fp32_rows(residuals[i], "residual", m, ni, dev, f32)
         else:
@@ -413,7 +415,7 @@ def matvec_glu(kind: int, wtype: int, x, gate, up, f: int, out=None, workspace=N
     m, k = x.shape
     px, ldx = _fp32_rows(x, "x", m, k, dev, f32)
     size, need = _matvec_sizes(wtype, m, k, (f, f))
-    out = torch.empty((m, f), dtype=f32, device=dev) if out is None else out
+    out = x.new_empty((m, f)) if out is None else out
     py, ldy = _fp32_rows(out, "out", m, f, dev, f32)
     keep, ws, ws_bytes = _matvec_workspace(workspace, need, dev)
     check(lib().zest_matvec_glu(kind, wtype, px, m, k, ldx, _gguf(gate, "gate", wtype, size, f, k, dev, u8),

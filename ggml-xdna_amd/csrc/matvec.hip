@@ -393,7 +393,7 @@ template <int TYPE, int H> constexpr int WAVE_BYTES = TRADE<TYPE> * 64 > H * 102
 // x's cells lie in shared memory, all of K's or a segment's. The waves of a tile (a.wk of
 // them) each take a run of its steps; AHEAD steps of a wave are in flight while it computes
 // the AHEAD before them (twice as many were slower: 154 us for 115), and the waves' sums are
-// joined in shared memory. 151936 rows of 2560 IQ4_XS by 16: 104 us, of which the loads alone
+// joined in shared memory. 151936 rows of 2560 IQ4_XS by 16: 100 us, of which the loads alone
 // take 76 and the products alone 82; with products of a lane's own 16 codes, a row of x at a
 // time as below, 190.
 template <int TYPE, int H, int S> __global__ __launch_bounds__(1024) void matvec_kernel(matvec_args a) {
@@ -697,10 +697,13 @@ __device__ inline call_row row_of(const matvec_args & a, int r) {
 // costs a lane a conversion and a few fused products for a row of x.
 //
 // HBM bound: a weight's bytes once. They come not chunk by chunk into registers, where an
-// instruction touches 16 lines or more and a line is asked for three times, but as whole granules of contiguous bytes straight into shared memory:
-// RING pieces (two units of 16 rows, 4.6 KB) a wave, requested as soon as their place
+// instruction touches 16 lines or more and a line is asked for three times, but as whole
+// granules of contiguous bytes straight into shared memory: RING pieces (two units of 16 rows, 4.6 KB) a wave, requested as soon as their place
 // is read. A workgroup's last 16 rows are as many as are left of its share: a row that
-// is not there is its neighbour again. So all CUs stream whatever the number of rows.
+// is not there is its neighbour again. So all CUs stream whatever the number of rows. A
+// GLU's two weights of 17408 rows of 5120 Q4_K by 4 rows: 29 to 32 us, 3.2 to 3.5 TB/s; 2560
+// rows of 9728 Q8_0 by one: 10.8, 1024 of 1024 Q4_0 by 3: 6.1 (a chain of x, its digits and
+// the weights). Deeper rings with one workgroup a CU: 38 us for the first.
 template <int TYPE, int M, int S, int RING, bool READY>
 __global__ __launch_bounds__(STREAM_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void stream_kernel(matvec_args a) {
     typedef quant<TYPE> Q;
