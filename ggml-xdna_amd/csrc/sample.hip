@@ -645,6 +645,9 @@ __global__ __launch_bounds__(THREADS) void collect_kernel(sample_args a) {
     const row_top t(a, s, p);
     if (threadIdx.x == 0) at = 0;
     __syncthreads();
+    // before the last bin all have a weight: they are nearer than 255 / 256 width, where it is
+    // e^-31.875 > 2^-46 at least (unless bins cannot be as narrow as the width asks)
+    const bool fine = t.bins.per < 3e38f;
     u64 above = 0;
     uint32_t mine = 0, place[STEPS][4];
 #pragma unroll
@@ -656,7 +659,7 @@ __global__ __launch_bounds__(THREADS) void collect_kernel(sample_args a) {
             if (b < from && p.m > 0.0 && !(t.top - x[j][e] > p.near)) {
                 const weight w = weight_of(x[j][e], t.top, p.scale);
                 above += p.fits(w) ? whole(w) : 0;
-            } else if (b >= from && b <= to && whole(weight_of(x[j][e], t.top, p.scale))) {
+            } else if (b >= from && b <= to && ((fine && b < BINS - 1) || whole(weight_of(x[j][e], t.top, p.scale)))) {
                 place[j][e] = atomicAdd(&at, 1u);
             }
         }

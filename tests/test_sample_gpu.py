@@ -121,16 +121,28 @@ def test_masked_and_odd_logits(s, vocab):
             assert tokens[7] % 2 == 1
 
 
-def test_odd_parameters(s):
+@pytest.mark.parametrize("vocab", [777, 20001])
+def test_odd_parameters(s, vocab):
     """NaN, infinite and negative parameters are read as the header says."""
-    x = _logits(9, 777, seed=5)
+    x = _logits(9, vocab, seed=5)
     nan, inf = math.nan, math.inf
     _check(s, x, [nan, -1.0, 1.0, 2.0, inf, -inf, 0.5, 0.5, 0.5])
     u = [0.6] * 9
     _check(s, x, u, [nan, -1.0, inf, 1e-30, 1e-45, 1e30, 0.0, -inf, 1.0])
-    _check(s, x, u, None, [-5, 0, 1, 776, 777, 778, 2 ** 31 - 1, -2 ** 31, 2])
+    _check(s, x, u, None, [-5, 0, 1, vocab - 1, vocab, vocab + 1, 2 ** 31 - 1, -2 ** 31, 2])
     _check(s, x, u, None, None, [nan, -1.0, 0.0, 1e-45, 1.0, inf, -inf, 0.5, 2.0])
     _check(s, x, u, None, None, None, [nan, -1.0, 0.0, 1e-45, 1.0, inf, -inf, 0.5, 2.0])
+
+
+@pytest.mark.parametrize("vocab", [777, 20001])
+def test_tiny_temperatures(s, vocab):
+    """Logits that lie closer than a histogram's narrowest bin, but far apart by their temperature."""
+    x = 1e-42 * _logits(4, vocab, seed=6, spread=1.0)
+    u = [0.0, 0.3, 0.6, 0.999]
+    for t in (1e-45, 1e-43, 1e-42, 1e-30):
+        _check(s, x, u, [t] * 4)
+        _check(s, x, u, [t] * 4, [3, 50, 700, 5000])
+        _check(s, x, u, [t] * 4, None, [0.1, 0.9, 0.99, 0.5])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
