@@ -17,7 +17,7 @@
 // finish_kernel cuts and draws. (With the last workgroup of a row to finish going on by
 // itself, in three launches, the fences that takes cost 300 us for 64 rows of 151936.) In us:
 // one row of 151936 with a top-k and a top-p 3.9, 6.7, 6.4, 6.5 and 13.3, 64 rows with a top-p
-// 12, 23, 8, 21 and 15 (the 64-bit series twice), 256 of 16 bits with a min-p 26, 30 and 7
+// 11, 23, 8, 18 and 15 (the 64-bit series in the second), 256 of 16 bits with a min-p 26, 30 and 7
 // (two readings at 2.6 to 3 TB/s).
 #include <algorithm>
 
