@@ -962,7 +962,7 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) __attribute__((amdgpu_waves_per_
 struct matvec_plan {
     int ring;             // of stream_kernel; 0: matvec_kernel
     int wk, wr, height, workgroups, seg_steps, segs, pieces;
-    bool copy;            // x is prepared by a kernel of its own
+    bool copy;            // of stream_kernel: x is prepared by a kernel of its own
     size_t lds, bytes;
 };
 
@@ -1042,7 +1042,6 @@ matvec_plan plan_of(int type, int64_t M, int64_t K, int n, const int64_t * N, bo
     const size_t cell = z.cell, own = (size_t) p.wk * p.wr * z.wave;
     p.seg_steps = (int) std::min<size_t>(steps, (LDS_MOST - own) / ((size_t) GROUPS * B * cell));
     p.segs = (steps + p.seg_steps - 1) / p.seg_steps;
-    p.copy = true;
     p.lds = (size_t) std::min(p.seg_steps * GROUPS, chunks) * B * cell + own;
     p.workgroups = (int) std::min<int64_t>((tiles + p.wr - 1) / p.wr, 2 * CUS);
     if (p.lds > LDS_MOST / 2 || p.wk * p.wr > 8) p.workgroups = std::min(p.workgroups, CUS);
